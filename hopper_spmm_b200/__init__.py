@@ -7,7 +7,8 @@ benchmark inputs.
 from .spmm import (BTCF_MTX_NO_BITMAP, CSR2BTCFNOBITMAP, CSR_MTX, DENSE_MTX, DeviceBtcf, IDX_MAX, PERF_RESULT, ROW_WINDOW, RUNS,
                    WARMUP_RUNS, ShardedSpmm, SpmmPlan, fp16_spmm, rewindow, shard_rows, tf32_spmm, transpose_tiles)
 
+from .fp4 import Fp4Matrix, fp4_quantize, fp4_quantize_both
 from .formats import BTCF2GBTCF, BTCF_MTX, CSR2BTCF, GBTCF_MTX, load_matrix, validateBTCF2GBTCFConversion
 
-__all__ = ["BTCF2GBTCF", "BTCF_MTX", "CSR2BTCF", "GBTCF_MTX", "load_matrix", "validateBTCF2GBTCFConversion", "BTCF_MTX_NO_BITMAP", "CSR2BTCFNOBITMAP", "CSR_MTX", "DENSE_MTX", "DeviceBtcf", "IDX_MAX", "PERF_RESULT", "ROW_WINDOW",
+__all__ = ["BTCF2GBTCF", "BTCF_MTX", "CSR2BTCF", "GBTCF_MTX", "load_matrix", "validateBTCF2GBTCFConversion", "BTCF_MTX_NO_BITMAP", "CSR2BTCFNOBITMAP", "CSR_MTX", "DENSE_MTX", "DeviceBtcf", "Fp4Matrix", "fp4_quantize", "fp4_quantize_both", "IDX_MAX", "PERF_RESULT", "ROW_WINDOW",
            "RUNS", "WARMUP_RUNS", "ShardedSpmm", "SpmmPlan", "fp16_spmm", "rewindow", "shard_rows", "tf32_spmm", "transpose_tiles"]

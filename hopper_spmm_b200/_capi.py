@@ -12,6 +12,8 @@ ERR_INVALID_ARG, ERR_BAD_CSR, ERR_UNSUPPORTED, ERR_NO_MEMORY, ERR_CUDA, ERR_NO_D
     -1, -2, -3, -4, -5, -6, -7)
 F16, TF32 = 0, 1
 C_F32, C_F16 = 0, 1
+NVFP4, MXFP4 = 0, 1
+T_F32, T_F16, T_BF16 = 0, 1, 2
 
 u64, i64, u32, i32, vp = C.c_uint64, C.c_int64, C.c_uint32, C.c_int32, C.c_void_p
 
@@ -25,6 +27,10 @@ class LaunchInfo(C.Structure):
     _fields_ = [("n_ctas", i32), ("threads", i32), ("stages", i32), ("feature_slab", i32), ("n_slabs", i32),
                 ("smem_bytes", i64), ("kernel_launches", i64), ("tma_gather", i32), ("bitmap_tiles", i32),
                 ("row_window", i32)]
+
+
+class Fp4(C.Structure):
+    _fields_ = [("rows", u64), ("cols", u64), ("format", i32), ("device", i32), ("values", vp), ("scales", vp), ("tensor_scale", vp)]
 
 
 class KatMma(C.Structure):
@@ -113,6 +119,13 @@ SIGNATURES = {
     "b200spmm_plan_pair_info": (C.c_int, [vp, C.POINTER(BtcfInfo)]),
     "b200spmm_plan_pair_copy_to_host": (C.c_int, [vp, vp, vp, vp, vp]),
     "b200spmm_plan_launch_info": (C.c_int, [vp, C.POINTER(LaunchInfo)]),
+    "b200spmm_fp4_sizes": (C.c_int, [u64, u64, C.c_int] + [C.POINTER(u64)] * 4),
+    "b200spmm_fp4_quantize": (C.c_int, [vp, i64, C.c_int, C.c_int, vp, C.POINTER(Fp4), vp, vp]),
+    "b200spmm_fp4_quantize_both": (C.c_int, [vp, i64, C.c_int, vp, C.POINTER(Fp4), C.POINTER(Fp4), vp, vp]),
+    "b200spmm_fp4_dequantize": (C.c_int, [C.POINTER(Fp4), vp, i64, C.c_int, vp]),
+    "b200spmm_fp4_product": (C.c_int, [C.POINTER(Fp4), C.POINTER(Fp4), vp, i64, C.c_int, C.c_int, vp]),
+    "b200spmm_fp4_dense_product": (C.c_int, [C.POINTER(Fp4), vp, i64, i64, C.c_int, C.c_int, vp, i64, C.c_int, C.c_int, vp]),
+    "b200spmm_fp4_status": (C.c_int, [C.c_int, vp]),
     "b200spmm_kat_umma": (C.c_int, [vp, u32, C.POINTER(KatMma), C.c_int, C.c_int, vp, C.c_int]),
     "b200spmm_kat_umma_pair": (C.c_int, [vp, u32, C.POINTER(KatMma), C.c_int, C.c_int, vp, C.c_int]),
     "b200spmm_kat_wait_limit": (C.c_uint64, [C.c_uint64]),

@@ -1,0 +1,80 @@
+// From accumulators to C: the tensors' scales, the element type, either order of C.
+#pragma once
+
+#include "fp4_convert.cuh"
+
+namespace b200spmm {
+namespace fp4 {
+
+// The product of two tensors' scales, applied in steps none of which leaves fp32's range unless the result does: the mantissa (1 for
+// powers of two), then both halves of the exponent.
+struct Factor {
+    float mantissa, half0, half1;
+    B200_DEVICE Factor(float a, float b) {
+        const double ab = (double)a * (double)b;
+        const int64_t bits = __double_as_longlong(ab);
+        const int e = (int)(bits >> 52 & 0x7FF) - 1023;  // (a product of two fp32 numbers is never subnormal in 64 bits)
+        if (e == 1024 || e == -1023) {  // NaN, infinity or zero
+            mantissa = (float)ab;
+            half0 = half1 = 1.f;
+            return;
+        }
+        mantissa = (float)__longlong_as_double((bits & ~(0x7FFll << 52)) | (1023ll << 52));
+        const int e0 = e / 2, e1 = e - e0;
+        half0 = ldexpf(1.f, e0);
+        half1 = ldexpf(1.f, e1);
+    }
+    B200_DEVICE float apply(float v) const { return v * mantissa * half0 * half1; }
+};
+
+struct Target {
+    uint8_t *ptr;
+    int64_t ldc;  // elements
+    int type;     // B200SPMM_T_*
+    bool transposed;  // element (row, col) at [col * ldc + row]
+    bool wide;    // rows start on 16 bytes
+};
+
+inline Target target_of(void *c, int64_t ldc, int type, bool transposed) {
+    const int64_t esz = type == B200SPMM_T_F32 ? 4 : 2;
+    return {static_cast<uint8_t *>(c), ldc, type, transposed, reinterpret_cast<uintptr_t>(c) % 16u == 0 && ldc * esz % 16 == 0};
+}
+
+template <typename T, int N>
+B200_DEVICE void store_row_as(const Target &c, uint32_t row, uint32_t col, uint32_t n, const float (&v)[N]) {
+    T *out = reinterpret_cast<T *>(c.ptr);
+    if (c.transposed) {  // lanes hold neighbouring rows: every store is one run
+        T *dst = out + (int64_t)col * c.ldc + row;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (col + i < n) dst[(int64_t)i * c.ldc] = Elem<T>::from_float(v[i]);
+        return;
+    }
+    T *dst = out + (int64_t)row * c.ldc + col;
+    constexpr int kPer = 16 / sizeof(T);
+    if (N % kPer == 0 && c.wide && n - col >= (uint32_t)N) {
+#pragma unroll
+        for (int i = 0; i < N / kPer; ++i) {
+            uint4 four;
+            T *e = reinterpret_cast<T *>(&four);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) e[j] = Elem<T>::from_float(v[i * kPer + j]);
+            reinterpret_cast<uint4 *>(dst)[i] = four;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (col + i < n) dst[i] = Elem<T>::from_float(v[i]);
+    }
+}
+
+// N neighbours of a row, from column `col` (a multiple of N) on; those at `n` and behind do not exist.
+template <int N>
+B200_DEVICE void store_row(const Target &c, uint32_t row, uint32_t col, uint32_t n, const float (&v)[N]) {
+    if (c.type == B200SPMM_T_F32) store_row_as<float>(c, row, col, n, v);
+    else if (c.type == B200SPMM_T_F16) store_row_as<__half>(c, row, col, n, v);
+    else store_row_as<__nv_bfloat16>(c, row, col, n, v);
+}
+
+}  // namespace fp4
+}  // namespace b200spmm

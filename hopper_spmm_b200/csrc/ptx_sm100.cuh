@@ -474,6 +474,32 @@ B200_DEVICE void umma_tf32_ss_lohi_if(uint32_t on, uint32_t d_tmem, uint32_t a_l
         : "memory");
 }
 
+// ------------------------------------------------------------------ block-scaled 4-bit MMA
+// D (+)= (scaled A) * (scaled B): e2m1 operands, K-major, 64 values a call, whose scales lie in tensor memory: row r of a 128-row block
+// in lane r % 32 (the same in each quarter of the lanes), column r / 32, four scales to a 32-bit word.  Instruction descriptor:
+//   [4,6) which scale of B's words   [7,10) A format, [10,12) B format (1 = e2m1)   [17,23) N >> 3
+//   [23] scales are e8m0 (0: e4m3)   [27,29) M >> 7   [29,31) which scale of A's words
+// nvfp4 takes all four scales of a word (16 values each), mxfp4 two of them (32 values each): 0 or 2 in the descriptor.
+__host__ __device__ constexpr uint32_t make_fp4_instr_desc(bool e8m0, uint32_t m, uint32_t n, uint32_t scale_id) {
+    return (scale_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((e8m0 ? 1u : 0u) << 23) | ((m >> 7) << 27) | (scale_id << 29);
+}
+template <bool kMx>
+B200_DEVICE void umma_fp4_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales, uint32_t b_scales, uint32_t accumulate) {
+    if constexpr (kMx)
+        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+                     "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+                     ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+                     "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+                     ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory");
+}
+// 32 lanes x 16 bytes from shared memory (core matrices of eight lanes) to four columns of every quarter of the lanes; runs in
+// order with the MMAs that the thread issues after it.
+B200_DEVICE void tmem_copy_scales(uint32_t taddr, uint64_t smem_desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc) : "memory");
+}
+
 // Makes `bar` receive one arrival when every tcgen05.mma this thread issued so far has
 // finished (implies tcgen05.fence::before_thread_sync).
 B200_DEVICE void umma_commit(uint32_t bar) {

@@ -108,7 +108,206 @@ PyObject *spmm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
-PyMethodDef methods[] = {{"spmm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(spmm)), METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
+// ---- 4-bit matrices.  A matrix is (values, scales, tensor_scale, rows, cols, format) in the arguments.
+
+// An argument that is a CUDA tensor, or null.
+const at::Tensor *cuda_tensor(PyObject *o) {
+    if (!THPVariable_Check(o)) return nullptr;
+    const at::Tensor &t = THPVariable_Unpack(o);
+    return t.is_cuda() ? &t : nullptr;
+}
+
+int type_code(at::ScalarType t) {
+    return t == at::kFloat ? B200SPMM_T_F32 : t == at::kHalf ? B200SPMM_T_F16 : t == at::kBFloat16 ? B200SPMM_T_BF16 : -1;
+}
+at::ScalarType type_of(long code) { return code == B200SPMM_T_F16 ? at::kHalf : code == B200SPMM_T_BF16 ? at::kBFloat16 : at::kFloat; }
+
+// A dense matrix with one dimension of neighbours: `transposed` where that is the first.
+struct Dense {
+    void *ptr;
+    int64_t ld;
+    bool transposed;
+};
+bool dense_of(const at::Tensor &t, Dense *d) {
+    if (t.dim() != 2 || t.layout() != at::kStrided) return false;
+    const int64_t r = t.size(0), c = t.size(1), sr = t.stride(0), sc = t.stride(1);
+    if ((sc == 1 || c <= 1) && (r <= 1 || sr >= c)) *d = {nullptr, r <= 1 ? c : sr, false};
+    else if ((sr == 1 || r <= 1) && (c <= 1 || sc >= r)) *d = {nullptr, c <= 1 ? r : sc, true};
+    else return false;
+    d->ptr = t.data_ptr();
+    return true;
+}
+
+bool matrix_of(PyObject *const *args, b200spmm_fp4_t *m) {
+    const at::Tensor *v = cuda_tensor(args[0]), *s = cuda_tensor(args[1]), *w = cuda_tensor(args[2]);
+    if (!v || !s || !w || v->get_device() != s->get_device() || v->get_device() != w->get_device()) return false;
+    m->values = v->data_ptr();
+    m->scales = s->data_ptr();
+    m->tensor_scale = static_cast<float *>(w->data_ptr());
+    m->rows = PyLong_AsUnsignedLongLong(args[3]);
+    m->cols = PyLong_AsUnsignedLongLong(args[4]);
+    m->format = (int32_t)PyLong_AsLong(args[5]);
+    m->device = (int32_t)v->get_device();
+    return true;
+}
+
+// fp4_quantize(X, matrix or None, matrix or None, given scale or None) -> None or a status: X by rows and by columns
+PyObject *fp4_quantize(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 14) {
+        PyErr_SetString(PyExc_TypeError, "fp4_quantize takes 14 arguments");
+        return nullptr;
+    }
+    const char *bad_x = "X must be a two-dimensional CUDA tensor of float32, float16 or bfloat16 with unit stride along rows or columns";
+    const at::Tensor *X = cuda_tensor(args[0]);
+    Dense x;
+    if (!X || type_code(X->scalar_type()) < 0 || !dense_of(*X, &x)) return refuse(bad_x);
+    b200spmm_fp4_t by_rows{}, by_cols{};
+    const bool rows = args[1] != Py_None, cols = args[7] != Py_None;
+    if ((rows && !matrix_of(args + 1, &by_rows)) || (cols && !matrix_of(args + 7, &by_cols))) return refuse("the matrix must be on one CUDA device");
+    if (PyErr_Occurred()) return nullptr;
+    const b200spmm_fp4_t &one = rows ? by_rows : by_cols;
+    if (X->get_device() != one.device) return refuse("X and the matrix must be on the same device");
+    const uint64_t r = (uint64_t)X->size(0), c = (uint64_t)X->size(1);
+    if ((rows && (by_rows.rows != r || by_rows.cols != c)) || (cols && (by_cols.rows != c || by_cols.cols != r))) return refuse("the matrix does not have the shape of X");
+    const float *given = nullptr;
+    if (args[13] != Py_None) {
+        const at::Tensor *g = cuda_tensor(args[13]);
+        if (!g || g->scalar_type() != at::kFloat || g->numel() != 1 || g->get_device() != one.device)
+            return refuse("tensor_scale must be a float32 tensor of one element on X's device");
+        given = static_cast<const float *>(g->data_ptr());
+    }
+    at::Tensor workspace;
+    if (one.format == B200SPMM_NVFP4 && !given) {
+        uint64_t bytes = 0;
+        b200spmm_fp4_sizes(0, 0, one.format, nullptr, nullptr, nullptr, &bytes);
+        workspace = new_cuda(1, (int64_t)bytes, at::kByte, *X);
+    }
+    void *ws = workspace.defined() ? workspace.data_ptr() : nullptr;
+    void *stream = c10::cuda::getCurrentCUDAStream(X->get_device()).stream();
+    const int code = type_code(X->scalar_type());
+    const b200spmm_fp4_t *first = x.transposed ? (cols ? &by_cols : nullptr) : (rows ? &by_rows : nullptr);   // along the rows as they lie
+    const b200spmm_fp4_t *second = x.transposed ? (rows ? &by_rows : nullptr) : (cols ? &by_cols : nullptr);  // ... across them
+    int st;
+    {
+        const ThreadsAllowed threads;
+        if (first && second) st = b200spmm_fp4_quantize_both(x.ptr, x.ld, code, given, first, second, ws, stream);
+        else st = b200spmm_fp4_quantize(x.ptr, x.ld, code, second != nullptr, given, first ? first : second, ws, stream);
+    }
+    if (st != B200SPMM_OK) return PyLong_FromLong(st);
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// C for a product of `rows` x `n`: the caller's, or a new one.  Null with an error set where it does not fit.
+bool output_of(PyObject *arg, int64_t rows, int64_t n, long type, const at::Tensor &like, at::Tensor *C, Dense *c) {
+    const char *bad = "C has the wrong shape, dtype, device or layout";
+    if (arg == Py_None) {
+        *C = new_cuda(rows, n, type_of(type), like);
+    } else {
+        const at::Tensor *t = cuda_tensor(arg);
+        if (!t || t->scalar_type() != type_of(type) || t->dim() != 2 || t->size(0) != rows || t->size(1) != n || t->get_device() != like.get_device()) {
+            refuse(bad);
+            return false;
+        }
+        *C = *t;
+    }
+    if (!dense_of(*C, c)) {
+        refuse(bad);
+        return false;
+    }
+    return true;
+}
+
+PyObject *result_of(int st, PyObject *arg, at::Tensor &&C) {
+    if (st != B200SPMM_OK) return PyLong_FromLong(st);
+    if (arg != Py_None) {
+        Py_INCREF(arg);
+        return arg;
+    }
+    return THPVariable_Wrap(std::move(C));
+}
+
+// fp4_dequantize(matrix, X or None, type) -> X or a status
+PyObject *fp4_dequantize(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    b200spmm_fp4_t a{};
+    if (n_args != 8 || !matrix_of(args, &a)) return refuse("the matrix must be on one CUDA device");
+    const long type = PyLong_AsLong(args[7]);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor &like = *cuda_tensor(args[0]);
+    at::Tensor X;
+    Dense x;
+    if (!output_of(args[6], (int64_t)a.rows, (int64_t)a.cols, type, like, &X, &x)) return nullptr;
+    if (x.transposed) return refuse("the values are written row by row: unit stride along the rows");
+    void *stream = c10::cuda::getCurrentCUDAStream(like.get_device()).stream();
+    int st;
+    {
+        const ThreadsAllowed threads;
+        st = b200spmm_fp4_dequantize(&a, x.ptr, x.ld, (int)type, stream);
+    }
+    return result_of(st, args[6], std::move(X));
+    END_HANDLE_TH_ERRORS
+}
+
+// fp4_product(matrix, matrix, C or None, type) -> C or a status
+PyObject *fp4_product(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    b200spmm_fp4_t a{}, b{};
+    if (n_args != 14 || !matrix_of(args, &a) || !matrix_of(args + 6, &b)) return refuse("the matrices must be on one CUDA device");
+    const long type = PyLong_AsLong(args[13]);
+    if (PyErr_Occurred()) return nullptr;
+    if (a.device != b.device) return refuse("the matrices must be on one CUDA device");
+    if (a.cols != b.cols) return refuse("the matrices must have the same number of columns");
+    const at::Tensor &like = *cuda_tensor(args[0]);
+    at::Tensor C;
+    Dense c;
+    if (!output_of(args[12], (int64_t)a.rows, (int64_t)b.rows, type, like, &C, &c)) return nullptr;
+    void *stream = c10::cuda::getCurrentCUDAStream(like.get_device()).stream();
+    int st;
+    {
+        const ThreadsAllowed threads;
+        st = b200spmm_fp4_product(&a, &b, c.ptr, c.ld, (int)type, c.transposed, stream);
+    }
+    return result_of(st, args[12], std::move(C));
+    END_HANDLE_TH_ERRORS
+}
+
+// fp4_dense_product(matrix, B, C or None, type) -> C or a status
+PyObject *fp4_dense_product(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    b200spmm_fp4_t a{};
+    if (n_args != 9 || !matrix_of(args, &a)) return refuse("the matrix must be on one CUDA device");
+    const long type = PyLong_AsLong(args[8]);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor *B = cuda_tensor(args[6]);
+    const int b_type = B ? type_code(B->scalar_type()) : -1;
+    Dense b;
+    if (!B || b_type < 0 || b_type == B200SPMM_T_F32 || !dense_of(*B, &b) || (uint64_t)B->size(0) != a.cols || B->get_device() != a.device)
+        return refuse("B must be a CUDA float16 or bfloat16 tensor of shape [cols, n] on the matrix's device with unit stride along rows or columns");
+    at::Tensor C;
+    Dense c;
+    if (!output_of(args[7], (int64_t)a.rows, B->size(1), type, *B, &C, &c)) return nullptr;
+    void *stream = c10::cuda::getCurrentCUDAStream(B->get_device()).stream();
+    const int64_t n = B->size(1);
+    int st;
+    {
+        const ThreadsAllowed threads;
+        st = b200spmm_fp4_dense_product(&a, b.ptr, b.ld, n, b_type, b.transposed, c.ptr, c.ld, (int)type, c.transposed, stream);
+    }
+    return result_of(st, args[7], std::move(C));
+    END_HANDLE_TH_ERRORS
+}
+
+template <PyObject *(*kFn)(PyObject *, PyObject *const *, Py_ssize_t)>
+PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kFn)); }
+
+PyMethodDef methods[] = {{"spmm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(spmm)), METH_FASTCALL, nullptr},
+                         {"fp4_quantize", fast<fp4_quantize>(), METH_FASTCALL, nullptr},
+                         {"fp4_dequantize", fast<fp4_dequantize>(), METH_FASTCALL, nullptr},
+                         {"fp4_product", fast<fp4_product>(), METH_FASTCALL, nullptr},
+                         {"fp4_dense_product", fast<fp4_dense_product>(), METH_FASTCALL, nullptr},
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

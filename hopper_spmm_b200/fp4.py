@@ -1,0 +1,199 @@
+"""Dense matrices in 4 bits a value, and their products (b200spmm_fp4_* of the C ABI).
+
+Beside the sparse forms of a weight matrix (``SpmmPlan``) stands the other way to make one smaller, fewer bits: e2m1 values with
+one scale per block of 16 (``nvfp4``) or 32 (``mxfp4``) neighbours of a row.  The reference has no such form (src/common.h:14-43).
+
+    W = fp4_quantize(weights)                      # [rows, cols] float32 / float16 / bfloat16, once
+    C = W.matmul(B)                                # B [cols, n] float16 or bfloat16: [rows, n], as SpmmPlan.spmm
+    C = W.matmul(fp4_quantize(X))                  # X [n, cols], both operands in 4 bits
+    W.matmul(x.t(), y.t(), dtype=y.dtype)          # activations that lie token by token, x [n, cols], y [n, rows]
+
+As everywhere in this package, what computes runs in libb200spmm.so; there is no fallback.
+"""
+from __future__ import annotations
+
+import contextlib
+
+from . import _capi as capi
+
+FORMATS = {"nvfp4": capi.NVFP4, "mxfp4": capi.MXFP4}
+_BLOCK = {"nvfp4": 16, "mxfp4": 32}
+
+_native = None
+
+
+def _lib():
+    """The native half of these calls; like the library itself it has no fallback."""
+    global _native
+    if _native is None:
+        import torch  # noqa: F401  (the module links against torch's libraries)
+        capi.lib()
+        try:
+            from . import _torch_binding
+        except ImportError as e:
+            raise RuntimeError("hopper_spmm_b200/_torch_binding.so is missing or unusable: build it with "
+                               "`python -m hopper_spmm_b200.build`") from e
+        _native = _torch_binding
+    return _native
+
+
+def _type_code(dtype):
+    import torch
+    try:
+        return {torch.float32: capi.T_F32, torch.float16: capi.T_F16, torch.bfloat16: capi.T_BF16}[dtype]
+    except KeyError:
+        raise TypeError("dtype must be float32, float16 or bfloat16") from None
+
+
+@contextlib.contextmanager
+def _on(stream, *tensors):
+    """Work and new tensors on `stream`, which the caching allocator is told about for the tensors of the call."""
+    import torch
+    with torch.cuda.stream(stream):
+        yield
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+
+
+class Fp4Matrix:
+    """A rows x cols matrix in 4 bits.  ``values`` uint8 [rows, pitch], ``scales`` uint8 and ``tensor_scale`` float32 [1] are CUDA
+    tensors in the layout that include/b200_spmm.h describes: give them (a checkpoint in that layout), or leave them
+    out for a matrix that ``fp4_quantize(..., out=)`` fills."""
+
+    __slots__ = ("rows", "cols", "format", "values", "scales", "tensor_scale", "_m")
+
+    def __init__(self, rows: int, cols: int, format: str = "nvfp4", *, values=None, scales=None, tensor_scale=None, device=None):
+        import torch
+        if format not in FORMATS:
+            raise ValueError(f"format must be one of {', '.join(FORMATS)}")
+        rows, cols = int(rows), int(cols)
+        if rows < 0 or cols < 0 or rows > 0x7FFFFFFF - 128 or cols > 0x7FFFFFFF - 256:
+            raise ValueError("rows and cols must lie between 0 and 2^31")
+        blk = _BLOCK[format]
+        pitch, n_scales = (cols + 31) // 32 * 16, (rows + 127) // 128 * ((cols + 4 * blk - 1) // (4 * blk)) * 512
+        if values is None and scales is None:
+            if tensor_scale is not None:
+                raise ValueError("values and scales are given together")
+            device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+            values = torch.empty((rows, pitch), dtype=torch.uint8, device=device)
+            scales = torch.empty(n_scales, dtype=torch.uint8, device=device)
+            tensor_scale = torch.empty(1, dtype=torch.float32, device=device)
+        elif values is None or scales is None or (tensor_scale is None and format == "nvfp4"):
+            raise ValueError("values, scales and, for nvfp4, tensor_scale are given together")
+        else:
+            if tensor_scale is None:
+                tensor_scale = torch.ones(1, dtype=torch.float32, device=values.device)
+            if (values.dtype != torch.uint8 or values.numel() != rows * pitch or scales.dtype != torch.uint8 or
+                    scales.numel() != n_scales or tensor_scale.dtype != torch.float32 or tensor_scale.numel() != 1 or
+                    not (values.is_contiguous() and scales.is_contiguous())):
+                raise ValueError(f"a {rows} x {cols} {format} matrix takes contiguous uint8 values of {rows * pitch} bytes and scales of "
+                                 f"{n_scales} bytes, and one float32 tensor_scale")
+        self.rows, self.cols, self.format = rows, cols, format
+        self.values, self.scales, self.tensor_scale = values, scales, tensor_scale
+        self._m = (values, scales, tensor_scale, rows, cols, FORMATS[format])
+
+    @property
+    def device(self):
+        return self.values.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.values.numel() + self.scales.numel() + 4
+
+    def dequantize(self, out=None, dtype=None, stream=None):
+        """The values it stands for, [rows, cols] in ``dtype`` (float32; with ``out``, its type)."""
+        import torch
+        dtype = (out.dtype if out is not None else torch.float32) if dtype is None else dtype
+        if stream is not None:
+            with _on(stream, self.values, self.scales, self.tensor_scale, out):
+                return self.dequantize(out, dtype)
+        out = _lib().fp4_dequantize(*self._m, out, _type_code(dtype))
+        if type(out) is int:
+            raise capi.SpmmError(out, "b200spmm_fp4_dequantize")
+        return out
+
+    def matmul(self, B, C_out=None, dtype=None, stream=None, sync: bool = True):
+        """This matrix times B: a float16 or bfloat16 tensor [cols, n] (mxfp4: bfloat16), or an Fp4Matrix of n rows with
+        blocks along the same columns, whose transpose is meant.  Returns C [rows, n] in ``dtype`` (float32; with
+        ``C_out``, its type).  B and C may lie row by row or column by column (``x.t()``)."""
+        import torch
+        dtype = (C_out.dtype if C_out is not None else torch.float32) if dtype is None else dtype
+        if stream is not None:
+            mine = (self.values, self.scales, self.tensor_scale, C_out)
+            with _on(stream, *mine, *((B.values, B.scales, B.tensor_scale) if isinstance(B, Fp4Matrix) else (B,))):
+                C_out = self.matmul(B, C_out, dtype, None, False)
+            if sync:
+                self.sync(stream)
+            return C_out
+        if isinstance(B, Fp4Matrix):
+            if B.format != self.format:
+                raise ValueError("both matrices must have the same format")
+            C_out, where = _lib().fp4_product(*self._m, *B._m, C_out, _type_code(dtype)), "b200spmm_fp4_product"
+        else:
+            if self.format == "mxfp4" and getattr(B, "dtype", None) == torch.float16:
+                raise ValueError("an mxfp4 matrix takes bfloat16: its scales go beyond the range of float16")
+            C_out, where = _lib().fp4_dense_product(*self._m, B, C_out, _type_code(dtype)), "b200spmm_fp4_dense_product"
+        if type(C_out) is int:
+            raise capi.SpmmError(C_out, where)
+        if sync:
+            self.sync()
+        return C_out
+
+    def sync(self, stream=None):
+        """Waits for ``stream`` (the current one) and raises if a product on this device ran out of time."""
+        import torch
+        s = (stream or torch.cuda.current_stream(self.values.device)).cuda_stream
+        capi.check(capi.lib().b200spmm_fp4_status(self.values.device.index, s), "b200spmm_fp4_status")
+
+
+_NONE = (None,) * 6
+
+
+def _check_x(X, format):
+    if format not in FORMATS:
+        raise ValueError(f"format must be one of {', '.join(FORMATS)}")
+    if getattr(X, "ndim", 0) != 2 or not X.is_cuda:
+        raise ValueError("X must be a two-dimensional CUDA tensor of float32, float16 or bfloat16 with unit stride along rows or columns")
+
+
+def _quantize(X, by_rows, by_cols, tensor_scale):
+    st = _lib().fp4_quantize(X, *(_NONE if by_rows is None else by_rows._m), *(_NONE if by_cols is None else by_cols._m), tensor_scale)
+    if st is not None:
+        raise capi.SpmmError(st, "b200spmm_fp4_quantize")
+
+
+def fp4_quantize(X, format: str = "nvfp4", axis: int = 1, tensor_scale=None, out: Fp4Matrix | None = None, stream=None) -> Fp4Matrix:
+    """X in 4 bits.  ``axis`` 1: blocks along X's rows, a matrix of X's shape; 0: along its columns, and the matrix is X's
+    transpose (the axis that a product sums over has to be the matrix's rows).  ``tensor_scale``: for nvfp4, a float32 tensor of
+    one element (say, calibrated) in place of a pass over X for its largest value.  ``out``: a matrix to fill, else a new one."""
+    _check_x(X, format)
+    if axis not in (0, 1):
+        raise ValueError("axis must be 0 or 1")
+    if stream is not None:
+        with _on(stream, X, tensor_scale, *(() if out is None else (out.values, out.scales, out.tensor_scale))):
+            return fp4_quantize(X, format, axis, tensor_scale, out)
+    rows, cols = X.shape if axis else (X.shape[1], X.shape[0])
+    if out is None:
+        out = Fp4Matrix(rows, cols, format, device=X.device)
+    elif out.format != format or (out.rows, out.cols) != (rows, cols):
+        raise ValueError(f"out must be a {rows} x {cols} matrix of {format}")
+    _quantize(X, out if axis else None, None if axis else out, tensor_scale)
+    return out
+
+
+def fp4_quantize_both(X, format: str = "nvfp4", tensor_scale=None, stream=None) -> tuple[Fp4Matrix, Fp4Matrix]:
+    """``fp4_quantize(X, axis=1)`` and ``fp4_quantize(X, axis=0)`` from one read of X: what training needs.  For Y = X Wᵀ the
+    forward pass sums over X's columns, the weights' gradient dYᵀ X over its rows:
+
+        X, Xt = fp4_quantize_both(x);  W, Wt = fp4_quantize_both(w);  dY, dYt = fp4_quantize_both(dy)
+        y, dx, dw = X.matmul(W), dY.matmul(Wt), dYt.matmul(Xt)
+    """
+    _check_x(X, format)
+    if stream is not None:
+        with _on(stream, X, tensor_scale):
+            return fp4_quantize_both(X, format, tensor_scale)
+    r, c = X.shape
+    both = Fp4Matrix(r, c, format, device=X.device), Fp4Matrix(c, r, format, device=X.device)
+    _quantize(X, *both, tensor_scale)
+    return both

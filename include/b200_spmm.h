@@ -489,6 +489,80 @@ typedef struct {
 } b200spmm_launch_info_t;
 int b200spmm_plan_launch_info(const b200spmm_plan_t *p, b200spmm_launch_info_t *info);
 
+/* ------------------------------------------------------------------ 4-bit matrices */
+
+/*
+ * A dense weight or activation matrix in 4 bits a value, and its products.  No counterpart in the reference, whose
+ * element types are fp16 and tf32 (src/common.h:14-43).  A value is
+ *     e2m1 code (0 0.5 1 1.5 2 3 4 6 and their negatives)  x  its block's scale  x  the tensor's scale
+ *   B200SPMM_NVFP4  blocks of 16 neighbours of a row, scales e4m3 (sign 0)
+ *   B200SPMM_MXFP4  blocks of 32, scales e8m0 (2^(byte - 127), 255 is NaN), tensor scale unused
+ * The arrays are the caller's, on `device`:
+ *   values        rows of `pitch` bytes (b200spmm_fp4_sizes: 16 for every 32 columns begun), two codes to a byte, the lower half
+ *                 first; zeros behind the last column; 16-byte aligned
+ *   scales        blocks of 128 rows x 4 scales in 512 bytes: scale j of row r at (r % 32) * 16 + (r / 32 % 4) * 4 + j % 4 of block
+ *                 (r / 128) * ceil(scales of a row / 4) + j / 4; zeros behind a row's last scale, anything in rows behind the last;
+ *                 16-byte aligned
+ *   tensor_scale  one fp32 number
+ */
+enum { B200SPMM_NVFP4 = 0, B200SPMM_MXFP4 = 1 };
+/* Element types of the dense matrices; the first two are B200SPMM_C_F32 and B200SPMM_C_F16. */
+enum { B200SPMM_T_F32 = 0, B200SPMM_T_F16 = 1, B200SPMM_T_BF16 = 2 };
+typedef struct {
+    uint64_t rows, cols;
+    int32_t format, device;
+    void *values, *scales;
+    float *tensor_scale;
+} b200spmm_fp4_t;
+
+/* Bytes of the arrays (any pointer may be null), and of the workspace of a quantisation.  Needs no device. */
+int b200spmm_fp4_sizes(uint64_t rows, uint64_t cols, int format, uint64_t *pitch, uint64_t *values_bytes, uint64_t *scales_bytes,
+                       uint64_t *workspace_bytes);
+
+/*
+ * Fills `out` from X, row-major with ldx elements between rows.  transposed == 0: blocks lie along the rows of X, out is
+ * rows x cols like X; else they lie along its columns and out is its transpose.
+ *   MXFP4  scale 2^(floor(log2 amax) - 2) of the block's largest magnitude amax, the exponent kept in [-127, 127]
+ *   NVFP4  tensor scale 2^k, the smallest power of two (k in [-126, 127]; 1 for zeros) with amax(X) / 2^k <= 2688; block scale
+ *          amax / 6 / 2^k rounded to e4m3.  With d_tensor_scale, a positive number on the device, 2^k is that number rounded up to
+ *          a power of two, X is read once, and what is too large for it becomes the largest value of its block.
+ *   codes  x / (block scale x tensor scale) rounded to the nearest, ties to the even code, at most 6; 0 where the scale is 0.
+ * All roundings are those of the real quotients.  A block with an infinity or a NaN becomes NaN as a whole (scale NaN, codes 0); such
+ * values do not count for amax(X).
+ * `workspace` (b200spmm_fp4_sizes; null for MXFP4 or with d_tensor_scale) belongs to the call until it is done on `stream`.
+ */
+int b200spmm_fp4_quantize(const void *d_X, int64_t ldx, int x_dtype, int transposed, const float *d_tensor_scale,
+                          const b200spmm_fp4_t *out, void *workspace, void *stream);
+/* Both ways from one call, with the same tensor scale: what a training step needs of a matrix that two of its products sum over. */
+int b200spmm_fp4_quantize_both(const void *d_X, int64_t ldx, int x_dtype, const float *d_tensor_scale, const b200spmm_fp4_t *by_rows,
+                               const b200spmm_fp4_t *by_cols, void *workspace, void *stream);
+
+/* X [rows, cols] = the values that `a` stands for, rounded to x_dtype. */
+int b200spmm_fp4_dequantize(const b200spmm_fp4_t *a, void *d_X, int64_t ldx, int x_dtype, void *stream);
+
+/*
+ * C[a.rows, b.rows] = A B^T of two matrices of one format and as many columns; sums in fp32.  C has ldc elements between rows;
+ * c_transposed != 0: between columns, which lie contiguously.
+ */
+int b200spmm_fp4_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *d_C, int64_t ldc, int c_dtype, int c_transposed,
+                         void *stream);
+
+/*
+ * C[a.rows, n] = A B with B [a.cols, n] in fp16 or bf16 (MXFP4: bf16, whose range its scales have; else
+ * B200SPMM_ERR_UNSUPPORTED); sums in fp32.  B and C have ldb and ldc elements between rows, or, where transposed, between columns:
+ * activations that lie token by token.  Any n, strides and alignment of B and C to their element; starts and strides that are
+ * multiples of 16 bytes are faster.
+ */
+int b200spmm_fp4_dense_product(const b200spmm_fp4_t *a, const void *d_B, int64_t ldb, int64_t n, int b_dtype, int b_transposed,
+                               void *d_C, int64_t ldc, int c_dtype, int c_transposed, void *stream);
+
+/*
+ * All of these are asynchronous on `stream`, run on the matrices' device whichever is current, allocate nothing and may be captured
+ * into CUDA graphs; calls that share no output or workspace may overlap.  This one waits for `stream` and returns
+ * B200SPMM_ERR_DEVICE_TIMEOUT if a bounded wait of a product on that device gave up since it was last asked.
+ */
+int b200spmm_fp4_status(int device, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
