@@ -59,8 +59,10 @@ int launch_dequantize(const b200spmm_fp4_t *a, void *x, int64_t ldx, int x_dtype
 int launch_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *c, int64_t ldc, int c_dtype, bool c_transposed,
                    cudaStream_t stream);
 int launch_dense_product(const b200spmm_fp4_t *a, const void *b, int64_t ldb, int64_t n, int b_dtype, bool b_transposed, void *c,
-                         int64_t ldc, int c_dtype, bool c_transposed, cudaStream_t stream);
+                         int64_t ldc, int c_dtype, bool c_transposed, float *workspace, uint64_t workspace_bytes, cudaStream_t stream);
+int dense_product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t *bytes);
 
+constexpr int kMaxDevices = 64;
 // The word in which kernels report a wait that ran out, on the current device.
 cudaError_t status_word(uint32_t **word);
 // Multiprocessors of the current device.

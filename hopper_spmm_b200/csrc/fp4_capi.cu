@@ -10,7 +10,6 @@ namespace {
 
 __device__ uint32_t g_status;  // of each device that loads the library
 
-constexpr int kMaxDevices = 64;
 std::atomic<uint32_t *> g_status_word[kMaxDevices];
 std::atomic<int> g_sms[kMaxDevices];
 
@@ -158,7 +157,19 @@ int b200spmm_fp4_dequantize(const b200spmm_fp4_t *a, void *d_X, int64_t ldx, int
     return on_device(a->device, [&]() -> int { return is_empty(a) ? B200SPMM_OK : launch_dequantize(a, d_X, ldx, x_dtype, static_cast<cudaStream_t>(stream)); });
 }
 
-int b200spmm_fp4_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *d_C, int64_t ldc, int c_dtype, int c_transposed, void *stream) {
+int b200spmm_fp4_product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t *bytes) {
+    if (!bytes || n < 0) return B200SPMM_ERR_INVALID_ARG;
+    *bytes = 0;
+    const int st = check_matrix(a);
+    if (st != B200SPMM_OK) return st;
+    if (n > 0x7FFFFFFF - 256) return B200SPMM_ERR_UNSUPPORTED;
+    return on_device(a->device, [&]() -> int { return is_empty(a) ? B200SPMM_OK : dense_product_workspace(a, n, bytes); });
+}
+
+int b200spmm_fp4_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *d_C, int64_t ldc, int c_dtype, int c_transposed, void *workspace,
+                         uint64_t workspace_bytes, void *stream) {
+    (void)workspace;
+    (void)workspace_bytes;
     int st = check_matrix(a);
     if (st == B200SPMM_OK) st = check_matrix(b);
     if (st != B200SPMM_OK) return st;
@@ -176,13 +187,14 @@ int b200spmm_fp4_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void 
 }
 
 int b200spmm_fp4_dense_product(const b200spmm_fp4_t *a, const void *d_B, int64_t ldb, int64_t n, int b_dtype, int b_transposed, void *d_C, int64_t ldc,
-                               int c_dtype, int c_transposed, void *stream) {
+                               int c_dtype, int c_transposed, void *workspace, uint64_t workspace_bytes, void *stream) {
     int st = check_matrix(a);
     if (st != B200SPMM_OK) return st;
     if (n < 0) return B200SPMM_ERR_INVALID_ARG;
     if (n > 0x7FFFFFFF - 256) return B200SPMM_ERR_UNSUPPORTED;
     st = check_dense(d_B, b_dtype, b_transposed ? (uint64_t)n : a->cols, b_transposed ? a->cols : (uint64_t)n, ldb);
     if (st != B200SPMM_OK) return st;
+    if (!aligned(workspace, 4)) return B200SPMM_ERR_INVALID_ARG;
     if (b_dtype == B200SPMM_T_F32 || (a->format == B200SPMM_MXFP4 && b_dtype != B200SPMM_T_BF16)) return B200SPMM_ERR_UNSUPPORTED;
     const uint64_t rows = c_transposed ? (uint64_t)n : a->rows, cols = c_transposed ? a->rows : (uint64_t)n;
     st = check_dense(d_C, c_dtype, rows, cols, ldc);
@@ -191,7 +203,7 @@ int b200spmm_fp4_dense_product(const b200spmm_fp4_t *a, const void *d_B, int64_t
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
         if (rows == 0 || cols == 0) return B200SPMM_OK;
         if (a->cols == 0) return zero_output(d_C, ldc, c_dtype, rows, cols, s);
-        return launch_dense_product(a, d_B, ldb, n, b_dtype, b_transposed != 0, d_C, ldc, c_dtype, c_transposed != 0, s);
+        return launch_dense_product(a, d_B, ldb, n, b_dtype, b_transposed != 0, d_C, ldc, c_dtype, c_transposed != 0, static_cast<float *>(workspace), workspace_bytes, s);
     });
 }
 

@@ -1,10 +1,13 @@
 // Product of a 4-bit matrix with a 16-bit dense one.
 #include <algorithm>
+#include <atomic>
 
 #include "common.hpp"
 #include "fp4.hpp"
 #include "fp4_dense_narrow.cuh"
+#include "fp4_dense_wide.cuh"
 #include "launch.hpp"
+#include "tensormap.hpp"
 
 namespace b200spmm {
 namespace fp4 {
@@ -39,10 +42,88 @@ int launch_narrow_rows(const DenseParams &prm, int device, cudaStream_t stream) 
     return launch_narrow<T, kMx, 2, 1, kTokens>(prm, device, stream);
 }
 
+// Pairs of CTAs of the wide kernel that the current device runs at once (its instances take the same room).
+int wide_pairs(int device, uint32_t *out) {
+    static std::atomic<uint32_t> known[kMaxDevices];
+    *out = known[device].load(std::memory_order_relaxed);
+    if (*out) return B200SPMM_OK;
+    auto kernel = fp4_wide_kernel<__half, false, true>;
+    B200_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WideCfg::kSmemBytes));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)sm_count() / 2u * 2u);
+    cfg.blockDim = dim3(WideCfg::kThreads);
+    cfg.dynamicSmemBytes = WideCfg::kSmemBytes;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    B200_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+    if (n < 1) return B200SPMM_ERR_UNSUPPORTED;
+    *out = (uint32_t)n;
+    known[device].store(*out, std::memory_order_relaxed);
+    return B200SPMM_OK;
+}
+
+template <typename T, bool kMx, bool kTokens>
+int launch_wide(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
+    uint32_t pairs = 0;
+    const int st = wide_pairs(a->device, &pairs);
+    if (st != B200SPMM_OK) return st;
+    auto kernel = fp4_wide_kernel<T, kMx, kTokens>;
+    static thread_local int configured = -1;
+    if (configured != a->device) {
+        B200_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WideCfg::kSmemBytes));
+        configured = a->device;
+    }
+    WideParams prm{};
+    prm.d = d;
+    prm.split = wide_split(d.m, d.n, d.k, pairs);
+    if (prm.split.parts > 1 && (!workspace || workspace_bytes < wide_workspace(prm.split))) prm.split = wide_split(d.m, d.n, d.k, 1);
+    prm.row_blocks = (d.m + 127u) / 128u;
+    prm.partial = workspace;
+    B200_CUDA_TRY(status_word(&prm.status));
+    prm.wait_limit_ns = kDeviceWaitLimitNs;
+    CUtensorMap ma, mb;
+    const auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const uint64_t pitch_b = (d.n > 1 || !kTokens) && (d.k > 1 || kTokens) ? (uint64_t)d.ldb * 2u : ((uint64_t)(kTokens ? d.k : d.n) * 2u + 15u) / 16u * 16u;
+    if (!encode_2d(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, d.pitch, d.m, d.pitch, kWideK / 2, 128, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) ||
+        !encode_2d(&mb, type, d.b, kTokens ? d.k : d.n, kTokens ? d.n : d.k, pitch_b, 64, kTokens ? prm.split.cols / 2u : kWideK, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) {
+        set_last_error_static("a tensor map of a product with a 4-bit matrix could not be made");
+        return B200SPMM_ERR_CUDA;
+    }
+    B200_CUDA_TRY(launch_after(kernel, dim3(2 * std::min(pairs, prm.split.items)), WideCfg::kThreads, WideCfg::kSmemBytes, 2, stream, ma, mb, prm));
+    if (prm.split.parts > 1)
+        B200_CUDA_TRY(launch_after(fp4_join_kernel, dim3((prm.split.items - prm.split.whole) / prm.split.parts, prm.split.cols / 32u), kWideRows, 0, 1, stream, prm.split,
+                                   (const float *)workspace, d.m, d.n, Widen<T, kMx>::kLeft, kMx ? (const float *)nullptr : d.whole, d.c));
+    return B200SPMM_OK;
+}
+
+// Up to 16 columns, and operands that no tensor map describes.
+bool is_narrow(const DenseParams &d) { return d.n <= 16 || !d.b_wide; }
+
+template <typename T, bool kMx, bool kTokens>
+int launch_dense(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
+    return is_narrow(d) ? launch_narrow_rows<T, kMx, kTokens>(d, a->device, stream) : launch_wide<T, kMx, kTokens>(a, d, workspace, workspace_bytes, stream);
+}
+
 }  // namespace
 
+int dense_product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t *bytes) {
+    *bytes = 0;
+    if (n <= 16) return B200SPMM_OK;
+    uint32_t pairs = 0;
+    const int st = wide_pairs(a->device, &pairs);
+    if (st != B200SPMM_OK) return st;
+    *bytes = wide_workspace(wide_split((uint32_t)a->rows, (uint32_t)n, (uint32_t)a->cols, pairs));
+    return B200SPMM_OK;
+}
+
 int launch_dense_product(const b200spmm_fp4_t *a, const void *b, int64_t ldb, int64_t n, int b_dtype, bool b_transposed, void *c, int64_t ldc, int c_dtype,
-                         bool c_transposed, cudaStream_t stream) {
+                         bool c_transposed, float *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
     const Layout l = layout_of(a->rows, a->cols, a->format);
     DenseParams prm{};
     prm.values = static_cast<const uint8_t *>(a->values);
@@ -57,11 +138,14 @@ int launch_dense_product(const b200spmm_fp4_t *a, const void *b, int64_t ldb, in
     prm.n = (uint32_t)n;
     prm.b_wide = reinterpret_cast<uintptr_t>(b) % 16u == 0 && ldb % 8 == 0;
     prm.c = target_of(c, ldc, c_dtype, c_transposed);
-    if (a->format == B200SPMM_MXFP4)
-        return b_transposed ? launch_narrow_rows<__nv_bfloat16, true, true>(prm, a->device, stream) : launch_narrow_rows<__nv_bfloat16, true, false>(prm, a->device, stream);
-    if (b_dtype == B200SPMM_T_F16)
-        return b_transposed ? launch_narrow_rows<__half, false, true>(prm, a->device, stream) : launch_narrow_rows<__half, false, false>(prm, a->device, stream);
-    return b_transposed ? launch_narrow_rows<__nv_bfloat16, false, true>(prm, a->device, stream) : launch_narrow_rows<__nv_bfloat16, false, false>(prm, a->device, stream);
+    auto run = [&](auto type, auto mx) {
+        using T = decltype(type);
+        constexpr bool kMx = decltype(mx)::value;
+        return b_transposed ? launch_dense<T, kMx, true>(a, prm, workspace, workspace_bytes, stream)
+                            : launch_dense<T, kMx, false>(a, prm, workspace, workspace_bytes, stream);
+    };
+    if (a->format == B200SPMM_MXFP4) return run(__nv_bfloat16(), std::true_type());
+    return b_dtype == B200SPMM_T_F16 ? run(__half(), std::false_type()) : run(__nv_bfloat16(), std::false_type());
 }
 
 }  // namespace fp4

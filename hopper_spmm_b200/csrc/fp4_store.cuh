@@ -1,6 +1,7 @@
 // From accumulators to C: the tensors' scales, the element type, either order of C.
 #pragma once
 
+#include "fp4.hpp"
 #include "fp4_convert.cuh"
 
 namespace b200spmm {

@@ -219,6 +219,13 @@ bool output_of(PyObject *arg, int64_t rows, int64_t n, long type, const at::Tens
     return true;
 }
 
+// The workspace of a product of `a` with n columns; nothing where it needs none (or cannot be asked: the product will say why).
+at::Tensor product_workspace(const b200spmm_fp4_t &a, int64_t n, const at::Tensor &like, uint64_t *bytes) {
+    *bytes = 0;
+    if (b200spmm_fp4_product_workspace(&a, n, bytes) != B200SPMM_OK || *bytes == 0) return at::Tensor();
+    return new_cuda(1, (int64_t)*bytes, at::kByte, like);
+}
+
 PyObject *result_of(int st, PyObject *arg, at::Tensor &&C) {
     if (st != B200SPMM_OK) return PyLong_FromLong(st);
     if (arg != Py_None) {
@@ -267,7 +274,7 @@ PyObject *fp4_product(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     int st;
     {
         const ThreadsAllowed threads;
-        st = b200spmm_fp4_product(&a, &b, c.ptr, c.ld, (int)type, c.transposed, stream);
+        st = b200spmm_fp4_product(&a, &b, c.ptr, c.ld, (int)type, c.transposed, nullptr, 0, stream);
     }
     return result_of(st, args[12], std::move(C));
     END_HANDLE_TH_ERRORS
@@ -290,10 +297,13 @@ PyObject *fp4_dense_product(PyObject *, PyObject *const *args, Py_ssize_t n_args
     if (!output_of(args[7], (int64_t)a.rows, B->size(1), type, *B, &C, &c)) return nullptr;
     void *stream = c10::cuda::getCurrentCUDAStream(B->get_device()).stream();
     const int64_t n = B->size(1);
+    uint64_t bytes;
+    const at::Tensor workspace = product_workspace(a, n, *B, &bytes);
+    void *ws = workspace.defined() ? workspace.data_ptr() : nullptr;
     int st;
     {
         const ThreadsAllowed threads;
-        st = b200spmm_fp4_dense_product(&a, b.ptr, b.ld, n, b_type, b.transposed, c.ptr, c.ld, (int)type, c.transposed, stream);
+        st = b200spmm_fp4_dense_product(&a, b.ptr, b.ld, n, b_type, b.transposed, c.ptr, c.ld, (int)type, c.transposed, ws, bytes, stream);
     }
     return result_of(st, args[7], std::move(C));
     END_HANDLE_TH_ERRORS

@@ -545,7 +545,7 @@ int b200spmm_fp4_dequantize(const b200spmm_fp4_t *a, void *d_X, int64_t ldx, int
  * c_transposed != 0: between columns, which lie contiguously.
  */
 int b200spmm_fp4_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *d_C, int64_t ldc, int c_dtype, int c_transposed,
-                         void *stream);
+                         void *workspace, uint64_t workspace_bytes, void *stream);
 
 /*
  * C[a.rows, n] = A B with B [a.cols, n] in fp16 or bf16 (MXFP4: bf16, whose range its scales have; else
@@ -554,7 +554,14 @@ int b200spmm_fp4_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void 
  * multiples of 16 bytes are faster.
  */
 int b200spmm_fp4_dense_product(const b200spmm_fp4_t *a, const void *d_B, int64_t ldb, int64_t n, int b_dtype, int b_transposed,
-                               void *d_C, int64_t ldc, int c_dtype, int c_transposed, void *stream);
+                               void *d_C, int64_t ldc, int c_dtype, int c_transposed, void *workspace, uint64_t workspace_bytes,
+                               void *stream);
+/*
+ * Bytes of the workspace with which a product of `a` with n columns shares out its work best: tiles that would leave part of the
+ * GPU without any are cut along k, and their sums meet there.  With less, or none (null), products run without.  It belongs to the
+ * call until that is done on `stream`.
+ */
+int b200spmm_fp4_product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t *bytes);
 
 /*
  * All of these are asynchronous on `stream`, run on the matrices' device whichever is current, allocate nothing and may be captured
