@@ -178,33 +178,40 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, 2) fp4_narrow_kernel(const 
             ptx::cp_async_commit();
             const uint32_t at = ring + i % kNarrowAhead * Cfg::kStepBytes;
             const uint4 sc = ptx::ld_shared_v4(at + 4u * 512u);
-#pragma unroll
-            for (uint32_t tile = 0; tile < 2; ++tile) {
+            auto multiply = [&](auto twice, uint32_t tile) {
+                constexpr bool kTwice = decltype(twice)::value;
                 const uint4 lo = ptx::ld_shared_v4(at + tile * 1024u), hi = ptx::ld_shared_v4(at + tile * 1024u + 512u);
                 const uint32_t s_lo = tile ? sc.z : sc.x, s_hi = tile ? sc.w : sc.y;
                 uint32_t sl[2], sh[2];
                 if constexpr (kMx) {
-                    sl[0] = sl[1] = W::scale(s_lo >> t * 8u & 0xFFu);
-                    sh[0] = sh[1] = W::scale(s_hi >> t * 8u & 0xFFu);
+                    sl[0] = sl[1] = W::template scale<kTwice>(s_lo >> t * 8u & 0xFFu);
+                    sh[0] = sh[1] = W::template scale<kTwice>(s_hi >> t * 8u & 0xFFu);
                 } else {
                     const uint32_t at_byte = (t & 1u) * 16u;
-                    sl[0] = W::scale(s_lo >> at_byte & 0xFFu);
-                    sl[1] = W::scale(s_lo >> (at_byte + 8u) & 0xFFu);
-                    sh[0] = W::scale(s_hi >> at_byte & 0xFFu);
-                    sh[1] = W::scale(s_hi >> (at_byte + 8u) & 0xFFu);
+                    sl[0] = W::template scale<kTwice>(s_lo >> at_byte & 0xFFu);
+                    sl[1] = W::template scale<kTwice>(s_lo >> (at_byte + 8u) & 0xFFu);
+                    sh[0] = W::template scale<kTwice>(s_hi >> at_byte & 0xFFu);
+                    sh[1] = W::template scale<kTwice>(s_hi >> (at_byte + 8u) & 0xFFu);
                 }
                 const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                 for (uint32_t w = 0; w < 4; ++w) {
-                    const uint32_t a0 = W::template pair<12>(wl[w], sl[w >> 1]), a1 = W::template pair<12>(wh[w], sh[w >> 1]);
-                    const uint32_t a2 = W::template pair<8>(wl[w], sl[w >> 1]), a3 = W::template pair<8>(wh[w], sh[w >> 1]);
+                    const uint32_t a0 = W::template pair<kTwice, 0>(wl[w], sl[w >> 1]), a1 = W::template pair<kTwice, 0>(wh[w], sh[w >> 1]);
+                    const uint32_t a2 = W::template pair<kTwice, 1>(wl[w], sl[w >> 1]), a3 = W::template pair<kTwice, 1>(wh[w], sh[w >> 1]);
 #pragma unroll
                     for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) mma_16x8x16<T>(acc[u][tile][nb], a0, a1, a2, a3, bf[nb][w][0], bf[nb][w][1]);
-                    const uint32_t c0 = W::template pair<4>(wl[w], sl[w >> 1]), c1 = W::template pair<4>(wh[w], sh[w >> 1]);
-                    const uint32_t c2 = W::template pair<0>(wl[w], sl[w >> 1]), c3 = W::template pair<0>(wh[w], sh[w >> 1]);
+                    const uint32_t c0 = W::template pair<kTwice, 2>(wl[w], sl[w >> 1]), c1 = W::template pair<kTwice, 2>(wh[w], sh[w >> 1]);
+                    const uint32_t c2 = W::template pair<kTwice, 3>(wl[w], sl[w >> 1]), c3 = W::template pair<kTwice, 3>(wh[w], sh[w >> 1]);
 #pragma unroll
                     for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) mma_16x8x16<T>(acc[u][tile][nb], c0, c1, c2, c3, bf[nb][w][2], bf[nb][w][3]);
                 }
+            };
+            if (kMx && __any_sync(0xFFFFFFFFu, W::needs_two(sc.x) || W::needs_two(sc.y) || W::needs_two(sc.z) || W::needs_two(sc.w))) {
+                multiply(std::true_type(), 0);
+                multiply(std::true_type(), 1);
+            } else {
+                multiply(std::false_type(), 0);
+                multiply(std::false_type(), 1);
             }
         }
     }

@@ -5,18 +5,18 @@
 // Bound: the tensor core's 16-bit rate, and below a hundred columns or so one read of A.  Two CTAs on neighbouring SMs share MMAs
 // of 256 rows x up to 256 columns (tcgen05.mma.cta_group::2): each brings half of B's columns, so that an SM fetches
 // 40 bytes a clock from L2 at the full rate where a CTA alone would need 72, more than that path gives (about 51).
-// A arrives packed, is widened by eight warps (exactly, see Widen) and goes through registers into tensor memory, from where the
+// A arrives packed, is widened by sixteen warps (exactly, see Widen) and goes through registers into tensor memory, from where the
 // MMA takes it: shared memory, which B keeps busy, sees its 4 bits only once.
 //
-// A step is 128 values of k.  Warps 0-7 of a CTA widen: lane = row of the warp's quarter of tensor memory, warps w and w + 4
-// take a half of the step each; after an item's last step they take the accumulator to C.  Warp 8 of the even CTA issues the
-// MMAs, warp 9 loads.
+// A step is 128 values of k.  Warps 0-15 of a CTA widen: lane = row of the warp's quarter of tensor memory, warps 4 g .. 4 g + 3
+// every fourth step, so that what a step has to wait for (its stage, its way to tensor memory) overlaps with three others;
+// after an item's last step they take the accumulator to C.  Warp 16 of the even CTA issues the MMAs, warp 17 loads.
 //
 //   full[s]   stage s has landed (TMA bytes, each CTA its own): the widening warps wait for it, with B's part of it
-//   ready[b]  buffer b of widened A is written in both CTAs (16 warps arrive at the even CTA)
+//   ready[b]  buffer b of widened A is written in both CTAs (eight warps arrive at the even CTA)
 //   empty[s]  the MMAs of the step in stage s are done (commit, in both CTAs): the stage and its buffer of widened A are free
-//   done      the accumulator of an item is complete (commit, in both CTAs).  The widening warps read it before they write the next item's
-//             first buffer, so ready[] also says that the accumulator is free.
+//   done      the accumulator of an item is complete (commit, in both CTAs)
+//   taken     all 32 warps have read it (they arrive at the even CTA)
 //
 // Items are tiles of C.  Those of the last, incomplete round are cut along k into parts, so that every pair has something to
 // do; their sums go to the workspace and a second kernel adds them up in order.
@@ -58,9 +58,11 @@ struct WideCfg {
     static constexpr uint32_t kBytesA = 128 * kWideK / 2, kBytesScales = 1024, kBoxBytes = 64 * 2 * 128, kBytesB = 2 * kBoxBytes;
     static constexpr uint32_t kStageBytes = kBytesA + kBytesScales + kBytesB, kStages = 5;
     static constexpr uint32_t kBuffers = 4, kBufferCols = kWideK / 2;  // of widened A, in tensor memory behind the accumulator
-    static constexpr int kWarps = 10, kThreads = 32 * kWarps;
+    static constexpr uint32_t kWideners = 16;
+    static_assert(kBuffers == kWideners / 4, "a group of four warps has a buffer of its own");
+    static constexpr int kWarps = kWideners + 2, kThreads = 32 * kWarps;
     static constexpr uint32_t kTmemCols = 512;
-    static constexpr uint32_t kBarriers = 2 * kStages + kBuffers + 2;
+    static constexpr uint32_t kBarriers = 2 * kStages + kBuffers + 3;
     static constexpr size_t kSmemBytes = 1024 + (size_t)kStages * kStageBytes + kBarriers * 8 + 16;
     static_assert(kWideCols + kBuffers * kBufferCols <= kTmemCols && kSmemBytes <= 227 * 1024, "memory of an SM");
 };
@@ -107,7 +109,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     auto full_bar = [&](uint32_t s) { return bars_addr + 8u * s; };
     auto empty_bar = [&](uint32_t s) { return bars_addr + 8u * (kStages + s); };
     auto ready_bar = [&](uint32_t b) { return bars_addr + 8u * (2 * kStages + b); };
-    const uint32_t done_bar = bars_addr + 8u * (2 * kStages + Cfg::kBuffers), drain_bar = done_bar + 8u;
+    const uint32_t done_bar = bars_addr + 8u * (2 * kStages + Cfg::kBuffers), taken_bar = done_bar + 8u, drain_bar = done_bar + 16u;
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(bars + Cfg::kBarriers);
     uint32_t *tmem_slot = const_cast<uint32_t *>(abort_flag) + 1;
 
@@ -121,15 +123,16 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             ptx::mbar_init(full_bar(s), 1);
             ptx::mbar_init(empty_bar(s), 1);
         }
-        for (uint32_t b = 0; b < Cfg::kBuffers; ++b) ptx::mbar_init(ready_bar(b), 16);
+        for (uint32_t b = 0; b < Cfg::kBuffers; ++b) ptx::mbar_init(ready_bar(b), 8);
         ptx::mbar_init(done_bar, 1);
+        ptx::mbar_init(taken_bar, 2 * Cfg::kWideners);
         ptx::mbar_init(drain_bar, 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&tmap_a);
         ptx::prefetch_tensormap(&tmap_b);
     }
-    if (warp == 8) {
+    if (warp == Cfg::kWideners) {
         ptx::tmem_alloc_pair(ptx::smem_u32(tmem_slot), Cfg::kTmemCols);
         ptx::tmem_relinquish_alloc_permit_pair();
     }
@@ -141,7 +144,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     ptx::tcgen05_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 9) {
+    if (warp == Cfg::kWideners + 1) {
         // =========================================================== loads
         uint32_t it = 0;
         bool alive = lane == 0;
@@ -166,7 +169,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 }
             }
         }
-    } else if (warp == 8) {
+    } else if (warp == Cfg::kWideners) {
         // =========================================================== MMAs (even CTA)
         if (rank == 0 && lane == 0) {
             constexpr uint32_t fmt = std::is_same<T, __half>::value ? ptx::kFmtF16 : ptx::kFmtBF16;
@@ -174,11 +177,12 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             // B [n][k]: 64 values of k a row of the swizzle, eight rows 1024 bytes.  [k][n]: 64 columns a row, eight k 1024 bytes, the next 64
             // columns a box away.
             const uint64_t b_desc0 = ptx::make_smem_desc(b_addr, kTokens ? 16u : Cfg::kBoxBytes, 1024, ptx::kSwizzle128B);
-            uint32_t it = 0;
+            uint32_t it = 0, round = 0;
             bool alive = true;
-            for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs) {
+            for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs, ++round) {
                 const WideItem w = wide_item(p.split, item);
-                for (uint32_t step = w.first; step < w.last; ++step, ++it) {
+                if (round) alive = ptx::mbar_wait_cluster(taken_bar, (round - 1u) & 1u, abort_flag, limit);
+                for (uint32_t step = w.first; alive && step < w.last; ++step, ++it) {
                     const uint32_t s = it % kStages, b = it % Cfg::kBuffers;
                     alive = ptx::mbar_wait_cluster(ready_bar(b), it / Cfg::kBuffers & 1u, abort_flag, limit);
                     if (!alive) break;
@@ -200,9 +204,12 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         }
     } else {
         // =========================================================== widening, and C
-        const uint32_t q = warp & 3u, half = warp >> 2, row = q * 32u + lane;
+        const uint32_t q = warp & 3u, mine = warp >> 2, row = q * 32u + lane;
         const uint32_t lanes = (q * 32u) << 16;
         const float whole = (kMx ? 1.f : *reinterpret_cast<const volatile float *>(p.d.whole));
+        const uint32_t ready = rank == 0 ? ready_bar(mine) : ptx::map_to_cta(ready_bar(mine), 0);
+        const uint32_t taken = rank == 0 ? taken_bar : ptx::map_to_cta(taken_bar, 0);
+        const uint32_t buffer = tmem + lanes + kWideCols + mine * Cfg::kBufferCols;
         uint32_t it = 0, round = 0;
         bool alive = true;
         auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -212,54 +219,63 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         };
         for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs, ++round) {
             const WideItem w = wide_item(p.split, item);
-            for (uint32_t step = w.first; step < w.last; ++step, ++it) {
-                const uint32_t s = it % kStages, b = it % Cfg::kBuffers;
-                alive = wait(full_bar(s), it / kStages & 1u);
-                if (alive && it >= Cfg::kBuffers) {
-                    const uint32_t old = it - Cfg::kBuffers;
-                    alive = wait(empty_bar(old % kStages), old / kStages & 1u);
-                }
+            const uint32_t skip = (mine - it) % Cfg::kBuffers;  // steps until this warp's first one
+            for (uint32_t step = w.first + skip; step < w.last; step += Cfg::kBuffers) {
+                const uint32_t now = it + (step - w.first), s = now % kStages;
+                alive = wait(full_bar(s), now / kStages & 1u);
                 if (!alive) break;
-                // 64 values: bytes 32 half .. + 31 of the row's 64, pieces of 16 bytes in the order of the 64-byte swizzle
+                // the row's 64 bytes, pieces of 16 in the order of the 64-byte swizzle, and its words of scales
                 const uint32_t src = a_addr + s * Cfg::kBytesA + row * 64u, turn = row >> 1 & 3u;
-                uint32_t codes[8];
+                uint4 codes[4];
 #pragma unroll
-                for (uint32_t i = 0; i < 2; ++i) {
-                    const uint4 v = ptx::ld_shared_v4(src + ((half * 2u + i) ^ turn) * 16u);
-                    codes[4 * i] = v.x; codes[4 * i + 1] = v.y; codes[4 * i + 2] = v.z; codes[4 * i + 3] = v.w;
-                }
-                const uint32_t group = kMx ? 0u : half;
-                uint32_t four = 0;  // scales of what lies past the last column: zeros (there is no group that was not loaded)
-                if (step * kWideK + half * 64u < p.d.k)
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(four) : "r"(s_addr + s * Cfg::kBytesScales + group * 512u + lane * 16u + q * 4u) : "memory");
-                uint32_t out[32];
+                for (uint32_t i = 0; i < 4; ++i) codes[i] = ptx::ld_shared_v4(src + (i ^ turn) * 16u);
+                uint32_t four[2] = {0u, 0u};  // scales of what lies past the last column: zeros (there is no group that was not loaded)
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) {  // eight values each
-                    const uint32_t sc = kMx ? W::scale(four >> (half * 16u + i / 4u * 8u) & 0xFFu) : W::scale(four >> (i / 2u * 8u) & 0xFFu);
-                    const uint32_t p0 = W::template pair<12>(codes[i], sc), p1 = W::template pair<8>(codes[i], sc);
-                    const uint32_t p2 = W::template pair<4>(codes[i], sc), p3 = W::template pair<0>(codes[i], sc);
-                    out[4 * i] = __byte_perm(p0, p1, 0x5410);  // (0, 4) and (1, 5) to (0, 1) and (4, 5)
-                    out[4 * i + 1] = __byte_perm(p2, p3, 0x5410);
-                    out[4 * i + 2] = __byte_perm(p0, p1, 0x7632);
-                    out[4 * i + 3] = __byte_perm(p2, p3, 0x7632);
+                for (uint32_t g = 0; g < (kMx ? 1u : 2u); ++g)
+                    if (step * kWideK + g * 64u < p.d.k)
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(four[g]) : "r"(s_addr + s * Cfg::kBytesScales + g * 512u + lane * 16u + q * 4u) : "memory");
+                const bool two = W::needs_two(four[0]) || W::needs_two(four[1]);
+                const bool any_two = kMx && __any_sync(0xFFFFFFFFu, two);
+                if (now >= Cfg::kBuffers) {
+                    const uint32_t old = now - Cfg::kBuffers;
+                    alive = wait(empty_bar(old % kStages), old / kStages & 1u);
+                    if (!alive) break;
                 }
                 ptx::tcgen05_fence_after_sync();
-                ptx::tmem_st_32x32b_x32(tmem + lanes + kWideCols + b * Cfg::kBufferCols + half * 32u, out);
+                auto widen = [&](auto twice, uint32_t h) {
+                    uint32_t out[32];
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i) {  // eight values each
+                        const uint4 &c4 = codes[2 * h + i / 4];
+                        const uint32_t c = i % 4 == 0 ? c4.x : i % 4 == 1 ? c4.y : i % 4 == 2 ? c4.z : c4.w;
+                        const uint32_t sc = W::template scale<decltype(twice)::value>(kMx ? four[0] >> (h * 16u + i / 4u * 8u) & 0xFFu : four[h] >> (i / 2u * 8u) & 0xFFu);
+                        W::template eight<decltype(twice)::value>(c, sc, out + 4 * i);
+                    }
+                    ptx::tmem_st_32x32b_x32(buffer + h * 32u, out);
+                };
+                if (any_two) {
+                    widen(std::true_type(), 0);
+                    widen(std::true_type(), 1);
+                } else {
+                    widen(std::false_type(), 0);
+                    widen(std::false_type(), 1);
+                }
                 ptx::tmem_st_wait();
                 ptx::tcgen05_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
-                    if (rank == 0) ptx::mbar_arrive(ready_bar(b));
-                    else ptx::mbar_arrive_cluster_relaxed(ptx::map_to_cta(ready_bar(b), 0));
+                    if (rank == 0) ptx::mbar_arrive(ready);
+                    else ptx::mbar_arrive_cluster_relaxed(ready);
                 }
             }
             if (!alive) break;
+            it += w.last - w.first;
             alive = wait(done_bar, round & 1u);
             if (!alive) break;
             ptx::tcgen05_fence_after_sync();
             const uint32_t c_row = w.m0 + rank * 128u + row;
 #pragma unroll 1
-            for (uint32_t c = half * 32u; c < p.split.cols; c += 64u) {
+            for (uint32_t c = mine * 32u; c < p.split.cols; c += 128u) {
                 uint32_t r[32];
                 ptx::tmem_ld_32x32b_x32(tmem + lanes + c, r);
                 ptx::tmem_ld_wait();
@@ -275,6 +291,11 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 }
             }
             ptx::tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if (rank == 0) ptx::mbar_arrive(taken);
+                else ptx::mbar_arrive_cluster_relaxed(taken);
+            }
         }
     }
     __syncwarp();
@@ -287,7 +308,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     __syncthreads();
     ptx::cluster_arrive();  // neither CTA lets go of what the other's MMAs, commits or arrives may still reach
     ptx::cluster_wait();
-    if (warp == 8) {
+    if (warp == Cfg::kWideners) {
         ptx::tcgen05_fence_after_sync();
         ptx::tmem_dealloc_pair(tmem, Cfg::kTmemCols);
     }
