@@ -57,7 +57,8 @@ int launch_quantize(const void *x, int64_t ldx, int x_dtype, uint64_t x_rows, ui
                     const b200spmm_fp4_t *by_rows, const b200spmm_fp4_t *by_cols, float *workspace, cudaStream_t stream);
 int launch_dequantize(const b200spmm_fp4_t *a, void *x, int64_t ldx, int x_dtype, cudaStream_t stream);
 int launch_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *c, int64_t ldc, int c_dtype, bool c_transposed,
-                   cudaStream_t stream);
+                   float *workspace, uint64_t workspace_bytes, cudaStream_t stream);
+int product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t *bytes);
 int launch_dense_product(const b200spmm_fp4_t *a, const void *b, int64_t ldb, int64_t n, int b_dtype, bool b_transposed, void *c,
                          int64_t ldc, int c_dtype, bool c_transposed, float *workspace, uint64_t workspace_bytes, cudaStream_t stream);
 int dense_product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t *bytes);

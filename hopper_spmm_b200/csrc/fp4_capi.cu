@@ -163,17 +163,23 @@ int b200spmm_fp4_product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t 
     const int st = check_matrix(a);
     if (st != B200SPMM_OK) return st;
     if (n > 0x7FFFFFFF - 256) return B200SPMM_ERR_UNSUPPORTED;
-    return on_device(a->device, [&]() -> int { return is_empty(a) ? B200SPMM_OK : dense_product_workspace(a, n, bytes); });
+    return on_device(a->device, [&]() -> int { 
+        if (is_empty(a)) return B200SPMM_OK;
+        uint64_t four = 0, sixteen = 0;
+        int s = product_workspace(a, n, &four);
+        if (s == B200SPMM_OK) s = dense_product_workspace(a, n, &sixteen);
+        if (s == B200SPMM_OK) *bytes = four > sixteen ? four : sixteen;
+        return s;
+    });
 }
 
 int b200spmm_fp4_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *d_C, int64_t ldc, int c_dtype, int c_transposed, void *workspace,
                          uint64_t workspace_bytes, void *stream) {
-    (void)workspace;
-    (void)workspace_bytes;
     int st = check_matrix(a);
     if (st == B200SPMM_OK) st = check_matrix(b);
     if (st != B200SPMM_OK) return st;
     if (a->cols != b->cols || a->device != b->device) return B200SPMM_ERR_INVALID_ARG;
+    if (!aligned(workspace, 4)) return B200SPMM_ERR_INVALID_ARG;
     if (a->format != b->format) return B200SPMM_ERR_UNSUPPORTED;
     const uint64_t rows = c_transposed ? b->rows : a->rows, cols = c_transposed ? a->rows : b->rows;
     st = check_dense(d_C, c_dtype, rows, cols, ldc);
@@ -182,7 +188,7 @@ int b200spmm_fp4_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void 
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
         if (rows == 0 || cols == 0) return B200SPMM_OK;
         if (a->cols == 0) return zero_output(d_C, ldc, c_dtype, rows, cols, s);
-        return launch_product(a, b, d_C, ldc, c_dtype, c_transposed != 0, s);
+        return launch_product(a, b, d_C, ldc, c_dtype, c_transposed != 0, static_cast<float *>(workspace), workspace_bytes, s);
     });
 }
 

@@ -42,29 +42,17 @@ int launch_narrow_rows(const DenseParams &prm, int device, cudaStream_t stream) 
     return launch_narrow<T, kMx, 2, 1, kTokens>(prm, device, stream);
 }
 
+// Columns shared out evenly over as few tiles as there can be; a part has at least four steps: shorter ones are not worth their
+// sums' way through memory.
+Split wide_split(uint32_t m, uint32_t n, uint32_t k, uint32_t pairs) {
+    const uint32_t tiles_n = (n + kPairCols4 - 1) / kPairCols4, cols = ((n + tiles_n - 1) / tiles_n + 31u) / 32u * 32u;
+    return make_split(m, n, cols, (k + kWideK - 1) / kWideK, 4, pairs);
+}
+
 // Pairs of CTAs of the wide kernel that the current device runs at once (its instances take the same room).
 int wide_pairs(int device, uint32_t *out) {
     static std::atomic<uint32_t> known[kMaxDevices];
-    *out = known[device].load(std::memory_order_relaxed);
-    if (*out) return B200SPMM_OK;
-    auto kernel = fp4_wide_kernel<__half, false, true>;
-    B200_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WideCfg::kSmemBytes));
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)sm_count() / 2u * 2u);
-    cfg.blockDim = dim3(WideCfg::kThreads);
-    cfg.dynamicSmemBytes = WideCfg::kSmemBytes;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    B200_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
-    if (n < 1) return B200SPMM_ERR_UNSUPPORTED;
-    *out = (uint32_t)n;
-    known[device].store(*out, std::memory_order_relaxed);
-    return B200SPMM_OK;
+    return max_pairs(fp4_wide_kernel<__half, false, true>, WideCfg::kThreads, WideCfg::kSmemBytes, known[device], out);
 }
 
 template <typename T, bool kMx, bool kTokens>
@@ -81,7 +69,7 @@ int launch_wide(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace,
     WideParams prm{};
     prm.d = d;
     prm.split = wide_split(d.m, d.n, d.k, pairs);
-    if (prm.split.parts > 1 && (!workspace || workspace_bytes < wide_workspace(prm.split))) prm.split = wide_split(d.m, d.n, d.k, 1);
+    if (prm.split.parts > 1 && (!workspace || workspace_bytes < split_workspace(prm.split))) prm.split = wide_split(d.m, d.n, d.k, 1);
     prm.row_blocks = (d.m + 127u) / 128u;
     prm.partial = workspace;
     B200_CUDA_TRY(status_word(&prm.status));
@@ -97,8 +85,8 @@ int launch_wide(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace,
     }
     B200_CUDA_TRY(launch_after(kernel, dim3(2 * std::min(pairs, prm.split.items)), WideCfg::kThreads, WideCfg::kSmemBytes, 2, stream, ma, mb, prm));
     if (prm.split.parts > 1)
-        B200_CUDA_TRY(launch_after(fp4_join_kernel, dim3((prm.split.items - prm.split.whole) / prm.split.parts, prm.split.cols / 32u), kWideRows, 0, 1, stream, prm.split,
-                                   (const float *)workspace, d.m, d.n, Widen<T, kMx>::kLeft, kMx ? (const float *)nullptr : d.whole, d.c));
+        B200_CUDA_TRY(launch_after(fp4_join_kernel, dim3((prm.split.items - prm.split.whole) / prm.split.parts, prm.split.cols / 32u), kPairRows4, 0, 1, stream, prm.split,
+                                   (const float *)workspace, d.m, d.n, kMx ? (const float *)nullptr : d.whole, (const float *)nullptr, Widen<T, kMx>::kLeft, d.c));
     return B200SPMM_OK;
 }
 
@@ -118,7 +106,7 @@ int dense_product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t *bytes)
     uint32_t pairs = 0;
     const int st = wide_pairs(a->device, &pairs);
     if (st != B200SPMM_OK) return st;
-    *bytes = wide_workspace(wide_split((uint32_t)a->rows, (uint32_t)n, (uint32_t)a->cols, pairs));
+    *bytes = split_workspace(wide_split((uint32_t)a->rows, (uint32_t)n, (uint32_t)a->cols, pairs));
     return B200SPMM_OK;
 }
 

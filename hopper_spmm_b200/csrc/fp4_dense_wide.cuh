@@ -18,41 +18,15 @@
 //   done      the accumulator of an item is complete (commit, in both CTAs)
 //   taken     all 32 warps have read it (they arrive at the even CTA)
 //
-// Items are tiles of C.  Those of the last, incomplete round are cut along k into parts, so that every pair has something to
-// do; their sums go to the workspace and a second kernel adds them up in order.
 #pragma once
 
+#include "fp4_split.cuh"
 #include "fp4_widen.cuh"
 
 namespace b200spmm {
 namespace fp4 {
 
-constexpr uint32_t kWideK = 128, kWideRows = 256, kWideCols = 256;
-
-// How C is shared out over `pairs` pairs: tiles of 256 rows x `cols` columns, row blocks of them one after the other.
-struct WideSplit {
-    uint32_t cols;        // of a tile, a multiple of 32
-    uint32_t tiles_n;     // tiles side by side
-    uint32_t whole;       // tiles that one pair makes alone
-    uint32_t parts;       // of the others
-    uint32_t items;
-    uint32_t steps;       // of k
-};
-
-inline WideSplit wide_split(uint32_t m, uint32_t n, uint32_t k, uint32_t pairs) {
-    WideSplit s{};
-    s.tiles_n = (n + kWideCols - 1) / kWideCols;
-    s.cols = ((n + s.tiles_n - 1) / s.tiles_n + 31u) / 32u * 32u;
-    s.steps = (k + kWideK - 1) / kWideK;
-    const uint32_t tiles = (m + kWideRows - 1) / kWideRows * s.tiles_n, rest = tiles % pairs;
-    // a part has at least four steps: shorter ones are not worth their sums' way through memory
-    s.parts = rest ? std::min(pairs / rest, s.steps / 4) : 1;
-    if (s.parts < 2) s.parts = 1;
-    s.whole = s.parts > 1 ? tiles - rest : tiles;
-    s.items = s.whole + (tiles - s.whole) * s.parts;
-    return s;
-}
-inline uint64_t wide_workspace(const WideSplit &s) { return (uint64_t)(s.items - s.whole) * kWideRows * s.cols * sizeof(float); }
+constexpr uint32_t kWideK = 128;  // of a step
 
 struct WideCfg {
     static constexpr uint32_t kBytesA = 128 * kWideK / 2, kBytesScales = 1024, kBoxBytes = 64 * 2 * 128, kBytesB = 2 * kBoxBytes;
@@ -64,33 +38,17 @@ struct WideCfg {
     static constexpr uint32_t kTmemCols = 512;
     static constexpr uint32_t kBarriers = 2 * kStages + kBuffers + 3;
     static constexpr size_t kSmemBytes = 1024 + (size_t)kStages * kStageBytes + kBarriers * 8 + 16;
-    static_assert(kWideCols + kBuffers * kBufferCols <= kTmemCols && kSmemBytes <= 227 * 1024, "memory of an SM");
+    static_assert(kPairCols4 + kBuffers * kBufferCols <= kTmemCols && kSmemBytes <= 227 * 1024, "memory of an SM");
 };
 
 struct WideParams {
     DenseParams d;
-    WideSplit split;
+    Split split;
     uint32_t row_blocks;
     float *partial;
     uint32_t *status;
     unsigned long long wait_limit_ns;
 };
-
-struct WideItem {
-    uint32_t m0, n0, first, last;  // steps [first, last)
-    uint32_t slot;                 // of a part, else ~0
-};
-B200_DEVICE WideItem wide_item(const WideSplit &s, uint32_t i) {
-    uint32_t tile = i, part = 0, parts = 1, slot = ~0u;
-    if (i >= s.whole) {
-        slot = i - s.whole;
-        tile = s.whole + slot / s.parts;
-        part = slot % s.parts;
-        parts = s.parts;
-    }
-    if (parts == 1) slot = ~0u;
-    return {tile / s.tiles_n * kWideRows, tile % s.tiles_n * s.cols, part * s.steps / parts, (part + 1) * s.steps / parts, slot};
-}
 
 template <typename T, bool kMx, bool kTokens>
 __global__ void __launch_bounds__(WideCfg::kThreads, 1)
@@ -149,7 +107,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         uint32_t it = 0;
         bool alive = lane == 0;
         for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs) {
-            const WideItem w = wide_item(p.split, item);
+            const Item w = split_item(p.split, item);
             const uint32_t row_block = w.m0 / 128u + rank;
             const uint32_t n0 = w.n0 + rank * cols_half;
             const uint32_t boxes = kTokens ? 2u : (cols_half + 63u) / 64u;
@@ -173,14 +131,14 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         // =========================================================== MMAs (even CTA)
         if (rank == 0 && lane == 0) {
             constexpr uint32_t fmt = std::is_same<T, __half>::value ? ptx::kFmtF16 : ptx::kFmtBF16;
-            const uint32_t idesc = ptx::make_instr_desc(fmt, kWideRows, p.split.cols, false, !kTokens);
+            const uint32_t idesc = ptx::make_instr_desc(fmt, kPairRows4, p.split.cols, false, !kTokens);
             // B [n][k]: 64 values of k a row of the swizzle, eight rows 1024 bytes.  [k][n]: 64 columns a row, eight k 1024 bytes, the next 64
             // columns a box away.
             const uint64_t b_desc0 = ptx::make_smem_desc(b_addr, kTokens ? 16u : Cfg::kBoxBytes, 1024, ptx::kSwizzle128B);
             uint32_t it = 0, round = 0;
             bool alive = true;
             for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs, ++round) {
-                const WideItem w = wide_item(p.split, item);
+                const Item w = split_item(p.split, item);
                 if (round) alive = ptx::mbar_wait_cluster(taken_bar, (round - 1u) & 1u, abort_flag, limit);
                 for (uint32_t step = w.first; alive && step < w.last; ++step, ++it) {
                     const uint32_t s = it % kStages, b = it % Cfg::kBuffers;
@@ -188,7 +146,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     if (!alive) break;
                     ptx::tcgen05_fence_after_sync();
                     const uint32_t n_mma = min(kWideK / 16u, (p.d.k - step * kWideK + 15u) / 16u);
-                    const uint32_t a = tmem + kWideCols + b * Cfg::kBufferCols;
+                    const uint32_t a = tmem + kPairCols4 + b * Cfg::kBufferCols;
                     for (uint32_t i = 0; i < n_mma; ++i) {
                         const uint32_t at = s * Cfg::kBytesB + (kTokens ? i / 4u * Cfg::kBoxBytes + i % 4u * 32u : i * 2048u);
                         ptx::umma_pair_f16_ts(tmem, a + i * 8u, b_desc0 + (at >> 4), idesc, step > w.first || i ? 1u : 0u);
@@ -209,7 +167,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const float whole = (kMx ? 1.f : *reinterpret_cast<const volatile float *>(p.d.whole));
         const uint32_t ready = rank == 0 ? ready_bar(mine) : ptx::map_to_cta(ready_bar(mine), 0);
         const uint32_t taken = rank == 0 ? taken_bar : ptx::map_to_cta(taken_bar, 0);
-        const uint32_t buffer = tmem + lanes + kWideCols + mine * Cfg::kBufferCols;
+        const uint32_t buffer = tmem + lanes + kPairCols4 + mine * Cfg::kBufferCols;
         uint32_t it = 0, round = 0;
         bool alive = true;
         auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -218,7 +176,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0u;
         };
         for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs, ++round) {
-            const WideItem w = wide_item(p.split, item);
+            const Item w = split_item(p.split, item);
             const uint32_t skip = (mine - it) % Cfg::kBuffers;  // steps until this warp's first one
             for (uint32_t step = w.first + skip; step < w.last; step += Cfg::kBuffers) {
                 const uint32_t now = it + (step - w.first), s = now % kStages;
@@ -280,9 +238,9 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 ptx::tmem_ld_32x32b_x32(tmem + lanes + c, r);
                 ptx::tmem_ld_wait();
                 if (w.slot != ~0u) {  // column by column: neighbouring lanes write neighbours
-                    float *dst = p.partial + ((uint64_t)w.slot * p.split.cols + c) * kWideRows + rank * 128u + row;
+                    float *dst = p.partial + ((uint64_t)w.slot * p.split.cols + c) * kPairRows4 + rank * 128u + row;
 #pragma unroll
-                    for (uint32_t i = 0; i < 32; ++i) dst[i * kWideRows] = __uint_as_float(r[i]);
+                    for (uint32_t i = 0; i < 32; ++i) dst[i * kPairRows4] = __uint_as_float(r[i]);
                 } else if (c_row < p.d.m && w.n0 + c < p.d.n) {
                     float v[32];
 #pragma unroll
@@ -313,25 +271,6 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         ptx::tmem_dealloc_pair(tmem, Cfg::kTmemCols);
     }
     if (tid == 0 && *abort_flag) atomicOr(p.status, kDevStatusTimeout);
-}
-
-// C of the tiles that were cut: the parts' sums in order.  A thread a row and 32 columns.
-__global__ void __launch_bounds__(kWideRows) fp4_join_kernel(const WideSplit s, const float *__restrict__ partial, uint32_t m, uint32_t n, float left,
-                                                             const float *__restrict__ whole, const Target c) {
-    ptx::wait_for_grids_before();
-    const float f = left * (whole ? *reinterpret_cast<const volatile float *>(whole) : 1.f);
-    const uint32_t tile = s.whole + blockIdx.x, col = blockIdx.y * 32u;
-    const uint32_t row = tile / s.tiles_n * kWideRows + threadIdx.x, n0 = tile % s.tiles_n * s.cols + col;
-    if (row >= m || n0 >= n) return;
-    float v[32] = {};
-    for (uint32_t part = 0; part < s.parts; ++part) {
-        const float *src = partial + ((uint64_t)(blockIdx.x * s.parts + part) * s.cols + col) * kWideRows + threadIdx.x;
-#pragma unroll
-        for (uint32_t i = 0; i < 32; ++i) v[i] += src[i * kWideRows];
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < 32; ++i) v[i] *= f;
-    store_row(c, row, n0, n, v);
 }
 
 }  // namespace fp4

@@ -2,17 +2,20 @@
 //
 //     C[m, n] = s_A s_B  sum over k  (a[m, k] sa[m, k / block]) (b[n, k] sb[n, k / block])
 //
+// Two kernels.  Few columns (up to 64, decoding): blocks of threads of their own, below; bound by one read of the longer operand.
+// More: pairs of CTAs (fp4_product_pair.cuh).
+//
 // tcgen05.mma takes 128 rows of A, up to 256 of B and 64 values of k a call and applies the scales itself.  A block of
 // threads makes a tile of C: one thread brings stages of 256 values of k (128 bytes of a row: one swizzled TMA box an operand,
-// and the scales, which lie as they are needed, by bulk copies), one thread copies the scales to tensor memory and issues the
-// MMAs, four warps take the finished accumulator to C.
+// and the scales, which lie as they are needed, by bulk copies), four warps bring the scales to tensor memory and at the end
+// the accumulator to C, one thread issues the MMAs.
 #include <algorithm>
-#include <cmath>
+#include <atomic>
 
 #include "common.hpp"
 #include "fp4.hpp"
 #include "fp4_convert.cuh"
-#include "fp4_store.cuh"
+#include "fp4_product_pair.cuh"
 #include "launch.hpp"
 #include "tensormap.hpp"
 
@@ -20,33 +23,23 @@ namespace b200spmm {
 namespace fp4 {
 namespace {
 
-constexpr uint32_t kTileM = 128, kStageK = 256, kMmaK = 64;
-constexpr unsigned long long kLingerNs = 20000000ull;  // after a wait that ran out: what was under way to shared memory arrives
-
-struct ProductParams {
-    const uint8_t *a_scales, *b_scales;
-    const float *a_whole, *b_whole;
-    uint32_t m, n, k, groups;
-    Target c;
-    uint32_t *status;
-    unsigned long long wait_limit_ns;
-};
+constexpr uint32_t kTileM = 128;
 
 template <bool kMx, int kN>
 struct ProductCfg {
+    static_assert(kN <= 64, "wider ones are made by pairs");
     static constexpr uint32_t kGroupsPerStage = kMx ? 2 : 4;                   // scale groups of a stage
-    static constexpr uint32_t kBlocksB = (kN + 127) / 128;                     // 128-row blocks of B's scales
     static constexpr uint32_t kBytesA = kTileM * kStageK / 2, kBytesB = kN * kStageK / 2;
-    static constexpr uint32_t kScaleBytesA = kGroupsPerStage * 512, kScaleBytesB = kBlocksB * kScaleBytesA;
+    static constexpr uint32_t kScaleBytesA = kGroupsPerStage * 512, kScaleBytesB = kScaleBytesA;
     static constexpr uint32_t kStageBytes = kBytesA + kBytesB + kScaleBytesA + kScaleBytesB;
     static constexpr uint32_t kPerSm = kN <= 64 ? 2 : 1;                       // resident blocks
     static constexpr uint32_t kStages = (kPerSm == 2 ? 110u * 1024u : 220u * 1024u) / kStageBytes < 6 ? (kPerSm == 2 ? 110u * 1024u : 220u * 1024u) / kStageBytes : 6;
-    static constexpr uint32_t kScaleCols = kGroupsPerStage * 4 * (1 + kBlocksB);  // tensor memory columns of a stage's scales
+    static constexpr uint32_t kScaleCols = kGroupsPerStage * 8;  // tensor memory columns of a stage's scales
     static constexpr uint32_t kNeedCols = kN + kStages * kScaleCols;
     static constexpr uint32_t kTmemCols = kNeedCols <= 64 ? 64 : kNeedCols <= 128 ? 128 : kNeedCols <= 256 ? 256 : 512;
     static_assert(kNeedCols <= 512 && kTmemCols * kPerSm <= 512 && kStages >= 3, "tensor memory of an SM");
     static constexpr int kThreads = 192;  // warps 0-3: epilogue, 4: loads, 5: MMAs
-    static constexpr size_t kSmemBytes = 1024 + (size_t)kStages * kStageBytes + (2 * kStages + 1) * 8 + 16;
+    static constexpr size_t kSmemBytes = 1024 + (size_t)kStages * kStageBytes + (3 * kStages + 1) * 8 + 16;
 };
 
 template <bool kMx, int kN>
@@ -64,19 +57,21 @@ fp4_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     const uint32_t bars_addr = ptx::smem_u32(bars);
     auto full_bar = [&](uint32_t s) { return bars_addr + 8u * s; };
     auto empty_bar = [&](uint32_t s) { return bars_addr + 8u * (kStages + s); };
-    const uint32_t done_bar = bars_addr + 8u * 2u * kStages;
-    volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(bars + 2 * kStages + 1);
+    auto ready_bar = [&](uint32_t s) { return bars_addr + 8u * (2 * kStages + s); };
+    const uint32_t done_bar = bars_addr + 8u * 3u * kStages;
+    volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(bars + 3 * kStages + 1);
     uint32_t *tmem_slot = const_cast<uint32_t *>(abort_flag) + 1;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint64_t limit = p.wait_limit_ns;
-    const uint32_t n0 = blockIdx.x * kN, m0 = blockIdx.y * kTileM;
+    const uint32_t m0 = blockIdx.x * kTileM;
     const uint32_t n_stages = (p.k + kStageK - 1) / kStageK;
 
     if (tid == 0) {
         for (uint32_t s = 0; s < kStages; ++s) {
             ptx::mbar_init(full_bar(s), 1);
             ptx::mbar_init(empty_bar(s), 1);
+            ptx::mbar_init(ready_bar(s), 4);
         }
         ptx::mbar_init(done_bar, 1);
         *abort_flag = 0;
@@ -100,41 +95,28 @@ fp4_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                 const uint32_t s = it % kStages;
                 if (!ptx::mbar_wait(empty_bar(s), (it / kStages & 1u) ^ 1u, abort_flag, limit)) break;
                 const uint32_t g0 = it * Cfg::kGroupsPerStage, bytes = min(Cfg::kGroupsPerStage, p.groups - g0) * 512u;
-                uint32_t n_blocks = 0;
-#pragma unroll
-                for (uint32_t j = 0; j < Cfg::kBlocksB; ++j) n_blocks += n0 + j * 128u < p.n ? 1u : 0u;
-                ptx::mbar_arrive_expect_tx(full_bar(s), Cfg::kBytesA + Cfg::kBytesB + bytes * (1u + n_blocks));
+                ptx::mbar_arrive_expect_tx(full_bar(s), Cfg::kBytesA + Cfg::kBytesB + bytes * 2u);
                 ptx::tma_load_2d(a_addr + s * Cfg::kBytesA, &tmap_a, (int32_t)(it * (kStageK / 2)), (int32_t)m0, full_bar(s));
-                ptx::tma_load_2d(b_addr + s * Cfg::kBytesB, &tmap_b, (int32_t)(it * (kStageK / 2)), (int32_t)n0, full_bar(s));
+                ptx::tma_load_2d(b_addr + s * Cfg::kBytesB, &tmap_b, (int32_t)(it * (kStageK / 2)), 0, full_bar(s));
                 ptx::bulk_load(sa_addr + s * Cfg::kScaleBytesA, p.a_scales + ((uint64_t)(m0 / 128u) * p.groups + g0) * 512u, bytes, full_bar(s));
-                for (uint32_t j = 0; j < n_blocks; ++j)
-                    ptx::bulk_load(sb_addr + s * Cfg::kScaleBytesB + j * Cfg::kScaleBytesA, p.b_scales + ((uint64_t)(n0 / 128u + j) * p.groups + g0) * 512u, bytes, full_bar(s));
+                ptx::bulk_load(sb_addr + s * Cfg::kScaleBytesB, p.b_scales + (uint64_t)g0 * 512u, bytes, full_bar(s));
             }
         }
     } else if (warp == 5) {
         if (lane == 0) {
             const uint64_t a_desc0 = ptx::make_smem_desc(a_addr, 16, 1024, ptx::kSwizzle128B), b_desc0 = ptx::make_smem_desc(b_addr, 16, 1024, ptx::kSwizzle128B);
-            const uint64_t sa_desc0 = ptx::make_smem_desc(sa_addr, 0, 128, ptx::kSwizzleNone), sb_desc0 = ptx::make_smem_desc(sb_addr, 0, 128, ptx::kSwizzleNone);
             bool alive = true;
             for (uint32_t it = 0; it < n_stages; ++it) {
                 const uint32_t s = it % kStages;
-                alive = ptx::mbar_wait(full_bar(s), it / kStages & 1u, abort_flag, limit);
+                alive = ptx::mbar_wait(ready_bar(s), it / kStages & 1u, abort_flag, limit);
                 if (!alive) break;
                 ptx::tcgen05_fence_after_sync();
                 const uint32_t steps = min(kStageK / kMmaK, (p.k - it * kStageK + kMmaK - 1) / kMmaK);
-                const uint32_t n_groups = min(Cfg::kGroupsPerStage, p.groups - it * Cfg::kGroupsPerStage);
-                // A stage's scales have columns of their own: they are overwritten when the stage is, after its MMAs
                 const uint32_t sa = tmem_scales + s * Cfg::kScaleCols, sb = sa + Cfg::kGroupsPerStage * 4u;
-                for (uint32_t g = 0; g < n_groups; ++g) {
-                    ptx::tmem_copy_scales(sa + g * 4u, sa_desc0 + ((s * Cfg::kScaleBytesA + g * 512u) >> 4));
-#pragma unroll
-                    for (uint32_t j = 0; j < Cfg::kBlocksB; ++j)
-                        ptx::tmem_copy_scales(sb + (g * Cfg::kBlocksB + j) * 4u, sb_desc0 + ((s * Cfg::kScaleBytesB + j * Cfg::kScaleBytesA + g * 512u) >> 4));
-                }
                 for (uint32_t i = 0; i < steps; ++i) {
                     const uint32_t g = kMx ? i / 2 : i, id = kMx ? (i & 1u) * 2u : 0u;
                     ptx::umma_fp4_ss<kMx>(tmem, a_desc0 + ((s * Cfg::kBytesA + i * 32u) >> 4), b_desc0 + ((s * Cfg::kBytesB + i * 32u) >> 4),
-                                          ptx::make_fp4_instr_desc(kMx, kTileM, kN, id), sa + g * 4u, sb + g * Cfg::kBlocksB * 4u, (it | i) ? 1u : 0u);
+                                          ptx::make_fp4_instr_desc(kMx, kTileM, kN, id), sa + g * 4u, sb + g * 4u, (it | i) ? 1u : 0u);
                 }
                 ptx::umma_commit(empty_bar(s));
             }
@@ -142,6 +124,27 @@ fp4_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             if (!alive) ptx::mbar_wait_bounded(done_bar, 0, limit);
         }
     } else {
+        const uint32_t lanes = ((uint32_t)warp * 32u) << 16;
+        for (uint32_t it = 0; it < n_stages; ++it) {
+            const uint32_t s = it % kStages;
+            uint32_t ok = 1;
+            if (lane == 0) ok = ptx::mbar_wait(full_bar(s), it / kStages & 1u, abort_flag, limit) ? 1u : 0u;
+            if (!__shfl_sync(0xFFFFFFFFu, ok, 0)) break;
+            // A stage's scales have columns of their own: they are overwritten when the stage is, after its MMAs
+            uint4 a[Cfg::kGroupsPerStage], b[Cfg::kGroupsPerStage];
+#pragma unroll
+            for (uint32_t g = 0; g < Cfg::kGroupsPerStage; ++g) {
+                a[g] = ptx::ld_shared_v4(sa_addr + s * Cfg::kScaleBytesA + g * 512u + (uint32_t)lane * 16u);
+                b[g] = ptx::ld_shared_v4(sb_addr + s * Cfg::kScaleBytesB + g * 512u + (uint32_t)lane * 16u);
+            }
+            ptx::tcgen05_fence_after_sync();
+            ptx::tmem_st_v4(tmem_scales + lanes + s * Cfg::kScaleCols, a);
+            ptx::tmem_st_v4(tmem_scales + lanes + s * Cfg::kScaleCols + Cfg::kGroupsPerStage * 4u, b);
+            ptx::tmem_st_wait();
+            ptx::tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(ready_bar(s));
+        }
         const Factor f(*reinterpret_cast<const volatile float *>(p.a_whole), *reinterpret_cast<const volatile float *>(p.b_whole));
         uint32_t ok = 1;
         if (lane == 0) ok = ptx::mbar_wait(done_bar, 0, abort_flag, limit) ? 1u : 0u;
@@ -151,7 +154,7 @@ fp4_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             const uint32_t row = m0 + (uint32_t)warp * 32u + (uint32_t)lane;
             constexpr uint32_t kCols = kN < 32 ? 16 : 32;
 #pragma unroll 1
-            for (uint32_t c = 0; c < (uint32_t)kN && n0 + c < p.n; c += kCols) {
+            for (uint32_t c = 0; c < (uint32_t)kN && c < p.n; c += kCols) {
                 uint32_t r[kCols];
                 if constexpr (kCols == 16) ptx::tmem_ld_32x32b_x16(tmem + (((uint32_t)warp * 32u) << 16) + c, r);
                 else ptx::tmem_ld_32x32b_x32(tmem + (((uint32_t)warp * 32u) << 16) + c, r);
@@ -159,7 +162,7 @@ fp4_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                 float v[kCols];
 #pragma unroll
                 for (uint32_t i = 0; i < kCols; ++i) v[i] = f.apply(__uint_as_float(r[i]));
-                if (row < p.m) store_row(p.c, row, n0 + c, p.n, v);
+                if (row < p.m) store_row(p.c, row, c, p.n, v);
             }
         }
     }
@@ -199,26 +202,81 @@ int launch_width(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, const Product
         set_last_error_static("a tensor map of a 4-bit matrix could not be made");
         return B200SPMM_ERR_CUDA;
     }
-    const dim3 grid((prm.n + kN - 1) / kN, (prm.m + kTileM - 1) / kTileM);
-    if (grid.y > 65535u) return B200SPMM_ERR_UNSUPPORTED;
-    B200_CUDA_TRY(launch_after(kernel, grid, Cfg::kThreads, Cfg::kSmemBytes, 1, stream, ma, mb, prm));
+    B200_CUDA_TRY(launch_after(kernel, dim3((prm.m + kTileM - 1) / kTileM), Cfg::kThreads, Cfg::kSmemBytes, 1, stream, ma, mb, prm));
+    return B200SPMM_OK;
+}
+
+// Tiles of 128 or 256 columns, the scales' blocks being 128 rows long, with fewer columns past the end; a single tile as wide as it has to be.
+Split pair_split(uint32_t m, uint32_t n, uint32_t k, uint32_t pairs) {
+    const uint32_t cols = n <= kPairCols4 ? (n + 31u) / 32u * 32u : (n + 127u) / 128u * 128u < (n + 255u) / 256u * 256u ? 128u : 256u;
+    return make_split(m, n, cols, (k + kStageK - 1) / kStageK, 2, pairs);
+}
+
+int product_pairs(int device, uint32_t *out) {
+    static std::atomic<uint32_t> known[kMaxDevices];
+    return max_pairs(fp4_product_pair_kernel<false>, PairCfg4<false>::kThreads, PairCfg4<false>::kSmemBytes, known[device], out);
+}
+
+template <bool kMx>
+int launch_pairs(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, const ProductParams &from, float *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
+    using Cfg = PairCfg4<kMx>;
+    uint32_t pairs = 0;
+    const int st = product_pairs(a->device, &pairs);
+    if (st != B200SPMM_OK) return st;
+    auto kernel = fp4_product_pair_kernel<kMx>;
+    static thread_local int configured = -1;
+    if (configured != a->device) {
+        B200_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::kSmemBytes));
+        configured = a->device;
+    }
+    ProductParams prm = from;
+    prm.split = pair_split(prm.m, prm.n, prm.k, pairs);
+    if (prm.split.parts > 1 && (!workspace || workspace_bytes < split_workspace(prm.split))) prm.split = pair_split(prm.m, prm.n, prm.k, 1);
+    prm.partial = workspace;
+    CUtensorMap ma, mb;
+    if (!encode_values(&ma, a, layout_of(a->rows, a->cols, a->format), 128) || !encode_values(&mb, b, layout_of(b->rows, b->cols, b->format), prm.split.cols / 2u)) {
+        set_last_error_static("a tensor map of a 4-bit matrix could not be made");
+        return B200SPMM_ERR_CUDA;
+    }
+    B200_CUDA_TRY(launch_after(kernel, dim3(2 * std::min(pairs, prm.split.items)), Cfg::kThreads, Cfg::kSmemBytes, 2, stream, ma, mb, prm));
+    if (prm.split.parts > 1)
+        B200_CUDA_TRY(launch_after(fp4_join_kernel, dim3((prm.split.items - prm.split.whole) / prm.split.parts, prm.split.cols / 32u), kPairRows4, 0, 1, stream, prm.split,
+                                   (const float *)workspace, prm.m, prm.n, prm.a_whole, prm.b_whole, 1.f, prm.c));
     return B200SPMM_OK;
 }
 
 template <bool kMx>
-int launch_format(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, const ProductParams &prm, cudaStream_t stream) {
+int launch_format(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, const ProductParams &prm, float *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
     if (prm.n <= 16) return launch_width<kMx, 16>(a, b, prm, stream);
     if (prm.n <= 32) return launch_width<kMx, 32>(a, b, prm, stream);
     if (prm.n <= 64) return launch_width<kMx, 64>(a, b, prm, stream);
-    if (prm.n <= 128) return launch_width<kMx, 128>(a, b, prm, stream);
-    return launch_width<kMx, 256>(a, b, prm, stream);
+    return launch_pairs<kMx>(a, b, prm, workspace, workspace_bytes, stream);
+}
+
+// Which operand gives the rows of the MMA, true: b.  C^T = B A^T, so either may.  Up to 64 columns have to be columns.  Else the rows are those
+// that are neighbours in C: a warp's lanes hold them, and write 64 or 128 bytes in a row, where row by row every lane
+// would write to a line of its own.
+bool rows_from_b(uint64_t a_rows, uint64_t b_rows, bool c_transposed) {
+    if (std::min(a_rows, b_rows) <= 64) return a_rows < b_rows;
+    return !c_transposed;
 }
 
 }  // namespace
 
-int launch_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *c, int64_t ldc, int c_dtype, bool c_transposed, cudaStream_t stream) {
-    // C^T = B A^T: the longer side of C goes to the 128 rows of the MMA, the shorter one to its columns, which may be few
-    if (a->rows < b->rows) {
+int product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t *bytes) {
+    *bytes = 0;
+    if (std::min<uint64_t>(a->rows, (uint64_t)n) <= 64) return B200SPMM_OK;
+    uint32_t pairs = 0;
+    const int st = product_pairs(a->device, &pairs);
+    if (st != B200SPMM_OK) return st;
+    const uint32_t m = (uint32_t)a->rows, k = (uint32_t)a->cols;
+    *bytes = std::max(split_workspace(pair_split(m, (uint32_t)n, k, pairs)), split_workspace(pair_split((uint32_t)n, m, k, pairs)));
+    return B200SPMM_OK;
+}
+
+int launch_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *c, int64_t ldc, int c_dtype, bool c_transposed, float *workspace,
+                   uint64_t workspace_bytes, cudaStream_t stream) {
+    if (rows_from_b(a->rows, b->rows, c_transposed)) {
         std::swap(a, b);
         c_transposed = !c_transposed;
     }
@@ -234,7 +292,8 @@ int launch_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *c, in
     prm.c = target_of(c, ldc, c_dtype, c_transposed);
     B200_CUDA_TRY(status_word(&prm.status));
     prm.wait_limit_ns = kDeviceWaitLimitNs;
-    return a->format == B200SPMM_MXFP4 ? launch_format<true>(a, b, prm, stream) : launch_format<false>(a, b, prm, stream);
+    return a->format == B200SPMM_MXFP4 ? launch_format<true>(a, b, prm, workspace, workspace_bytes, stream)
+                                         : launch_format<false>(a, b, prm, workspace, workspace_bytes, stream);
 }
 
 }  // namespace fp4

@@ -1,7 +1,10 @@
 // How the kernels of a product are launched.
 #pragma once
 
+#include <atomic>
 #include <cuda_runtime.h>
+
+#include "common.hpp"
 
 namespace b200spmm {
 
@@ -26,6 +29,30 @@ cudaError_t launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
+// How many clusters of two CTAs of a kernel the current device runs at once; `known` keeps the answer.
+template <typename... P>
+int max_pairs(void (*kernel)(P...), unsigned threads, size_t smem, std::atomic<uint32_t> &known, uint32_t *out) {
+    *out = known.load(std::memory_order_relaxed);
+    if (*out) return B200SPMM_OK;
+    B200_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(2 * 148);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    B200_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+    if (n < 1) return B200SPMM_ERR_UNSUPPORTED;
+    *out = (uint32_t)n;
+    known.store(*out, std::memory_order_relaxed);
+    return B200SPMM_OK;
 }
 
 }  // namespace b200spmm

@@ -509,10 +509,29 @@ B200_DEVICE void umma_fp4_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, 
                      "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
                      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory");
 }
-// 32 lanes x 16 bytes from shared memory (core matrices of eight lanes) to four columns of every quarter of the lanes; runs in
-// order with the MMAs that the thread issues after it.
-B200_DEVICE void tmem_copy_scales(uint32_t taddr, uint64_t smem_desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc) : "memory");
+// The same shared by a pair: 256 rows, the scales of A each CTA's own, those of B in both.  Issued by one thread of the even CTA.
+template <bool kMx>
+B200_DEVICE void umma_pair_fp4_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales, uint32_t b_scales, uint32_t accumulate) {
+    if constexpr (kMx)
+        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+                     "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+                     ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+                     "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+                     ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory");
+}
+// 16 bytes of shared memory a lane to four columns of the warp's quarter of tensor memory, for kN addresses one after the other.
+template <int kN>
+B200_DEVICE void tmem_st_v4(uint32_t taddr, const uint4 (&v)[kN]) {
+    static_assert(kN == 2 || kN == 4, "columns of one store");
+    if constexpr (kN == 2)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                     ::"r"(taddr), "r"(v[0].x), "r"(v[0].y), "r"(v[0].z), "r"(v[0].w), "r"(v[1].x), "r"(v[1].y), "r"(v[1].z), "r"(v[1].w) : "memory");
+    else
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                     ::"r"(taddr), "r"(v[0].x), "r"(v[0].y), "r"(v[0].z), "r"(v[0].w), "r"(v[1].x), "r"(v[1].y), "r"(v[1].z), "r"(v[1].w),
+                       "r"(v[2].x), "r"(v[2].y), "r"(v[2].z), "r"(v[2].w), "r"(v[3].x), "r"(v[3].y), "r"(v[3].z), "r"(v[3].w) : "memory");
 }
 
 // Makes `bar` receive one arrival when every tcgen05.mma this thread issued so far has

@@ -271,10 +271,13 @@ PyObject *fp4_product(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     Dense c;
     if (!output_of(args[12], (int64_t)a.rows, (int64_t)b.rows, type, like, &C, &c)) return nullptr;
     void *stream = c10::cuda::getCurrentCUDAStream(like.get_device()).stream();
+    uint64_t bytes;
+    const at::Tensor workspace = product_workspace(a, (int64_t)b.rows, like, &bytes);
+    void *ws = workspace.defined() ? workspace.data_ptr() : nullptr;
     int st;
     {
         const ThreadsAllowed threads;
-        st = b200spmm_fp4_product(&a, &b, c.ptr, c.ld, (int)type, c.transposed, nullptr, 0, stream);
+        st = b200spmm_fp4_product(&a, &b, c.ptr, c.ld, (int)type, c.transposed, ws, bytes, stream);
     }
     return result_of(st, args[12], std::move(C));
     END_HANDLE_TH_ERRORS
