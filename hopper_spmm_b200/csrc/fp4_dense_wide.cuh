@@ -71,7 +71,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(bars + Cfg::kBarriers);
     uint32_t *tmem_slot = const_cast<uint32_t *>(abort_flag) + 1;
 
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31u;  // (the shuffle: a warp is known to be one)
     const uint64_t limit = p.wait_limit_ns;
     const uint32_t rank = ptx::cluster_cta_rank(), pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
     const uint32_t cols_half = p.split.cols / 2u;  // of B, this CTA's
@@ -129,33 +129,39 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         }
     } else if (warp == Cfg::kWideners) {
         // =========================================================== MMAs (even CTA)
-        if (rank == 0 && lane == 0) {
+        if (rank == 0) {
+            const uint32_t on = lane == 0 ? 1u : 0u;
             constexpr uint32_t fmt = std::is_same<T, __half>::value ? ptx::kFmtF16 : ptx::kFmtBF16;
             const uint32_t idesc = ptx::make_instr_desc(fmt, kPairRows4, p.split.cols, false, !kTokens);
             // B [n][k]: 64 values of k a row of the swizzle, eight rows 1024 bytes.  [k][n]: 64 columns a row, eight k 1024 bytes, the next 64
             // columns a box away.
-            const uint64_t b_desc0 = ptx::make_smem_desc(b_addr, kTokens ? 16u : Cfg::kBoxBytes, 1024, ptx::kSwizzle128B);
-            uint32_t it = 0, round = 0;
+            const uint64_t b_desc = ptx::make_smem_desc(b_addr, kTokens ? 16u : Cfg::kBoxBytes, 1024, ptx::kSwizzle128B);
+            const uint32_t b_lo = (uint32_t)b_desc, b_hi = (uint32_t)(b_desc >> 32);
+            uint32_t s = 0, buffer = 0, phase = 0, round = 0;
             bool alive = true;
             for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs, ++round) {
                 const Item w = split_item(p.split, item);
-                if (round) alive = ptx::mbar_wait_cluster(taken_bar, (round - 1u) & 1u, abort_flag, limit);
-                for (uint32_t step = w.first; alive && step < w.last; ++step, ++it) {
-                    const uint32_t s = it % kStages, b = it % Cfg::kBuffers;
-                    alive = ptx::mbar_wait_cluster(ready_bar(b), it / Cfg::kBuffers & 1u, abort_flag, limit);
+                if (round) alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait_cluster(taken_bar, (round - 1u) & 1u, abort_flag, limit));
+                uint32_t accumulate = 0, left = p.d.k - w.first * kWideK;  // values of k from this step on
+                for (uint32_t step = w.first; alive && step < w.last; ++step) {
+                    alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait_cluster(ready_bar(buffer), phase, abort_flag, limit));
                     if (!alive) break;
                     ptx::tcgen05_fence_after_sync();
-                    const uint32_t n_mma = min(kWideK / 16u, (p.d.k - step * kWideK + 15u) / 16u);
-                    const uint32_t a = tmem + kPairCols4 + b * Cfg::kBufferCols;
-                    for (uint32_t i = 0; i < n_mma; ++i) {
-                        const uint32_t at = s * Cfg::kBytesB + (kTokens ? i / 4u * Cfg::kBoxBytes + i % 4u * 32u : i * 2048u);
-                        ptx::umma_pair_f16_ts(tmem, a + i * 8u, b_desc0 + (at >> 4), idesc, step > w.first || i ? 1u : 0u);
-                    }
-                    ptx::umma_commit_pair(empty_bar(s));
+                    const uint32_t a = tmem + kPairCols4 + buffer * Cfg::kBufferCols, b = b_lo + s * (Cfg::kBytesB >> 4);
+#pragma unroll
+                    for (uint32_t i = 0; i < kWideK / 16u; ++i)
+                        ptx::umma_pair_f16_ts_if(on & (left > i * 16u ? 1u : 0u), tmem, a + i * 8u, b + ((kTokens ? i / 4u * Cfg::kBoxBytes + i % 4u * 32u : i * 2048u) >> 4), b_hi, idesc,
+                                                 i ? 1u : accumulate);
+                    ptx::umma_commit_pair_if(on, empty_bar(s));
+                    accumulate = 1;
+                    left -= kWideK;
+                    s = s + 1 == kStages ? 0u : s + 1;
+                    buffer = buffer + 1 == Cfg::kBuffers ? 0u : buffer + 1;
+                    phase ^= buffer == 0 ? 1u : 0u;
                 }
-                if (alive) ptx::umma_commit_pair(done_bar);
+                if (alive) ptx::umma_commit_pair_if(on, done_bar);
             }
-            if (!alive) {
+            if (!alive && on) {
                 ptx::umma_commit_pair_local(drain_bar);
                 ptx::mbar_wait_bounded(drain_bar, 0, limit);
             }

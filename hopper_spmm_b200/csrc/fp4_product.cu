@@ -62,7 +62,7 @@ fp4_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(bars + 3 * kStages + 1);
     uint32_t *tmem_slot = const_cast<uint32_t *>(abort_flag) + 1;
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;  // (the shuffle: a warp is known to be one)
     const uint64_t limit = p.wait_limit_ns;
     const uint32_t m0 = blockIdx.x * kTileM;
     const uint32_t n_stages = (p.k + kStageK - 1) / kStageK;
@@ -103,26 +103,30 @@ fp4_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             }
         }
     } else if (warp == 5) {
-        if (lane == 0) {
-            const uint64_t a_desc0 = ptx::make_smem_desc(a_addr, 16, 1024, ptx::kSwizzle128B), b_desc0 = ptx::make_smem_desc(b_addr, 16, 1024, ptx::kSwizzle128B);
-            bool alive = true;
-            for (uint32_t it = 0; it < n_stages; ++it) {
-                const uint32_t s = it % kStages;
-                alive = ptx::mbar_wait(ready_bar(s), it / kStages & 1u, abort_flag, limit);
-                if (!alive) break;
-                ptx::tcgen05_fence_after_sync();
-                const uint32_t steps = min(kStageK / kMmaK, (p.k - it * kStageK + kMmaK - 1) / kMmaK);
-                const uint32_t sa = tmem_scales + s * Cfg::kScaleCols, sb = sa + Cfg::kGroupsPerStage * 4u;
-                for (uint32_t i = 0; i < steps; ++i) {
-                    const uint32_t g = kMx ? i / 2 : i, id = kMx ? (i & 1u) * 2u : 0u;
-                    ptx::umma_fp4_ss<kMx>(tmem, a_desc0 + ((s * Cfg::kBytesA + i * 32u) >> 4), b_desc0 + ((s * Cfg::kBytesB + i * 32u) >> 4),
-                                          ptx::make_fp4_instr_desc(kMx, kTileM, kN, id), sa + g * 4u, sb + g * 4u, (it | i) ? 1u : 0u);
-                }
-                ptx::umma_commit(empty_bar(s));
+        const uint32_t on = lane == 0 ? 1u : 0u;
+        const uint64_t a_desc = ptx::make_smem_desc(a_addr, 16, 1024, ptx::kSwizzle128B), b_desc = ptx::make_smem_desc(b_addr, 16, 1024, ptx::kSwizzle128B);
+        const uint32_t a_lo = (uint32_t)a_desc, a_hi = (uint32_t)(a_desc >> 32), b_lo = (uint32_t)b_desc, b_hi = (uint32_t)(b_desc >> 32);
+        bool alive = true;
+        uint32_t s = 0, phase = 0, left = p.k;
+        for (uint32_t it = 0; it < n_stages; ++it) {
+            alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait(ready_bar(s), phase, abort_flag, limit));
+            if (!alive) break;
+            ptx::tcgen05_fence_after_sync();
+            const uint32_t sa = tmem_scales + s * Cfg::kScaleCols, sb = sa + Cfg::kGroupsPerStage * 4u;
+            const uint32_t a = a_lo + s * (Cfg::kBytesA >> 4), b = b_lo + s * (Cfg::kBytesB >> 4);
+#pragma unroll
+            for (uint32_t i = 0; i < kStageK / kMmaK; ++i) {
+                const uint32_t g = kMx ? i / 2 : i;
+                ptx::umma_fp4_ss_if<kMx, 1>(on & (left > i * kMmaK ? 1u : 0u), tmem, a + i * 2u, a_hi, b + i * 2u, b_hi,
+                                            ptx::make_fp4_instr_desc(kMx, kTileM, kN, kMx ? i % 2 * 2u : 0u), sa + g * 4u, sb + g * 4u, (it | i) ? 1u : 0u);
             }
-            ptx::umma_commit(done_bar);
-            if (!alive) ptx::mbar_wait_bounded(done_bar, 0, limit);
+            ptx::umma_commit_if(on, empty_bar(s));
+            left -= kStageK;
+            s = s + 1 == kStages ? 0u : s + 1;
+            phase ^= s == 0 ? 1u : 0u;
         }
+        ptx::umma_commit_if(on, done_bar);
+        if (!alive && on) ptx::mbar_wait_bounded(done_bar, 0, limit);
     } else {
         const uint32_t lanes = ((uint32_t)warp * 32u) << 16;
         for (uint32_t it = 0; it < n_stages; ++it) {

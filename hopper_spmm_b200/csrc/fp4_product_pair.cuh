@@ -68,7 +68,7 @@ fp4_product_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(bars + Cfg::kBarriers);
     uint32_t *tmem_slot = const_cast<uint32_t *>(abort_flag) + 1;
 
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31u;  // (the shuffle: a warp is known to be one)
     const uint64_t limit = p.wait_limit_ns;
     const uint32_t rank = ptx::cluster_cta_rank(), pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
 
@@ -123,33 +123,39 @@ fp4_product_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         }
     } else if (warp == Cfg::kMmaWarp) {
         // =========================================================== MMAs (even CTA)
-        if (rank == 0 && lane == 0) {
-            const uint64_t a_desc0 = ptx::make_smem_desc(a_addr, 16, 1024, ptx::kSwizzle128B), b_desc0 = ptx::make_smem_desc(b_addr, 16, 1024, ptx::kSwizzle128B);
-            const uint32_t idesc0 = ptx::make_fp4_instr_desc(kMx, kPairRows4, p.split.cols, 0), idesc2 = ptx::make_fp4_instr_desc(kMx, kPairRows4, p.split.cols, 2);
-            uint32_t it = 0, round = 0;
+        if (rank == 0) {
+            const uint32_t on = lane == 0 ? 1u : 0u;
+            const uint64_t a_desc = ptx::make_smem_desc(a_addr, 16, 1024, ptx::kSwizzle128B), b_desc = ptx::make_smem_desc(b_addr, 16, 1024, ptx::kSwizzle128B);
+            const uint32_t a_lo = (uint32_t)a_desc, a_hi = (uint32_t)(a_desc >> 32), b_lo = (uint32_t)b_desc, b_hi = (uint32_t)(b_desc >> 32);
+            const uint32_t idesc = ptx::make_fp4_instr_desc(kMx, kPairRows4, p.split.cols, 0);
+            constexpr uint32_t kSecond = ptx::make_fp4_instr_desc(false, 0, 0, 2) ^ ptx::make_fp4_instr_desc(false, 0, 0, 0);  // of a word's pairs of scales
+            uint32_t s = 0, phase = 0, round = 0;
             bool alive = true;
             for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs, ++round) {
                 const Item w = split_item(p.split, item);
-                if (round) alive = ptx::mbar_wait_cluster(taken_bar, (round - 1u) & 1u, abort_flag, limit);
-                for (uint32_t step = w.first; alive && step < w.last; ++step, ++it) {
-                    const uint32_t s = it % kStages;
-                    alive = ptx::mbar_wait_cluster(ready_bar(s), it / kStages & 1u, abort_flag, limit);
+                if (round) alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait_cluster(taken_bar, (round - 1u) & 1u, abort_flag, limit));
+                uint32_t accumulate = 0, left = p.k - w.first * kStageK;  // values of k from this step on
+                for (uint32_t step = w.first; alive && step < w.last; ++step) {
+                    alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait_cluster(ready_bar(s), phase, abort_flag, limit));
                     if (!alive) break;
                     ptx::tcgen05_fence_after_sync();
-                    const uint32_t n_mma = min(kStageK / kMmaK, (p.k - step * kStageK + kMmaK - 1) / kMmaK);
                     const uint32_t sa = tmem_scales + s * Cfg::kScaleCols, sb = sa + Cfg::kGroups * 4u;
+                    const uint32_t a = a_lo + s * (Cfg::kBytesA >> 4), b = b_lo + s * (Cfg::kBytesB >> 4);
 #pragma unroll
                     for (uint32_t i = 0; i < kStageK / kMmaK; ++i) {
-                        if (i >= n_mma) break;
                         const uint32_t g = kMx ? i / 2 : i;
-                        ptx::umma_pair_fp4_ss<kMx>(tmem, a_desc0 + ((s * Cfg::kBytesA + i * 32u) >> 4), b_desc0 + ((s * Cfg::kBytesB + i * 32u) >> 4),
-                                                   kMx && i % 2 ? idesc2 : idesc0, sa + g * 4u, sb + g * 8u, step > w.first || i ? 1u : 0u);
+                        ptx::umma_fp4_ss_if<kMx, 2>(on & (left > i * kMmaK ? 1u : 0u), tmem, a + i * 2u, a_hi, b + i * 2u, b_hi, kMx && i % 2 ? idesc | kSecond : idesc,
+                                                    sa + g * 4u, sb + g * 8u, i ? 1u : accumulate);
                     }
-                    ptx::umma_commit_pair(empty_bar(s));
+                    ptx::umma_commit_pair_if(on, empty_bar(s));
+                    accumulate = 1;
+                    left -= kStageK;
+                    s = s + 1 == kStages ? 0u : s + 1;
+                    phase ^= s == 0 ? 1u : 0u;
                 }
-                if (alive) ptx::umma_commit_pair(done_bar);
+                if (alive) ptx::umma_commit_pair_if(on, done_bar);
             }
-            if (!alive) {
+            if (!alive && on) {
                 ptx::umma_commit_pair_local(drain_bar);
                 ptx::mbar_wait_bounded(drain_bar, 0, limit);
             }

@@ -325,10 +325,22 @@ B200_DEVICE void umma_pair_sparse_f16_if(uint32_t on, uint32_t d_tmem, uint32_t 
 B200_DEVICE void tmem_copy_pair_128x128b(uint32_t taddr, uint64_t smem_desc) {
     asm volatile("tcgen05.cp.cta_group::2.128x128b [%0], %1;" ::"r"(taddr), "l"(smem_desc) : "memory");
 }
+// Forms for a warp that goes through its loop as one, with `on` set in a single lane: addresses and descriptors then stay in uniform
+// registers, which is where these instructions want them.  A lone lane moves each there: 90 clocks an MMA, and the tensor pipe waits.
 // A in tensor memory (row = lane, two 16-bit values of k a column) in both CTAs, each with its own 128 rows.
-B200_DEVICE void umma_pair_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-                 ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+B200_DEVICE void umma_pair_f16_ts_if(uint32_t on, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p, q;\n.reg .b64 db;\nmov.b64 db, {%2, %3};\nsetp.ne.b32 p, %5, 0;\nsetp.ne.b32 q, %6, 0;\n"
+                 "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], db, %4, p;\n}\n"
+                 ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
+}
+B200_DEVICE void umma_commit_pair_if(uint32_t on, uint32_t bar) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %2, 0;\n"
+                 "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n"
+                 ::"r"(bar), "h"((uint16_t)3), "r"(on) : "memory");
+}
+B200_DEVICE void umma_commit_if(uint32_t on, uint32_t bar) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %1, 0;\n"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar), "r"(on) : "memory");
 }
 // One arrival on the barrier at offset `bar` in BOTH CTAs of the pair (mask 0b11) when every MMA this
 // thread issued so far has finished.
@@ -494,32 +506,24 @@ B200_DEVICE void umma_tf32_ss_lohi_if(uint32_t on, uint32_t d_tmem, uint32_t a_l
 // in lane r % 32 (the same in each quarter of the lanes), column r / 32, four scales to a 32-bit word.  Instruction descriptor:
 //   [4,6) which scale of B's words   [7,10) A format, [10,12) B format (1 = e2m1)   [17,23) N >> 3
 //   [23] scales are e8m0 (0: e4m3)   [27,29) M >> 7   [29,31) which scale of A's words
+// kCtas 2: shared by a pair, 256 rows, the scales of A each CTA's own, those of B in both.  `on` set in a single lane, see above.
 // nvfp4 takes all four scales of a word (16 values each), mxfp4 two of them (32 values each): 0 or 2 in the descriptor.
 __host__ __device__ constexpr uint32_t make_fp4_instr_desc(bool e8m0, uint32_t m, uint32_t n, uint32_t scale_id) {
     return (scale_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((e8m0 ? 1u : 0u) << 23) | ((m >> 7) << 27) | (scale_id << 29);
 }
-template <bool kMx>
-B200_DEVICE void umma_fp4_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales, uint32_t b_scales, uint32_t accumulate) {
-    if constexpr (kMx)
-        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
-                     "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
-                     ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory");
-    else
-        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
-                     "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
-                     ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory");
-}
-// The same shared by a pair: 256 rows, the scales of A each CTA's own, those of B in both.  Issued by one thread of the even CTA.
-template <bool kMx>
-B200_DEVICE void umma_pair_fp4_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales, uint32_t b_scales, uint32_t accumulate) {
-    if constexpr (kMx)
-        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
-                     "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
-                     ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory");
-    else
-        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
-                     "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
-                     ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory");
+template <bool kMx, int kCtas>
+B200_DEVICE void umma_fp4_ss_if(uint32_t on, uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t a_scales,
+                                uint32_t b_scales, uint32_t accumulate) {
+#define B200_FP4_MMA(ctas, kind)                                                                                              \
+    asm volatile("{\n.reg .pred p, q;\n.reg .b64 da, db;\nmov.b64 da, {%1, %2};\nmov.b64 db, {%3, %4};\n"                     \
+                 "setp.ne.b32 p, %8, 0;\nsetp.ne.b32 q, %9, 0;\n"                                                              \
+                 "@q tcgen05.mma.cta_group::" ctas ".kind::" kind " [%0], da, db, %5, [%6], [%7], p;\n}\n"                       \
+                 ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate), "r"(on) : "memory")
+    if constexpr (kMx && kCtas == 1) B200_FP4_MMA("1", "mxf4.block_scale.scale_vec::2X");
+    else if constexpr (kMx) B200_FP4_MMA("2", "mxf4.block_scale.scale_vec::2X");
+    else if constexpr (kCtas == 1) B200_FP4_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
+    else B200_FP4_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
+#undef B200_FP4_MMA
 }
 // 16 bytes of shared memory a lane to four columns of the warp's quarter of tensor memory, for kN addresses one after the other.
 template <int kN>
