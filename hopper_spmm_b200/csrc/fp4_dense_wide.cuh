@@ -10,7 +10,7 @@
 //
 // A step is 128 values of k.  Warps 0-15 of a CTA widen: lane = row of the warp's quarter of tensor memory, warps 4 g .. 4 g + 3
 // every fourth step, so that what a step has to wait for (its stage, its way to tensor memory) overlaps with three others;
-// after an item's last step they take the accumulator to C.  Warp 16 of the even CTA issues the MMAs, warp 17 loads.
+// after an item's last step they take the accumulator to C.  Warp 16 of the even CTA issues the MMAs, warps 17 and 18 load.
 //
 //   full[s]   stage s has landed (TMA bytes, each CTA its own): the widening warps wait for it, with B's part of it
 //   ready[b]  buffer b of widened A is written in both CTAs (eight warps arrive at the even CTA)
@@ -34,7 +34,7 @@ struct WideCfg {
     static constexpr uint32_t kBuffers = 4, kBufferCols = kWideK / 2;  // of widened A, in tensor memory behind the accumulator
     static constexpr uint32_t kWideners = 16;
     static_assert(kBuffers == kWideners / 4, "a group of four warps has a buffer of its own");
-    static constexpr int kWarps = kWideners + 2, kThreads = 32 * kWarps;
+    static constexpr int kWarps = kWideners + 3, kThreads = 32 * kWarps;
     static constexpr uint32_t kTmemCols = 512;
     static constexpr uint32_t kBarriers = 2 * kStages + kBuffers + 3;
     static constexpr size_t kSmemBytes = 1024 + (size_t)kStages * kStageBytes + kBarriers * 8 + 16;
@@ -78,7 +78,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 
     if (tid == 0) {
         for (uint32_t s = 0; s < kStages; ++s) {
-            ptx::mbar_init(full_bar(s), 1);
+            ptx::mbar_init(full_bar(s), 2);
             ptx::mbar_init(empty_bar(s), 1);
         }
         for (uint32_t b = 0; b < Cfg::kBuffers; ++b) ptx::mbar_init(ready_bar(b), 8);
@@ -102,29 +102,40 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     ptx::tcgen05_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == Cfg::kWideners + 1) {
+    if (warp > Cfg::kWideners) {
         // =========================================================== loads
-        uint32_t it = 0;
-        bool alive = lane == 0;
+        // One warp A and its scales, one B: an instruction holds its warp for some 130 clocks.
+        const uint32_t on = lane == 0 ? 1u : 0u;
+        const bool is_a = warp == Cfg::kWideners + 1;
+        constexpr uint32_t kGroups = kMx ? 1 : 2;
+        const uint32_t boxes = kTokens ? 2u : (cols_half + 63u) / 64u, box_bytes = kTokens ? cols_half * 128u : Cfg::kBoxBytes;
+        uint32_t s = 0, phase = 1;
+        bool alive = true;
         for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs) {
             const Item w = split_item(p.split, item);
             const uint32_t row_block = w.m0 / 128u + rank;
             const uint32_t n0 = w.n0 + rank * cols_half;
-            const uint32_t boxes = kTokens ? 2u : (cols_half + 63u) / 64u;
-            const uint32_t box_bytes = kTokens ? cols_half * 128u : Cfg::kBoxBytes;
-            for (uint32_t step = w.first; step < w.last; ++step, ++it) {
-                const uint32_t s = it % kStages;
-                alive = ptx::mbar_wait(empty_bar(s), (it / kStages & 1u) ^ 1u, abort_flag, limit);
+            const bool has_scales = row_block < p.row_blocks;
+            const uint8_t *scales = p.d.scales + (uint64_t)row_block * p.d.groups * 512u;
+            for (uint32_t step = w.first; step < w.last; ++step) {
+                alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait(empty_bar(s), phase, abort_flag, limit));
                 if (!alive) break;
-                constexpr uint32_t kGroups = kMx ? 1 : 2;
-                const uint32_t g0 = step * kGroups, scale_bytes = row_block < p.row_blocks ? min(kGroups, p.d.groups - g0) * 512u : 0u;
-                ptx::mbar_arrive_expect_tx(full_bar(s), Cfg::kBytesA + scale_bytes + boxes * box_bytes);
-                ptx::tma_load_2d(a_addr + s * Cfg::kBytesA, &tmap_a, (int32_t)(step * (kWideK / 2)), (int32_t)(w.m0 + rank * 128u), full_bar(s));
-                if (scale_bytes) ptx::bulk_load(s_addr + s * Cfg::kBytesScales, p.d.scales + ((uint64_t)row_block * p.d.groups + g0) * 512u, scale_bytes, full_bar(s));
-                for (uint32_t i = 0; i < boxes; ++i) {
-                    if constexpr (kTokens) ptx::tma_load_2d(b_addr + s * Cfg::kBytesB + i * Cfg::kBoxBytes, &tmap_b, (int32_t)(step * kWideK + i * 64u), (int32_t)n0, full_bar(s));
-                    else ptx::tma_load_2d(b_addr + s * Cfg::kBytesB + i * Cfg::kBoxBytes, &tmap_b, (int32_t)(n0 + i * 64u), (int32_t)(step * kWideK), full_bar(s));
+                if (is_a) {
+                    const uint32_t g0 = step * kGroups, scale_bytes = has_scales ? min(kGroups, p.d.groups - g0) * 512u : 0u;
+                    ptx::mbar_arrive_expect_tx_if(on, full_bar(s), Cfg::kBytesA + scale_bytes);
+                    ptx::tma_load_2d_if(on, a_addr + s * Cfg::kBytesA, &tmap_a, (int32_t)(step * (kWideK / 2)), (int32_t)(w.m0 + rank * 128u), full_bar(s));
+                    ptx::bulk_load_if(on & (has_scales ? 1u : 0u), s_addr + s * Cfg::kBytesScales, scales + (uint64_t)g0 * 512u, scale_bytes, full_bar(s));
+                } else {
+                    ptx::mbar_arrive_expect_tx_if(on, full_bar(s), boxes * box_bytes);
+#pragma unroll
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        const uint32_t there = on & (i < boxes ? 1u : 0u);
+                        if constexpr (kTokens) ptx::tma_load_2d_if(there, b_addr + s * Cfg::kBytesB + i * Cfg::kBoxBytes, &tmap_b, (int32_t)(step * kWideK + i * 64u), (int32_t)n0, full_bar(s));
+                        else ptx::tma_load_2d_if(there, b_addr + s * Cfg::kBytesB + i * Cfg::kBoxBytes, &tmap_b, (int32_t)(n0 + i * 64u), (int32_t)(step * kWideK), full_bar(s));
+                    }
                 }
+                s = s + 1 == kStages ? 0u : s + 1;
+                phase ^= s == 0 ? 1u : 0u;
             }
         }
     } else if (warp == Cfg::kWideners) {

@@ -90,17 +90,19 @@ fp4_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     const uint32_t tmem = *tmem_slot, tmem_scales = tmem + kN;
 
     if (warp == 4) {
-        if (lane == 0) {
-            for (uint32_t it = 0; it < n_stages; ++it) {
-                const uint32_t s = it % kStages;
-                if (!ptx::mbar_wait(empty_bar(s), (it / kStages & 1u) ^ 1u, abort_flag, limit)) break;
-                const uint32_t g0 = it * Cfg::kGroupsPerStage, bytes = min(Cfg::kGroupsPerStage, p.groups - g0) * 512u;
-                ptx::mbar_arrive_expect_tx(full_bar(s), Cfg::kBytesA + Cfg::kBytesB + bytes * 2u);
-                ptx::tma_load_2d(a_addr + s * Cfg::kBytesA, &tmap_a, (int32_t)(it * (kStageK / 2)), (int32_t)m0, full_bar(s));
-                ptx::tma_load_2d(b_addr + s * Cfg::kBytesB, &tmap_b, (int32_t)(it * (kStageK / 2)), 0, full_bar(s));
-                ptx::bulk_load(sa_addr + s * Cfg::kScaleBytesA, p.a_scales + ((uint64_t)(m0 / 128u) * p.groups + g0) * 512u, bytes, full_bar(s));
-                ptx::bulk_load(sb_addr + s * Cfg::kScaleBytesB, p.b_scales + (uint64_t)g0 * 512u, bytes, full_bar(s));
-            }
+        const uint32_t on = lane == 0 ? 1u : 0u;
+        const uint8_t *scales = p.a_scales + (uint64_t)(m0 / 128u) * p.groups * 512u;
+        uint32_t s = 0, phase = 1;
+        for (uint32_t it = 0; it < n_stages; ++it) {
+            if (!__all_sync(0xFFFFFFFFu, ptx::mbar_wait(empty_bar(s), phase, abort_flag, limit))) break;
+            const uint32_t g0 = it * Cfg::kGroupsPerStage, bytes = min(Cfg::kGroupsPerStage, p.groups - g0) * 512u;
+            ptx::mbar_arrive_expect_tx_if(on, full_bar(s), Cfg::kBytesA + Cfg::kBytesB + bytes * 2u);
+            ptx::tma_load_2d_if(on, a_addr + s * Cfg::kBytesA, &tmap_a, (int32_t)(it * (kStageK / 2)), (int32_t)m0, full_bar(s));
+            ptx::bulk_load_if(on, sa_addr + s * Cfg::kScaleBytesA, scales + (uint64_t)g0 * 512u, bytes, full_bar(s));
+            ptx::tma_load_2d_if(on, b_addr + s * Cfg::kBytesB, &tmap_b, (int32_t)(it * (kStageK / 2)), 0, full_bar(s));
+            ptx::bulk_load_if(on, sb_addr + s * Cfg::kScaleBytesB, p.b_scales + (uint64_t)g0 * 512u, bytes, full_bar(s));
+            s = s + 1 == kStages ? 0u : s + 1;
+            phase ^= s == 0 ? 1u : 0u;
         }
     } else if (warp == 5) {
         const uint32_t on = lane == 0 ? 1u : 0u;

@@ -5,7 +5,7 @@
 // either.
 // Warps 0-7 take accumulators to C, warps 8-15 bring scales to tensor memory (four of them a stage, each its quarter of the lanes;
 // tcgen05.cp does the same, but in line with the MMAs: 110 clocks a copy of 512 bytes, twelve a stage, doubled the time),
-// warp 16 of the even CTA issues the MMAs, warp 17 loads.
+// warp 16 of the even CTA issues the MMAs, warps 17 and 18 load.
 //
 //   full[s]   stage s has landed (TMA bytes, each CTA its own): the scales' warps wait for it
 //   ready[s]  ... and its scales are in tensor memory, in both CTAs (eight warps arrive at the even CTA)
@@ -41,7 +41,7 @@ struct PairCfg4 {
     static constexpr uint32_t kStages = 5;
     static constexpr uint32_t kScaleCols = kGroups * 12;  // of tensor memory: four for A, eight for B's 256 rows, a group
     static constexpr uint32_t kTmemCols = 512;
-    static constexpr int kEpilogueWarps = 8, kScaleWarps = 8, kMmaWarp = kEpilogueWarps + kScaleWarps, kThreads = 32 * (kMmaWarp + 2);
+    static constexpr int kEpilogueWarps = 8, kScaleWarps = 8, kMmaWarp = kEpilogueWarps + kScaleWarps, kThreads = 32 * (kMmaWarp + 3);
     static constexpr uint32_t kBarriers = 3 * kStages + 3;
     static constexpr size_t kSmemBytes = 1024 + (size_t)kStages * kStageBytes + kBarriers * 8 + 16;
     static_assert(kPairCols4 + kStages * kScaleCols <= kTmemCols && kSmemBytes <= 227 * 1024, "memory of an SM");
@@ -74,7 +74,7 @@ fp4_product_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
 
     if (tid == 0) {
         for (uint32_t s = 0; s < kStages; ++s) {
-            ptx::mbar_init(full_bar(s), 1);
+            ptx::mbar_init(full_bar(s), 2);
             ptx::mbar_init(ready_bar(s), 8);
             ptx::mbar_init(empty_bar(s), 1);
         }
@@ -98,27 +98,36 @@ fp4_product_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     ptx::tcgen05_fence_after_sync();
     const uint32_t tmem = *tmem_slot, tmem_scales = tmem + kPairCols4;
 
-    if (warp == Cfg::kMmaWarp + 1) {
+    if (warp > Cfg::kMmaWarp) {
         // =========================================================== loads
-        uint32_t it = 0;
-        bool alive = lane == 0;
+        // One warp A and its scales, one B: an instruction holds its warp for some 130 clocks, and a stage has five.
+        const uint32_t on = lane == 0 ? 1u : 0u;
+        const bool is_a = warp == Cfg::kMmaWarp + 1;
+        uint32_t s = 0, phase = 1;
+        bool alive = true;
         for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs) {
             const Item w = split_item(p.split, item);
-            const uint32_t row_block = w.m0 / 128u + rank;
-            const bool has_a = row_block * 128u < p.m;
-            uint32_t blocks_b = 0;
-            for (uint32_t j = 0; j < (p.split.cols + 127u) / 128u; ++j) blocks_b += w.n0 + j * 128u < p.n ? 1u : 0u;
-            for (uint32_t step = w.first; step < w.last; ++step, ++it) {
-                const uint32_t s = it % kStages;
-                alive = ptx::mbar_wait(empty_bar(s), (it / kStages & 1u) ^ 1u, abort_flag, limit);
+            const uint32_t row_block = is_a ? w.m0 / 128u + rank : w.n0 / 128u;
+            const uint32_t rows = is_a ? p.m : p.n;
+            const uint32_t half = p.split.cols / 2u;
+            // blocks of scales: one of A, B's all, in as far as they exist
+            const uint32_t blocks = (row_block * 128u < rows ? 1u : 0u) + (!is_a && p.split.cols > 128u && (row_block + 1u) * 128u < rows ? 1u : 0u);
+            const int32_t y = (int32_t)(is_a ? w.m0 + rank * 128u : w.n0 + rank * half);
+            const uint32_t tile_bytes = is_a ? Cfg::kBytesA : half * 128u;
+            const uint32_t dst = is_a ? a_addr : b_addr, dst_scales = is_a ? sa_addr : sb_addr;
+            const uint32_t stage = is_a ? Cfg::kBytesA : Cfg::kBytesB, stage_scales = is_a ? Cfg::kScaleBytesA : Cfg::kScaleBytesB;
+            const void *map = is_a ? &tmap_a : &tmap_b;
+            const uint8_t *scales = (is_a ? p.a_scales : p.b_scales) + (uint64_t)row_block * p.groups * 512u;
+            for (uint32_t step = w.first; step < w.last; ++step) {
+                alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait(empty_bar(s), phase, abort_flag, limit));
                 if (!alive) break;
                 const uint32_t g0 = step * Cfg::kGroups, bytes = min(Cfg::kGroups, p.groups - g0) * 512u;
-                ptx::mbar_arrive_expect_tx(full_bar(s), Cfg::kBytesA + p.split.cols / 2u * 128u + bytes * ((has_a ? 1u : 0u) + blocks_b));
-                ptx::tma_load_2d(a_addr + s * Cfg::kBytesA, &tmap_a, (int32_t)(step * (kStageK / 2)), (int32_t)(w.m0 + rank * 128u), full_bar(s));
-                ptx::tma_load_2d(b_addr + s * Cfg::kBytesB, &tmap_b, (int32_t)(step * (kStageK / 2)), (int32_t)(w.n0 + rank * (p.split.cols / 2u)), full_bar(s));
-                if (has_a) ptx::bulk_load(sa_addr + s * Cfg::kScaleBytesA, p.a_scales + ((uint64_t)row_block * p.groups + g0) * 512u, bytes, full_bar(s));
-                for (uint32_t j = 0; j < blocks_b; ++j)
-                    ptx::bulk_load(sb_addr + s * Cfg::kScaleBytesB + j * Cfg::kScaleBytesA, p.b_scales + ((uint64_t)(w.n0 / 128u + j) * p.groups + g0) * 512u, bytes, full_bar(s));
+                ptx::mbar_arrive_expect_tx_if(on, full_bar(s), tile_bytes + bytes * blocks);
+                ptx::tma_load_2d_if(on, dst + s * stage, map, (int32_t)(step * (kStageK / 2)), y, full_bar(s));
+                ptx::bulk_load_if(on & (blocks > 0 ? 1u : 0u), dst_scales + s * stage_scales, scales + (uint64_t)g0 * 512u, bytes, full_bar(s));
+                if (!is_a) ptx::bulk_load_if(on & (blocks > 1 ? 1u : 0u), dst_scales + s * stage_scales + Cfg::kScaleBytesA, scales + (uint64_t)(p.groups + g0) * 512u, bytes, full_bar(s));
+                s = s + 1 == kStages ? 0u : s + 1;
+                phase ^= s == 0 ? 1u : 0u;
             }
         }
     } else if (warp == Cfg::kMmaWarp) {

@@ -163,6 +163,21 @@ B200_DEVICE void tma_gather4_2d(uint32_t dst, const void *tmap, int32_t x, int32
         : "memory");
 }
 
+// The same for a warp that goes through its loop as one, with `on` set in a single lane (see umma_pair_f16_ts_if).
+B200_DEVICE void mbar_arrive_expect_tx_if(uint32_t on, uint32_t bar, uint32_t bytes) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %2, 0;\n@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}\n" ::"r"(bar), "r"(bytes), "r"(on) : "memory");
+}
+B200_DEVICE void tma_load_2d_if(uint32_t on, uint32_t dst, const void *tmap, int32_t x, int32_t y, uint32_t bar) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %5, 0;\n"
+                 "@q cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n}\n"
+                 ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(bar), "r"(on) : "memory");
+}
+B200_DEVICE void bulk_load_if(uint32_t on, uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %4, 0;\n"
+                 "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n}\n"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "r"(on) : "memory");
+}
+
 B200_DEVICE uint4 ld_shared_v4(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
