@@ -9,9 +9,8 @@
 //
 // A warp takes steps of 32 rows x 128 values of k.  The rows are i, i + 32, i + 64, i + 96 of a block of 128 for eight neighbouring i:
 // their scales are whole 16-byte pieces.  Lane 4 g + t reads 16 bytes of values, 32 codes, of each of its four rows i0 + g + 32 q from k = 32 t on, and
-// one piece with the scales.  Which k an operand position of the MMA stands for is free as long as both operands agree; lane t's
-// positions of MMA j are codes 8 (j / 2) + 2 (j % 2) + {0, 4, 1, 5} of its 32: those that lie so in a word that two of them are widened by
-// one shift and two masks.
+// one piece with the scales.  Which k an operand position of the MMA stands for is free as long as both operands agree: lane t's
+// positions of MMA j are pairs 2 (j % 2) and 2 (j % 2) + 1 of word j / 2 of its four, as Widen makes them.
 // The eight warps of a block share out k, 128 values at a time, and their sums meet in shared memory in a fixed order.
 #pragma once
 
@@ -114,7 +113,8 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, 2) fp4_narrow_kernel(const 
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
                 const uint32_t kk = j * 32u + lane, k = k0 + kk;
-                const uint32_t in_lane = kk & 31u, slot = (((in_lane & ~7u) | (in_lane & 3u) << 1 | (in_lane >> 2 & 1u)) << 2) + (kk >> 5);
+                const uint32_t in_lane = kk & 31u, 
+                               order = W::kNeighbours ? in_lane : (in_lane & ~7u) | (in_lane & 3u) << 1 | (in_lane >> 2 & 1u), slot = (order << 2) + (kk >> 5);
 #pragma unroll
                 for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
                     const uint32_t col = n0 + nb * 8u, at = buf * Cfg::kBBytes + nb * (kNarrowK * 16u) + slot * 16u;
@@ -159,12 +159,12 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, 2) fp4_narrow_kernel(const 
                     for (uint32_t w = 0; w < 4; ++w) {
                         if constexpr (kTokens) {
                             const uint4 v = ptx::ld_shared_v4(buf + (nb * 4u + w) * 512u + lane * 16u);
-                            bf[nb][w][0] = __byte_perm(v.x, v.z, 0x5410);  // k 0, 4
-                            bf[nb][w][1] = __byte_perm(v.x, v.z, 0x7632);  // 1, 5
-                            bf[nb][w][2] = __byte_perm(v.y, v.w, 0x5410);  // 2, 6
-                            bf[nb][w][3] = __byte_perm(v.y, v.w, 0x7632);  // 3, 7
+                            bf[nb][w][0] = W::kNeighbours ? v.x : __byte_perm(v.x, v.z, 0x5410);  // k 0, 1 or 0, 4
+                            bf[nb][w][1] = W::kNeighbours ? v.y : __byte_perm(v.x, v.z, 0x7632);  // 2, 3 or 1, 5
+                            bf[nb][w][2] = W::kNeighbours ? v.z : __byte_perm(v.y, v.w, 0x5410);  // 4, 5 or 2, 6
+                            bf[nb][w][3] = W::kNeighbours ? v.w : __byte_perm(v.y, v.w, 0x7632);  // 6, 7 or 3, 7
                         } else {
-                            // matrix i holds k 8 w + i and 8 w + i + 4 of the four lanes' ranges, lane's row at slot 4 (8 w + 2 i + lane % 2) + lane / 2
+                            // matrix i holds the values of k of pair i of word w of the four lanes' ranges, its row r at slot 4 (8 w + 2 i + r % 2) + r / 2
                             const uint32_t mat = lane >> 3, r = lane & 7u;
                             ldmatrix_x4_trans(buf + nb * (kNarrowK * 16u) + (((w * 8u + mat * 2u + (r & 1u)) << 2) + (r >> 1)) * 16u, bf[nb][w]);
                         }
@@ -196,14 +196,14 @@ __global__ void __launch_bounds__(32 * kNarrowWarps, 2) fp4_narrow_kernel(const 
                 const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                 for (uint32_t w = 0; w < 4; ++w) {
-                    const uint32_t a0 = W::template pair<kTwice, 0>(wl[w], sl[w >> 1]), a1 = W::template pair<kTwice, 0>(wh[w], sh[w >> 1]);
-                    const uint32_t a2 = W::template pair<kTwice, 1>(wl[w], sl[w >> 1]), a3 = W::template pair<kTwice, 1>(wh[w], sh[w >> 1]);
+                    uint32_t pl[4], ph[4];
+                    W::template pairs<kTwice>(wl[w], sl[w >> 1], pl);
+                    W::template pairs<kTwice>(wh[w], sh[w >> 1], ph);
 #pragma unroll
-                    for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) mma_16x8x16<T>(acc[u][tile][nb], a0, a1, a2, a3, bf[nb][w][0], bf[nb][w][1]);
-                    const uint32_t c0 = W::template pair<kTwice, 2>(wl[w], sl[w >> 1]), c1 = W::template pair<kTwice, 2>(wh[w], sh[w >> 1]);
-                    const uint32_t c2 = W::template pair<kTwice, 3>(wl[w], sl[w >> 1]), c3 = W::template pair<kTwice, 3>(wh[w], sh[w >> 1]);
+                    for (uint32_t j = 0; j < 2; ++j)
 #pragma unroll
-                    for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) mma_16x8x16<T>(acc[u][tile][nb], c0, c1, c2, c3, bf[nb][w][2], bf[nb][w][3]);
+                        for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
+                            mma_16x8x16<T>(acc[u][tile][nb], pl[2 * j], ph[2 * j], pl[2 * j + 1], ph[2 * j + 1], bf[nb][w][2 * j], bf[nb][w][2 * j + 1]);
                 }
             };
             if (kMx && __any_sync(0xFFFFFFFFu, W::needs_two(sc.x) || W::needs_two(sc.y) || W::needs_two(sc.z) || W::needs_two(sc.w))) {
