@@ -13,33 +13,43 @@ namespace b200spmm {
 namespace fp4 {
 namespace {
 
-template <typename T, bool kMx, int kNB, int kU, bool kTokens>
-int launch_narrow(const DenseParams &prm, int device, cudaStream_t stream) {
-    using Cfg = NarrowCfg<kNB, kU>;
-    auto kernel = fp4_narrow_kernel<T, kMx, kNB, kU, kTokens>;
+template <typename T, bool kMx, int kNB, bool kTokens>
+int launch_narrow(const b200spmm_fp4_t *a, const DenseParams &d, cudaStream_t stream) {
+    constexpr uint32_t kMostBytes = 226u * 1024u;
+    auto kernel = fp4_narrow_kernel<T, kMx, kNB, kTokens>;
     static thread_local int configured = -1;
-    if (configured != device) {
-        B200_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::kSmemBytes));
-        B200_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-        configured = device;
+    if (configured != a->device) {
+        B200_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostBytes));
+        configured = a->device;
     }
-    const dim3 grid((prm.m + 127u) / 128u * (4 / kU), (prm.n + 8 * kNB - 1) / (8 * kNB));
-    if (grid.y > 65535u) return B200SPMM_ERR_UNSUPPORTED;
-    B200_CUDA_TRY(launch_after(kernel, grid, 32 * kNarrowWarps, Cfg::kSmemBytes, 1, stream, prm));
+    const uint32_t passes = (d.n + 8 * kNB - 1) / (8 * kNB);
+    if (passes > 65535u) return B200SPMM_ERR_UNSUPPORTED;
+    NarrowParams prm{};
+    prm.d = d;
+    prm.tiles = (d.m + 15u) / 16u;
+    // a block's tiles, each sliced as far as there are warps and steps
+    const uint32_t blocks = std::min(prm.tiles, (uint32_t)sm_count()), of_block = (prm.tiles + blocks - 1) / blocks;
+    prm.at_once = std::min(of_block, kNarrowTiles);
+    prm.slices = std::max<uint32_t>(1, std::min(kNarrowWarps / prm.at_once, (d.k + kNarrowStep - 1) / kNarrowStep));
+    prm.row_blocks = (prm.at_once * 16u + 126u) / 128u + 1u;
+    const uint32_t stage = narrow_stage(kMx, prm.at_once, prm.row_blocks, kNB).bytes(), warps = prm.at_once * prm.slices;
+    const uint32_t sums = prm.slices > 1 ? warps * 16u * 8u * kNB * (uint32_t)sizeof(float) : 0u;
+    prm.stages = std::min({kNarrowMaxStages, (kMostBytes - 384u - sums) / stage, std::max<uint32_t>(2, (d.k + kNarrowStage - 1) / kNarrowStage)});
+    B200_CUDA_TRY(status_word(&prm.status));
+    prm.wait_limit_ns = kDeviceWaitLimitNs;
+    CUtensorMap ma;
+    if (!encode_2d(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, d.pitch, d.m, d.pitch, kNarrowStep / 2, prm.at_once * 16u, CU_TENSOR_MAP_SWIZZLE_NONE,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) {
+        set_last_error_static("a tensor map of a 4-bit matrix could not be made");
+        return B200SPMM_ERR_CUDA;
+    }
+    B200_CUDA_TRY(launch_after(kernel, dim3(blocks, passes), 32 * (warps + 2), 384u + prm.stages * stage + sums, 1, stream, ma, prm));
     return B200SPMM_OK;
 }
 
 template <typename T, bool kMx, bool kTokens>
-int launch_narrow_rows(const DenseParams &prm, int device, cudaStream_t stream) {
-    // A block of threads reads all of B: as many rows a block as leave a block for every SM
-    const uint32_t blocks = (prm.m + 127u) / 128u, sms = (uint32_t)sm_count();
-    if (prm.n <= 8) {
-        if (blocks >= sms) return launch_narrow<T, kMx, 1, 4, kTokens>(prm, device, stream);
-        if (blocks * 2 >= sms) return launch_narrow<T, kMx, 1, 2, kTokens>(prm, device, stream);
-        return launch_narrow<T, kMx, 1, 1, kTokens>(prm, device, stream);
-    }
-    if (blocks * 2 >= sms) return launch_narrow<T, kMx, 2, 2, kTokens>(prm, device, stream);
-    return launch_narrow<T, kMx, 2, 1, kTokens>(prm, device, stream);
+int launch_narrow_columns(const b200spmm_fp4_t *a, const DenseParams &d, cudaStream_t stream) {
+    return d.n <= 8 ? launch_narrow<T, kMx, 1, kTokens>(a, d, stream) : launch_narrow<T, kMx, 2, kTokens>(a, d, stream);
 }
 
 // Columns shared out evenly over as few tiles as there can be; a part has at least four steps: shorter ones are not worth their
@@ -95,7 +105,7 @@ bool is_narrow(const DenseParams &d) { return d.n <= 16 || !d.b_wide; }
 
 template <typename T, bool kMx, bool kTokens>
 int launch_dense(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
-    return is_narrow(d) ? launch_narrow_rows<T, kMx, kTokens>(d, a->device, stream) : launch_wide<T, kMx, kTokens>(a, d, workspace, workspace_bytes, stream);
+    return is_narrow(d) ? launch_narrow_columns<T, kMx, kTokens>(a, d, stream) : launch_wide<T, kMx, kTokens>(a, d, workspace, workspace_bytes, stream);
 }
 
 }  // namespace
@@ -126,6 +136,11 @@ int launch_dense_product(const b200spmm_fp4_t *a, const void *b, int64_t ldb, in
     prm.n = (uint32_t)n;
     prm.b_wide = reinterpret_cast<uintptr_t>(b) % 16u == 0 && ldb % 8 == 0;
     prm.c = target_of(c, ldc, c_dtype, c_transposed);
+    if (n == 1 && !b_transposed && ldb == 1) {  // one column, contiguous
+        b_transposed = true;
+        prm.ldb = prm.k;
+    }
+    if (n == 1 && b_transposed) prm.b_wide = reinterpret_cast<uintptr_t>(b) % 16u == 0;
     auto run = [&](auto type, auto mx) {
         using T = decltype(type);
         constexpr bool kMx = decltype(mx)::value;

@@ -208,7 +208,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 #pragma unroll
                 for (uint32_t g = 0; g < (kMx ? 1u : 2u); ++g)
                     if (step * kWideK + g * 64u < p.d.k)
-                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(four[g]) : "r"(s_addr + s * Cfg::kBytesScales + g * 512u + lane * 16u + q * 4u) : "memory");
+                        four[g] = ptx::ld_shared_u32(s_addr + s * Cfg::kBytesScales + g * 512u + lane * 16u + q * 4u);
                 const bool two = W::needs_two(four[0]) || W::needs_two(four[1]);
                 const bool any_two = kMx && __any_sync(0xFFFFFFFFu, two);
                 if (now >= Cfg::kBuffers) {

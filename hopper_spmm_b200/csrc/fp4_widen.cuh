@@ -59,6 +59,18 @@ template <typename T, bool kMx> struct Widen {
             return (__float_as_uint(from_e4m3(byte) * 0x1p118f) >> 16) * 0x10001u;  // (exact: four bits, or NaN)
         }
     }
+    // The scales in the two low bytes of `word`.
+    B200_DEVICE static void two_scales(uint32_t word, uint32_t (&out)[2]) {
+        if constexpr (kHalf) {
+            uint32_t r;
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)word));
+            out[0] = __byte_perm(r, r, 0x1010);
+            out[1] = __byte_perm(r, r, 0x3232);
+        } else {
+            out[0] = scale<false>(word & 0xFFu);
+            out[1] = scale<false>(word >> 8 & 0xFFu);
+        }
+    }
     // The four pairs of a word.
     template <bool kTwice> B200_DEVICE static void pairs(uint32_t w, uint32_t s, uint32_t (&out)[4]) {
         if constexpr (kHalf) {
