@@ -34,16 +34,16 @@ int launch_narrow(const b200spmm_fp4_t *a, const DenseParams &d, cudaStream_t st
     prm.row_blocks = (prm.at_once * 16u + 126u) / 128u + 1u;
     const uint32_t stage = narrow_stage(kMx, prm.at_once, prm.row_blocks, kNB).bytes(), warps = prm.at_once * prm.slices;
     const uint32_t sums = prm.slices > 1 ? warps * 16u * 8u * kNB * (uint32_t)sizeof(float) : 0u;
-    prm.stages = std::min({kNarrowMaxStages, (kMostBytes - 384u - sums) / stage, std::max<uint32_t>(2, (d.k + kNarrowStage - 1) / kNarrowStage)});
+    prm.stages = std::min({kNarrowMaxStages, (kMostBytes - 1280u - sums) / stage, std::max<uint32_t>(2, (d.k + kNarrowStage - 1) / kNarrowStage)});
     B200_CUDA_TRY(status_word(&prm.status));
     prm.wait_limit_ns = kDeviceWaitLimitNs;
     CUtensorMap ma;
-    if (!encode_2d(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, d.pitch, d.m, d.pitch, kNarrowStep / 2, prm.at_once * 16u, CU_TENSOR_MAP_SWIZZLE_NONE,
+    if (!encode_2d(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, d.pitch, d.m, d.pitch, kNarrowStage / 2, prm.at_once * 16u, CU_TENSOR_MAP_SWIZZLE_128B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) {
         set_last_error_static("a tensor map of a 4-bit matrix could not be made");
         return B200SPMM_ERR_CUDA;
     }
-    B200_CUDA_TRY(launch_after(kernel, dim3(blocks, passes), 32 * (warps + 2), 384u + prm.stages * stage + sums, 1, stream, ma, prm));
+    B200_CUDA_TRY(launch_after(kernel, dim3(blocks, passes), 32 * (warps + kNarrowLoaders), 1280u + prm.stages * stage + sums, 1, stream, ma, prm));
     return B200SPMM_OK;
 }
 

@@ -7,12 +7,13 @@
 // at this width a product is a small part of the work, and for tcgen05 the numbers would have to go through shared or tensor memory).
 //
 // Tiles of 16 rows are shared out evenly over the SMs, one block of threads each, which goes through k with up to 13 of them at a time: one warp
-// brings stages of 256 values of k of all their rows, one the same of B, put in the order of the MMAs' operands, and 26
-// multiply, a tile or, k being sliced, a part of one each.  The slices' sums meet in shared memory, in order, at the end.  (Row blocks of
+// brings stages of 256 values of k of all their rows, two take turns with the same of B, put in the order of the MMAs' operands (one
+// alone kept the others waiting, 5 us for 8,192 values of k), and 26 multiply, a tile or, k being sliced, a part of one each.  The slices' sums meet in shared memory, in order, at the end.  (Row blocks of
 // 128 whose eight warps sliced k and fetched for themselves came to 38 us for 28672 x 8192 times one column: 224 blocks on 148 SMs, and 18
 // operations for eight values.)
 //
-// Lane 4 g + t takes 16 bytes of values, 32 codes, of rows g and g + 8 of its tile from k = 32 t of a step of 128 on.  Which k an operand
+// Lane 4 g + t takes 16 bytes of values, 32 codes, of rows r(g) and r(g) + 8 of its tile from k = 32 t of a step of 128 on; r puts rows that are
+// four apart side by side, whose pieces of a step lie in different halves of the swizzled 128 bytes.  Which k an operand
 // position of the MMA stands for is free as long as both operands agree: lane t's positions of MMA j are pairs 2 (j % 2) and
 // 2 (j % 2) + 1 of word j / 2 of its four, as Widen makes them.
 #pragma once
@@ -28,7 +29,7 @@ namespace fp4 {
 
 constexpr uint32_t kNarrowStep = 128, kNarrowStage = 256;  // values of k
 constexpr uint32_t kNarrowTiles = 13;                      // of 16 rows at a time
-constexpr uint32_t kNarrowWarps = 26;                      // that multiply, at most; two more load
+constexpr uint32_t kNarrowWarps = 26, kNarrowLoaders = 3;  // that multiply, at most, and load
 constexpr uint32_t kNarrowMaxStages = 8;
 
 struct NarrowParams {
@@ -45,10 +46,10 @@ struct NarrowParams {
 // Bytes of a stage: values, scales, B.
 struct NarrowStage {
     uint32_t values, scales, b;
-    __host__ __device__ uint32_t bytes() const { return values + scales + b; }
+    __host__ __device__ uint32_t bytes() const { return (values + scales + b + 1023u) / 1024u * 1024u; }  // (the swizzle's period)
 };
 __host__ __device__ inline NarrowStage narrow_stage(bool mx, uint32_t at_once, uint32_t row_blocks, uint32_t nb) {
-    return {2u * at_once * 16u * 64u, row_blocks * (mx ? 2u : 4u) * 512u, nb * kNarrowStage * 16u};
+    return {at_once * 16u * (kNarrowStage / 2), row_blocks * (mx ? 2u : 4u) * 512u, nb * kNarrowStage * 16u};
 }
 
 template <typename T>
@@ -68,18 +69,18 @@ B200_DEVICE void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
 
 // kNB: columns / 8.  kTokens: B lies [n][k], else [k][n].
 template <typename T, bool kMx, int kNB, bool kTokens>
-__global__ void __launch_bounds__(32 * (kNarrowWarps + 2), 1) fp4_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const NarrowParams p) {
+__global__ void __launch_bounds__(32 * (kNarrowWarps + kNarrowLoaders), 1) fp4_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const NarrowParams p) {
     using W = Widen<T, kMx>;
     constexpr uint32_t kGroups = kMx ? 2 : 4, kCols = 8 * kNB, kStepB = kNB * kNarrowStep * 16u;
     extern __shared__ uint8_t smem_raw[];
-    const uint32_t raw_addr = ptx::smem_u32(smem_raw), pad = (128u - (raw_addr & 127u)) & 127u, base = raw_addr + pad;
+    const uint32_t raw_addr = ptx::smem_u32(smem_raw), pad = (1024u - (raw_addr & 1023u)) & 1023u, base = raw_addr + pad;
     uint8_t *smem = smem_raw + pad;
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31u, g = lane >> 2, t = lane & 3u;
     const NarrowStage size = narrow_stage(kMx, p.at_once, p.row_blocks, kNB);
     const uint32_t stage_bytes = size.bytes(), consumers = p.at_once * p.slices;
-    const uint32_t bars = base, full = bars, empty = bars + 8u * kNarrowMaxStages, first_stage = base + 256u;
-    volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + 16 * kNarrowMaxStages);
-    float *sums = reinterpret_cast<float *>(smem + 256 + (size_t)p.stages * stage_bytes);
+    const uint32_t bars = base + p.stages * stage_bytes, full = bars, empty = bars + 8u * kNarrowMaxStages, first_stage = base;
+    volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + (size_t)p.stages * stage_bytes + 16 * kNarrowMaxStages);
+    float *sums = reinterpret_cast<float *>(smem + (size_t)p.stages * stage_bytes + 256);
     const uint32_t n0 = blockIdx.y * kCols;
     const uint32_t tile_begin = (uint32_t)((uint64_t)p.tiles * blockIdx.x / gridDim.x), tile_end = (uint32_t)((uint64_t)p.tiles * (blockIdx.x + 1u) / gridDim.x);
     const uint32_t k_stages = (p.d.k + kNarrowStage - 1) / kNarrowStage;
@@ -93,6 +94,9 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + 2), 1) fp4_narrow_kernel(
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&tmap_a);
     }
+    // columns past the end stay zeros, as far as B's warps do not come to them
+    for (uint32_t i = tid; i < p.stages * (size.b / 16u); i += blockDim.x)
+        ptx::st_shared_v4(first_stage + i / (size.b / 16u) * stage_bytes + size.values + size.scales + i % (size.b / 16u) * 16u, make_uint4(0u, 0u, 0u, 0u));
     ptx::wait_for_grids_before();
     __syncthreads();
     uint32_t s = 0, phase = 0;
@@ -104,7 +108,7 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + 2), 1) fp4_narrow_kernel(
     auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, ptx::mbar_wait(bar, parity, abort_flag, p.wait_limit_ns)) != 0; };
 
     if (warp == consumers) {
-        // =========================================================== A: values as two boxes of 64 bytes a row, scales by row blocks
+        // =========================================================== A: values in one box, 128 bytes a row, scales by row blocks
         const uint32_t on = lane == 0 ? 1u : 0u;
         for (uint32_t tile0 = tile_begin; alive && tile0 < tile_end; tile0 += p.at_once) {
             const uint32_t m0 = tile0 * 16u, rows = min(min(p.at_once, tile_end - tile0) * 16u, p.d.m - m0);
@@ -116,30 +120,36 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + 2), 1) fp4_narrow_kernel(
                 const uint32_t at = first_stage + s * stage_bytes, g0 = ks * kGroups, bytes = min(kGroups, p.d.groups - g0) * 512u;
                 ptx::mbar_arrive_expect_tx_if(on, full + 8u * s, size.values + blocks * bytes);
                 ptx::tma_load_2d_if(on, at, &tmap_a, (int32_t)(ks * (kNarrowStage / 2)), (int32_t)m0, full + 8u * s);
-                ptx::tma_load_2d_if(on, at + size.values / 2u, &tmap_a, (int32_t)(ks * (kNarrowStage / 2) + kNarrowStep / 2), (int32_t)m0, full + 8u * s);
                 for (uint32_t b = 0; b < blocks; ++b)
                     ptx::bulk_load_if(on, at + size.values + b * (kGroups * 512u), scales + ((uint64_t)b * p.d.groups + g0) * 512u, bytes, full + 8u * s);
                 step_on();
             }
         }
-    } else if (warp == consumers + 1u) {
+    } else if (warp > consumers) {
         // =========================================================== B.  [n][k]: 16 bytes of a column for each lane and word of codes;
         // [k][n]: rows of 8 columns, in the order that puts the eight which one operand needs side by side
         const T *b = reinterpret_cast<const T *>(p.d.b);
+        const uint32_t loads = kTokens ? min((uint32_t)kCols, p.d.n - n0) : kNB * 8u;
+        bool mine = warp == consumers + 1u;
         for (uint32_t tile0 = tile_begin; alive && tile0 < tile_end; tile0 += p.at_once) {
-            for (uint32_t ks = 0; ks < k_stages; ++ks) {
+            for (uint32_t ks = 0; ks < k_stages; ++ks, mine = !mine) {
+                if (!mine) {
+                    step_on();
+                    continue;
+                }
                 alive = wait(empty + 8u * s, phase ^ 1u);
                 if (!alive) break;
                 const uint32_t to = first_stage + s * stage_bytes + size.values + size.scales;
 #pragma unroll
                 for (uint32_t i = 0; i < (uint32_t)kNB * 8u; ++i) {
+                    if (i >= loads) break;
                     uint32_t at, left;
                     const T *src;
                     if constexpr (kTokens) {  // lane: which 16 bytes of a column's 512
-                        const uint32_t col = n0 + i, k = ks * kNarrowStage + lane * 8u, step = lane / 16u, tt = lane / 4u % 4u, w = lane % 4u;
+                        const uint32_t k = ks * kNarrowStage + lane * 8u, step = lane / 16u, tt = lane / 4u % 4u, w = lane % 4u;
                         at = step * kStepB + ((i / 8u * 4u + w) * 32u + i % 8u * 4u + tt) * 16u;
-                        left = col < p.d.n && k < p.d.k ? min(8u, p.d.k - k) : 0u;
-                        src = b + (int64_t)col * p.d.ldb + k;
+                        left = k < p.d.k ? min(8u, p.d.k - k) : 0u;
+                        src = b + (int64_t)(n0 + i) * p.d.ldb + k;
                     } else {
                         const uint32_t nb = i / 8u, kk = i % 4u * 32u + lane, k = ks * kNarrowStage + i % 8u * 32u + lane, col = n0 + nb * 8u;
                         const uint32_t order = W::kNeighbours ? lane : (lane & ~7u) | (lane & 3u) << 1 | (lane >> 2 & 1u);
@@ -164,12 +174,12 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + 2), 1) fp4_narrow_kernel(
         ptx::cp_async_commit();
         ptx::cp_async_wait_group<0>();
     } else if (warp < consumers) {
-        const uint32_t mine = warp / p.slices, slice = warp % p.slices;
+        const uint32_t mine = warp / p.slices, slice = warp % p.slices, r_of_g = (g >> 1) | (g & 1u) << 2;
         const float left = W::kLeft * (kMx ? 1.f : *reinterpret_cast<const volatile float *>(p.d.whole));
         for (uint32_t tile0 = tile_begin; alive && tile0 < tile_end; tile0 += p.at_once) {
-            const uint32_t m0 = tile0 * 16u, row = m0 + mine * 16u + g;
+            const uint32_t m0 = tile0 * 16u, row = m0 + mine * 16u + r_of_g;
             const bool busy = tile0 + mine < tile_end;
-            const uint32_t values_at = (mine * 16u + g) * 64u + t * 16u;
+            const uint32_t values_at = (mine * 16u + r_of_g) * 128u;
             // the words of scales of rows `row` and `row` + 8; those of a tile past the end may be anywhere in the stage
             auto scale_at = [&](uint32_t r) { return size.values + (busy ? r / 128u - m0 / 128u : 0u) * (kGroups * 512u) + (r & 31u) * 16u + (r >> 5 & 3u) * 4u; };
             const uint32_t lo_at = scale_at(row), hi_at = scale_at(row + 8u);
@@ -186,7 +196,8 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + 2), 1) fp4_narrow_kernel(
                     }
                     turn = p.slices - 1u;
                     const uint32_t at = first_stage + s * stage_bytes, b_at = at + size.values + size.scales + step * kStepB;
-                    const uint4 lo = ptx::ld_shared_v4(at + step * (size.values / 2u) + values_at), hi = ptx::ld_shared_v4(at + step * (size.values / 2u) + values_at + 8u * 64u);
+                    const uint32_t piece = at + values_at + ((step * 4u + t) ^ r_of_g) * 16u;
+                    const uint4 lo = ptx::ld_shared_v4(piece), hi = ptx::ld_shared_v4(piece + 8u * 128u);
                     const uint32_t group = kMx ? step : step * 2u + (t >> 1);
                     uint32_t f_lo = ptx::ld_shared_u32(at + lo_at + group * 512u), f_hi = ptx::ld_shared_u32(at + hi_at + group * 512u);
                     if (ks * kGroups + group >= p.d.groups) f_lo = f_hi = 0u;  // (not loaded)
@@ -237,7 +248,7 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + 2), 1) fp4_narrow_kernel(
 #pragma unroll
                 for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
 #pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) sums[(warp * kCols + nb * 8u + t * 2u + (e & 1u)) * 16u + (e >> 1) * 8u + g] = acc[nb][e];
+                    for (uint32_t e = 0; e < 4; ++e) sums[(warp * kCols + nb * 8u + t * 2u + (e & 1u)) * 16u + (e >> 1) * 8u + r_of_g] = acc[nb][e];
                 asm volatile("bar.sync 1, %0;" ::"r"(consumers * 32u) : "memory");
                 for (uint32_t i = tid; i < p.at_once * 16u * kCols; i += consumers * 32u) {
                     const uint32_t r = i % 16u, col = i / 16u % kCols, tile = i / (16u * kCols);
