@@ -20,23 +20,6 @@ struct Dest {
     uint32_t pitch, groups;
 };
 
-// 16 neighbours of a row as fp32, zeros behind `count`.  kWide: the address is a multiple of 16 bytes.
-template <typename T>
-B200_DEVICE void load16(const T *src, uint32_t count, bool wide, float (&v)[16]) {
-    if (wide && count >= 16u) {
-        constexpr int kVecs = 16 * sizeof(T) / 16;
-        uint4 raw[kVecs];
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) raw[i] = ptx::ld_global_v4(reinterpret_cast<const uint4 *>(src) + i);
-        const T *e = reinterpret_cast<const T *>(raw);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = Elem<T>::to_float(e[i]);
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) v[i] = i < count ? Elem<T>::to_float(src[i]) : 0.f;
-    }
-}
-
 // The bits of the largest magnitude (NaN above infinity above all numbers).
 template <int N>
 B200_DEVICE uint32_t top_bits(const float (&v)[N]) {
@@ -46,7 +29,8 @@ B200_DEVICE uint32_t top_bits(const float (&v)[N]) {
     return m;
 }
 
-// (row, unit) of a walk over rows of `units` units each, `step` units at a time.
+// (row, unit) of a walk over rows of `units` units each, `step` units at a time.  Rows are counted from the last one on where a pass follows
+// another over the same matrix: what that one read last is still in L2.
 struct Walk {
     uint32_t row, unit, row_step, unit_step, units;
     B200_DEVICE Walk(uint32_t units_, uint64_t first, uint64_t step) : units(max(units_, 1u)) {
@@ -75,26 +59,73 @@ B200_DEVICE uint32_t block_max(uint32_t m, uint32_t *shared) {
     return m;
 }
 
-// partial[block] = the largest finite magnitude that the block has seen.  Bound: one read of the matrix.
+// 16 neighbours as they are, zeros behind `count`.
+template <typename T>
+struct Raw16 {
+    uint4 v[sizeof(T)];
+    B200_DEVICE void load(const T *src, uint32_t count, bool wide) {
+        if (wide && count >= 16u) {
+#pragma unroll
+            for (uint32_t i = 0; i < sizeof(T); ++i) v[i] = ptx::ld_global_v4(reinterpret_cast<const uint4 *>(src) + i);
+        } else {
+            T *e = reinterpret_cast<T *>(v);
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) e[i] = i < count ? src[i] : Elem<T>::from_float(0.f);
+        }
+    }
+    // The bits of the largest magnitude, as those of an fp32 number; 16-bit types two at a time.
+    B200_DEVICE uint32_t top() const {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(v);
+        uint32_t m = 0;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+            return m;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+            const uint16_t one = (uint16_t)max(m & 0xFFFFu, m >> 16);
+            return __float_as_uint(Elem<T>::to_float(*reinterpret_cast<const T *>(&one)));
+        }
+    }
+    B200_DEVICE void floats(float (&f)[16]) const {
+        const T *e = reinterpret_cast<const T *>(v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = Elem<T>::to_float(e[i]);
+    }
+    // ... of those that are finite.
+    B200_DEVICE uint32_t finite_top() const {
+        const uint32_t t = top();
+        if (t < kInfBits) return t;
+        float f[16];
+        floats(f);
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t b = __float_as_uint(f[i]) & 0x7FFFFFFFu;
+            m = max(m, b < kInfBits ? b : 0u);
+        }
+        return m;
+    }
+};
+
+// partial[block] = the largest finite magnitude that the block has seen.  Bound: one read of the matrix; 64 bytes a thread are under way.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) amax_kernel(const T *__restrict__ x, int64_t ldx, uint32_t rows, uint32_t cols, bool wide,
                                                         float *__restrict__ partial) {
+    constexpr int kAhead = sizeof(T) == 4 ? 1 : 2;
     __shared__ uint32_t shared[kThreads / 32];
     ptx::wait_for_grids_before();
     uint32_t m = 0;
-    for (Walk w((cols + 15u) / 16u, (uint64_t)blockIdx.x * kThreads + threadIdx.x, (uint64_t)gridDim.x * kThreads); w.row < rows; w.next()) {
-        float v[16];
-        load16(x + (int64_t)w.row * ldx + w.unit * 16u, cols - w.unit * 16u, wide, v);
-        uint32_t t = top_bits(v);
-        if (t >= kInfBits) {  // only what is finite counts
-            t = 0;
+    for (Walk w((cols + 15u) / 16u, (uint64_t)blockIdx.x * kThreads + threadIdx.x, (uint64_t)gridDim.x * kThreads); w.row < rows;) {
+        Raw16<T> v[kAhead];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-                t = max(t, b < kInfBits ? b : 0u);
-            }
+        for (int i = 0; i < kAhead; ++i) {
+            v[i].load(x + (int64_t)w.row * ldx + w.unit * 16u, w.row < rows ? cols - w.unit * 16u : 0u, wide);
+            w.next();
         }
-        m = max(m, t);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) m = max(m, v[i].finite_top());
     }
     m = block_max(m, shared);
     if (threadIdx.x == 0) partial[blockIdx.x] = __uint_as_float(m);
@@ -108,72 +139,114 @@ B200_DEVICE int find_exponent(const float *partial, uint32_t n_partial, const fl
     return tensor_exponent(__uint_as_float(block_max(m, shared)));
 }
 
-// Blocks along the rows of x.  A thread takes 16 neighbours; four (nvfp4) or eight (mxfp4) lanes together hold the four scales
-// that lie in one word.  Rows end with units that hold nothing: the scales behind the last column, which the products read, are zeros.
+// One unit of 16 neighbours of a row, `raw`, to codes and scales.  Four (nvfp4) or eight (mxfp4) lanes together hold the four scales that lie
+// in one word; all lanes of a warp take part.
 template <typename T, bool kMx>
-__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T *__restrict__ x, int64_t ldx, bool wide, const float *partial, uint32_t n_partial,
-                                                                 const float *given, const Dest d) {
+B200_DEVICE void quantize_unit(const Raw16<T> &raw, float inv_tensor, bool here, uint32_t row, uint32_t unit, const Dest &d) {
+    constexpr uint32_t kLanes = kMx ? 8 : 4;
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t top = raw.top(), byte;
+    float v[16];
+    raw.floats(v);
+    uint2 codes;
+    if constexpr (kMx) {
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        float factor;
+        byte = block_scale_mx(top, factor);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = byte == 0xFFu ? 0.f : v[i] * factor;
+        codes = make_uint2(to_e2m1x8(v), to_e2m1x8(v + 8));
+        byte <<= (lane >> 1 & 3u) * 8u;
+        byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 2);
+        byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 4);
+    } else {
+        byte = quantize_block_nv(v, top, inv_tensor, codes) << (lane & 3u) * 8u;
+        byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 1);
+        byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 2);
+    }
+    if (!here) return;
+    if (unit * 8u < d.pitch) *reinterpret_cast<uint2 *>(d.values + (uint64_t)row * d.pitch + unit * 8u) = codes;
+    if (lane % kLanes == 0) *reinterpret_cast<uint32_t *>(d.scales + scale_word(row, unit / kLanes, d.groups)) = byte;
+}
+
+B200_DEVICE float inverse_exp2(int k) { return k == 127 ? __uint_as_float(0x00400000u) : exp2_int(-k); }
+
+// Blocks along the rows of x, a unit a thread.  Rows end with units that hold nothing: the scales behind the last column, which the
+// products read, are zeros.  Bound: reading x once (after amax_kernel, which leaves its last rows in L2: they come first) and writing the
+// codes: 28672 x 8192 fp16 103 us in mxfp4, 5.9 TB/s.
+template <typename T, bool kMx>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T *__restrict__ x, int64_t ldx, const float *partial, uint32_t n_partial, const float *given,
+                                                                 const Dest d) {
     __shared__ uint32_t shared[kThreads / 32];
     ptx::wait_for_grids_before();
     float inv_tensor = 1.f;
     if constexpr (!kMx) {
         const int k = find_exponent(partial, n_partial, given, shared);
         if (blockIdx.x == 0 && threadIdx.x == 0) *d.tensor_scale = exp2_int(k);
-        inv_tensor = k == 127 ? __uint_as_float(0x00400000u) : exp2_int(-k);
+        inv_tensor = inverse_exp2(k);
     } else if (blockIdx.x == 0 && threadIdx.x == 0) {
         *d.tensor_scale = 1.f;
     }
-    constexpr uint32_t kLanes = kMx ? 8 : 4;  // of a word of scales
-    const uint32_t lane = threadIdx.x & 31u;
-    for (Walk w(d.groups * kLanes, (uint64_t)blockIdx.x * kThreads + threadIdx.x, (uint64_t)gridDim.x * kThreads);
+    for (Walk w(d.groups * (kMx ? 8u : 4u), (uint64_t)blockIdx.x * kThreads + threadIdx.x, (uint64_t)gridDim.x * kThreads);
          __any_sync(0xFFFFFFFFu, w.row < d.rows); w.next()) {
         const bool here = w.row < d.rows;
-        const uint32_t col = w.unit * 16u;
-        float v[16];
-        load16(x + (int64_t)w.row * ldx + col, here && col < d.cols ? d.cols - col : 0u, wide, v);
-        uint32_t top = top_bits(v), byte;
-        uint2 codes;
-        if constexpr (kMx) {
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            float factor;
-            byte = block_scale_mx(top, factor);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = byte == 0xFFu ? 0.f : v[i] * factor;
-            codes = make_uint2(to_e2m1x8(v), to_e2m1x8(v + 8));
-            byte <<= (lane >> 1 & 3u) * 8u;
-            byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 2);
-            byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 4);
-        } else {
-            byte = quantize_block_nv(v, top, inv_tensor, codes) << (lane & 3u) * 8u;
-            byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 1);
-            byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 2);
-        }
-        if (!here) continue;  // (no lane leaves the loop alone: the condition is the warp's)
-        if (col / 2u < d.pitch) *reinterpret_cast<uint2 *>(d.values + (uint64_t)w.row * d.pitch + col / 2u) = codes;
-        if (lane % kLanes == 0) *reinterpret_cast<uint32_t *>(d.scales + scale_word(w.row, w.unit / kLanes, d.groups)) = byte;
+        const uint32_t col = w.unit * 16u, row = d.rows - 1u - w.row;
+        Raw16<T> raw;
+        raw.load(x + (int64_t)row * ldx + col, here && col < d.cols ? d.cols - col : 0u, true);
+        quantize_unit<T, kMx>(raw, inv_tensor, here, row, w.unit, d);
     }
 }
 
-// Blocks along the columns of x (kCols: the 4-bit matrix is the transpose), along the rows, or both from one read.  A block of
-// threads takes 128 x 64 of x through shared memory, which is read once along either axis; what goes to the transpose is put
-// together there as well, so that 64 neighbouring bytes are written.
+// A small matrix in nvfp4, a unit for every thread of one cluster: its largest value is found and used in the same launch.  Bound: latency
+// (8 x 8192, the activations of eight tokens).
+constexpr unsigned kClusterCtas = 8, kClusterThreads = 1024;
+template <typename T>
+__global__ void __launch_bounds__(kClusterThreads) quantize_cluster_kernel(const T *__restrict__ x, int64_t ldx, const Dest d) {
+    __shared__ uint32_t shared[kClusterThreads / 32], all[kClusterCtas];
+    ptx::wait_for_grids_before();
+    const uint32_t units = max(d.groups * 4u, 1u), at = blockIdx.x * blockDim.x + threadIdx.x, row = at / units, unit = at % units;
+    const bool here = row < d.rows;
+    Raw16<T> raw;
+    raw.load(x + (int64_t)row * ldx + unit * 16u, here && unit * 16u < d.cols ? d.cols - unit * 16u : 0u, true);
+    uint32_t m = __reduce_max_sync(0xFFFFFFFFu, raw.finite_top());
+    if ((threadIdx.x & 31u) == 0) shared[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x < 32u) {
+        m = __reduce_max_sync(0xFFFFFFFFu, threadIdx.x < blockDim.x / 32u ? shared[threadIdx.x] : 0u);
+        // to every CTA of the cluster, each its own place
+        if (threadIdx.x < gridDim.x) ptx::st_cluster_u32(ptx::map_to_cta(ptx::smem_u32(all + blockIdx.x), threadIdx.x), m);
+    }
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+    m = 0;
+    for (uint32_t i = 0; i < gridDim.x; ++i) m = max(m, all[i]);
+    const int k = tensor_exponent(__uint_as_float(m));
+    if (at == 0) *d.tensor_scale = exp2_int(k);
+    quantize_unit<T, false>(raw, inverse_exp2(k), here, row, unit, d);
+}
+
+// Blocks along the columns of x (kCols: the 4-bit matrix is the transpose), along the rows, or both from one read; also rows that start on
+// any element.  A block of threads takes 128 x 64 of x through shared memory, where it is read along either axis: columns two at a time and 16
+// rows a thread, the other 16 of an mxfp4 block being 16 lanes away.  Rows lie in shared memory with their halves exchanged
+// where bit 4 of their number is set, so that those lanes do not collide.  What goes to the transpose is put together there as
+// well, and leaves 64 neighbouring bytes at a time.
 constexpr uint32_t kTileR = 128, kTileC = 64, kOutPitch = kTileR / 2 + 16;
 
 template <typename T, bool kMx, bool kRows, bool kCols>
 __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T *__restrict__ x, int64_t ldx, uint32_t x_rows, uint32_t x_cols, bool wide,
                                                                   const float *partial, uint32_t n_partial, const float *given, const Dest by_rows,
                                                                   const Dest by_cols, uint32_t tiles_c, uint64_t tiles) {
-    constexpr uint32_t kPitch = kTileC + 16 / sizeof(T);  // elements: 16 bytes more than a row, so that neither way of reading collides
-    __shared__ __align__(16) T tile[kTileR * kPitch];
-    __shared__ __align__(16) uint8_t out[kTileC * kOutPitch];
-    __shared__ __align__(16) uint8_t out_scale[kTileC * 8];
+    constexpr uint32_t kPer = 16 / sizeof(T), kVecs = kTileC / kPer;  // elements of a piece, pieces of a row
+    __shared__ __align__(16) uint4 tile[kTileR * kVecs];
+    __shared__ __align__(16) uint8_t out[kCols ? kTileC * kOutPitch : 16];
+    __shared__ __align__(16) uint8_t out_scale[kCols ? kTileC * 8 : 16];
     __shared__ uint32_t shared[kThreads / 32];
     ptx::wait_for_grids_before();
-    const uint32_t tid = threadIdx.x;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u;
     float inv_tensor = 1.f;
     if constexpr (!kMx) {
         const int k = find_exponent(partial, n_partial, given, shared);
-        inv_tensor = k == 127 ? __uint_as_float(0x00400000u) : exp2_int(-k);
+        inv_tensor = inverse_exp2(k);
         if (blockIdx.x == 0 && tid == 0) {
             if (kRows) *by_rows.tensor_scale = exp2_int(k);
             if (kCols) *by_cols.tensor_scale = exp2_int(k);
@@ -182,40 +255,38 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T *__res
         if (kRows) *by_rows.tensor_scale = 1.f;
         if (kCols) *by_cols.tensor_scale = 1.f;
     }
+    auto piece = [&](uint32_t r, uint32_t p) { return r * kVecs + (p ^ ((r >> 4 & 1u) * (kVecs / 2u))); };
     for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const uint32_t r0 = (uint32_t)(t / tiles_c) * kTileR, c0 = (uint32_t)(t % tiles_c) * kTileC;
-        if (wide) {
-            constexpr uint32_t kPer = 16 / sizeof(T), kVecs = kTileC / kPer;
-            for (uint32_t i = tid; i < kTileR * kVecs; i += kThreads) {
-                const uint32_t r = i / kVecs, c = i % kVecs * kPer;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (r0 + r < x_rows) {
-                    const T *src = x + (int64_t)(r0 + r) * ldx + c0 + c;
-                    if (c0 + c + kPer <= x_cols) {
-                        v = ptx::ld_global_v4(src);
-                    } else {
-                        T *e = reinterpret_cast<T *>(&v);
-                        for (uint32_t j = 0; j < kPer; ++j)
-                            if (c0 + c + j < x_cols) e[j] = src[j];
-                    }
-                }
-                *reinterpret_cast<uint4 *>(tile + r * kPitch + c) = v;
+        const uint64_t u = tiles - 1u - t;  // from the end on, see Walk
+        const uint32_t r0 = (uint32_t)(u / tiles_c) * kTileR, c0 = (uint32_t)(u % tiles_c) * kTileC;
+        if (wide && c0 + kTileC <= x_cols) {
+            uint4 v[kTileR * kVecs / kThreads];
+#pragma unroll
+            for (uint32_t i = 0; i < kTileR * kVecs / kThreads; ++i) {
+                const uint32_t r = (i * kThreads + tid) / kVecs, p = (i * kThreads + tid) % kVecs;
+                v[i] = r0 + r < x_rows ? ptx::ld_global_v4(x + (int64_t)(r0 + r) * ldx + c0 + p * kPer) : make_uint4(0u, 0u, 0u, 0u);
             }
+#pragma unroll
+            for (uint32_t i = 0; i < kTileR * kVecs / kThreads; ++i) tile[piece((i * kThreads + tid) / kVecs, (i * kThreads + tid) % kVecs)] = v[i];
         } else {
+#pragma unroll 8
             for (uint32_t i = tid; i < kTileR * kTileC; i += kThreads) {
                 const uint32_t r = i / kTileC, c = i % kTileC;
-                tile[r * kPitch + c] = r0 + r < x_rows && c0 + c < x_cols ? x[(int64_t)(r0 + r) * ldx + c0 + c] : Elem<T>::from_float(0.f);
+                reinterpret_cast<T *>(tile + piece(r, c / kPer))[c % kPer] =
+                    r0 + r < x_rows && c0 + c < x_cols ? x[(int64_t)(r0 + r) * ldx + c0 + c] : Elem<T>::from_float(0.f);
             }
         }
         __syncthreads();
         if constexpr (kRows) {
-            for (uint32_t i = tid; i < kTileR * (kTileC / 16); i += kThreads) {
-                const uint32_t r = i / 4, u = i % 4, row = r0 + r, col = c0 + u * 16;
-                float v[16];
-                const T *src = tile + r * kPitch + u * 16;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = Elem<T>::to_float(src[j]);
-                uint32_t top = top_bits(v), byte;
+            for (uint32_t i = tid; i < kTileR * (kTileC / 16); i += kThreads) {
+                const uint32_t r = i / 4, q = i % 4, row = r0 + r, col = c0 + q * 16;
+                Raw16<T> raw;
+#pragma unroll
+                for (uint32_t j = 0; j < sizeof(T); ++j) raw.v[j] = tile[piece(r, q * sizeof(T) + j)];
+                uint32_t top = raw.top(), byte;
+                float v[16];
+                raw.floats(v);
                 uint2 codes;
                 if constexpr (kMx) {
                     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
@@ -224,16 +295,16 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T *__res
 #pragma unroll
                     for (int j = 0; j < 16; ++j) v[j] = byte == 0xFFu ? 0.f : v[j] * factor;
                     codes = make_uint2(to_e2m1x8(v), to_e2m1x8(v + 8));
-                    byte <<= (u >> 1) * 8u;
+                    byte <<= (q >> 1) * 8u;
                     byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 2);
                 } else {
-                    byte = quantize_block_nv(v, top, inv_tensor, codes) << u * 8u;
+                    byte = quantize_block_nv(v, top, inv_tensor, codes) << q * 8u;
                     byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 1);
                     byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 2);
                 }
                 if (row < by_rows.rows) {
                     if (col / 2u < by_rows.pitch) *reinterpret_cast<uint2 *>(by_rows.values + (uint64_t)row * by_rows.pitch + col / 2u) = codes;
-                    if (u == 0) {
+                    if (q == 0) {
                         if constexpr (kMx) {  // a tile is half a word of scales wide
                             if (c0 / 128u < by_rows.groups)
                                 *reinterpret_cast<uint16_t *>(by_rows.scales + scale_word(row, c0 / 128u, by_rows.groups) + (c0 / 64u & 1u) * 2u) = (uint16_t)byte;
@@ -245,71 +316,121 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T *__res
             }
         }
         if constexpr (kCols) {
-            constexpr uint32_t kBlk = kMx ? 32 : 16;
-            for (uint32_t i = tid; i < kTileC * (kTileR / kBlk); i += kThreads) {
-                const uint32_t c = i % kTileC, b = i / kTileC;
-                float v[kBlk];
+            // lanes 0-15 and 16-31: 16 rows each, of columns 2 (lane % 16) and + 1 of a half of the tile
+            const uint32_t b = (tid >> 6) * 2u + (lane >> 4), c = ((tid >> 5 & 1u) * 16u + (lane & 15u)) * 2u;
+            float v[2][16];
+            uint32_t top[2] = {0u, 0u};
 #pragma unroll
-                for (uint32_t j = 0; j < kBlk; ++j) v[j] = Elem<T>::to_float(tile[(b * kBlk + j) * kPitch + c]);
-                const uint32_t top = top_bits(v);
+            for (uint32_t j = 0; j < 16; ++j) {
+                const T *e = reinterpret_cast<const T *>(tile + piece(b * 16u + j, c / kPer)) + c % kPer;
+                struct alignas(2 * sizeof(T)) Two { T a, b; };
+                const Two two = *reinterpret_cast<const Two *>(e);
+                v[0][j] = Elem<T>::to_float(two.a);
+                v[1][j] = Elem<T>::to_float(two.b);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 2; ++k) {
+                top[k] = top_bits(v[k]);
+                uint2 codes;
                 if constexpr (kMx) {
+                    const uint32_t both = max(top[k], __shfl_xor_sync(0xFFFFFFFFu, top[k], 16));
                     float factor;
-                    const uint32_t byte = block_scale_mx(top, factor);
+                    const uint32_t byte = block_scale_mx(both, factor);
 #pragma unroll
-                    for (uint32_t j = 0; j < kBlk; ++j) v[j] = byte == 0xFFu ? 0.f : v[j] * factor;
-                    *reinterpret_cast<uint4 *>(out + c * kOutPitch + b * 16u) =
-                        make_uint4(to_e2m1x8(v), to_e2m1x8(v + 8), to_e2m1x8(v + 16), to_e2m1x8(v + 24));
-                    out_scale[c * 8u + b] = (uint8_t)byte;
+                    for (uint32_t j = 0; j < 16; ++j) v[k][j] = byte == 0xFFu ? 0.f : v[k][j] * factor;
+                    codes = make_uint2(to_e2m1x8(v[k]), to_e2m1x8(v[k] + 8));
+                    if (lane < 16u) out_scale[(c + k) * 8u + b / 2u] = (uint8_t)byte;
                 } else {
-                    uint2 codes;
-                    out_scale[c * 8u + b] = (uint8_t)quantize_block_nv(v, top, inv_tensor, codes);
-                    *reinterpret_cast<uint2 *>(out + c * kOutPitch + b * 8u) = codes;
+                    out_scale[(c + k) * 8u + b] = (uint8_t)quantize_block_nv(v[k], top[k], inv_tensor, codes);
                 }
+                *reinterpret_cast<uint2 *>(out + (c + k) * kOutPitch + b * 8u) = codes;
             }
             __syncthreads();
             for (uint32_t i = tid; i < kTileC * 4u; i += kThreads) {
-                const uint32_t c = i / 4, q = i % 4, row = c0 + c, at = r0 / 2u + q * 16u;
+                const uint32_t col = i / 4, q = i % 4, row = c0 + col, at = r0 / 2u + q * 16u;
                 if (row < by_cols.rows && at < by_cols.pitch)
-                    *reinterpret_cast<uint4 *>(by_cols.values + (uint64_t)row * by_cols.pitch + at) = *reinterpret_cast<const uint4 *>(out + c * kOutPitch + q * 16u);
+                    *reinterpret_cast<uint4 *>(by_cols.values + (uint64_t)row * by_cols.pitch + at) = *reinterpret_cast<const uint4 *>(out + col * kOutPitch + q * 16u);
             }
             constexpr uint32_t kWords = kMx ? 1 : 2;  // of scales for a column of the tile
             for (uint32_t i = tid; i < kTileC * kWords; i += kThreads) {
-                const uint32_t c = i / kWords, w = i % kWords, row = c0 + c, group = r0 / kTileR * kWords + w;
+                const uint32_t col = i / kWords, w = i % kWords, row = c0 + col, group = r0 / kTileR * kWords + w;
                 if (row < by_cols.rows && group < by_cols.groups)
-                    *reinterpret_cast<uint32_t *>(by_cols.scales + scale_word(row, group, by_cols.groups)) = *reinterpret_cast<const uint32_t *>(out_scale + c * 8u + w * 4u);
+                    *reinterpret_cast<uint32_t *>(by_cols.scales + scale_word(row, group, by_cols.groups)) = *reinterpret_cast<const uint32_t *>(out_scale + col * 8u + w * 4u);
             }
         }
         __syncthreads();  // the next tile overwrites what this one reads
     }
 }
 
-// A thread takes 16 values and their scale.  Bound: reading the matrix and writing x once.
+// A thread takes eight values, a word of codes, and writes them in one piece; where rows start anywhere, a warp's 256 values go through
+// shuffles and leave 32 neighbours at a time.  Bound: reading the matrix and writing x once.
 template <typename T, bool kMx>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t *__restrict__ values, const uint8_t *__restrict__ scales,
                                                               const float *__restrict__ tensor_scale, uint32_t rows, uint32_t cols, uint32_t pitch,
                                                               uint32_t groups, T *__restrict__ x, int64_t ldx, bool wide) {
+    constexpr uint32_t kAhead = 4;
     ptx::wait_for_grids_before();
+    const uint32_t lane = threadIdx.x & 31u;
     const float whole = kMx ? 1.f : *reinterpret_cast<const volatile float *>(tensor_scale);
-    for (Walk w((cols + 15u) / 16u, (uint64_t)blockIdx.x * kThreads + threadIdx.x, (uint64_t)gridDim.x * kThreads); w.row < rows; w.next()) {
-        const uint2 codes = *reinterpret_cast<const uint2 *>(values + (uint64_t)w.row * pitch + w.unit * 8u);
-        const uint32_t block = kMx ? w.unit / 2u : w.unit;
-        const uint32_t byte = scales[scale_word(w.row, block / 4u, groups) + block % 4u];
-        const float s = kMx ? from_e8m0(byte) : from_e4m3(byte);
-        T out[16];
+    // a warp's unit: 256 columns of a row
+    for (Walk w((cols + 255u) / 256u, ((uint64_t)blockIdx.x * kThreads + threadIdx.x) / 32u, (uint64_t)gridDim.x * (kThreads / 32u)); w.row < rows;) {
+        uint32_t codes[kAhead], row[kAhead], col[kAhead];
+        uint8_t bytes[kAhead];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float2 two = __half22float2(from_e2m1x2((i < 4 ? codes.x : codes.y) >> (i & 3) * 8));
-            out[2 * i] = Elem<T>::from_float(two.x * s * whole);  // code times scale is exact: one rounding, and one to T
-            out[2 * i + 1] = Elem<T>::from_float(two.y * s * whole);
+        for (uint32_t a = 0; a < kAhead; ++a) {
+            row[a] = w.row;
+            col[a] = w.unit * 256u + lane * 8u;
+            const bool here = w.row < rows && col[a] < cols;
+            const uint32_t block = col[a] / (kMx ? 32u : 16u);
+            codes[a] = here ? *reinterpret_cast<const uint32_t *>(values + (uint64_t)row[a] * pitch + col[a] / 2u) : 0u;
+            bytes[a] = here ? scales[scale_word(row[a], block / 4u, groups) + block % 4u] : (uint8_t)0u;
+            w.next();
         }
-        T *dst = x + (int64_t)w.row * ldx + w.unit * 16u;
-        if (wide && cols - w.unit * 16u >= 16u) {
 #pragma unroll
-            for (uint32_t i = 0; i < 16 * sizeof(T) / 16; ++i) reinterpret_cast<uint4 *>(dst)[i] = reinterpret_cast<const uint4 *>(out)[i];
-        } else {
+        for (uint32_t a = 0; a < kAhead; ++a) {
+            const float s = kMx ? from_e8m0(bytes[a]) : from_e4m3(bytes[a]);
+            const bool here = row[a] < rows;  // (the warp's)
+            float v[8];
 #pragma unroll
-            for (uint32_t i = 0; i < 16; ++i)
-                if (w.unit * 16u + i < cols) dst[i] = out[i];
+            for (int i = 0; i < 4; ++i) {
+                const float2 two = __half22float2(from_e2m1x2(codes[a] >> i * 8));
+                v[2 * i] = two.x * s * whole;  // code times scale is exact: one rounding, and one to T
+                v[2 * i + 1] = two.y * s * whole;
+            }
+            T *dst = x + (int64_t)row[a] * ldx + col[a];
+            if (wide && here && col[a] + 8u <= cols) {
+                uint4 out[sizeof(T) / 2];
+                T *e = reinterpret_cast<T *>(out);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = Elem<T>::from_float(v[i]);
+                if constexpr (sizeof(T) == 4) {
+                    if ((reinterpret_cast<uintptr_t>(dst) & 31u) == 0) {
+                        ptx::st_global_v8(dst, reinterpret_cast<const uint32_t *>(out));
+                    } else {
+                        reinterpret_cast<uint4 *>(dst)[0] = out[0];
+                        reinterpret_cast<uint4 *>(dst)[1] = out[1];
+                    }
+                } else {
+                    *reinterpret_cast<uint4 *>(dst) = out[0];
+                }
+            } else if (wide) {
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    if (here && col[a] + i < cols) dst[i] = Elem<T>::from_float(v[i]);
+            } else if (here) {
+                const uint32_t first = col[a] - lane * 8u;
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {  // value 32 i + lane of the warp's: lane 4 i + lane / 8 has it, as its value lane % 8
+                    float mine = 0.f;
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; ++j) {
+                        const float f = __shfl_sync(0xFFFFFFFFu, v[j], (int)(i * 4u + lane / 8u));
+                        if (lane % 8u == j) mine = f;
+                    }
+                    const uint32_t c = first + i * 32u + lane;
+                    if (c < cols) x[(int64_t)row[a] * ldx + c] = Elem<T>::from_float(mine);
+                }
+            }
         }
     }
 }
@@ -328,23 +449,27 @@ int quantize_typed(const T *x, int64_t ldx, uint32_t x_rows, uint32_t x_cols, co
                    const b200spmm_fp4_t *by_cols, float *workspace, cudaStream_t stream) {
     const bool wide = reinterpret_cast<uintptr_t>(x) % 16u == 0 && ldx * (int64_t)sizeof(T) % 16 == 0;
     uint32_t n_partial = 0;
+    const uint64_t row_units = by_rows ? (uint64_t)dest_of(by_rows).rows * dest_of(by_rows).groups * (kMx ? 8u : 4u) : 0;
+    if (!kMx && !given && !by_cols && wide && row_units <= kClusterCtas * kClusterThreads) {
+        const unsigned ctas = (unsigned)std::max<uint64_t>(1, (row_units + kClusterThreads - 1) / kClusterThreads);
+        B200_CUDA_TRY(launch_after(quantize_cluster_kernel<T>, dim3(ctas), kClusterThreads, 0, ctas, stream, x, ldx, dest_of(by_rows)));
+        return B200SPMM_OK;
+    }
     if (!kMx && !given) {
         const uint64_t units = (uint64_t)x_rows * ((x_cols + 15u) / 16u);
         n_partial = std::min(kAmaxBlocks, grid_for((units + kThreads - 1) / kThreads));
         B200_CUDA_TRY(launch_after(amax_kernel<T>, dim3(n_partial), kThreads, 0, 1, stream, x, ldx, x_rows, x_cols, wide, workspace));
     }
-    if (!by_cols) {
-        const Dest d = dest_of(by_rows);
-        const uint64_t units = (uint64_t)d.rows * d.groups * (kMx ? 8u : 4u);
-        B200_CUDA_TRY(launch_after(quantize_rows_kernel<T, kMx>, dim3(grid_for((units + kThreads - 1) / kThreads)), kThreads, 0, 1, stream, x, ldx, wide,
-                                   (const float *)workspace, n_partial, given, d));
+    if (!by_cols && wide) {
+        B200_CUDA_TRY(launch_after(quantize_rows_kernel<T, kMx>, dim3(grid_for((row_units + kThreads - 1) / kThreads)), kThreads, 0, 1, stream, x, ldx,
+                                   (const float *)workspace, n_partial, given, dest_of(by_rows)));
         return B200SPMM_OK;
     }
-    const Dest rows = by_rows ? dest_of(by_rows) : Dest{}, cols = dest_of(by_cols);
+    const Dest rows = by_rows ? dest_of(by_rows) : Dest{}, cols = by_cols ? dest_of(by_cols) : Dest{};
     // the tiles cover the padded scales of either matrix, too
     const uint32_t tiles_c = std::max<uint32_t>((x_cols + kTileC - 1) / kTileC, rows.groups * (kMx ? 2u : 1u));
     const uint64_t tiles = (uint64_t)tiles_c * ((x_rows + kTileR - 1) / kTileR);
-    auto kernel = by_rows ? quantize_tiles_kernel<T, kMx, true, true> : quantize_tiles_kernel<T, kMx, false, true>;
+    auto kernel = !by_cols ? quantize_tiles_kernel<T, kMx, true, false> : by_rows ? quantize_tiles_kernel<T, kMx, true, true> : quantize_tiles_kernel<T, kMx, false, true>;
     B200_CUDA_TRY(launch_after(kernel, dim3(grid_for(tiles)), kThreads, 0, 1, stream, x, ldx, x_rows, x_cols, wide, (const float *)workspace, n_partial,
                                given, rows, cols, tiles_c, tiles));
     return B200SPMM_OK;
@@ -354,7 +479,7 @@ template <typename T>
 int dequantize_typed(const b200spmm_fp4_t *a, T *x, int64_t ldx, cudaStream_t stream) {
     const Dest d = dest_of(a);
     const bool wide = reinterpret_cast<uintptr_t>(x) % 16u == 0 && ldx * (int64_t)sizeof(T) % 16 == 0;
-    const uint64_t units = (uint64_t)d.rows * ((d.cols + 15u) / 16u);
+    const uint64_t units = (uint64_t)d.rows * ((d.cols + 255u) / 256u) * 8u;  // a warp's four at a time
     auto kernel = a->format == B200SPMM_MXFP4 ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
     B200_CUDA_TRY(launch_after(kernel, dim3(grid_for((units + kThreads - 1) / kThreads)), kThreads, 0, 1, stream, (const uint8_t *)d.values,
                                (const uint8_t *)d.scales, (const float *)d.tensor_scale, d.rows, d.cols, d.pitch, d.groups, x, ldx, wide));

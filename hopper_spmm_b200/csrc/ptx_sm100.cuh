@@ -45,6 +45,12 @@ B200_DEVICE void ld_global_v8(const void *p, uint32_t *v) {
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "l"(p) : "memory");
 }
 
+// 32 bytes, 32-byte aligned.
+B200_DEVICE void st_global_v8(void *p, const uint32_t *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
 // A load of a stream that nothing writes: what is not in L2 comes with the 256 bytes around it, the next of the stream.  (The
 // entries of row units, of which a lane group has one batch under way: 300,000 nodes, 64 / 128 features 77.6 / 141 -> 73.4 / 136
 // us, 2^20 nodes, 64 features 230 -> 220; an instruction of its own that fetches ahead costs 5 to 20 % instead.)
