@@ -71,28 +71,42 @@ B200_DEVICE int exponent_above(float scale) {
 // scale = e4m3(amax / 6 / 2^k), codes e2m1(x / scale / 2^k).  Both quotients have to be rounded as real numbers are, or values next
 // to a border between two codes - many, where x has few digits - would fall on the wrong side.  A rounded fp32 quotient does that:
 // the borders have at most seven bits after multiplication by the divisor, so an fp32 dividend that is not on one is far enough from
-// it for its rounded quotient not to be on one either.  x / scale is rounded by Markstein's method (multiply by the rounded
-// reciprocal, add the remainder times it), three operations for an element instead of a division.
-B200_DEVICE uint32_t quantize_block_nv(const float (&v)[16], uint32_t top, float inv_tensor, uint2 &codes) {
+// it for its rounded quotient not to be on one either.  x / (scale 2^k) is rounded by Markstein's method (multiply by the rounded
+// reciprocal, add the remainder times it), three operations for an element instead of a division.  The remainder is exact; it is
+// rounded down only so that it is -0 where it vanishes, which leaves the quotient of -0 its sign.
+struct TensorScale {
+    float up, down;  // 2^k, 2^-k
+    bool plain;      // neither block scales nor their reciprocals leave fp32's normal range with it
+    B200_DEVICE explicit TensorScale(int k) {
+        up = exp2_int(k);
+        down = k == 127 ? __uint_as_float(0x00400000u) : exp2_int(-k);
+        plain = k > -100 && k < 100;
+    }
+};
+B200_DEVICE uint32_t quantize_block_nv(const float (&v)[16], uint32_t top, const TensorScale &tensor, uint2 &codes) {
     if (top >= kInfBits) {  // infinity or NaN: the block is NaN
         codes = make_uint2(0u, 0u);
         return 0x7Fu;
     }
     const float amax = __uint_as_float(top);
-    const uint32_t byte = to_e4m3(__fdiv_rn(amax, 6.f) * inv_tensor);
+    const uint32_t byte = to_e4m3(__fdiv_rn(amax, 6.f) * tensor.down);
     const float s = from_e4m3(byte);
     const float r = byte ? __frcp_rn(s) : 0.f;
     float q[16];
-    if (amax * inv_tensor < 1e30f) {
+    if (tensor.plain && amax * tensor.down < 1e30f) {
+        const float rs = r * tensor.down, ss = -s * tensor.up;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float x = v[i] * inv_tensor;
-            const float q0 = x * r;
-            q[i] = copysignf(__fmaf_rn(__fmaf_rn(-q0, s, x), r, q0), x);  // (-0 would come out as 0)
+            const float q0 = v[i] * rs;
+            q[i] = __fmaf_rn(__fmaf_rd(q0, ss, v[i]), rs, q0);
         }
-    } else {  // a given tensor scale far too small: everything that is not small is beyond 6
+    } else {
+        // 2^-k first, which changes no digits of what matters; a given tensor scale far too small leaves numbers that are all beyond 6
 #pragma unroll
-        for (int i = 0; i < 16; ++i) q[i] = fminf(fmaxf(v[i] * inv_tensor, -1e30f), 1e30f) * r;
+        for (int i = 0; i < 16; ++i) {
+            const float x = fminf(fmaxf(v[i] * tensor.down, -1e30f), 1e30f), q0 = x * r;
+            q[i] = __fmaf_rn(__fmaf_rd(q0, -s, x), r, q0);
+        }
     }
     codes = make_uint2(to_e2m1x8(q), to_e2m1x8(q + 8));
     return byte;

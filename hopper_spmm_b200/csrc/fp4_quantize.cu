@@ -142,7 +142,7 @@ B200_DEVICE int find_exponent(const float *partial, uint32_t n_partial, const fl
 // One unit of 16 neighbours of a row, `raw`, to codes and scales.  Four (nvfp4) or eight (mxfp4) lanes together hold the four scales that lie
 // in one word; all lanes of a warp take part.
 template <typename T, bool kMx>
-B200_DEVICE void quantize_unit(const Raw16<T> &raw, float inv_tensor, bool here, uint32_t row, uint32_t unit, const Dest &d) {
+B200_DEVICE void quantize_unit(const Raw16<T> &raw, const TensorScale &tensor, bool here, uint32_t row, uint32_t unit, const Dest &d) {
     constexpr uint32_t kLanes = kMx ? 8 : 4;
     const uint32_t lane = threadIdx.x & 31u;
     uint32_t top = raw.top(), byte;
@@ -160,7 +160,7 @@ B200_DEVICE void quantize_unit(const Raw16<T> &raw, float inv_tensor, bool here,
         byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 2);
         byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 4);
     } else {
-        byte = quantize_block_nv(v, top, inv_tensor, codes) << (lane & 3u) * 8u;
+        byte = quantize_block_nv(v, top, tensor, codes) << (lane & 3u) * 8u;
         byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 1);
         byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 2);
     }
@@ -168,8 +168,6 @@ B200_DEVICE void quantize_unit(const Raw16<T> &raw, float inv_tensor, bool here,
     if (unit * 8u < d.pitch) *reinterpret_cast<uint2 *>(d.values + (uint64_t)row * d.pitch + unit * 8u) = codes;
     if (lane % kLanes == 0) *reinterpret_cast<uint32_t *>(d.scales + scale_word(row, unit / kLanes, d.groups)) = byte;
 }
-
-B200_DEVICE float inverse_exp2(int k) { return k == 127 ? __uint_as_float(0x00400000u) : exp2_int(-k); }
 
 // Blocks along the rows of x, a unit a thread.  Rows end with units that hold nothing: the scales behind the last column, which the
 // products read, are zeros.  Bound: reading x once (after amax_kernel, which leaves its last rows in L2: they come first) and writing the
@@ -179,21 +177,15 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T *__rest
                                                                  const Dest d) {
     __shared__ uint32_t shared[kThreads / 32];
     ptx::wait_for_grids_before();
-    float inv_tensor = 1.f;
-    if constexpr (!kMx) {
-        const int k = find_exponent(partial, n_partial, given, shared);
-        if (blockIdx.x == 0 && threadIdx.x == 0) *d.tensor_scale = exp2_int(k);
-        inv_tensor = inverse_exp2(k);
-    } else if (blockIdx.x == 0 && threadIdx.x == 0) {
-        *d.tensor_scale = 1.f;
-    }
+    const TensorScale tensor(kMx ? 0 : find_exponent(partial, n_partial, given, shared));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *d.tensor_scale = tensor.up;
     for (Walk w(d.groups * (kMx ? 8u : 4u), (uint64_t)blockIdx.x * kThreads + threadIdx.x, (uint64_t)gridDim.x * kThreads);
          __any_sync(0xFFFFFFFFu, w.row < d.rows); w.next()) {
         const bool here = w.row < d.rows;
         const uint32_t col = w.unit * 16u, row = d.rows - 1u - w.row;
         Raw16<T> raw;
         raw.load(x + (int64_t)row * ldx + col, here && col < d.cols ? d.cols - col : 0u, true);
-        quantize_unit<T, kMx>(raw, inv_tensor, here, row, w.unit, d);
+        quantize_unit<T, kMx>(raw, tensor, here, row, w.unit, d);
     }
 }
 
@@ -220,9 +212,9 @@ __global__ void __launch_bounds__(kClusterThreads) quantize_cluster_kernel(const
     ptx::cluster_wait();
     m = 0;
     for (uint32_t i = 0; i < gridDim.x; ++i) m = max(m, all[i]);
-    const int k = tensor_exponent(__uint_as_float(m));
-    if (at == 0) *d.tensor_scale = exp2_int(k);
-    quantize_unit<T, false>(raw, inverse_exp2(k), here, row, unit, d);
+    const TensorScale tensor(tensor_exponent(__uint_as_float(m)));
+    if (at == 0) *d.tensor_scale = tensor.up;
+    quantize_unit<T, false>(raw, tensor, here, row, unit, d);
 }
 
 // Blocks along the columns of x (kCols: the 4-bit matrix is the transpose), along the rows, or both from one read; also rows that start on
@@ -243,17 +235,10 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T *__res
     __shared__ uint32_t shared[kThreads / 32];
     ptx::wait_for_grids_before();
     const uint32_t tid = threadIdx.x, lane = tid & 31u;
-    float inv_tensor = 1.f;
-    if constexpr (!kMx) {
-        const int k = find_exponent(partial, n_partial, given, shared);
-        inv_tensor = inverse_exp2(k);
-        if (blockIdx.x == 0 && tid == 0) {
-            if (kRows) *by_rows.tensor_scale = exp2_int(k);
-            if (kCols) *by_cols.tensor_scale = exp2_int(k);
-        }
-    } else if (blockIdx.x == 0 && tid == 0) {
-        if (kRows) *by_rows.tensor_scale = 1.f;
-        if (kCols) *by_cols.tensor_scale = 1.f;
+    const TensorScale tensor(kMx ? 0 : find_exponent(partial, n_partial, given, shared));
+    if (blockIdx.x == 0 && tid == 0) {
+        if (kRows) *by_rows.tensor_scale = tensor.up;
+        if (kCols) *by_cols.tensor_scale = tensor.up;
     }
     auto piece = [&](uint32_t r, uint32_t p) { return r * kVecs + (p ^ ((r >> 4 & 1u) * (kVecs / 2u))); };
     for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
@@ -298,7 +283,7 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T *__res
                     byte <<= (q >> 1) * 8u;
                     byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 2);
                 } else {
-                    byte = quantize_block_nv(v, top, inv_tensor, codes) << q * 8u;
+                    byte = quantize_block_nv(v, top, tensor, codes) << q * 8u;
                     byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 1);
                     byte |= __shfl_xor_sync(0xFFFFFFFFu, byte, 2);
                 }
@@ -341,7 +326,7 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T *__res
                     codes = make_uint2(to_e2m1x8(v[k]), to_e2m1x8(v[k] + 8));
                     if (lane < 16u) out_scale[(c + k) * 8u + b / 2u] = (uint8_t)byte;
                 } else {
-                    out_scale[(c + k) * 8u + b] = (uint8_t)quantize_block_nv(v[k], top[k], inv_tensor, codes);
+                    out_scale[(c + k) * 8u + b] = (uint8_t)quantize_block_nv(v[k], top[k], tensor, codes);
                 }
                 *reinterpret_cast<uint2 *>(out + (c + k) * kOutPitch + b * 8u) = codes;
             }
@@ -364,60 +349,55 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T *__res
 
 // A thread takes eight values, a word of codes, and writes them in one piece; where rows start anywhere, a warp's 256 values go through
 // shuffles and leave 32 neighbours at a time.  Bound: reading the matrix and writing x once.
-template <typename T, bool kMx>
+template <typename T, bool kMx, bool kWide>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t *__restrict__ values, const uint8_t *__restrict__ scales,
                                                               const float *__restrict__ tensor_scale, uint32_t rows, uint32_t cols, uint32_t pitch,
-                                                              uint32_t groups, T *__restrict__ x, int64_t ldx, bool wide) {
+                                                              uint32_t groups, T *__restrict__ x, int64_t ldx) {
     constexpr uint32_t kAhead = 4;
     ptx::wait_for_grids_before();
     const uint32_t lane = threadIdx.x & 31u;
     const float whole = kMx ? 1.f : *reinterpret_cast<const volatile float *>(tensor_scale);
     // a warp's unit: 256 columns of a row
     for (Walk w((cols + 255u) / 256u, ((uint64_t)blockIdx.x * kThreads + threadIdx.x) / 32u, (uint64_t)gridDim.x * (kThreads / 32u)); w.row < rows;) {
-        uint32_t codes[kAhead], row[kAhead], col[kAhead];
-        uint8_t bytes[kAhead];
+        uint32_t codes[kAhead], row[kAhead], col[kAhead], bytes[kAhead];
 #pragma unroll
         for (uint32_t a = 0; a < kAhead; ++a) {
             row[a] = w.row;
             col[a] = w.unit * 256u + lane * 8u;
-            const bool here = w.row < rows && col[a] < cols;
             const uint32_t block = col[a] / (kMx ? 32u : 16u);
-            codes[a] = here ? *reinterpret_cast<const uint32_t *>(values + (uint64_t)row[a] * pitch + col[a] / 2u) : 0u;
-            bytes[a] = here ? scales[scale_word(row[a], block / 4u, groups) + block % 4u] : (uint8_t)0u;
+            codes[a] = bytes[a] = 0u;
+            if (w.row < rows && col[a] < cols) {
+                codes[a] = __ldg(reinterpret_cast<const uint32_t *>(values + (uint64_t)row[a] * pitch + col[a] / 2u));
+                bytes[a] = __ldg(scales + scale_word(row[a], block / 4u, groups) + block % 4u);
+            }
             w.next();
         }
 #pragma unroll
         for (uint32_t a = 0; a < kAhead; ++a) {
+            if (row[a] >= rows) break;  // (the warp's)
             const float s = kMx ? from_e8m0(bytes[a]) : from_e4m3(bytes[a]);
-            const bool here = row[a] < rows;  // (the warp's)
             float v[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float2 two = __half22float2(from_e2m1x2(codes[a] >> i * 8));
-                v[2 * i] = two.x * s * whole;  // code times scale is exact: one rounding, and one to T
-                v[2 * i + 1] = two.y * s * whole;
+                v[2 * i] = kMx ? two.x * s : two.x * s * whole;  // code times scale is exact: one rounding, and one to T
+                v[2 * i + 1] = kMx ? two.y * s : two.y * s * whole;
             }
             T *dst = x + (int64_t)row[a] * ldx + col[a];
-            if (wide && here && col[a] + 8u <= cols) {
-                uint4 out[sizeof(T) / 2];
-                T *e = reinterpret_cast<T *>(out);
+            if constexpr (kWide) {
+                if (col[a] + 8u <= cols) {
+                    uint4 out[sizeof(T) / 2];
+                    T *e = reinterpret_cast<T *>(out);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = Elem<T>::from_float(v[i]);
-                if constexpr (sizeof(T) == 4) {
-                    if ((reinterpret_cast<uintptr_t>(dst) & 31u) == 0) {
-                        ptx::st_global_v8(dst, reinterpret_cast<const uint32_t *>(out));
-                    } else {
-                        reinterpret_cast<uint4 *>(dst)[0] = out[0];
-                        reinterpret_cast<uint4 *>(dst)[1] = out[1];
-                    }
+                    for (int i = 0; i < 8; ++i) e[i] = Elem<T>::from_float(v[i]);
+                    if constexpr (sizeof(T) == 4) ptx::st_global_v8(dst, reinterpret_cast<const uint32_t *>(out));
+                    else *reinterpret_cast<uint4 *>(dst) = out[0];
                 } else {
-                    *reinterpret_cast<uint4 *>(dst) = out[0];
-                }
-            } else if (wide) {
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i)
-                    if (here && col[a] + i < cols) dst[i] = Elem<T>::from_float(v[i]);
-            } else if (here) {
+                    for (uint32_t i = 0; i < 8; ++i)
+                        if (col[a] + i < cols) dst[i] = Elem<T>::from_float(v[i]);
+                }
+            } else {
                 const uint32_t first = col[a] - lane * 8u;
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) {  // value 32 i + lane of the warp's: lane 4 i + lane / 8 has it, as its value lane % 8
@@ -478,11 +458,12 @@ int quantize_typed(const T *x, int64_t ldx, uint32_t x_rows, uint32_t x_cols, co
 template <typename T>
 int dequantize_typed(const b200spmm_fp4_t *a, T *x, int64_t ldx, cudaStream_t stream) {
     const Dest d = dest_of(a);
-    const bool wide = reinterpret_cast<uintptr_t>(x) % 16u == 0 && ldx * (int64_t)sizeof(T) % 16 == 0;
-    const uint64_t units = (uint64_t)d.rows * ((d.cols + 255u) / 256u) * 8u;  // a warp's four at a time
-    auto kernel = a->format == B200SPMM_MXFP4 ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
-    B200_CUDA_TRY(launch_after(kernel, dim3(grid_for((units + kThreads - 1) / kThreads)), kThreads, 0, 1, stream, (const uint8_t *)d.values,
-                               (const uint8_t *)d.scales, (const float *)d.tensor_scale, d.rows, d.cols, d.pitch, d.groups, x, ldx, wide));
+    const bool wide = reinterpret_cast<uintptr_t>(x) % (8 * sizeof(T)) == 0 && ldx % 8 == 0, mx = a->format == B200SPMM_MXFP4;
+    const uint64_t warps = ((uint64_t)d.rows * ((d.cols + 255u) / 256u) + 3u) / 4u;  // with four units each
+    auto kernel = mx ? (wide ? dequantize_kernel<T, true, true> : dequantize_kernel<T, true, false>)
+                     : (wide ? dequantize_kernel<T, false, true> : dequantize_kernel<T, false, false>);
+    B200_CUDA_TRY(launch_after(kernel, dim3(grid_for((warps + kThreads / 32u - 1) / (kThreads / 32u))), kThreads, 0, 1, stream, (const uint8_t *)d.values,
+                               (const uint8_t *)d.scales, (const float *)d.tensor_scale, d.rows, d.cols, d.pitch, d.groups, x, ldx));
     return B200SPMM_OK;
 }
 
