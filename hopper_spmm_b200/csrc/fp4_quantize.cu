@@ -1,5 +1,6 @@
 // Dense matrices to 4 bits and back (layout: fp4.hpp).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 #include "fp4.hpp"
@@ -82,8 +83,19 @@ struct Raw16 {
             for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
             return m;
         } else {
+            if constexpr (std::is_same<T, __half>::value) {
+                const __half2 *h = reinterpret_cast<const __half2 *>(v);
+                __half2 most = __habs2(h[0]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+                for (int i = 1; i < 8; ++i) most = __hmax2_nan(most, __habs2(h[i]));
+                m = *reinterpret_cast<const uint32_t *>(&most);
+            } else {
+                const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(v);
+                __nv_bfloat162 most = __habs2(h[0]);
+#pragma unroll
+                for (int i = 1; i < 8; ++i) most = __hmax2_nan(most, __habs2(h[i]));
+                m = *reinterpret_cast<const uint32_t *>(&most);
+            }
             const uint16_t one = (uint16_t)max(m & 0xFFFFu, m >> 16);
             return __float_as_uint(Elem<T>::to_float(*reinterpret_cast<const T *>(&one)));
         }
@@ -225,7 +237,7 @@ __global__ void __launch_bounds__(kClusterThreads) quantize_cluster_kernel(const
 constexpr uint32_t kTileR = 128, kTileC = 64, kOutPitch = kTileR / 2 + 16;
 
 template <typename T, bool kMx, bool kRows, bool kCols>
-__global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T *__restrict__ x, int64_t ldx, uint32_t x_rows, uint32_t x_cols, bool wide,
+__global__ void __launch_bounds__(kThreads, 4) quantize_tiles_kernel(const T *__restrict__ x, int64_t ldx, uint32_t x_rows, uint32_t x_cols, bool wide,
                                                                   const float *partial, uint32_t n_partial, const float *given, const Dest by_rows,
                                                                   const Dest by_cols, uint32_t tiles_c, uint64_t tiles) {
     constexpr uint32_t kPer = 16 / sizeof(T), kVecs = kTileC / kPer;  // elements of a piece, pieces of a row
@@ -263,7 +275,7 @@ __global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const T *__res
         }
         __syncthreads();
         if constexpr (kRows) {
-#pragma unroll
+#pragma unroll 1
             for (uint32_t i = tid; i < kTileR * (kTileC / 16); i += kThreads) {
                 const uint32_t r = i / 4, q = i % 4, row = r0 + r, col = c0 + q * 16;
                 Raw16<T> raw;
