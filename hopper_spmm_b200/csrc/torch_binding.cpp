@@ -46,14 +46,14 @@ at::Tensor empty_direct(long, at::IntArrayRef, Type, at::Device) {
 // A new CUDA tensor.  Through the dispatcher it is 1.2 of the 4.1 us that a small product takes the host, directly 0.9.  The
 // dispatcher is left out only where nothing would happen in it but the allocation: no mode, tracer, transform or inference mode
 // (the thread's keys are the default ones), no profiler or other observer of calls, and no fill that deterministic runs ask for.
-at::Tensor new_cuda(int64_t rows, int64_t n, at::ScalarType type, const at::Tensor &like) {
+at::Tensor new_cuda(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor &like) {
     const c10::impl::LocalDispatchKeySet keys = c10::impl::tls_local_dispatch_key_set();
     if (keys.included_ == c10::default_included_set && keys.excluded_ == c10::default_excluded_set && !at::hasCallbacks() &&
         !at::globalContext().deterministicAlgorithms()) {
-        at::Tensor out = empty_direct(0, {rows, n}, type, like.device());
+        at::Tensor out = empty_direct(0, sizes, type, like.device());
         if (out.defined()) return out;
     }
-    return at::empty({rows, n}, like.options().dtype(type).requires_grad(false));
+    return at::empty(sizes, like.options().dtype(type).requires_grad(false));
 }
 
 // spmm(plan, is_f16, rows, cols, B, C or None, c_half, stream or None) -> C, or a status code that is not 0
@@ -89,7 +89,7 @@ PyObject *spmm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
         stream = PyLong_AsVoidPtr(args[7]);
         if (PyErr_Occurred()) return nullptr;
     }
-    if (args[5] == Py_None) C = new_cuda(rows, n, c_type, B);
+    if (args[5] == Py_None) C = new_cuda({rows, n}, c_type, B);
     if (args[7] == Py_None) stream = c10::cuda::getCurrentCUDAStream(B.get_device()).stream();
     const void *b = B.data_ptr();
     void *c = C.data_ptr();
@@ -151,51 +151,105 @@ bool matrix_of(PyObject *const *args, b200spmm_fp4_t *m) {
     return true;
 }
 
-// fp4_quantize(X, matrix or None, matrix or None, given scale or None) -> None or a status: X by rows and by columns
-PyObject *fp4_quantize(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
-    HANDLE_TH_ERRORS
-    if (n_args != 14) {
-        PyErr_SetString(PyExc_TypeError, "fp4_quantize takes 14 arguments");
-        return nullptr;
-    }
-    const char *bad_x = "X must be a two-dimensional CUDA tensor of float32, float16 or bfloat16 with unit stride along rows or columns";
-    const at::Tensor *X = cuda_tensor(args[0]);
-    Dense x;
-    if (!X || type_code(X->scalar_type()) < 0 || !dense_of(*X, &x)) return refuse(bad_x);
-    b200spmm_fp4_t by_rows{}, by_cols{};
-    const bool rows = args[1] != Py_None, cols = args[7] != Py_None;
-    if ((rows && !matrix_of(args + 1, &by_rows)) || (cols && !matrix_of(args + 7, &by_cols))) return refuse("the matrix must be on one CUDA device");
-    if (PyErr_Occurred()) return nullptr;
-    const b200spmm_fp4_t &one = rows ? by_rows : by_cols;
-    if (X->get_device() != one.device) return refuse("X and the matrix must be on the same device");
-    const uint64_t r = (uint64_t)X->size(0), c = (uint64_t)X->size(1);
-    if ((rows && (by_rows.rows != r || by_rows.cols != c)) || (cols && (by_cols.rows != c || by_cols.cols != r))) return refuse("the matrix does not have the shape of X");
-    const float *given = nullptr;
-    if (args[13] != Py_None) {
-        const at::Tensor *g = cuda_tensor(args[13]);
-        if (!g || g->scalar_type() != at::kFloat || g->numel() != 1 || g->get_device() != one.device)
-            return refuse("tensor_scale must be a float32 tensor of one element on X's device");
-        given = static_cast<const float *>(g->data_ptr());
-    }
+// What X is quantised into, filled in on `stream`; the status.
+int quantize_into(const at::Tensor &X, const Dense &x, const b200spmm_fp4_t *by_rows, const b200spmm_fp4_t *by_cols, const float *given) {
+    const b200spmm_fp4_t &one = by_rows ? *by_rows : *by_cols;
     at::Tensor workspace;
     if (one.format == B200SPMM_NVFP4 && !given) {
         uint64_t bytes = 0;
         b200spmm_fp4_sizes(0, 0, one.format, nullptr, nullptr, nullptr, &bytes);
-        workspace = new_cuda(1, (int64_t)bytes, at::kByte, *X);
+        workspace = new_cuda({(int64_t)bytes}, at::kByte, X);
     }
     void *ws = workspace.defined() ? workspace.data_ptr() : nullptr;
-    void *stream = c10::cuda::getCurrentCUDAStream(X->get_device()).stream();
-    const int code = type_code(X->scalar_type());
-    const b200spmm_fp4_t *first = x.transposed ? (cols ? &by_cols : nullptr) : (rows ? &by_rows : nullptr);   // along the rows as they lie
-    const b200spmm_fp4_t *second = x.transposed ? (rows ? &by_rows : nullptr) : (cols ? &by_cols : nullptr);  // ... across them
-    int st;
-    {
-        const ThreadsAllowed threads;
-        if (first && second) st = b200spmm_fp4_quantize_both(x.ptr, x.ld, code, given, first, second, ws, stream);
-        else st = b200spmm_fp4_quantize(x.ptr, x.ld, code, second != nullptr, given, first ? first : second, ws, stream);
+    void *stream = c10::cuda::getCurrentCUDAStream(X.get_device()).stream();
+    const int code = type_code(X.scalar_type());
+    const b200spmm_fp4_t *along = x.transposed ? by_cols : by_rows, *across = x.transposed ? by_rows : by_cols;  // the rows of X as they lie
+    const ThreadsAllowed threads;
+    if (along && across) return b200spmm_fp4_quantize_both(x.ptr, x.ld, code, given, along, across, ws, stream);
+    return b200spmm_fp4_quantize(x.ptr, x.ld, code, across != nullptr, given, along ? along : across, ws, stream);
+}
+
+// X and a given scale (or None) as arguments; false with an error set where they will not do.
+bool quantize_arguments(PyObject *const *args, const at::Tensor **X, Dense *x, const float **given) {
+    *X = cuda_tensor(args[0]);
+    if (!*X || type_code((*X)->scalar_type()) < 0 || !dense_of(**X, x)) {
+        refuse("X must be a two-dimensional CUDA tensor of float32, float16 or bfloat16 with unit stride along rows or columns");
+        return false;
     }
+    *given = nullptr;
+    if (args[1] != Py_None) {
+        const at::Tensor *g = cuda_tensor(args[1]);
+        if (!g || g->scalar_type() != at::kFloat || g->numel() != 1 || g->get_device() != (*X)->get_device()) {
+            refuse("tensor_scale must be a float32 tensor of one element on X's device");
+            return false;
+        }
+        *given = static_cast<const float *>(g->data_ptr());
+    }
+    return true;
+}
+
+// fp4_quantize(X, given scale or None, matrix, across) -> None or a status: into arrays that are there
+PyObject *fp4_quantize(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 9) {
+        PyErr_SetString(PyExc_TypeError, "fp4_quantize takes 9 arguments");
+        return nullptr;
+    }
+    const at::Tensor *X;
+    Dense x;
+    const float *given;
+    if (!quantize_arguments(args, &X, &x, &given)) return nullptr;
+    b200spmm_fp4_t m{};
+    const bool across = args[8] == Py_True;
+    if (!matrix_of(args + 2, &m) || X->get_device() != m.device) return refuse("X and the matrix must be on the same CUDA device");
+    if (PyErr_Occurred()) return nullptr;
+    if (m.rows != (uint64_t)X->size(across ? 1 : 0) || m.cols != (uint64_t)X->size(across ? 0 : 1)) return refuse("the matrix does not have the shape of X");
+    const int st = quantize_into(*X, x, across ? nullptr : &m, across ? &m : nullptr, given);
     if (st != B200SPMM_OK) return PyLong_FromLong(st);
     Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// fp4_quantize_new(X, given scale or None, format, by rows, by columns) -> values, scales, scale of either (one after the other), or a status
+PyObject *fp4_quantize_new(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 5) {
+        PyErr_SetString(PyExc_TypeError, "fp4_quantize_new takes 5 arguments");
+        return nullptr;
+    }
+    const at::Tensor *X;
+    Dense x;
+    const float *given;
+    if (!quantize_arguments(args, &X, &x, &given)) return nullptr;
+    const long format = PyLong_AsLong(args[2]);
+    if (PyErr_Occurred()) return nullptr;
+    const bool want[2] = {args[3] == Py_True, args[4] == Py_True};
+    at::Tensor made[2][3];
+    b200spmm_fp4_t m[2] = {};
+    for (int i = 0; i < 2; ++i) {
+        if (!want[i]) continue;
+        m[i].rows = (uint64_t)X->size(i);
+        m[i].cols = (uint64_t)X->size(1 - i);
+        m[i].format = (int32_t)format;
+        m[i].device = (int32_t)X->get_device();
+        uint64_t pitch = 0, scales = 0;
+        const int st = b200spmm_fp4_sizes(m[i].rows, m[i].cols, (int)format, &pitch, nullptr, &scales, nullptr);
+        if (st != B200SPMM_OK) return PyLong_FromLong(st);
+        made[i][0] = new_cuda({(int64_t)m[i].rows, (int64_t)pitch}, at::kByte, *X);
+        made[i][1] = new_cuda({(int64_t)scales}, at::kByte, *X);
+        made[i][2] = new_cuda({1}, at::kFloat, *X);
+        m[i].values = made[i][0].data_ptr();
+        m[i].scales = made[i][1].data_ptr();
+        m[i].tensor_scale = static_cast<float *>(made[i][2].data_ptr());
+    }
+    const int st = quantize_into(*X, x, want[0] ? &m[0] : nullptr, want[1] ? &m[1] : nullptr, given);
+    if (st != B200SPMM_OK) return PyLong_FromLong(st);
+    PyObject *out = PyTuple_New(want[0] && want[1] ? 6 : 3);
+    if (!out) return nullptr;
+    Py_ssize_t at = 0;
+    for (int i = 0; i < 2; ++i)
+        for (int j = 0; want[i] && j < 3; ++j) PyTuple_SET_ITEM(out, at++, THPVariable_Wrap(std::move(made[i][j])));
+    return out;
     END_HANDLE_TH_ERRORS
 }
 
@@ -203,7 +257,7 @@ PyObject *fp4_quantize(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
 bool output_of(PyObject *arg, int64_t rows, int64_t n, long type, const at::Tensor &like, at::Tensor *C, Dense *c) {
     const char *bad = "C has the wrong shape, dtype, device or layout";
     if (arg == Py_None) {
-        *C = new_cuda(rows, n, type_of(type), like);
+        *C = new_cuda({rows, n}, type_of(type), like);
     } else {
         const at::Tensor *t = cuda_tensor(arg);
         if (!t || t->scalar_type() != type_of(type) || t->dim() != 2 || t->size(0) != rows || t->size(1) != n || t->get_device() != like.get_device()) {
@@ -223,7 +277,7 @@ bool output_of(PyObject *arg, int64_t rows, int64_t n, long type, const at::Tens
 at::Tensor product_workspace(const b200spmm_fp4_t &a, int64_t n, const at::Tensor &like, uint64_t *bytes) {
     *bytes = 0;
     if (b200spmm_fp4_product_workspace(&a, n, bytes) != B200SPMM_OK || *bytes == 0) return at::Tensor();
-    return new_cuda(1, (int64_t)*bytes, at::kByte, like);
+    return new_cuda({(int64_t)*bytes}, at::kByte, like);
 }
 
 PyObject *result_of(int st, PyObject *arg, at::Tensor &&C) {
@@ -317,6 +371,7 @@ PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void 
 
 PyMethodDef methods[] = {{"spmm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(spmm)), METH_FASTCALL, nullptr},
                          {"fp4_quantize", fast<fp4_quantize>(), METH_FASTCALL, nullptr},
+                         {"fp4_quantize_new", fast<fp4_quantize_new>(), METH_FASTCALL, nullptr},
                          {"fp4_dequantize", fast<fp4_dequantize>(), METH_FASTCALL, nullptr},
                          {"fp4_product", fast<fp4_product>(), METH_FASTCALL, nullptr},
                          {"fp4_dense_product", fast<fp4_dense_product>(), METH_FASTCALL, nullptr},

@@ -37,11 +37,16 @@ def _lib():
     return _native
 
 
+_types = {}
+
+
 def _type_code(dtype):
-    import torch
+    if not _types:
+        import torch
+        _types.update({torch.float32: capi.T_F32, torch.float16: capi.T_F16, torch.bfloat16: capi.T_BF16})
     try:
-        return {torch.float32: capi.T_F32, torch.float16: capi.T_F16, torch.bfloat16: capi.T_BF16}[dtype]
-    except KeyError:
+        return _types[dtype]
+    except (KeyError, TypeError):
         raise TypeError("dtype must be float32, float16 or bfloat16") from None
 
 
@@ -103,12 +108,11 @@ class Fp4Matrix:
 
     def dequantize(self, out=None, dtype=None, stream=None):
         """The values it stands for, [rows, cols] in ``dtype`` (float32; with ``out``, its type)."""
-        import torch
-        dtype = (out.dtype if out is not None else torch.float32) if dtype is None else dtype
+        code = _type_code(dtype) if dtype is not None else _type_code(out.dtype) if out is not None else capi.T_F32
         if stream is not None:
             with _on(stream, self.values, self.scales, self.tensor_scale, out):
                 return self.dequantize(out, dtype)
-        out = _lib().fp4_dequantize(*self._m, out, _type_code(dtype))
+        out = _lib().fp4_dequantize(*self._m, out, code)
         if type(out) is int:
             raise capi.SpmmError(out, "b200spmm_fp4_dequantize")
         return out
@@ -117,8 +121,7 @@ class Fp4Matrix:
         """This matrix times B: a float16 or bfloat16 tensor [cols, n] (mxfp4: bfloat16), or an Fp4Matrix of n rows with
         blocks along the same columns, whose transpose is meant.  Returns C [rows, n] in ``dtype`` (float32; with
         ``C_out``, its type).  B and C may lie row by row or column by column (``x.t()``)."""
-        import torch
-        dtype = (C_out.dtype if C_out is not None else torch.float32) if dtype is None else dtype
+        code = _type_code(dtype) if dtype is not None else _type_code(C_out.dtype) if C_out is not None else capi.T_F32
         if stream is not None:
             mine = (self.values, self.scales, self.tensor_scale, C_out)
             with _on(stream, *mine, *((B.values, B.scales, B.tensor_scale) if isinstance(B, Fp4Matrix) else (B,))):
@@ -129,11 +132,11 @@ class Fp4Matrix:
         if isinstance(B, Fp4Matrix):
             if B.format != self.format:
                 raise ValueError("both matrices must have the same format")
-            C_out, where = _lib().fp4_product(*self._m, *B._m, C_out, _type_code(dtype)), "b200spmm_fp4_product"
+            C_out, where = _lib().fp4_product(*self._m, *B._m, C_out, code), "b200spmm_fp4_product"
         else:
-            if self.format == "mxfp4" and getattr(B, "dtype", None) == torch.float16:
+            if self.format == "mxfp4" and str(getattr(B, "dtype", None)) == "torch.float16":
                 raise ValueError("an mxfp4 matrix takes bfloat16: its scales go beyond the range of float16")
-            C_out, where = _lib().fp4_dense_product(*self._m, B, C_out, _type_code(dtype)), "b200spmm_fp4_dense_product"
+            C_out, where = _lib().fp4_dense_product(*self._m, B, C_out, code), "b200spmm_fp4_dense_product"
         if type(C_out) is int:
             raise capi.SpmmError(C_out, where)
         if sync:
@@ -147,38 +150,46 @@ class Fp4Matrix:
         capi.check(capi.lib().b200spmm_fp4_status(self.values.device.index, s), "b200spmm_fp4_status")
 
 
-_NONE = (None,) * 6
+def _matrix(rows, cols, format, values, scales, tensor_scale) -> Fp4Matrix:
+    """Arrays that were made for it (the checks of Fp4Matrix cost as much as a launch)."""
+    m = object.__new__(Fp4Matrix)
+    m.rows, m.cols, m.format = rows, cols, format
+    m.values, m.scales, m.tensor_scale = values, scales, tensor_scale
+    m._m = (values, scales, tensor_scale, rows, cols, FORMATS[format])
+    return m
 
 
-def _check_x(X, format):
-    if format not in FORMATS:
-        raise ValueError(f"format must be one of {', '.join(FORMATS)}")
-    if getattr(X, "ndim", 0) != 2 or not X.is_cuda:
-        raise ValueError("X must be a two-dimensional CUDA tensor of float32, float16 or bfloat16 with unit stride along rows or columns")
+def _format_code(format):
+    try:
+        return FORMATS[format]
+    except (KeyError, TypeError):
+        raise ValueError(f"format must be one of {', '.join(FORMATS)}") from None
 
 
-def _quantize(X, by_rows, by_cols, tensor_scale):
-    st = _lib().fp4_quantize(X, *(_NONE if by_rows is None else by_rows._m), *(_NONE if by_cols is None else by_cols._m), tensor_scale)
-    if st is not None:
-        raise capi.SpmmError(st, "b200spmm_fp4_quantize")
+def _quantized(X, format, tensor_scale, by_rows, by_cols):
+    made = _lib().fp4_quantize_new(X, tensor_scale, _format_code(format), by_rows, by_cols)
+    if type(made) is int:
+        raise capi.SpmmError(made, "b200spmm_fp4_quantize")
+    return made
 
 
 def fp4_quantize(X, format: str = "nvfp4", axis: int = 1, tensor_scale=None, out: Fp4Matrix | None = None, stream=None) -> Fp4Matrix:
     """X in 4 bits.  ``axis`` 1: blocks along X's rows, a matrix of X's shape; 0: along its columns, and the matrix is X's
     transpose (the axis that a product sums over has to be the matrix's rows).  ``tensor_scale``: for nvfp4, a float32 tensor of
     one element (say, calibrated) in place of a pass over X for its largest value.  ``out``: a matrix to fill, else a new one."""
-    _check_x(X, format)
     if axis not in (0, 1):
         raise ValueError("axis must be 0 or 1")
     if stream is not None:
         with _on(stream, X, tensor_scale, *(() if out is None else (out.values, out.scales, out.tensor_scale))):
             return fp4_quantize(X, format, axis, tensor_scale, out)
-    rows, cols = X.shape if axis else (X.shape[1], X.shape[0])
     if out is None:
-        out = Fp4Matrix(rows, cols, format, device=X.device)
-    elif out.format != format or (out.rows, out.cols) != (rows, cols):
-        raise ValueError(f"out must be a {rows} x {cols} matrix of {format}")
-    _quantize(X, out if axis else None, None if axis else out, tensor_scale)
+        made = _quantized(X, format, tensor_scale, axis == 1, axis == 0)
+        return _matrix(X.shape[1 - axis], X.shape[axis], format, *made)
+    if out.format != format:
+        raise ValueError(f"out must be a matrix of {format}")
+    st = _lib().fp4_quantize(X, tensor_scale, *out._m, axis == 0)
+    if st is not None:
+        raise capi.SpmmError(st, "b200spmm_fp4_quantize")
     return out
 
 
@@ -189,11 +200,9 @@ def fp4_quantize_both(X, format: str = "nvfp4", tensor_scale=None, stream=None) 
         X, Xt = fp4_quantize_both(x);  W, Wt = fp4_quantize_both(w);  dY, dYt = fp4_quantize_both(dy)
         y, dx, dw = X.matmul(W), dY.matmul(Wt), dYt.matmul(Xt)
     """
-    _check_x(X, format)
     if stream is not None:
         with _on(stream, X, tensor_scale):
             return fp4_quantize_both(X, format, tensor_scale)
+    made = _quantized(X, format, tensor_scale, True, True)
     r, c = X.shape
-    both = Fp4Matrix(r, c, format, device=X.device), Fp4Matrix(c, r, format, device=X.device)
-    _quantize(X, *both, tensor_scale)
-    return both
+    return _matrix(r, c, format, *made[:3]), _matrix(c, r, format, *made[3:])
