@@ -125,7 +125,7 @@ SIGNATURES = {
     "b200spmm_fp4_dequantize": (C.c_int, [C.POINTER(Fp4), vp, i64, C.c_int, vp]),
     "b200spmm_fp4_product": (C.c_int, [C.POINTER(Fp4), C.POINTER(Fp4), vp, i64, C.c_int, C.c_int, vp, u64, vp]),
     "b200spmm_fp4_dense_product": (C.c_int, [C.POINTER(Fp4), vp, i64, i64, C.c_int, C.c_int, vp, i64, C.c_int, C.c_int, vp, u64, vp]),
-    "b200spmm_fp4_product_workspace": (C.c_int, [C.POINTER(Fp4), i64, C.POINTER(u64)]),
+    "b200spmm_fp4_product_workspace": (C.c_int, [C.POINTER(Fp4), vp, i64, i64, C.c_int, C.POINTER(u64)]),
     "b200spmm_fp4_status": (C.c_int, [C.c_int, vp]),
     "b200spmm_kat_umma": (C.c_int, [vp, u32, C.POINTER(KatMma), C.c_int, C.c_int, vp, C.c_int]),
     "b200spmm_kat_umma_pair": (C.c_int, [vp, u32, C.POINTER(KatMma), C.c_int, C.c_int, vp, C.c_int]),

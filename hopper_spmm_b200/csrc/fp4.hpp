@@ -60,8 +60,8 @@ int launch_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *c, in
                    float *workspace, uint64_t workspace_bytes, cudaStream_t stream);
 int product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t *bytes);
 int launch_dense_product(const b200spmm_fp4_t *a, const void *b, int64_t ldb, int64_t n, int b_dtype, bool b_transposed, void *c,
-                         int64_t ldc, int c_dtype, bool c_transposed, float *workspace, uint64_t workspace_bytes, cudaStream_t stream);
-int dense_product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t *bytes);
+                         int64_t ldc, int c_dtype, bool c_transposed, uint8_t *workspace, uint64_t workspace_bytes, cudaStream_t stream);
+int dense_product_workspace(const b200spmm_fp4_t *a, const void *b, int64_t ldb, int64_t n, bool b_transposed, uint64_t *bytes);
 
 constexpr int kMaxDevices = 64;
 // The word in which kernels report a wait that ran out, on the current device.

@@ -157,19 +157,15 @@ int b200spmm_fp4_dequantize(const b200spmm_fp4_t *a, void *d_X, int64_t ldx, int
     return on_device(a->device, [&]() -> int { return is_empty(a) ? B200SPMM_OK : launch_dequantize(a, d_X, ldx, x_dtype, static_cast<cudaStream_t>(stream)); });
 }
 
-int b200spmm_fp4_product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t *bytes) {
+int b200spmm_fp4_product_workspace(const b200spmm_fp4_t *a, const void *d_B, int64_t ldb, int64_t n, int b_transposed, uint64_t *bytes) {
     if (!bytes || n < 0) return B200SPMM_ERR_INVALID_ARG;
     *bytes = 0;
     const int st = check_matrix(a);
     if (st != B200SPMM_OK) return st;
     if (n > 0x7FFFFFFF - 256) return B200SPMM_ERR_UNSUPPORTED;
-    return on_device(a->device, [&]() -> int { 
-        if (is_empty(a)) return B200SPMM_OK;
-        uint64_t four = 0, sixteen = 0;
-        int s = product_workspace(a, n, &four);
-        if (s == B200SPMM_OK) s = dense_product_workspace(a, n, &sixteen);
-        if (s == B200SPMM_OK) *bytes = four > sixteen ? four : sixteen;
-        return s;
+    return on_device(a->device, [&]() -> int {
+        if (is_empty(a) || n == 0) return B200SPMM_OK;
+        return d_B ? dense_product_workspace(a, d_B, ldb, n, b_transposed != 0, bytes) : product_workspace(a, n, bytes);
     });
 }
 
@@ -179,7 +175,7 @@ int b200spmm_fp4_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void 
     if (st == B200SPMM_OK) st = check_matrix(b);
     if (st != B200SPMM_OK) return st;
     if (a->cols != b->cols || a->device != b->device) return B200SPMM_ERR_INVALID_ARG;
-    if (!aligned(workspace, 4)) return B200SPMM_ERR_INVALID_ARG;
+    if (!aligned(workspace, 16)) return B200SPMM_ERR_INVALID_ARG;
     if (a->format != b->format) return B200SPMM_ERR_UNSUPPORTED;
     const uint64_t rows = c_transposed ? b->rows : a->rows, cols = c_transposed ? a->rows : b->rows;
     st = check_dense(d_C, c_dtype, rows, cols, ldc);
@@ -200,7 +196,7 @@ int b200spmm_fp4_dense_product(const b200spmm_fp4_t *a, const void *d_B, int64_t
     if (n > 0x7FFFFFFF - 256) return B200SPMM_ERR_UNSUPPORTED;
     st = check_dense(d_B, b_dtype, b_transposed ? (uint64_t)n : a->cols, b_transposed ? a->cols : (uint64_t)n, ldb);
     if (st != B200SPMM_OK) return st;
-    if (!aligned(workspace, 4)) return B200SPMM_ERR_INVALID_ARG;
+    if (!aligned(workspace, 16)) return B200SPMM_ERR_INVALID_ARG;
     if (b_dtype == B200SPMM_T_F32 || (a->format == B200SPMM_MXFP4 && b_dtype != B200SPMM_T_BF16)) return B200SPMM_ERR_UNSUPPORTED;
     const uint64_t rows = c_transposed ? (uint64_t)n : a->rows, cols = c_transposed ? a->rows : (uint64_t)n;
     st = check_dense(d_C, c_dtype, rows, cols, ldc);
@@ -209,7 +205,7 @@ int b200spmm_fp4_dense_product(const b200spmm_fp4_t *a, const void *d_B, int64_t
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
         if (rows == 0 || cols == 0) return B200SPMM_OK;
         if (a->cols == 0) return zero_output(d_C, ldc, c_dtype, rows, cols, s);
-        return launch_dense_product(a, d_B, ldb, n, b_dtype, b_transposed != 0, d_C, ldc, c_dtype, c_transposed != 0, static_cast<float *>(workspace), workspace_bytes, s);
+        return launch_dense_product(a, d_B, ldb, n, b_dtype, b_transposed != 0, d_C, ldc, c_dtype, c_transposed != 0, static_cast<uint8_t *>(workspace), workspace_bytes, s);
     });
 }
 

@@ -56,7 +56,7 @@ int launch_narrow_columns(const b200spmm_fp4_t *a, const DenseParams &d, cudaStr
 // sums' way through memory.
 Split wide_split(uint32_t m, uint32_t n, uint32_t k, uint32_t pairs) {
     const uint32_t tiles_n = (n + kPairCols4 - 1) / kPairCols4, cols = ((n + tiles_n - 1) / tiles_n + 31u) / 32u * 32u;
-    return make_split(m, n, cols, (k + kWideK - 1) / kWideK, 4, pairs);
+    return make_split(m, n, cols, (k + kWideK - 1) / kWideK, 4, 0.55, 256 * kWideK * 2, pairs);
 }
 
 // Pairs of CTAs of the wide kernel that the current device runs at once (its instances take the same room).
@@ -81,6 +81,7 @@ int launch_wide(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace,
     prm.split = wide_split(d.m, d.n, d.k, pairs);
     if (prm.split.parts > 1 && (!workspace || workspace_bytes < split_workspace(prm.split))) prm.split = wide_split(d.m, d.n, d.k, 1);
     prm.row_blocks = (d.m + 127u) / 128u;
+    prm.stages = WideCfg::stages(kTokens, prm.split.cols);
     prm.partial = workspace;
     B200_CUDA_TRY(status_word(&prm.status));
     prm.wait_limit_ns = kDeviceWaitLimitNs;
@@ -93,35 +94,62 @@ int launch_wide(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace,
         set_last_error_static("a tensor map of a product with a 4-bit matrix could not be made");
         return B200SPMM_ERR_CUDA;
     }
-    B200_CUDA_TRY(launch_after(kernel, dim3(2 * std::min(pairs, prm.split.items)), WideCfg::kThreads, WideCfg::kSmemBytes, 2, stream, ma, mb, prm));
+    B200_CUDA_TRY(launch_after(kernel, dim3(2 * std::min(pairs, prm.split.items)), WideCfg::kThreads, WideCfg::smem_bytes(kTokens, prm.split.cols), 2, stream, ma, mb, prm));
     if (prm.split.parts > 1)
         B200_CUDA_TRY(launch_after(fp4_join_kernel, dim3((prm.split.items - prm.split.whole) / prm.split.parts, prm.split.cols / 32u), kPairRows4, 0, 1, stream, prm.split,
                                    (const float *)workspace, d.m, d.n, kMx ? (const float *)nullptr : d.whole, (const float *)nullptr, Widen<T, kMx>::kLeft, d.c));
     return B200SPMM_OK;
 }
 
-// Up to 16 columns, and operands that no tensor map describes.
-bool is_narrow(const DenseParams &d) { return d.n <= 16 || !d.b_wide; }
+// B, whose rows start anywhere, with rows that start on 16 bytes.
+__global__ void __launch_bounds__(256) fp4_align_kernel(const uint16_t *__restrict__ src, int64_t ld, uint32_t rows, uint32_t cols, uint4 *__restrict__ dst, uint32_t pieces) {
+    ptx::wait_for_grids_before();
+    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < (uint64_t)rows * pieces; i += (uint64_t)gridDim.x * 256u) {
+        const uint32_t row = (uint32_t)(i / pieces), col = (uint32_t)(i % pieces) * 8u;
+        const uint16_t *from = src + (int64_t)row * ld + col;
+        uint16_t v[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) v[e] = col + e < cols ? from[e] : (uint16_t)0;
+        dst[i] = *reinterpret_cast<const uint4 *>(v);
+    }
+}
+
+// Up to 16 columns go to the narrow kernel, which reads any B.
+constexpr uint32_t kNarrowColumns = 16;
+bool is_aligned(const void *b, int64_t ldb) { return reinterpret_cast<uintptr_t>(b) % 16u == 0 && ldb % 8 == 0; }
+uint64_t aligned_bytes(uint64_t rows, uint64_t cols) { return rows * ((cols + 7u) / 8u) * 16u; }
 
 template <typename T, bool kMx, bool kTokens>
-int launch_dense(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
-    return is_narrow(d) ? launch_narrow_columns<T, kMx, kTokens>(a, d, stream) : launch_wide<T, kMx, kTokens>(a, d, workspace, workspace_bytes, stream);
+int launch_dense(const b200spmm_fp4_t *a, const DenseParams &d, uint8_t *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
+    const uint64_t rows = kTokens ? d.n : d.k, cols = kTokens ? d.k : d.n, need = aligned_bytes(rows, cols);
+    if (d.n <= kNarrowColumns || (!d.b_wide && (!workspace || workspace_bytes < need))) return launch_narrow_columns<T, kMx, kTokens>(a, d, stream);
+    if (d.b_wide) return launch_wide<T, kMx, kTokens>(a, d, reinterpret_cast<float *>(workspace), workspace_bytes, stream);
+    // no tensor map describes B: a copy that one does goes first into the workspace
+    const uint32_t pieces = (uint32_t)((cols + 7u) / 8u);
+    B200_CUDA_TRY(launch_after(fp4_align_kernel, dim3((unsigned)std::min<uint64_t>((rows * pieces + 255u) / 256u, (uint64_t)sm_count() * 8u)), 256, 0, 1, stream,
+                               reinterpret_cast<const uint16_t *>(d.b), d.ldb, (uint32_t)rows, (uint32_t)cols, reinterpret_cast<uint4 *>(workspace), pieces));
+    DenseParams with = d;
+    with.b = workspace;
+    with.ldb = (int64_t)pieces * 8;
+    with.b_wide = true;
+    return launch_wide<T, kMx, kTokens>(a, with, reinterpret_cast<float *>(workspace + need), workspace_bytes - need, stream);
 }
 
 }  // namespace
 
-int dense_product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t *bytes) {
+int dense_product_workspace(const b200spmm_fp4_t *a, const void *b, int64_t ldb, int64_t n, bool b_transposed, uint64_t *bytes) {
     *bytes = 0;
-    if (n <= 16) return B200SPMM_OK;
+    if (n <= kNarrowColumns) return B200SPMM_OK;
     uint32_t pairs = 0;
     const int st = wide_pairs(a->device, &pairs);
     if (st != B200SPMM_OK) return st;
     *bytes = split_workspace(wide_split((uint32_t)a->rows, (uint32_t)n, (uint32_t)a->cols, pairs));
+    if (!is_aligned(b, ldb)) *bytes += aligned_bytes(b_transposed ? (uint64_t)n : a->cols, b_transposed ? a->cols : (uint64_t)n);
     return B200SPMM_OK;
 }
 
 int launch_dense_product(const b200spmm_fp4_t *a, const void *b, int64_t ldb, int64_t n, int b_dtype, bool b_transposed, void *c, int64_t ldc, int c_dtype,
-                         bool c_transposed, float *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
+                         bool c_transposed, uint8_t *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
     const Layout l = layout_of(a->rows, a->cols, a->format);
     DenseParams prm{};
     prm.values = static_cast<const uint8_t *>(a->values);
@@ -134,7 +162,7 @@ int launch_dense_product(const b200spmm_fp4_t *a, const void *b, int64_t ldb, in
     prm.b = static_cast<const uint8_t *>(b);
     prm.ldb = ldb;
     prm.n = (uint32_t)n;
-    prm.b_wide = reinterpret_cast<uintptr_t>(b) % 16u == 0 && ldb % 8 == 0;
+    prm.b_wide = is_aligned(b, ldb);
     prm.c = target_of(c, ldc, c_dtype, c_transposed);
     if (n == 1 && !b_transposed && ldb == 1) {  // one column, contiguous
         b_transposed = true;

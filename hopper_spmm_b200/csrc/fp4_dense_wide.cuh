@@ -29,22 +29,35 @@ namespace fp4 {
 constexpr uint32_t kWideK = 128;  // of a step
 
 struct WideCfg {
-    static constexpr uint32_t kBytesA = 128 * kWideK / 2, kBytesScales = 1024, kBoxBytes = 64 * 2 * 128, kBytesB = 2 * kBoxBytes;
-    static constexpr uint32_t kStageBytes = kBytesA + kBytesScales + kBytesB, kStages = 5;
+    static constexpr uint32_t kBytesA = 128 * kWideK / 2, kBytesScales = 1024;
+    static constexpr uint32_t kMinStages = 5, kMaxStages = 12;
     static constexpr uint32_t kBuffers = 4, kBufferCols = kWideK / 2;  // of widened A, in tensor memory behind the accumulator
     static constexpr uint32_t kWideners = 16;
     static_assert(kBuffers == kWideners / 4, "a group of four warps has a buffer of its own");
     static constexpr int kWarps = kWideners + 3, kThreads = 32 * kWarps;
     static constexpr uint32_t kTmemCols = 512;
-    static constexpr uint32_t kBarriers = 2 * kStages + kBuffers + 3;
-    static constexpr size_t kSmemBytes = 1024 + (size_t)kStages * kStageBytes + kBarriers * 8 + 16;
-    static_assert(kPairCols4 + kBuffers * kBufferCols <= kTmemCols && kSmemBytes <= 227 * 1024, "memory of an SM");
+    static constexpr uint32_t kBarriers = 2 * kMaxStages + kBuffers + 3;
+    static constexpr uint32_t kOtherBytes = 1024 + kBarriers * 8 + 16;
+    static constexpr size_t kSmemBytes = 227 * 1024;  // at most
+    static_assert(kPairCols4 + kBuffers * kBufferCols <= kTmemCols, "tensor memory of an SM");
+    // A box of B, 128 bytes wide, and the boxes of a stage: [n][k] two of 64 values of k for each of a CTA's columns, [k][n] 64 columns each.
+    __host__ __device__ static constexpr uint32_t box_bytes(bool tokens, uint32_t cols) { return tokens ? cols / 2u * 128u : kWideK * 128u; }
+    __host__ __device__ static constexpr uint32_t boxes(bool tokens, uint32_t cols) { return tokens ? 2u : (cols / 2u + 63u) / 64u; }
+    __host__ __device__ static constexpr uint32_t b_bytes(bool tokens, uint32_t cols) { return box_bytes(tokens, cols) * boxes(tokens, cols); }
+    // Few columns leave room for more stages: A is what they have to bring.
+    static uint32_t stages(bool tokens, uint32_t cols) {
+        const uint32_t stage = kBytesA + kBytesScales + b_bytes(tokens, cols);
+        return std::min<uint32_t>(kMaxStages, ((uint32_t)kSmemBytes - kOtherBytes) / stage);
+    }
+    static size_t smem_bytes(bool tokens, uint32_t cols) { return kOtherBytes + (size_t)stages(tokens, cols) * (kBytesA + kBytesScales + b_bytes(tokens, cols)); }
 };
+static_assert((WideCfg::kSmemBytes - WideCfg::kOtherBytes) / (WideCfg::kBytesA + WideCfg::kBytesScales + WideCfg::b_bytes(false, 256)) >= WideCfg::kMinStages, "shared memory");
 
 struct WideParams {
     DenseParams d;
     Split split;
     uint32_t row_blocks;
+    uint32_t stages;
     float *partial;
     uint32_t *status;
     unsigned long long wait_limit_ns;
@@ -55,19 +68,19 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
 fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const WideParams p) {
     using Cfg = WideCfg;
     using W = Widen<T, kMx>;
-    constexpr uint32_t kStages = Cfg::kStages;
+    const uint32_t stages = p.stages, box_bytes = Cfg::box_bytes(kTokens, p.split.cols), boxes = Cfg::boxes(kTokens, p.split.cols), bytes_b = box_bytes * boxes;
     extern __shared__ uint8_t smem_raw[];
     // the same offsets in both CTAs: descriptors and multicast commits rely on it
     const uint32_t raw_addr = ptx::smem_u32(smem_raw);
     const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
     uint8_t *base = smem_raw + pad;
-    const uint32_t b_addr = raw_addr + pad, a_addr = b_addr + kStages * Cfg::kBytesB, s_addr = a_addr + kStages * Cfg::kBytesA;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(base + (size_t)kStages * Cfg::kStageBytes);
+    const uint32_t b_addr = raw_addr + pad, a_addr = b_addr + stages * bytes_b, s_addr = a_addr + stages * Cfg::kBytesA;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(base + (size_t)stages * (bytes_b + Cfg::kBytesA + Cfg::kBytesScales));
     const uint32_t bars_addr = ptx::smem_u32(bars);
     auto full_bar = [&](uint32_t s) { return bars_addr + 8u * s; };
-    auto empty_bar = [&](uint32_t s) { return bars_addr + 8u * (kStages + s); };
-    auto ready_bar = [&](uint32_t b) { return bars_addr + 8u * (2 * kStages + b); };
-    const uint32_t done_bar = bars_addr + 8u * (2 * kStages + Cfg::kBuffers), taken_bar = done_bar + 8u, drain_bar = done_bar + 16u;
+    auto empty_bar = [&](uint32_t s) { return bars_addr + 8u * (Cfg::kMaxStages + s); };
+    auto ready_bar = [&](uint32_t b) { return bars_addr + 8u * (2 * Cfg::kMaxStages + b); };
+    const uint32_t done_bar = bars_addr + 8u * (2 * Cfg::kMaxStages + Cfg::kBuffers), taken_bar = done_bar + 8u, drain_bar = done_bar + 16u;
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(bars + Cfg::kBarriers);
     uint32_t *tmem_slot = const_cast<uint32_t *>(abort_flag) + 1;
 
@@ -77,7 +90,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     const uint32_t cols_half = p.split.cols / 2u;  // of B, this CTA's
 
     if (tid == 0) {
-        for (uint32_t s = 0; s < kStages; ++s) {
+        for (uint32_t s = 0; s < stages; ++s) {
             ptx::mbar_init(full_bar(s), 2);
             ptx::mbar_init(empty_bar(s), 1);
         }
@@ -108,7 +121,6 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const uint32_t on = lane == 0 ? 1u : 0u;
         const bool is_a = warp == Cfg::kWideners + 1;
         constexpr uint32_t kGroups = kMx ? 1 : 2;
-        const uint32_t boxes = kTokens ? 2u : (cols_half + 63u) / 64u, box_bytes = kTokens ? cols_half * 128u : Cfg::kBoxBytes;
         uint32_t s = 0, phase = 1;
         bool alive = true;
         for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs) {
@@ -130,11 +142,11 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 #pragma unroll
                     for (uint32_t i = 0; i < 2; ++i) {
                         const uint32_t there = on & (i < boxes ? 1u : 0u);
-                        if constexpr (kTokens) ptx::tma_load_2d_if(there, b_addr + s * Cfg::kBytesB + i * Cfg::kBoxBytes, &tmap_b, (int32_t)(step * kWideK + i * 64u), (int32_t)n0, full_bar(s));
-                        else ptx::tma_load_2d_if(there, b_addr + s * Cfg::kBytesB + i * Cfg::kBoxBytes, &tmap_b, (int32_t)(n0 + i * 64u), (int32_t)(step * kWideK), full_bar(s));
+                        if constexpr (kTokens) ptx::tma_load_2d_if(there, b_addr + s * bytes_b + i * box_bytes, &tmap_b, (int32_t)(step * kWideK + i * 64u), (int32_t)n0, full_bar(s));
+                        else ptx::tma_load_2d_if(there, b_addr + s * bytes_b + i * box_bytes, &tmap_b, (int32_t)(n0 + i * 64u), (int32_t)(step * kWideK), full_bar(s));
                     }
                 }
-                s = s + 1 == kStages ? 0u : s + 1;
+                s = s + 1 == stages ? 0u : s + 1;
                 phase ^= s == 0 ? 1u : 0u;
             }
         }
@@ -146,7 +158,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             const uint32_t idesc = ptx::make_instr_desc(fmt, kPairRows4, p.split.cols, false, !kTokens);
             // B [n][k]: 64 values of k a row of the swizzle, eight rows 1024 bytes.  [k][n]: 64 columns a row, eight k 1024 bytes, the next 64
             // columns a box away.
-            const uint64_t b_desc = ptx::make_smem_desc(b_addr, kTokens ? 16u : Cfg::kBoxBytes, 1024, ptx::kSwizzle128B);
+            const uint64_t b_desc = ptx::make_smem_desc(b_addr, kTokens ? 16u : box_bytes, 1024, ptx::kSwizzle128B);
             const uint32_t b_lo = (uint32_t)b_desc, b_hi = (uint32_t)(b_desc >> 32);
             uint32_t s = 0, buffer = 0, phase = 0, round = 0;
             bool alive = true;
@@ -158,15 +170,15 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait_cluster(ready_bar(buffer), phase, abort_flag, limit));
                     if (!alive) break;
                     ptx::tcgen05_fence_after_sync();
-                    const uint32_t a = tmem + kPairCols4 + buffer * Cfg::kBufferCols, b = b_lo + s * (Cfg::kBytesB >> 4);
+                    const uint32_t a = tmem + kPairCols4 + buffer * Cfg::kBufferCols, b = b_lo + s * (bytes_b >> 4);
 #pragma unroll
                     for (uint32_t i = 0; i < kWideK / 16u; ++i)
-                        ptx::umma_pair_f16_ts_if(on & (left > i * 16u ? 1u : 0u), tmem, a + i * 8u, b + ((kTokens ? i / 4u * Cfg::kBoxBytes + i % 4u * 32u : i * 2048u) >> 4), b_hi, idesc,
+                        ptx::umma_pair_f16_ts_if(on & (left > i * 16u ? 1u : 0u), tmem, a + i * 8u, b + ((kTokens ? i / 4u * box_bytes + i % 4u * 32u : i * 2048u) >> 4), b_hi, idesc,
                                                  i ? 1u : accumulate);
                     ptx::umma_commit_pair_if(on, empty_bar(s));
                     accumulate = 1;
                     left -= kWideK;
-                    s = s + 1 == kStages ? 0u : s + 1;
+                    s = s + 1 == stages ? 0u : s + 1;
                     buffer = buffer + 1 == Cfg::kBuffers ? 0u : buffer + 1;
                     phase ^= buffer == 0 ? 1u : 0u;
                 }
@@ -185,8 +197,10 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const uint32_t ready = rank == 0 ? ready_bar(mine) : ptx::map_to_cta(ready_bar(mine), 0);
         const uint32_t taken = rank == 0 ? taken_bar : ptx::map_to_cta(taken_bar, 0);
         const uint32_t buffer = tmem + lanes + kPairCols4 + mine * Cfg::kBufferCols;
-        uint32_t it = 0, round = 0;
-        bool alive = true;
+        // its next step: stage and phase, and whether there was one before, whose MMAs have to leave the buffer
+        uint32_t s = mine, phase = 0, before_s = 0, before_phase = 0, round = 0, skip = mine;
+        while (s >= stages) s -= stages;  // (there are more stages than groups)
+        bool alive = true, again = false;
         auto wait = [&](uint32_t bar, uint32_t parity) {
             uint32_t ok = 1;
             if (lane == 0) ok = ptx::mbar_wait(bar, parity, abort_flag, limit) ? 1u : 0u;
@@ -194,10 +208,9 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         };
         for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs, ++round) {
             const Item w = split_item(p.split, item);
-            const uint32_t skip = (mine - it) % Cfg::kBuffers;  // steps until this warp's first one
-            for (uint32_t step = w.first + skip; step < w.last; step += Cfg::kBuffers) {
-                const uint32_t now = it + (step - w.first), s = now % kStages;
-                alive = wait(full_bar(s), now / kStages & 1u);
+            uint32_t step = w.first + skip;
+            for (; step < w.last; step += Cfg::kBuffers) {
+                alive = wait(full_bar(s), phase);
                 if (!alive) break;
                 // the row's 64 bytes, pieces of 16 in the order of the 64-byte swizzle, and its words of scales
                 const uint32_t src = a_addr + s * Cfg::kBytesA + row * 64u, turn = row >> 1 & 3u;
@@ -211,9 +224,8 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                         four[g] = ptx::ld_shared_u32(s_addr + s * Cfg::kBytesScales + g * 512u + lane * 16u + q * 4u);
                 const bool two = W::needs_two(four[0]) || W::needs_two(four[1]);
                 const bool any_two = kMx && __any_sync(0xFFFFFFFFu, two);
-                if (now >= Cfg::kBuffers) {
-                    const uint32_t old = now - Cfg::kBuffers;
-                    alive = wait(empty_bar(old % kStages), old / kStages & 1u);
+                if (again) {
+                    alive = wait(empty_bar(before_s), before_phase);
                     if (!alive) break;
                 }
                 ptx::tcgen05_fence_after_sync();
@@ -242,35 +254,73 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     if (rank == 0) ptx::mbar_arrive(ready);
                     else ptx::mbar_arrive_cluster_relaxed(ready);
                 }
+                again = true;
+                before_s = s;
+                before_phase = phase;
+                s += Cfg::kBuffers;
+                if (s >= stages) {
+                    s -= stages;
+                    phase ^= 1u;
+                }
             }
             if (!alive) break;
-            it += w.last - w.first;
+            skip = step - w.last;  // steps of the next item until this warp's
             alive = wait(done_bar, round & 1u);
             if (!alive) break;
             ptx::tcgen05_fence_after_sync();
             const uint32_t c_row = w.m0 + rank * 128u + row;
-#pragma unroll 1
-            for (uint32_t c = mine * 32u; c < p.split.cols; c += 128u) {
-                uint32_t r[32];
-                ptx::tmem_ld_32x32b_x32(tmem + lanes + c, r);
+            auto free_accumulator = [&]() {
+                ptx::tcgen05_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if (rank == 0) ptx::mbar_arrive(taken);
+                    else ptx::mbar_arrive_cluster_relaxed(taken);
+                }
+            };
+            auto scaled = [&](uint32_t c, float (&v)[16]) {
+                uint32_t r[16];
+                ptx::tmem_ld_32x32b_x16(tmem + lanes + c, r);
                 ptx::tmem_ld_wait();
+#pragma unroll
+                for (uint32_t i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) * W::kLeft * whole;
+            };
+            if (w.slot == ~0u && p.d.c.type != B200SPMM_T_F32) {
+                // the accumulator as 16-bit numbers to registers first: the next item's MMAs run while they are written
+                uint32_t packed[2][16];
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const uint32_t c = mine * 32u + j / 2u * 128u;
+                    if (c >= p.split.cols) break;
+                    float v[16];
+                    scaled(c + j % 2u * 16u, v);
+                    pack_row(p.d.c.type, v, packed[j / 2u] + j % 2u * 8u);
+                }
+                free_accumulator();
+#pragma unroll
+                for (uint32_t j = 0; j < 2; ++j) {
+                    const uint32_t c = mine * 32u + j * 128u;
+                    if (c < p.split.cols && c_row < p.d.m && w.n0 + c < p.d.n) store_packed_row(p.d.c, c_row, w.n0 + c, p.d.n, packed[j]);
+                }
+                continue;
+            }
+#pragma unroll 1
+            for (uint32_t j = 0; j < 4; ++j) {
+                const uint32_t c = mine * 32u + j / 2u * 128u + j % 2u * 16u;
+                if (c >= p.split.cols) break;
                 if (w.slot != ~0u) {  // column by column: neighbouring lanes write neighbours
+                    uint32_t r[16];
+                    ptx::tmem_ld_32x32b_x16(tmem + lanes + c, r);
+                    ptx::tmem_ld_wait();
                     float *dst = p.partial + ((uint64_t)w.slot * p.split.cols + c) * kPairRows4 + rank * 128u + row;
 #pragma unroll
-                    for (uint32_t i = 0; i < 32; ++i) dst[i * kPairRows4] = __uint_as_float(r[i]);
-                } else if (c_row < p.d.m && w.n0 + c < p.d.n) {
-                    float v[32];
-#pragma unroll
-                    for (uint32_t i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * W::kLeft * whole;
-                    store_row(p.d.c, c_row, w.n0 + c, p.d.n, v);
+                    for (uint32_t i = 0; i < 16; ++i) dst[i * kPairRows4] = __uint_as_float(r[i]);
+                } else {
+                    float v[16];
+                    scaled(c, v);
+                    if (c_row < p.d.m && w.n0 + c < p.d.n) store_row(p.d.c, c_row, w.n0 + c, p.d.n, v);
                 }
             }
-            ptx::tcgen05_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                if (rank == 0) ptx::mbar_arrive(taken);
-                else ptx::mbar_arrive_cluster_relaxed(taken);
-            }
+            free_accumulator();
         }
     }
     __syncwarp();

@@ -215,7 +215,7 @@ int launch_width(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, const Product
 // Tiles of 128 or 256 columns, the scales' blocks being 128 rows long, with fewer columns past the end; a single tile as wide as it has to be.
 Split pair_split(uint32_t m, uint32_t n, uint32_t k, uint32_t pairs) {
     const uint32_t cols = n <= kPairCols4 ? (n + 31u) / 32u * 32u : (n + 127u) / 128u * 128u < (n + 255u) / 256u * 256u ? 128u : 256u;
-    return make_split(m, n, cols, (k + kStageK - 1) / kStageK, 2, pairs);
+    return make_split(m, n, cols, (k + kStageK - 1) / kStageK, 2, 0.45, 256 * kStageK * 9 / 16, pairs);
 }
 
 int product_pairs(int device, uint32_t *out) {

@@ -225,6 +225,40 @@ fp4_product_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
             if (!__shfl_sync(0xFFFFFFFFu, ok, 0)) break;
             ptx::tcgen05_fence_after_sync();
             const uint32_t c_row = w.m0 + rank * 128u + row;
+            auto free_accumulator = [&]() {
+                ptx::tcgen05_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if (rank == 0) ptx::mbar_arrive(taken);
+                    else ptx::mbar_arrive_cluster_relaxed(taken);
+                }
+            };
+            if (w.slot == ~0u && p.c.type != B200SPMM_T_F32) {
+                // the accumulator as 16-bit numbers to registers first: the next item's MMAs run while they are written
+                uint32_t packed[4][16];
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const uint32_t c = half * 32u + j * 64u;
+                    if (c >= p.split.cols) break;
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h) {
+                        uint32_t r[16];
+                        ptx::tmem_ld_32x32b_x16(tmem + lanes + c + h * 16u, r);
+                        ptx::tmem_ld_wait();
+                        float v[16];
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i) v[i] = f.apply(__uint_as_float(r[i]));
+                        pack_row(p.c.type, v, packed[j] + h * 8u);
+                    }
+                }
+                free_accumulator();
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const uint32_t c = half * 32u + j * 64u;
+                    if (c < p.split.cols && c_row < p.m && w.n0 + c < p.n) store_packed_row(p.c, c_row, w.n0 + c, p.n, packed[j]);
+                }
+                continue;
+            }
 #pragma unroll 1
             for (uint32_t c = half * 32u; c < p.split.cols; c += 64u) {
                 uint32_t r[32];
@@ -241,12 +275,7 @@ fp4_product_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                     store_row(p.c, c_row, w.n0 + c, p.n, v);
                 }
             }
-            ptx::tcgen05_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                if (rank == 0) ptx::mbar_arrive(taken);
-                else ptx::mbar_arrive_cluster_relaxed(taken);
-            }
+            free_accumulator();
         }
     }
     __syncwarp();

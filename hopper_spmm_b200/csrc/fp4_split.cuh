@@ -13,24 +13,42 @@ namespace fp4 {
 
 constexpr uint32_t kPairRows4 = 256, kPairCols4 = 256;
 
-// Tiles of 256 rows x `cols` columns, side by side before one below the other.
+// Tiles of 256 rows x `cols` columns.  The side with fewer tiles is gone through in groups that L2 holds while the other one streams
+// by: 28672 x 8192 nvfp4 times 2,048 columns, the long side in the columns, took 267 us side by side and 220 the other way round.
 struct Split {
-    uint32_t cols;        // of a tile, a multiple of 32
-    uint32_t tiles_n;     // tiles side by side
-    uint32_t whole;       // tiles that one pair makes alone
-    uint32_t parts;       // of the others
+    uint32_t cols;              // of a tile, a multiple of 32
+    uint32_t inner, outer;      // tiles of either side
+    uint32_t group;             // inner tiles at a time
+    bool inner_rows;            // the inner side is the rows'
+    uint32_t whole;             // tiles that one pair makes alone
+    uint32_t parts;             // of the others
     uint32_t items;
-    uint32_t steps;       // of k
+    uint32_t steps;             // of k
 };
 
-inline Split make_split(uint32_t m, uint32_t n, uint32_t cols, uint32_t steps, uint32_t min_steps, uint32_t pairs) {
+// `step_us`: what a step of a tile of 256 columns takes; `step_bytes`: of 256 rows or columns of either operand in a step, the larger.
+inline Split make_split(uint32_t m, uint32_t n, uint32_t cols, uint32_t steps, uint32_t min_steps, double step_us, uint32_t step_bytes, uint32_t pairs) {
     Split s{};
     s.cols = cols;
-    s.tiles_n = (n + cols - 1) / cols;
     s.steps = steps;
-    const uint32_t tiles = (m + kPairRows4 - 1) / kPairRows4 * s.tiles_n, rest = tiles % pairs;
-    s.parts = rest ? std::min(pairs / rest, steps / min_steps) : 1;
-    if (s.parts < 2) s.parts = 1;
+    const uint32_t tiles_m = (m + kPairRows4 - 1) / kPairRows4, tiles_n = (n + cols - 1) / cols, tiles = tiles_m * tiles_n, rest = tiles % pairs;
+    s.inner_rows = tiles_m < tiles_n;
+    s.inner = std::min(tiles_m, tiles_n);
+    s.outer = std::max(tiles_m, tiles_n);
+    const uint32_t fit = (uint32_t)std::max<uint64_t>(4, (48ull << 20) / ((uint64_t)step_bytes * steps));  // of the 126 MB of L2
+    const uint32_t groups = (s.inner + fit - 1) / fit;
+    s.group = (s.inner + groups - 1) / groups;
+    // Parts of the last round's tiles: as many as make it shortest, their sums' way through memory and the second launch, some 3 us, counted
+    const double tile_us = step_us * steps * cols / kPairCols4, sums_us = (double)rest * kPairRows4 * cols * 8. / 5e6;
+    s.parts = 1;
+    double best = tile_us;
+    for (uint32_t parts = 2; rest && parts <= 32 && parts * min_steps <= steps; ++parts) {
+        const double time = tile_us * ((rest * parts + pairs - 1) / pairs) / parts + sums_us * parts + 3.;
+        if (time < best) {
+            best = time;
+            s.parts = parts;
+        }
+    }
     s.whole = s.parts > 1 ? tiles - rest : tiles;
     s.items = s.whole + (tiles - s.whole) * s.parts;
     return s;
@@ -41,16 +59,24 @@ struct Item {
     uint32_t m0, n0, first, last;  // steps [first, last)
     uint32_t slot;                 // of a part, else ~0
 };
+B200_DEVICE void split_tile(const Split &s, uint32_t tile, uint32_t &m0, uint32_t &n0) {
+    const uint32_t of_group = s.group * s.outer, first = tile / of_group * s.group, in_group = tile % of_group, size = min(s.group, s.inner - first);
+    const uint32_t inner = first + in_group % size, outer = in_group / size;
+    m0 = (s.inner_rows ? inner : outer) * kPairRows4;
+    n0 = (s.inner_rows ? outer : inner) * s.cols;
+}
 B200_DEVICE Item split_item(const Split &s, uint32_t i) {
-    uint32_t tile = i, part = 0, parts = 1, slot = ~0u;
+    Item w{0, 0, 0, s.steps, ~0u};
+    uint32_t tile = i;
     if (i >= s.whole) {
-        slot = i - s.whole;
-        tile = s.whole + slot / s.parts;
-        part = slot % s.parts;
-        parts = s.parts;
+        w.slot = i - s.whole;
+        tile = s.whole + w.slot / s.parts;
+        const uint32_t part = w.slot % s.parts;
+        w.first = part * s.steps / s.parts;
+        w.last = (part + 1) * s.steps / s.parts;
     }
-    if (parts == 1) slot = ~0u;
-    return {tile / s.tiles_n * kPairRows4, tile % s.tiles_n * s.cols, part * s.steps / parts, (part + 1) * s.steps / parts, slot};
+    split_tile(s, tile, w.m0, w.n0);
+    return w;
 }
 
 // C of the tiles that were cut: the parts' sums in order.  A thread a row and 32 columns.
@@ -58,8 +84,11 @@ static __global__ void __launch_bounds__(kPairRows4) fp4_join_kernel(const Split
                                                              const float *__restrict__ b_whole, float left, const Target c) {
     ptx::wait_for_grids_before();
     const Factor f(a_whole ? *reinterpret_cast<const volatile float *>(a_whole) : 1.f, b_whole ? *reinterpret_cast<const volatile float *>(b_whole) : left);
-    const uint32_t tile = s.whole + blockIdx.x, col = blockIdx.y * 32u;
-    const uint32_t row = tile / s.tiles_n * kPairRows4 + threadIdx.x, n0 = tile % s.tiles_n * s.cols + col;
+    const uint32_t col = blockIdx.y * 32u;
+    uint32_t row, n0;
+    split_tile(s, s.whole + blockIdx.x, row, n0);
+    row += threadIdx.x;
+    n0 += col;
     if (row >= m || n0 >= n) return;
     float v[32] = {};
     for (uint32_t part = 0; part < s.parts; ++part) {

@@ -77,5 +77,38 @@ B200_DEVICE void store_row(const Target &c, uint32_t row, uint32_t col, uint32_t
     else store_row_as<__nv_bfloat16>(c, row, col, n, v);
 }
 
+// The same in two steps, for sums that have to leave their place before they are written: 16 of them as 16-bit numbers, and 32 of those to C.
+B200_DEVICE void pack_row(int type, const float (&v)[16], uint32_t *out) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (type == B200SPMM_T_F16) {
+            const __half2 two = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            out[i] = *reinterpret_cast<const uint32_t *>(&two);
+        } else {
+            const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            out[i] = *reinterpret_cast<const uint32_t *>(&two);
+        }
+    }
+}
+B200_DEVICE void store_packed_row(const Target &c, uint32_t row, uint32_t col, uint32_t n, const uint32_t (&v)[16]) {
+    uint16_t *out = reinterpret_cast<uint16_t *>(c.ptr);
+    if (c.transposed) {
+        uint16_t *dst = out + (int64_t)col * c.ldc + row;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (col + i < n) dst[(int64_t)i * c.ldc] = (uint16_t)(v[i / 2] >> (i & 1) * 16);
+        return;
+    }
+    uint16_t *dst = out + (int64_t)row * c.ldc + col;
+    if (c.wide && n - col >= 32u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4 *>(dst)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (col + i < n) dst[i] = (uint16_t)(v[i / 2] >> (i & 1) * 16);
+    }
+}
+
 }  // namespace fp4
 }  // namespace b200spmm

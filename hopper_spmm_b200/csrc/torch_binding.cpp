@@ -274,9 +274,9 @@ bool output_of(PyObject *arg, int64_t rows, int64_t n, long type, const at::Tens
 }
 
 // The workspace of a product of `a` with n columns; nothing where it needs none (or cannot be asked: the product will say why).
-at::Tensor product_workspace(const b200spmm_fp4_t &a, int64_t n, const at::Tensor &like, uint64_t *bytes) {
+at::Tensor product_workspace(const b200spmm_fp4_t &a, const Dense *b, int64_t n, const at::Tensor &like, uint64_t *bytes) {
     *bytes = 0;
-    if (b200spmm_fp4_product_workspace(&a, n, bytes) != B200SPMM_OK || *bytes == 0) return at::Tensor();
+    if (b200spmm_fp4_product_workspace(&a, b ? b->ptr : nullptr, b ? b->ld : 0, n, b && b->transposed, bytes) != B200SPMM_OK || *bytes == 0) return at::Tensor();
     return new_cuda({(int64_t)*bytes}, at::kByte, like);
 }
 
@@ -326,7 +326,7 @@ PyObject *fp4_product(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     if (!output_of(args[12], (int64_t)a.rows, (int64_t)b.rows, type, like, &C, &c)) return nullptr;
     void *stream = c10::cuda::getCurrentCUDAStream(like.get_device()).stream();
     uint64_t bytes;
-    const at::Tensor workspace = product_workspace(a, (int64_t)b.rows, like, &bytes);
+    const at::Tensor workspace = product_workspace(a, nullptr, (int64_t)b.rows, like, &bytes);
     void *ws = workspace.defined() ? workspace.data_ptr() : nullptr;
     int st;
     {
@@ -355,7 +355,7 @@ PyObject *fp4_dense_product(PyObject *, PyObject *const *args, Py_ssize_t n_args
     void *stream = c10::cuda::getCurrentCUDAStream(B->get_device()).stream();
     const int64_t n = B->size(1);
     uint64_t bytes;
-    const at::Tensor workspace = product_workspace(a, n, *B, &bytes);
+    const at::Tensor workspace = product_workspace(a, &b, n, *B, &bytes);
     void *ws = workspace.defined() ? workspace.data_ptr() : nullptr;
     int st;
     {

@@ -557,11 +557,12 @@ int b200spmm_fp4_dense_product(const b200spmm_fp4_t *a, const void *d_B, int64_t
                                void *d_C, int64_t ldc, int c_dtype, int c_transposed, void *workspace, uint64_t workspace_bytes,
                                void *stream);
 /*
- * Bytes of the workspace with which a product of `a` with n columns shares out its work best: tiles that would leave part of the
- * GPU without any are cut along k, and their sums meet there.  With less, or none (null), products run without.  It belongs to the
- * call until that is done on `stream`.
+ * Bytes of the workspace with which a product of `a` with n columns shares out its work best: d_B, ldb and b_transposed as
+ * b200spmm_fp4_dense_product gets them, d_B null for b200spmm_fp4_product with a matrix of n rows.  Tiles that would leave part of the GPU
+ * without any are cut along k, and their sums meet there; a B that starts anywhere is brought to 16 bytes there.  With less, or none
+ * (null), products run without.  16-byte aligned; it belongs to the call until that is done on `stream`.
  */
-int b200spmm_fp4_product_workspace(const b200spmm_fp4_t *a, int64_t n, uint64_t *bytes);
+int b200spmm_fp4_product_workspace(const b200spmm_fp4_t *a, const void *d_B, int64_t ldb, int64_t n, int b_transposed, uint64_t *bytes);
 
 /*
  * All of these are asynchronous on `stream`, run on the matrices' device whichever is current, allocate nothing and may be captured
