@@ -117,7 +117,8 @@ __global__ void __launch_bounds__(256) fp4_align_kernel(const uint16_t *__restri
 // Up to 16 columns go to the narrow kernel, which reads any B.
 constexpr uint32_t kNarrowColumns = 16;
 bool is_aligned(const void *b, int64_t ldb) { return reinterpret_cast<uintptr_t>(b) % 16u == 0 && ldb % 8 == 0; }
-uint64_t aligned_bytes(uint64_t rows, uint64_t cols) { return rows * ((cols + 7u) / 8u) * 16u; }
+uint64_t aligned_pieces(uint64_t cols) { return (cols + 63u) / 64u * 8u; }  // of 16 bytes, whole lines of 128: boxes then touch no more of them than they have to
+uint64_t aligned_bytes(uint64_t rows, uint64_t cols) { return rows * aligned_pieces(cols) * 16u; }
 
 template <typename T, bool kMx, bool kTokens>
 int launch_dense(const b200spmm_fp4_t *a, const DenseParams &d, uint8_t *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
@@ -125,7 +126,7 @@ int launch_dense(const b200spmm_fp4_t *a, const DenseParams &d, uint8_t *workspa
     if (d.n <= kNarrowColumns || (!d.b_wide && (!workspace || workspace_bytes < need))) return launch_narrow_columns<T, kMx, kTokens>(a, d, stream);
     if (d.b_wide) return launch_wide<T, kMx, kTokens>(a, d, reinterpret_cast<float *>(workspace), workspace_bytes, stream);
     // no tensor map describes B: a copy that one does goes first into the workspace
-    const uint32_t pieces = (uint32_t)((cols + 7u) / 8u);
+    const uint32_t pieces = (uint32_t)aligned_pieces(cols);
     B200_CUDA_TRY(launch_after(fp4_align_kernel, dim3((unsigned)std::min<uint64_t>((rows * pieces + 255u) / 256u, (uint64_t)sm_count() * 8u)), 256, 0, 1, stream,
                                reinterpret_cast<const uint16_t *>(d.b), d.ldb, (uint32_t)rows, (uint32_t)cols, reinterpret_cast<uint4 *>(workspace), pieces));
     DenseParams with = d;

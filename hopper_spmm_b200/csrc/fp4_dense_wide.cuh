@@ -171,10 +171,14 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     if (!alive) break;
                     ptx::tcgen05_fence_after_sync();
                     const uint32_t a = tmem + kPairCols4 + buffer * Cfg::kBufferCols, b = b_lo + s * (bytes_b >> 4);
-#pragma unroll
-                    for (uint32_t i = 0; i < kWideK / 16u; ++i)
-                        ptx::umma_pair_f16_ts_if(on & (left > i * 16u ? 1u : 0u), tmem, a + i * 8u, b + ((kTokens ? i / 4u * box_bytes + i % 4u * 32u : i * 2048u) >> 4), b_hi, idesc,
-                                                 i ? 1u : accumulate);
+                    if (left >= kWideK) {
+                        constexpr uint32_t kNext = kTokens ? 2u : 128u;
+                        ptx::umma_pair_f16_ts_x4_if<kNext>(on, tmem, a, b, b_hi, idesc, accumulate);
+                        ptx::umma_pair_f16_ts_x4_if<kNext>(on, tmem, a + 32u, b + (kTokens ? box_bytes >> 4 : 512u), b_hi, idesc, 1u);
+                    } else {
+                        for (uint32_t i = 0; i * 16u < left; ++i)
+                            ptx::umma_pair_f16_ts_if(on, tmem, a + i * 8u, b + ((kTokens ? i / 4u * box_bytes + i % 4u * 32u : i * 2048u) >> 4), b_hi, idesc, i ? 1u : accumulate);
+                    }
                     ptx::umma_commit_pair_if(on, empty_bar(s));
                     accumulate = 1;
                     left -= kWideK;
@@ -299,7 +303,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 #pragma unroll
                 for (uint32_t j = 0; j < 2; ++j) {
                     const uint32_t c = mine * 32u + j * 128u;
-                    if (c < p.split.cols && c_row < p.d.m && w.n0 + c < p.d.n) store_packed_row(p.d.c, c_row, w.n0 + c, p.d.n, packed[j]);
+                    if (c < p.split.cols && w.n0 + c < p.d.n) store_words(p.d.c, c_row - lane, p.d.m, w.n0 + c, p.d.n, packed[j]);
                 }
                 continue;
             }
@@ -317,7 +321,10 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 } else {
                     float v[16];
                     scaled(c, v);
-                    if (c_row < p.d.m && w.n0 + c < p.d.n) store_row(p.d.c, c_row, w.n0 + c, p.d.n, v);
+                    uint32_t words[16];
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i) words[i] = __float_as_uint(v[i]);
+                    if (w.n0 + c < p.d.n) store_words(p.d.c, c_row - lane, p.d.m, w.n0 + c, p.d.n, words);
                 }
             }
             free_accumulator();

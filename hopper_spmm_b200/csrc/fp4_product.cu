@@ -116,11 +116,14 @@ fp4_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             ptx::tcgen05_fence_after_sync();
             const uint32_t sa = tmem_scales + s * Cfg::kScaleCols, sb = sa + Cfg::kGroupsPerStage * 4u;
             const uint32_t a = a_lo + s * (Cfg::kBytesA >> 4), b = b_lo + s * (Cfg::kBytesB >> 4);
-#pragma unroll
-            for (uint32_t i = 0; i < kStageK / kMmaK; ++i) {
-                const uint32_t g = kMx ? i / 2 : i;
-                ptx::umma_fp4_ss_if<kMx, 1>(on & (left > i * kMmaK ? 1u : 0u), tmem, a + i * 2u, a_hi, b + i * 2u, b_hi,
-                                            ptx::make_fp4_instr_desc(kMx, kTileM, kN, kMx ? i % 2 * 2u : 0u), sa + g * 4u, sb + g * 4u, (it | i) ? 1u : 0u);
+            constexpr uint32_t idesc = ptx::make_fp4_instr_desc(kMx, kTileM, kN, 0);
+            if (left >= kStageK) {
+                ptx::umma_fp4_ss_x4_if<kMx, 1>(on, tmem, a, a_hi, b, b_hi, idesc, sa, sb, 4, it ? 1u : 0u);
+            } else {
+                for (uint32_t i = 0; i * kMmaK < left; ++i) {
+                    const uint32_t g = kMx ? i / 2 : i;
+                    ptx::umma_fp4_ss_if<kMx, 1>(on, tmem, a + i * 2u, a_hi, b + i * 2u, b_hi, kMx && i % 2 ? idesc | ptx::kSecondScales : idesc, sa + g * 4u, sb + g * 4u, (it | i) ? 1u : 0u);
+                }
             }
             ptx::umma_commit_if(on, empty_bar(s));
             left -= kStageK;

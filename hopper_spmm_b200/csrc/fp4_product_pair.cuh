@@ -3,6 +3,7 @@
 // Bound: the tensor core's 4-bit rate, four times that of 16 bits, which is more than L2 feeds: a pair's tile brings 72 KB
 // for 512 clocks of it, 70 bytes a clock and SM.  The pair shares B: each CTA brings 128 rows of A, half of B's rows and all the scales of
 // either.
+// C lies column by column (the operands are exchanged where it does not), so that lanes, which hold rows, write neighbours.
 // Warps 0-7 take accumulators to C, warps 8-15 bring scales to tensor memory (four of them a stage, each its quarter of the lanes;
 // tcgen05.cp does the same, but in line with the MMAs: 110 clocks a copy of 512 bytes, twelve a stage, doubled the time),
 // warp 16 of the even CTA issues the MMAs, warps 17 and 18 load.
@@ -137,7 +138,6 @@ fp4_product_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
             const uint64_t a_desc = ptx::make_smem_desc(a_addr, 16, 1024, ptx::kSwizzle128B), b_desc = ptx::make_smem_desc(b_addr, 16, 1024, ptx::kSwizzle128B);
             const uint32_t a_lo = (uint32_t)a_desc, a_hi = (uint32_t)(a_desc >> 32), b_lo = (uint32_t)b_desc, b_hi = (uint32_t)(b_desc >> 32);
             const uint32_t idesc = ptx::make_fp4_instr_desc(kMx, kPairRows4, p.split.cols, 0);
-            constexpr uint32_t kSecond = ptx::make_fp4_instr_desc(false, 0, 0, 2) ^ ptx::make_fp4_instr_desc(false, 0, 0, 0);  // of a word's pairs of scales
             uint32_t s = 0, phase = 0, round = 0;
             bool alive = true;
             for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs, ++round) {
@@ -150,11 +150,14 @@ fp4_product_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                     ptx::tcgen05_fence_after_sync();
                     const uint32_t sa = tmem_scales + s * Cfg::kScaleCols, sb = sa + Cfg::kGroups * 4u;
                     const uint32_t a = a_lo + s * (Cfg::kBytesA >> 4), b = b_lo + s * (Cfg::kBytesB >> 4);
-#pragma unroll
-                    for (uint32_t i = 0; i < kStageK / kMmaK; ++i) {
-                        const uint32_t g = kMx ? i / 2 : i;
-                        ptx::umma_fp4_ss_if<kMx, 2>(on & (left > i * kMmaK ? 1u : 0u), tmem, a + i * 2u, a_hi, b + i * 2u, b_hi, kMx && i % 2 ? idesc | kSecond : idesc,
-                                                    sa + g * 4u, sb + g * 8u, i ? 1u : accumulate);
+                    if (left >= kStageK) {
+                        ptx::umma_fp4_ss_x4_if<kMx, 2>(on, tmem, a, a_hi, b, b_hi, idesc, sa, sb, 8, accumulate);
+                    } else {
+                        for (uint32_t i = 0; i * kMmaK < left; ++i) {
+                            const uint32_t g = kMx ? i / 2 : i;
+                            ptx::umma_fp4_ss_if<kMx, 2>(on, tmem, a + i * 2u, a_hi, b + i * 2u, b_hi, kMx && i % 2 ? idesc | ptx::kSecondScales : idesc, sa + g * 4u, sb + g * 8u,
+                                                        i ? 1u : accumulate);
+                        }
                     }
                     ptx::umma_commit_pair_if(on, empty_bar(s));
                     accumulate = 1;
@@ -255,7 +258,7 @@ fp4_product_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
 #pragma unroll
                 for (uint32_t j = 0; j < 4; ++j) {
                     const uint32_t c = half * 32u + j * 64u;
-                    if (c < p.split.cols && c_row < p.m && w.n0 + c < p.n) store_packed_row(p.c, c_row, w.n0 + c, p.n, packed[j]);
+                    if (c < p.split.cols && c_row < p.m && w.n0 + c < p.n) store_packed_column(p.c, c_row, w.n0 + c, p.n, packed[j]);
                 }
                 continue;
             }

@@ -90,23 +90,64 @@ B200_DEVICE void pack_row(int type, const float (&v)[16], uint32_t *out) {
         }
     }
 }
-B200_DEVICE void store_packed_row(const Target &c, uint32_t row, uint32_t col, uint32_t n, const uint32_t (&v)[16]) {
-    uint16_t *out = reinterpret_cast<uint16_t *>(c.ptr);
-    if (c.transposed) {
-        uint16_t *dst = out + (int64_t)col * c.ldc + row;
+// 32 16-bit numbers of a row as 16 words, to a C that lies column by column: lanes hold neighbouring rows.
+B200_DEVICE void store_packed_column(const Target &c, uint32_t row, uint32_t col, uint32_t n, const uint32_t (&v)[16]) {
+    uint16_t *dst = reinterpret_cast<uint16_t *>(c.ptr) + (int64_t)col * c.ldc + row;
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (col + i < n) dst[(int64_t)i * c.ldc] = (uint16_t)(v[i / 2] >> (i & 1) * 16);
+    for (int i = 0; i < 32; ++i)
+        if (col + i < n) dst[(int64_t)i * c.ldc] = (uint16_t)(v[i / 2] >> (i & 1) * 16);
+}
+// 16 words of each lane, transposed between the 16 lanes of either half of the warp: word i of lane l goes to word l % 16 of lane i (of its half).
+B200_DEVICE void transpose_16(uint32_t (&v)[16], uint32_t lane) {
+#pragma unroll
+    for (uint32_t d = 1; d < 16; d <<= 1)
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i)
+            if (!(i & d)) {
+                const bool upper = (lane & d) != 0;
+                const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, upper ? v[i] : v[i | d], d);
+                if (upper) v[i] = got;
+                else v[i | d] = got;
+            }
+}
+// A warp's 32 rows of C from `row0` on, 16 words of each (32 16-bit numbers, or 16 fp32 ones) from column `col` on; words[] is lost.  Row by
+// row the words change places first, so that 16 lanes write 64 neighbouring bytes of a row.  All lanes take part.
+B200_DEVICE void store_words(const Target &c, uint32_t row0, uint32_t rows, uint32_t col, uint32_t n, uint32_t (&v)[16]) {
+    const uint32_t lane = threadIdx.x & 31u;
+    const bool half = c.type != B200SPMM_T_F32;
+    if (c.transposed) {  // lanes hold neighbouring rows
+        const uint32_t row = row0 + lane;
+        if (row >= rows) return;
+        if (half) {
+            store_packed_column(c, row, col, n, v);
+        } else {
+            uint32_t *dst = reinterpret_cast<uint32_t *>(c.ptr) + (int64_t)col * c.ldc + row;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (col + i < n) dst[(int64_t)i * c.ldc] = v[i];
+        }
         return;
     }
-    uint16_t *dst = out + (int64_t)row * c.ldc + col;
-    if (c.wide && n - col >= 32u) {
+    transpose_16(v, lane);
+    const uint32_t first = row0 + (lane & 16u), at = col + (lane & 15u) * (half ? 2u : 1u);
+    if (half) {
+        uint16_t *dst = reinterpret_cast<uint16_t *>(c.ptr) + (int64_t)first * c.ldc + at;
+        const bool pairs = reinterpret_cast<uintptr_t>(c.ptr) % 4u == 0 && c.ldc % 2 == 0;  // (columns come in pairs, too)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4 *>(dst)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        for (uint32_t i = 0; i < 16; ++i, dst += c.ldc) {
+            if (first + i >= rows) break;
+            if (pairs && at + 1u < n) {
+                *reinterpret_cast<uint32_t *>(dst) = v[i];
+            } else {
+                if (at < n) dst[0] = (uint16_t)v[i];
+                if (at + 1u < n) dst[1] = (uint16_t)(v[i] >> 16);
+            }
+        }
     } else {
+        uint32_t *dst = reinterpret_cast<uint32_t *>(c.ptr) + (int64_t)first * c.ldc + at;
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (col + i < n) dst[i] = (uint16_t)(v[i / 2] >> (i & 1) * 16);
+        for (uint32_t i = 0; i < 16; ++i, dst += c.ldc)
+            if (first + i < rows && at < n) *dst = v[i];
     }
 }
 

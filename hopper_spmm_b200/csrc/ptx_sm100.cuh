@@ -361,6 +361,16 @@ B200_DEVICE void umma_pair_f16_ts_if(uint32_t on, uint32_t d_tmem, uint32_t a_tm
                  "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], db, %4, p;\n}\n"
                  ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
 }
+// Four in a row: 64 values of k, eight columns of A further each time and `kNext` units of 16 bytes of B.
+template <uint32_t kNext>
+B200_DEVICE void umma_pair_f16_ts_x4_if(uint32_t on, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p, q, t;\n.reg .b64 db;\n.reg .b32 la, lb;\nsetp.ne.b32 p, %5, 0;\nsetp.ne.b32 q, %6, 0;\nsetp.eq.b32 t, %0, %0;\n"
+                 "mov.b64 db, {%2, %3};\n@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], db, %4, p;\n"
+                 "add.u32 la, %1, 8;\nadd.u32 lb, %2, %7;\nmov.b64 db, {lb, %3};\n@q tcgen05.mma.cta_group::2.kind::f16 [%0], [la], db, %4, t;\n"
+                 "add.u32 la, %1, 16;\nadd.u32 lb, %2, %8;\nmov.b64 db, {lb, %3};\n@q tcgen05.mma.cta_group::2.kind::f16 [%0], [la], db, %4, t;\n"
+                 "add.u32 la, %1, 24;\nadd.u32 lb, %2, %9;\nmov.b64 db, {lb, %3};\n@q tcgen05.mma.cta_group::2.kind::f16 [%0], [la], db, %4, t;\n}\n"
+                 ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(on), "n"(kNext), "n"(2 * kNext), "n"(3 * kNext) : "memory");
+}
 B200_DEVICE void umma_commit_pair_if(uint32_t on, uint32_t bar) {
     asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %2, 0;\n"
                  "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n"
@@ -553,6 +563,34 @@ B200_DEVICE void umma_fp4_ss_if(uint32_t on, uint32_t d_tmem, uint32_t a_lo, uin
     else B200_FP4_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
 #undef B200_FP4_MMA
 }
+constexpr uint32_t kSecondScales = make_fp4_instr_desc(false, 0, 0, 2) ^ make_fp4_instr_desc(false, 0, 0, 0);  // the second pair of a word's scales
+// Four in a row, 256 values of k: 32 bytes further in either operand, the scales' words `next_b` (B) and four (A) columns on - for mxfp4
+// the second and the fourth take the second pair of a word.
+template <bool kMx, int kCtas>
+B200_DEVICE void umma_fp4_ss_x4_if(uint32_t on, uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t a_scales,
+                                   uint32_t b_scales, uint32_t next_b, uint32_t accumulate) {
+    const uint32_t idesc1 = kMx ? idesc | kSecondScales : idesc;
+    const uint32_t a1 = a_scales + (kMx ? 0u : 4u), a2 = a_scales + (kMx ? 4u : 8u), a3 = a_scales + (kMx ? 4u : 12u);
+    const uint32_t b1 = b_scales + (kMx ? 0u : next_b), b2 = b_scales + (kMx ? 1u : 2u) * next_b, b3 = b_scales + (kMx ? 1u : 3u) * next_b;
+#define B200_FP4_MMA4(ctas, kind)                                                                                                          \
+    asm volatile("{\n.reg .pred p, q, t;\n.reg .b64 da, db;\n.reg .b32 la, lb;\nsetp.ne.b32 p, %14, 0;\nsetp.ne.b32 q, %15, 0;\nsetp.eq.b32 t, %0, %0;\n" \
+                 "mov.b64 da, {%1, %2};\nmov.b64 db, {%3, %4};\n"                                                                           \
+                 "@q tcgen05.mma.cta_group::" ctas ".kind::" kind " [%0], da, db, %5, [%6], [%10], p;\n"                                      \
+                 "add.u32 la, %1, 2;\nadd.u32 lb, %3, 2;\nmov.b64 da, {la, %2};\nmov.b64 db, {lb, %4};\n"                                    \
+                 "@q tcgen05.mma.cta_group::" ctas ".kind::" kind " [%0], da, db, %16, [%7], [%11], t;\n"                                     \
+                 "add.u32 la, %1, 4;\nadd.u32 lb, %3, 4;\nmov.b64 da, {la, %2};\nmov.b64 db, {lb, %4};\n"                                    \
+                 "@q tcgen05.mma.cta_group::" ctas ".kind::" kind " [%0], da, db, %5, [%8], [%12], t;\n"                                      \
+                 "add.u32 la, %1, 6;\nadd.u32 lb, %3, 6;\nmov.b64 da, {la, %2};\nmov.b64 db, {lb, %4};\n"                                    \
+                 "@q tcgen05.mma.cta_group::" ctas ".kind::" kind " [%0], da, db, %16, [%9], [%13], t;\n}\n"                                  \
+                 ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(a_scales), "r"(a1), "r"(a2), "r"(a3), "r"(b_scales), "r"(b1),   \
+                   "r"(b2), "r"(b3), "r"(accumulate), "r"(on), "r"(idesc1) : "memory")
+    if constexpr (kMx && kCtas == 1) B200_FP4_MMA4("1", "mxf4.block_scale.scale_vec::2X");
+    else if constexpr (kMx) B200_FP4_MMA4("2", "mxf4.block_scale.scale_vec::2X");
+    else if constexpr (kCtas == 1) B200_FP4_MMA4("1", "mxf4nvf4.block_scale.scale_vec::4X");
+    else B200_FP4_MMA4("2", "mxf4nvf4.block_scale.scale_vec::4X");
+#undef B200_FP4_MMA4
+}
+
 // 16 bytes of shared memory a lane to four columns of the warp's quarter of tensor memory, for kN addresses one after the other.
 template <int kN>
 B200_DEVICE void tmem_st_v4(uint32_t taddr, const uint4 (&v)[kN]) {
