@@ -52,11 +52,11 @@ int launch_narrow_columns(const b200spmm_fp4_t *a, const DenseParams &d, cudaStr
     return d.n <= 8 ? launch_narrow<T, kMx, 1, kTokens>(a, d, stream) : launch_narrow<T, kMx, 2, kTokens>(a, d, stream);
 }
 
-// Columns shared out evenly over as few tiles as there can be; a part has at least four steps: shorter ones are not worth their
+// Columns shared out evenly over as few tiles as there can be, 64 at least (fewer take longer: 24 of 28672 x 8192 84 us as 32, 69 as 64); a part has at least four steps: shorter ones are not worth their
 // sums' way through memory.
 Split wide_split(uint32_t m, uint32_t n, uint32_t k, uint32_t pairs) {
-    const uint32_t tiles_n = (n + kPairCols4 - 1) / kPairCols4, cols = ((n + tiles_n - 1) / tiles_n + 31u) / 32u * 32u;
-    return make_split(m, n, cols, (k + kWideK - 1) / kWideK, 4, 0.55, 256 * kWideK * 2, pairs);
+    const uint32_t tiles_n = (n + kPairCols4 - 1) / kPairCols4, cols = std::max(64u, ((n + tiles_n - 1) / tiles_n + 31u) / 32u * 32u);
+    return make_split(m, n, cols, (k + kWideK - 1) / kWideK, 4, 0.55, 0.5, 256 * kWideK * 2, pairs);
 }
 
 // Pairs of CTAs of the wide kernel that the current device runs at once (its instances take the same room).
@@ -81,7 +81,8 @@ int launch_wide(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace,
     prm.split = wide_split(d.m, d.n, d.k, pairs);
     if (prm.split.parts > 1 && (!workspace || workspace_bytes < split_workspace(prm.split))) prm.split = wide_split(d.m, d.n, d.k, 1);
     prm.row_blocks = (d.m + 127u) / 128u;
-    prm.stages = WideCfg::stages(kTokens, prm.split.cols);
+    prm.stages_a = WideCfg::stages_a(kTokens, prm.split.cols);
+    prm.stages_b = WideCfg::stages_b(kTokens, prm.split.cols);
     prm.partial = workspace;
     B200_CUDA_TRY(status_word(&prm.status));
     prm.wait_limit_ns = kDeviceWaitLimitNs;

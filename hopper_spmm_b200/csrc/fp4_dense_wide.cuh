@@ -12,9 +12,12 @@
 // every fourth step, so that what a step has to wait for (its stage, its way to tensor memory) overlaps with three others;
 // after an item's last step they take the accumulator to C.  Warp 16 of the even CTA issues the MMAs, warps 17 and 18 load.
 //
-//   full[s]   stage s has landed (TMA bytes, each CTA its own): the widening warps wait for it, with B's part of it
-//   ready[b]  buffer b of widened A is written in both CTAs (eight warps arrive at the even CTA)
-//   empty[s]  the MMAs of the step in stage s are done (commit, in both CTAs): the stage and its buffer of widened A are free
+// A and B have stages of their own: those of A, which comes from memory, are free again as soon as they have been read.
+//
+//   full a, full b   a stage has landed (TMA bytes, each CTA its own): the widening warps wait for both
+//   empty a   the four warps that widen it have read it
+//   ready[g]  group g's buffer of widened A is written in both CTAs, and B's stage is there (eight warps arrive at the even CTA)
+//   empty b   the MMAs of the step are done (commit, in both CTAs): the stage of B and the buffer of widened A are free
 //   done      the accumulator of an item is complete (commit, in both CTAs)
 //   taken     all 32 warps have read it (they arrive at the even CTA)
 //
@@ -30,13 +33,13 @@ constexpr uint32_t kWideK = 128;  // of a step
 
 struct WideCfg {
     static constexpr uint32_t kBytesA = 128 * kWideK / 2, kBytesScales = 1024;
-    static constexpr uint32_t kMinStages = 5, kMaxStages = 12;
+    static constexpr uint32_t kStageA = kBytesA + kBytesScales, kMinA = 6, kMaxA = 12, kMaxB = 8;  // stages
     static constexpr uint32_t kBuffers = 4, kBufferCols = kWideK / 2;  // of widened A, in tensor memory behind the accumulator
     static constexpr uint32_t kWideners = 16;
     static_assert(kBuffers == kWideners / 4, "a group of four warps has a buffer of its own");
     static constexpr int kWarps = kWideners + 3, kThreads = 32 * kWarps;
     static constexpr uint32_t kTmemCols = 512;
-    static constexpr uint32_t kBarriers = 2 * kMaxStages + kBuffers + 3;
+    static constexpr uint32_t kBarriers = 2 * kMaxA + 2 * kMaxB + kBuffers + 3;
     static constexpr uint32_t kOtherBytes = 1024 + kBarriers * 8 + 16;
     static constexpr size_t kSmemBytes = 227 * 1024;  // at most
     static_assert(kPairCols4 + kBuffers * kBufferCols <= kTmemCols, "tensor memory of an SM");
@@ -44,20 +47,22 @@ struct WideCfg {
     __host__ __device__ static constexpr uint32_t box_bytes(bool tokens, uint32_t cols) { return tokens ? cols / 2u * 128u : kWideK * 128u; }
     __host__ __device__ static constexpr uint32_t boxes(bool tokens, uint32_t cols) { return tokens ? 2u : (cols / 2u + 63u) / 64u; }
     __host__ __device__ static constexpr uint32_t b_bytes(bool tokens, uint32_t cols) { return box_bytes(tokens, cols) * boxes(tokens, cols); }
-    // Few columns leave room for more stages: A is what they have to bring.
-    static uint32_t stages(bool tokens, uint32_t cols) {
-        const uint32_t stage = kBytesA + kBytesScales + b_bytes(tokens, cols);
-        return std::min<uint32_t>(kMaxStages, ((uint32_t)kSmemBytes - kOtherBytes) / stage);
+    // Few columns leave room for more stages.
+    static uint32_t stages_b(bool tokens, uint32_t cols) { return std::min<uint32_t>(kMaxB, ((uint32_t)kSmemBytes - kOtherBytes - kMinA * kStageA) / b_bytes(tokens, cols)); }
+    static uint32_t stages_a(bool tokens, uint32_t cols) {
+        return std::min<uint32_t>(kMaxA, ((uint32_t)kSmemBytes - kOtherBytes - stages_b(tokens, cols) * b_bytes(tokens, cols)) / kStageA);
     }
-    static size_t smem_bytes(bool tokens, uint32_t cols) { return kOtherBytes + (size_t)stages(tokens, cols) * (kBytesA + kBytesScales + b_bytes(tokens, cols)); }
+    static size_t smem_bytes(bool tokens, uint32_t cols) {
+        return kOtherBytes + (size_t)stages_a(tokens, cols) * kStageA + (size_t)stages_b(tokens, cols) * b_bytes(tokens, cols);
+    }
 };
-static_assert((WideCfg::kSmemBytes - WideCfg::kOtherBytes) / (WideCfg::kBytesA + WideCfg::kBytesScales + WideCfg::b_bytes(false, 256)) >= WideCfg::kMinStages, "shared memory");
+static_assert((WideCfg::kSmemBytes - WideCfg::kOtherBytes - WideCfg::kMinA * WideCfg::kStageA) / WideCfg::b_bytes(false, 256) >= 5, "shared memory");
 
 struct WideParams {
     DenseParams d;
     Split split;
     uint32_t row_blocks;
-    uint32_t stages;
+    uint32_t stages_a, stages_b;
     float *partial;
     uint32_t *status;
     unsigned long long wait_limit_ns;
@@ -68,19 +73,21 @@ __global__ void __launch_bounds__(WideCfg::kThreads, 1)
 fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const WideParams p) {
     using Cfg = WideCfg;
     using W = Widen<T, kMx>;
-    const uint32_t stages = p.stages, box_bytes = Cfg::box_bytes(kTokens, p.split.cols), boxes = Cfg::boxes(kTokens, p.split.cols), bytes_b = box_bytes * boxes;
+    const uint32_t stages_a = p.stages_a, stages_b = p.stages_b, box_bytes = Cfg::box_bytes(kTokens, p.split.cols), boxes = Cfg::boxes(kTokens, p.split.cols), bytes_b = box_bytes * boxes;
     extern __shared__ uint8_t smem_raw[];
     // the same offsets in both CTAs: descriptors and multicast commits rely on it
     const uint32_t raw_addr = ptx::smem_u32(smem_raw);
     const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
     uint8_t *base = smem_raw + pad;
-    const uint32_t b_addr = raw_addr + pad, a_addr = b_addr + stages * bytes_b, s_addr = a_addr + stages * Cfg::kBytesA;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(base + (size_t)stages * (bytes_b + Cfg::kBytesA + Cfg::kBytesScales));
+    const uint32_t b_addr = raw_addr + pad, a_addr = b_addr + stages_b * bytes_b, s_addr = a_addr + stages_a * Cfg::kBytesA;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(base + (size_t)stages_b * bytes_b + (size_t)stages_a * Cfg::kStageA);
     const uint32_t bars_addr = ptx::smem_u32(bars);
-    auto full_bar = [&](uint32_t s) { return bars_addr + 8u * s; };
-    auto empty_bar = [&](uint32_t s) { return bars_addr + 8u * (Cfg::kMaxStages + s); };
-    auto ready_bar = [&](uint32_t b) { return bars_addr + 8u * (2 * Cfg::kMaxStages + b); };
-    const uint32_t done_bar = bars_addr + 8u * (2 * Cfg::kMaxStages + Cfg::kBuffers), taken_bar = done_bar + 8u, drain_bar = done_bar + 16u;
+    auto full_b = [&](uint32_t s) { return bars_addr + 8u * s; };
+    auto empty_b = [&](uint32_t s) { return bars_addr + 8u * (Cfg::kMaxB + s); };
+    auto full_a = [&](uint32_t s) { return bars_addr + 8u * (2 * Cfg::kMaxB + s); };
+    auto empty_a = [&](uint32_t s) { return bars_addr + 8u * (2 * Cfg::kMaxB + Cfg::kMaxA + s); };
+    auto ready_bar = [&](uint32_t b) { return bars_addr + 8u * (2 * Cfg::kMaxB + 2 * Cfg::kMaxA + b); };
+    const uint32_t done_bar = bars_addr + 8u * (2 * Cfg::kMaxB + 2 * Cfg::kMaxA + Cfg::kBuffers), taken_bar = done_bar + 8u, drain_bar = done_bar + 16u;
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(bars + Cfg::kBarriers);
     uint32_t *tmem_slot = const_cast<uint32_t *>(abort_flag) + 1;
 
@@ -90,9 +97,13 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     const uint32_t cols_half = p.split.cols / 2u;  // of B, this CTA's
 
     if (tid == 0) {
-        for (uint32_t s = 0; s < stages; ++s) {
-            ptx::mbar_init(full_bar(s), 2);
-            ptx::mbar_init(empty_bar(s), 1);
+        for (uint32_t s = 0; s < stages_a; ++s) {
+            ptx::mbar_init(full_a(s), 1);
+            ptx::mbar_init(empty_a(s), 4);
+        }
+        for (uint32_t s = 0; s < stages_b; ++s) {
+            ptx::mbar_init(full_b(s), 1);
+            ptx::mbar_init(empty_b(s), 1);
         }
         for (uint32_t b = 0; b < Cfg::kBuffers; ++b) ptx::mbar_init(ready_bar(b), 8);
         ptx::mbar_init(done_bar, 1);
@@ -121,6 +132,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const uint32_t on = lane == 0 ? 1u : 0u;
         const bool is_a = warp == Cfg::kWideners + 1;
         constexpr uint32_t kGroups = kMx ? 1 : 2;
+        const uint32_t stages = is_a ? stages_a : stages_b;
         uint32_t s = 0, phase = 1;
         bool alive = true;
         for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs) {
@@ -130,20 +142,20 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             const bool has_scales = row_block < p.row_blocks;
             const uint8_t *scales = p.d.scales + (uint64_t)row_block * p.d.groups * 512u;
             for (uint32_t step = w.first; step < w.last; ++step) {
-                alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait(empty_bar(s), phase, abort_flag, limit));
+                alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait(is_a ? empty_a(s) : empty_b(s), phase, abort_flag, limit));
                 if (!alive) break;
                 if (is_a) {
                     const uint32_t g0 = step * kGroups, scale_bytes = has_scales ? min(kGroups, p.d.groups - g0) * 512u : 0u;
-                    ptx::mbar_arrive_expect_tx_if(on, full_bar(s), Cfg::kBytesA + scale_bytes);
-                    ptx::tma_load_2d_if(on, a_addr + s * Cfg::kBytesA, &tmap_a, (int32_t)(step * (kWideK / 2)), (int32_t)(w.m0 + rank * 128u), full_bar(s));
-                    ptx::bulk_load_if(on & (has_scales ? 1u : 0u), s_addr + s * Cfg::kBytesScales, scales + (uint64_t)g0 * 512u, scale_bytes, full_bar(s));
+                    ptx::mbar_arrive_expect_tx_if(on, full_a(s), Cfg::kBytesA + scale_bytes);
+                    ptx::tma_load_2d_if(on, a_addr + s * Cfg::kBytesA, &tmap_a, (int32_t)(step * (kWideK / 2)), (int32_t)(w.m0 + rank * 128u), full_a(s));
+                    ptx::bulk_load_if(on & (has_scales ? 1u : 0u), s_addr + s * Cfg::kBytesScales, scales + (uint64_t)g0 * 512u, scale_bytes, full_a(s));
                 } else {
-                    ptx::mbar_arrive_expect_tx_if(on, full_bar(s), boxes * box_bytes);
+                    ptx::mbar_arrive_expect_tx_if(on, full_b(s), boxes * box_bytes);
 #pragma unroll
                     for (uint32_t i = 0; i < 2; ++i) {
                         const uint32_t there = on & (i < boxes ? 1u : 0u);
-                        if constexpr (kTokens) ptx::tma_load_2d_if(there, b_addr + s * bytes_b + i * box_bytes, &tmap_b, (int32_t)(step * kWideK + i * 64u), (int32_t)n0, full_bar(s));
-                        else ptx::tma_load_2d_if(there, b_addr + s * bytes_b + i * box_bytes, &tmap_b, (int32_t)(n0 + i * 64u), (int32_t)(step * kWideK), full_bar(s));
+                        if constexpr (kTokens) ptx::tma_load_2d_if(there, b_addr + s * bytes_b + i * box_bytes, &tmap_b, (int32_t)(step * kWideK + i * 64u), (int32_t)n0, full_b(s));
+                        else ptx::tma_load_2d_if(there, b_addr + s * bytes_b + i * box_bytes, &tmap_b, (int32_t)(n0 + i * 64u), (int32_t)(step * kWideK), full_b(s));
                     }
                 }
                 s = s + 1 == stages ? 0u : s + 1;
@@ -179,10 +191,10 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                         for (uint32_t i = 0; i * 16u < left; ++i)
                             ptx::umma_pair_f16_ts_if(on, tmem, a + i * 8u, b + ((kTokens ? i / 4u * box_bytes + i % 4u * 32u : i * 2048u) >> 4), b_hi, idesc, i ? 1u : accumulate);
                     }
-                    ptx::umma_commit_pair_if(on, empty_bar(s));
+                    ptx::umma_commit_pair_if(on, empty_b(s));
                     accumulate = 1;
                     left -= kWideK;
-                    s = s + 1 == stages ? 0u : s + 1;
+                    s = s + 1 == stages_b ? 0u : s + 1;
                     buffer = buffer + 1 == Cfg::kBuffers ? 0u : buffer + 1;
                     phase ^= buffer == 0 ? 1u : 0u;
                 }
@@ -201,9 +213,8 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const uint32_t ready = rank == 0 ? ready_bar(mine) : ptx::map_to_cta(ready_bar(mine), 0);
         const uint32_t taken = rank == 0 ? taken_bar : ptx::map_to_cta(taken_bar, 0);
         const uint32_t buffer = tmem + lanes + kPairCols4 + mine * Cfg::kBufferCols;
-        // its next step: stage and phase, and whether there was one before, whose MMAs have to leave the buffer
-        uint32_t s = mine, phase = 0, before_s = 0, before_phase = 0, round = 0, skip = mine;
-        while (s >= stages) s -= stages;  // (there are more stages than groups)
+        // its next step's stages and phases, and whether there was one before, whose MMAs have to leave the buffer (there are more stages than groups)
+        uint32_t s = mine, phase = 0, sb = mine, phase_b = 0, before_s = 0, before_phase = 0, round = 0, skip = mine;
         bool alive = true, again = false;
         auto wait = [&](uint32_t bar, uint32_t parity) {
             uint32_t ok = 1;
@@ -214,7 +225,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             const Item w = split_item(p.split, item);
             uint32_t step = w.first + skip;
             for (; step < w.last; step += Cfg::kBuffers) {
-                alive = wait(full_bar(s), phase);
+                alive = wait(full_a(s), phase);
                 if (!alive) break;
                 // the row's 64 bytes, pieces of 16 in the order of the 64-byte swizzle, and its words of scales
                 const uint32_t src = a_addr + s * Cfg::kBytesA + row * 64u, turn = row >> 1 & 3u;
@@ -226,10 +237,12 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 for (uint32_t g = 0; g < (kMx ? 1u : 2u); ++g)
                     if (step * kWideK + g * 64u < p.d.k)
                         four[g] = ptx::ld_shared_u32(s_addr + s * Cfg::kBytesScales + g * 512u + lane * 16u + q * 4u);
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(empty_a(s));
                 const bool two = W::needs_two(four[0]) || W::needs_two(four[1]);
                 const bool any_two = kMx && __any_sync(0xFFFFFFFFu, two);
                 if (again) {
-                    alive = wait(empty_bar(before_s), before_phase);
+                    alive = wait(empty_b(before_s), before_phase);
                     if (!alive) break;
                 }
                 ptx::tcgen05_fence_after_sync();
@@ -253,18 +266,24 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 }
                 ptx::tmem_st_wait();
                 ptx::tcgen05_fence_before_sync();
-                __syncwarp();
+                alive = wait(full_b(sb), phase_b);
+                if (!alive) break;
                 if (lane == 0) {
                     if (rank == 0) ptx::mbar_arrive(ready);
                     else ptx::mbar_arrive_cluster_relaxed(ready);
                 }
                 again = true;
-                before_s = s;
-                before_phase = phase;
+                before_s = sb;
+                before_phase = phase_b;
                 s += Cfg::kBuffers;
-                if (s >= stages) {
-                    s -= stages;
+                if (s >= stages_a) {
+                    s -= stages_a;
                     phase ^= 1u;
+                }
+                sb += Cfg::kBuffers;
+                if (sb >= stages_b) {
+                    sb -= stages_b;
+                    phase_b ^= 1u;
                 }
             }
             if (!alive) break;

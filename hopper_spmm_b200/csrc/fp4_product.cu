@@ -154,7 +154,7 @@ fp4_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(ready_bar(s));
         }
-        const Factor f(*reinterpret_cast<const volatile float *>(p.a_whole), *reinterpret_cast<const volatile float *>(p.b_whole));
+        const Factor f(p.a_whole ? *reinterpret_cast<const volatile float *>(p.a_whole) : 1.f, p.b_whole ? *reinterpret_cast<const volatile float *>(p.b_whole) : 1.f);
         uint32_t ok = 1;
         if (lane == 0) ok = ptx::mbar_wait(done_bar, 0, abort_flag, limit) ? 1u : 0u;
         ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
@@ -218,7 +218,7 @@ int launch_width(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, const Product
 // Tiles of 128 or 256 columns, the scales' blocks being 128 rows long, with fewer columns past the end; a single tile as wide as it has to be.
 Split pair_split(uint32_t m, uint32_t n, uint32_t k, uint32_t pairs) {
     const uint32_t cols = n <= kPairCols4 ? (n + 31u) / 32u * 32u : (n + 127u) / 128u * 128u < (n + 255u) / 256u * 256u ? 128u : 256u;
-    return make_split(m, n, cols, (k + kStageK - 1) / kStageK, 2, 0.45, 256 * kStageK * 9 / 16, pairs);
+    return make_split(m, n, cols, (k + kStageK - 1) / kStageK, 2, 0.45, 0.35, 256 * kStageK * 9 / 16, pairs);
 }
 
 int product_pairs(int device, uint32_t *out) {
@@ -292,8 +292,10 @@ int launch_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *c, in
     ProductParams prm{};
     prm.a_scales = static_cast<const uint8_t *>(a->scales);
     prm.b_scales = static_cast<const uint8_t *>(b->scales);
-    prm.a_whole = a->tensor_scale;
-    prm.b_whole = b->tensor_scale;
+    if (a->format == B200SPMM_NVFP4) {  // (mxfp4 has no scale of the tensor)
+        prm.a_whole = a->tensor_scale;
+        prm.b_whole = b->tensor_scale;
+    }
     prm.m = (uint32_t)a->rows;
     prm.n = (uint32_t)b->rows;
     prm.k = (uint32_t)a->cols;

@@ -218,7 +218,7 @@ fp4_product_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     } else {
         // =========================================================== C
         const uint32_t q = warp & 3u, half = warp >> 2, row = q * 32u + lane, lanes = (q * 32u) << 16;
-        const Factor f(*reinterpret_cast<const volatile float *>(p.a_whole), *reinterpret_cast<const volatile float *>(p.b_whole));
+        const Factor f(p.a_whole ? *reinterpret_cast<const volatile float *>(p.a_whole) : 1.f, p.b_whole ? *reinterpret_cast<const volatile float *>(p.b_whole) : 1.f);
         const uint32_t taken = rank == 0 ? taken_bar : ptx::map_to_cta(taken_bar, 0);
         uint32_t round = 0;
         for (uint32_t item = pair; item < p.split.items; item += n_pairs, ++round) {

@@ -26,8 +26,8 @@ struct Split {
     uint32_t steps;             // of k
 };
 
-// `step_us`: what a step of a tile of 256 columns takes; `step_bytes`: of 256 rows or columns of either operand in a step, the larger.
-inline Split make_split(uint32_t m, uint32_t n, uint32_t cols, uint32_t steps, uint32_t min_steps, double step_us, uint32_t step_bytes, uint32_t pairs) {
+// `step_us`: what a step of a tile of 256 columns takes, `least_us` one of few; `step_bytes`: of 256 rows or columns of either operand in a step, the larger.
+inline Split make_split(uint32_t m, uint32_t n, uint32_t cols, uint32_t steps, uint32_t min_steps, double step_us, double least_us, uint32_t step_bytes, uint32_t pairs) {
     Split s{};
     s.cols = cols;
     s.steps = steps;
@@ -38,12 +38,12 @@ inline Split make_split(uint32_t m, uint32_t n, uint32_t cols, uint32_t steps, u
     const uint32_t fit = (uint32_t)std::max<uint64_t>(4, (48ull << 20) / ((uint64_t)step_bytes * steps));  // of the 126 MB of L2
     const uint32_t groups = (s.inner + fit - 1) / fit;
     s.group = (s.inner + groups - 1) / groups;
-    // Parts of the last round's tiles: as many as make it shortest, their sums' way through memory and the second launch, some 3 us, counted
-    const double tile_us = step_us * steps * cols / kPairCols4, sums_us = (double)rest * kPairRows4 * cols * 8. / 5e6;
+    // Parts of the last round's tiles: as many as make it shortest, their sums' way through memory and the second launch, some 8 us, counted
+    const double tile_us = std::max(least_us, step_us * cols / kPairCols4) * steps, sums_us = (double)rest * kPairRows4 * cols * 8. / 5e6;
     s.parts = 1;
     double best = tile_us;
     for (uint32_t parts = 2; rest && parts <= 32 && parts * min_steps <= steps; ++parts) {
-        const double time = tile_us * ((rest * parts + pairs - 1) / pairs) / parts + sums_us * parts + 3.;
+        const double time = tile_us * ((rest * parts + pairs - 1) / pairs) / parts + sums_us * parts + 8.;
         if (time < best) {
             best = time;
             s.parts = parts;

@@ -164,3 +164,305 @@ def test_product_with_a_dense_matrix(m, n, k, fmt, dtype):
         for out_type, out in [(F32, None), (dtype, None)] + [(dtype, o) for o in outputs(m, n, dtype)]:
             got = A.matmul(B, out, dtype=out_type)
             ref.check_product(got, a, B.double(), 16)
+
+
+# ---------------------------------------------------------------- masks of a kind: infinities, NaN, empty rows, padding
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_nan_blocks_infinities_and_empty_rows(fmt):
+    a, b = normal(300, 400, 1), normal(70, 400, 2)
+    a[5, 17], a[299, 399], a[7] = torch.nan, torch.inf, 0.0
+    b[3, 100], b[64] = -torch.inf, 0.0
+    A, B = hs.fp4_quantize(a, fmt), hs.fp4_quantize(b, fmt)
+    for m, n in ((A, B), (B, A), (A, hs.fp4_quantize(b[:9], fmt))):
+        x, y = ref.matrix_values(m), ref.matrix_values(n)
+        ref.check_product(m.matmul(n), x, y.t(), 64)
+    for n in (1, 9, 70):
+        dense = normal(400, n, 3, BF16)
+        dense[10, 0] = torch.inf
+        want = ref.matrix_values(A) @ dense.double()
+        got = A.matmul(dense)
+        # (an infinity times a code of 0 is NaN, as in any product)
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+        clean = dense.clone()
+        clean[10, 0] = 1.0
+        ref.check_product(A.matmul(clean), ref.matrix_values(A), clean.double(), 16)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_what_lies_in_the_padding_of_scales_does_not_matter(fmt):
+    # rows of scales past the last row, full of NaN
+    x = normal(133, 200, 4)
+    m = hs.fp4_quantize(x, fmt)
+    rows = ref.scale_index(256, (m.scales.numel() // 512 // 2) * 4).cuda()[133:]
+    m.scales[rows.reshape(-1)] = 255 if fmt == "mxfp4" else 127
+    a = ref.matrix_values(m)
+    for n in (3, 40, 150):
+        other = hs.fp4_quantize(normal(n, 200, 5), fmt)
+        ref.check_product(m.matmul(other), a, ref.matrix_values(other).t(), 64)
+        ref.check_product(other.matmul(m), ref.matrix_values(other), a.t(), 64)
+        dense = normal(200, n, 6, BF16)
+        ref.check_product(m.matmul(dense), a, dense.double(), 16)
+    assert torch.equal(m.dequantize(), a.float())
+
+
+@pytest.mark.parametrize("n", [2, 20, 100])
+def test_scales_over_the_whole_range(n):
+    # mxfp4: every power of two that bf16 and fp32 have room for beside the sum; nvfp4: every e4m3 scale and a tensor scale of any number
+    g = torch.Generator().manual_seed(n)
+    for fmt in FORMATS:
+        code = torch.randint(0, 16, (150, 1000), generator=g, dtype=torch.uint8)
+        blocks = -(-1000 // ref.BLOCK[fmt])
+        byte = torch.randint(0, 127, (150, blocks), generator=g, dtype=torch.uint8)
+        if fmt == "mxfp4":  # rows of one size each, 2^-127 to 2^100
+            byte = (torch.arange(150)[:, None] * 227 // 149 + torch.randint(0, 2, (150, blocks), generator=g)).to(torch.uint8)
+        values, scales = ref.pack(code, byte, fmt)
+        m = hs.Fp4Matrix(150, 1000, fmt, values=values.cuda(), scales=scales.cuda(), tensor_scale=torch.tensor([0.0371], device="cuda"))
+        a = ref.matrix_values(m)
+        dense = normal(1000, n, 9, BF16)
+        got, want = m.matmul(dense), a @ dense.double()
+        # (one rounding more: the tensor's scale is no power of two)
+        bound = (a.abs() @ dense.double().abs()) * (80 * 2.0 ** -22 + 2.0 ** -23) + 2.0 ** -148
+        assert ((got.double() - want).abs() <= bound).all()
+        other = hs.fp4_quantize(normal(n, 1000, 8), fmt)
+        got, b = m.matmul(other), ref.matrix_values(other)
+        bound = (a.abs() @ b.abs().t()) * (80 * 2.0 ** -22 + 2.0 ** -23) + 2.0 ** -148
+        assert ((got.double() - a @ b.t()).abs() <= bound).all()
+
+
+# ---------------------------------------------------------------- streams, graphs, workspaces, repetition
+
+def test_the_same_call_gives_the_same_bits():
+    A, B, x = hs.fp4_quantize(normal(1500, 2048, 1)), hs.fp4_quantize(normal(700, 2048, 2)), normal(2048, 300, 3, F16)
+    for f in (lambda: A.matmul(B), lambda: A.matmul(x), lambda: A.matmul(x[:, :7]), lambda: hs.fp4_quantize(x).values):
+        first = f()
+        for _ in range(3):
+            assert torch.equal(f(), first)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_without_a_workspace(fmt):
+    # 74 and some tiles: the last ones are cut along k where there is room for their sums
+    A, x = hs.fp4_quantize(normal(300 * 64, 4096, 1), fmt), normal(4096, 256, 2, BF16)
+    B = hs.fp4_quantize(x.t().contiguous(), fmt)
+    want = A.matmul(x)
+    m = capi.Fp4(A.rows, A.cols, capi.MXFP4 if fmt == "mxfp4" else capi.NVFP4, 0, A.values.data_ptr(), A.scales.data_ptr(), A.tensor_scale.data_ptr())
+    b = capi.Fp4(B.rows, B.cols, m.format, 0, B.values.data_ptr(), B.scales.data_ptr(), B.tensor_scale.data_ptr())
+    stream = torch.cuda.current_stream().cuda_stream
+    for bytes_ in (0, 64):
+        ws = torch.empty(64, dtype=torch.uint8, device="cuda")
+        got = torch.empty_like(want)
+        assert capi.lib().b200spmm_fp4_dense_product(C.byref(m), x.data_ptr(), x.stride(0), 256, capi.T_BF16, 0, got.data_ptr(), 256, capi.T_F32, 0,
+                                                     ws.data_ptr(), bytes_, stream) == capi.OK
+        ref.check_product(got, ref.matrix_values(A), x.double(), 16)
+        assert capi.lib().b200spmm_fp4_product(C.byref(m), C.byref(b), got.data_ptr(), 256, capi.T_F32, 0, ws.data_ptr(), bytes_, stream) == capi.OK
+        ref.check_product(got, ref.matrix_values(A), ref.matrix_values(B).t(), 64)
+        # a B that starts on any element goes in passes of 16 columns then
+        odd = normal(4096, 41, 5, BF16)[:, 1:34]
+        out = torch.empty(A.rows, 33, device="cuda")
+        assert capi.lib().b200spmm_fp4_dense_product(C.byref(m), odd.data_ptr(), odd.stride(0), 33, capi.T_BF16, 0, out.data_ptr(), 33, capi.T_F32, 0,
+                                                     ws.data_ptr(), bytes_, stream) == capi.OK
+        ref.check_product(out, ref.matrix_values(A), odd.double(), 16)
+    assert capi.lib().b200spmm_fp4_status(0, stream) == capi.OK
+
+
+def test_empty_products_and_matrices():
+    for fmt in FORMATS:
+        none, some = hs.fp4_quantize(torch.empty(0, 40, device="cuda"), fmt), hs.fp4_quantize(normal(5, 40, 1), fmt)
+        assert none.matmul(some).shape == (0, 5) and some.matmul(none).shape == (5, 0) and none.dequantize().shape == (0, 40)
+        assert some.matmul(torch.empty(40, 0, dtype=BF16, device="cuda")).shape == (5, 0)
+        flat = hs.fp4_quantize(torch.empty(5, 0, device="cuda"), fmt)
+        assert float(flat.tensor_scale) == 1
+        assert torch.equal(flat.matmul(flat), torch.zeros(5, 5, device="cuda"))
+        assert torch.equal(flat.matmul(torch.empty(0, 3, dtype=BF16, device="cuda"), dtype=BF16), torch.zeros(5, 3, dtype=BF16, device="cuda"))
+        both = hs.fp4_quantize_both(torch.empty(5, 0, device="cuda"), fmt)
+        assert (both[1].rows, both[1].cols) == (0, 5)
+
+
+def test_out_matrices_and_results_are_filled_in_place():
+    m = hs.Fp4Matrix(100, 300)
+    for seed in (1, 2):
+        x = normal(100, 300, seed)
+        assert hs.fp4_quantize(x, out=m) is m
+        check_quantized(m, x)
+        t = hs.Fp4Matrix(300, 100, device=x.device)
+        check_quantized(hs.fp4_quantize(x, axis=0, out=t), x.t())
+    with pytest.raises(ValueError, match="shape"):
+        hs.fp4_quantize(normal(101, 300, 1), out=m)
+    with pytest.raises(ValueError, match="mxfp4"):
+        hs.fp4_quantize(normal(100, 300, 1), "mxfp4", out=m)
+
+
+def test_refusals_on_the_gpu():
+    x = normal(40, 64, 1)
+    m = hs.fp4_quantize(x)
+    for bad in (x.double(), x.int(), x[None], x[:, ::2], x.expand(40, 64)[:1].expand(40, 64), x.cpu()):
+        with pytest.raises(ValueError, match="X must be"):
+            hs.fp4_quantize(bad)
+    for scale in (torch.ones(2, device="cuda"), torch.ones(1), torch.ones(1, dtype=F16, device="cuda"), 1.0):
+        with pytest.raises(ValueError, match="tensor_scale"):
+            hs.fp4_quantize(x, tensor_scale=scale)
+    for bad in (x.t(), x.half(), normal(64, 3, 1), normal(64, 6, 1, F16)[:, ::2], normal(64, 3, 1, F16).cpu(), None):
+        with pytest.raises(ValueError):
+            m.matmul(bad)
+    b = normal(64, 9, 1, F16)
+    for bad in (torch.empty(40, 8, device="cuda"), torch.empty(40, 9), torch.empty(40, 9, dtype=F16, device="cuda"), torch.empty(40, 18, device="cuda")[:, ::2],
+                torch.empty(40, 1, device="cuda").expand(40, 9)):
+        with pytest.raises(ValueError, match="C has"):
+            m.matmul(b, bad, dtype=F32)
+    with pytest.raises(ValueError, match="number of columns"):
+        m.matmul(hs.fp4_quantize(normal(3, 65, 1)))
+    with pytest.raises(ValueError, match="bfloat16"):
+        hs.fp4_quantize(x, "mxfp4").matmul(b)
+    with pytest.raises(capi.SpmmError) as e:
+        hs.Fp4Matrix(40, 64, values=torch.zeros(40 * 32 + 8, dtype=torch.uint8, device="cuda")[8:], scales=m.scales, tensor_scale=m.tensor_scale).dequantize()
+    assert e.value.status == capi.ERR_UNSUPPORTED
+
+
+def test_two_streams_at_once():
+    W, x = hs.fp4_quantize(normal(4096, 2048, 1)), normal(2048, 600, 2, F16)
+    X = hs.fp4_quantize(x.t().contiguous())
+    want = [(W.matmul(x[:, :5]), W.matmul(x), W.matmul(X), hs.fp4_quantize(x).values)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            got.append((W.matmul(x[:, :5], stream=s, sync=False), W.matmul(x, stream=s, sync=False), W.matmul(X, stream=s, sync=False),
+                        hs.fp4_quantize(x, stream=s).values))
+    for s in streams:
+        W.sync(s)
+    torch.cuda.synchronize()
+    for g in got:
+        for a, b in zip(g, want[0]):
+            assert torch.equal(a, b)
+
+
+def test_captured_calls_replay_on_new_inputs():
+    W = hs.fp4_quantize(normal(3000, 1024, 1))
+    x = normal(200, 1024, 2, BF16)
+    scale = torch.tensor([0.25], device="cuda")
+
+    def step():
+        X = hs.fp4_quantize(x)
+        y = W.matmul(X, sync=False)
+        z = W.matmul(x.t()[:, :6], sync=False)
+        a, b = hs.fp4_quantize_both(x, tensor_scale=scale)
+        return y, z, W.matmul(x.t(), dtype=BF16, sync=False), a.dequantize(), b.dequantize(dtype=F16)
+
+    graphs = []
+    for _ in range(2):  # two graphs, whose workspaces are their own
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out))
+    for seed in (3, 4):
+        x.copy_(normal(200, 1024, seed, BF16))
+        want = step()
+        for g, out in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for g, out in graphs:
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch, hopper_spmm_b200 as hs
+x = torch.randn(300, 512, device="cuda").half()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    W = hs.fp4_quantize(x)
+    y, z, v = W.matmul(W, sync=False), W.matmul(x.t()[:, :3], sync=False), W.matmul(x.t(), sync=False)
+g.replay()
+torch.cuda.synchronize()
+V = hs.fp4_quantize(x)
+assert torch.equal(y, V.matmul(V)) and torch.equal(z, V.matmul(x.t()[:, :3])) and torch.equal(v, V.matmul(x.t()))
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+# ---------------------------------------------------------------- together
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tokens", [1, 37, 300])
+def test_two_layers_in_4_bits(tokens, fmt):
+    # up, down, with the activations brought to 4 bits between them: each step against the definition on the values it was given
+    W1, W2 = normal(700, 260, 1, BF16, 0.05), normal(260, 700, 2, BF16, 0.05)
+    x = normal(tokens, 260, 3, BF16)
+    Q1, Q2 = hs.fp4_quantize(W1, fmt), hs.fp4_quantize(W2, fmt)
+    X = hs.fp4_quantize(x, fmt)
+    check_quantized(X, x)
+    h = X.matmul(Q1, dtype=BF16)
+    ref.check_product(h, ref.matrix_values(X), ref.matrix_values(Q1).t(), 64)
+    h = torch.relu(h)
+    H = hs.fp4_quantize(h, fmt)
+    check_quantized(H, h)
+    y = H.matmul(Q2)
+    ref.check_product(y, ref.matrix_values(H), ref.matrix_values(Q2).t(), 64)
+    # the second layer with 16-bit activations
+    z = torch.empty(tokens, 260, dtype=BF16, device="cuda")
+    Q2.matmul(h.t(), z.t())
+    ref.check_product(z.t(), ref.matrix_values(Q2), h.t().double(), 16)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_gradients_of_a_linear_layer(fmt):
+    n, k, m = 90, 150, 210
+    x, w, dy = normal(n, k, 1), normal(m, k, 2, spread=0.1), normal(n, m, 3, spread=0.01)
+    (X, Xt), (W, Wt), (dY, dYt) = (hs.fp4_quantize_both(t, fmt) for t in (x, w, dy))
+    v = ref.matrix_values
+    dx, dw = dY.matmul(Wt), dYt.matmul(Xt)
+    ref.check_product(dx, v(dY), v(Wt).t(), 64)
+    ref.check_product(dw, v(dYt), v(Xt).t(), 64)
+    # against differences of the loss <dy, x wᵀ>, with the values that each product's operands stand for: linear in x and in w, so that a step
+    # of any size gives the gradient along it
+    g = torch.Generator(device="cuda").manual_seed(5)
+    of_x = lambda t: (v(dY) * (t @ v(Wt))).sum()
+    of_w = lambda t: (v(dYt).t() * (v(Xt).t() @ t.t())).sum()
+    for loss, at, grad in ((of_x, x, dx), (of_w, w, dw)):
+        step = torch.randn(at.shape, generator=g, device="cuda", dtype=torch.float64)
+        difference = float(loss(at.double() + step) - loss(at.double()))
+        got = float((grad.double() * step).sum())
+        # fp32 sums of at most 210 products, each addition off by 2^-22 of the sum of magnitudes
+        size = float(((v(dY).abs() @ v(Wt).abs().t() if grad is dx else v(dYt).abs() @ v(Xt).abs().t()) * step.abs()).sum())
+        assert abs(got - difference) <= size * 16 * 2.0 ** -22 + 1e-9 * size
+
+
+def test_offsets_past_32_bits():
+    free, _ = torch.cuda.mem_get_info()
+    if free < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    rows, cols = 70100, 131072  # 4.6 GB of codes; C of it with 8 columns, x of 18 GB
+    g = torch.Generator(device="cuda").manual_seed(1)
+    values = torch.randint(0, 256, (rows, cols // 2), generator=g, dtype=torch.uint8, device="cuda")
+    scales = torch.randint(40, 60, (-(-rows // 128) * (cols // 64) * 512,), generator=g, dtype=torch.uint8, device="cuda")
+    m = hs.Fp4Matrix(rows, cols, values=values, scales=scales, tensor_scale=torch.ones(1, device="cuda"))
+    last = torch.arange(rows - 40, rows)
+    code = torch.stack([values[-40:] & 15, values[-40:] >> 4], 2).view(40, cols)
+    n = cols // 16
+    base = (last // 128) * (n // 4) * 512 + (last % 32) * 16 + (last // 32 % 4) * 4
+    where = base[:, None] + (torch.arange(n) // 4 * 512 + torch.arange(n) % 4)[None, :]
+    a = ref.values(code, scales[where.cuda()], 0, "nvfp4")
+    for k in (3, 40):
+        x = normal(cols, k, 2, F16)
+        ref.check_product(m.matmul(x)[-40:], a, x.double(), 16)
+    other = hs.fp4_quantize(normal(100, cols, 3))
+    ref.check_product(m.matmul(other)[-40:], a, ref.matrix_values(other).t(), 64)
+    ref.check_product(other.matmul(m)[:, -40:], ref.matrix_values(other), a.t(), 64)
+    out = m.dequantize(dtype=F16)
+    assert torch.equal(out[-40:], a.half())
+    again = hs.fp4_quantize(out, tensor_scale=torch.ones(1, device="cuda"))
+    code, byte, _ = ref.quantize(out[-40:], "nvfp4", 0)
+    assert torch.equal(again.values[-40:], ref.pack(code, byte, "nvfp4")[0]) and torch.equal(again.scales[where.cuda()], byte)
+    del again
+    t = hs.fp4_quantize(out, axis=0, tensor_scale=torch.ones(1, device="cuda"))
+    code, byte, _ = ref.quantize(out[:, -9:].t().contiguous(), "nvfp4", 0)
+    assert torch.equal(t.values[-9:], ref.pack(code, byte, "nvfp4")[0])
