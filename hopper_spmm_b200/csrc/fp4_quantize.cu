@@ -207,6 +207,8 @@ constexpr unsigned kClusterCtas = 8, kClusterThreads = 1024;
 template <typename T>
 __global__ void __launch_bounds__(kClusterThreads) quantize_cluster_kernel(const T *__restrict__ x, int64_t ldx, const Dest d) {
     __shared__ uint32_t shared[kClusterThreads / 32], all[kClusterCtas];
+    ptx::cluster_arrive();  // no CTA writes to another one's shared memory before that one runs
+    ptx::cluster_wait();
     ptx::wait_for_grids_before();
     const uint32_t units = max(d.groups * 4u, 1u), at = blockIdx.x * blockDim.x + threadIdx.x, row = at / units, unit = at % units;
     const bool here = row < d.rows;
