@@ -54,23 +54,23 @@ int launch_narrow_columns(const b200spmm_fp4_t *a, const DenseParams &d, cudaStr
 
 // Columns shared out evenly over as few tiles as there can be, 64 at least (fewer take longer: 24 of 28672 x 8192 84 us as 32, 69 as 64); a part has at least four steps: shorter ones are not worth their
 // sums' way through memory.
-Split wide_split(uint32_t m, uint32_t n, uint32_t k, uint32_t pairs) {
-    const uint32_t tiles_n = (n + kPairCols4 - 1) / kPairCols4, cols = std::max(64u, ((n + tiles_n - 1) / tiles_n + 31u) / 32u * 32u);
+Split wide_split(uint32_t m, uint32_t n, uint32_t k, bool exact, uint32_t pairs) {
+    const uint32_t most = exact ? WideCfg::kExactCols : kPairCols4, tiles_n = (n + most - 1) / most, cols = std::max(64u, ((n + tiles_n - 1) / tiles_n + 31u) / 32u * 32u);
     return make_split(m, n, cols, (k + kWideK - 1) / kWideK, 4, 0.55, 0.5, 256 * kWideK * 2, pairs);
 }
 
 // Pairs of CTAs of the wide kernel that the current device runs at once (its instances take the same room).
 int wide_pairs(int device, uint32_t *out) {
     static std::atomic<uint32_t> known[kMaxDevices];
-    return max_pairs(fp4_wide_kernel<__half, false, true>, WideCfg::kThreads, WideCfg::kSmemBytes, known[device], out);
+    return max_pairs(fp4_wide_kernel<__half, false, true, false>, WideCfg::kThreads, WideCfg::kSmemBytes, known[device], out);
 }
 
-template <typename T, bool kMx, bool kTokens>
+template <typename T, bool kMx, bool kTokens, bool kExact>
 int launch_wide(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
     uint32_t pairs = 0;
     const int st = wide_pairs(a->device, &pairs);
     if (st != B200SPMM_OK) return st;
-    auto kernel = fp4_wide_kernel<T, kMx, kTokens>;
+    auto kernel = fp4_wide_kernel<T, kMx, kTokens, kExact>;
     static thread_local int configured = -1;
     if (configured != a->device) {
         B200_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WideCfg::kSmemBytes));
@@ -78,11 +78,11 @@ int launch_wide(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace,
     }
     WideParams prm{};
     prm.d = d;
-    prm.split = wide_split(d.m, d.n, d.k, pairs);
-    if (prm.split.parts > 1 && (!workspace || workspace_bytes < split_workspace(prm.split))) prm.split = wide_split(d.m, d.n, d.k, 1);
+    prm.split = wide_split(d.m, d.n, d.k, kExact, pairs);
+    if (prm.split.parts > 1 && (!workspace || workspace_bytes < split_workspace(prm.split))) prm.split = wide_split(d.m, d.n, d.k, kExact, 1);
     prm.row_blocks = (d.m + 127u) / 128u;
-    prm.stages_a = WideCfg::stages_a(kTokens, prm.split.cols);
-    prm.stages_b = WideCfg::stages_b(kTokens, prm.split.cols);
+    prm.stages_a = WideCfg::stages_a(kTokens, kExact, prm.split.cols);
+    prm.stages_b = WideCfg::stages_b(kTokens, kExact, prm.split.cols);
     prm.partial = workspace;
     B200_CUDA_TRY(status_word(&prm.status));
     prm.wait_limit_ns = kDeviceWaitLimitNs;
@@ -95,7 +95,7 @@ int launch_wide(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace,
         set_last_error_static("a tensor map of a product with a 4-bit matrix could not be made");
         return B200SPMM_ERR_CUDA;
     }
-    B200_CUDA_TRY(launch_after(kernel, dim3(2 * std::min(pairs, prm.split.items)), WideCfg::kThreads, WideCfg::smem_bytes(kTokens, prm.split.cols), 2, stream, ma, mb, prm));
+    B200_CUDA_TRY(launch_after(kernel, dim3(2 * std::min(pairs, prm.split.items)), WideCfg::kThreads, WideCfg::smem_bytes(kTokens, kExact, prm.split.cols), 2, stream, ma, mb, prm));
     if (prm.split.parts > 1)
         B200_CUDA_TRY(launch_after(fp4_join_kernel, dim3((prm.split.items - prm.split.whole) / prm.split.parts, prm.split.cols / 32u), kPairRows4, 0, 1, stream, prm.split,
                                    (const float *)workspace, d.m, d.n, kMx ? (const float *)nullptr : d.whole, (const float *)nullptr, Widen<T, kMx>::kLeft, d.c));
@@ -125,7 +125,11 @@ template <typename T, bool kMx, bool kTokens>
 int launch_dense(const b200spmm_fp4_t *a, const DenseParams &d, uint8_t *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
     const uint64_t rows = kTokens ? d.n : d.k, cols = kTokens ? d.k : d.n, need = aligned_bytes(rows, cols);
     if (d.n <= kNarrowColumns || (!d.b_wide && (!workspace || workspace_bytes < need))) return launch_narrow_columns<T, kMx, kTokens>(a, d, stream);
-    if (d.b_wide) return launch_wide<T, kMx, kTokens>(a, d, reinterpret_cast<float *>(workspace), workspace_bytes, stream);
+    auto wide = [&](const DenseParams &with, uint8_t *ws, uint64_t bytes) {
+        return with.c.type == B200SPMM_T_F32 ? launch_wide<T, kMx, kTokens, true>(a, with, reinterpret_cast<float *>(ws), bytes, stream)
+                                             : launch_wide<T, kMx, kTokens, false>(a, with, reinterpret_cast<float *>(ws), bytes, stream);
+    };
+    if (d.b_wide) return wide(d, workspace, workspace_bytes);
     // no tensor map describes B: a copy that one does goes first into the workspace
     const uint32_t pieces = (uint32_t)aligned_pieces(cols);
     B200_CUDA_TRY(launch_after(fp4_align_kernel, dim3((unsigned)std::min<uint64_t>((rows * pieces + 255u) / 256u, (uint64_t)sm_count() * 8u)), 256, 0, 1, stream,
@@ -134,7 +138,7 @@ int launch_dense(const b200spmm_fp4_t *a, const DenseParams &d, uint8_t *workspa
     with.b = workspace;
     with.ldb = (int64_t)pieces * 8;
     with.b_wide = true;
-    return launch_wide<T, kMx, kTokens>(a, with, reinterpret_cast<float *>(workspace + need), workspace_bytes - need, stream);
+    return wide(with, workspace + need, workspace_bytes - need);
 }
 
 }  // namespace
@@ -145,7 +149,8 @@ int dense_product_workspace(const b200spmm_fp4_t *a, const void *b, int64_t ldb,
     uint32_t pairs = 0;
     const int st = wide_pairs(a->device, &pairs);
     if (st != B200SPMM_OK) return st;
-    *bytes = split_workspace(wide_split((uint32_t)a->rows, (uint32_t)n, (uint32_t)a->cols, pairs));
+    const uint32_t m = (uint32_t)a->rows, k = (uint32_t)a->cols;
+    *bytes = std::max(split_workspace(wide_split(m, (uint32_t)n, k, false, pairs)), split_workspace(wide_split(m, (uint32_t)n, k, true, pairs)));
     if (!is_aligned(b, ldb)) *bytes += aligned_bytes(b_transposed ? (uint64_t)n : a->cols, b_transposed ? a->cols : (uint64_t)n);
     return B200SPMM_OK;
 }

@@ -21,6 +21,10 @@
 //   done      the accumulator of an item is complete (commit, in both CTAs)
 //   taken     all 32 warps have read it (they arrive at the even CTA)
 //
+// The tensor core cuts what it adds to an accumulator off to fp32, which over 512 MMAs (8,192 values of k) leaves sums off by 4e-6 of their
+// size.  That is nothing beside the rounding of a 16-bit C; for an fp32 one (kExact) the accumulator, of up to 128 columns, is emptied
+// every four steps into rounded fp32 sums in shared memory, 4e-7, while a second one fills.
+//
 #pragma once
 
 #include "fp4_split.cuh"
@@ -36,10 +40,11 @@ struct WideCfg {
     static constexpr uint32_t kStageA = kBytesA + kBytesScales, kMinA = 6, kMaxA = 12, kMaxB = 8;  // stages
     static constexpr uint32_t kBuffers = 4, kBufferCols = kWideK / 2;  // of widened A, in tensor memory behind the accumulator
     static constexpr uint32_t kWideners = 16;
-    static_assert(kBuffers == kWideners / 4, "a group of four warps has a buffer of its own");
+    static_assert(kBuffers == kWideners / 4 && kBuffers < kMinA, "a group of four warps has a buffer of its own; a stage's step before was read by the MMAs of four steps ago");
     static constexpr int kWarps = kWideners + 3, kThreads = 32 * kWarps;
     static constexpr uint32_t kTmemCols = 512;
-    static constexpr uint32_t kBarriers = 2 * kMaxA + 2 * kMaxB + kBuffers + 3;
+    static constexpr uint32_t kBarriers = 2 * kMaxA + 2 * kMaxB + kBuffers + 5;
+    static constexpr uint32_t kExactCols = 128, kExactBytes = kExactCols * 128 * 4, kRun = 4;  // kExact: columns, their sums, steps of an accumulator
     static constexpr uint32_t kOtherBytes = 1024 + kBarriers * 8 + 16;
     static constexpr size_t kSmemBytes = 227 * 1024;  // at most
     static_assert(kPairCols4 + kBuffers * kBufferCols <= kTmemCols, "tensor memory of an SM");
@@ -48,15 +53,17 @@ struct WideCfg {
     __host__ __device__ static constexpr uint32_t boxes(bool tokens, uint32_t cols) { return tokens ? 2u : (cols / 2u + 63u) / 64u; }
     __host__ __device__ static constexpr uint32_t b_bytes(bool tokens, uint32_t cols) { return box_bytes(tokens, cols) * boxes(tokens, cols); }
     // Few columns leave room for more stages.
-    static uint32_t stages_b(bool tokens, uint32_t cols) { return std::min<uint32_t>(kMaxB, ((uint32_t)kSmemBytes - kOtherBytes - kMinA * kStageA) / b_bytes(tokens, cols)); }
-    static uint32_t stages_a(bool tokens, uint32_t cols) {
-        return std::min<uint32_t>(kMaxA, ((uint32_t)kSmemBytes - kOtherBytes - stages_b(tokens, cols) * b_bytes(tokens, cols)) / kStageA);
+    static constexpr uint32_t room(bool exact) { return (uint32_t)kSmemBytes - kOtherBytes - (exact ? kExactBytes : 0u); }
+    static uint32_t stages_b(bool tokens, bool exact, uint32_t cols) { return std::min<uint32_t>(kMaxB, (room(exact) - kMinA * kStageA) / b_bytes(tokens, cols)); }
+    static uint32_t stages_a(bool tokens, bool exact, uint32_t cols) {
+        return std::min<uint32_t>(kMaxA, (room(exact) - stages_b(tokens, exact, cols) * b_bytes(tokens, cols)) / kStageA);
     }
-    static size_t smem_bytes(bool tokens, uint32_t cols) {
-        return kOtherBytes + (size_t)stages_a(tokens, cols) * kStageA + (size_t)stages_b(tokens, cols) * b_bytes(tokens, cols);
+    static size_t smem_bytes(bool tokens, bool exact, uint32_t cols) {
+        return kOtherBytes + (exact ? kExactBytes : 0u) + (size_t)stages_a(tokens, exact, cols) * kStageA + (size_t)stages_b(tokens, exact, cols) * b_bytes(tokens, cols);
     }
 };
-static_assert((WideCfg::kSmemBytes - WideCfg::kOtherBytes - WideCfg::kMinA * WideCfg::kStageA) / WideCfg::b_bytes(false, 256) >= 5, "shared memory");
+static_assert((WideCfg::room(true) - WideCfg::kMinA * WideCfg::kStageA) / WideCfg::b_bytes(false, WideCfg::kExactCols) >= 5, "shared memory");
+static_assert((WideCfg::room(false) - WideCfg::kMinA * WideCfg::kStageA) / WideCfg::b_bytes(false, 256) >= 5, "shared memory");
 
 struct WideParams {
     DenseParams d;
@@ -68,7 +75,7 @@ struct WideParams {
     unsigned long long wait_limit_ns;
 };
 
-template <typename T, bool kMx, bool kTokens>
+template <typename T, bool kMx, bool kTokens, bool kExact>
 __global__ void __launch_bounds__(WideCfg::kThreads, 1)
 fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const WideParams p) {
     using Cfg = WideCfg;
@@ -87,7 +94,8 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     auto full_a = [&](uint32_t s) { return bars_addr + 8u * (2 * Cfg::kMaxB + s); };
     auto empty_a = [&](uint32_t s) { return bars_addr + 8u * (2 * Cfg::kMaxB + Cfg::kMaxA + s); };
     auto ready_bar = [&](uint32_t b) { return bars_addr + 8u * (2 * Cfg::kMaxB + 2 * Cfg::kMaxA + b); };
-    const uint32_t done_bar = bars_addr + 8u * (2 * Cfg::kMaxB + 2 * Cfg::kMaxA + Cfg::kBuffers), taken_bar = done_bar + 8u, drain_bar = done_bar + 16u;
+    const uint32_t done_bar = bars_addr + 8u * (2 * Cfg::kMaxB + 2 * Cfg::kMaxA + Cfg::kBuffers), taken_bar = done_bar + 16u, drain_bar = done_bar + 32u;  // done and taken: two, of which kExact uses the second, too
+    float *exact_sums = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(bars) + Cfg::kBarriers * 8 + 16);  // kExact: [column][row]
     volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(bars + Cfg::kBarriers);
     uint32_t *tmem_slot = const_cast<uint32_t *>(abort_flag) + 1;
 
@@ -106,8 +114,10 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             ptx::mbar_init(empty_b(s), 1);
         }
         for (uint32_t b = 0; b < Cfg::kBuffers; ++b) ptx::mbar_init(ready_bar(b), 8);
-        ptx::mbar_init(done_bar, 1);
-        ptx::mbar_init(taken_bar, 2 * Cfg::kWideners);
+        for (uint32_t d = 0; d < 2; ++d) {
+            ptx::mbar_init(done_bar + 8u * d, 1);
+            ptx::mbar_init(taken_bar + 8u * d, 2 * Cfg::kWideners);
+        }
         ptx::mbar_init(drain_bar, 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
@@ -172,33 +182,38 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             // columns a box away.
             const uint64_t b_desc = ptx::make_smem_desc(b_addr, kTokens ? 16u : box_bytes, 1024, ptx::kSwizzle128B);
             const uint32_t b_lo = (uint32_t)b_desc, b_hi = (uint32_t)(b_desc >> 32);
-            uint32_t s = 0, buffer = 0, phase = 0, round = 0;
+            uint32_t s = 0, buffer = 0, phase = 0, round = 0;  // rounds: items, or with kExact runs of four steps
             bool alive = true;
-            for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs, ++round) {
+            for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs) {
                 const Item w = split_item(p.split, item);
-                if (round) alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait_cluster(taken_bar, (round - 1u) & 1u, abort_flag, limit));
-                uint32_t accumulate = 0, left = p.d.k - w.first * kWideK;  // values of k from this step on
-                for (uint32_t step = w.first; alive && step < w.last; ++step) {
-                    alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait_cluster(ready_bar(buffer), phase, abort_flag, limit));
-                    if (!alive) break;
-                    ptx::tcgen05_fence_after_sync();
-                    const uint32_t a = tmem + kPairCols4 + buffer * Cfg::kBufferCols, b = b_lo + s * (bytes_b >> 4);
-                    if (left >= kWideK) {
-                        constexpr uint32_t kNext = kTokens ? 2u : 128u;
-                        ptx::umma_pair_f16_ts_x4_if<kNext>(on, tmem, a, b, b_hi, idesc, accumulate);
-                        ptx::umma_pair_f16_ts_x4_if<kNext>(on, tmem, a + 32u, b + (kTokens ? box_bytes >> 4 : 512u), b_hi, idesc, 1u);
-                    } else {
-                        for (uint32_t i = 0; i * 16u < left; ++i)
-                            ptx::umma_pair_f16_ts_if(on, tmem, a + i * 8u, b + ((kTokens ? i / 4u * box_bytes + i % 4u * 32u : i * 2048u) >> 4), b_hi, idesc, i ? 1u : accumulate);
+                uint32_t left = p.d.k - w.first * kWideK;  // values of k from the next step on
+                for (uint32_t step = w.first; alive && step < w.last; ++round) {
+                    const uint32_t end = kExact ? min(step + Cfg::kRun, w.last) : w.last, which = kExact ? round & 1u : 0u, d = tmem + which * Cfg::kExactCols;
+                    if (kExact ? round >= 2 : round >= 1)
+                        alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait_cluster(taken_bar + 8u * which, (kExact ? (round >> 1) - 1u : round - 1u) & 1u, abort_flag, limit));
+                    uint32_t accumulate = 0;
+                    for (; alive && step < end; ++step) {
+                        alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait_cluster(ready_bar(buffer), phase, abort_flag, limit));
+                        if (!alive) break;
+                        ptx::tcgen05_fence_after_sync();
+                        const uint32_t a = tmem + kPairCols4 + buffer * Cfg::kBufferCols, b = b_lo + s * (bytes_b >> 4);
+                        if (left >= kWideK) {
+                            constexpr uint32_t kNext = kTokens ? 2u : 128u;
+                            ptx::umma_pair_f16_ts_x4_if<kNext>(on, d, a, b, b_hi, idesc, accumulate);
+                            ptx::umma_pair_f16_ts_x4_if<kNext>(on, d, a + 32u, b + (kTokens ? box_bytes >> 4 : 512u), b_hi, idesc, 1u);
+                        } else {
+                            for (uint32_t i = 0; i * 16u < left; ++i)
+                                ptx::umma_pair_f16_ts_if(on, d, a + i * 8u, b + ((kTokens ? i / 4u * box_bytes + i % 4u * 32u : i * 2048u) >> 4), b_hi, idesc, i ? 1u : accumulate);
+                        }
+                        ptx::umma_commit_pair_if(on, empty_b(s));
+                        accumulate = 1;
+                        left -= kWideK;
+                        s = s + 1 == stages_b ? 0u : s + 1;
+                        buffer = buffer + 1 == Cfg::kBuffers ? 0u : buffer + 1;
+                        phase ^= buffer == 0 ? 1u : 0u;
                     }
-                    ptx::umma_commit_pair_if(on, empty_b(s));
-                    accumulate = 1;
-                    left -= kWideK;
-                    s = s + 1 == stages_b ? 0u : s + 1;
-                    buffer = buffer + 1 == Cfg::kBuffers ? 0u : buffer + 1;
-                    phase ^= buffer == 0 ? 1u : 0u;
+                    if (alive) ptx::umma_commit_pair_if(on, done_bar + 8u * which);
                 }
-                if (alive) ptx::umma_commit_pair_if(on, done_bar);
             }
             if (!alive && on) {
                 ptx::umma_commit_pair_local(drain_bar);
@@ -213,140 +228,177 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const uint32_t ready = rank == 0 ? ready_bar(mine) : ptx::map_to_cta(ready_bar(mine), 0);
         const uint32_t taken = rank == 0 ? taken_bar : ptx::map_to_cta(taken_bar, 0);
         const uint32_t buffer = tmem + lanes + kPairCols4 + mine * Cfg::kBufferCols;
-        // its next step's stages and phases, and whether there was one before, whose MMAs have to leave the buffer (there are more stages than groups)
-        uint32_t s = mine, phase = 0, sb = mine, phase_b = 0, before_s = 0, before_phase = 0, round = 0, skip = mine;
+        // its next step's stages and phases, and whether there was one before
+        uint32_t s = mine, phase = 0, sb = mine, phase_b = 0, round = 0;
         bool alive = true, again = false;
         auto wait = [&](uint32_t bar, uint32_t parity) {
             uint32_t ok = 1;
             if (lane == 0) ok = ptx::mbar_wait(bar, parity, abort_flag, limit) ? 1u : 0u;
             return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0u;
         };
-        for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs, ++round) {
-            const Item w = split_item(p.split, item);
-            uint32_t step = w.first + skip;
-            for (; step < w.last; step += Cfg::kBuffers) {
-                alive = wait(full_a(s), phase);
-                if (!alive) break;
-                // the row's 64 bytes, pieces of 16 in the order of the 64-byte swizzle, and its words of scales
-                const uint32_t src = a_addr + s * Cfg::kBytesA + row * 64u, turn = row >> 1 & 3u;
-                uint4 codes[4];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) codes[i] = ptx::ld_shared_v4(src + (i ^ turn) * 16u);
-                uint32_t four[2] = {0u, 0u};  // scales of what lies past the last column: zeros (there is no group that was not loaded)
-#pragma unroll
-                for (uint32_t g = 0; g < (kMx ? 1u : 2u); ++g)
-                    if (step * kWideK + g * 64u < p.d.k)
-                        four[g] = ptx::ld_shared_u32(s_addr + s * Cfg::kBytesScales + g * 512u + lane * 16u + q * 4u);
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(empty_a(s));
-                const bool two = W::needs_two(four[0]) || W::needs_two(four[1]);
-                const bool any_two = kMx && __any_sync(0xFFFFFFFFu, two);
-                if (again) {
-                    alive = wait(empty_b(before_s), before_phase);
-                    if (!alive) break;
-                }
-                ptx::tcgen05_fence_after_sync();
-                auto widen = [&](auto twice, uint32_t h) {
-                    uint32_t out[32];
-#pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i) {  // eight values each
-                        const uint4 &c4 = codes[2 * h + i / 4];
-                        const uint32_t c = i % 4 == 0 ? c4.x : i % 4 == 1 ? c4.y : i % 4 == 2 ? c4.z : c4.w;
-                        const uint32_t sc = W::template scale<decltype(twice)::value>(kMx ? four[0] >> (h * 16u + i / 4u * 8u) & 0xFFu : four[h] >> (i / 2u * 8u) & 0xFFu);
-                        W::template eight<decltype(twice)::value>(c, sc, out + 4 * i);
-                    }
-                    ptx::tmem_st_32x32b_x32(buffer + h * 32u, out);
-                };
-                if (any_two) {
-                    widen(std::true_type(), 0);
-                    widen(std::true_type(), 1);
-                } else {
-                    widen(std::false_type(), 0);
-                    widen(std::false_type(), 1);
-                }
-                ptx::tmem_st_wait();
-                ptx::tcgen05_fence_before_sync();
-                alive = wait(full_b(sb), phase_b);
-                if (!alive) break;
-                if (lane == 0) {
-                    if (rank == 0) ptx::mbar_arrive(ready);
-                    else ptx::mbar_arrive_cluster_relaxed(ready);
-                }
-                again = true;
-                before_s = sb;
-                before_phase = phase_b;
-                s += Cfg::kBuffers;
-                if (s >= stages_a) {
-                    s -= stages_a;
-                    phase ^= 1u;
-                }
-                sb += Cfg::kBuffers;
-                if (sb >= stages_b) {
-                    sb -= stages_b;
-                    phase_b ^= 1u;
-                }
+        auto widen_step = [&](uint32_t step) {
+            // The MMAs of the step four before leave the buffer, and every step up to that one has been read then: the last of A's stage, too,
+            // which were other warps' (without this a warp might be two phases of `full a` behind, which a parity does not tell apart).
+            if (again) {
+                const bool wrapped = sb < Cfg::kBuffers;  // (B's stage of that step)
+                alive = wait(empty_b(wrapped ? sb + stages_b - Cfg::kBuffers : sb - Cfg::kBuffers), wrapped ? phase_b ^ 1u : phase_b);
+                if (!alive) return;
             }
-            if (!alive) break;
-            skip = step - w.last;  // steps of the next item until this warp's
-            alive = wait(done_bar, round & 1u);
-            if (!alive) break;
+            alive = wait(full_a(s), phase);
+            if (!alive) return;
+            // the row's 64 bytes, pieces of 16 in the order of the 64-byte swizzle, and its words of scales
+            const uint32_t src = a_addr + s * Cfg::kBytesA + row * 64u, turn = row >> 1 & 3u;
+            uint32_t four[2] = {0u, 0u};  // scales of what lies past the last column: zeros (there is no group that was not loaded)
+#pragma unroll
+            for (uint32_t g = 0; g < (kMx ? 1u : 2u); ++g)
+                if (step * kWideK + g * 64u < p.d.k)
+                    four[g] = ptx::ld_shared_u32(s_addr + s * Cfg::kBytesScales + g * 512u + lane * 16u + q * 4u);
+            const bool two = W::needs_two(four[0]) || W::needs_two(four[1]);
+            const bool any_two = kMx && __any_sync(0xFFFFFFFFu, two);
             ptx::tcgen05_fence_after_sync();
-            const uint32_t c_row = w.m0 + rank * 128u + row;
-            auto free_accumulator = [&]() {
-                ptx::tcgen05_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) {
-                    if (rank == 0) ptx::mbar_arrive(taken);
-                    else ptx::mbar_arrive_cluster_relaxed(taken);
+            auto widen = [&](auto twice, uint32_t h) {
+                const uint4 lo = ptx::ld_shared_v4(src + ((2u * h) ^ turn) * 16u), hi = ptx::ld_shared_v4(src + ((2u * h + 1u) ^ turn) * 16u);
+                if (h == 1) {
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(empty_a(s));
                 }
+                const uint32_t codes[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                uint32_t out[32];
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {  // eight values each
+                    const uint32_t c = codes[i];
+                    const uint32_t sc = W::template scale<decltype(twice)::value>(kMx ? four[0] >> (h * 16u + i / 4u * 8u) & 0xFFu : four[h] >> (i / 2u * 8u) & 0xFFu);
+                    W::template eight<decltype(twice)::value>(c, sc, out + 4 * i);
+                }
+                ptx::tmem_st_32x32b_x32(buffer + h * 32u, out);
             };
-            auto scaled = [&](uint32_t c, float (&v)[16]) {
-                uint32_t r[16];
-                ptx::tmem_ld_32x32b_x16(tmem + lanes + c, r);
-                ptx::tmem_ld_wait();
-#pragma unroll
-                for (uint32_t i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) * W::kLeft * whole;
-            };
-            if (w.slot == ~0u && p.d.c.type != B200SPMM_T_F32) {
-                // the accumulator as 16-bit numbers to registers first: the next item's MMAs run while they are written
-                uint32_t packed[2][16];
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    const uint32_t c = mine * 32u + j / 2u * 128u;
-                    if (c >= p.split.cols) break;
-                    float v[16];
-                    scaled(c + j % 2u * 16u, v);
-                    pack_row(p.d.c.type, v, packed[j / 2u] + j % 2u * 8u);
-                }
-                free_accumulator();
-#pragma unroll
-                for (uint32_t j = 0; j < 2; ++j) {
-                    const uint32_t c = mine * 32u + j * 128u;
-                    if (c < p.split.cols && w.n0 + c < p.d.n) store_words(p.d.c, c_row - lane, p.d.m, w.n0 + c, p.d.n, packed[j]);
-                }
-                continue;
+            if (any_two) {
+                widen(std::true_type(), 0);
+                widen(std::true_type(), 1);
+            } else {
+                widen(std::false_type(), 0);
+                widen(std::false_type(), 1);
             }
-#pragma unroll 1
-            for (uint32_t j = 0; j < 4; ++j) {
-                const uint32_t c = mine * 32u + j / 2u * 128u + j % 2u * 16u;
-                if (c >= p.split.cols) break;
-                if (w.slot != ~0u) {  // column by column: neighbouring lanes write neighbours
-                    uint32_t r[16];
-                    ptx::tmem_ld_32x32b_x16(tmem + lanes + c, r);
-                    ptx::tmem_ld_wait();
-                    float *dst = p.partial + ((uint64_t)w.slot * p.split.cols + c) * kPairRows4 + rank * 128u + row;
+            ptx::tmem_st_wait();
+            ptx::tcgen05_fence_before_sync();
+            alive = wait(full_b(sb), phase_b);
+            if (!alive) return;
+            if (lane == 0) {
+                if (rank == 0) ptx::mbar_arrive(ready);
+                else ptx::mbar_arrive_cluster_relaxed(ready);
+            }
+            again = true;
+            s += Cfg::kBuffers;
+            if (s >= stages_a) {
+                s -= stages_a;
+                phase ^= 1u;
+            }
+            sb += Cfg::kBuffers;
+            if (sb >= stages_b) {
+                sb -= stages_b;
+                phase_b ^= 1u;
+            }
+        };
+        // The 16 columns from c on of accumulator `which`.
+        auto columns = [&](uint32_t which, uint32_t c, float (&v)[16]) {
+            uint32_t r[16];
+            ptx::tmem_ld_32x32b_x16(tmem + lanes + which * Cfg::kExactCols + c, r);
+            ptx::tmem_ld_wait();
 #pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i) dst[i * kPairRows4] = __uint_as_float(r[i]);
+            for (uint32_t i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+        };
+        auto free_accumulator = [&](uint32_t which) {
+            ptx::tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if (rank == 0) ptx::mbar_arrive(taken + 8u * which);
+                else ptx::mbar_arrive_cluster_relaxed(taken + 8u * which);
+            }
+        };
+        auto store_part = [&](const Item &w, uint32_t c, const float (&v)[16]) {  // column by column: neighbouring lanes write neighbours
+            float *dst = p.partial + ((uint64_t)w.slot * p.split.cols + c) * kPairRows4 + rank * 128u + row;
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) dst[i * kPairRows4] = v[i];
+        };
+        uint32_t before = 0;  // steps of the items before
+        for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs) {
+            const Item w = split_item(p.split, item);
+            const uint32_t c_row0 = w.m0 + rank * 128u + q * 32u, steps = w.last - w.first;
+            if constexpr (kExact) {
+                // a step of each run is this warp's; a run's sums are taken when its step of the next one is under way
+                const uint32_t runs = (steps + Cfg::kRun - 1) / Cfg::kRun;
+                for (uint32_t run = 0; run <= runs; ++run) {
+                    const uint32_t step = run * Cfg::kRun + ((mine - before) & (Cfg::kRun - 1u));
+                    if (run < runs && step < steps) widen_step(w.first + step);
+                    if (!alive) break;
+                    if (run == 0) continue;
+                    alive = wait(done_bar + 8u * (round & 1u), round >> 1 & 1u);
+                    if (!alive) break;
+                    ptx::tcgen05_fence_after_sync();
+#pragma unroll
+                    for (uint32_t j = 0; j < 2; ++j) {
+                        const uint32_t c = mine * 32u + j * 16u;
+                        if (c >= p.split.cols) break;
+                        float v[16];
+                        columns(round & 1u, c, v);
+                        float *sum = exact_sums + c * 128u + row;
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i) {
+                            if (run > 1) v[i] += sum[i * 128u];
+                            if (run < runs) sum[i * 128u] = v[i];
+                        }
+                        if (run < runs) continue;
+                        if (w.slot != ~0u) {
+                            store_part(w, c, v);
+                        } else if (w.n0 + c < p.d.n) {
+                            uint32_t words[16];
+#pragma unroll
+                            for (uint32_t i = 0; i < 16; ++i) words[i] = __float_as_uint(v[i] * W::kLeft * whole);
+                            store_words(p.d.c, c_row0, p.d.m, w.n0 + c, p.d.n, words);
+                        }
+                    }
+                    free_accumulator(round & 1u);
+                    ++round;
+                }
+            } else {
+                for (uint32_t step = (mine - before) & (Cfg::kBuffers - 1u); alive && step < steps; step += Cfg::kBuffers) widen_step(w.first + step);
+                if (!alive) break;
+                alive = wait(done_bar, round & 1u);
+                if (!alive) break;
+                ptx::tcgen05_fence_after_sync();
+                if (w.slot == ~0u) {
+                    // the accumulator as 16-bit numbers to registers first: the next item's MMAs run while they are written
+                    uint32_t packed[2][16];
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const uint32_t c = mine * 32u + j / 2u * 128u;
+                        if (c >= p.split.cols) break;
+                        float v[16];
+                        columns(0, c + j % 2u * 16u, v);
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i) v[i] = v[i] * W::kLeft * whole;
+                        pack_row(p.d.c.type, v, packed[j / 2u] + j % 2u * 8u);
+                    }
+                    free_accumulator(0);
+#pragma unroll
+                    for (uint32_t j = 0; j < 2; ++j) {
+                        const uint32_t c = mine * 32u + j * 128u;
+                        if (c < p.split.cols && w.n0 + c < p.d.n) store_words(p.d.c, c_row0, p.d.m, w.n0 + c, p.d.n, packed[j]);
+                    }
                 } else {
-                    float v[16];
-                    scaled(c, v);
-                    uint32_t words[16];
-#pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i) words[i] = __float_as_uint(v[i]);
-                    if (w.n0 + c < p.d.n) store_words(p.d.c, c_row - lane, p.d.m, w.n0 + c, p.d.n, words);
+#pragma unroll 1
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const uint32_t c = mine * 32u + j / 2u * 128u + j % 2u * 16u;
+                        if (c >= p.split.cols) break;
+                        float v[16];
+                        columns(0, c, v);
+                        store_part(w, c, v);
+                    }
+                    free_accumulator(0);
                 }
+                ++round;
             }
-            free_accumulator();
+            before += steps;
         }
     }
     __syncwarp();

@@ -183,8 +183,11 @@ fp4_product_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
             for (uint32_t step = w.first; step < w.last; ++step, ++it) {
                 if ((it & 1u) != mine) continue;
                 const uint32_t s = it % kStages;
+                // The stage's last step was the other four warps', so that this warp may be two phases of `full` behind, which a parity does not
+                // tell apart: it waits for that step's MMAs first, as the load did.
+                const uint32_t phase = it / kStages & 1u;
                 uint32_t ok = 1;
-                if (lane == 0) ok = ptx::mbar_wait(full_bar(s), it / kStages & 1u, abort_flag, limit) ? 1u : 0u;
+                if (lane == 0) ok = (it < kStages || ptx::mbar_wait(empty_bar(s), phase ^ 1u, abort_flag, limit)) && ptx::mbar_wait(full_bar(s), phase, abort_flag, limit) ? 1u : 0u;
                 alive = __shfl_sync(0xFFFFFFFFu, ok, 0) != 0u;
                 if (!alive) break;
                 // A stage's scales have columns of their own: they are overwritten when the stage is, after its MMAs.  (Groups that were

@@ -466,3 +466,49 @@ def test_offsets_past_32_bits():
     t = hs.fp4_quantize(out, axis=0, tensor_scale=torch.ones(1, device="cuda"))
     code, byte, _ = ref.quantize(out[:, -9:].t().contiguous(), "nvfp4", 0)
     assert torch.equal(t.values[-9:], ref.pack(code, byte, "nvfp4")[0])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_sums_of_fp32_results(fmt):
+    # An MMA cuts its sum off to fp32, at most 2^-23 of it, and sums in fp32 are taken over from the tensor core after at most 32 of them (512
+    # values of k; the product of two 4-bit matrices and one of few columns: their MMAs cover 64 and 16 and are followed below).  Over a run of
+    # random values the sum grows with the root, the mean of which is 2/3 of its last value: 32 * 2/3 * 2^-23, and the errors of different
+    # runs, of either sign, add like the runs themselves.  16 rounded additions of runs: at most 16 * 2^-24 more.
+    k = 8192
+    w = normal(700, k, 1, spread=k ** -0.5)
+    W = hs.fp4_quantize(w, fmt)
+    a = ref.matrix_values(W)
+    for n in (40, 100, 300):
+        for dtype in (F16, BF16) if fmt == "nvfp4" else (BF16,):
+            x = normal(k, n, 2, dtype)
+            want = a @ x.double()
+            error = float((W.matmul(x, dtype=F32).double() - want).norm() / want.norm())
+            assert error <= (32 * 2 / 3 + 8) * 2.0 ** -23, (n, dtype, error)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_operands_larger_than_the_cache(fmt):
+    # What is read from memory arrives in another order than it was asked for; every run has the same sums, whichever side is the long one.
+    rows, cols = 40100, 32768
+    g = torch.Generator(device="cuda").manual_seed(1)
+    values = torch.randint(0, 256, (rows, cols // 2), generator=g, dtype=torch.uint8, device="cuda")
+    low, high, per = (40, 60, 64) if fmt == "nvfp4" else (118, 128, 128)
+    scales = torch.randint(low, high, (-(-rows // 128) * (cols // per) * 512,), generator=g, dtype=torch.uint8, device="cuda")
+    whole = {"tensor_scale": torch.ones(1, device="cuda")} if fmt == "nvfp4" else {"format": fmt}
+    m = hs.Fp4Matrix(rows, cols, values=values, scales=scales, **whole)
+    other = hs.fp4_quantize(normal(100, cols, 3), fmt)
+    dense = F16 if fmt == "nvfp4" else BF16
+    x = other.dequantize(dtype=dense).t()
+    at = torch.arange(0, rows, 97, device="cuda")
+    a = m.dequantize()[at].double()
+    for n in (20, 100):
+        small = other if n == 100 else hs.fp4_quantize(normal(n, cols, 4), fmt)
+        got = m.matmul(small)
+        ref.check_product(got[at], a, ref.matrix_values(small).t(), 64)
+        for _ in range(6):
+            assert torch.equal(m.matmul(small), got) and torch.equal(small.matmul(m), got.t())
+    for n, dtype in ((3, dense), (40, dense), (100, dense), (100, F32)):
+        got = m.matmul(x[:, :n], dtype=dtype)
+        ref.check_product(got[at], a, x[:, :n].double(), 16)
+        for _ in range(6):
+            assert torch.equal(m.matmul(x[:, :n], dtype=dtype), got)
