@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + kNarrowLoaders), 1) fp4_n
         ptx::cp_async_wait_group<0>();
     } else if (warp < consumers) {
         const uint32_t mine = warp / p.slices, slice = warp % p.slices, r_of_g = (g >> 1) | (g & 1u) << 2;
-        const float left = W::kLeft * (kMx ? 1.f : *reinterpret_cast<const volatile float *>(p.d.whole));
+        const LeftOver rest(W::kLeft, kMx ? 1.f : *reinterpret_cast<const volatile float *>(p.d.whole));
         for (uint32_t tile0 = tile_begin; alive && tile0 < tile_end; tile0 += p.at_once) {
             const uint32_t m0 = tile0 * 16u, row = m0 + mine * 16u + r_of_g;
             const bool busy = tile0 + mine < tile_end;
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + kNarrowLoaders), 1) fp4_n
                     const uint32_t r = i % 16u, col = i / 16u % kCols, tile = i / (16u * kCols);
                     float v[1] = {0.f};
                     for (uint32_t z = 0; z < p.slices; ++z) v[0] += sums[((tile * p.slices + z) * kCols + col) * 16u + r];
-                    v[0] *= left;
+                    v[0] = rest.apply(v[0]);
                     const uint32_t c_row = m0 + tile * 16u + r;
                     if (tile0 + tile < tile_end && c_row < p.d.m && n0 + col < p.d.n) store_row(p.d.c, c_row, n0 + col, p.d.n, v);
                 }
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + kNarrowLoaders), 1) fp4_n
 #pragma unroll
                     for (uint32_t e = 0; e < 4; ++e) {
                         const uint32_t col = n0 + nb * 8u + t * 2u + (e & 1u), c_row = row + (e >> 1) * 8u;
-                        float v[1] = {acc[nb][e] * left};
+                        float v[1] = {rest.apply(acc[nb][e])};
                         if (c_row < p.d.m && col < p.d.n) store_row(p.d.c, c_row, col, p.d.n, v);
                     }
             }

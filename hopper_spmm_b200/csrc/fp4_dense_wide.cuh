@@ -224,7 +224,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         // =========================================================== widening, and C
         const uint32_t q = warp & 3u, mine = warp >> 2, row = q * 32u + lane;
         const uint32_t lanes = (q * 32u) << 16;
-        const float whole = (kMx ? 1.f : *reinterpret_cast<const volatile float *>(p.d.whole));
+        const LeftOver rest(W::kLeft, kMx ? 1.f : *reinterpret_cast<const volatile float *>(p.d.whole));
         const uint32_t ready = rank == 0 ? ready_bar(mine) : ptx::map_to_cta(ready_bar(mine), 0);
         const uint32_t taken = rank == 0 ? taken_bar : ptx::map_to_cta(taken_bar, 0);
         const uint32_t buffer = tmem + lanes + kPairCols4 + mine * Cfg::kBufferCols;
@@ -353,7 +353,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                         } else if (w.n0 + c < p.d.n) {
                             uint32_t words[16];
 #pragma unroll
-                            for (uint32_t i = 0; i < 16; ++i) words[i] = __float_as_uint(v[i] * W::kLeft * whole);
+                            for (uint32_t i = 0; i < 16; ++i) words[i] = __float_as_uint(rest.apply(v[i]));
                             store_words(p.d.c, c_row0, p.d.m, w.n0 + c, p.d.n, words);
                         }
                     }
@@ -376,7 +376,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                         float v[16];
                         columns(0, c + j % 2u * 16u, v);
 #pragma unroll
-                        for (uint32_t i = 0; i < 16; ++i) v[i] = v[i] * W::kLeft * whole;
+                        for (uint32_t i = 0; i < 16; ++i) v[i] = rest.apply(v[i]);
                         pack_row(p.d.c.type, v, packed[j / 2u] + j % 2u * 8u);
                     }
                     free_accumulator(0);

@@ -32,8 +32,8 @@ struct ProductCfg {
     static constexpr uint32_t kBytesA = kTileM * kStageK / 2, kBytesB = kN * kStageK / 2;
     static constexpr uint32_t kScaleBytesA = kGroupsPerStage * 512, kScaleBytesB = kScaleBytesA;
     static constexpr uint32_t kStageBytes = kBytesA + kBytesB + kScaleBytesA + kScaleBytesB;
-    static constexpr uint32_t kPerSm = kN <= 64 ? 2 : 1;                       // resident blocks
-    static constexpr uint32_t kStages = (kPerSm == 2 ? 110u * 1024u : 220u * 1024u) / kStageBytes < 6 ? (kPerSm == 2 ? 110u * 1024u : 220u * 1024u) / kStageBytes : 6;
+    static constexpr uint32_t kPerSm = 2;                                      // resident blocks
+    static constexpr uint32_t kStages = 110u * 1024u / kStageBytes < 6 ? 110u * 1024u / kStageBytes : 6;
     static constexpr uint32_t kScaleCols = kGroupsPerStage * 8;  // tensor memory columns of a stage's scales
     static constexpr uint32_t kNeedCols = kN + kStages * kScaleCols;
     static constexpr uint32_t kTmemCols = kNeedCols <= 64 ? 64 : kNeedCols <= 128 ? 128 : kNeedCols <= 256 ? 256 : 512;

@@ -102,5 +102,13 @@ template <typename T, bool kMx> struct Widen {
     }
 };
 
+// What a sum still lacks: the power of two that Widen left, 1 at least, and the tensor's scale.  In this order no step leaves fp32's range unless
+// the result does.
+struct LeftOver {
+    float first, second;
+    B200_DEVICE LeftOver(float left, float whole) : first(whole < 1.f ? whole * left : left), second(whole < 1.f ? 1.f : whole) {}
+    B200_DEVICE float apply(float v) const { return v * first * second; }
+};
+
 }  // namespace fp4
 }  // namespace b200spmm

@@ -54,6 +54,8 @@ def _type_code(dtype):
 def _on(stream, *tensors):
     """Work and new tensors on `stream`, which the caching allocator is told about for the tensors of the call."""
     import torch
+    if any(getattr(t, "device", stream.device) != stream.device for t in tensors):
+        raise ValueError("the stream and the tensors must be on one device")
     with torch.cuda.stream(stream):
         yield
     for t in tensors:
@@ -66,7 +68,7 @@ class Fp4Matrix:
     tensors in the layout that include/b200_spmm.h describes: give them (a checkpoint in that layout), or leave them
     out for a matrix that ``fp4_quantize(..., out=)`` fills."""
 
-    __slots__ = ("rows", "cols", "format", "values", "scales", "tensor_scale", "_m")
+    __slots__ = ("format", "_m")  # the format's name; values, scales, tensor_scale, rows, cols, the format's code
 
     def __init__(self, rows: int, cols: int, format: str = "nvfp4", *, values=None, scales=None, tensor_scale=None, device=None):
         import torch
@@ -94,9 +96,14 @@ class Fp4Matrix:
                     not (values.is_contiguous() and scales.is_contiguous())):
                 raise ValueError(f"a {rows} x {cols} {format} matrix takes contiguous uint8 values of {rows * pitch} bytes and scales of "
                                  f"{n_scales} bytes, and one float32 tensor_scale")
-        self.rows, self.cols, self.format = rows, cols, format
-        self.values, self.scales, self.tensor_scale = values, scales, tensor_scale
+        self.format = format
         self._m = (values, scales, tensor_scale, rows, cols, FORMATS[format])
+
+    values = property(lambda self: self._m[0])
+    scales = property(lambda self: self._m[1])
+    tensor_scale = property(lambda self: self._m[2])
+    rows = property(lambda self: self._m[3])
+    cols = property(lambda self: self._m[4])
 
     @property
     def device(self):
@@ -153,8 +160,7 @@ class Fp4Matrix:
 def _matrix(rows, cols, format, values, scales, tensor_scale) -> Fp4Matrix:
     """Arrays that were made for it (the checks of Fp4Matrix cost as much as a launch)."""
     m = object.__new__(Fp4Matrix)
-    m.rows, m.cols, m.format = rows, cols, format
-    m.values, m.scales, m.tensor_scale = values, scales, tensor_scale
+    m.format = format
     m._m = (values, scales, tensor_scale, rows, cols, FORMATS[format])
     return m
 

@@ -143,3 +143,21 @@ def test_the_reference_stores_what_it_reads(fmt):
     blk = ref.BLOCK[fmt]
     top = torch.nn.functional.pad(x.abs(), (0, -77 % blk)).view(200, -1, blk).amax(2).repeat_interleave(blk, 1)[:, :77]
     assert (off <= top.double() * (17 / 96 if fmt == "nvfp4" else 1 / 4) * 1.0001).all()
+
+
+def test_a_stream_of_another_device_is_refused():
+    class Stream:
+        device = torch.device("cuda", 1)
+    x, one = torch.zeros(4, 20), torch.ones(1)
+    m = hs.Fp4Matrix(4, 20, values=torch.zeros(64, dtype=torch.uint8), scales=torch.zeros(512, dtype=torch.uint8), tensor_scale=one)
+    for call in (lambda: hs.fp4_quantize(x, stream=Stream()), lambda: hs.fp4_quantize_both(x, stream=Stream()), lambda: hs.fp4_quantize(x, out=m, stream=Stream()),
+                 lambda: m.dequantize(stream=Stream()), lambda: m.matmul(x.t().half(), stream=Stream()), lambda: m.matmul(m, stream=Stream())):
+        with pytest.raises(ValueError, match="one device"):
+            call()
+
+
+def test_the_arrays_of_a_matrix_are_not_exchanged():
+    m = hs.Fp4Matrix(4, 20, values=torch.zeros(64, dtype=torch.uint8), scales=torch.zeros(512, dtype=torch.uint8), tensor_scale=torch.ones(1))
+    for name in ("values", "scales", "tensor_scale", "rows", "cols"):
+        with pytest.raises(AttributeError):
+            setattr(m, name, getattr(m, name))

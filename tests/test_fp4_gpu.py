@@ -512,3 +512,23 @@ def test_operands_larger_than_the_cache(fmt):
         ref.check_product(got[at], a, x[:, :n].double(), 16)
         for _ in range(6):
             assert torch.equal(m.matmul(x[:, :n], dtype=dtype), got)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
+def test_tensor_scales_at_the_ends_of_their_range(dtype):
+    # the result is an ordinary number, the other operand makes up for the scale; 64 products of magnitudes that fp32 holds
+    for whole, size in ((2.0 ** -126, 1e35), (2.0 ** 127, 1e-37), (1.5 * 2.0 ** -140, 1e35), (1.5 * 2.0 ** 125, 1e-37)):
+        if dtype == F16:
+            size = 100.0 if size > 1 else 1e-5
+        W = hs.fp4_quantize(normal(200, 64, 1, spread=4), tensor_scale=torch.ones(1, device="cuda"))
+        a = ref.matrix_values(W)
+        W.tensor_scale.fill_(whole)
+        for n in (1, 16, 40, 300):
+            g = torch.Generator(device="cuda").manual_seed(n)
+            x = (torch.randn(64, n, generator=g, device="cuda") * size).to(dtype)
+            got, want, mag = W.matmul(x).double(), a @ x.double() * whole, a.abs() @ x.double().abs() * whole
+            # sums of at most 16 additions and two roundings of the scales, in fp32, whose numbers end at 2^-149; where they end is infinity
+            bound = mag * 18 * 2.0 ** -22 + 2.0 ** -148
+            inf = want.abs() > 3.4e38
+            assert torch.equal(got.isinf(), inf) and not got.isnan().any()
+            assert bool(((got - want).abs() <= bound)[~inf].all()), (whole, n)
