@@ -299,10 +299,10 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 phase_b ^= 1u;
             }
         };
-        // The 16 columns from c on of accumulator `which`.
-        auto columns = [&](uint32_t which, uint32_t c, float (&v)[16]) {
+        // The accumulator's 16 columns from c on.
+        auto columns = [&](uint32_t c, float (&v)[16]) {
             uint32_t r[16];
-            ptx::tmem_ld_32x32b_x16(tmem + lanes + which * Cfg::kExactCols + c, r);
+            ptx::tmem_ld_32x32b_x16(tmem + lanes + c, r);
             ptx::tmem_ld_wait();
 #pragma unroll
             for (uint32_t i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
@@ -336,29 +336,33 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     if (!alive) break;
                     ptx::tcgen05_fence_after_sync();
 #pragma unroll
-                    for (uint32_t j = 0; j < 2; ++j) {
-                        const uint32_t c = mine * 32u + j * 16u;
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const uint32_t c = mine * 32u + j * 8u;
                         if (c >= p.split.cols) break;
-                        float v[16];
-                        columns(round & 1u, c, v);
+                        uint32_t r[8];
+                        ptx::tmem_ld_32x32b_x8(tmem + lanes + (round & 1u) * Cfg::kExactCols + c, r);
+                        ptx::tmem_ld_wait();
                         float *sum = exact_sums + c * 128u + row;
 #pragma unroll
-                        for (uint32_t i = 0; i < 16; ++i) {
-                            if (run > 1) v[i] += sum[i * 128u];
-                            if (run < runs) sum[i * 128u] = v[i];
-                        }
-                        if (run < runs) continue;
-                        if (w.slot != ~0u) {
-                            store_part(w, c, v);
-                        } else if (w.n0 + c < p.d.n) {
-                            uint32_t words[16];
-#pragma unroll
-                            for (uint32_t i = 0; i < 16; ++i) words[i] = __float_as_uint(rest.apply(v[i]));
-                            store_words(p.d.c, c_row0, p.d.m, w.n0 + c, p.d.n, words);
-                        }
+                        for (uint32_t i = 0; i < 8; ++i) sum[i * 128u] = run > 1 ? sum[i * 128u] + __uint_as_float(r[i]) : __uint_as_float(r[i]);
                     }
                     free_accumulator(round & 1u);
                     ++round;
+                }
+                if (!alive) break;
+#pragma unroll 1
+                for (uint32_t c = mine * 32u; c < min(mine * 32u + 32u, p.split.cols); c += 16u) {
+                    float v[16];
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i) v[i] = exact_sums[(c + i) * 128u + row];
+                    if (w.slot != ~0u) {
+                        store_part(w, c, v);
+                    } else if (w.n0 + c < p.d.n) {
+                        uint32_t words[16];
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i) words[i] = __float_as_uint(rest.apply(v[i]));
+                        store_words(p.d.c, c_row0, p.d.m, w.n0 + c, p.d.n, words);
+                    }
                 }
             } else {
                 for (uint32_t step = (mine - before) & (Cfg::kBuffers - 1u); alive && step < steps; step += Cfg::kBuffers) widen_step(w.first + step);
@@ -374,7 +378,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                         const uint32_t c = mine * 32u + j / 2u * 128u;
                         if (c >= p.split.cols) break;
                         float v[16];
-                        columns(0, c + j % 2u * 16u, v);
+                        columns(c + j % 2u * 16u, v);
 #pragma unroll
                         for (uint32_t i = 0; i < 16; ++i) v[i] = rest.apply(v[i]);
                         pack_row(p.d.c.type, v, packed[j / 2u] + j % 2u * 8u);
@@ -391,7 +395,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                         const uint32_t c = mine * 32u + j / 2u * 128u + j % 2u * 16u;
                         if (c >= p.split.cols) break;
                         float v[16];
-                        columns(0, c, v);
+                        columns(c, v);
                         store_part(w, c, v);
                     }
                     free_accumulator(0);

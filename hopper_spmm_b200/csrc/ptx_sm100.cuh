@@ -235,6 +235,11 @@ B200_DEVICE void tmem_dealloc(uint32_t taddr, uint32_t n_cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(n_cols) : "memory");
 }
 
+// 32 lanes x 8 consecutive 32-bit columns.
+B200_DEVICE void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+}
 // 32 lanes x 16 consecutive 32-bit columns: thread i of the warp receives lane
 // (taddr.lane + i), columns taddr.col .. +15.  A warp may only touch the 32 lanes of its own
 // quarter: lanes 32*(warp_id % 4) .. +31.

@@ -488,7 +488,8 @@ def test_sums_of_fp32_results(fmt):
 
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_operands_larger_than_the_cache(fmt):
-    # What is read from memory arrives in another order than it was asked for; every run has the same sums, whichever side is the long one.
+    # What is read from memory arrives in another order than it was asked for; every run has the same sums.  (With the sides exchanged tiles
+    # are others, k is cut elsewhere, and fp32 sums add up in another order: that result has its own bound.)
     rows, cols = 40100, 32768
     g = torch.Generator(device="cuda").manual_seed(1)
     values = torch.randint(0, 256, (rows, cols // 2), generator=g, dtype=torch.uint8, device="cuda")
@@ -503,10 +504,11 @@ def test_operands_larger_than_the_cache(fmt):
     a = m.dequantize()[at].double()
     for n in (20, 100):
         small = other if n == 100 else hs.fp4_quantize(normal(n, cols, 4), fmt)
-        got = m.matmul(small)
+        got, other_way = m.matmul(small), small.matmul(m)
         ref.check_product(got[at], a, ref.matrix_values(small).t(), 64)
+        ref.check_product(other_way[:, at], ref.matrix_values(small), a.t(), 64)
         for _ in range(6):
-            assert torch.equal(m.matmul(small), got) and torch.equal(small.matmul(m), got.t())
+            assert torch.equal(m.matmul(small), got) and torch.equal(small.matmul(m), other_way)
     for n, dtype in ((3, dense), (40, dense), (100, dense), (100, F32)):
         got = m.matmul(x[:, :n], dtype=dtype)
         ref.check_product(got[at], a, x[:, :n].double(), 16)
