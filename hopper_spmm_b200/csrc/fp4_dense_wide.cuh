@@ -40,7 +40,7 @@ struct WideCfg {
     static constexpr uint32_t kStageA = kBytesA + kBytesScales, kMinA = 6, kMaxA = 12, kMaxB = 8;  // stages
     static constexpr uint32_t kBuffers = 4, kBufferCols = kWideK / 2;  // of widened A, in tensor memory behind the accumulator
     static constexpr uint32_t kWideners = 16;
-    static_assert(kBuffers == kWideners / 4 && kBuffers < kMinA, "a group of four warps has a buffer of its own; a stage's step before was read by the MMAs of four steps ago");
+    static_assert(kBuffers == kWideners / 4 && kBuffers < kMinA, "a group of four warps has a buffer of its own");
     static constexpr int kWarps = kWideners + 3, kThreads = 32 * kWarps;
     static constexpr uint32_t kTmemCols = 512;
     static constexpr uint32_t kBarriers = 2 * kMaxA + 2 * kMaxB + kBuffers + 5;
@@ -231,20 +231,11 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         // its next step's stages and phases, and whether there was one before
         uint32_t s = mine, phase = 0, sb = mine, phase_b = 0, round = 0;
         bool alive = true, again = false;
-        auto wait = [&](uint32_t bar, uint32_t parity) {
-            uint32_t ok = 1;
-            if (lane == 0) ok = ptx::mbar_wait(bar, parity, abort_flag, limit) ? 1u : 0u;
-            return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0u;
-        };
+        auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, ptx::mbar_wait(bar, parity, abort_flag, limit)) != 0; };
         auto widen_step = [&](uint32_t step) {
-            // The MMAs of the step four before leave the buffer, and every step up to that one has been read then: the last of A's stage, too,
-            // which were other warps' (without this a warp might be two phases of `full a` behind, which a parity does not tell apart).
-            if (again) {
-                const bool wrapped = sb < Cfg::kBuffers;  // (B's stage of that step)
-                alive = wait(empty_b(wrapped ? sb + stages_b - Cfg::kBuffers : sb - Cfg::kBuffers), wrapped ? phase_b ^ 1u : phase_b);
-                if (!alive) return;
-            }
-            alive = wait(full_a(s), phase);
+            // The stage's last step was other warps', so that this one might be two phases of `full a` behind, which a parity does not tell
+            // apart: that step's warps have read it first, as for the load.
+            alive = wait(empty_a(s), phase ^ 1u) && wait(full_a(s), phase);
             if (!alive) return;
             // the row's 64 bytes, pieces of 16 in the order of the 64-byte swizzle, and its words of scales
             const uint32_t src = a_addr + s * Cfg::kBytesA + row * 64u, turn = row >> 1 & 3u;
@@ -255,7 +246,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     four[g] = ptx::ld_shared_u32(s_addr + s * Cfg::kBytesScales + g * 512u + lane * 16u + q * 4u);
             const bool two = W::needs_two(four[0]) || W::needs_two(four[1]);
             const bool any_two = kMx && __any_sync(0xFFFFFFFFu, two);
-            ptx::tcgen05_fence_after_sync();
+            uint32_t out[32];
             auto widen = [&](auto twice, uint32_t h) {
                 const uint4 lo = ptx::ld_shared_v4(src + ((2u * h) ^ turn) * 16u), hi = ptx::ld_shared_v4(src + ((2u * h + 1u) ^ turn) * 16u);
                 if (h == 1) {
@@ -263,26 +254,32 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     if (lane == 0) ptx::mbar_arrive(empty_a(s));
                 }
                 const uint32_t codes[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                uint32_t out[32];
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) {  // eight values each
                     const uint32_t c = codes[i];
                     const uint32_t sc = W::template scale<decltype(twice)::value>(kMx ? four[0] >> (h * 16u + i / 4u * 8u) & 0xFFu : four[h] >> (i / 2u * 8u) & 0xFFu);
                     W::template eight<decltype(twice)::value>(c, sc, out + 4 * i);
                 }
-                ptx::tmem_st_32x32b_x32(buffer + h * 32u, out);
             };
-            if (any_two) {
-                widen(std::true_type(), 0);
-                widen(std::true_type(), 1);
-            } else {
-                widen(std::false_type(), 0);
-                widen(std::false_type(), 1);
+            // half of it before the buffer is free
+            if (any_two) widen(std::true_type(), 0);
+            else widen(std::false_type(), 0);
+            if (again) {  // the MMAs of the step four before leave the buffer
+                const bool wrapped = sb < Cfg::kBuffers;  // (B's stage of that step)
+                alive = wait(empty_b(wrapped ? sb + stages_b - Cfg::kBuffers : sb - Cfg::kBuffers), wrapped ? phase_b ^ 1u : phase_b);
+                if (!alive) return;
             }
-            ptx::tmem_st_wait();
-            ptx::tcgen05_fence_before_sync();
+            ptx::tcgen05_fence_after_sync();
+            ptx::tmem_st_32x32b_x32(buffer, out);
+            if (any_two) widen(std::true_type(), 1);
+            else widen(std::false_type(), 1);
+            ptx::tmem_st_32x32b_x32(buffer + 32u, out);
+            // (B's stage was last that of a step that is done by now, at least as old as the one waited for)
             alive = wait(full_b(sb), phase_b);
             if (!alive) return;
+            ptx::tmem_st_wait();
+            ptx::tcgen05_fence_before_sync();
+            __syncwarp();
             if (lane == 0) {
                 if (rank == 0) ptx::mbar_arrive(ready);
                 else ptx::mbar_arrive_cluster_relaxed(ready);
