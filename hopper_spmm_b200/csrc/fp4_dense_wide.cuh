@@ -10,7 +10,8 @@
 //
 // A step is 128 values of k.  Warps 0-15 of a CTA widen: lane = row of the warp's quarter of tensor memory, warps 4 g .. 4 g + 3
 // every fourth step, so that what a step has to wait for (its stage, its way to tensor memory) overlaps with three others;
-// after an item's last step they take the accumulator to C.  Warp 16 of the even CTA issues the MMAs, warps 17 and 18 load.
+// after an item's last step they take the accumulator to C.  Warp 16 of the even CTA issues the MMAs, warps 17 and 18 load.  Up to 128
+// columns, where issuing a step's MMAs takes longer than they do, warp 19 issues those of every second step, to an accumulator of its own.
 //
 // A and B have stages of their own: those of A, which comes from memory, are free again as soon as they have been read.
 //
@@ -18,7 +19,7 @@
 //   empty a   the four warps that widen it have read it
 //   ready[g]  group g's buffer of widened A is written in both CTAs, and B's stage is there (eight warps arrive at the even CTA)
 //   empty b   the MMAs of the step are done (commit, in both CTAs): the stage of B and the buffer of widened A are free
-//   done      the accumulator of an item is complete (commit, in both CTAs)
+//   done      the accumulators of an item are complete (commits, in both CTAs)
 //   taken     all 32 warps have read it (they arrive at the even CTA)
 //
 // The tensor core cuts what it adds to an accumulator off to fp32, which over 512 MMAs (8,192 values of k) leaves sums off by 4e-6 of their
@@ -41,9 +42,10 @@ struct WideCfg {
     static constexpr uint32_t kBuffers = 4, kBufferCols = kWideK / 2;  // of widened A, in tensor memory behind the accumulator
     static constexpr uint32_t kWideners = 16;
     static_assert(kBuffers == kWideners / 4 && kBuffers < kMinA, "a group of four warps has a buffer of its own");
-    static constexpr int kWarps = kWideners + 3, kThreads = 32 * kWarps;
+    static constexpr int kSecondMma = kWideners + 3, kWarps = kWideners + 4, kThreads = 32 * kWarps;
+    static constexpr uint32_t kTwoCols = 128;  // up to which two warps issue MMAs
     static constexpr uint32_t kTmemCols = 512;
-    static constexpr uint32_t kBarriers = 2 * kMaxA + 2 * kMaxB + kBuffers + 5;
+    static constexpr uint32_t kBarriers = 2 * kMaxA + 2 * kMaxB + kBuffers + 6;
     static constexpr uint32_t kExactCols = 128, kExactBytes = kExactCols * 128 * 4, kRun = 4;  // kExact: columns, their sums, steps of an accumulator
     static constexpr uint32_t kOtherBytes = 1024 + kBarriers * 8 + 16;
     static constexpr size_t kSmemBytes = 227 * 1024;  // at most
@@ -64,6 +66,8 @@ struct WideCfg {
 };
 static_assert((WideCfg::room(true) - WideCfg::kMinA * WideCfg::kStageA) / WideCfg::b_bytes(false, WideCfg::kExactCols) >= 5, "shared memory");
 static_assert((WideCfg::room(false) - WideCfg::kMinA * WideCfg::kStageA) / WideCfg::b_bytes(false, 256) >= 5, "shared memory");
+static_assert((WideCfg::room(false) - WideCfg::kMinA * WideCfg::kStageA) / WideCfg::b_bytes(false, WideCfg::kTwoCols) >= WideCfg::kMaxB && WideCfg::kMaxB % 2 == 0,
+              "where two warps issue MMAs, a stage of B always belongs to the same one");
 
 struct WideParams {
     DenseParams d;
@@ -103,6 +107,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     const uint64_t limit = p.wait_limit_ns;
     const uint32_t rank = ptx::cluster_cta_rank(), pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
     const uint32_t cols_half = p.split.cols / 2u;  // of B, this CTA's
+    const bool two_mma = !kExact && p.split.cols <= Cfg::kTwoCols;
 
     if (tid == 0) {
         for (uint32_t s = 0; s < stages_a; ++s) {
@@ -115,10 +120,10 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         }
         for (uint32_t b = 0; b < Cfg::kBuffers; ++b) ptx::mbar_init(ready_bar(b), 8);
         for (uint32_t d = 0; d < 2; ++d) {
-            ptx::mbar_init(done_bar + 8u * d, 1);
+            ptx::mbar_init(done_bar + 8u * d, two_mma ? 2u : 1u);
             ptx::mbar_init(taken_bar + 8u * d, 2 * Cfg::kWideners);
         }
-        ptx::mbar_init(drain_bar, 1);
+        for (uint32_t d = 0; d < 2; ++d) ptx::mbar_init(drain_bar + 8u * d, 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&tmap_a);
@@ -136,7 +141,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     ptx::tcgen05_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp > Cfg::kWideners) {
+    if (warp == Cfg::kWideners + 1 || warp == Cfg::kWideners + 2) {
         // =========================================================== loads
         // One warp A and its scales, one B: an instruction holds its warp for some 130 clocks.
         const uint32_t on = lane == 0 ? 1u : 0u;
@@ -172,31 +177,36 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 phase ^= s == 0 ? 1u : 0u;
             }
         }
-    } else if (warp == Cfg::kWideners) {
-        // =========================================================== MMAs (even CTA)
-        if (rank == 0) {
+    } else if (warp >= Cfg::kWideners) {
+        // =========================================================== MMAs (even CTA): every step, or every second one each
+        const uint32_t which_warp = warp == Cfg::kWideners ? 0u : 1u;
+        if (rank == 0 && (which_warp == 0 || two_mma)) {
             const uint32_t on = lane == 0 ? 1u : 0u;
             constexpr uint32_t fmt = std::is_same<T, __half>::value ? ptx::kFmtF16 : ptx::kFmtBF16;
             const uint32_t idesc = ptx::make_instr_desc(fmt, kPairRows4, p.split.cols, false, !kTokens);
             // B [n][k]: 64 values of k a row of the swizzle, eight rows 1024 bytes.  [k][n]: 64 columns a row, eight k 1024 bytes, the next 64
             // columns a box away.
             const uint64_t b_desc = ptx::make_smem_desc(b_addr, kTokens ? 16u : box_bytes, 1024, ptx::kSwizzle128B);
-            const uint32_t b_lo = (uint32_t)b_desc, b_hi = (uint32_t)(b_desc >> 32);
-            uint32_t s = 0, buffer = 0, phase = 0, round = 0;  // rounds: items, or with kExact runs of four steps
+            const uint32_t b_lo = (uint32_t)b_desc, b_hi = (uint32_t)(b_desc >> 32), by = two_mma ? 2u : 1u;
+            uint32_t s = which_warp, buffer = which_warp, phase = 0, round = 0;  // rounds: items, or with kExact runs of four steps
+            uint32_t before = 0;                                                 // steps of the items before
             bool alive = true;
             for (uint32_t item = pair; alive && item < p.split.items; item += n_pairs) {
                 const Item w = split_item(p.split, item);
-                uint32_t left = p.d.k - w.first * kWideK;  // values of k from the next step on
-                for (uint32_t step = w.first; alive && step < w.last; ++round) {
-                    const uint32_t end = kExact ? min(step + Cfg::kRun, w.last) : w.last, which = kExact ? round & 1u : 0u, d = tmem + which * Cfg::kExactCols;
+                uint32_t step = w.first + (two_mma ? (which_warp ^ before) & 1u : 0u);
+                before += w.last - w.first;
+                do {
+                    const uint32_t end = kExact ? min(step + Cfg::kRun, w.last) : w.last, which = kExact ? round & 1u : which_warp, d = tmem + which * Cfg::kExactCols;
+                    const uint32_t bar = kExact ? 8u * which : 0u;
                     if (kExact ? round >= 2 : round >= 1)
-                        alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait_cluster(taken_bar + 8u * which, (kExact ? (round >> 1) - 1u : round - 1u) & 1u, abort_flag, limit));
+                        alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait_cluster(taken_bar + bar, (kExact ? (round >> 1) - 1u : round - 1u) & 1u, abort_flag, limit));
                     uint32_t accumulate = 0;
-                    for (; alive && step < end; ++step) {
+                    for (; alive && step < end; step += by) {
                         alive = __all_sync(0xFFFFFFFFu, ptx::mbar_wait_cluster(ready_bar(buffer), phase, abort_flag, limit));
                         if (!alive) break;
                         ptx::tcgen05_fence_after_sync();
                         const uint32_t a = tmem + kPairCols4 + buffer * Cfg::kBufferCols, b = b_lo + s * (bytes_b >> 4);
+                        const uint32_t left = p.d.k - step * kWideK;  // values of k from this step on
                         if (left >= kWideK) {
                             constexpr uint32_t kNext = kTokens ? 2u : 128u;
                             ptx::umma_pair_f16_ts_x4_if<kNext>(on, d, a, b, b_hi, idesc, accumulate);
@@ -207,17 +217,21 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                         }
                         ptx::umma_commit_pair_if(on, empty_b(s));
                         accumulate = 1;
-                        left -= kWideK;
-                        s = s + 1 == stages_b ? 0u : s + 1;
-                        buffer = buffer + 1 == Cfg::kBuffers ? 0u : buffer + 1;
-                        phase ^= buffer == 0 ? 1u : 0u;
+                        s += by;
+                        if (s >= stages_b) s -= stages_b;
+                        buffer += by;
+                        if (buffer >= Cfg::kBuffers) {
+                            buffer -= Cfg::kBuffers;
+                            phase ^= 1u;
+                        }
                     }
-                    if (alive) ptx::umma_commit_pair_if(on, done_bar + 8u * which);
-                }
+                    if (alive) ptx::umma_commit_pair_if(on, done_bar + bar);
+                    ++round;
+                } while (alive && step < w.last);
             }
             if (!alive && on) {
-                ptx::umma_commit_pair_local(drain_bar);
-                ptx::mbar_wait_bounded(drain_bar, 0, limit);
+                ptx::umma_commit_pair_local(drain_bar + 8u * which_warp);
+                ptx::mbar_wait_bounded(drain_bar + 8u * which_warp, 0, limit);
             }
         }
     } else {
@@ -296,13 +310,18 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 phase_b ^= 1u;
             }
         };
-        // The accumulator's 16 columns from c on.
-        auto columns = [&](uint32_t c, float (&v)[16]) {
+        // The sum's 16 columns from c on, of the first accumulator, the second or both.
+        auto columns = [&](uint32_t c, bool first, bool second, float (&v)[16]) {
             uint32_t r[16];
-            ptx::tmem_ld_32x32b_x16(tmem + lanes + c, r);
+            ptx::tmem_ld_32x32b_x16(tmem + lanes + (first ? 0u : Cfg::kExactCols) + c, r);
             ptx::tmem_ld_wait();
 #pragma unroll
             for (uint32_t i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+            if (!(first && second)) return;
+            ptx::tmem_ld_32x32b_x16(tmem + lanes + Cfg::kExactCols + c, r);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) v[i] += __uint_as_float(r[i]);
         };
         auto free_accumulator = [&](uint32_t which) {
             ptx::tcgen05_fence_before_sync();
@@ -364,6 +383,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             } else {
                 for (uint32_t step = (mine - before) & (Cfg::kBuffers - 1u); alive && step < steps; step += Cfg::kBuffers) widen_step(w.first + step);
                 if (!alive) break;
+                const bool first = !two_mma || steps > 1u || (before & 1u) == 0u, second = two_mma && (steps > 1u || (before & 1u) != 0u);
                 alive = wait(done_bar, round & 1u);
                 if (!alive) break;
                 ptx::tcgen05_fence_after_sync();
@@ -375,7 +395,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                         const uint32_t c = mine * 32u + j / 2u * 128u;
                         if (c >= p.split.cols) break;
                         float v[16];
-                        columns(c + j % 2u * 16u, v);
+                        columns(c + j % 2u * 16u, first, second, v);
 #pragma unroll
                         for (uint32_t i = 0; i < 16; ++i) v[i] = rest.apply(v[i]);
                         pack_row(p.d.c.type, v, packed[j / 2u] + j % 2u * 8u);
@@ -392,7 +412,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                         const uint32_t c = mine * 32u + j / 2u * 128u + j % 2u * 16u;
                         if (c >= p.split.cols) break;
                         float v[16];
-                        columns(c, v);
+                        columns(c, first, second, v);
                         store_part(w, c, v);
                     }
                     free_accumulator(0);
