@@ -56,7 +56,7 @@ int launch_narrow_columns(const b200spmm_fp4_t *a, const DenseParams &d, cudaStr
 // sums' way through memory.
 Split wide_split(uint32_t m, uint32_t n, uint32_t k, bool exact, uint32_t pairs) {
     const uint32_t most = exact ? WideCfg::kExactCols : kPairCols4, tiles_n = (n + most - 1) / most, cols = std::max(64u, ((n + tiles_n - 1) / tiles_n + 31u) / 32u * 32u);
-    return make_split(m, n, cols, (k + kWideK - 1) / kWideK, 4, 0.55, 0.5, 256 * kWideK * 2, pairs);
+    return make_split(m, n, cols, (k + kWideK - 1) / kWideK, 4, 0.55, exact ? 0.6 : cols <= WideCfg::kTwoCols ? 0.33 : 0.5, 256 * kWideK * 2, pairs);
 }
 
 // Pairs of CTAs of the wide kernel that the current device runs at once (its instances take the same room).
@@ -115,21 +115,32 @@ __global__ void __launch_bounds__(256) fp4_align_kernel(const uint16_t *__restri
     }
 }
 
-// Up to 16 columns go to the narrow kernel, which reads any B.
+// Up to 16 columns go to the narrow kernel (9 to 16 take either one 44 to 48 us with 28672 x 8192 in fp16), which reads any B, though rows that
+// start anywhere element by element.  From some 16,000 elements on, those that a block then reads one by one (8 a row of few columns), a
+// copy pays: 28672 x 8192 x 9 columns 88 -> 48 us, 4096 x 2048 x 3 11.1 -> 9.1, but 3 tokens there 7.1 -> 8.2.
 constexpr uint32_t kNarrowColumns = 16;
-bool is_aligned(const void *b, int64_t ldb) { return reinterpret_cast<uintptr_t>(b) % 16u == 0 && ldb % 8 == 0; }
-uint64_t aligned_pieces(uint64_t cols) { return (cols + 63u) / 64u * 8u; }  // of 16 bytes, whole lines of 128: boxes then touch no more of them than they have to
+constexpr uint64_t kCopyFrom = 16384;
+// Whether B's rows, as they lie, start on 16 bytes; a single column's neighbours are one row.
+bool rows_aligned(const void *b, int64_t ldb, int64_t n, bool b_transposed) { return reinterpret_cast<uintptr_t>(b) % 16u == 0 && (ldb % 8 == 0 || (n == 1 && b_transposed)); }
+void one_column(int64_t n, int64_t *ldb, bool *b_transposed, uint32_t k) {
+    if (n != 1 || *b_transposed || *ldb != 1) return;
+    *b_transposed = true;
+    *ldb = k;
+}
+// Pieces of 16 bytes of a row of the copy: whole lines of 128, of which boxes then touch no more than they have to, and single ones for the narrow kernel.
+uint64_t aligned_pieces(uint64_t cols) { return cols <= kNarrowColumns ? (cols + 7u) / 8u : (cols + 63u) / 64u * 8u; }
 uint64_t aligned_bytes(uint64_t rows, uint64_t cols) { return rows * aligned_pieces(cols) * 16u; }
 
 template <typename T, bool kMx, bool kTokens>
 int launch_dense(const b200spmm_fp4_t *a, const DenseParams &d, uint8_t *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
     const uint64_t rows = kTokens ? d.n : d.k, cols = kTokens ? d.k : d.n, need = aligned_bytes(rows, cols);
-    if (d.n <= kNarrowColumns || (!d.b_wide && (!workspace || workspace_bytes < need))) return launch_narrow_columns<T, kMx, kTokens>(a, d, stream);
+    const bool copy = !d.b_wide && workspace && workspace_bytes >= need && (d.n > kNarrowColumns || (uint64_t)d.k * (kTokens ? d.n : 8u) >= kCopyFrom);
+    if (!copy && (d.n <= kNarrowColumns || !d.b_wide)) return launch_narrow_columns<T, kMx, kTokens>(a, d, stream);
     auto wide = [&](const DenseParams &with, uint8_t *ws, uint64_t bytes) {
         return with.c.type == B200SPMM_T_F32 ? launch_wide<T, kMx, kTokens, true>(a, with, reinterpret_cast<float *>(ws), bytes, stream)
                                              : launch_wide<T, kMx, kTokens, false>(a, with, reinterpret_cast<float *>(ws), bytes, stream);
     };
-    if (d.b_wide) return wide(d, workspace, workspace_bytes);
+    if (!copy) return wide(d, workspace, workspace_bytes);
     // no tensor map describes B: a copy that one does goes first into the workspace
     const uint32_t pieces = (uint32_t)aligned_pieces(cols);
     B200_CUDA_TRY(launch_after(fp4_align_kernel, dim3((unsigned)std::min<uint64_t>((rows * pieces + 255u) / 256u, (uint64_t)sm_count() * 8u)), 256, 0, 1, stream,
@@ -138,6 +149,7 @@ int launch_dense(const b200spmm_fp4_t *a, const DenseParams &d, uint8_t *workspa
     with.b = workspace;
     with.ldb = (int64_t)pieces * 8;
     with.b_wide = true;
+    if (d.n <= kNarrowColumns) return launch_narrow_columns<T, kMx, kTokens>(a, with, stream);
     return wide(with, workspace + need, workspace_bytes - need);
 }
 
@@ -145,13 +157,15 @@ int launch_dense(const b200spmm_fp4_t *a, const DenseParams &d, uint8_t *workspa
 
 int dense_product_workspace(const b200spmm_fp4_t *a, const void *b, int64_t ldb, int64_t n, bool b_transposed, uint64_t *bytes) {
     *bytes = 0;
-    if (n <= kNarrowColumns) return B200SPMM_OK;
-    uint32_t pairs = 0;
-    const int st = wide_pairs(a->device, &pairs);
-    if (st != B200SPMM_OK) return st;
     const uint32_t m = (uint32_t)a->rows, k = (uint32_t)a->cols;
-    *bytes = std::max(split_workspace(wide_split(m, (uint32_t)n, k, false, pairs)), split_workspace(wide_split(m, (uint32_t)n, k, true, pairs)));
-    if (!is_aligned(b, ldb)) *bytes += aligned_bytes(b_transposed ? (uint64_t)n : a->cols, b_transposed ? a->cols : (uint64_t)n);
+    if (n > kNarrowColumns) {
+        uint32_t pairs = 0;
+        const int st = wide_pairs(a->device, &pairs);
+        if (st != B200SPMM_OK) return st;
+        *bytes = std::max(split_workspace(wide_split(m, (uint32_t)n, k, false, pairs)), split_workspace(wide_split(m, (uint32_t)n, k, true, pairs)));
+    }
+    one_column(n, &ldb, &b_transposed, k);
+    if (!rows_aligned(b, ldb, n, b_transposed)) *bytes += aligned_bytes(b_transposed ? (uint64_t)n : a->cols, b_transposed ? a->cols : (uint64_t)n);
     return B200SPMM_OK;
 }
 
@@ -167,15 +181,11 @@ int launch_dense_product(const b200spmm_fp4_t *a, const void *b, int64_t ldb, in
     prm.pitch = l.pitch;
     prm.groups = l.groups;
     prm.b = static_cast<const uint8_t *>(b);
+    one_column(n, &ldb, &b_transposed, prm.k);
     prm.ldb = ldb;
     prm.n = (uint32_t)n;
-    prm.b_wide = is_aligned(b, ldb);
+    prm.b_wide = rows_aligned(b, ldb, n, b_transposed);
     prm.c = target_of(c, ldc, c_dtype, c_transposed);
-    if (n == 1 && !b_transposed && ldb == 1) {  // one column, contiguous
-        b_transposed = true;
-        prm.ldb = prm.k;
-    }
-    if (n == 1 && b_transposed) prm.b_wide = reinterpret_cast<uintptr_t>(b) % 16u == 0;
     auto run = [&](auto type, auto mx) {
         using T = decltype(type);
         constexpr bool kMx = decltype(mx)::value;

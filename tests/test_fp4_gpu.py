@@ -534,3 +534,15 @@ def test_tensor_scales_at_the_ends_of_their_range(dtype):
             inf = want.abs() > 3.4e38
             assert torch.equal(got.isinf(), inf) and not got.isnan().any()
             assert bool(((got - want).abs() <= bound)[~inf].all()), (whole, n)
+
+
+@pytest.mark.parametrize("n", [1, 3, 9, 16, 17])
+def test_columns_that_start_on_any_element(n):
+    # few and many of them: read one by one, or copied first
+    for k in (1000, 2050, 17000):
+        W = hs.fp4_quantize(normal(300, k, 1))
+        a = ref.matrix_values(W)
+        whole = normal(k + 1, 2 * n + 3, 2, BF16)
+        for x in (whole[1:, 1:n + 1], whole[:k, 1::2][:, :n].contiguous(), whole[:k, 3:3 + n], whole.t().contiguous()[1:n + 1, 1:].t()):
+            ref.check_product(W.matmul(x), a, x.double(), 16)
+            ref.check_product(W.matmul(x, dtype=BF16), a, x.double(), 16)
