@@ -52,8 +52,8 @@ int launch_narrow_columns(const b200spmm_fp4_t *a, const DenseParams &d, cudaStr
     return d.n <= 8 ? launch_narrow<T, kMx, 1, kTokens>(a, d, stream) : launch_narrow<T, kMx, 2, kTokens>(a, d, stream);
 }
 
-// Columns shared out evenly over as few tiles as there can be, 64 at least (fewer take longer: 24 of 28672 x 8192 84 us as 32, 69 as 64); a part has at least four steps: shorter ones are not worth their
-// sums' way through memory.
+// Columns shared out evenly over as few tiles as there can be, 64 at least (fewer take longer: 24 with 28672 x 8192 88 us as 32, 66 as 64); a
+// part has at least four steps: shorter ones are not worth their sums' way through memory.
 Split wide_split(uint32_t m, uint32_t n, uint32_t k, bool exact, uint32_t pairs) {
     const uint32_t most = exact ? WideCfg::kExactCols : kPairCols4, tiles_n = (n + most - 1) / most, cols = std::max(64u, ((n + tiles_n - 1) / tiles_n + 31u) / 32u * 32u);
     return make_split(m, n, cols, (k + kWideK - 1) / kWideK, 4, 0.55, exact ? 0.6 : cols <= WideCfg::kTwoCols ? 0.33 : 0.5, 256 * kWideK * 2, pairs);

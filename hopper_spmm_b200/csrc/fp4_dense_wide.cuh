@@ -5,6 +5,7 @@
 // Bound: the tensor core's 16-bit rate, and below a hundred columns or so one read of A.  Two CTAs on neighbouring SMs share MMAs
 // of 256 rows x up to 256 columns (tcgen05.mma.cta_group::2): each brings half of B's columns, so that an SM fetches
 // 40 bytes a clock from L2 at the full rate where a CTA alone would need 72, more than that path gives (about 51).
+// 28672 x 8192 nvfp4 x fp16: 2,048 columns 616 us (1,560 TFLOP/s), 192 77 (112 tiles for 74 pairs, two rounds where 1.5 would do), 64 48.
 // A arrives packed, is widened by sixteen warps (exactly, see Widen) and goes through registers into tensor memory, from where the
 // MMA takes it: shared memory, which B keeps busy, sees its 4 bits only once.
 //
