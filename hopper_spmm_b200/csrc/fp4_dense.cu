@@ -97,7 +97,7 @@ int launch_wide(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace,
     }
     B200_CUDA_TRY(launch_after(kernel, dim3(2 * std::min(pairs, prm.split.items)), WideCfg::kThreads, WideCfg::smem_bytes(kTokens, kExact, prm.split.cols), 2, stream, ma, mb, prm));
     if (prm.split.parts > 1)
-        B200_CUDA_TRY(launch_after(fp4_join_kernel, dim3((prm.split.items - prm.split.whole) / prm.split.parts, prm.split.cols / 32u), kPairRows4, 0, 1, stream, prm.split,
+        B200_CUDA_TRY(launch_after(fp4_join_kernel, dim3((prm.split.items - prm.split.whole) / prm.split.parts, prm.split.cols / kJoinCols), kPairRows4, 0, 1, stream, prm.split,
                                    (const float *)workspace, d.m, d.n, kMx ? (const float *)nullptr : d.whole, (const float *)nullptr, Widen<T, kMx>::kLeft, d.c));
     return B200SPMM_OK;
 }

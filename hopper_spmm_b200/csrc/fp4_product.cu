@@ -250,7 +250,7 @@ int launch_pairs(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, const Product
     }
     B200_CUDA_TRY(launch_after(kernel, dim3(2 * std::min(pairs, prm.split.items)), Cfg::kThreads, Cfg::kSmemBytes, 2, stream, ma, mb, prm));
     if (prm.split.parts > 1)
-        B200_CUDA_TRY(launch_after(fp4_join_kernel, dim3((prm.split.items - prm.split.whole) / prm.split.parts, prm.split.cols / 32u), kPairRows4, 0, 1, stream, prm.split,
+        B200_CUDA_TRY(launch_after(fp4_join_kernel, dim3((prm.split.items - prm.split.whole) / prm.split.parts, prm.split.cols / kJoinCols), kPairRows4, 0, 1, stream, prm.split,
                                    (const float *)workspace, prm.m, prm.n, prm.a_whole, prm.b_whole, 1.f, prm.c));
     return B200SPMM_OK;
 }

@@ -79,25 +79,27 @@ B200_DEVICE Item split_item(const Split &s, uint32_t i) {
     return w;
 }
 
-// C of the tiles that were cut: the parts' sums in order.  A thread a row and 32 columns.
+constexpr uint32_t kJoinCols = 8;
+// C of the tiles that were cut: the parts' sums in order.  A thread a row and 8 columns: few loads are under way
+// in all, and with 32 they were behind one another.
 static __global__ void __launch_bounds__(kPairRows4) fp4_join_kernel(const Split s, const float *__restrict__ partial, uint32_t m, uint32_t n, const float *__restrict__ a_whole,
                                                              const float *__restrict__ b_whole, float left, const Target c) {
     ptx::wait_for_grids_before();
     const Factor f(a_whole ? *reinterpret_cast<const volatile float *>(a_whole) : 1.f, b_whole ? *reinterpret_cast<const volatile float *>(b_whole) : left);
-    const uint32_t col = blockIdx.y * 32u;
+    const uint32_t col = blockIdx.y * kJoinCols;
     uint32_t row, n0;
     split_tile(s, s.whole + blockIdx.x, row, n0);
     row += threadIdx.x;
     n0 += col;
     if (row >= m || n0 >= n) return;
-    float v[32] = {};
+    float v[kJoinCols] = {};
     for (uint32_t part = 0; part < s.parts; ++part) {
         const float *src = partial + ((uint64_t)(blockIdx.x * s.parts + part) * s.cols + col) * kPairRows4 + threadIdx.x;
 #pragma unroll
-        for (uint32_t i = 0; i < 32; ++i) v[i] += src[i * kPairRows4];
+        for (uint32_t i = 0; i < kJoinCols; ++i) v[i] += src[i * kPairRows4];
     }
 #pragma unroll
-    for (uint32_t i = 0; i < 32; ++i) v[i] = f.apply(v[i]);
+    for (uint32_t i = 0; i < kJoinCols; ++i) v[i] = f.apply(v[i]);
     store_row(c, row, n0, n, v);
 }
 
