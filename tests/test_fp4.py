@@ -118,7 +118,7 @@ def test_python_refusals():
 
 
 def test_the_reference_rounds_as_the_types_do():
-    # torch's own e4m3 as the judge of the table and of ties
+    # torch's own e4m3 for the table and for ties
     a = torch.cat([ref.e4m3_values(), (ref.e4m3_values()[1:] + ref.e4m3_values()[:-1]) / 2, torch.rand(4000, dtype=torch.float64) * 448])
     assert torch.equal(ref.e4m3_values()[ref.nearest(a, ref.e4m3_values())], a.float().to(torch.float8_e4m3fn).double())
     # ties of e2m1 go to even codes
