@@ -60,14 +60,25 @@ B200_DEVICE uint32_t block_max(uint32_t m, uint32_t *shared) {
     return m;
 }
 
-// 16 neighbours as they are, zeros behind `count`.
+// N pieces of memory, as wide as its alignment allows.
+template <typename V, uint32_t N>
+B200_DEVICE void load_pieces(void *to, const void *from) {
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) static_cast<V *>(to)[i] = __ldg(static_cast<const V *>(from) + i);
+}
+
+// 16 neighbours as they are, zeros behind `count`.  `align`: what all rows' starts are multiples of, bytes.
 template <typename T>
 struct Raw16 {
     uint4 v[sizeof(T)];
-    B200_DEVICE void load(const T *src, uint32_t count, bool wide) {
-        if (wide && count >= 16u) {
+    B200_DEVICE void load(const T *src, uint32_t count, uint32_t align) {
+        if (align >= 16u && count >= 16u) {
 #pragma unroll
             for (uint32_t i = 0; i < sizeof(T); ++i) v[i] = ptx::ld_global_v4(reinterpret_cast<const uint4 *>(src) + i);
+        } else if (align >= 8u && count >= 16u) {
+            load_pieces<uint2, 2 * sizeof(T)>(v, src);
+        } else if (align >= 4u && count >= 16u) {
+            load_pieces<uint32_t, 4 * sizeof(T)>(v, src);
         } else {
             T *e = reinterpret_cast<T *>(v);
 #pragma unroll
@@ -123,7 +134,7 @@ struct Raw16 {
 
 // partial[block] = the largest finite magnitude that the block has seen.  Bound: one read of the matrix; 64 bytes a thread are under way.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) amax_kernel(const T *__restrict__ x, int64_t ldx, uint32_t rows, uint32_t cols, bool wide,
+__global__ void __launch_bounds__(kThreads) amax_kernel(const T *__restrict__ x, int64_t ldx, uint32_t rows, uint32_t cols, uint32_t align,
                                                         float *__restrict__ partial) {
     constexpr int kAhead = sizeof(T) == 4 ? 1 : 2;
     __shared__ uint32_t shared[kThreads / 32];
@@ -133,7 +144,7 @@ __global__ void __launch_bounds__(kThreads) amax_kernel(const T *__restrict__ x,
         Raw16<T> v[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            v[i].load(x + (int64_t)w.row * ldx + w.unit * 16u, w.row < rows ? cols - w.unit * 16u : 0u, wide);
+            v[i].load(x + (int64_t)w.row * ldx + w.unit * 16u, w.row < rows ? cols - w.unit * 16u : 0u, align);
             w.next();
         }
 #pragma unroll
@@ -196,7 +207,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T *__rest
         const bool here = w.row < d.rows;
         const uint32_t col = w.unit * 16u, row = d.rows - 1u - w.row;
         Raw16<T> raw;
-        raw.load(x + (int64_t)row * ldx + col, here && col < d.cols ? d.cols - col : 0u, true);
+        raw.load(x + (int64_t)row * ldx + col, here && col < d.cols ? d.cols - col : 0u, 16u);
         quantize_unit<T, kMx>(raw, tensor, here, row, w.unit, d);
     }
 }
@@ -213,7 +224,7 @@ __global__ void __launch_bounds__(kClusterThreads) quantize_cluster_kernel(const
     const uint32_t units = max(d.groups * 4u, 1u), at = blockIdx.x * blockDim.x + threadIdx.x, row = at / units, unit = at % units;
     const bool here = row < d.rows;
     Raw16<T> raw;
-    raw.load(x + (int64_t)row * ldx + unit * 16u, here && unit * 16u < d.cols ? d.cols - unit * 16u : 0u, true);
+    raw.load(x + (int64_t)row * ldx + unit * 16u, here && unit * 16u < d.cols ? d.cols - unit * 16u : 0u, 16u);
     uint32_t m = __reduce_max_sync(0xFFFFFFFFu, raw.finite_top());
     if ((threadIdx.x & 31u) == 0) shared[threadIdx.x >> 5] = m;
     __syncthreads();
@@ -240,7 +251,7 @@ __global__ void __launch_bounds__(kClusterThreads) quantize_cluster_kernel(const
 constexpr uint32_t kTileR = 128, kTileC = 64, kOutPitch = kTileR / 2 + 16;
 
 template <typename T, bool kMx, bool kRows, bool kCols>
-__global__ void __launch_bounds__(kThreads, 4) quantize_tiles_kernel(const T *__restrict__ x, int64_t ldx, uint32_t x_rows, uint32_t x_cols, bool wide,
+__global__ void __launch_bounds__(kThreads, 4) quantize_tiles_kernel(const T *__restrict__ x, int64_t ldx, uint32_t x_rows, uint32_t x_cols, uint32_t align,
                                                                   const float *partial, uint32_t n_partial, const float *given, const Dest by_rows,
                                                                   const Dest by_cols, uint32_t tiles_c, uint64_t tiles) {
     constexpr uint32_t kPer = 16 / sizeof(T), kVecs = kTileC / kPer;  // elements of a piece, pieces of a row
@@ -256,10 +267,27 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_tiles_kernel(const T *__
         if (kCols) *by_cols.tensor_scale = tensor.up;
     }
     auto piece = [&](uint32_t r, uint32_t p) { return r * kVecs + (p ^ ((r >> 4 & 1u) * (kVecs / 2u))); };
+    // A tile whose rows start on 8 or 4 bytes, in pieces of as many.
+    auto load_tile = [&](auto bytes, uint32_t r0, uint32_t c0) {
+        using V = std::conditional_t<decltype(bytes)::value == 8, uint2, uint32_t>;
+        constexpr uint32_t kIn = sizeof(V) / sizeof(T), kRow = kTileC / kIn, kLoads = kTileR * kRow / kThreads;
+        V v[kLoads];
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            const uint32_t r = (i * kThreads + tid) / kRow, c = (i * kThreads + tid) % kRow * kIn;
+            v[i] = V();
+            if (r0 + r < x_rows) v[i] = __ldg(reinterpret_cast<const V *>(x + (int64_t)(r0 + r) * ldx + c0 + c));
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; ++i) {
+            const uint32_t r = (i * kThreads + tid) / kRow, c = (i * kThreads + tid) % kRow * kIn;
+            *reinterpret_cast<V *>(reinterpret_cast<T *>(tile + piece(r, c / kPer)) + c % kPer) = v[i];
+        }
+    };
     for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
         const uint64_t u = tiles - 1u - t;  // from the end on, see Walk
         const uint32_t r0 = (uint32_t)(u / tiles_c) * kTileR, c0 = (uint32_t)(u % tiles_c) * kTileC;
-        if (wide && c0 + kTileC <= x_cols) {
+        if (align >= 16u && c0 + kTileC <= x_cols) {
             uint4 v[kTileR * kVecs / kThreads];
 #pragma unroll
             for (uint32_t i = 0; i < kTileR * kVecs / kThreads; ++i) {
@@ -268,6 +296,10 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_tiles_kernel(const T *__
             }
 #pragma unroll
             for (uint32_t i = 0; i < kTileR * kVecs / kThreads; ++i) tile[piece((i * kThreads + tid) / kVecs, (i * kThreads + tid) % kVecs)] = v[i];
+        } else if (align >= 8u && c0 + kTileC <= x_cols) {
+            load_tile(std::integral_constant<uint32_t, 8>(), r0, c0);
+        } else if (sizeof(T) < 4 && align >= 4u && c0 + kTileC <= x_cols) {
+            load_tile(std::integral_constant<uint32_t, sizeof(T) < 4 ? 4 : 8>(), r0, c0);
         } else {
 #pragma unroll 8
             for (uint32_t i = tid; i < kTileR * kTileC; i += kThreads) {
@@ -443,7 +475,10 @@ unsigned grid_for(uint64_t work) { return (unsigned)std::max<uint64_t>(1, std::m
 template <typename T, bool kMx>
 int quantize_typed(const T *x, int64_t ldx, uint32_t x_rows, uint32_t x_cols, const float *given, const b200spmm_fp4_t *by_rows,
                    const b200spmm_fp4_t *by_cols, float *workspace, cudaStream_t stream) {
-    const bool wide = reinterpret_cast<uintptr_t>(x) % 16u == 0 && ldx * (int64_t)sizeof(T) % 16 == 0;
+    // what all rows start on, in bytes: 16 or less
+    const uint64_t starts = reinterpret_cast<uintptr_t>(x) | (x_rows > 1 ? (uint64_t)ldx * sizeof(T) : 0u) | 16u;
+    const uint32_t align = (uint32_t)(starts & (~starts + 1u));
+    const bool wide = align == 16u;
     uint32_t n_partial = 0;
     const uint64_t row_units = by_rows ? (uint64_t)dest_of(by_rows).rows * dest_of(by_rows).groups * (kMx ? 8u : 4u) : 0;
     if (!kMx && !given && !by_cols && wide && row_units <= kClusterCtas * kClusterThreads) {
@@ -454,7 +489,7 @@ int quantize_typed(const T *x, int64_t ldx, uint32_t x_rows, uint32_t x_cols, co
     if (!kMx && !given) {
         const uint64_t units = (uint64_t)x_rows * ((x_cols + 15u) / 16u);
         n_partial = std::min(kAmaxBlocks, grid_for((units + kThreads - 1) / kThreads));
-        B200_CUDA_TRY(launch_after(amax_kernel<T>, dim3(n_partial), kThreads, 0, 1, stream, x, ldx, x_rows, x_cols, wide, workspace));
+        B200_CUDA_TRY(launch_after(amax_kernel<T>, dim3(n_partial), kThreads, 0, 1, stream, x, ldx, x_rows, x_cols, align, workspace));
     }
     if (!by_cols && wide) {
         B200_CUDA_TRY(launch_after(quantize_rows_kernel<T, kMx>, dim3(grid_for((row_units + kThreads - 1) / kThreads)), kThreads, 0, 1, stream, x, ldx,
@@ -466,7 +501,7 @@ int quantize_typed(const T *x, int64_t ldx, uint32_t x_rows, uint32_t x_cols, co
     const uint32_t tiles_c = std::max<uint32_t>((x_cols + kTileC - 1) / kTileC, rows.groups * (kMx ? 2u : 1u));
     const uint64_t tiles = (uint64_t)tiles_c * ((x_rows + kTileR - 1) / kTileR);
     auto kernel = !by_cols ? quantize_tiles_kernel<T, kMx, true, false> : by_rows ? quantize_tiles_kernel<T, kMx, true, true> : quantize_tiles_kernel<T, kMx, false, true>;
-    B200_CUDA_TRY(launch_after(kernel, dim3(grid_for(tiles)), kThreads, 0, 1, stream, x, ldx, x_rows, x_cols, wide, (const float *)workspace, n_partial,
+    B200_CUDA_TRY(launch_after(kernel, dim3(grid_for(tiles)), kThreads, 0, 1, stream, x, ldx, x_rows, x_cols, align, (const float *)workspace, n_partial,
                                given, rows, cols, tiles_c, tiles));
     return B200SPMM_OK;
 }

@@ -546,3 +546,18 @@ def test_columns_that_start_on_any_element(n):
         for x in (whole[1:, 1:n + 1], whole[:k, 1::2][:, :n].contiguous(), whole[:k, 3:3 + n], whole.t().contiguous()[1:n + 1, 1:].t()):
             ref.check_product(W.matmul(x), a, x.double(), 16)
             ref.check_product(W.matmul(x, dtype=BF16), a, x.double(), 16)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=IDS)
+@pytest.mark.parametrize("cols, first", [(700, 0), (702, 0), (704, 2), (704, 4), (708, 1), (701, 0)])
+def test_rows_that_start_on_8_4_or_2_bytes(cols, first, dtype, fmt):
+    x = normal(261, cols, 5, dtype)[:, first:]
+    x[7, 70] = torch.inf
+    check_quantized(hs.fp4_quantize(x, fmt), x)
+    check_quantized(hs.fp4_quantize(x, fmt, axis=0), x.t())
+    a, b = hs.fp4_quantize_both(x, fmt)
+    check_quantized(a, x)
+    check_quantized(b, x.t())
+    one = x[3:4]
+    check_quantized(hs.fp4_quantize(one, fmt), one)
