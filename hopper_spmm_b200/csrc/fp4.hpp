@@ -69,5 +69,10 @@ cudaError_t status_word(uint32_t **word);
 // Multiprocessors of the current device.
 int sm_count();
 
+// How long waits of a product that this thread launches may last, and the rows of the box that a stage of A (operand 0) or B (1) arrives in:
+// two seconds and `rows`, but for b200spmm_kat_fp4_starve.
+unsigned long long wait_limit_ns();
+uint32_t rows_of_box(int operand, uint32_t rows);
+
 }  // namespace fp4
 }  // namespace b200spmm

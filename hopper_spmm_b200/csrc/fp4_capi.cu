@@ -1,6 +1,7 @@
 // C entry points of the 4-bit matrices (include/b200_spmm.h): argument checks, the device, the status word.
 #include <atomic>
 
+#include "../../include/b200_spmm_kat.h"
 #include "common.hpp"
 #include "fp4.hpp"
 
@@ -12,6 +13,10 @@ __device__ uint32_t g_status;  // of each device that loads the library
 
 std::atomic<uint32_t *> g_status_word[kMaxDevices];
 std::atomic<int> g_sms[kMaxDevices];
+
+// What b200spmm_kat_fp4_starve asked for; a limit of 0 is none.
+thread_local unsigned long long t_starve_ns = 0;
+thread_local int t_starve_operand = 0;
 
 // Calls that a capturing thread may not make otherwise (they touch no stream).
 struct RelaxedCapture {
@@ -104,6 +109,9 @@ int sm_count() {
     cudaGetDevice(&device);
     return device >= 0 && device < kMaxDevices && g_sms[device] > 0 ? g_sms[device].load() : 148;
 }
+
+unsigned long long wait_limit_ns() { return t_starve_ns ? t_starve_ns : kDeviceWaitLimitNs; }
+uint32_t rows_of_box(int operand, uint32_t rows) { return t_starve_ns && operand == t_starve_operand ? rows / 2u : rows; }
 
 cudaError_t status_word(uint32_t **word) {
     int device = 0;
@@ -223,6 +231,14 @@ int b200spmm_fp4_status(int device, void *stream) {
         B200_CUDA_TRY(cudaMemset(word, 0, sizeof(status)));
         return B200SPMM_ERR_DEVICE_TIMEOUT;
     });
+}
+
+/* Declared in b200_spmm_kat.h: products whose stages can never be complete. */
+int b200spmm_kat_fp4_starve(unsigned long long limit_ns, int operand) {
+    if (limit_ns > kDeviceWaitLimitNs || (operand != 0 && operand != 1)) return B200SPMM_ERR_INVALID_ARG;
+    t_starve_ns = limit_ns;
+    t_starve_operand = operand;
+    return B200SPMM_OK;
 }
 
 }  // extern "C"

@@ -36,9 +36,9 @@ int launch_narrow(const b200spmm_fp4_t *a, const DenseParams &d, cudaStream_t st
     const uint32_t sums = prm.slices > 1 ? warps * 16u * 8u * kNB * (uint32_t)sizeof(float) : 0u;
     prm.stages = std::min({kNarrowMaxStages, (kMostBytes - 1280u - sums) / stage, std::max<uint32_t>(2, (d.k + kNarrowStage - 1) / kNarrowStage)});
     B200_CUDA_TRY(status_word(&prm.status));
-    prm.wait_limit_ns = kDeviceWaitLimitNs;
+    prm.wait_limit_ns = wait_limit_ns();
     CUtensorMap ma;
-    if (!encode_2d(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, d.pitch, d.m, d.pitch, kNarrowStage / 2, prm.at_once * 16u, CU_TENSOR_MAP_SWIZZLE_128B,
+    if (!encode_2d(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, d.pitch, d.m, d.pitch, kNarrowStage / 2, rows_of_box(0, prm.at_once * 16u), CU_TENSOR_MAP_SWIZZLE_128B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) {
         set_last_error_static("a tensor map of a 4-bit matrix could not be made");
         return B200SPMM_ERR_CUDA;
@@ -85,12 +85,12 @@ int launch_wide(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace,
     prm.stages_b = WideCfg::stages_b(kTokens, kExact, prm.split.cols);
     prm.partial = workspace;
     B200_CUDA_TRY(status_word(&prm.status));
-    prm.wait_limit_ns = kDeviceWaitLimitNs;
+    prm.wait_limit_ns = wait_limit_ns();
     CUtensorMap ma, mb;
     const auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const uint64_t pitch_b = (d.n > 1 || !kTokens) && (d.k > 1 || kTokens) ? (uint64_t)d.ldb * 2u : ((uint64_t)(kTokens ? d.k : d.n) * 2u + 15u) / 16u * 16u;
-    if (!encode_2d(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, d.pitch, d.m, d.pitch, kWideK / 2, 128, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) ||
-        !encode_2d(&mb, type, d.b, kTokens ? d.k : d.n, kTokens ? d.n : d.k, pitch_b, 64, kTokens ? prm.split.cols / 2u : kWideK, CU_TENSOR_MAP_SWIZZLE_128B,
+    if (!encode_2d(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, d.pitch, d.m, d.pitch, kWideK / 2, rows_of_box(0, 128), CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) ||
+        !encode_2d(&mb, type, d.b, kTokens ? d.k : d.n, kTokens ? d.n : d.k, pitch_b, 64, rows_of_box(1, kTokens ? prm.split.cols / 2u : kWideK), CU_TENSOR_MAP_SWIZZLE_128B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) {
         set_last_error_static("a tensor map of a product with a 4-bit matrix could not be made");
         return B200SPMM_ERR_CUDA;

@@ -243,14 +243,14 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + kNarrowLoaders), 1) fp4_n
                 if (lane == 0) ptx::mbar_arrive(empty + 8u * s);
                 step_on();
             }
-            if (!alive) break;
-            // ---- to C, over shared memory where k was sliced: [warp][column][row]
+            // ---- to C, over shared memory where k was sliced: [warp][column][row].  A warp whose wait gave up comes to the barrier as well: the
+            // others, whose waits may have ended in time, count on it there, and no wait of theirs would end it.  All leave then.
             if (p.slices > 1) {
 #pragma unroll
                 for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
 #pragma unroll
                     for (uint32_t e = 0; e < 4; ++e) sums[(warp * kCols + nb * 8u + t * 2u + (e & 1u)) * 16u + (e >> 1) * 8u + r_of_g] = acc[nb][e];
-                asm volatile("bar.sync 1, %0;" ::"r"(consumers * 32u) : "memory");
+                if (ptx::bar_or(1, consumers * 32u, !alive)) break;
                 for (uint32_t i = tid; i < p.at_once * 16u * kCols; i += consumers * 32u) {
                     const uint32_t r = i % 16u, col = i / 16u % kCols, tile = i / (16u * kCols);
                     float v[1] = {0.f};
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + kNarrowLoaders), 1) fp4_n
                     if (tile0 + tile < tile_end && c_row < p.d.m && n0 + col < p.d.n) store_row(p.d.c, c_row, n0 + col, p.d.n, v);
                 }
                 asm volatile("bar.sync 1, %0;" ::"r"(consumers * 32u) : "memory");  // (the next tiles' sums go there)
-            } else if (busy) {
+            } else if (busy && alive) {
 #pragma unroll
                 for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
 #pragma unroll

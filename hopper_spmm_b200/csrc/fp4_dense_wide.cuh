@@ -291,8 +291,8 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             ptx::tmem_st_32x32b_x32(buffer + 32u, out);
             // (B's stage was last that of a step that is done by now, at least as old as the one waited for)
             alive = wait(full_b(sb), phase_b);
+            ptx::tmem_st_wait();  // (tensor memory is let go of after a wait that ran out, too)
             if (!alive) return;
-            ptx::tmem_st_wait();
             ptx::tcgen05_fence_before_sync();
             __syncwarp();
             if (lane == 0) {

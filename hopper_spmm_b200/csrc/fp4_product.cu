@@ -208,7 +208,7 @@ int launch_width(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, const Product
         configured = a->device;
     }
     CUtensorMap ma, mb;
-    if (!encode_values(&ma, a, layout_of(a->rows, a->cols, a->format), kTileM) || !encode_values(&mb, b, layout_of(b->rows, b->cols, b->format), kN)) {
+    if (!encode_values(&ma, a, layout_of(a->rows, a->cols, a->format), rows_of_box(0, kTileM)) || !encode_values(&mb, b, layout_of(b->rows, b->cols, b->format), rows_of_box(1, kN))) {
         set_last_error_static("a tensor map of a 4-bit matrix could not be made");
         return B200SPMM_ERR_CUDA;
     }
@@ -244,7 +244,7 @@ int launch_pairs(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, const Product
     if (prm.split.parts > 1 && (!workspace || workspace_bytes < split_workspace(prm.split))) prm.split = pair_split(prm.m, prm.n, prm.k, 1);
     prm.partial = workspace;
     CUtensorMap ma, mb;
-    if (!encode_values(&ma, a, layout_of(a->rows, a->cols, a->format), 128) || !encode_values(&mb, b, layout_of(b->rows, b->cols, b->format), prm.split.cols / 2u)) {
+    if (!encode_values(&ma, a, layout_of(a->rows, a->cols, a->format), rows_of_box(0, 128)) || !encode_values(&mb, b, layout_of(b->rows, b->cols, b->format), rows_of_box(1, prm.split.cols / 2u))) {
         set_last_error_static("a tensor map of a 4-bit matrix could not be made");
         return B200SPMM_ERR_CUDA;
     }
@@ -303,7 +303,7 @@ int launch_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *c, in
     prm.groups = layout_of(a->rows, a->cols, a->format).groups;
     prm.c = target_of(c, ldc, c_dtype, c_transposed);
     B200_CUDA_TRY(status_word(&prm.status));
-    prm.wait_limit_ns = kDeviceWaitLimitNs;
+    prm.wait_limit_ns = wait_limit_ns();
     return a->format == B200SPMM_MXFP4 ? launch_format<true>(a, b, prm, workspace, workspace_bytes, stream)
                                          : launch_format<false>(a, b, prm, workspace, workspace_bytes, stream);
 }

@@ -124,6 +124,14 @@ B200_DEVICE bool mbar_wait_bounded(uint32_t bar, uint32_t parity, uint64_t limit
     }
 }
 
+// Waits at barrier `id` for `threads` threads, whole warps, and tells all of them alike whether one of them brought `mine`.
+B200_DEVICE bool bar_or(uint32_t id, uint32_t threads, bool mine) {
+    uint32_t any;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 q, %3, 0;\nbar.red.or.pred p, %1, %2, q;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(any) : "r"(id), "r"(threads), "r"(mine ? 1u : 0u) : "memory");
+    return any != 0;
+}
+
 // ------------------------------------------------------------------ proxies and fences
 
 // Orders this thread's generic-proxy shared-memory accesses with async-proxy accesses

@@ -74,6 +74,14 @@ int b200spmm_kat_spmm_starved(struct b200spmm_plan *plan, const void *d_B, int64
                               int64_t ldc, unsigned long long limit_ns, void *stream);
 
 /*
+ * The same for products of 4-bit matrices (b200spmm_fp4_product, b200spmm_fp4_dense_product): those that the calling thread launches
+ * from here on get a tensor map over operand 0 (the rows of the tiles) or 1 (their columns; with up to 16 columns of 16 bits there is none,
+ * and nothing changes) whose box has half the rows that a stage counts on, and waits of limit_ns (at most two seconds).
+ * They must unwind and b200spmm_fp4_status must say B200SPMM_ERR_DEVICE_TIMEOUT.  0 ends it.
+ */
+int b200spmm_kat_fp4_starve(unsigned long long limit_ns, int operand);
+
+/*
  * From here on a launch of `plan` that needs a scratch buffer of more than `bytes` asks for more memory than any device
  * has, and finds none, as where others hold it.  A buffer that is there and large enough serves on.
  */

@@ -161,3 +161,9 @@ def test_the_arrays_of_a_matrix_are_not_exchanged():
     for name in ("values", "scales", "tensor_scale", "rows", "cols"):
         with pytest.raises(AttributeError):
             setattr(m, name, getattr(m, name))
+
+
+def test_the_starving_of_products_takes_a_limit_and_an_operand():
+    starve = capi.lib().b200spmm_kat_fp4_starve
+    assert starve(2_000_000_001, 0) == starve(1, 2) == starve(1, -1) == capi.ERR_INVALID_ARG
+    assert starve(5_000_000, 1) == starve(0, 0) == capi.OK

@@ -561,3 +561,49 @@ def test_rows_that_start_on_8_4_or_2_bytes(cols, first, dtype, fmt):
     check_quantized(b, x.t())
     one = x[3:4]
     check_quantized(hs.fp4_quantize(one, fmt), one)
+
+
+# ---------------------------------------------------------------- waits that run out
+
+@pytest.fixture
+def starve():
+    yield capi.lib().b200spmm_kat_fp4_starve
+    assert capi.lib().b200spmm_kat_fp4_starve(0, 0) == capi.OK
+
+
+STARVED = [(300, 4096, 1, F16, F16), (300, 128, 16, BF16, F32), (40000, 512, 3, F16, F32), (300, 1000, 40, BF16, BF16), (700, 2048, 300, F16, F16), (700, 2048, 300, BF16, F32)]
+
+
+@pytest.mark.parametrize("operand", [0, 1])
+@pytest.mark.parametrize("m,k,n,dtype,out", STARVED, ids=str)
+def test_a_starved_product_with_dense_columns_ends_and_says_so(m, k, n, dtype, out, operand, starve):
+    # A failure made on the host: boxes of half the rows, so that no stage is ever complete.  Every role has to leave its waits, the barriers
+    # between them included, and the next product is an ordinary one.
+    W, x = hs.fp4_quantize(normal(m, k, 1)), normal(k, n, 2, dtype)
+    for B in (x, x.t().contiguous().t()):
+        assert starve(5_000_000, operand) == capi.OK
+        W.matmul(B, dtype=out, sync=False)
+        assert starve(0, 0) == capi.OK
+        if operand == 1 and n <= 16:  # few columns have no box of B
+            W.sync()
+        else:
+            with pytest.raises(capi.SpmmError) as e:
+                W.sync()
+            assert e.value.status == capi.ERR_DEVICE_TIMEOUT
+        W.sync()  # said once
+        ref.check_product(W.matmul(B, dtype=out), ref.matrix_values(W), B.double(), 16)
+
+
+@pytest.mark.parametrize("operand", [0, 1])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,k,n", [(300, 4096, 8), (300, 1000, 50), (700, 2048, 300), (257, 100, 65)])
+def test_a_starved_product_of_two_matrices_ends_and_says_so(m, k, n, fmt, operand, starve):
+    A, B = hs.fp4_quantize(normal(m, k, 1), fmt), hs.fp4_quantize(normal(n, k, 2), fmt)
+    assert starve(5_000_000, operand) == capi.OK
+    A.matmul(B, sync=False)
+    assert starve(0, 0) == capi.OK
+    with pytest.raises(capi.SpmmError) as e:
+        A.sync()
+    assert e.value.status == capi.ERR_DEVICE_TIMEOUT
+    A.sync()
+    ref.check_product(A.matmul(B), ref.matrix_values(A), ref.matrix_values(B).t(), 64)
