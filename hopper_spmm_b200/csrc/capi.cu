@@ -311,14 +311,6 @@ int grow_buffer(T **buf, size_t bytes) {
     return B200SPMM_OK;
 }
 
-// (The default stream does not answer while another one is being captured; a launch there will say so.)
-bool is_captured(cudaStream_t stream) {
-    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(stream, &capture) == cudaSuccess) return capture != cudaStreamCaptureStatusNone;
-    cudaGetLastError();
-    return true;
-}
-
 // Scratch for a launch on `stream`.  A captured launch has it like any other, so that a graph holds the kernels that the call
 // would run; but a capture allows no wait for the device, and what is outgrown then may be in use.
 int take_scratch(b200spmm_plan *p, b200spmm_plan::Scratch *s, size_t bytes, cudaStream_t stream) {

@@ -27,6 +27,14 @@ int guarded(Fn &&body) noexcept {
     }
 }
 
+// (The default stream does not answer while another one is being captured; a launch there will say so.)
+inline bool is_captured(cudaStream_t stream) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &capture) == cudaSuccess) return capture != cudaStreamCaptureStatusNone;
+    cudaGetLastError();
+    return true;
+}
+
 // How long a device-side wait may spin before the kernel gives up (nanoseconds).
 constexpr unsigned long long kDeviceWaitLimitNs = 2000000000ull;
 

@@ -64,8 +64,8 @@ int launch_dense_product(const b200spmm_fp4_t *a, const void *b, int64_t ldb, in
 int dense_product_workspace(const b200spmm_fp4_t *a, const void *b, int64_t ldb, int64_t n, bool b_transposed, uint64_t *bytes);
 
 constexpr int kMaxDevices = 64;
-// The word in which kernels report a wait that ran out, on the current device.
-cudaError_t status_word(uint32_t **word);
+// The word in which kernels count waits that ran out, on the current device, for a launch on `stream` by this thread.
+cudaError_t status_of_launch(cudaStream_t stream, uint32_t **word);
 // Multiprocessors of the current device.
 int sm_count();
 

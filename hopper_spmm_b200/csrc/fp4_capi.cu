@@ -1,5 +1,7 @@
 // C entry points of the 4-bit matrices (include/b200_spmm.h): argument checks, the device, the status word.
 #include <atomic>
+#include <map>
+#include <utility>
 
 #include "../../include/b200_spmm_kat.h"
 #include "common.hpp"
@@ -9,10 +11,27 @@ namespace b200spmm {
 namespace fp4 {
 namespace {
 
-__device__ uint32_t g_status;  // of each device that loads the library
+// Waits that ran out on each device that loads the library.  Only counted up: whoever asks compares with what it was told last, so that nobody's
+// asking hides a failure from others.
+__device__ uint32_t g_status;
 
 std::atomic<uint32_t *> g_status_word[kMaxDevices];
+std::atomic<uint32_t> g_counted[kMaxDevices];  // the largest count that anybody has read
 std::atomic<int> g_sms[kMaxDevices];
+
+// What this thread knows of a device's count, each one more than that (0: it has not come to the device yet): `first`, what anybody had read when
+// it came; `told`, the most it was told since.  And for each stream that it launches to or asks for, by device and handle, what it goes by
+// there: at the first launch what it had been told by then, later what it was told there.  (A handle that comes back as another stream finds
+// an older count: that may say a failure twice, and hides none.)
+struct Known {
+    uint64_t first, told;
+};
+thread_local Known t_known[kMaxDevices];
+thread_local std::map<std::pair<int, cudaStream_t>, uint32_t> t_streams;
+
+void come(int device) {
+    if (!t_known[device].first) t_known[device].first = t_known[device].told = 1ull + g_counted[device].load();
+}
 
 // What b200spmm_kat_fp4_starve asked for; a limit of 0 is none.
 thread_local unsigned long long t_starve_ns = 0;
@@ -81,6 +100,18 @@ int on_device(int device, Fn &&body) {
     });
 }
 
+// The word of the device, which is current.
+cudaError_t status_word(int device, uint32_t **word) {
+    *word = g_status_word[device].load(std::memory_order_relaxed);
+    if (*word) return cudaSuccess;
+    void *p = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&p, g_status);
+    if (e != cudaSuccess) return e;
+    *word = static_cast<uint32_t *>(p);
+    g_status_word[device].store(*word, std::memory_order_relaxed);
+    return cudaSuccess;
+}
+
 int quantize(const void *x, int64_t ldx, int x_dtype, const float *tensor_scale, const b200spmm_fp4_t *by_rows, const b200spmm_fp4_t *by_cols,
              float *workspace, void *stream) {
     for (const b200spmm_fp4_t *m : {by_rows, by_cols})
@@ -113,18 +144,13 @@ int sm_count() {
 unsigned long long wait_limit_ns() { return t_starve_ns ? t_starve_ns : kDeviceWaitLimitNs; }
 uint32_t rows_of_box(int operand, uint32_t rows) { return t_starve_ns && operand == t_starve_operand ? rows / 2u : rows; }
 
-cudaError_t status_word(uint32_t **word) {
+cudaError_t status_of_launch(cudaStream_t stream, uint32_t **word) {
     int device = 0;
     const cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return e;
-    *word = g_status_word[device].load(std::memory_order_relaxed);
-    if (*word) return cudaSuccess;
-    void *p = nullptr;
-    const cudaError_t f = cudaGetSymbolAddress(&p, g_status);
-    if (f != cudaSuccess) return f;
-    *word = static_cast<uint32_t *>(p);
-    g_status_word[device].store(*word, std::memory_order_relaxed);
-    return cudaSuccess;
+    come(device);
+    t_streams.try_emplace({device, stream}, (uint32_t)(t_known[device].told - 1u));
+    return status_word(device, word);
 }
 
 }  // namespace fp4
@@ -217,18 +243,21 @@ int b200spmm_fp4_dense_product(const b200spmm_fp4_t *a, const void *d_B, int64_t
     });
 }
 
-int b200spmm_fp4_status(int device, void *stream) {
-    return guarded([&]() -> int {
-        const int st = check_device(device);
-        if (st != B200SPMM_OK) return st;
-        const DeviceGuard guard(device);
-        B200_CUDA_TRY(guard.status);
-        uint32_t *word = nullptr, status = 0;
-        B200_CUDA_TRY(status_word(&word));
-        B200_CUDA_TRY(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
-        B200_CUDA_TRY(cudaMemcpy(&status, word, sizeof(status), cudaMemcpyDeviceToHost));
-        if (!(status & kDevStatusTimeout)) return B200SPMM_OK;
-        B200_CUDA_TRY(cudaMemset(word, 0, sizeof(status)));
+int b200spmm_fp4_status(int device, void *stream_v) {
+    return on_device(device, [&]() -> int {
+        const cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+        if (is_captured(stream)) return B200SPMM_ERR_UNSUPPORTED;
+        uint32_t *word = nullptr, count = 0;
+        come(device);
+        B200_CUDA_TRY(status_word(device, &word));
+        B200_CUDA_TRY(cudaMemcpyAsync(&count, word, sizeof(count), cudaMemcpyDeviceToHost, stream));
+        B200_CUDA_TRY(cudaStreamSynchronize(stream));
+        if (count == 0) return B200SPMM_OK;
+        for (uint32_t most = g_counted[device].load(); most < count && !g_counted[device].compare_exchange_weak(most, count);) {}
+        uint32_t &known = t_streams.try_emplace({device, stream}, (uint32_t)(t_known[device].first - 1u)).first->second;
+        if (known == count) return B200SPMM_OK;
+        known = count;
+        t_known[device].told = 1ull + count;
         return B200SPMM_ERR_DEVICE_TIMEOUT;
     });
 }

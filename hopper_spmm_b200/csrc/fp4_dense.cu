@@ -35,7 +35,7 @@ int launch_narrow(const b200spmm_fp4_t *a, const DenseParams &d, cudaStream_t st
     const uint32_t stage = narrow_stage(kMx, prm.at_once, prm.row_blocks, kNB).bytes(), warps = prm.at_once * prm.slices;
     const uint32_t sums = prm.slices > 1 ? warps * 16u * 8u * kNB * (uint32_t)sizeof(float) : 0u;
     prm.stages = std::min({kNarrowMaxStages, (kMostBytes - 1280u - sums) / stage, std::max<uint32_t>(2, (d.k + kNarrowStage - 1) / kNarrowStage)});
-    B200_CUDA_TRY(status_word(&prm.status));
+    B200_CUDA_TRY(status_of_launch(stream, &prm.status));
     prm.wait_limit_ns = wait_limit_ns();
     CUtensorMap ma;
     if (!encode_2d(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, d.pitch, d.m, d.pitch, kNarrowStage / 2, rows_of_box(0, prm.at_once * 16u), CU_TENSOR_MAP_SWIZZLE_128B,
@@ -84,7 +84,7 @@ int launch_wide(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace,
     prm.stages_a = WideCfg::stages_a(kTokens, kExact, prm.split.cols);
     prm.stages_b = WideCfg::stages_b(kTokens, kExact, prm.split.cols);
     prm.partial = workspace;
-    B200_CUDA_TRY(status_word(&prm.status));
+    B200_CUDA_TRY(status_of_launch(stream, &prm.status));
     prm.wait_limit_ns = wait_limit_ns();
     CUtensorMap ma, mb;
     const auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;

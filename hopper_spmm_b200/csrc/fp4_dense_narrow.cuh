@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + kNarrowLoaders), 1) fp4_n
     if (*abort_flag) {
         const uint64_t t0 = ptx::global_timer_ns();
         while (ptx::global_timer_ns() - t0 < 20000000ull) __nanosleep(1000);  // what is under way to shared memory arrives
-        if (lane == 0) atomicOr(p.status, kDevStatusTimeout);
+        if (lane == 0) atomicAdd(p.status, 1u);
     }
 }
 

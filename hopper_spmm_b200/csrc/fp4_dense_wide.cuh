@@ -437,7 +437,7 @@ fp4_wide_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         ptx::tcgen05_fence_after_sync();
         ptx::tmem_dealloc_pair(tmem, Cfg::kTmemCols);
     }
-    if (tid == 0 && *abort_flag) atomicOr(p.status, kDevStatusTimeout);
+    if (tid == 0 && *abort_flag) atomicAdd(p.status, 1u);
 }
 
 }  // namespace fp4

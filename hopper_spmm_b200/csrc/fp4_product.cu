@@ -182,7 +182,7 @@ fp4_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     if (*abort_flag) {
         const uint64_t t0 = ptx::global_timer_ns();
         while (ptx::global_timer_ns() - t0 < kLingerNs) __nanosleep(1000);
-        if (tid == 0) atomicOr(p.status, kDevStatusTimeout);
+        if (tid == 0) atomicAdd(p.status, 1u);
         __syncthreads();
     }
     if (warp == 5) {
@@ -302,7 +302,7 @@ int launch_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void *c, in
     prm.k = (uint32_t)a->cols;
     prm.groups = layout_of(a->rows, a->cols, a->format).groups;
     prm.c = target_of(c, ldc, c_dtype, c_transposed);
-    B200_CUDA_TRY(status_word(&prm.status));
+    B200_CUDA_TRY(status_of_launch(stream, &prm.status));
     prm.wait_limit_ns = wait_limit_ns();
     return a->format == B200SPMM_MXFP4 ? launch_format<true>(a, b, prm, workspace, workspace_bytes, stream)
                                          : launch_format<false>(a, b, prm, workspace, workspace_bytes, stream);

@@ -151,7 +151,8 @@ class Fp4Matrix:
         return C_out
 
     def sync(self, stream=None):
-        """Waits for ``stream`` (the current one) and raises if a product on this device ran out of time."""
+        """Waits for ``stream`` (the current one) and raises if a product on this device ran out of time: on whatever stream it
+        was, for a thread is told of it on every stream that it uses.  Not while the stream is captured (pass ``sync=False`` there)."""
         import torch
         s = (stream or torch.cuda.current_stream(self.values.device)).cuda_stream
         capi.check(capi.lib().b200spmm_fp4_status(self.values.device.index, s), "b200spmm_fp4_status")

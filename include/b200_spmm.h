@@ -566,8 +566,11 @@ int b200spmm_fp4_product_workspace(const b200spmm_fp4_t *a, const void *d_B, int
 
 /*
  * All of these are asynchronous on `stream`, run on the matrices' device whichever is current, allocate nothing and may be captured
- * into CUDA graphs; calls that share no output or workspace may overlap.  This one waits for `stream` and returns
- * B200SPMM_ERR_DEVICE_TIMEOUT if a bounded wait of a product on that device gave up since it was last asked.
+ * into CUDA graphs; calls that share no output or workspace may overlap.  This one waits for `stream`, and for nothing else, and returns
+ * B200SPMM_ERR_DEVICE_TIMEOUT if a bounded wait of a product on that device, on any stream, gave up since this thread last asked for this
+ * stream, or else first launched a product to it.  (Where it has done neither, since its first call here.)  That others ask, or that it asks
+ * for another stream, takes nothing from what it is told.  A stream that is being captured is refused (B200SPMM_ERR_UNSUPPORTED), and its
+ * capture goes on.
  */
 int b200spmm_fp4_status(int device, void *stream);
 

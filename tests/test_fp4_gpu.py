@@ -569,6 +569,8 @@ def test_rows_that_start_on_8_4_or_2_bytes(cols, first, dtype, fmt):
 def starve():
     yield capi.lib().b200spmm_kat_fp4_starve
     assert capi.lib().b200spmm_kat_fp4_starve(0, 0) == capi.OK
+    torch.cuda.synchronize()
+    capi.lib().b200spmm_fp4_status(0, torch.cuda.current_stream().cuda_stream)  # (every stream that was launched to is told of every failure)
 
 
 STARVED = [(300, 4096, 1, F16, F16), (300, 128, 16, BF16, F32), (40000, 512, 3, F16, F32), (300, 1000, 40, BF16, BF16), (700, 2048, 300, F16, F16), (700, 2048, 300, BF16, F32)]
@@ -607,3 +609,120 @@ def test_a_starved_product_of_two_matrices_ends_and_says_so(m, k, n, fmt, operan
     assert e.value.status == capi.ERR_DEVICE_TIMEOUT
     A.sync()
     ref.check_product(A.matmul(B), ref.matrix_values(A), ref.matrix_values(B).t(), 64)
+
+
+def starved_product(starve, W, x, stream, limit_ns=5_000_000, out=None):
+    assert starve(limit_ns, 0) == capi.OK
+    y = W.matmul(x, out, stream=stream, sync=False)
+    assert starve(0, 0) == capi.OK
+    return y
+
+
+def status(stream):
+    return capi.lib().b200spmm_fp4_status(0, stream.cuda_stream)
+
+
+def test_asking_for_one_stream_does_not_hide_a_failure_from_others(starve):
+    import threading
+    W, x = hs.fp4_quantize(normal(300, 512, 1)), normal(512, 8, 2, F16)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    W.matmul(x)
+    torch.cuda.synchronize()
+    starved_product(starve, W, x, a)
+    torch.cuda.synchronize()
+    assert status(b) == capi.ERR_DEVICE_TIMEOUT  # somewhere on the device, and said once
+    assert status(b) == capi.OK
+    assert status(a) == capi.ERR_DEVICE_TIMEOUT  # ... and still to who launched it
+    assert status(a) == capi.OK
+    W.matmul(x, stream=torch.cuda.Stream())  # a stream of which the thread has known nothing until it was told
+    # two threads on one stream: either is told
+    ready, asked, told = threading.Barrier(2), threading.Event(), {}
+
+    def other():
+        W.matmul(x, stream=a, sync=False)
+        ready.wait()
+        asked.wait()
+        told["other"] = [status(a), status(a)]
+    t = threading.Thread(target=other)
+    t.start()
+    ready.wait()
+    starved_product(starve, W, x, a)
+    told["this"] = [status(a), status(a)]
+    asked.set()
+    t.join()
+    assert told["this"] == told["other"] == [capi.ERR_DEVICE_TIMEOUT, capi.OK]
+    # who comes later is not told what others have read
+    t = threading.Thread(target=lambda: told.update(late=[status(a), status(b)]))
+    t.start()
+    t.join()
+    assert told["late"] == [capi.OK, capi.OK]
+    W.matmul(x, stream=a)
+
+
+def test_every_replay_of_a_starved_product_is_reported(starve):
+    W, x = hs.fp4_quantize(normal(300, 512, 1)), normal(512, 40, 2, F16)
+    out = W.matmul(x)
+    s, other, g = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        starved_product(starve, W, x, None, out=out)
+    for on in (s, other, s):
+        with torch.cuda.stream(on):
+            g.replay()
+        assert status(on) == capi.ERR_DEVICE_TIMEOUT
+    assert status(s) == capi.OK and status(other) == capi.ERR_DEVICE_TIMEOUT  # (the third one, for who asks there)
+    del g
+    assert status(torch.cuda.current_stream()) == capi.ERR_DEVICE_TIMEOUT
+    W.matmul(x)
+
+
+def test_waiting_for_a_product_waits_for_its_stream_alone():
+    W, x = hs.fp4_quantize(normal(300, 512, 1)), normal(512, 8, 2, F16)
+    want = W.matmul(x)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    assert torch.cuda.current_stream() == torch.cuda.default_stream()
+    torch.cuda._sleep(2_000_000_000)  # about a second
+    with torch.cuda.stream(s):
+        got = W.matmul(x)
+    assert not torch.cuda.default_stream().query(), "waited for another stream"
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_waiting_while_another_thread_captures():
+    import threading
+    W, x = hs.fp4_quantize(normal(300, 512, 1)), normal(512, 8, 2, F16)
+    want, room, mine = W.matmul(x), torch.empty(300, 8, device="cuda"), torch.empty(300, 8, device="cuda")
+    side, g, went = torch.cuda.Stream(), torch.cuda.CUDAGraph(), {}
+    torch.cuda.synchronize()
+
+    def other():
+        try:
+            with torch.cuda.stream(side):
+                W.matmul(x, mine)
+            went["ok"] = True
+        except Exception as e:  # noqa: BLE001
+            went["error"] = e
+    with torch.cuda.graph(g):
+        W.matmul(x, room, sync=False)
+        t = threading.Thread(target=other)
+        t.start()
+        t.join()
+    assert went == {"ok": True}
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(room, want) and torch.equal(mine, want)
+
+
+def test_waiting_for_a_stream_that_is_captured_is_refused():
+    W, x = hs.fp4_quantize(normal(300, 512, 1)), normal(512, 8, 2, F16)
+    want, out, g = W.matmul(x), torch.empty(300, 8, device="cuda"), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        with pytest.raises(capi.SpmmError) as e:
+            W.matmul(x, out)
+    assert e.value.status == capi.ERR_UNSUPPORTED
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
