@@ -8,6 +8,8 @@
 //           them to the tensor memory columns that the block-scaled MMA reads - row block by row block, with zeros where the
 //           matrix ends inside a block;
 //   tensor_scale  one fp32 number, a power of two (1 for mxfp4).
+// The kernels are launched with programmatic serialization (launch_after) and read what a kernel before them may have written, inputs of the
+// caller's included: by ordinary loads only, with no pointer that promises the compiler data which nobody writes, and after their wait for that kernel.
 // The reference has no 4-bit form (src/common.h:14-43: fp16 and tf32).
 #pragma once
 

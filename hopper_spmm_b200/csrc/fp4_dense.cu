@@ -103,12 +103,12 @@ int launch_wide(const b200spmm_fp4_t *a, const DenseParams &d, float *workspace,
 }
 
 // B, whose rows start anywhere, with rows that start on 16 bytes.
-__global__ void __launch_bounds__(256) fp4_align_kernel(const uint16_t *__restrict__ src, int64_t ld, uint32_t rows, uint32_t cols, uint4 *__restrict__ dst, uint32_t pieces) {
+__global__ void __launch_bounds__(256) fp4_align_kernel(const uint16_t *src, int64_t ld, uint32_t rows, uint32_t cols, uint4 *dst, uint32_t pieces) {
     ptx::wait_for_grids_before();
     for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < (uint64_t)rows * pieces; i += (uint64_t)gridDim.x * 256u) {
         const uint32_t row = (uint32_t)(i / pieces), col = (uint32_t)(i % pieces) * 8u;
         const uint16_t *from = src + (int64_t)row * ld + col;
-        uint16_t v[8];
+        alignas(16) uint16_t v[8];
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) v[e] = col + e < cols ? from[e] : (uint16_t)0;
         dst[i] = *reinterpret_cast<const uint4 *>(v);

@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + kNarrowLoaders), 1) fp4_n
                     if (p.d.b_wide) {
                         ptx::cp_async_16(to + at, left ? src : b, left * 2u);
                     } else {
-                        T v[8];
+                        alignas(16) T v[8];
 #pragma unroll
                         for (uint32_t e = 0; e < 8; ++e) v[e] = e < left ? src[e] : Elem<T>::from_float(0.f);
                         ptx::st_shared_v4(to + at, *reinterpret_cast<const uint4 *>(v));

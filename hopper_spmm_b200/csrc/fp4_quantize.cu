@@ -70,7 +70,7 @@ struct Raw16 {
             for (uint32_t i = 0; i < sizeof(T); ++i) v[i] = ptx::ld_global_v4(reinterpret_cast<const uint4 *>(src) + i);
         } else if (align >= 8u && count >= 16u) {
 #pragma unroll
-            for (uint32_t i = 0; i < 2 * sizeof(T); ++i) reinterpret_cast<uint2 *>(v)[i] = __ldg(reinterpret_cast<const uint2 *>(src) + i);
+            for (uint32_t i = 0; i < 2 * sizeof(T); ++i) reinterpret_cast<uint2 *>(v)[i] = reinterpret_cast<const uint2 *>(src)[i];
         } else {
             T *e = reinterpret_cast<T *>(v);
 #pragma unroll
@@ -126,8 +126,8 @@ struct Raw16 {
 
 // partial[block] = the largest finite magnitude that the block has seen.  Bound: one read of the matrix; 64 bytes a thread are under way.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) amax_kernel(const T *__restrict__ x, int64_t ldx, uint32_t rows, uint32_t cols, uint32_t align,
-                                                        float *__restrict__ partial) {
+__global__ void __launch_bounds__(kThreads) amax_kernel(const T *x, int64_t ldx, uint32_t rows, uint32_t cols, uint32_t align,
+                                                        float *partial) {
     constexpr int kAhead = sizeof(T) == 4 ? 1 : 2;
     __shared__ uint32_t shared[kThreads / 32];
     ptx::wait_for_grids_before();
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kThreads) amax_kernel(const T *__restrict__ x,
 // The same of rows that start on less than 8 bytes: a warp takes 512 of a row, lanes neighbours (28672 x 8191 fp16 quantised in 409 us, 535 with
 // 16 neighbours a lane).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) amax_any_kernel(const T *__restrict__ x, int64_t ldx, uint32_t rows, uint32_t cols, float *__restrict__ partial) {
+__global__ void __launch_bounds__(kThreads) amax_any_kernel(const T *x, int64_t ldx, uint32_t rows, uint32_t cols, float *partial) {
     __shared__ uint32_t shared[kThreads / 32];
     ptx::wait_for_grids_before();
     const uint32_t lane = threadIdx.x & 31u;
@@ -209,7 +209,7 @@ B200_DEVICE void quantize_unit(const Raw16<T> &raw, const TensorScale &tensor, b
 // products read, are zeros.  Bound: reading x once (after amax_kernel, which leaves its last rows in L2: they come first) and writing the
 // codes: 28672 x 8192 fp16 91 us in mxfp4, 6.5 TB/s; with the pass before it, 181 in nvfp4.
 template <typename T, bool kMx>
-__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T *__restrict__ x, int64_t ldx, const float *partial, uint32_t n_partial, const float *given,
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T *x, int64_t ldx, const float *partial, uint32_t n_partial, const float *given,
                                                                  const Dest d) {
     __shared__ uint32_t shared[kThreads / 32];
     ptx::wait_for_grids_before();
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T *__rest
 // (8 x 8192, the activations of eight tokens: 10 us a call, most of it the host's).
 constexpr unsigned kClusterCtas = 8, kClusterThreads = 1024;
 template <typename T>
-__global__ void __launch_bounds__(kClusterThreads) quantize_cluster_kernel(const T *__restrict__ x, int64_t ldx, const Dest d) {
+__global__ void __launch_bounds__(kClusterThreads) quantize_cluster_kernel(const T *x, int64_t ldx, const Dest d) {
     __shared__ uint32_t shared[kClusterThreads / 32], all[kClusterCtas];
     ptx::cluster_arrive();  // no CTA writes to another one's shared memory before that one runs
     ptx::cluster_wait();
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kClusterThreads) quantize_cluster_kernel(const
 constexpr uint32_t kTileR = 128, kTileC = 64, kOutPitch = kTileR / 2 + 16;
 
 template <typename T, bool kMx, bool kRows, bool kCols>
-__global__ void __launch_bounds__(kThreads, 4) quantize_tiles_kernel(const T *__restrict__ x, int64_t ldx, uint32_t x_rows, uint32_t x_cols, uint32_t align,
+__global__ void __launch_bounds__(kThreads, 4) quantize_tiles_kernel(const T *x, int64_t ldx, uint32_t x_rows, uint32_t x_cols, uint32_t align,
                                                                   const float *partial, uint32_t n_partial, const float *given, const Dest by_rows,
                                                                   const Dest by_cols, uint32_t tiles_c, uint64_t tiles) {
     constexpr uint32_t kPer = 16 / sizeof(T), kVecs = kTileC / kPer;  // elements of a piece, pieces of a row
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_tiles_kernel(const T *__
         for (uint32_t i = 0; i < kLoads; ++i) {
             const uint32_t r = (i * kThreads + tid) / kRow, c = (i * kThreads + tid) % kRow * kIn;
             v[i] = V();
-            if (r0 + r < x_rows) v[i] = __ldg(reinterpret_cast<const V *>(x + (int64_t)(r0 + r) * ldx + c0 + c));
+            if (r0 + r < x_rows) v[i] = *reinterpret_cast<const V *>(x + (int64_t)(r0 + r) * ldx + c0 + c);
         }
 #pragma unroll
         for (uint32_t i = 0; i < kLoads; ++i) {
@@ -411,9 +411,9 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_tiles_kernel(const T *__
 // shuffles and leave 32 neighbours at a time.  Bound: reading the matrix and writing x once:
 // 28672 x 8192 nvfp4 118 us to fp16, 191 to fp32, 5.1 and 5.6 TB/s.
 template <typename T, bool kMx, bool kWide>
-__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t *__restrict__ values, const uint8_t *__restrict__ scales,
-                                                              const float *__restrict__ tensor_scale, uint32_t rows, uint32_t cols, uint32_t pitch,
-                                                              uint32_t groups, T *__restrict__ x, int64_t ldx) {
+__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t *values, const uint8_t *scales,
+                                                              const float *tensor_scale, uint32_t rows, uint32_t cols, uint32_t pitch,
+                                                              uint32_t groups, T *x, int64_t ldx) {
     constexpr uint32_t kAhead = 4;
     ptx::wait_for_grids_before();
     const uint32_t lane = threadIdx.x & 31u;
@@ -428,8 +428,8 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t *__r
             const uint32_t block = col[a] / (kMx ? 32u : 16u);
             codes[a] = bytes[a] = 0u;
             if (w.row < rows && col[a] < cols) {
-                codes[a] = __ldg(reinterpret_cast<const uint32_t *>(values + (uint64_t)row[a] * pitch + col[a] / 2u));
-                bytes[a] = __ldg(scales + scale_word(row[a], block / 4u, groups) + block % 4u);
+                codes[a] = *reinterpret_cast<const uint32_t *>(values + (uint64_t)row[a] * pitch + col[a] / 2u);
+                bytes[a] = scales[scale_word(row[a], block / 4u, groups) + block % 4u];
             }
             w.next();
         }

@@ -82,8 +82,8 @@ B200_DEVICE Item split_item(const Split &s, uint32_t i) {
 constexpr uint32_t kJoinCols = 8;
 // C of the tiles that were cut: the parts' sums in order.  A thread a row and 8 columns: few loads are under way
 // in all, and with 32 they were behind one another.
-static __global__ void __launch_bounds__(kPairRows4) fp4_join_kernel(const Split s, const float *__restrict__ partial, uint32_t m, uint32_t n, const float *__restrict__ a_whole,
-                                                             const float *__restrict__ b_whole, float left, const Target c) {
+static __global__ void __launch_bounds__(kPairRows4) fp4_join_kernel(const Split s, const float *partial, uint32_t m, uint32_t n, const float *a_whole,
+                                                             const float *b_whole, float left, const Target c) {
     ptx::wait_for_grids_before();
     const Factor f(a_whole ? *reinterpret_cast<const volatile float *>(a_whole) : 1.f, b_whole ? *reinterpret_cast<const volatile float *>(b_whole) : left);
     const uint32_t col = blockIdx.y * kJoinCols;

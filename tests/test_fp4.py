@@ -167,3 +167,18 @@ def test_the_starving_of_products_takes_a_limit_and_an_operand():
     starve = capi.lib().b200spmm_kat_fp4_starve
     assert starve(2_000_000_001, 0) == starve(1, 2) == starve(1, -1) == capi.ERR_INVALID_ARG
     assert starve(5_000_000, 1) == starve(0, 0) == capi.OK
+
+
+def test_no_kernel_reads_through_the_read_only_path():
+    # What the kernels read may be written while they start (they wait for it inside); a load through the read-only path, or one that the compiler
+    # may take for such (const and restrict), could be moved before that wait.
+    import glob
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.abspath(hs.__file__)), "csrc")
+    files = sorted(glob.glob(os.path.join(csrc, "fp4*")))
+    assert len(files) >= 10
+    for f in files:
+        with open(f) as source:
+            found = re.findall(r"__ldg\w*|__restrict\w*|\w*global_nc\w*|ld\.global\.nc", source.read())
+        assert not found, (f, found)
