@@ -13,10 +13,10 @@ namespace b200spmm {
 namespace fp4 {
 namespace {
 
-template <typename T, bool kMx, int kNB, bool kTokens>
+template <typename T, bool kMx, int kNB, bool kTokens, bool kExact>
 int launch_narrow(const b200spmm_fp4_t *a, const DenseParams &d, cudaStream_t stream) {
     constexpr uint32_t kMostBytes = 226u * 1024u;
-    auto kernel = fp4_narrow_kernel<T, kMx, kNB, kTokens>;
+    auto kernel = fp4_narrow_kernel<T, kMx, kNB, kTokens, kExact>;
     static thread_local int configured = -1;
     if (configured != a->device) {
         B200_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostBytes));
@@ -49,7 +49,8 @@ int launch_narrow(const b200spmm_fp4_t *a, const DenseParams &d, cudaStream_t st
 
 template <typename T, bool kMx, bool kTokens>
 int launch_narrow_columns(const b200spmm_fp4_t *a, const DenseParams &d, cudaStream_t stream) {
-    return d.n <= 8 ? launch_narrow<T, kMx, 1, kTokens>(a, d, stream) : launch_narrow<T, kMx, 2, kTokens>(a, d, stream);
+    if (d.c.type == B200SPMM_T_F32) return d.n <= 8 ? launch_narrow<T, kMx, 1, kTokens, true>(a, d, stream) : launch_narrow<T, kMx, 2, kTokens, true>(a, d, stream);
+    return d.n <= 8 ? launch_narrow<T, kMx, 1, kTokens, false>(a, d, stream) : launch_narrow<T, kMx, 2, kTokens, false>(a, d, stream);
 }
 
 // Columns shared out evenly over as few tiles as there can be, 64 at least (fewer take longer: 24 with 28672 x 8192 88 us as 32, 66 as 64); a

@@ -32,6 +32,7 @@ constexpr uint32_t kNarrowStep = 128, kNarrowStage = 256;  // values of k
 constexpr uint32_t kNarrowTiles = 13;                      // of 16 rows at a time
 constexpr uint32_t kNarrowWarps = 26, kNarrowLoaders = 3;  // that multiply, at most, and load
 constexpr uint32_t kNarrowMaxStages = 8;
+constexpr uint32_t kNarrowRun = 4;                         // steps of a warp between two roundings of its sums, for an fp32 C
 
 struct NarrowParams {
     DenseParams d;
@@ -68,8 +69,10 @@ B200_DEVICE void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
-// kNB: columns / 8.  kTokens: B lies [n][k], else [k][n].
-template <typename T, bool kMx, int kNB, bool kTokens>
+// kNB: columns / 8.  kTokens: B lies [n][k], else [k][n].  kExact: an fp32 C.  mma.sync cuts its sums off as tcgen05.mma does (fp4_dense_wide.cuh):
+// the 4,096 values of k that a warp has of 28672 x 8192 left them off by 3.5e-6 of their size.  They are therefore added, rounded, to others every
+// 512: 3e-7, for 0 to 2.6 us of 33 to 58.
+template <typename T, bool kMx, int kNB, bool kTokens, bool kExact>
 __global__ void __launch_bounds__(32 * (kNarrowWarps + kNarrowLoaders), 1) fp4_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const NarrowParams p) {
     using W = Widen<T, kMx>;
     constexpr uint32_t kGroups = kMx ? 2 : 4, kCols = 8 * kNB, kStepB = kNB * kNarrowStep * 16u;
@@ -184,8 +187,9 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + kNarrowLoaders), 1) fp4_n
             // the words of scales of rows `row` and `row` + 8; those of a tile past the end may be anywhere in the stage
             auto scale_at = [&](uint32_t r) { return size.values + (busy ? r / 128u - m0 / 128u : 0u) * (kGroups * 512u) + (r & 31u) * 16u + (r >> 5 & 3u) * 4u; };
             const uint32_t lo_at = scale_at(row), hi_at = scale_at(row + 8u);
-            float acc[kNB][4] = {};
+            float acc[kNB][4] = {}, sum[kNB][4] = {};
             uint32_t turn = slice;  // steps until this warp's next one
+            uint32_t taken = 0;     // steps that are in `acc`
             for (uint32_t ks = 0; ks < k_stages; ++ks) {
                 alive = wait(full + 8u * s, phase);
                 if (!alive) break;
@@ -238,10 +242,26 @@ __global__ void __launch_bounds__(32 * (kNarrowWarps + kNarrowLoaders), 1) fp4_n
                     };
                     if (kMx && __any_sync(0xFFFFFFFFu, W::needs_two(f_lo) || W::needs_two(f_hi))) multiply(std::true_type());
                     else multiply(std::false_type());
+                    if (kExact && ++taken == kNarrowRun) {
+                        taken = 0;
+#pragma unroll
+                        for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e) {
+                                sum[nb][e] += acc[nb][e];
+                                acc[nb][e] = 0.f;
+                            }
+                    }
                 }
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(empty + 8u * s);
                 step_on();
+            }
+            if constexpr (kExact) {
+#pragma unroll
+                for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) acc[nb][e] += sum[nb][e];
             }
             // ---- to C, over shared memory where k was sliced: [warp][column][row].  A warp whose wait gave up comes to the barrier as well: the
             // others, whose waits may have ended in time, count on it there, and no wait of theirs would end it.  All leave then.

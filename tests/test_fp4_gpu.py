@@ -726,3 +726,38 @@ def test_waiting_for_a_stream_that_is_captured_is_refused():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+# What an MMA drops of a sum is anywhere between nothing and 2^-23 of it, half of that on the average.  Over a run of MMAs of random values the sum
+# grows with the root, and the mean of its size is 2/3 of its last: runs of r MMAs leave r/3 * 2^-23 of the run.  Runs, and what they leave, add
+# like one another; their rounded additions, of either sign, leave less than one 2^-23 more.
+def left_by_runs(mmas):
+    return (mmas / 3 + 1) * 2.0 ** -23
+
+
+@pytest.mark.parametrize("fmt,dtype", [("nvfp4", F16), ("nvfp4", BF16), ("mxfp4", BF16)], ids=str)
+@pytest.mark.parametrize("rows", [700, 28672])
+def test_sums_of_fp32_results_of_few_columns(rows, fmt, dtype):
+    # whatever share of k a warp has (all rows are multiplied; some hundred are looked at): 512 values of k, 16 an MMA, a run
+    k = 8192
+    W = hs.fp4_quantize(normal(rows, k, 1, spread=k ** -0.5), fmt)
+    at = torch.arange(0, rows, max(1, rows // 700), device="cuda")
+    a = W.dequantize()[at].double()
+    for n in (1, 8, 16):
+        x = normal(k, n, 2, dtype)
+        want = a @ x.double()
+        error = float((W.matmul(x)[at].double() - want).norm() / want.norm())
+        assert error <= left_by_runs(32), (n, error)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_sums_of_fp32_results_of_two_matrices(fmt):
+    # all of k in one accumulator, 64 values of it an MMA
+    k = 8192
+    W = hs.fp4_quantize(normal(700, k, 1, spread=k ** -0.5), fmt)
+    a = ref.matrix_values(W)
+    for n in (8, 50, 300):
+        X = hs.fp4_quantize(normal(n, k, 2), fmt)
+        want = a @ ref.matrix_values(X).t()
+        error = float((W.matmul(X).double() - want).norm() / want.norm())
+        assert error <= left_by_runs(k // 64), (n, error)
