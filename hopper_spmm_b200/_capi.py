@@ -130,6 +130,7 @@ SIGNATURES = {
     "b200spmm_kat_umma": (C.c_int, [vp, u32, C.POINTER(KatMma), C.c_int, C.c_int, vp, C.c_int]),
     "b200spmm_kat_umma_pair": (C.c_int, [vp, u32, C.POINTER(KatMma), C.c_int, C.c_int, vp, C.c_int]),
     "b200spmm_kat_wait_limit": (C.c_uint64, [C.c_uint64]),
+    "b200spmm_kat_fp4_narrow_share": (C.c_int, [u64, u64, u32] + [C.POINTER(u32)] * 4),
     "b200spmm_kat_fp4_starve": (C.c_int, [C.c_uint64, C.c_int]),
     "b200spmm_kat_spmm_starved": (C.c_int, [vp, vp, i64, i64, vp, i64, C.c_uint64, vp]),
     "b200spmm_kat_scratch_limit": (C.c_int, [vp, C.c_uint64]),

@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "../../include/b200_spmm_kat.h"
 #include "common.hpp"
 #include "fp4.hpp"
 #include "fp4_dense_narrow.cuh"
@@ -27,10 +28,9 @@ int launch_narrow(const b200spmm_fp4_t *a, const DenseParams &d, cudaStream_t st
     NarrowParams prm{};
     prm.d = d;
     prm.tiles = (d.m + 15u) / 16u;
-    // a block's tiles, each sliced as far as there are warps and steps
-    const uint32_t blocks = std::min(prm.tiles, (uint32_t)sm_count()), of_block = (prm.tiles + blocks - 1) / blocks;
-    prm.at_once = std::min(of_block, kNarrowTiles);
-    prm.slices = std::max<uint32_t>(1, std::min(kNarrowWarps / prm.at_once, (d.k + kNarrowStep - 1) / kNarrowStep));
+    const NarrowShare share = narrow_share(prm.tiles, d.k, (uint32_t)sm_count());
+    prm.at_once = share.at_once;
+    prm.slices = share.slices;
     prm.row_blocks = (prm.at_once * 16u + 126u) / 128u + 1u;
     const uint32_t stage = narrow_stage(kMx, prm.at_once, prm.row_blocks, kNB).bytes(), warps = prm.at_once * prm.slices;
     const uint32_t sums = prm.slices > 1 ? warps * 16u * 8u * kNB * (uint32_t)sizeof(float) : 0u;
@@ -43,7 +43,7 @@ int launch_narrow(const b200spmm_fp4_t *a, const DenseParams &d, cudaStream_t st
         set_last_error_static("a tensor map of a 4-bit matrix could not be made");
         return B200SPMM_ERR_CUDA;
     }
-    B200_CUDA_TRY(launch_after(kernel, dim3(blocks, passes), 32 * (warps + kNarrowLoaders), 1280u + prm.stages * stage + sums, 1, stream, ma, prm));
+    B200_CUDA_TRY(launch_after(kernel, dim3(share.blocks, passes), 32 * (warps + kNarrowLoaders), 1280u + prm.stages * stage + sums, 1, stream, ma, prm));
     return B200SPMM_OK;
 }
 
@@ -199,3 +199,15 @@ int launch_dense_product(const b200spmm_fp4_t *a, const void *b, int64_t ldb, in
 
 }  // namespace fp4
 }  // namespace b200spmm
+
+/* Declared in b200_spmm_kat.h: how a product with few 16-bit columns is shared out. */
+extern "C" int b200spmm_kat_fp4_narrow_share(uint64_t rows, uint64_t cols, uint32_t sms, uint32_t *blocks, uint32_t *rounds, uint32_t *at_once, uint32_t *slices) {
+    using namespace b200spmm::fp4;
+    if (!rows || !cols || rows > 0x7FFFFFFFull - 128 || cols > 0x7FFFFFFFull - 256 || !sms || !blocks || !rounds || !at_once || !slices) return B200SPMM_ERR_INVALID_ARG;
+    const NarrowShare s = narrow_share((uint32_t)((rows + 15) / 16), (uint32_t)cols, sms);
+    *blocks = s.blocks;
+    *rounds = s.rounds;
+    *at_once = s.at_once;
+    *slices = s.slices;
+    return B200SPMM_OK;
+}

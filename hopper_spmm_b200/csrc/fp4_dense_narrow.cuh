@@ -6,9 +6,9 @@
 // become 16-bit numbers in registers and meet eight columns of B at a time there (mma.sync, 16 rows x 8 columns x 16 values of k;
 // at this width a product is a small part of the work, and for tcgen05 the numbers would have to go through shared or tensor memory).
 //
-// Tiles of 16 rows are shared out evenly over the SMs, one block of threads each, which goes through k with up to 13 of them at a time: one warp
+// Tiles of 16 rows are shared out evenly over the SMs, one block of threads each, which goes through k with up to 14 of them at a time: one warp
 // brings stages of 256 values of k of all their rows, two take turns with the same of B, put in the order of the MMAs' operands (one
-// alone kept the others waiting, 5 us for 8,192 values of k), and 26 multiply, a tile or, k being sliced, a part of one each.  The slices' sums meet in shared memory, in order, at the end.  (Row blocks of
+// alone kept the others waiting, 5 us for 8,192 values of k), and up to 28 multiply, a tile or, k being sliced, a part of one each.  The slices' sums meet in shared memory, in order, at the end.  (Row blocks of
 // 128 whose eight warps sliced k and fetched for themselves came to 38 us for 28672 x 8192 times one column: 224 blocks on 148 SMs, and 18
 // operations for eight values.)  28672 x 8192 nvfp4, whose 132 MB take 20 us to read: one column in fp16 33 us, 8 35, 16 47; in bf16, which takes
 // twice the operations to widen, 50, 50 and 60.
@@ -29,8 +29,9 @@ namespace b200spmm {
 namespace fp4 {
 
 constexpr uint32_t kNarrowStep = 128, kNarrowStage = 256;  // values of k
-constexpr uint32_t kNarrowTiles = 13;                      // of 16 rows at a time
-constexpr uint32_t kNarrowWarps = 26, kNarrowLoaders = 3;  // that multiply, at most, and load
+constexpr uint32_t kNarrowTiles = 14;                      // of 16 rows at a time, at most: two warps for each, and those that load, are a block's 32
+constexpr uint32_t kNarrowWarps = 2 * kNarrowTiles, kNarrowLoaders = 3;  // that multiply, at most, and load
+static_assert(kNarrowWarps + kNarrowLoaders <= 32 && 2 * (kNarrowTiles + 1) + kNarrowLoaders > 32 && 16 * kNarrowTiles <= 256, "a block's warps, a box's rows");
 constexpr uint32_t kNarrowMaxStages = 8;
 constexpr uint32_t kNarrowRun = 4;                         // steps of a warp between two roundings of its sums, for an fp32 C
 
@@ -44,6 +45,22 @@ struct NarrowParams {
     uint32_t* status;
     unsigned long long wait_limit_ns;
 };
+
+// How a block's tiles are gone through: as many at a time in every round (x 8192 times one fp16 column: 32,000 rows as 13 tiles and 1 of 14 took 59 us, as
+// 14 35; 66,304 as 13, 13 and 2 86, as 14 and 14 62), each sliced as far as there are steps and warps: two for a tile, or 26 in all.  (28 in all: 2048
+// rows 11.8 us for 11.3, 14336 times 16 columns 32.3 for 30.8; 4096 times 16 24.4 for 25.1.)
+struct NarrowShare {
+    uint32_t blocks, rounds, at_once, slices;
+};
+inline NarrowShare narrow_share(uint32_t tiles, uint32_t k, uint32_t sms) {
+    NarrowShare s{};
+    s.blocks = std::min(tiles, sms);
+    const uint32_t of_block = (tiles + s.blocks - 1) / s.blocks;
+    s.rounds = (of_block + kNarrowTiles - 1) / kNarrowTiles;
+    s.at_once = (of_block + s.rounds - 1) / s.rounds;
+    s.slices = std::max<uint32_t>(1, std::min(std::max(2u, 26u / s.at_once), (k + kNarrowStep - 1) / kNarrowStep));
+    return s;
+}
 
 // Bytes of a stage: values, scales, B.
 struct NarrowStage {

@@ -82,6 +82,13 @@ int b200spmm_kat_spmm_starved(struct b200spmm_plan *plan, const void *d_B, int64
 int b200spmm_kat_fp4_starve(unsigned long long limit_ns, int operand);
 
 /*
+ * How the product of a rows x cols 4-bit matrix with up to 16 columns of 16 bits is shared out on a GPU of `sms` multiprocessors: blocks of
+ * threads, each of which goes through its tiles of 16 rows in `rounds` of at most `at_once`, with `slices` warps for a tile.  Needs no device.
+ */
+int b200spmm_kat_fp4_narrow_share(uint64_t rows, uint64_t cols, uint32_t sms, uint32_t *blocks, uint32_t *rounds, uint32_t *at_once,
+                                  uint32_t *slices);
+
+/*
  * From here on a launch of `plan` that needs a scratch buffer of more than `bytes` asks for more memory than any device
  * has, and finds none, as where others hold it.  A buffer that is there and large enough serves on.
  */

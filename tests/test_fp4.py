@@ -182,3 +182,18 @@ def test_no_kernel_reads_through_the_read_only_path():
         with open(f) as source:
             found = re.findall(r"__ldg\w*|__restrict\w*|\w*global_nc\w*|ld\.global\.nc", source.read())
         assert not found, (f, found)
+
+
+@pytest.mark.parametrize("sms", [148, 132, 7])
+def test_few_columns_are_shared_out_evenly(sms):
+    # no round goes through all of k for a few tiles left over: all rounds together have room for less than one tile a round more than there are
+    for rows in [1, 16, 17, 128, 1000, 2048, 4096, 14331, 28672, 30000, 32000, 32768, 50257, 57344, 128256, 151936, 256000, 1000003]:
+        for cols in (1, 100, 4096):
+            out = [C.c_uint32() for _ in range(4)]
+            assert capi.lib().b200spmm_kat_fp4_narrow_share(rows, cols, sms, *(C.byref(o) for o in out)) == capi.OK
+            blocks, rounds, at_once, slices = (o.value for o in out)
+            tiles = -(-rows // 16)
+            most = -(-tiles // blocks)  # of a block
+            assert blocks == min(tiles, sms) and most <= rounds * at_once < most + rounds
+            assert 1 <= slices <= max(1, -(-cols // 128)) and at_once * slices + 3 <= 32 and at_once * 16 <= 256
+    assert capi.lib().b200spmm_kat_fp4_narrow_share(16, 16, 0, *(C.byref(o) for o in out)) == capi.ERR_INVALID_ARG

@@ -761,3 +761,16 @@ def test_sums_of_fp32_results_of_two_matrices(fmt):
         want = a @ ref.matrix_values(X).t()
         error = float((W.matmul(X).double() - want).norm() / want.norm())
         assert error <= left_by_runs(k // 64), (n, error)
+
+
+@pytest.mark.parametrize("fmt,dtype", [("nvfp4", F16), ("mxfp4", BF16)], ids=str)
+@pytest.mark.parametrize("rows", [28672, 31000, 32777, 34000, 66300, 128256])
+def test_few_columns_of_matrices_of_many_rows(rows, fmt, dtype):
+    # blocks with one to several rounds of tiles, of different sizes
+    W = hs.fp4_quantize(normal(rows, 300, 1), fmt)
+    a = ref.matrix_values(W)
+    for n in (1, 7, 16):
+        x = normal(300, n, 2, dtype)
+        for out in (F32, dtype):
+            ref.check_product(W.matmul(x, dtype=out), a, x.double(), 16)
+            ref.check_product(W.matmul(x.t().contiguous().t(), dtype=out), a, x.double(), 16)
