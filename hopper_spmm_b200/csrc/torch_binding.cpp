@@ -110,11 +110,11 @@ PyObject *spmm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
 
 // ---- 4-bit matrices.  A matrix is (values, scales, tensor_scale, rows, cols, format) in the arguments.
 
-// An argument that is a CUDA tensor, or null.
+// An argument that is a CUDA tensor, or null.  One whose numbers are to be negated when they are read (the imaginary part of a conjugate) is none.
 const at::Tensor *cuda_tensor(PyObject *o) {
     if (!THPVariable_Check(o)) return nullptr;
     const at::Tensor &t = THPVariable_Unpack(o);
-    return t.is_cuda() ? &t : nullptr;
+    return t.is_cuda() && !t.is_neg() ? &t : nullptr;
 }
 
 int type_code(at::ScalarType t) {

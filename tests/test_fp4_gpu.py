@@ -774,3 +774,25 @@ def test_few_columns_of_matrices_of_many_rows(rows, fmt, dtype):
         for out in (F32, dtype):
             ref.check_product(W.matmul(x, dtype=out), a, x.double(), 16)
             ref.check_product(W.matmul(x.t().contiguous().t(), dtype=out), a, x.double(), 16)
+
+
+@pytest.mark.filterwarnings("ignore:ComplexHalf")
+def test_a_tensor_with_a_pending_negation_is_refused():
+    # the imaginary part of a conjugate: torch keeps the numbers as they were and a mark that they are to be negated
+    z = torch.complex(normal(40, 1, 1), normal(40, 1, 2))
+    x = z.conj().imag
+    assert x.is_neg() and not x.resolve_neg().is_neg()
+    for call in (lambda: hs.fp4_quantize(x), lambda: hs.fp4_quantize(x, axis=0), lambda: hs.fp4_quantize_both(x, "mxfp4")):
+        with pytest.raises(ValueError, match="X must be"):
+            call()
+    check_quantized(hs.fp4_quantize(x.resolve_neg()), x.resolve_neg())
+    W = hs.fp4_quantize(normal(1, 40, 3))
+    y = torch.complex(normal(40, 1, 1).half(), normal(40, 1, 2).half()).conj().imag
+    with pytest.raises(ValueError, match="B must be"):
+        W.matmul(y)
+    ref.check_product(W.matmul(y.resolve_neg()), ref.matrix_values(W), y.resolve_neg().double(), 16)
+    c = torch.complex(normal(1, 1, 1), normal(1, 1, 2)).conj().imag
+    with pytest.raises(ValueError, match="C has"):
+        W.matmul(y.resolve_neg(), c, dtype=F32)
+    with pytest.raises(ValueError, match="C has"):
+        hs.fp4_quantize(normal(1, 1, 3)).dequantize(c)
