@@ -2,16 +2,17 @@
 //
 //     C[m, 0..n) = s_A  sum over k  (a[m, k] sa[m, k / block]) B[k, 0..n)
 //
-// Bound: one read of A, and nearly as much the widening of its codes, a dozen operations for eight values whatever n is.  Codes
-// become 16-bit numbers in registers and meet eight columns of B at a time there (mma.sync, 16 rows x 8 columns x 16 values of k;
+// Bound: one read of A; what it waits for is latency.  The widening of its codes, a dozen operations for eight values whatever n is, fills half of the
+// issue slots (52 % with 8 columns of fp16) while memory gives 61 % of its rate: a warp has one step between two waits for a stage that all of them
+// share.  Codes become 16-bit numbers in registers and meet eight columns of B at a time there (mma.sync, 16 rows x 8 columns x 16 values of k;
 // at this width a product is a small part of the work, and for tcgen05 the numbers would have to go through shared or tensor memory).
 //
 // Tiles of 16 rows are shared out evenly over the SMs, one block of threads each, which goes through k with up to 14 of them at a time: one warp
 // brings stages of 256 values of k of all their rows, two take turns with the same of B, put in the order of the MMAs' operands (one
 // alone kept the others waiting, 5 us for 8,192 values of k), and up to 28 multiply, a tile or, k being sliced, a part of one each.  The slices' sums meet in shared memory, in order, at the end.  (Row blocks of
 // 128 whose eight warps sliced k and fetched for themselves came to 38 us for 28672 x 8192 times one column: 224 blocks on 148 SMs, and 18
-// operations for eight values.)  28672 x 8192 nvfp4, whose 132 MB take 20 us to read: one column in fp16 33 us, 8 35, 16 47; in bf16, which takes
-// twice the operations to widen, 50, 50 and 60.
+// operations for eight values.)  28672 x 8192 nvfp4, whose 132 MB take 20 us to read: one column in fp16 33 us, 8 34, 16 47; in bf16, which takes
+// twice the operations to widen, 50, 48 and 57.
 //
 // Lane 4 g + t takes 16 bytes of values, 32 codes, of rows r(g) and r(g) + 8 of its tile from k = 32 t of a step of 128 on; r puts rows that are
 // four apart side by side, whose pieces of a step lie in different halves of the swizzled 128 bytes.  Which k an operand

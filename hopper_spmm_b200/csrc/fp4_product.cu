@@ -217,6 +217,8 @@ int launch_width(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, const Product
 }
 
 // Tiles of 128 or 256 columns, the scales' blocks being 128 rows long, with fewer columns past the end; a single tile as wide as it has to be.
+// A step of 256 values of k of tiles that fill the GPU (18,944 rows) measured 0.56 us with 96 columns and 0.63 with 256 in nvfp4, 0.53 and 0.60 in mxfp4;
+// the estimates are a third below that, so that tiles are cut a little later than they might; a part has at least 512 values of k.
 Split pair_split(uint32_t m, uint32_t n, uint32_t k, uint32_t pairs) {
     const uint32_t cols = n <= kPairCols4 ? (n + 31u) / 32u * 32u : (n + 127u) / 128u * 128u < (n + 255u) / 256u * 256u ? 128u : 256u;
     return make_split(m, n, cols, (k + kStageK - 1) / kStageK, 2, 0.45, 0.35, 256 * kStageK * 9 / 16, pairs);

@@ -259,8 +259,8 @@ __global__ void __launch_bounds__(kClusterThreads) quantize_cluster_kernel(const
 // any element.  A block of threads takes 128 x 64 of x through shared memory, where it is read along either axis: columns two at a time and 16
 // rows a thread, the other 16 of an mxfp4 block being 16 lanes away.  Rows lie in shared memory with their halves exchanged
 // where bit 4 of their number is set, so that those lanes do not collide.  What goes to the transpose is put together there as
-// well, and leaves 64 neighbouring bytes at a time.  Bound: shared memory and issue: 28672 x 8192 fp16 to the transpose 135 us in mxfp4, both
-// ways with the largest value's pass 311 in nvfp4, of which two reads and the writing would be 236.
+// well, and leaves 64 neighbouring bytes at a time.  Bound: shared memory and issue: 28672 x 8192 fp16 to the transpose 134 us in mxfp4, of
+// which one read and the writing would be 91; both ways with the largest value's pass 307 in nvfp4, of which two reads and the writing would be 184.
 constexpr uint32_t kTileR = 128, kTileC = 64, kOutPitch = kTileR / 2 + 16;
 
 template <typename T, bool kMx, bool kRows, bool kCols>
@@ -409,7 +409,8 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_tiles_kernel(const T *x,
 
 // A thread takes eight values, a word of codes, and writes them in one piece; where rows start anywhere, a warp's 256 values go through
 // shuffles and leave 32 neighbours at a time.  Bound: reading the matrix and writing x once:
-// 28672 x 8192 nvfp4 118 us to fp16, 191 to fp32, 5.1 and 5.6 TB/s.
+// 28672 x 8192 nvfp4 117 us to fp16, 187 to fp32, 5.1 and 5.7 TB/s; to fp32 rows that start anywhere, 4090 x 5001
+// mxfp4, 31, where its bytes are 14: the shuffles.
 template <typename T, bool kMx, bool kWide>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t *values, const uint8_t *scales,
                                                               const float *tensor_scale, uint32_t rows, uint32_t cols, uint32_t pitch,

@@ -182,8 +182,10 @@ def _quantized(X, format, tensor_scale, by_rows, by_cols):
 
 def fp4_quantize(X, format: str = "nvfp4", axis: int = 1, tensor_scale=None, out: Fp4Matrix | None = None, stream=None) -> Fp4Matrix:
     """X in 4 bits.  ``axis`` 1: blocks along X's rows, a matrix of X's shape; 0: along its columns, and the matrix is X's
-    transpose (the axis that a product sums over has to be the matrix's rows).  ``tensor_scale``: for nvfp4, a float32 tensor of
-    one element (say, calibrated) in place of a pass over X for its largest value.  ``out``: a matrix to fill, else a new one."""
+    transpose (the axis that a product sums over has to be the matrix's rows).  ``tensor_scale``: for nvfp4 (mxfp4 has none), a
+    positive float32 tensor of one element, say a calibrated one, in place of a pass over X for its largest value.  It is rounded
+    up to a power of two, which is the scale that X gets: codes and block scales are those for that one, not for the number as
+    it was given.  ``out``: a matrix to fill, else a new one."""
     if axis not in (0, 1):
         raise ValueError("axis must be 0 or 1")
     if stream is not None:
@@ -201,8 +203,9 @@ def fp4_quantize(X, format: str = "nvfp4", axis: int = 1, tensor_scale=None, out
 
 
 def fp4_quantize_both(X, format: str = "nvfp4", tensor_scale=None, stream=None) -> tuple[Fp4Matrix, Fp4Matrix]:
-    """``fp4_quantize(X, axis=1)`` and ``fp4_quantize(X, axis=0)`` from one read of X: what training needs.  For Y = X Wᵀ the
-    forward pass sums over X's columns, the weights' gradient dYᵀ X over its rows:
+    """``fp4_quantize(X, axis=1)`` and ``fp4_quantize(X, axis=0)`` from one read of X (nvfp4 without ``tensor_scale`` reads it for its
+    largest value before): what training needs.  For Y = X Wᵀ the forward pass sums over X's columns, the weights' gradient dYᵀ X
+    over its rows:
 
         X, Xt = fp4_quantize_both(x);  W, Wt = fp4_quantize_both(w);  dY, dYt = fp4_quantize_both(dy)
         y, dx, dw = X.matmul(W), dY.matmul(Wt), dYt.matmul(Xt)

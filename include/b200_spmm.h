@@ -549,7 +549,7 @@ int b200spmm_fp4_product(const b200spmm_fp4_t *a, const b200spmm_fp4_t *b, void 
 
 /*
  * C[a.rows, n] = A B with B [a.cols, n] in fp16 or bf16 (MXFP4: bf16, whose range its scales have; else
- * B200SPMM_ERR_UNSUPPORTED); sums in fp32.  B and C have ldb and ldc elements between rows, or, where transposed, between columns:
+ * B200SPMM_ERR_UNSUPPORTED); sums in fp32.  Values of A beyond bf16's range, 2 x 2^127 and more in MXFP4, are infinite.  B and C have ldb and ldc elements between rows, or, where transposed, between columns:
  * activations that lie token by token.  Any n, strides and alignment of B and C to their element; starts and strides that are
  * multiples of 16 bytes are faster.
  */

@@ -197,3 +197,12 @@ def test_few_columns_are_shared_out_evenly(sms):
             assert blocks == min(tiles, sms) and most <= rounds * at_once < most + rounds
             assert 1 <= slices <= max(1, -(-cols // 128)) and at_once * slices + 3 <= 32 and at_once * 16 <= 256
     assert capi.lib().b200spmm_kat_fp4_narrow_share(16, 16, 0, *(C.byref(o) for o in out)) == capi.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("rows,blocks", [(1, 1), (128, 4), (130, 5), (300, 33)])
+def test_scales_that_lie_row_by_row_are_brought_into_order(rows, blocks):
+    # the two lines that the documents give for checkpoints
+    s = torch.randint(0, 127, (rows, blocks), dtype=torch.uint8, generator=torch.Generator().manual_seed(rows))
+    R, G = -(-rows // 128), -(-s.shape[1] // 4)
+    scales = torch.nn.functional.pad(s, (0, G * 4 - s.shape[1], 0, R * 128 - rows)).view(R, 4, 32, G, 4).permute(0, 3, 2, 1, 4).reshape(-1)
+    assert torch.equal(scales, ref.pack(torch.zeros(rows, blocks * 16, dtype=torch.uint8), s, "nvfp4")[1])
