@@ -85,7 +85,8 @@ def draw(rng):
 
     if op == "norm":
         dtype = rng.choice(["f32", "f16", "bf16"])
-        return _norm(None, size(1, 8192), size(64, 8192), dtype, rng.choice(["", "f32", dtype]), rng.choice(["e4m3", "e4m3", dtype]), rng.choice([0, 32, 64, 128]))
+        out = rng.choice(["e4m3", "e4m3", dtype])
+        return _norm(None, size(1, 8192), size(64, 8192), dtype, rng.choice(["", "f32", dtype]), out, rng.choice([0, 32, 64, 128]) if out == "e4m3" else 0)
     if op == "int4":
         return _int4(None, size(256, 28672), size(128, 8192), _log_int(rng, 1, 33), rng.choice([32, 64, 128]), dtype, rng.choice([dtype, "f32"]), rng.random() < 0.5,
                      rng.choice([-1, -1, 0, 32, 64, 128]))
