@@ -13,7 +13,7 @@ ERR_INVALID_ARG, ERR_BAD_CSR, ERR_UNSUPPORTED, ERR_NO_MEMORY, ERR_CUDA, ERR_NO_D
 F16, TF32 = 0, 1
 C_F32, C_F16 = 0, 1
 NVFP4, MXFP4 = 0, 1
-T_F32, T_F16, T_BF16 = 0, 1, 2
+T_F32, T_F16, T_BF16, T_E4M3 = 0, 1, 2, 3
 
 u64, i64, u32, i32, vp = C.c_uint64, C.c_int64, C.c_uint32, C.c_int32, C.c_void_p
 
@@ -31,6 +31,11 @@ class LaunchInfo(C.Structure):
 
 class Fp4(C.Structure):
     _fields_ = [("rows", u64), ("cols", u64), ("format", i32), ("device", i32), ("values", vp), ("scales", vp), ("tensor_scale", vp)]
+
+
+class RmsNorm(C.Structure):
+    _fields_ = ([("rows", u64), ("cols", u64)] + [(n, i32) for n in ("x_dtype", "r_dtype", "w_dtype", "out_dtype", "group", "device")] +
+                [(n, vp) for n in ("x", "residual", "weight", "sum", "out", "scales")] + [(n, i64) for n in ("ldx", "ldr", "lds", "ldo")] + [("eps", C.c_float)])
 
 
 class KatMma(C.Structure):
@@ -127,6 +132,7 @@ SIGNATURES = {
     "b200spmm_fp4_dense_product": (C.c_int, [C.POINTER(Fp4), vp, i64, i64, C.c_int, C.c_int, vp, i64, C.c_int, C.c_int, vp, u64, vp]),
     "b200spmm_fp4_product_workspace": (C.c_int, [C.POINTER(Fp4), vp, i64, i64, C.c_int, C.POINTER(u64)]),
     "b200spmm_fp4_status": (C.c_int, [C.c_int, vp]),
+    "b200spmm_rms_norm": (C.c_int, [C.POINTER(RmsNorm), vp]),
     "b200spmm_kat_umma": (C.c_int, [vp, u32, C.POINTER(KatMma), C.c_int, C.c_int, vp, C.c_int]),
     "b200spmm_kat_umma_pair": (C.c_int, [vp, u32, C.POINTER(KatMma), C.c_int, C.c_int, vp, C.c_int]),
     "b200spmm_kat_wait_limit": (C.c_uint64, [C.c_uint64]),

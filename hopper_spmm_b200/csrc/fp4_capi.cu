@@ -4,8 +4,7 @@
 #include <utility>
 
 #include "../../include/b200_spmm_kat.h"
-#include "common.hpp"
-#include "fp4.hpp"
+#include "entry.hpp"
 
 namespace b200spmm {
 namespace fp4 {
@@ -37,12 +36,7 @@ void come(int device) {
 thread_local unsigned long long t_starve_ns = 0;
 thread_local int t_starve_operand = 0;
 
-// Calls that a capturing thread may not make otherwise (they touch no stream).
-struct RelaxedCapture {
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
-    ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
-};
+}  // namespace
 
 int check_device(int device) {
     if (device < 0 || device >= kMaxDevices) return B200SPMM_ERR_NO_DEVICE;
@@ -59,9 +53,8 @@ int check_device(int device) {
     return B200SPMM_OK;
 }
 
-bool aligned(const void *p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
-bool is_type(int t) { return t == B200SPMM_T_F32 || t == B200SPMM_T_F16 || t == B200SPMM_T_BF16; }
-uintptr_t size_of(int t) { return t == B200SPMM_T_F32 ? 4 : 2; }
+namespace {
+
 bool is_empty(const b200spmm_fp4_t *m) { return m->rows == 0 || m->cols == 0; }
 
 int check_matrix(const b200spmm_fp4_t *m) {
@@ -72,32 +65,6 @@ int check_matrix(const b200spmm_fp4_t *m) {
     if (!m->values || !m->scales) return B200SPMM_ERR_INVALID_ARG;
     if (!aligned(m->values, 16) || !aligned(m->scales, 16)) return B200SPMM_ERR_UNSUPPORTED;
     return B200SPMM_OK;
-}
-
-// A dense matrix of rows x cols, rows `ld` elements apart.
-int check_dense(const void *p, int type, uint64_t rows, uint64_t cols, int64_t ld) {
-    if (!is_type(type)) return B200SPMM_ERR_INVALID_ARG;
-    if (rows == 0 || cols == 0) return B200SPMM_OK;
-    if (!p || (rows > 1 && ld < (int64_t)cols) || !aligned(p, size_of(type))) return B200SPMM_ERR_INVALID_ARG;
-    return B200SPMM_OK;
-}
-
-int zero_output(void *c, int64_t ldc, int type, uint64_t rows, uint64_t cols, cudaStream_t stream) {
-    const size_t esz = size_of(type), width = cols * esz;
-    B200_CUDA_TRY(cudaMemset2DAsync(c, rows > 1 ? (size_t)ldc * esz : width, 0, width, rows, stream));
-    return B200SPMM_OK;
-}
-
-template <class Fn>
-int on_device(int device, Fn &&body) {
-    return guarded([&]() -> int {
-        const int st = check_device(device);
-        if (st != B200SPMM_OK) return st;
-        const DeviceGuard guard(device);
-        B200_CUDA_TRY(guard.status);
-        const RelaxedCapture relaxed;
-        return body();
-    });
 }
 
 // The word of the device, which is current.

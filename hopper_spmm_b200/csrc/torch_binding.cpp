@@ -12,6 +12,7 @@
 #include <ATen/record_function.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAStream.h>
+#include <ATen/core/grad_mode.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -366,6 +367,142 @@ PyObject *fp4_dense_product(PyObject *, PyObject *const *args, Py_ssize_t n_args
     END_HANDLE_TH_ERRORS
 }
 
+// ---- around weights in few bits
+
+// Whether a gradient would be lost: the tensor wants one and gradients are recorded.
+bool wants_gradient(const at::Tensor &t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+constexpr const char *kNoGradient = "there is no backward pass: call it under torch.no_grad(), or with tensors that require no gradient";
+
+// Rows of neighbours: the address and the distance of rows, in elements.
+struct Rows {
+    void *ptr;
+    int64_t ld;
+};
+bool rows_of(const at::Tensor &t, Rows *r) {
+    if (t.dim() != 2 || t.layout() != at::kStrided) return false;
+    const int64_t n = t.size(0), c = t.size(1);
+    if ((c > 1 && t.stride(1) != 1) || (n > 1 && t.stride(0) < c)) return false;
+    *r = {t.data_ptr(), n <= 1 ? c : t.stride(0)};
+    return true;
+}
+
+PyObject *three(PyObject *a, PyObject *b, PyObject *c) {
+    PyObject *out = a && b && c ? PyTuple_New(3) : nullptr;
+    if (!out) {
+        Py_XDECREF(a);
+        Py_XDECREF(b);
+        Py_XDECREF(c);
+        return nullptr;
+    }
+    PyTuple_SET_ITEM(out, 0, a);
+    PyTuple_SET_ITEM(out, 1, b);
+    PyTuple_SET_ITEM(out, 2, c);
+    return out;
+}
+PyObject *again(PyObject *o) {
+    Py_INCREF(o);
+    return o;
+}
+
+// rms_norm(X, weight or None, eps, residual or None, sum or None, out or None, scales or None, out's type, group) -> (out, scales or None, sum or
+// None), the first of them a status where it is a number
+PyObject *rms_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 9) {
+        PyErr_SetString(PyExc_TypeError, "rms_norm takes 9 arguments");
+        return nullptr;
+    }
+    b200spmm_rms_norm_t p{};
+    const at::Tensor *X = cuda_tensor(args[0]);
+    Rows x, r, o, h;
+    if (!X || type_code(X->scalar_type()) < 0 || !rows_of(*X, &x))
+        return refuse("X must be a two-dimensional CUDA tensor of float32, float16 or bfloat16 with unit stride along its rows");
+    p.eps = (float)PyFloat_AsDouble(args[2]);
+    const long type = PyLong_AsLong(args[7]), group = PyLong_AsLong(args[8]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!(p.eps >= 0.f)) return refuse("eps must not be negative");
+    const bool e4m3 = type == B200SPMM_T_E4M3;
+    const int64_t rows = X->size(0), cols = X->size(1);
+    bool lost = wants_gradient(*X);
+    auto beside = [&](const at::Tensor *t) { return t && t->get_device() == X->get_device(); };
+    if (args[1] != Py_None) {
+        const at::Tensor *w = cuda_tensor(args[1]);
+        if (!beside(w) || type_code(w->scalar_type()) < 0 || w->layout() != at::kStrided || w->dim() != 1 || w->size(0) != cols || (cols > 1 && w->stride(0) != 1))
+            return refuse("weight must be a contiguous tensor of X's number of columns, float32, float16 or bfloat16, on X's device");
+        lost = lost || wants_gradient(*w);
+        p.weight = w->data_ptr();
+        p.w_dtype = type_code(w->scalar_type());
+    }
+    auto like_x = [&](const at::Tensor *t, at::ScalarType kind, Rows *at) {
+        return beside(t) && t->scalar_type() == kind && t->dim() == 2 && t->size(0) == rows && t->size(1) == cols && rows_of(*t, at);
+    };
+    at::Tensor sum, out, scales;
+    if (args[3] != Py_None) {
+        const at::Tensor *t = cuda_tensor(args[3]);
+        if (!t || (t->scalar_type() != X->scalar_type() && t->scalar_type() != at::kFloat) || !like_x(t, t->scalar_type(), &r))
+            return refuse("residual must be a tensor of X's shape, on X's device, of X's type or float32, with unit stride along its rows");
+        lost = lost || wants_gradient(*t);
+        p.residual = r.ptr;
+        p.ldr = r.ld;
+        p.r_dtype = type_code(t->scalar_type());
+        if (args[4] != Py_None) {
+            const at::Tensor *s = cuda_tensor(args[4]);
+            if (!like_x(s, t->scalar_type(), &h)) return refuse("sum_out must be a tensor like residual with unit stride along its rows");
+            lost = lost || wants_gradient(*s);
+        }
+    } else if (args[4] != Py_None) {
+        return refuse("sum_out is for a call with a residual");
+    }
+    const at::ScalarType out_type = e4m3 ? at::kFloat8_e4m3fn : type_of(type);
+    const int64_t groups = group ? (cols + group - 1) / group : 1;
+    if (args[5] != Py_None) {
+        const at::Tensor *t = cuda_tensor(args[5]), *s = args[6] == Py_None ? nullptr : cuda_tensor(args[6]);
+        if (!like_x(t, out_type, &o) || (e4m3 && (!beside(s) || s->scalar_type() != at::kFloat || s->dim() != 2 || s->size(0) != rows || s->size(1) != groups || !s->is_contiguous())))
+            return refuse("out has the wrong shape, type, device or layout");
+        lost = lost || wants_gradient(*t);
+        if (e4m3) p.scales = static_cast<float *>(s->data_ptr());
+    }
+    if (lost) return refuse(kNoGradient);
+    if (args[5] == Py_None) {
+        out = new_cuda({rows, cols}, out_type, *X);
+        o = {out.data_ptr(), cols};
+        if (e4m3) {
+            scales = new_cuda({rows, groups}, at::kFloat, *X);
+            p.scales = static_cast<float *>(scales.data_ptr());
+        }
+    }
+    if (args[3] != Py_None && args[4] == Py_None) {  // (an empty tensor has no address)
+        sum = new_cuda({rows, cols}, p.r_dtype == B200SPMM_T_F32 ? at::kFloat : X->scalar_type(), *X);
+        h = {sum.data_ptr(), cols};
+    }
+    p.rows = (uint64_t)rows;
+    p.cols = (uint64_t)cols;
+    p.x_dtype = type_code(X->scalar_type());
+    p.out_dtype = (int32_t)type;
+    p.group = (int32_t)group;
+    p.device = (int32_t)X->get_device();
+    p.x = x.ptr;
+    p.ldx = x.ld;
+    p.out = o.ptr;
+    p.ldo = o.ld;
+    if (args[3] != Py_None) {
+        p.sum = h.ptr;
+        p.lds = h.ld;
+    }
+    void *stream = c10::cuda::getCurrentCUDAStream(X->get_device()).stream();
+    int st;
+    {
+        const ThreadsAllowed threads;
+        st = b200spmm_rms_norm(&p, stream);
+    }
+    if (st != B200SPMM_OK) return three(PyLong_FromLong(st), again(Py_None), again(Py_None));
+    PyObject *a = out.defined() ? THPVariable_Wrap(std::move(out)) : again(args[5]);
+    PyObject *b = scales.defined() ? THPVariable_Wrap(std::move(scales)) : again(Py_None);
+    PyObject *c = sum.defined() ? THPVariable_Wrap(std::move(sum)) : again(args[4]);
+    return three(a, b, c);
+    END_HANDLE_TH_ERRORS
+}
+
 template <PyObject *(*kFn)(PyObject *, PyObject *const *, Py_ssize_t)>
 PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kFn)); }
 
@@ -375,6 +512,7 @@ PyMethodDef methods[] = {{"spmm", reinterpret_cast<PyCFunction>(reinterpret_cast
                          {"fp4_dequantize", fast<fp4_dequantize>(), METH_FASTCALL, nullptr},
                          {"fp4_product", fast<fp4_product>(), METH_FASTCALL, nullptr},
                          {"fp4_dense_product", fast<fp4_dense_product>(), METH_FASTCALL, nullptr},
+                         {"rms_norm", fast<rms_norm>(), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -506,8 +506,8 @@ int b200spmm_plan_launch_info(const b200spmm_plan_t *p, b200spmm_launch_info_t *
  *   tensor_scale  one fp32 number
  */
 enum { B200SPMM_NVFP4 = 0, B200SPMM_MXFP4 = 1 };
-/* Element types of the dense matrices; the first two are B200SPMM_C_F32 and B200SPMM_C_F16. */
-enum { B200SPMM_T_F32 = 0, B200SPMM_T_F16 = 1, B200SPMM_T_BF16 = 2 };
+/* Element types of the dense matrices; the first two are B200SPMM_C_F32 and B200SPMM_C_F16.  E4M3, with scales beside it, is for calls that name it. */
+enum { B200SPMM_T_F32 = 0, B200SPMM_T_F16 = 1, B200SPMM_T_BF16 = 2, B200SPMM_T_E4M3 = 3 };
 typedef struct {
     uint64_t rows, cols;
     int32_t format, device;
@@ -573,6 +573,32 @@ int b200spmm_fp4_product_workspace(const b200spmm_fp4_t *a, const void *d_B, int
  * capture goes on.
  */
 int b200spmm_fp4_status(int device, void *stream);
+
+/* ------------------------------------------------------------------ around weights in few bits: what a decoding step does */
+
+/*
+ * The residual's addition and the RMS norm, row by row (no counterpart in the reference, as for all below):
+ *     h = x + r        sum = h rounded to r_dtype        y = h / sqrt(mean(h^2) + eps) * w
+ * with h in fp32 and y rounded once, to out_dtype: fp32, fp16, bf16, or e4m3.  e4m3 has a scale max |y| / 448 for each row (group 0) or for every
+ * `group` (32, 64, 128) neighbours of a row begun, in scales [rows, groups of a row], contiguous: y is value x scale, values are rounded to the
+ * nearest, at most 448; a group of zeros has the scale 0, one with an infinity or NaN the scale NaN and zeros as values.
+ * Squares that leave fp32's range are summed up again from scaled values.
+ * residual, sum and weight may be null (0, nothing kept, 1); x_dtype any of the three, r_dtype that or fp32, w_dtype any of the three.  Rows lie ld*
+ * elements apart, each starting on any element; rows that start on 16 bytes are faster.  out may be x, and sum may be x or residual (at the same place, rows as far
+ * apart, the same type); else nothing overlaps.
+ */
+typedef struct {
+    uint64_t rows, cols;
+    int32_t x_dtype, r_dtype, w_dtype, out_dtype, group, device;
+    const void *x, *residual, *weight;
+    void *sum, *out;
+    float *scales;
+    int64_t ldx, ldr, lds, ldo;
+    float eps;
+} b200spmm_rms_norm_t;
+int b200spmm_rms_norm(const b200spmm_rms_norm_t *p, void *stream);
+
+/* Asynchronous on `stream`, on the device that the structure names; allocates nothing and may be captured. */
 
 #ifdef __cplusplus
 }
