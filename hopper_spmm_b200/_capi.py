@@ -38,6 +38,10 @@ class RmsNorm(C.Structure):
                 [(n, vp) for n in ("x", "residual", "weight", "sum", "out", "scales")] + [(n, i64) for n in ("ldx", "ldr", "lds", "ldo")] + [("eps", C.c_float)])
 
 
+class Int4(C.Structure):
+    _fields_ = [("rows", u64), ("cols", u64), ("group", i32), ("scale_dtype", i32), ("device", i32), ("values", vp), ("scales", vp), ("zeros", vp)]
+
+
 class KatMma(C.Structure):
     _fields_ = [(n, u32) for n in ("a_off", "a_lbo", "a_sbo", "a_swizzle", "b_off", "b_lbo", "b_sbo", "b_swizzle",
                                    "idesc", "d_col", "accumulate", "kind")]
@@ -133,6 +137,7 @@ SIGNATURES = {
     "b200spmm_fp4_product_workspace": (C.c_int, [C.POINTER(Fp4), vp, i64, i64, C.c_int, C.POINTER(u64)]),
     "b200spmm_fp4_status": (C.c_int, [C.c_int, vp]),
     "b200spmm_rms_norm": (C.c_int, [C.POINTER(RmsNorm), vp]),
+    "b200spmm_int4_product": (C.c_int, [C.POINTER(Int4), vp, i64, i64, C.c_int, C.c_int, vp, C.c_int, vp, i64, C.c_int, C.c_int, vp]),
     "b200spmm_kat_umma": (C.c_int, [vp, u32, C.POINTER(KatMma), C.c_int, C.c_int, vp, C.c_int]),
     "b200spmm_kat_umma_pair": (C.c_int, [vp, u32, C.POINTER(KatMma), C.c_int, C.c_int, vp, C.c_int]),
     "b200spmm_kat_wait_limit": (C.c_uint64, [C.c_uint64]),

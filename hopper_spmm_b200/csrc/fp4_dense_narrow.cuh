@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "fp4_widen.cuh"
+#include "mma_16x8x16.cuh"
 
 namespace b200spmm {
 namespace fp4 {
@@ -70,16 +71,6 @@ struct NarrowStage {
 };
 __host__ __device__ inline NarrowStage narrow_stage(bool mx, uint32_t at_once, uint32_t row_blocks, uint32_t nb) {
     return {at_once * 16u * (kNarrowStage / 2), row_blocks * (mx ? 2u : 4u) * 512u, nb * kNarrowStage * 16u};
-}
-
-template <typename T>
-B200_DEVICE void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 B200_DEVICE void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {

@@ -1,0 +1,176 @@
+// Product of a matrix of 4-bit integers with a few columns.
+//
+//     C[m, j] = sum over groups g of k  scale[g, m] (sum over k in g  (code[m, k] - zero[g, m]) B[k, j])
+//
+// The inner sums are of exact products (a code less its zero is a small whole number, columns have 16 bits, or 8 with scales of their own), 128 values of k at most, the
+// outer one is rounded in fp32 for each: what the MMA cuts off never grows with k.  How it is done: narrow.cuh.
+#include "entry.hpp"
+#include "fp4_store.cuh"
+#include "launch.hpp"
+#include "int4.hpp"
+
+namespace b200spmm {
+namespace narrow {
+namespace {
+
+using fp4::Target;
+
+struct Int4Params {
+    Matrix m;
+    uint32_t rows, k, n;
+    const void *x;
+    int64_t along, across;
+    bool wide;
+    const float *x_scales;
+    uint32_t x_groups, x_shift;
+    Target c;
+    uint32_t tiles, warps, steps, chunk, cols;  // of all blocks together; of a block; of a row; that the columns have room for; of a pass, at most
+};
+
+constexpr int kRing = 3;  // stages of a warp
+template <int kNB>
+constexpr uint32_t kMaxWarps = kNB <= 1 ? 28 : kNB <= 2 ? 24 : 16;
+
+template <typename T, int kSpan, int kNB, bool kScaled>
+__global__ void __launch_bounds__(32 * kMaxWarps<kNB>, 1) int4_kernel(const Int4Params p) {
+    using W = Weights<T, kSpan>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const uint32_t base = ptx::smem_u32(smem), warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u, g = lane >> 2;
+    constexpr uint32_t ring_bytes = kRing * kStageBytes, ring_floats = ring_bytes / 4u;
+    const uint32_t j0 = blockIdx.y * (8u * kNB), n = min(8u * kNB, p.n - j0);
+    Columns c;
+    c.base = base + p.warps * ring_bytes;
+    c.pitch = column_pitch<W>(p.chunk);
+    c.plane = 0;
+    c.scales = c.base + p.cols * c.pitch;
+    c.groups = p.x_groups;
+    c.shift = p.x_shift;
+    c.steps = p.chunk;
+    const uint32_t tile_begin = (uint32_t)((uint64_t)p.tiles * blockIdx.x / gridDim.x), tile_end = (uint32_t)((uint64_t)p.tiles * (blockIdx.x + 1u) / gridDim.x);
+    const Split split(tile_end - tile_begin, p.steps, p.warps);
+    ptx::wait_for_grids_before();
+    if constexpr (kScaled) {
+        float *to = reinterpret_cast<float *>(smem + (c.scales - base));
+        for (uint32_t i = threadIdx.x; i < n * p.x_groups; i += blockDim.x) to[i] = p.x_scales[(uint64_t)j0 * p.x_groups + i];
+    }
+    auto stage = [&](uint32_t first, uint32_t count) {
+        if constexpr (kScaled)
+            stage_columns<W>(Eights{static_cast<const uint8_t *>(p.x) + (int64_t)j0 * p.across, p.across, p.wide, p.k}, c, first, count, n, false);
+        else
+            stage_columns<W>(Plain<T>{static_cast<const T *>(p.x) + (int64_t)j0 * p.across, p.along, p.across, p.wide, p.k}, c, first, count, n, p.along != 1);
+    };
+    bool staged = false;
+    for (uint32_t tile0 = tile_begin; tile0 < tile_end; tile0 += split.at_once) {
+        const uint32_t mine = warp / split.slices, tile = tile0 + mine;
+        Share s;
+        s.slice = warp % split.slices;
+        s.slices = split.slices;
+        s.steps = p.steps;
+        s.ring = base + warp * ring_bytes;
+        s.busy = mine < split.at_once && tile < tile_end;
+        s.row_lo = min(tile * kTileRows + g, p.rows - 1u);
+        s.row_hi = min(tile * kTileRows + g + 8u, p.rows - 1u);
+        float sums[kNB][4] = {};
+        accumulate<W, kNB, 1, kScaled, kRing>(p.m, s, c, n, staged, stage, sums);
+        staged = p.chunk >= p.steps;
+        __syncwarp();
+        if (s.busy) leave_sums<kNB>(reinterpret_cast<float *>(smem + warp * ring_bytes), sums);
+        __syncthreads();
+        const uint32_t here = min(split.at_once, tile_end - tile0);
+        for (uint32_t i = threadIdx.x; i < here * kTileRows * n; i += blockDim.x) {
+            const uint32_t r = i % kTileRows, j = i / kTileRows % n, of = i / (kTileRows * n), row = (tile0 + of) * kTileRows + r;
+            const float v[1] = {joined(reinterpret_cast<const float *>(smem), ring_floats, of * split.slices, split.slices, j, r)};
+            if (row < p.rows) fp4::store_row(p.c, row, j0 + j, p.n, v);
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int kSpan, int kNB, bool kScaled>
+int launch(Int4Params p, cudaStream_t stream) {
+    using W = Weights<T, kSpan>;
+    auto kernel = int4_kernel<T, kSpan, kNB, kScaled>;
+    const uint32_t blocks = std::min<uint32_t>(p.tiles, fp4::sm_count()), passes = (p.n + 8 * kNB - 1) / (8 * kNB);
+    p.steps = (p.k + W::kStep - 1) / W::kStep;
+    p.cols = std::min<uint32_t>(8 * kNB, p.n);
+    const uint32_t scales = kScaled ? p.cols * p.x_groups * 4u : 0u;
+    const Split split((p.tiles + blocks - 1) / blocks, p.steps, kMaxWarps<kNB>);
+    p.warps = split.at_once * split.slices;
+    // the columns as a whole, or as much of them as there is room for
+    const uint64_t ring = (uint64_t)p.warps * kRing * kStageBytes;
+    p.chunk = steps_that_fit<W>(p.cols, p.steps, ring + scales);
+    if (p.chunk == 0) return B200SPMM_ERR_UNSUPPORTED;
+    const uint32_t bytes = (uint32_t)ring + scales + p.cols * column_pitch<W>(p.chunk);
+    static std::atomic<uint64_t> allowed{0};
+    B200_CUDA_TRY(allow_smem(kernel, allowed));
+    B200_CUDA_TRY(launch_after(kernel, dim3(blocks, passes), 32u * p.warps, bytes, 1, stream, p));
+    return B200SPMM_OK;
+}
+
+template <typename T, int kSpan, bool kScaled>
+int launch_width(const Int4Params &p, cudaStream_t stream) {
+    if (p.n <= 8) return launch<T, kSpan, 1, kScaled>(p, stream);
+    if (p.n <= 16) return launch<T, kSpan, 2, kScaled>(p, stream);
+    return launch<T, kSpan, 4, kScaled>(p, stream);
+}
+template <typename T, bool kScaled>
+int launch_span(const Int4Params &p, uint32_t span, cudaStream_t stream) {
+    if (span == 32) return launch_width<T, 32, kScaled>(p, stream);
+    if (span == 64) return launch_width<T, 64, kScaled>(p, stream);
+    return launch_width<T, 128, kScaled>(p, stream);
+}
+
+}  // namespace
+}  // namespace narrow
+}  // namespace b200spmm
+
+using namespace b200spmm;
+using namespace b200spmm::fp4;
+
+extern "C" int b200spmm_int4_product(const b200spmm_int4_t *a, const void *d_B, int64_t ldb, int64_t n, int b_dtype, int b_transposed, const float *d_b_scales, int b_group,
+                                     void *d_C, int64_t ldc, int c_dtype, int c_transposed, void *stream) {
+    int st = narrow::check_int4(a);
+    if (st != B200SPMM_OK) return st;
+    if (n < 0) return B200SPMM_ERR_INVALID_ARG;
+    if (n > 65535) return B200SPMM_ERR_UNSUPPORTED;
+    const bool eights = b_dtype == B200SPMM_T_E4M3;
+    if (eights) {
+        if (!b_transposed || (b_group != 0 && b_group != 32 && b_group != 64 && b_group != 128)) return B200SPMM_ERR_INVALID_ARG;
+        if (n > 0 && a->cols > 0 && (!d_B || (n > 1 && ldb < (int64_t)a->cols) || !d_b_scales || !aligned(d_b_scales, 4))) return B200SPMM_ERR_INVALID_ARG;
+    } else {
+        st = check_dense(d_B, b_dtype, b_transposed ? (uint64_t)n : a->cols, b_transposed ? a->cols : (uint64_t)n, ldb);
+        if (st != B200SPMM_OK) return st;
+        if (d_b_scales || b_group) return B200SPMM_ERR_INVALID_ARG;
+        if (b_dtype == B200SPMM_T_F32) return B200SPMM_ERR_UNSUPPORTED;
+    }
+    const uint64_t rows = c_transposed ? (uint64_t)n : a->rows, cols = c_transposed ? a->rows : (uint64_t)n;
+    st = check_dense(d_C, c_dtype, rows, cols, ldc);
+    if (st != B200SPMM_OK) return st;
+    return on_device(a->device, [&]() -> int {
+        const cudaStream_t s = static_cast<cudaStream_t>(stream);
+        if (rows == 0 || cols == 0) return B200SPMM_OK;
+        if (a->cols == 0) return zero_output(d_C, ldc, c_dtype, rows, cols, s);
+        narrow::Int4Params p{};
+        p.m = narrow::matrix_of(a);
+        p.rows = (uint32_t)a->rows;
+        p.k = (uint32_t)a->cols;
+        p.n = (uint32_t)n;
+        p.x = d_B;
+        p.along = b_transposed ? 1 : ldb;
+        p.across = b_transposed ? ldb : 1;
+        const uint32_t unit = eights ? 8 : 16;
+        p.wide = p.along == 1 && aligned(d_B, unit) && (n == 1 || p.across * (eights ? 1 : 2) % unit == 0);
+        p.x_scales = d_b_scales;
+        p.x_groups = b_group ? (p.k + b_group - 1) / b_group : 1;
+        p.x_shift = narrow::shift_of(b_group);
+        p.c = target_of(d_C, ldc, c_dtype, c_transposed != 0);
+        p.tiles = (p.rows + narrow::kTileRows - 1) / narrow::kTileRows;
+        uint32_t span = narrow::span_of(a);
+        if (eights) {
+            if (b_group) span = std::min<uint32_t>(span, b_group);
+            return narrow::launch_span<__half, true>(p, span, s);
+        }
+        if (b_dtype == B200SPMM_T_F16) return narrow::launch_span<__half, false>(p, span, s);
+        return narrow::launch_span<__nv_bfloat16, false>(p, span, s);
+    });
+}

@@ -503,6 +503,88 @@ PyObject *rms_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// A matrix of 4-bit integers: what the C ABI gets of it, behind a capsule.  The tensors stay alive beside it.
+constexpr const char *kInt4 = "b200spmm_int4_t";
+void free_int4(PyObject *capsule) { delete static_cast<b200spmm_int4_t *>(PyCapsule_GetPointer(capsule, kInt4)); }
+
+// int4_matrix(values, scales, zeros or None, rows, cols, group) -> capsule
+PyObject *int4_matrix(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 6) {
+        PyErr_SetString(PyExc_TypeError, "int4_matrix takes 6 arguments");
+        return nullptr;
+    }
+    const int64_t rows = PyLong_AsLongLong(args[3]), cols = PyLong_AsLongLong(args[4]), group = PyLong_AsLongLong(args[5]);
+    if (PyErr_Occurred()) return nullptr;
+    if (rows < 0 || cols < 0 || rows > 0x7FFFFFFF - 256 || cols > 0x7FFFFFFF - 512) return refuse("rows and cols must lie between 0 and 2^31");
+    if (group != 0 && (group < 32 || group > (1 << 30) || (group & (group - 1)) != 0)) return refuse("group must be None (a whole row) or a power of two from 32 on");
+    auto tensor = [&](PyObject *o, int64_t a, int64_t b) -> const at::Tensor * {
+        if (!THPVariable_Check(o)) return nullptr;
+        const at::Tensor &t = THPVariable_Unpack(o);
+        return t.layout() == at::kStrided && t.dim() == 2 && t.size(0) == a && t.size(1) == b && t.is_contiguous() && !t.is_neg() ? &t : nullptr;
+    };
+    const int64_t groups = group ? (cols + group - 1) / group : 1;
+    const at::Tensor *v = tensor(args[0], rows, (cols + 31) / 32 * 16), *s = tensor(args[1], groups, rows), *z = args[2] == Py_None ? nullptr : tensor(args[2], groups, rows);
+    if (!v || v->scalar_type() != at::kByte) return refuse("values must be a contiguous uint8 tensor [rows, 16 for every 32 columns begun]");
+    if (!s || (s->scalar_type() != at::kHalf && s->scalar_type() != at::kBFloat16)) return refuse("scales must be a contiguous float16 or bfloat16 tensor [groups of a row, rows]");
+    if (args[2] != Py_None && (!z || z->scalar_type() != at::kByte)) return refuse("zeros must be a contiguous uint8 tensor [groups of a row, rows]");
+    if (wants_gradient(*s)) return refuse(kNoGradient);
+    if (s->device() != v->device() || (z && z->device() != v->device())) return refuse("values, scales and zeros must be on one device");
+    if (!v->is_cuda()) return refuse("values, scales and zeros must be on a CUDA device");
+    auto *m = new b200spmm_int4_t{};
+    m->rows = (uint64_t)rows;
+    m->cols = (uint64_t)cols;
+    m->group = (int32_t)group;
+    m->scale_dtype = type_code(s->scalar_type());
+    m->device = (int32_t)v->get_device();
+    m->values = v->data_ptr();
+    m->scales = s->data_ptr();
+    m->zeros = z ? static_cast<const uint8_t *>(z->data_ptr()) : nullptr;
+    PyObject *out = PyCapsule_New(m, kInt4, free_int4);
+    if (!out) delete m;
+    return out;
+    END_HANDLE_TH_ERRORS
+}
+
+// int4_product(capsule, B or values, their scales or None, group, C or None, type, tokens first) -> C or a status.  Tokens first: B is [n, cols] and C
+// [n, rows], else [cols, n] and [rows, n]; 8-bit B always [n, cols].
+PyObject *int4_product(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 7) {
+        PyErr_SetString(PyExc_TypeError, "int4_product takes 7 arguments");
+        return nullptr;
+    }
+    const auto *a = static_cast<const b200spmm_int4_t *>(PyCapsule_GetPointer(args[0], kInt4));
+    const long group = PyLong_AsLong(args[3]), type = PyLong_AsLong(args[5]);
+    if (PyErr_Occurred()) return nullptr;
+    const bool first = args[6] == Py_True, eights = args[2] != Py_None;
+    const at::Tensor *B = cuda_tensor(args[1]), *s = eights ? cuda_tensor(args[2]) : nullptr;
+    Dense b;
+    const bool lies_first = first || eights;
+    if (!B || B->scalar_type() != (eights ? at::kFloat8_e4m3fn : B->scalar_type() == at::kHalf ? at::kHalf : at::kBFloat16) || !dense_of(*B, &b) || (eights && b.transposed && B->size(0) > 1) ||
+        B->size(lies_first ? 1 : 0) != (int64_t)a->cols || B->get_device() != a->device)
+        return refuse(eights ? "the 8-bit matrix must have the matrix's columns, on its device, with unit stride along its rows"
+                             : first ? "X must be a CUDA float16 or bfloat16 tensor of shape [n, cols] on the matrix's device with unit stride along rows or columns"
+                                     : "B must be a CUDA float16 or bfloat16 tensor of shape [cols, n] on the matrix's device with unit stride along rows or columns");
+    if (eights && (!s || s->get_device() != a->device)) return refuse("the 8-bit matrix's scales must be on the matrix's device");
+    if (wants_gradient(*B)) return refuse(kNoGradient);
+    const int64_t n = B->size(lies_first ? 0 : 1);
+    if (eights && b.transposed) b = {b.ptr, (int64_t)a->cols, false};  // (one row)
+    at::Tensor C;
+    Dense c;
+    if (!output_of(args[4], first ? n : (int64_t)a->rows, first ? (int64_t)a->rows : n, type, *B, &C, &c)) return nullptr;
+    if (wants_gradient(C)) return refuse(kNoGradient);
+    void *stream = c10::cuda::getCurrentCUDAStream(B->get_device()).stream();
+    int st;
+    {
+        const ThreadsAllowed threads;
+        st = b200spmm_int4_product(a, b.ptr, b.ld, n, eights ? B200SPMM_T_E4M3 : type_code(B->scalar_type()), lies_first != b.transposed,
+                                   eights ? static_cast<const float *>(s->data_ptr()) : nullptr, (int)group, c.ptr, c.ld, (int)type, first != c.transposed, stream);
+    }
+    return result_of(st, args[4], std::move(C));
+    END_HANDLE_TH_ERRORS
+}
+
 template <PyObject *(*kFn)(PyObject *, PyObject *const *, Py_ssize_t)>
 PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kFn)); }
 
@@ -513,6 +595,8 @@ PyMethodDef methods[] = {{"spmm", reinterpret_cast<PyCFunction>(reinterpret_cast
                          {"fp4_product", fast<fp4_product>(), METH_FASTCALL, nullptr},
                          {"fp4_dense_product", fast<fp4_dense_product>(), METH_FASTCALL, nullptr},
                          {"rms_norm", fast<rms_norm>(), METH_FASTCALL, nullptr},
+                         {"int4_matrix", fast<int4_matrix>(), METH_FASTCALL, nullptr},
+                         {"int4_product", fast<int4_product>(), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -598,7 +598,31 @@ typedef struct {
 } b200spmm_rms_norm_t;
 int b200spmm_rms_norm(const b200spmm_rms_norm_t *p, void *stream);
 
-/* Asynchronous on `stream`, on the device that the structure names; allocates nothing and may be captured. */
+/*
+ * A matrix in 4-bit integers: (code - zero) x scale, one scale and one zero for every `group` neighbours of a row begun (a power of two from 32
+ * on; 0: for the whole row).
+ *   values  as those of the 4-bit matrices above: rows of `pitch` bytes, 16 for every 32 columns begun, two codes (0 to 15) to a byte, the lower half
+ *           first, anything behind the last column; 16-byte aligned
+ *   scales  [groups of a row, rows], fp16 or bf16 (scale_dtype)
+ *   zeros   [groups of a row, rows], one byte each, 0 to 15 (of larger ones the low four bits count); null: 8 everywhere
+ */
+typedef struct {
+    uint64_t rows, cols;
+    int32_t group, scale_dtype, device;
+    const void *values, *scales;
+    const uint8_t *zeros;
+} b200spmm_int4_t;
+
+/*
+ * C[a.rows, n] = A B with few columns: A is read once for every 32.  B [a.cols, n] in fp16 or bf16, ldb elements between rows, or between columns where transposed; or in
+ * e4m3 (transposed only), column j being value x b_scales[j, k / b_group], b_scales [n, groups of a column] contiguous and b_group 0 (one scale for a column) or 32, 64
+ * or 128: what b200spmm_rms_norm writes.  b_scales and b_group are for e4m3 alone.  Sums in fp32, a
+ * scale multiplying the sum over its group (an infinite one gives infinities or NaN); C as that of b200spmm_fp4_dense_product.
+ */
+int b200spmm_int4_product(const b200spmm_int4_t *a, const void *d_B, int64_t ldb, int64_t n, int b_dtype, int b_transposed, const float *d_b_scales, int b_group,
+                          void *d_C, int64_t ldc, int c_dtype, int c_transposed, void *stream);
+
+/* Both are asynchronous on `stream`, run on the device that the structure names, allocate nothing and may be captured; no wait in them can run out. */
 
 #ifdef __cplusplus
 }
