@@ -27,7 +27,7 @@ struct Int4Params {
     uint32_t tiles, warps, steps, chunk, cols;  // of all blocks together; of a block; of a row; that the columns have room for; of a pass, at most
 };
 
-constexpr int kRing = 3;  // stages of a warp
+constexpr int kRing = 2;  // stages of a warp
 template <int kNB>
 constexpr uint32_t kMaxWarps = kNB <= 1 ? 28 : kNB <= 2 ? 24 : 16;
 
@@ -61,23 +61,21 @@ __global__ void __launch_bounds__(32 * kMaxWarps<kNB>, 1) int4_kernel(const Int4
     };
     bool staged = false;
     for (uint32_t tile0 = tile_begin; tile0 < tile_end; tile0 += split.at_once) {
-        const uint32_t mine = warp / split.slices, tile = tile0 + mine;
+        const uint32_t tiles = min(split.at_once, tile_end - tile0), mine = warp / split.slices;
         Share s;
         s.slice = warp % split.slices;
         s.slices = split.slices;
         s.steps = p.steps;
         s.ring = base + warp * ring_bytes;
-        s.busy = mine < split.at_once && tile < tile_end;
-        s.row_lo = min(tile * kTileRows + g, p.rows - 1u);
-        s.row_hi = min(tile * kTileRows + g + 8u, p.rows - 1u);
+        s.busy = mine < tiles;
+        s.row_lo = min((tile0 + mine) * kTileRows + g, p.rows - 1u);
+        s.row_hi = min((tile0 + mine) * kTileRows + g + 8u, p.rows - 1u);
         float sums[kNB][4] = {};
         accumulate<W, kNB, 1, kScaled, kRing>(p.m, s, c, n, staged, stage, sums);
         staged = p.chunk >= p.steps;
-        __syncwarp();
         if (s.busy) leave_sums<kNB>(reinterpret_cast<float *>(smem + warp * ring_bytes), sums);
         __syncthreads();
-        const uint32_t here = min(split.at_once, tile_end - tile0);
-        for (uint32_t i = threadIdx.x; i < here * kTileRows * n; i += blockDim.x) {
+        for (uint32_t i = threadIdx.x; i < tiles * kTileRows * n; i += blockDim.x) {
             const uint32_t r = i % kTileRows, j = i / kTileRows % n, of = i / (kTileRows * n), row = (tile0 + of) * kTileRows + r;
             const float v[1] = {joined(reinterpret_cast<const float *>(smem), ring_floats, of * split.slices, split.slices, j, r)};
             if (row < p.rows) fp4::store_row(p.c, row, j0 + j, p.n, v);
@@ -93,14 +91,13 @@ int launch(Int4Params p, cudaStream_t stream) {
     const uint32_t blocks = std::min<uint32_t>(p.tiles, fp4::sm_count()), passes = (p.n + 8 * kNB - 1) / (8 * kNB);
     p.steps = (p.k + W::kStep - 1) / W::kStep;
     p.cols = std::min<uint32_t>(8 * kNB, p.n);
-    const uint32_t scales = kScaled ? p.cols * p.x_groups * 4u : 0u;
     const Split split((p.tiles + blocks - 1) / blocks, p.steps, kMaxWarps<kNB>);
     p.warps = split.at_once * split.slices;
     // the columns as a whole, or as much of them as there is room for
-    const uint64_t ring = (uint64_t)p.warps * kRing * kStageBytes;
-    p.chunk = steps_that_fit<W>(p.cols, p.steps, ring + scales);
+    const uint64_t taken = (uint64_t)p.warps * kRing * kStageBytes + (kScaled ? (uint64_t)p.cols * p.x_groups * 4u : 0u);
+    p.chunk = steps_that_fit<W>(p.steps, p.cols, 1, taken);
     if (p.chunk == 0) return B200SPMM_ERR_UNSUPPORTED;
-    const uint32_t bytes = (uint32_t)ring + scales + p.cols * column_pitch<W>(p.chunk);
+    const uint32_t bytes = (uint32_t)taken + p.cols * column_pitch<W>(p.chunk);
     static std::atomic<uint64_t> allowed{0};
     B200_CUDA_TRY(allow_smem(kernel, allowed));
     B200_CUDA_TRY(launch_after(kernel, dim3(blocks, passes), 32u * p.warps, bytes, 1, stream, p));

@@ -13,6 +13,7 @@ inline int check_int4(const b200spmm_int4_t *m) {
     if (!m || (m->scale_dtype != B200SPMM_T_F16 && m->scale_dtype != B200SPMM_T_BF16)) return B200SPMM_ERR_INVALID_ARG;
     if (m->group != 0 && (m->group < 32 || (m->group & (m->group - 1)) != 0)) return B200SPMM_ERR_INVALID_ARG;
     if (m->rows > 0x7FFFFFFFull - 256 || m->cols > 0x7FFFFFFFull - 512) return B200SPMM_ERR_UNSUPPORTED;
+    if (m->group && m->rows * ((m->cols + m->group - 1) / m->group) > 0xFFFFFFFFull) return B200SPMM_ERR_UNSUPPORTED;  // (kernels count scales in 32 bits)
     if (m->rows == 0 || m->cols == 0) return B200SPMM_OK;
     if (!m->values || !m->scales || !fp4::aligned(m->scales, 2)) return B200SPMM_ERR_INVALID_ARG;
     if (!fp4::aligned(m->values, 16)) return B200SPMM_ERR_UNSUPPORTED;
@@ -35,21 +36,22 @@ inline Matrix matrix_of(const b200spmm_int4_t *m) {
     out.row_bytes = (uint32_t)out.pitch;
     out.shift = shift_of(m->group);
     out.groups = m->group ? (uint32_t)((m->cols + m->group - 1) / m->group) : 1;
-    out.rows = m->rows;
+    out.rows = (uint32_t)m->rows;
     out.scales = static_cast<const uint16_t *>(m->scales);
-    out.zeros = m->zeros;
+    out.zeros = m->zeros ? m->zeros : static_cast<const uint8_t *>(m->scales);
+    out.zero_mask = m->zeros ? 15u : 0u;
+    out.zero_else = m->zeros ? 0u : 8u;
     out.bf16_scales = m->scale_dtype == B200SPMM_T_BF16;
     return out;
 }
 
-// How many of `steps` of `cols` columns there is room for beside `taken` bytes of a block's shared memory.
+// How many of `steps` of `cols` columns, in `planes` parts, there is room for beside `taken` bytes of a block's shared memory.
 template <class W>
-uint32_t steps_that_fit(uint32_t cols, uint32_t steps, uint64_t taken) {
+uint32_t steps_that_fit(uint32_t steps, uint32_t cols, uint32_t planes, uint64_t taken) {
     if (taken >= kMaxSmem) return 0;
-    const uint64_t pitch = (kMaxSmem - taken) / std::max(cols, 1u);  // bytes that a column may take
+    const uint64_t pitch = (kMaxSmem - taken) / (cols * planes);  // bytes that a column may take
     if (pitch < column_pitch<W>(1)) return 0;
-    uint64_t fit = (pitch - 64) / 128 * 128 / (W::kUnits * 16u);
-    return (uint32_t)std::min<uint64_t>(fit, steps);
+    return (uint32_t)std::min<uint64_t>((pitch - 64) / 128 * 128 / (W::kUnits * 16u), steps);
 }
 
 // Lets a kernel have all the shared memory of a block, once for each device; `allowed` keeps which.

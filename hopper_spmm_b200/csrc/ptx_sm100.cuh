@@ -216,6 +216,9 @@ B200_DEVICE void st_shared_u16(uint32_t addr, uint16_t v) {
 B200_DEVICE void cp_async_16(uint32_t dst, const void *src, uint32_t src_bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
 }
+B200_DEVICE void cp_async_16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 // Copies 4 bytes global -> shared (cached in L1: neighbouring words are fetched next).
 B200_DEVICE void cp_async_4(uint32_t dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
