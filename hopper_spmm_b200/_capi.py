@@ -42,6 +42,11 @@ class Int4(C.Structure):
     _fields_ = [("rows", u64), ("cols", u64), ("group", i32), ("scale_dtype", i32), ("device", i32), ("values", vp), ("scales", vp), ("zeros", vp)]
 
 
+class Moe(C.Structure):
+    _fields_ = [("experts", u64), ("hidden", u64), ("inner", u64), ("top_k", i32), ("renormalize", i32), ("dtype", i32), ("device", i32), ("router", vp), ("ld_router", i64),
+                ("gate_up", C.POINTER(Int4)), ("down", C.POINTER(Int4)), ("gate_up_16", vp), ("down_16", vp), ("ld_gate_up", i64), ("ld_down", i64)]
+
+
 class KatMma(C.Structure):
     _fields_ = [(n, u32) for n in ("a_off", "a_lbo", "a_sbo", "a_swizzle", "b_off", "b_lbo", "b_sbo", "b_swizzle",
                                    "idesc", "d_col", "accumulate", "kind")]
@@ -138,6 +143,9 @@ SIGNATURES = {
     "b200spmm_fp4_status": (C.c_int, [C.c_int, vp]),
     "b200spmm_rms_norm": (C.c_int, [C.POINTER(RmsNorm), vp]),
     "b200spmm_int4_product": (C.c_int, [C.POINTER(Int4), vp, i64, i64, C.c_int, C.c_int, vp, C.c_int, vp, i64, C.c_int, C.c_int, vp]),
+    "b200spmm_moe_workspace": (C.c_int, [C.POINTER(Moe), i64, C.POINTER(u64)]),
+    "b200spmm_moe": (C.c_int, [C.POINTER(Moe), vp, i64, i64, vp, i64, vp, vp, vp, u64, vp]),
+    "b200spmm_moe_experts": (C.c_int, [C.POINTER(Moe), vp, i64, i64, vp, C.c_int, vp, vp, i64, vp, u64, vp]),
     "b200spmm_kat_umma": (C.c_int, [vp, u32, C.POINTER(KatMma), C.c_int, C.c_int, vp, C.c_int]),
     "b200spmm_kat_umma_pair": (C.c_int, [vp, u32, C.POINTER(KatMma), C.c_int, C.c_int, vp, C.c_int]),
     "b200spmm_kat_wait_limit": (C.c_uint64, [C.c_uint64]),

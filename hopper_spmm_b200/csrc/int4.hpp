@@ -54,13 +54,13 @@ uint32_t steps_that_fit(uint32_t steps, uint32_t cols, uint32_t planes, uint64_t
     return (uint32_t)std::min<uint64_t>((pitch - 64) / 128 * 128 / (W::kUnits * 16u), steps);
 }
 
-// Lets a kernel have all the shared memory of a block, once for each device; `allowed` keeps which.
+// Lets a kernel have so much shared memory, once for each device; `allowed` keeps which.
 template <typename... P>
-cudaError_t allow_smem(void (*kernel)(P...), std::atomic<uint64_t> &allowed) {
+cudaError_t allow_smem(void (*kernel)(P...), std::atomic<uint64_t> &allowed, uint32_t bytes = kMaxSmem) {
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess || (allowed.load(std::memory_order_relaxed) >> device & 1u)) return e;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e == cudaSuccess) allowed.fetch_or(1ull << device);
     return e;
 }

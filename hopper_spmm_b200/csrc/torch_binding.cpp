@@ -585,6 +585,156 @@ PyObject *int4_product(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// A mixture-of-experts layer: what the C ABI gets of it, behind a capsule.  dtype -1: no part of it has a 16-bit type, the input's will do.
+constexpr const char *kMoe = "b200spmm_moe_t";
+struct Moe {
+    b200spmm_moe_t m{};
+    b200spmm_int4_t gate_up{}, down{};
+};
+void free_moe(PyObject *capsule) { delete static_cast<Moe *>(PyCapsule_GetPointer(capsule, kMoe)); }
+
+// moe_layer(router or None, gate_up, down (capsules of Int4Matrix, or tensors), experts, hidden, inner, top_k, renormalize) -> capsule
+PyObject *moe_layer(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 8) {
+        PyErr_SetString(PyExc_TypeError, "moe_layer takes 8 arguments");
+        return nullptr;
+    }
+    const int64_t E = PyLong_AsLongLong(args[3]), H = PyLong_AsLongLong(args[4]), I = PyLong_AsLongLong(args[5]), top = PyLong_AsLongLong(args[6]);
+    if (PyErr_Occurred()) return nullptr;
+    if (E < 1 || E > 1024) return refuse("there must be between 1 and 1024 experts");
+    if (H < 1 || I < 1 || H > 0x1000000 || I > 0x1000000) return refuse("the hidden and inner sizes must lie between 1 and 2^24");
+    if (top < 1 || top > 32) return refuse("top_k must lie between 1 and 32");
+    if (args[0] != Py_None && top > E) return refuse("top_k must not be above the number of experts");
+    Moe made;
+    b200spmm_moe_t &m = made.m;
+    m.experts = (uint64_t)E;
+    m.hidden = (uint64_t)H;
+    m.inner = (uint64_t)I;
+    m.top_k = (int32_t)top;
+    m.renormalize = args[7] == Py_True;
+    m.dtype = m.device = -1;
+    bool lost = false, one_type = true, one_device = true, cuda = true;
+    auto joins = [&](const at::Tensor &t, bool typed) {
+        const int type = type_code(t.scalar_type()), device = t.is_cuda() ? (int)t.get_device() : -2;
+        cuda = cuda && t.is_cuda();
+        one_type = one_type && (!typed || m.dtype == -1 || m.dtype == type);
+        one_device = one_device && (m.device == -1 || m.device == device);
+        if (typed) m.dtype = type;
+        m.device = device;
+        lost = lost || wants_gradient(t);
+    };
+    auto is_16 = [](const at::Tensor &t) { return (t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16) && t.layout() == at::kStrided && !t.is_neg(); };
+    if (args[0] != Py_None) {
+        const at::Tensor *r = THPVariable_Check(args[0]) ? &THPVariable_Unpack(args[0]) : nullptr;
+        Rows at;
+        if (!r || !is_16(*r) || r->dim() != 2 || r->size(0) != E || r->size(1) != H || !rows_of(*r, &at))
+            return refuse("router must be a float16 or bfloat16 tensor [experts, hidden] with unit stride along its rows");
+        joins(*r, true);
+        m.router = at.ptr;
+        m.ld_router = at.ld;
+    }
+    if (PyCapsule_IsValid(args[1], kInt4) != PyCapsule_IsValid(args[2], kInt4)) return refuse("gate_up and down must both be Int4Matrix, or both 16-bit tensors");
+    if (PyCapsule_IsValid(args[1], kInt4)) {
+        made.gate_up = *static_cast<const b200spmm_int4_t *>(PyCapsule_GetPointer(args[1], kInt4));
+        made.down = *static_cast<const b200spmm_int4_t *>(PyCapsule_GetPointer(args[2], kInt4));
+        if (made.gate_up.rows != (uint64_t)(E * 2 * I) || made.gate_up.cols != (uint64_t)H || made.down.rows != (uint64_t)(E * H) || made.down.cols != (uint64_t)I)
+            return refuse("gate_up must have experts x 2 inner rows of the hidden size, down experts x hidden rows of the inner size");
+        one_device = one_device && made.gate_up.device == made.down.device && (m.device == -1 || m.device == made.gate_up.device);
+        m.device = made.gate_up.device;
+    } else {
+        const int64_t rows[2] = {2 * I, H}, cols[2] = {H, I};
+        for (int i = 0; i < 2; ++i) {
+            const at::Tensor *w = THPVariable_Check(args[1 + i]) ? &THPVariable_Unpack(args[1 + i]) : nullptr;
+            if (!w || !is_16(*w) || w->dim() != 3 || w->size(0) != E || w->size(1) != rows[i] || w->size(2) != cols[i])
+                return refuse("gate_up must be [experts, 2 inner, hidden] and down [experts, hidden, inner], float16 or bfloat16");
+            const int64_t ld = w->stride(1);
+            if ((cols[i] > 1 && w->stride(2) != 1) || ld < cols[i] || ld % 8 != 0 || (E > 1 && w->stride(0) != rows[i] * ld) || reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 != 0)
+                return refuse("rows of 16-bit experts must start on 16 bytes, a multiple of 8 elements apart, and experts follow one another: pad the last dimension");
+            joins(*w, true);
+            (i ? m.down_16 : m.gate_up_16) = w->data_ptr();
+            (i ? m.ld_down : m.ld_gate_up) = ld;
+        }
+    }
+    if (lost) return refuse(kNoGradient);
+    if (!one_type) return refuse("the router and 16-bit experts must have one type");
+    if (!cuda || !one_device) return refuse("all parts of the layer must be on one CUDA device");
+    PyObject *out = PyCapsule_New(new Moe(made), kMoe, free_moe);
+    return out;
+    END_HANDLE_TH_ERRORS
+}
+
+// moe(capsule, X, out or None, routing wanted, ids or None, shares or None) -> (out, ids or None, shares or None), the first a status where it is a number
+PyObject *moe(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 6) {
+        PyErr_SetString(PyExc_TypeError, "moe takes 6 arguments");
+        return nullptr;
+    }
+    const auto *layer = static_cast<const Moe *>(PyCapsule_GetPointer(args[0], kMoe));
+    if (!layer) return nullptr;
+    b200spmm_moe_t m = layer->m;
+    const at::Tensor *X = cuda_tensor(args[1]);
+    Rows x, y;
+    const bool typed = X && (X->scalar_type() == at::kHalf || X->scalar_type() == at::kBFloat16) && (m.dtype == -1 || type_code(X->scalar_type()) == m.dtype);
+    if (!typed || X->dim() != 2 || X->size(1) != (int64_t)m.hidden || X->get_device() != m.device || !rows_of(*X, &x))
+        return refuse("X must be a CUDA tensor [tokens, hidden] of the layer's 16-bit type, on its device, with unit stride along its rows");
+    const int64_t tokens = X->size(0);
+    if (tokens > 256) return refuse("a call takes up to 256 tokens");
+    m.dtype = type_code(X->scalar_type());
+    if (layer->gate_up.values || layer->gate_up.rows) {
+        m.gate_up = &layer->gate_up;
+        m.down = &layer->down;
+    }
+    const bool given = args[4] != Py_None, routing = args[3] == Py_True;
+    if (!given && !m.router) return refuse("the layer has no router: give it the experts' ids and shares");
+    bool lost = wants_gradient(*X);
+    const at::Tensor *ids = nullptr, *shares = nullptr;
+    if (given) {
+        ids = cuda_tensor(args[4]);
+        shares = cuda_tensor(args[5]);
+        auto fits = [&](const at::Tensor *t) { return t && t->get_device() == m.device && t->dim() == 2 && t->size(0) == tokens && t->size(1) == m.top_k && t->is_contiguous(); };
+        if (!fits(ids) || (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong)) return refuse("ids must be a contiguous int32 or int64 tensor [tokens, top_k] on the layer's device");
+        if (!fits(shares) || shares->scalar_type() != at::kFloat) return refuse("shares must be a contiguous float32 tensor [tokens, top_k] on the layer's device");
+        lost = lost || wants_gradient(*shares);
+    }
+    at::Tensor Y, new_ids, new_shares, workspace;
+    if (args[2] != Py_None) {
+        const at::Tensor *t = cuda_tensor(args[2]);
+        if (!t || t->scalar_type() != X->scalar_type() || t->get_device() != m.device || t->dim() != 2 || t->size(0) != tokens || t->size(1) != (int64_t)m.hidden || !rows_of(*t, &y))
+            return refuse("out must be a tensor like X with unit stride along its rows");
+        lost = lost || wants_gradient(*t);
+    }
+    if (lost) return refuse(kNoGradient);
+    if (args[2] == Py_None) {
+        Y = new_cuda({tokens, (int64_t)m.hidden}, X->scalar_type(), *X);
+        y = {Y.data_ptr(), (int64_t)m.hidden};
+    }
+    if (routing) {
+        new_ids = new_cuda({tokens, (int64_t)m.top_k}, at::kInt, *X);
+        new_shares = new_cuda({tokens, (int64_t)m.top_k}, at::kFloat, *X);
+    }
+    uint64_t bytes = 0;
+    int st = b200spmm_moe_workspace(&m, tokens, &bytes);
+    if (st == B200SPMM_OK) {
+        workspace = new_cuda({(int64_t)bytes}, at::kByte, *X);
+        void *ws = workspace.data_ptr(), *stream = c10::cuda::getCurrentCUDAStream(X->get_device()).stream();
+        int32_t *i = routing ? static_cast<int32_t *>(new_ids.data_ptr()) : nullptr;
+        float *s = routing ? static_cast<float *>(new_shares.data_ptr()) : nullptr;
+        const void *ids_in = given ? ids->data_ptr() : nullptr;
+        const float *shares_in = given ? static_cast<const float *>(shares->data_ptr()) : nullptr;
+        const int id_bytes = given && ids->scalar_type() == at::kLong ? 8 : 4;
+        const ThreadsAllowed threads;
+        st = given ? b200spmm_moe_experts(&m, x.ptr, x.ld, tokens, ids_in, id_bytes, shares_in, y.ptr, y.ld, ws, bytes, stream)
+                   : b200spmm_moe(&m, x.ptr, x.ld, tokens, y.ptr, y.ld, i, s, ws, bytes, stream);
+    }
+    if (st != B200SPMM_OK) return three(PyLong_FromLong(st), again(Py_None), again(Py_None));
+    PyObject *a = Y.defined() ? THPVariable_Wrap(std::move(Y)) : again(args[2]);
+    PyObject *b = routing ? THPVariable_Wrap(std::move(new_ids)) : again(Py_None), *c = routing ? THPVariable_Wrap(std::move(new_shares)) : again(Py_None);
+    return three(a, b, c);
+    END_HANDLE_TH_ERRORS
+}
+
 template <PyObject *(*kFn)(PyObject *, PyObject *const *, Py_ssize_t)>
 PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kFn)); }
 
@@ -597,6 +747,8 @@ PyMethodDef methods[] = {{"spmm", reinterpret_cast<PyCFunction>(reinterpret_cast
                          {"rms_norm", fast<rms_norm>(), METH_FASTCALL, nullptr},
                          {"int4_matrix", fast<int4_matrix>(), METH_FASTCALL, nullptr},
                          {"int4_product", fast<int4_product>(), METH_FASTCALL, nullptr},
+                         {"moe_layer", fast<moe_layer>(), METH_FASTCALL, nullptr},
+                         {"moe", fast<moe>(), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

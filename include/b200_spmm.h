@@ -622,7 +622,38 @@ typedef struct {
 int b200spmm_int4_product(const b200spmm_int4_t *a, const void *d_B, int64_t ldb, int64_t n, int b_dtype, int b_transposed, const float *d_b_scales, int b_group,
                           void *d_C, int64_t ldc, int c_dtype, int c_transposed, void *stream);
 
-/* Both are asynchronous on `stream`, run on the device that the structure names, allocate nothing and may be captured; no wait in them can run out. */
+/*
+ * A mixture-of-experts layer for up to 256 tokens, x [tokens, hidden]:
+ *     logits = x router^T, shares = softmax(logits), the top_k largest (of equal ones the first; NaN counts as the largest), their shares divided by
+ *     their sum where `renormalize`;     y = sum over them of share x down_e (silu(gate_e x) * (up_e x))
+ * x, y and the router have one type, fp16 or bf16.  Experts: experts x 2 inner rows of `hidden` columns (for each expert first the gate's rows, then up's) and experts x hidden rows
+ * of `inner` columns, one after the other: in 4-bit integers (gate_up, down), or in x's type (gate_up_16, down_16, rows ld elements apart, a multiple of 8, 16-byte
+ * aligned), the others null.  Logits are added up in 64 bits, the inner values kept in 32 and multiplied as a sum of two 16-bit numbers.
+ * experts up to 1024, top_k up to 32.  A row of x with NaN gives NaN in its own row of y alone.
+ */
+typedef struct {
+    uint64_t experts, hidden, inner;
+    int32_t top_k, renormalize, dtype, device;
+    const void *router;
+    int64_t ld_router;
+    const b200spmm_int4_t *gate_up, *down;
+    const void *gate_up_16, *down_16;
+    int64_t ld_gate_up, ld_down;
+} b200spmm_moe_t;
+
+/* Bytes of the workspace of a call for so many tokens; 16-byte aligned, it belongs to the call until that is done on `stream`.  Needs no device. */
+int b200spmm_moe_workspace(const b200spmm_moe_t *m, int64_t tokens, uint64_t *bytes);
+/* ids [tokens, top_k] int32 and shares [tokens, top_k] receive the routing; null where it is not wanted. */
+int b200spmm_moe(const b200spmm_moe_t *m, const void *d_x, int64_t ldx, int64_t tokens, void *d_y, int64_t ldy, int32_t *d_ids, float *d_shares, void *workspace,
+                 uint64_t workspace_bytes, void *stream);
+/*
+ * The experts alone, with a routing that is given: ids [tokens, top_k] contiguous, of 4 or 8 bytes (id_bytes), in any order; those below 0 or from `experts` on
+ * are left out (a padded token's row of y is zeros), and the same expert may come twice.  m's router and renormalize are not looked at.
+ */
+int b200spmm_moe_experts(const b200spmm_moe_t *m, const void *d_x, int64_t ldx, int64_t tokens, const void *d_ids, int id_bytes, const float *d_shares, void *d_y,
+                         int64_t ldy, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* These are asynchronous on `stream`, run on the device that their structure names, allocate nothing and may be captured; no wait in them can run out. */
 
 #ifdef __cplusplus
 }

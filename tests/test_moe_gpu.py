@@ -1,0 +1,331 @@
+"""The mixture-of-experts layer on the GPU against its formula in 64 bits."""
+import pytest
+import torch
+
+import hopper_spmm_b200 as hs
+import int4_ref as ref
+from fp4_ref import EPS, TINY
+from hopper_spmm_b200 import _capi as capi
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16, E4M3 = torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn
+IDS = {F32: "f32", F16: "f16", BF16: "bf16"}.get
+
+
+def rand(*shape, seed, dtype=F32, spread=1.0):
+    return (torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda") * spread).to(dtype)
+
+
+def tokens_of(n, hidden, seed, dtype):
+    x = rand(n, hidden, seed=seed)
+    x[:, ::37] *= 20
+    return x.to(dtype)
+
+
+class Case:
+    """A layer, and its experts in 64 bits."""
+
+    def __init__(self, experts, hidden, inner, top, dtype, group=0, seed=1, renormalize=True, router=True, zeros=True):
+        self.E, self.H, self.I, self.top, self.dtype, self.group, self.renormalize = experts, hidden, inner, top, dtype, group, renormalize
+        self.router = rand(experts, hidden, seed=seed, dtype=dtype, spread=hidden ** -0.5) if router else None
+        if group is None or group:
+            self.gate_up = ref.matrix(experts * 2 * inner, hidden, group, seed + 1, dtype, zeros, spread=0.4 * hidden ** -0.5)
+            self.down = ref.matrix(experts * hidden, inner, group, seed + 2, dtype, zeros, spread=0.4 * inner ** -0.5)
+        else:
+            # rows that start on 16 bytes, with something between them
+            def weights(r, c, s):
+                return rand(experts, r, (c + 7) // 8 * 8 + 8, seed=s, dtype=dtype, spread=c ** -0.5)[:, :, :c]
+            self.gate_up, self.down = weights(2 * inner, hidden, seed + 1), weights(hidden, inner, seed + 2)
+        self.layer = hs.MoeLayer(self.router, self.gate_up, self.down, top_k=top, renormalize=renormalize, experts=experts)
+
+    def expert(self, e):
+        if self.group is None or self.group:
+            return ref.values_of(self.gate_up, slice(e * 2 * self.I, (e + 1) * 2 * self.I)), ref.values_of(self.down, slice(e * self.H, (e + 1) * self.H))
+        return self.gate_up[e].double(), self.down[e].double()
+
+    def check(self, y, x, ids, shares):
+        """y against the formula for this routing, within what its roundings can be.
+
+        A sum of K products takes K / 16 additions of the MMA (16-bit experts) or span / 16 of them and one rounding of fp32 for each span (codes), and up to 24 that join parts:
+        `off` of the sum of magnitudes.  An inner value is off by what its gate (SiLU's slope is at most 1.1) and up are, and 2^-20 of itself for exp, the division and the product.
+        It is multiplied as two 16-bit numbers: 2^-16 is lost (bf16; fp16 2^-22, and 2^-38 of the pair's largest).  Their products take twice the additions."""
+        x, want, bound = x.double(), torch.zeros(x.shape, dtype=torch.float64, device="cuda"), torch.zeros(x.shape, dtype=torch.float64, device="cuda")
+        span = 0 if self.group == 0 else min(128, self.group or 128)
+
+        def off(k, planes):
+            if span:
+                return planes * span / 16 * 2.0 ** -22 + (-(-k // span) + 24 + 2) * 2.0 ** -24
+            return (planes * -(-k // 16) + 24) * 2.0 ** -22
+
+        lost = 2.0 ** -16 if span or self.dtype == BF16 else 2.0 ** -22
+        for e in range(self.E):
+            t, j = torch.where(ids == e)
+            if len(t) == 0:
+                continue
+            gate_up, down = self.expert(e)
+            (g, u), (mg, mu) = (x[t] @ gate_up.t()).split(self.I, 1), (x[t].abs() @ gate_up.abs().t()).split(self.I, 1)
+            dg, du = mg * off(self.H, 1), mu * off(self.H, 1)
+            silu = g * torch.sigmoid(g)
+            h = silu * u
+            dh = 1.1 * dg * (u.abs() + du) + silu.abs() * du + h.abs() * 2.0 ** -20
+            dh = dh + h.abs() * lost + h.abs().amax(1, keepdim=True) * 2.0 ** -38
+            out, mag = h @ down.t(), h.abs() @ down.abs().t()
+            d = mag * off(self.I, 2) + dh @ down.abs().t()
+            s = shares[t, j].double()[:, None]
+            want.index_add_(0, t, s * out)
+            bound.index_add_(0, t, s.abs() * (d + out.abs() * (self.top + 1) * 2.0 ** -24))
+        bound = bound + (want.abs() + bound) * EPS[y.dtype] + TINY[y.dtype]
+        err = (y.double() - want).abs()
+        assert y.shape == want.shape and not torch.isnan(y).any()
+        worst = float((err / bound).max())
+        assert worst <= 1, f"{worst:.2f} times the bound"
+
+    def check_routing(self, x, ids, shares):
+        """Choices by logits that are off by at most 8 roundings of their sum of magnitudes; shares by that, exp, the sum and the division."""
+        logits, mag = x.double() @ self.router.double().t(), x.double().abs() @ self.router.double().abs().t()
+        near = mag.amax(1, keepdim=True) * 8 * 2.0 ** -24
+        ids = ids.long()
+        mine = logits.gather(1, ids)
+        assert (mine[:, :-1] >= mine[:, 1:] - 2 * near).all()
+        rest = logits.clone().scatter_(1, ids, -torch.inf)
+        assert (ids.sort(1)[0].diff(dim=1) > 0).all() and (mine.amin(1) >= rest.amax(1) - 2 * near[:, 0]).all()
+        want = torch.softmax(logits, 1).gather(1, ids)
+        want = want / want.sum(1, keepdim=True) if self.renormalize else want
+        assert ((shares.double() / want - 1).abs() <= 4 * near + 2.0 ** -20).all()
+
+
+# experts, hidden, inner, chosen, tokens
+SIZES = [(4, 64, 40, 2, 1), (8, 256, 128, 3, 5), (10, 1000, 333, 4, 17), (64, 512, 96, 8, 3), (5, 130, 1000, 5, 40), (3, 2049, 64, 1, 9), (1, 72, 8, 1, 2), (300, 96, 24, 2, 33), (16, 4100, 70, 2, 12), (4, 48, 2500, 4, 70)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
+@pytest.mark.parametrize("group", [0, 32, 64, 128, None], ids=str)
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_layer(size, group, dtype):
+    experts, hidden, inner, top, n = size
+    c = Case(experts, hidden, inner, top, dtype, group, seed=sum(size), renormalize=n % 2 == 1, zeros=hidden % 2 == 0)
+    x = tokens_of(n, hidden, 9, dtype)
+    y, ids, shares = c.layer.forward(x, return_routing=True)
+    assert y.dtype == dtype and ids.dtype == torch.int32 and shares.dtype == F32
+    c.check_routing(x, ids, shares)
+    c.check(y, x, ids, shares)
+    assert torch.equal(c.layer.forward(x), y)
+    assert torch.equal(c.layer.experts(x, ids, shares), y)
+    assert torch.equal(c.layer.experts(x, ids.long(), shares), y)
+
+
+@pytest.mark.parametrize("group", [0, 64], ids=str)
+def test_given_routing_with_masked_places(group):
+    c = Case(6, 200, 88, 4, BF16, group, router=False)
+    x = tokens_of(23, 200, 2, BF16)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    ids = torch.randint(-3, 9, (23, 4), generator=g, device="cuda")
+    ids[5] = -1
+    ids[6] = torch.tensor([2**33, -2**40, 6, -1], device="cuda")  # none of them an expert's
+    ids[7] = 3  # the same expert four times
+    shares = torch.rand(23, 4, generator=g, device="cuda") - 0.3
+    shares[5] = torch.nan  # of nobody
+    shares[6, 0] = torch.inf
+    y = c.layer.experts(x, ids, shares)
+    assert not y[5].any() and not y[6].any()
+    c.check(y, x, torch.where((ids >= 0) & (ids < 6), ids, -1), shares.nan_to_num(posinf=0))
+    small = torch.where((ids >= 0) & (ids < 6), ids, -1).int()
+    assert torch.equal(c.layer.experts(x, small, shares), y)
+    # nobody at all
+    assert not c.layer.experts(x, torch.full_like(small, -1), shares).any()
+    # what the rows of masked tokens hold does not matter, not even to others
+    x[5] = torch.nan
+    x[6] = torch.inf
+    assert torch.equal(c.layer.experts(x, ids, shares), y)
+
+
+@pytest.mark.parametrize("group", [0, 32], ids=str)
+def test_all_tokens_to_one_expert(group):
+    c = Case(5, 300, 72, 2, F16, group)
+    x = tokens_of(256, 300, 2, F16)
+    ids = torch.full((256, 2), 4, device="cuda", dtype=torch.int32)
+    ids[:, 1] = -1
+    shares = torch.ones(256, 2, device="cuda")
+    c.check(c.layer.experts(x, ids, shares), x, ids, shares)
+    y, i, s = c.layer.forward(x, return_routing=True)
+    c.check_routing(x, i, s)
+    c.check(y, x, i, s)
+
+
+def test_the_largest_routing():
+    c = Case(1024, 16, 8, 32, BF16)
+    x = tokens_of(256, 16, 2, BF16)
+    y, i, s = c.layer.forward(x, return_routing=True)
+    c.check_routing(x, i, s)
+    c.check(y, x, i, s)
+
+
+def test_of_equal_logits_the_first_is_chosen_and_nan_is_the_largest():
+    c = Case(40, 64, 16, 4, BF16)
+    c.router[:] = c.router[0]  # all equal
+    c.router[7] *= 2  # (but one)
+    c.router[33] = c.router[7]
+    x = tokens_of(6, 64, 2, BF16)
+    _, ids, shares = c.layer.forward(x, return_routing=True)
+    l = x.double() @ c.router.double().t()
+    for t in range(6):
+        assert ids[t].tolist() == ([7, 33, 0, 1] if l[t, 7] > l[t, 0] else [0, 1, 2, 3])
+    x[0] = 0  # +0 and -0 are one
+    x[1] = -0.0
+    assert c.layer.forward(x, return_routing=True)[1][:2].tolist() == [[0, 1, 2, 3]] * 2
+    # a token with a NaN is NaN as a whole, and no other is
+    y = c.layer.forward(x)
+    x[3, 5] = torch.nan
+    z, ids, shares = c.layer.forward(x, return_routing=True)
+    assert torch.isnan(z[3]).all() and torch.isnan(shares[3]).all() and ids[3].tolist() == [0, 1, 2, 3]
+    others = [0, 1, 2, 4, 5]
+    assert torch.equal(z[others], y[others])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
+def test_inner_values_beyond_the_range_of_fp16_and_far_below_it(dtype):
+    for spread in (300.0, 1e-4):
+        c = Case(4, 128, 64, 2, dtype)
+        c.gate_up.mul_(spread)
+        c.down.mul_(1e-4 if spread > 1 else 1.0)
+        x = tokens_of(7, 128, 2, dtype)
+        ids, shares = torch.tensor([[0, 3]] * 7, device="cuda"), torch.full((7, 2), 0.5, device="cuda")
+        c.check(c.layer.experts(x, ids, shares), x, ids, shares)
+
+
+def test_strides_and_results_in_place():
+    c = Case(6, 200, 80, 2, F16, 32)
+    wide = tokens_of(20, 230, 2, F16)
+    for x in (wide[:, 3:203], wide[::2, 8:208], wide[:1, 1:201]):
+        y, ids, shares = c.layer.forward(x, return_routing=True)
+        c.check(y, x, ids, shares)
+        room = torch.full((x.shape[0] + 2, 217), -7.0, dtype=F16, device="cuda")
+        out = room[1:-1, 5:205]
+        assert c.layer.forward(x, out) is out and torch.equal(out, y)
+        out.fill_(-7)
+        assert (room == -7).all()
+    router = torch.zeros(6, 211, dtype=F16, device="cuda")
+    router[:, 3:203] = c.router
+    other = hs.MoeLayer(router[:, 3:203], c.gate_up, c.down, top_k=2)
+    x = wide[:, 3:203]
+    assert torch.equal(other.forward(x), c.layer.forward(x))
+
+
+def test_empty():
+    c = Case(6, 200, 80, 2, F16, 32)
+    x = torch.empty(0, 200, dtype=F16, device="cuda")
+    y, ids, shares = c.layer.forward(x, return_routing=True)
+    assert y.shape == (0, 200) and ids.shape == shares.shape == (0, 2)
+    assert c.layer.experts(x, ids, shares).shape == (0, 200)
+
+
+def test_refusals_on_the_gpu():
+    c = Case(6, 200, 80, 2, F16, 32)
+    x = tokens_of(4, 200, 2, F16)
+    ids, shares = torch.zeros(4, 2, dtype=torch.int32, device="cuda"), torch.ones(4, 2, device="cuda")
+    for bad in (x.float(), x.bfloat16(), x[:, :199], x[None], x.t().contiguous().t(), x.cpu(), x[:1].expand(4, 200), None):
+        with pytest.raises(ValueError, match="X must"):
+            c.layer.forward(bad)
+    for bad in (ids.float(), ids[:3], ids[:, :1], ids.cpu(), ids.t().contiguous().t(), 3):
+        with pytest.raises(ValueError, match="ids must"):
+            c.layer.experts(x, bad, shares)
+    for bad in (shares.half(), shares[:3], shares.cpu(), 3):
+        with pytest.raises(ValueError, match="shares must"):
+            c.layer.experts(x, ids, bad)
+    with pytest.raises(ValueError, match="together"):
+        c.layer.experts(x, ids, None)
+    for bad in (torch.empty(4, 199, dtype=F16, device="cuda"), torch.empty(4, 200, device="cuda"), torch.empty(4, 400, dtype=F16, device="cuda")[:, ::2]):
+        with pytest.raises(ValueError, match="out must"):
+            c.layer.forward(x, bad)
+    with pytest.raises(ValueError, match="256 tokens"):
+        c.layer.forward(tokens_of(257, 200, 2, F16))
+    with pytest.raises(ValueError, match="no router"):
+        hs.MoeLayer(None, c.gate_up, c.down, top_k=2, experts=6).forward(x)
+    with pytest.raises(ValueError, match="number of experts"):
+        hs.MoeLayer(None, c.gate_up, c.down, top_k=2)
+    with pytest.raises(ValueError, match="both"):
+        hs.MoeLayer(c.router, c.gate_up, torch.zeros(6, 200, 80, dtype=F16, device="cuda"), top_k=2)
+    with pytest.raises(ValueError, match="rows"):
+        hs.MoeLayer(c.router[:5], c.gate_up, c.down, top_k=2)
+    with pytest.raises(ValueError, match="no backward"):
+        c.layer.forward(x.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("group", [0, 64], ids=str)
+def test_the_same_bits_on_every_stream_and_in_graphs(group):
+    c = Case(16, 512, 256, 3, BF16, group)
+    x = tokens_of(9, 512, 2, BF16)
+    want = c.layer.forward(x)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [c.layer.forward(x, stream=s) for s in streams * 4]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = c.layer.forward(x, return_routing=True)
+        graphs.append((g, out))
+    for seed in (5, 6):
+        x.copy_(tokens_of(9, 512, seed, BF16))
+        want = c.layer.forward(x, return_routing=True)
+        for g, _ in graphs * 2:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_a_workspace_of_any_content():
+    import ctypes as C
+    c = Case(8, 256, 96, 3, F16)
+    x = tokens_of(6, 256, 2, F16)
+    want = c.layer.forward(x)
+    m = capi.Moe(experts=8, hidden=256, inner=96, top_k=3, renormalize=1, dtype=capi.T_F16, device=0, router=c.router.data_ptr(), ld_router=256, gate_up_16=c.gate_up.data_ptr(),
+                 down_16=c.down.data_ptr(), ld_gate_up=c.gate_up.stride(1), ld_down=c.down.stride(1))
+    size = C.c_uint64()
+    assert capi.lib().b200spmm_moe_workspace(C.byref(m), 6, C.byref(size)) == capi.OK
+    for fill in (0, 255, 127):
+        ws = torch.full((size.value + 64,), fill, dtype=torch.uint8, device="cuda")
+        y = torch.empty_like(x)
+        for _ in range(2):  # and as the last call left it
+            assert capi.lib().b200spmm_moe(C.byref(m), x.data_ptr(), 256, 6, y.data_ptr(), 256, None, None, ws.data_ptr(), size.value, torch.cuda.current_stream().cuda_stream) == capi.OK
+            assert torch.equal(y, want)
+        assert (ws[size.value:] == fill).all()
+
+
+# ---------------------------------------------------------------- together
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
+@pytest.mark.parametrize("n", [1, 6, 33])
+def test_a_decoding_step(n, dtype):
+    # norm to 8 bits, a product with 4-bit integers, the residual and the norm again, the experts: each against the definition on the values it was given
+    H = 384
+    x, h, w1, w2 = tokens_of(n, H, 1, dtype), tokens_of(n, H, 2, dtype), rand(H, seed=3, dtype=dtype, spread=0.2) + 1, rand(H, seed=4, dtype=dtype, spread=0.2) + 1
+    W = ref.matrix(H, H, 128, 5, dtype, spread=0.4 * H ** -0.5)
+    c = Case(8, H, 200, 2, dtype, 64)
+    a, h1 = hs.rms_norm(x, w1, residual=h, dtype=E4M3, group=128)
+    assert torch.equal(h1, (x.float() + h.float()).to(dtype))
+    y = W.linear(a, dtype=dtype)
+    av = a.values.double() * a.scales.double().repeat_interleave(128, 1)[:, :H]
+    ref.check_product(y.t(), ref.values_of(W), av.t(), 128)
+    b, h2 = hs.rms_norm(y, w2, residual=h1)
+    want = h1.double() + y.double()
+    want = want / want.square().mean(1, keepdim=True).add(1e-6).sqrt() * w2.double()
+    assert ((b.double() - want).abs() <= want.abs() * (EPS[dtype] + 2.0 ** -18) + TINY[dtype]).all()
+    z, ids, shares = c.layer.forward(b, return_routing=True)
+    c.check_routing(b, ids, shares)
+    c.check(z, b, ids, shares)
+    # the same as one graph
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        a2, k1 = hs.rms_norm(x, w1, residual=h, dtype=E4M3, group=128)
+        b2, k2 = hs.rms_norm(W.linear(a2, dtype=dtype), w2, residual=k1)
+        z2 = c.layer.forward(b2)
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(z2, z) and torch.equal(k2, h2)
