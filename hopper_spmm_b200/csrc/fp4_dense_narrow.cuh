@@ -25,7 +25,7 @@
 #include <type_traits>
 
 #include "fp4_widen.cuh"
-#include "mma_16x8x16.cuh"
+#include "warp_mma.cuh"
 
 namespace b200spmm {
 namespace fp4 {

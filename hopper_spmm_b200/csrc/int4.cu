@@ -24,70 +24,71 @@ struct Int4Params {
     const float *x_scales;
     uint32_t x_groups, x_shift;
     Target c;
-    uint32_t tiles, warps, steps, chunk, cols;  // of all blocks together; of a block; of a row; that the columns have room for; of a pass, at most
+    uint32_t tiles, warps, steps, window, cols;  // of all blocks together; of a block; of a row; that the columns have room for; of a pass, at most
 };
 
-constexpr int kRing = 2;  // stages of a warp
 template <int kNB>
 constexpr uint32_t kMaxWarps = kNB <= 1 ? 28 : kNB <= 2 ? 24 : 16;
 
-template <typename T, int kSpan, int kNB, bool kScaled>
+// A lane's sums to C.
+template <typename T, int kNB>
+B200_DEVICE void store_sums(const Target &c, uint32_t row, uint32_t rows, uint32_t j0, uint32_t n, const float (&sums)[kNB][4]) {
+    const int64_t along = c.transposed ? 1 : c.ldc, across = c.transposed ? c.ldc : 1;
+    const uint32_t t = threadIdx.x & 3u;
+    T *out = reinterpret_cast<T *>(c.ptr);
+#pragma unroll
+    for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            const uint32_t j = nb * 8u + t * 2u + (e & 1u), r = row + (e >> 1) * 8u;
+            if (j < n && r < rows) out[(int64_t)r * along + (int64_t)(j0 + j) * across] = fp4::Elem<T>::from_float(sums[nb][e]);
+        }
+}
+
+// kScaled: columns in e4m3 with scales.
+template <typename T, int kSpan, int kNB, bool kScaled, int kRing>
 __global__ void __launch_bounds__(32 * kMaxWarps<kNB>, 1) int4_kernel(const Int4Params p) {
     using W = Weights<T, kSpan>;
     extern __shared__ __align__(128) uint8_t smem[];
-    const uint32_t base = ptx::smem_u32(smem), warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u, g = lane >> 2;
-    constexpr uint32_t ring_bytes = kRing * kStageBytes, ring_floats = ring_bytes / 4u;
-    const uint32_t j0 = blockIdx.y * (8u * kNB), n = min(8u * kNB, p.n - j0);
+    const uint32_t base = ptx::smem_u32(smem), warp = warp_index(), g = (threadIdx.x & 31u) >> 2;
+    constexpr uint32_t ring_bytes = kRing * kStageBytes;
+    const uint32_t j0 = blockIdx.y * (8u * kNB);
     Columns c;
     c.base = base + p.warps * ring_bytes;
-    c.pitch = column_pitch<W>(p.chunk);
+    c.pitch = column_pitch<W>(p.window);
     c.plane = 0;
+    c.n = min(8u * kNB, p.n - j0);
     c.scales = c.base + p.cols * c.pitch;
     c.groups = p.x_groups;
     c.shift = p.x_shift;
-    c.steps = p.chunk;
-    const uint32_t tile_begin = (uint32_t)((uint64_t)p.tiles * blockIdx.x / gridDim.x), tile_end = (uint32_t)((uint64_t)p.tiles * (blockIdx.x + 1u) / gridDim.x);
-    const Split split(tile_end - tile_begin, p.steps, p.warps);
+    const uint32_t begin = (uint32_t)((uint64_t)p.tiles * blockIdx.x / gridDim.x), end = (uint32_t)((uint64_t)p.tiles * (blockIdx.x + 1u) / gridDim.x);
+    const Split split(end - begin, p.steps, p.warps);
+    const Share s(split, begin, end, warp, p.steps, p.window, base + warp * ring_bytes);
     ptx::wait_for_grids_before();
     if constexpr (kScaled) {
         float *to = reinterpret_cast<float *>(smem + (c.scales - base));
-        for (uint32_t i = threadIdx.x; i < n * p.x_groups; i += blockDim.x) to[i] = p.x_scales[(uint64_t)j0 * p.x_groups + i];
+        for (uint32_t i = threadIdx.x; i < c.n * p.x_groups; i += blockDim.x) to[i] = p.x_scales[(uint64_t)j0 * p.x_groups + i];
     }
-    auto stage = [&](uint32_t first, uint32_t count) {
-        if constexpr (kScaled)
-            stage_columns<W>(Eights{static_cast<const uint8_t *>(p.x) + (int64_t)j0 * p.across, p.across, p.wide, p.k}, c, first, count, n, false);
-        else
-            stage_columns<W>(Plain<T>{static_cast<const T *>(p.x) + (int64_t)j0 * p.across, p.along, p.across, p.wide, p.k}, c, first, count, n, p.along != 1);
-    };
-    bool staged = false;
-    for (uint32_t tile0 = tile_begin; tile0 < tile_end; tile0 += split.at_once) {
-        const uint32_t tiles = min(split.at_once, tile_end - tile0), mine = warp / split.slices;
-        Share s;
-        s.slice = warp % split.slices;
-        s.slices = split.slices;
-        s.steps = p.steps;
-        s.ring = base + warp * ring_bytes;
-        s.busy = mine < tiles;
-        s.row_lo = min((tile0 + mine) * kTileRows + g, p.rows - 1u);
-        s.row_hi = min((tile0 + mine) * kTileRows + g + 8u, p.rows - 1u);
-        float sums[kNB][4] = {};
-        accumulate<W, kNB, 1, kScaled, kRing>(p.m, s, c, n, staged, stage, sums);
-        staged = p.chunk >= p.steps;
-        if (s.busy) leave_sums<kNB>(reinterpret_cast<float *>(smem + warp * ring_bytes), sums);
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < tiles * kTileRows * n; i += blockDim.x) {
-            const uint32_t r = i % kTileRows, j = i / kTileRows % n, of = i / (kTileRows * n), row = (tile0 + of) * kTileRows + r;
-            const float v[1] = {joined(reinterpret_cast<const float *>(smem), ring_floats, of * split.slices, split.slices, j, r)};
-            if (row < p.rows) fp4::store_row(p.c, row, j0 + j, p.n, v);
-        }
-        __syncthreads();
-    }
+    multiply<W, kNB, 1, kScaled, kRing>(
+        p.m, s, [&](uint32_t tile, uint32_t r) { return (uint64_t)min(tile * kTileRows + r, p.rows - 1u); }, [&](uint32_t) { return c; },
+        [&](uint32_t first, uint32_t count) {
+            if constexpr (kScaled)
+                stage_columns<W>(Eights{static_cast<const uint8_t *>(p.x) + (int64_t)j0 * p.across, p.across, p.wide, p.k}, c.base, c.pitch, first, count, c.n, false);
+            else
+                stage_columns<W>(Plain<T>{static_cast<const T *>(p.x) + (int64_t)j0 * p.across, p.along, p.across, p.wide, p.k}, c.base, c.pitch, first, count, c.n, p.along != 1);
+        },
+        [&](uint32_t tile, const float(&sums)[kNB][4]) {
+            const uint32_t row = tile * kTileRows + g;
+            if (p.c.type == B200SPMM_T_F32) store_sums<float, kNB>(p.c, row, p.rows, j0, c.n, sums);
+            else if (p.c.type == B200SPMM_T_F16) store_sums<__half, kNB>(p.c, row, p.rows, j0, c.n, sums);
+            else store_sums<__nv_bfloat16, kNB>(p.c, row, p.rows, j0, c.n, sums);
+        });
 }
 
-template <typename T, int kSpan, int kNB, bool kScaled>
+template <typename T, int kSpan, int kNB, bool kScaled, int kRing>
 int launch(Int4Params p, cudaStream_t stream) {
     using W = Weights<T, kSpan>;
-    auto kernel = int4_kernel<T, kSpan, kNB, kScaled>;
+    auto kernel = int4_kernel<T, kSpan, kNB, kScaled, kRing>;
     const uint32_t blocks = std::min<uint32_t>(p.tiles, fp4::sm_count()), passes = (p.n + 8 * kNB - 1) / (8 * kNB);
     p.steps = (p.k + W::kStep - 1) / W::kStep;
     p.cols = std::min<uint32_t>(8 * kNB, p.n);
@@ -95,9 +96,10 @@ int launch(Int4Params p, cudaStream_t stream) {
     p.warps = split.at_once * split.slices;
     // the columns as a whole, or as much of them as there is room for
     const uint64_t taken = (uint64_t)p.warps * kRing * kStageBytes + (kScaled ? (uint64_t)p.cols * p.x_groups * 4u : 0u);
-    p.chunk = steps_that_fit<W>(p.steps, p.cols, 1, taken);
-    if (p.chunk == 0) return B200SPMM_ERR_UNSUPPORTED;
-    const uint32_t bytes = (uint32_t)taken + p.cols * column_pitch<W>(p.chunk);
+    p.window = steps_that_fit<W>(p.steps, p.cols, 1, taken);
+    if (kRing == 4 && p.window < p.steps) return launch<T, kSpan, kNB, kScaled, 2>(p, stream);  // (half the ring, more room)
+    if (p.window == 0) return B200SPMM_ERR_UNSUPPORTED;
+    const uint32_t bytes = (uint32_t)taken + p.cols * column_pitch<W>(p.window);
     static std::atomic<uint64_t> allowed{0};
     B200_CUDA_TRY(allow_smem(kernel, allowed));
     B200_CUDA_TRY(launch_after(kernel, dim3(blocks, passes), 32u * p.warps, bytes, 1, stream, p));
@@ -106,9 +108,9 @@ int launch(Int4Params p, cudaStream_t stream) {
 
 template <typename T, int kSpan, bool kScaled>
 int launch_width(const Int4Params &p, cudaStream_t stream) {
-    if (p.n <= 8) return launch<T, kSpan, 1, kScaled>(p, stream);
-    if (p.n <= 16) return launch<T, kSpan, 2, kScaled>(p, stream);
-    return launch<T, kSpan, 4, kScaled>(p, stream);
+    if (p.n <= 8) return launch<T, kSpan, 1, kScaled, 4>(p, stream);
+    if (p.n <= 16) return launch<T, kSpan, 2, kScaled, 4>(p, stream);
+    return launch<T, kSpan, 4, kScaled, 4>(p, stream);
 }
 template <typename T, bool kScaled>
 int launch_span(const Int4Params &p, uint32_t span, cudaStream_t stream) {

@@ -21,7 +21,7 @@ inline int check_int4(const b200spmm_int4_t *m) {
 }
 
 inline uint32_t shift_of(int group) {
-    uint32_t s = 31;  // one group, however long the row is
+    uint32_t s = kWholeGroup;
     if (group)
         for (s = 0; (1 << s) < group; ++s) {}
     return s;

@@ -1,12 +1,12 @@
-// A mixture-of-experts layer for a few tokens, in three kernels: logits; routing, gate, up and SiLU; down and the weighted sum.
+// A mixture-of-experts layer for a few tokens: logits; routing, gate, up and SiLU; down; the weighted sum.
 //
 //     y_t = sum over chosen experts e of  share_te  D_e (silu(G_e x_t) * (U_e x_t))
 //
-// Bound: one read of every chosen expert.  Work is counted in tiles of the chosen experts, one expert's after the other's, and shared out evenly over the SMs, whose blocks multiply
-// each tile with all tokens of its expert (narrow.cuh).  A tile of the first product is 8 rows of the gate and the same 8 of up: both values of an inner value
-// lie in one warp, and SiLU is taken where the sums are joined.  The second product's results are left for each token and expert; who comes last to 16 rows of
-// y adds them up in the order of the token's choices, so that the result is the same whoever that is.  Nobody waits for anybody.
-// The routing is cheap and needed by every block: each finds the chosen experts for itself, from the logits, before its first tile.
+// Bound: one read of every chosen expert.  The pairs of a token and a choice, sorted by expert and cut into runs of up to 16, are what an expert's tiles are multiplied with; the
+// tiles of all runs, one run's after the other's, are shared out evenly over the SMs, whose warps take a tile each, or a part of one, and run ahead into the next
+// (narrow.cuh).  A tile of the first product is 8 rows of the gate and the same 8 of up: both values of an inner value lie in one lane.  The second product's results are
+// left for each pair; a last kernel adds them up in the order of the token's choices.
+// The routing is cheap and needed by every block: each finds the runs for itself, from the logits, before its first tile.
 #include <type_traits>
 
 #include "entry.hpp"
@@ -18,15 +18,18 @@ namespace narrow {
 namespace {
 
 constexpr uint32_t kWarps = 24, kThreads = 32 * kWarps;
-constexpr int kRing = 2;
-constexpr uint32_t kRingBytes = kRing * kStageBytes, kRingFloats = kRingBytes / 4;
+constexpr uint32_t kRun = 16;  // columns that a tile meets at once, at most
+template <class W>
+constexpr int kRing = 4;  // stages of a warp
+template <class W>
+constexpr uint32_t kRingBytes = kRing<W> * kStageBytes;
 constexpr uint32_t kMaxTokens = 256, kMaxExperts = 1024, kMaxTop = 32;
-constexpr uint32_t kMoeSmem = kMaxSmem - 1024;  // beside a few numbers of a block's own
-constexpr uint32_t kLogitTokens = 8, kLogitThreads = 128;
+constexpr uint32_t kLogitTokens = 4, kLogitThreads = 256;
 
 struct MoeParams {
     Matrix gate_up, down;
     uint32_t experts, hidden, inner, top, tokens, pairs;
+    uint32_t up_run, up_columns, down_run, down_columns;  // columns of a run, and that a block has room for, in either product
     bool renormalize;
     const void *x, *router;
     int64_t ldx, ld_router, ldy;
@@ -38,7 +41,6 @@ struct MoeParams {
     int id_bytes;
     int32_t *ids;          // [pairs], as used: -1 for none
     float *shares;
-    uint32_t *arrived;     // for every 16 rows of y
     float *h;              // [pairs][h_ld]
     uint32_t h_ld;
     float *parts;          // [pairs][hidden]
@@ -95,21 +97,20 @@ B200_DEVICE uint64_t key_of(double v) {
 // A block's view of the routing, in shared memory.
 struct Routing {
     int32_t *ids;       // [pairs]
-    uint16_t *active;   // the chosen experts, ascending
-    uint16_t *counts;   // of their pairs
-    uint16_t *pairs;    // of the expert at hand, ascending
-    uint32_t *n_active;
-    uint8_t *flags;     // tiles of a round that a block has completed
+    uint16_t *pairs;    // [pairs] by expert, ascending
+    uint16_t *starts;   // [experts + 1]: of an expert's pairs
+    uint32_t *runs;     // expert << 16 | first of its pairs
+    uint32_t *n_runs;
 };
-__host__ __device__ inline uint32_t routing_bytes(uint32_t pairs, uint32_t experts) { return (4u * pairs + 4u * experts + 2u * pairs + 16u + 32u + 127u) / 128u * 128u; }
+// (an expert with n pairs has at most n runs)
+__host__ __device__ inline uint32_t routing_bytes(uint32_t pairs, uint32_t experts) { return (10u * pairs + 2u * experts + 2u + 16u + 15u + 127u) / 128u * 128u; }
 B200_DEVICE Routing routing_at(uint8_t *at, uint32_t pairs, uint32_t experts) {
     Routing r;
-    r.ids = reinterpret_cast<int32_t *>(at);
-    r.n_active = reinterpret_cast<uint32_t *>(at + 4u * pairs);
-    r.flags = at + 4u * pairs + 16u;
-    r.active = reinterpret_cast<uint16_t *>(at + 4u * pairs + 48u);
-    r.counts = r.active + experts;
-    r.pairs = r.counts + experts;
+    r.n_runs = reinterpret_cast<uint32_t *>(at);
+    r.ids = reinterpret_cast<int32_t *>(at + 16u);
+    r.runs = reinterpret_cast<uint32_t *>(r.ids + pairs);
+    r.pairs = reinterpret_cast<uint16_t *>(r.runs + pairs);
+    r.starts = r.pairs + pairs;
     return r;
 }
 
@@ -157,46 +158,72 @@ B200_DEVICE void choose(const MoeParams &p, uint32_t t, int32_t *ids, bool write
     }
 }
 
-// The chosen experts and how many pairs each has, from the ids in shared memory, by all threads.
-B200_DEVICE void find_active(const MoeParams &p, const Routing &r) {
+// The runs, of up to `most` pairs, from the ids in shared memory, by all threads.
+B200_DEVICE void find_runs(const MoeParams &p, const Routing &r, uint32_t most) {
     __syncthreads();
     for (uint32_t e = threadIdx.x; e < p.experts; e += kThreads) {
         uint32_t n = 0;
         for (uint32_t i = 0; i < p.pairs; ++i) n += r.ids[i] == (int32_t)e ? 1u : 0u;
-        r.counts[e] = (uint16_t)n;
+        r.starts[e] = (uint16_t)n;
     }
     __syncthreads();
-    if (threadIdx.x < 32u) {
-        uint32_t n = 0;
+    if (threadIdx.x < 32u) {  // the starts in place of the numbers, and the runs
+        uint32_t pairs = 0, runs = 0;
         for (uint32_t e0 = 0; e0 < p.experts; e0 += 32u) {
-            const uint32_t e = e0 + threadIdx.x;
-            const bool on = e < p.experts && r.counts[e] != 0;
-            const uint32_t all = __ballot_sync(0xFFFFFFFFu, on);
-            if (on) r.active[n + __popc(all & ((1u << threadIdx.x) - 1u))] = (uint16_t)e;
-            n += __popc(all);
+            const uint32_t e = e0 + threadIdx.x, n = e < p.experts ? r.starts[e] : 0u, m = (n + most - 1u) / most;
+            uint32_t n_to = n, m_to = m;  // up to this one
+#pragma unroll
+            for (uint32_t d = 1; d < 32u; d *= 2u) {
+                const uint32_t a = __shfl_up_sync(0xFFFFFFFFu, n_to, d), b = __shfl_up_sync(0xFFFFFFFFu, m_to, d);
+                if (threadIdx.x >= d) {
+                    n_to += a;
+                    m_to += b;
+                }
+            }
+            if (e < p.experts) r.starts[e] = (uint16_t)(pairs + n_to - n);
+            for (uint32_t i = 0; i < m; ++i) r.runs[runs + m_to - m + i] = e << 16 | (pairs + n_to - n + i * most);
+            pairs += __shfl_sync(0xFFFFFFFFu, n_to, 31);
+            runs += __shfl_sync(0xFFFFFFFFu, m_to, 31);
         }
-        if (threadIdx.x == 0) *r.n_active = n;
-    }
-    __syncthreads();
-}
-
-// The pairs of an expert, ascending, by the first warp; the others wait.
-B200_DEVICE void list_pairs(const MoeParams &p, const Routing &r, uint32_t expert) {
-    __syncthreads();
-    if (threadIdx.x < 32u) {
-        uint32_t n = 0;
-        for (uint32_t i0 = 0; i0 < p.pairs; i0 += 32u) {
-            const uint32_t i = i0 + threadIdx.x;
-            const bool on = i < p.pairs && r.ids[i] == (int32_t)expert;
-            const uint32_t all = __ballot_sync(0xFFFFFFFFu, on);
-            if (on) r.pairs[n + __popc(all & ((1u << threadIdx.x) - 1u))] = (uint16_t)i;
-            n += __popc(all);
+        if (threadIdx.x == 0) {
+            r.starts[p.experts] = (uint16_t)pairs;
+            *r.n_runs = runs;
         }
     }
     __syncthreads();
+    for (uint32_t e = threadIdx.x; e < p.experts; e += kThreads) {
+        uint32_t to = r.starts[e];
+        if (to == r.starts[e + 1u]) continue;
+        for (uint32_t i = 0; i < p.pairs; ++i)
+            if (r.ids[i] == (int32_t)e) r.pairs[to++] = (uint16_t)i;
+    }
+    __syncthreads();
+}
+B200_DEVICE uint32_t run_expert(const Routing &r, uint32_t run) { return r.runs[run] >> 16; }
+B200_DEVICE uint32_t run_start(const Routing &r, uint32_t run) { return r.runs[run] & 0xFFFFu; }
+B200_DEVICE uint32_t run_end(const Routing &r, uint32_t run) {  // (the last one ends with its expert's pairs)
+    return run + 1u < *r.n_runs ? run_start(r, run + 1u) : r.starts[run_expert(r, run) + 1u];
 }
 
-// Tokens of an expert as columns.
+// A block's share of `of_run` tiles of every run, in parts whose columns have room: part(first, end, first run's pairs, how many, the longest run's).
+template <class Part>
+B200_DEVICE void each_part(const Routing &r, uint32_t of_run, uint32_t room, Part &&part) {
+    const uint32_t all = *r.n_runs * of_run, end = (uint32_t)((uint64_t)all * (blockIdx.x + 1u) / gridDim.x);
+    for (uint32_t at = (uint32_t)((uint64_t)all * blockIdx.x / gridDim.x); at < end;) {
+        const uint32_t run0 = at / of_run, pair0 = run_start(r, run0);
+        uint32_t run = run0, longest = 0;
+        while (run * of_run < end && run < *r.n_runs && run_end(r, run) - pair0 <= room) {
+            longest = max(longest, run_end(r, run) - run_start(r, run));
+            ++run;
+        }
+        const uint32_t to = min(end, run * of_run);
+        part(at, to, pair0, run_end(r, run - 1u) - pair0, longest);
+        at = to;
+        __syncthreads();  // (the columns and the rings are free again)
+    }
+}
+
+// Tokens of pairs as columns.
 template <typename T>
 struct Gathered {
     Plain<T> x;
@@ -205,58 +232,45 @@ struct Gathered {
     B200_DEVICE uint4 operator()(uint32_t j, uint32_t u) const { return x(pairs[j] / top, u); }
 };
 
-// A part of a block's work: tiles of one expert.
-struct Segment {
-    uint32_t expert, n, tile, tiles;
-};
-
 // ------------------------------------------------------------------ gate, up, SiLU
 
 template <class W, int kNB>
-B200_DEVICE void gate_up_pass(const MoeParams &p, const Segment &g, const Routing &r, uint8_t *smem, uint32_t columns_at, uint32_t columns_bytes, uint32_t j0, uint32_t n) {
+B200_DEVICE void gate_up_part(const MoeParams &p, const Routing &r, uint8_t *smem, uint32_t columns_at, uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n) {
     using T = typename W::T;
-    const uint32_t base = ptx::smem_u32(smem), warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), row = (threadIdx.x & 31u) >> 2;
-    const uint32_t steps = (p.hidden + W::kStep - 1) / W::kStep;
-    Columns c{};
-    c.base = base + columns_at;
-    c.steps = min(steps, (columns_bytes / n - 64u) / 128u * 128u / (W::kUnits * 16u));
-    c.pitch = column_pitch<W>(c.steps);
-    const Split split(g.tiles, steps, kWarps);
-    auto stage = [&](uint32_t first, uint32_t count) {
-        stage_columns<W>(Gathered<T>{Plain<T>{static_cast<const T *>(p.x), 1, p.ldx, p.x_wide, p.hidden}, r.pairs + j0, p.top}, c, first, count, n, false);
-    };
-    bool staged = false;
-    for (uint32_t tile0 = 0; tile0 < g.tiles; tile0 += split.at_once) {
-        const uint32_t tiles = min(split.at_once, g.tiles - tile0), mine = warp / split.slices;
-        const uint32_t i = min((g.tile + tile0 + mine) * 8u + row, p.inner - 1u);
-        Share s;
-        s.slice = warp % split.slices;
-        s.slices = split.slices;
-        s.steps = steps;
-        s.ring = base + warp * kRingBytes;
-        s.busy = mine < tiles;
-        s.row_lo = (uint64_t)g.expert * 2u * p.inner + i;
-        s.row_hi = s.row_lo + p.inner;
-        float sums[kNB][4] = {};
-        accumulate<W, kNB, 1, false, kRing>(p.gate_up, s, c, n, staged, stage, sums);
-        staged = c.steps >= steps;
-        if (s.busy) leave_sums<kNB>(reinterpret_cast<float *>(smem + warp * kRingBytes), sums);
-        __syncthreads();
-        for (uint32_t k = threadIdx.x; k < tiles * 8u * n; k += kThreads) {
-            const uint32_t q = k % 8u, j = k / 8u % n, of = k / (8u * n), at = (g.tile + tile0 + of) * 8u + q;
-            const float a = joined(reinterpret_cast<const float *>(smem), kRingFloats, of * split.slices, split.slices, j, q);
-            const float b = joined(reinterpret_cast<const float *>(smem), kRingFloats, of * split.slices, split.slices, j, q + 8u);
-            if (at < p.inner) p.h[(uint64_t)r.pairs[j0 + j] * p.h_ld + at] = a / (1.f + expf(-a)) * b;
-        }
-        __syncthreads();
-    }
+    const uint32_t base = ptx::smem_u32(smem), warp = warp_index(), lane = threadIdx.x & 31u;
+    const uint32_t steps = (p.hidden + W::kStep - 1) / W::kStep, of_run = (p.inner + 7u) / 8u, pitch = column_pitch<W>(steps);
+    const Split split(end - begin, steps, kWarps);
+    const Share s(split, begin, end, warp, steps, steps, base + warp * kRingBytes<W>);
+    multiply<W, kNB, 1, false, kRing<W>>(
+        p.gate_up, s,
+        [&](uint32_t tile, uint32_t row) {
+            const uint32_t i = min(tile % of_run * 8u + row % 8u, p.inner - 1u);
+            return ((uint64_t)run_expert(r, tile / of_run) * 2u + row / 8u) * p.inner + i;
+        },
+        [&](uint32_t tile) {
+            const uint32_t run = tile / of_run;
+            return Columns{base + columns_at + (run_start(r, run) - pair0) * pitch, pitch, 0, run_end(r, run) - run_start(r, run), 0, 0, 0};
+        },
+        [&](uint32_t first, uint32_t count) {
+            stage_columns<W>(Gathered<T>{Plain<T>{static_cast<const T *>(p.x), 1, p.ldx, p.x_wide, p.hidden}, r.pairs + pair0, p.top}, base + columns_at, pitch, first, count, n, false);
+        },
+        [&](uint32_t tile, const float(&sums)[kNB][4]) {
+            const uint32_t run = tile / of_run, i = tile % of_run * 8u + (lane >> 2), start = run_start(r, run), of = run_end(r, run) - start;
+#pragma unroll
+            for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
+#pragma unroll
+                for (uint32_t e = 0; e < 2; ++e) {
+                    const uint32_t j = nb * 8u + (lane & 3u) * 2u + e;
+                    if (j < of && i < p.inner) p.h[(uint64_t)r.pairs[start + j] * p.h_ld + i] = sums[nb][e] / (1.f + expf(-sums[nb][e])) * sums[nb][e + 2];
+                }
+        });
 }
 
 template <class W>
 __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const MoeParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
-    const Routing r = routing_at(smem + kWarps * kRingBytes, p.pairs, p.experts);
-    const uint32_t columns_at = kWarps * kRingBytes + routing_bytes(p.pairs, p.experts), columns_bytes = kMoeSmem - columns_at;
+    const Routing r = routing_at(smem + kWarps * kRingBytes<W>, p.pairs, p.experts);
+    const uint32_t columns_at = kWarps * kRingBytes<W> + routing_bytes(p.pairs, p.experts);
     ptx::wait_for_grids_before();
     const bool write = blockIdx.x == 0;
     if (p.logits) {
@@ -269,175 +283,120 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const MoeParams p)
             if (write) p.ids[i] = id;
         }
     }
-    if (write)
-        for (uint32_t i = threadIdx.x; i < (p.hidden + kTileRows - 1u) / kTileRows; i += kThreads) p.arrived[i] = 0;
-    find_active(p, r);
-    const uint32_t of_expert = (p.inner + 7u) / 8u, all = *r.n_active * of_expert;
-    const uint32_t end = (uint32_t)((uint64_t)all * (blockIdx.x + 1u) / gridDim.x);
-    for (uint32_t at = (uint32_t)((uint64_t)all * blockIdx.x / gridDim.x); at < end;) {
-        Segment g;
-        g.expert = r.active[at / of_expert];
-        g.n = r.counts[g.expert];
-        g.tile = at % of_expert;
-        g.tiles = min(end - at, of_expert - g.tile);
-        list_pairs(p, r, g.expert);
-        for (uint32_t j0 = 0; j0 < g.n; j0 += 16u) {
-            const uint32_t n = min(16u, g.n - j0);
-            if (n <= 8u) gate_up_pass<W, 1>(p, g, r, smem, columns_at, columns_bytes, j0, n);
-            else gate_up_pass<W, 2>(p, g, r, smem, columns_at, columns_bytes, j0, n);
-        }
-        at += g.tiles;
-    }
+    find_runs(p, r, p.up_run);
+    each_part(r, (p.inner + 7u) / 8u, p.up_columns, [&](uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n, uint32_t longest) {
+        if (longest <= 8u) gate_up_part<W, 1>(p, r, smem, columns_at, begin, end, pair0, n);
+        else gate_up_part<W, 2>(p, r, smem, columns_at, begin, end, pair0, n);
+    });
 }
 
-// ------------------------------------------------------------------ down and the sum
+// ------------------------------------------------------------------ down
 
 // Inner values as a sum of two 16-bit numbers, the second what the first leaves over: fp16 has 22 digits that way, bf16 16.  fp16 gets them scaled by a power of two that takes
 // the pair's largest to [2^14, 2^15).
 template <typename T>
-struct Halves {
-    const float *h;
-    const uint16_t *pairs;
-    const float *scale;  // of column j; null: 1
-    uint32_t ld, k;
-    B200_DEVICE void operator()(uint32_t j, uint32_t u, uint4 *high, uint4 *low) const {
-        const float *from = h + (uint64_t)pairs[j] * ld + u * 8u, by = scale ? scale[j] : 1.f;
-        alignas(16) float v[8];
-        reinterpret_cast<float4 *>(v)[0] = reinterpret_cast<const float4 *>(from)[0];
-        reinterpret_cast<float4 *>(v)[1] = reinterpret_cast<const float4 *>(from)[1];
-        alignas(16) T a[8], b[8];
+B200_DEVICE void split_unit(const float *from, uint32_t left, float by, uint4 *high, uint4 *low) {
+    alignas(16) float v[8];
+    reinterpret_cast<float4 *>(v)[0] = reinterpret_cast<const float4 *>(from)[0];
+    reinterpret_cast<float4 *>(v)[1] = reinterpret_cast<const float4 *>(from)[1];
+    alignas(16) T a[8], b[8];
 #pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) {
-            const float x = u * 8u + e < k ? v[e] * by : 0.f;
-            a[e] = fp4::Elem<T>::from_float(x);
-            const float rest = x - fp4::Elem<T>::to_float(a[e]);
-            b[e] = fp4::Elem<T>::from_float(fabsf(rest) <= 3.0e38f ? rest : 0.f);  // (an infinity or NaN is the first number's)
-        }
-        *high = *reinterpret_cast<const uint4 *>(a);
-        *low = *reinterpret_cast<const uint4 *>(b);
+    for (uint32_t e = 0; e < 8; ++e) {
+        const float x = e < left ? v[e] * by : 0.f;
+        a[e] = fp4::Elem<T>::from_float(x);
+        const float rest = x - fp4::Elem<T>::to_float(a[e]);
+        b[e] = fp4::Elem<T>::from_float(fabsf(rest) <= 3.0e38f ? rest : 0.f);  // (an infinity or NaN is the first number's)
     }
-};
+    *high = *reinterpret_cast<const uint4 *>(a);
+    *low = *reinterpret_cast<const uint4 *>(b);
+}
 
 template <class W, int kNB>
-B200_DEVICE void down_pass(const MoeParams &p, const Segment &g, const Routing &r, uint8_t *smem, uint32_t columns_at, uint32_t columns_bytes, float *scales, uint32_t j0, uint32_t n, bool last) {
+B200_DEVICE void down_part(const MoeParams &p, const Routing &r, uint8_t *smem, uint32_t columns_at, uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n) {
     using T = typename W::T;
     constexpr bool kScale = std::is_same<T, __half>::value;
-    const uint32_t base = ptx::smem_u32(smem), warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u, row = lane >> 2;
-    const uint32_t steps = (p.inner + W::kStep - 1) / W::kStep;
-    Columns c{};
-    c.base = base + columns_at;
-    c.steps = min(steps, (columns_bytes / (2u * n) - 64u) / 128u * 128u / (W::kUnits * 16u));
-    c.pitch = column_pitch<W>(c.steps);
-    c.plane = n * c.pitch;
-    if constexpr (kScale) {
-        for (uint32_t j = warp; j < n; j += kWarps) {
-            const float *h = p.h + (uint64_t)r.pairs[j0 + j] * p.h_ld;
-            uint32_t top = 0;
-            for (uint32_t i = lane; i < p.inner; i += 32u) {
-                const uint32_t b = __float_as_uint(h[i]) & 0x7FFFFFFFu;
-                if (b < fp4::kInfBits) top = max(top, b);
+    const uint32_t base = ptx::smem_u32(smem), warp = warp_index(), lane = threadIdx.x & 31u;
+    const uint32_t steps = (p.inner + W::kStep - 1) / W::kStep, of_run = (p.hidden + kTileRows - 1u) / kTileRows, pitch = column_pitch<W>(steps), plane = p.down_columns * pitch;
+    float *scales = reinterpret_cast<float *>(smem + columns_at + 2u * plane);  // of the columns
+    const Split split(end - begin, steps, kWarps);
+    const Share s(split, begin, end, warp, steps, steps, base + warp * kRingBytes<W>);
+    multiply<W, kNB, 2, false, kRing<W>>(
+        p.down, s,
+        [&](uint32_t tile, uint32_t row) { return (uint64_t)run_expert(r, tile / of_run) * p.hidden + min(tile % of_run * kTileRows + row, p.hidden - 1u); },
+        [&](uint32_t tile) {
+            const uint32_t run = tile / of_run;
+            return Columns{base + columns_at + (run_start(r, run) - pair0) * pitch, pitch, plane, run_end(r, run) - run_start(r, run), 0, 0, 0};
+        },
+        [&](uint32_t, uint32_t count) {
+            const uint32_t units = count * W::kUnits;
+            for (uint32_t j = warp; j < n; j += kWarps) {
+                const float *h = p.h + (uint64_t)r.pairs[pair0 + j] * p.h_ld;
+                float by = 1.f;
+                if constexpr (kScale) {
+                    uint32_t top = 0;
+                    for (uint32_t i = lane; i < p.inner; i += 32u) {
+                        const uint32_t b = __float_as_uint(h[i]) & 0x7FFFFFFFu;
+                        if (b < fp4::kInfBits) top = max(top, b);
+                    }
+                    top = __reduce_max_sync(0xFFFFFFFFu, top);
+                    by = fp4::exp2_int(max(-126, min(126, 14 - ((int)(top >> 23) - 127))));
+                    if (lane == 0) scales[j] = by;
+                }
+                for (uint32_t u = lane; u < units; u += 32u) {
+                    uint4 high = make_uint4(0u, 0u, 0u, 0u), low = high;
+                    if (u * 8u < p.inner) split_unit<T>(h + u * 8u, p.inner - u * 8u, by, &high, &low);
+                    const uint32_t to = base + columns_at + j * pitch + unit_place<W>(u);
+                    ptx::st_shared_v4(to, unit_order<W>(high));
+                    ptx::st_shared_v4(to + plane, unit_order<W>(low));
+                }
             }
-            top = __reduce_max_sync(0xFFFFFFFFu, top);
-            if (lane == 0) scales[j] = fp4::exp2_int(max(-126, min(126, 14 - ((int)(top >> 23) - 127))));
-        }
-        __syncthreads();
-    }
-    const Split split(g.tiles, steps, kWarps);
-    auto stage = [&](uint32_t first, uint32_t count) {
-        const Halves<T> from{p.h, r.pairs + j0, kScale ? scales : nullptr, p.h_ld, p.inner};
-        const uint32_t units = count * W::kUnits, have = (p.inner + 7u) / 8u, u0 = first * W::kUnits;
-        for (uint32_t i = threadIdx.x; i < n * units; i += kThreads) {
-            const uint32_t j = i / units, u = i - j * units, to = c.base + j * c.pitch + unit_place<W>(u) * 16u;
-            uint4 high = make_uint4(0u, 0u, 0u, 0u), low = high;
-            if (u0 + u < have) from(j, u0 + u, &high, &low);
-            ptx::st_shared_v4(to, unit_order<W>(high));
-            ptx::st_shared_v4(to + c.plane, unit_order<W>(low));
-        }
-    };
-    bool staged = false;
-    for (uint32_t tile0 = 0; tile0 < g.tiles; tile0 += split.at_once) {
-        const uint32_t tiles = min(split.at_once, g.tiles - tile0), mine = warp / split.slices;
-        Share s;
-        s.slice = warp % split.slices;
-        s.slices = split.slices;
-        s.steps = steps;
-        s.ring = base + warp * kRingBytes;
-        s.busy = mine < tiles;
-        s.row_lo = (uint64_t)g.expert * p.hidden + min((g.tile + tile0 + mine) * kTileRows + row, p.hidden - 1u);
-        s.row_hi = (uint64_t)g.expert * p.hidden + min((g.tile + tile0 + mine) * kTileRows + row + 8u, p.hidden - 1u);
-        float sums[kNB][4] = {};
-        accumulate<W, kNB, 2, false, kRing>(p.down, s, c, n, staged, stage, sums);
-        staged = c.steps >= steps;
-        if (s.busy) leave_sums<kNB>(reinterpret_cast<float *>(smem + warp * kRingBytes), sums);
-        __syncthreads();
-        for (uint32_t k = threadIdx.x; k < tiles * kTileRows * n; k += kThreads) {
-            const uint32_t q = k % kTileRows, j = k / kTileRows % n, of = k / (kTileRows * n), at = (g.tile + tile0 + of) * kTileRows + q;
-            float v = joined(reinterpret_cast<const float *>(smem), kRingFloats, of * split.slices, split.slices, j, q);
-            if constexpr (kScale) v = v / scales[j];
-            if (at < p.hidden) p.parts[(uint64_t)r.pairs[j0 + j] * p.hidden + at] = v;
-        }
-        if (!last) {
-            __syncthreads();
-            continue;
-        }
-        // What this block left of these rows is there before its arrival is; who sees all the others' adds up.
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x < tiles) r.flags[threadIdx.x] = atomicAdd(p.arrived + g.tile + tile0 + threadIdx.x, 1u) + 1u == *r.n_active;
-        __threadfence();
-        __syncthreads();
-        for (uint32_t of = 0; of < tiles; ++of) {
-            if (!r.flags[of]) continue;
-            for (uint32_t k = threadIdx.x; k < kTileRows * p.tokens; k += kThreads) {
-                const uint32_t at = (g.tile + tile0 + of) * kTileRows + k % kTileRows, t = k / kTileRows;
-                if (at >= p.hidden) continue;
-                float v = 0.f;
-                for (uint32_t i = t * p.top; i < (t + 1u) * p.top; ++i)
-                    if (r.ids[i] >= 0) v = fmaf(p.shares[i], __ldcg(p.parts + (uint64_t)i * p.hidden + at), v);
-                static_cast<uint16_t *>(p.y)[(int64_t)t * p.ldy + at] = p.y_f16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
-            }
-        }
-        __syncthreads();
-    }
+        },
+        [&](uint32_t tile, const float(&sums)[kNB][4]) {
+            const uint32_t run = tile / of_run, row = tile % of_run * kTileRows + (lane >> 2), start = run_start(r, run), of = run_end(r, run) - start;
+#pragma unroll
+            for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    const uint32_t j = nb * 8u + (lane & 3u) * 2u + (e & 1u), at = row + (e >> 1) * 8u;
+                    if (j < of && at < p.hidden) p.parts[(uint64_t)r.pairs[start + j] * p.hidden + at] = kScale ? sums[nb][e] / scales[start + j - pair0] : sums[nb][e];
+                }
+        });
 }
 
 template <class W>
 __global__ void __launch_bounds__(kThreads, 1) down_kernel(const MoeParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float scales[16];
-    const Routing r = routing_at(smem + kWarps * kRingBytes, p.pairs, p.experts);
-    const uint32_t columns_at = kWarps * kRingBytes + routing_bytes(p.pairs, p.experts), columns_bytes = kMoeSmem - columns_at;
+    const Routing r = routing_at(smem + kWarps * kRingBytes<W>, p.pairs, p.experts);
+    const uint32_t columns_at = kWarps * kRingBytes<W> + routing_bytes(p.pairs, p.experts);
     ptx::wait_for_grids_before();
     for (uint32_t i = threadIdx.x; i < p.pairs; i += kThreads) r.ids[i] = p.ids[i];
-    find_active(p, r);
-    const uint32_t of_expert = (p.hidden + kTileRows - 1u) / kTileRows, all = *r.n_active * of_expert;
-    if (all == 0) {  // nobody was chosen
-        for (uint32_t t = blockIdx.x; t < p.tokens; t += gridDim.x)
-            for (uint32_t i = threadIdx.x; i < p.hidden; i += kThreads) static_cast<uint16_t *>(p.y)[(int64_t)t * p.ldy + i] = 0;
-        return;
-    }
-    const uint32_t end = (uint32_t)((uint64_t)all * (blockIdx.x + 1u) / gridDim.x);
-    for (uint32_t at = (uint32_t)((uint64_t)all * blockIdx.x / gridDim.x); at < end;) {
-        Segment g;
-        g.expert = r.active[at / of_expert];
-        g.n = r.counts[g.expert];
-        g.tile = at % of_expert;
-        g.tiles = min(end - at, of_expert - g.tile);
-        list_pairs(p, r, g.expert);
-        for (uint32_t j0 = 0; j0 < g.n; j0 += 16u) {
-            const uint32_t n = min(16u, g.n - j0);
-            if (n <= 8u) down_pass<W, 1>(p, g, r, smem, columns_at, columns_bytes, scales, j0, n, j0 + n == g.n);
-            else down_pass<W, 2>(p, g, r, smem, columns_at, columns_bytes, scales, j0, n, j0 + n == g.n);
-        }
-        at += g.tiles;
-    }
+    find_runs(p, r, p.down_run);
+    each_part(r, (p.hidden + kTileRows - 1u) / kTileRows, p.down_columns, [&](uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n, uint32_t longest) {
+        if (longest <= 8u) down_part<W, 1>(p, r, smem, columns_at, begin, end, pair0, n);
+        else down_part<W, 2>(p, r, smem, columns_at, begin, end, pair0, n);
+    });
+}
+
+// ------------------------------------------------------------------ the weighted sum, in the order of the choices
+
+constexpr uint32_t kSumThreads = 128;
+
+__global__ void __launch_bounds__(kSumThreads) sum_kernel(const MoeParams p) {
+    ptx::wait_for_grids_before();
+    const uint32_t at = blockIdx.x * kSumThreads + threadIdx.x, t = blockIdx.y;
+    if (at >= p.hidden) return;
+    float v = 0.f;
+#pragma unroll 8
+    for (uint32_t i = t * p.top; i < (t + 1u) * p.top; ++i)
+        if (p.ids[i] >= 0) v = fmaf(p.shares[i], p.parts[(uint64_t)i * p.hidden + at], v);
+    static_cast<uint16_t *>(p.y)[(int64_t)t * p.ldy + at] = p.y_f16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
 
 // ------------------------------------------------------------------ launches
 
 // Where the parts of the workspace begin.
 struct Layout {
-    uint64_t logits, ids, shares, arrived, h, parts, bytes;
+    uint64_t logits, ids, shares, h, parts, bytes;
     uint32_t h_ld;
 };
 Layout layout_of(const b200spmm_moe_t *m, uint64_t tokens) {
@@ -453,7 +412,6 @@ Layout layout_of(const b200spmm_moe_t *m, uint64_t tokens) {
     l.logits = take(tokens * m->experts * 8);
     l.ids = take(pairs * 4);
     l.shares = take(pairs * 4);
-    l.arrived = take((m->hidden + kTileRows - 1) / kTileRows * 4);
     l.h = take(pairs * l.h_ld * 4);
     l.parts = take(pairs * m->hidden * 4);
     l.bytes = at;
@@ -491,40 +449,55 @@ Matrix plain_matrix(const void *values, int64_t ld, uint64_t cols) {
     return out;
 }
 
+// Columns that a block has room for, in `planes` parts, and of a run.
 template <class W>
-int launch_gate_up(const MoeParams &p, uint32_t blocks, cudaStream_t stream) {
+bool room_for(const MoeParams &p, uint32_t k, uint32_t planes, uint32_t *columns, uint32_t *run) {
+    const uint32_t taken = kWarps * kRingBytes<W> + routing_bytes(p.pairs, p.experts), steps = (k + W::kStep - 1) / W::kStep;
+    const uint64_t each = (uint64_t)planes * ((uint64_t)steps * W::kUnits * 16u + 192u) + 4u;
+    *columns = (uint32_t)std::min<uint64_t>(p.pairs, (kMaxSmem - taken) / each);
+    *run = std::min(kRun, *columns);
+    return *columns > 0;
+}
+template <class W>
+int launch_gate_up(MoeParams *p, uint32_t blocks, cudaStream_t stream) {
     static std::atomic<uint64_t> allowed{0};
-    B200_CUDA_TRY(allow_smem(gate_up_kernel<W>, allowed, kMoeSmem));
-    B200_CUDA_TRY(launch_after(gate_up_kernel<W>, dim3(blocks), kThreads, kMoeSmem, 1, stream, p));
+    if (!room_for<W>(*p, p->hidden, 1, &p->up_columns, &p->up_run)) return B200SPMM_ERR_UNSUPPORTED;
+    B200_CUDA_TRY(allow_smem(gate_up_kernel<W>, allowed));
+    B200_CUDA_TRY(launch_after(gate_up_kernel<W>, dim3(blocks), kThreads, kMaxSmem, 1, stream, *p));
     return B200SPMM_OK;
 }
 template <class W>
-int launch_down(const MoeParams &p, uint32_t blocks, cudaStream_t stream) {
+int launch_down(MoeParams *p, uint32_t blocks, cudaStream_t stream) {
     static std::atomic<uint64_t> allowed{0};
-    B200_CUDA_TRY(allow_smem(down_kernel<W>, allowed, kMoeSmem));
-    B200_CUDA_TRY(launch_after(down_kernel<W>, dim3(blocks), kThreads, kMoeSmem, 1, stream, p));
+    if (!room_for<W>(*p, p->inner, 2, &p->down_columns, &p->down_run)) return B200SPMM_ERR_UNSUPPORTED;
+    B200_CUDA_TRY(allow_smem(down_kernel<W>, allowed));
+    B200_CUDA_TRY(launch_after(down_kernel<W>, dim3(blocks), kThreads, kMaxSmem, 1, stream, *p));
     return B200SPMM_OK;
 }
 
 template <typename T>
-int launch_moe(const b200spmm_moe_t *m, const MoeParams &p, double *logits, cudaStream_t stream) {
+int launch_moe(const b200spmm_moe_t *m, MoeParams p, double *logits, cudaStream_t stream) {
     if (logits) {
         B200_CUDA_TRY(launch_after(logits_kernel<T>, dim3(p.experts, (p.tokens + kLogitTokens - 1) / kLogitTokens), kLogitThreads, 0, 1, stream, p, logits));
     }
-    const uint64_t most = std::min<uint64_t>(p.experts, p.pairs);  // experts that may be chosen
+    const uint64_t most = p.pairs;  // runs that there may be
     auto blocks = [&](uint32_t tiles) { return (uint32_t)std::min<uint64_t>(fp4::sm_count(), most * tiles); };
     const uint32_t up = blocks((p.inner + 7) / 8), down = blocks((p.hidden + kTileRows - 1) / kTileRows);
     int st;
     if (m->gate_up) {
         const uint32_t a = span_of(m->gate_up), b = span_of(m->down);
-        st = a == 32 ? launch_gate_up<Weights<T, 32>>(p, up, stream) : a == 64 ? launch_gate_up<Weights<T, 64>>(p, up, stream) : launch_gate_up<Weights<T, 128>>(p, up, stream);
+        st = a == 32 ? launch_gate_up<Weights<T, 32>>(&p, up, stream) : a == 64 ? launch_gate_up<Weights<T, 64>>(&p, up, stream) : launch_gate_up<Weights<T, 128>>(&p, up, stream);
         if (st != B200SPMM_OK) return st;
         // bf16 for its range: inner values are as large as they are, and codes are exact in either type
         using B = __nv_bfloat16;
-        return b == 32 ? launch_down<Weights<B, 32>>(p, down, stream) : b == 64 ? launch_down<Weights<B, 64>>(p, down, stream) : launch_down<Weights<B, 128>>(p, down, stream);
+        st = b == 32 ? launch_down<Weights<B, 32>>(&p, down, stream) : b == 64 ? launch_down<Weights<B, 64>>(&p, down, stream) : launch_down<Weights<B, 128>>(&p, down, stream);
+    } else {
+        st = launch_gate_up<Weights<T, 0>>(&p, up, stream);
+        if (st == B200SPMM_OK) st = launch_down<Weights<T, 0>>(&p, down, stream);
     }
-    st = launch_gate_up<Weights<T, 0>>(p, up, stream);
-    return st != B200SPMM_OK ? st : launch_down<Weights<T, 0>>(p, down, stream);
+    if (st != B200SPMM_OK) return st;
+    B200_CUDA_TRY(launch_after(sum_kernel, dim3((p.hidden + kSumThreads - 1) / kSumThreads, p.tokens), kSumThreads, 0, 1, stream, p));
+    return B200SPMM_OK;
 }
 
 // ids null: they are found from the logits, and left, with the shares, at out_ids and out_shares where those are wanted.
@@ -557,7 +530,6 @@ int run_moe(const b200spmm_moe_t *m, const void *x, int64_t ldx, int64_t tokens,
     p.id_bytes = id_bytes;
     p.ids = out_ids ? out_ids : reinterpret_cast<int32_t *>(ws + l.ids);
     p.shares = shares ? const_cast<float *>(shares) : out_shares ? out_shares : reinterpret_cast<float *>(ws + l.shares);  // (given ones are only read)
-    p.arrived = reinterpret_cast<uint32_t *>(ws + l.arrived);
     p.h = reinterpret_cast<float *>(ws + l.h);
     p.h_ld = l.h_ld;
     p.parts = reinterpret_cast<float *>(ws + l.parts);

@@ -1,26 +1,31 @@
 // A few columns times rows of a weight matrix that is read once: what a block of threads does.
 //
 // Bound: one read of the matrix.  Each warp copies its own rows to a ring of its own in shared memory (cp.async, 16 bytes a lane), so no warp waits for
-// another while k goes by, and a wait is one for the lane's own copies.  A warp has a tile of 16 rows, or of every `slices`-th step of 128 bytes of those rows; the
-// columns lie in shared memory for all warps, as a whole where there is room, else piece by piece.  16 rows x 8 columns x 16 values of k meet in mma.sync: at
-// this width a product is a small part of the work, and for tcgen05 widened weights would have to go through shared or tensor memory.
+// another while k goes by, and a wait is one for the warp's own copies.  A warp has a tile of 16 rows at a time, or every `slices`-th step of 128 bytes of
+// those rows; its copies run ahead into its next tile.  The columns lie in shared memory for all warps, as a whole where there is room, else piece by piece.  16 rows x 8
+// columns meet in mma.sync: at this width a product is a small part of the work, and for tcgen05 widened weights would have to go through shared or tensor memory.
 //
 // Lane 4 g + t of a warp holds rows g and g + 8 of the tile.  Which values of k an operand position of the MMA stands for is free as long as both operands
 // agree, so a lane takes neighbours of its rows: of 4-bit integers kSpan / 4 of every kSpan, the widest span that has one scale (and one of the columns'
-// scales), whose sum is multiplied by them in fp32; of 16-bit values 8 of every 32.  Columns are stored in units of 16 bytes, 8 values of k, in the order in which lanes
-// t = 0..3 read them side by side, each unit in the order of the pairs that a mask takes out of a word of eight codes: 0 4, 1 5, 2 6, 3 7.
+// scales), whose sum is multiplied by them in fp32; of 16-bit values 8 of every 32.  Columns are stored in units of 8 values of k, in the order in which lanes
+// t = 0..3 read them side by side, each unit as the pairs that a mask takes out of a word of eight codes: 0 4, 1 5, 2 6, 3 7.
+// A step's first and second 64 bytes of a row are copied and waited for by themselves, so that less of the ring is idle.
+//
+// What it spends its time on is instructions, not bytes: the same copies with nothing else take 19.7 us for 28672 x 8192 codes, 120 MB.
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fp4_convert.cuh"
-#include "mma_16x8x16.cuh"
+#include "warp_mma.cuh"
 
 namespace b200spmm {
 namespace narrow {
 
-constexpr uint32_t kTileRows = 16, kStepBytes = 128, kStageBytes = kTileRows * kStepBytes;
+constexpr uint32_t kTileRows = 16, kStepBytes = 128, kHalfBytes = kStepBytes / 2, kStageBytes = kTileRows * kHalfBytes;  // (a stage is half a step)
 constexpr uint32_t kMaxSmem = 227 * 1024;
+constexpr uint32_t kWholeGroup = 31;  // a shift that leaves one group, however long a row is
 
 // Rows of weights: 4-bit integers or 16-bit values.
 struct Matrix {
@@ -35,31 +40,31 @@ struct Matrix {
     bool bf16_scales;
 };
 
-// T: the type of both operands of the MMA.  kSpan: columns of 4-bit integers that share their scales, 32, 64 or 128; 0: the weights are T themselves.
+// T: the type of the MMA's operands.  kSpan: columns of 4-bit integers that share their scales, 32, 64 or 128; 0: the weights are T themselves.
 template <typename T_, int kSpan_>
 struct Weights {
     using T = T_;
     static constexpr int kSpan = kSpan_;
     static constexpr bool kCodes = kSpan > 0;
     static constexpr uint32_t kStep = kCodes ? 2 * kStepBytes : kStepBytes / 2;  // values of k
-    static constexpr uint32_t kUnits = kStep / 8;                                // of a column
+    static constexpr uint32_t kUnits = kStep / 8;                                // of a column, in a step
     static constexpr uint32_t kBlocks = kCodes ? kStep / (kCodes ? kSpan : 1) : 2;  // of a step, with a scale each; halves
     static constexpr uint32_t kWords = kCodes ? 8 / kBlocks : 1;                 // of a lane in a block: units of 8 values
-    static constexpr uint32_t kEntries = kBlocks / 2;                            // scales that a lane fetches for its warp
+    static constexpr uint32_t kEntries = kCodes ? kBlocks / 2 : 1;               // scales that a lane fetches for its warp
 };
 
-// Where unit `u` (8 values of k from 8 u on) of a column lies.
+// Where unit `u` (8 values of k from 8 u on) of a column lies, in bytes.
 template <class W>
 B200_DEVICE uint32_t unit_place(uint32_t u) {
     if constexpr (W::kCodes) {
-        constexpr uint32_t n = W::kSpan / 8;
-        return u / n * n + u % (n / 4) * 4 + u % n / (n / 4);
+        constexpr uint32_t n = W::kSpan / 8, words = n / 4;
+        return (u / n * n + u % words * 4u + u % n / words) * 16u;
     } else {
-        return u;
+        return u * 16u;
     }
 }
 
-// The eight values of a unit in the order of its MMAs' operands.
+// The eight 16-bit values of a unit in the order of their MMAs' operands.
 template <class W>
 B200_DEVICE uint4 unit_order(uint4 v) {
     if constexpr (W::kCodes)
@@ -68,12 +73,9 @@ B200_DEVICE uint4 unit_order(uint4 v) {
         return v;
 }
 
-B200_DEVICE uint32_t shared_swizzle(uint32_t row) { return (row & 1u) << 2 | (row & 2u) | (row >> 2 & 1u); }  // of a row's eight pieces: no two lanes of a load meet in a bank
+B200_DEVICE uint32_t shared_swizzle(uint32_t row) { return (row & 2u) | (row >> 2 & 1u); }  // of a stage's four pieces of a row: no two lanes of a load meet in a bank
 
-// Eight codes less their zero, exactly: pairs 0 4, 1 5, 2 6, 3 7.  A code under the exponent of 1024 (or, four bits up, of 64 times 16; bf16: of 128) is that number and the
-// code; `minus` takes the number and the zero away.
-template <typename T> struct Widen;
-// (w & mask) | bits in one instruction: with both as constants the compiler makes two of it.
+// (w & mask) | bits in one instruction: with both as constants the compiler makes two of it (28672 x 8192 times one column: 38 us for 33).
 template <uint32_t kMask>
 B200_DEVICE uint32_t masked(uint32_t w, uint32_t bits) {
     uint32_t r;
@@ -85,11 +87,16 @@ B200_DEVICE uint32_t in_register(uint32_t constant) {
     asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(constant));
     return r;
 }
+
+// Eight codes less their zero, exactly: pairs 0 4, 1 5, 2 6, 3 7.  A code under the exponent of 1024 (or, four bits up, of 64 times 16; bf16: of 128) is that number and the
+// code; what is added takes the number and the zero away.
+template <typename T> struct Widen;
 template <>
 struct Widen<__half> {
-    uint32_t low, high;  // -(1024 + zero), -(64 + zero), twice
-    B200_DEVICE explicit Widen(uint32_t zero) : low(0xE400E400u | zero * 0x00010001u), high(0xD400D400u | zero * 0x00100010u) {}
     static constexpr uint32_t kBits = 0x64006400u;
+    B200_DEVICE static uint32_t minus(uint32_t zero) { return 0xE400E400u + zero * 0x00010001u; }
+    uint32_t low, high;  // -(1024 + zero), -(64 + zero), twice
+    B200_DEVICE explicit Widen(uint32_t minus) : low(minus), high(minus * 16u + (0xD400D400u - 0xE400E400u * 16u)) {}
     B200_DEVICE void operator()(uint32_t w, uint32_t bits, uint32_t (&out)[4]) const {
         const __half2 sixteenth = __half2half2(__ushort_as_half((unsigned short)0x2C00u));
 #pragma unroll
@@ -104,24 +111,24 @@ struct Widen<__half> {
 };
 template <>
 struct Widen<__nv_bfloat16> {
-    uint32_t minus;
-    B200_DEVICE explicit Widen(uint32_t zero) : minus(0xC300C300u | zero * 0x00010001u) {}
     static constexpr uint32_t kBits = 0x43004300u;
+    B200_DEVICE static uint32_t minus(uint32_t zero) { return 0xC300C300u + zero * 0x00010001u; }
+    uint32_t low;  // -(128 + zero), twice
+    B200_DEVICE explicit Widen(uint32_t minus) : low(minus) {}
     B200_DEVICE void operator()(uint32_t w, uint32_t bits, uint32_t (&out)[4]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i, w >>= 4) {
             const uint32_t a = masked<0x000F000Fu>(w, bits);
-            const __nv_bfloat162 x = __hadd2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&minus));
+            const __nv_bfloat162 x = __hadd2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&low));
             out[i] = *reinterpret_cast<const uint32_t *>(&x);
         }
     }
 };
 
-// The columns in shared memory: column j at base + j * pitch (and `plane` further on its second part, where it is the sum of two), and their scales, column by column.
+// The columns of a tile in shared memory: column j at base + j * pitch (and `plane` further on its second part, where it is the sum of two), and their scales.
 struct Columns {
-    uint32_t base, pitch, plane;
+    uint32_t base, pitch, plane, n;
     uint32_t scales, groups, shift;
-    uint32_t steps;  // that have room
 };
 
 template <int kBytes>
@@ -131,175 +138,8 @@ B200_DEVICE void ld_shared(uint32_t addr, uint32_t *v) {
     else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[0]) : "r"(addr) : "memory");
 }
 
-// What a warp does in a round of tiles.
-struct Share {
-    uint64_t row_lo, row_hi;  // of the matrix: rows g and g + 8 of the tile, as far as they exist
-    uint32_t slice, slices;   // steps slice, slice + slices, ...
-    uint32_t steps;           // of a whole row
-    uint32_t ring;            // shared memory
-    bool busy;
-};
-
-// sums[nb][e] += the products of the warp's steps: rows g (e < 2) and g + 8, columns 8 nb + 2 t + e % 2.  All threads of the block come here alike:
-// stage(step, count) brings these steps of the columns to shared memory; `staged` says that they are there as a whole.
-template <class W, int kNB, int kPlanes, bool kScaled, int kStages, class Stage>
-B200_DEVICE void accumulate(const Matrix &m, const Share &s, const Columns &c, uint32_t n, bool staged, Stage &&stage, float (&sums)[kNB][4]) {
-    using T = typename W::T;
-    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
-    // Copies run kStages steps ahead: rows g and g + 8, pieces t and t + 4.
-    const uint32_t own = g * kStepBytes + (t ^ shared_swizzle(g)) * 16u, ahead = s.slices * kStepBytes;
-    uint32_t copied = s.slice * kStepBytes + t * 16u;  // bytes of a row up to the next copy
-    const uint8_t *lo = m.values + s.row_lo * m.pitch + copied, *hi = m.values + s.row_hi * m.pitch + copied;
-    const uint32_t row_bytes = s.busy ? m.row_bytes : 0u;
-    auto issue = [&](uint32_t at) {
-        if constexpr (W::kCodes) {
-            // (codes behind a row's end meet zeros, whatever they are)
-            if (copied < row_bytes) {
-                ptx::cp_async_16(at + own, lo);
-                ptx::cp_async_16(at + own + 8u * kStepBytes, hi);
-            }
-            if (copied + 64u < row_bytes) {
-                ptx::cp_async_16(at + (own ^ 64u), lo + 64);
-                ptx::cp_async_16(at + (own ^ 64u) + 8u * kStepBytes, hi + 64);
-            }
-        } else {
-            if (copied - t * 16u < row_bytes) {
-#pragma unroll
-                for (uint32_t i = 0; i < 2; ++i) {  // zeros behind a row's end
-                    const uint32_t place = copied + i * 64u, left = place < row_bytes ? min(16u, row_bytes - place) : 0u, back = left ? i * 64u : 0u - copied;
-                    ptx::cp_async_16(at + (own ^ i * 64u), lo + (int32_t)back, left);
-                    ptx::cp_async_16(at + (own ^ i * 64u) + 8u * kStepBytes, hi + (int32_t)back, left);
-                }
-            }
-        }
-        ptx::cp_async_commit();
-        copied += ahead;
-        lo += ahead;
-        hi += ahead;
-    };
-    // Scales and zeros come by ordinary loads a step ahead, each to one lane of the four that need it: of row g (even t) or g + 8, blocks t / 2 + 2 i.
-    constexpr uint32_t kEntries = W::kCodes ? W::kEntries : 1u;
-    const uint32_t entry_row = (uint32_t)(t & 1u ? s.row_hi : s.row_lo);
-    uint32_t scale_next[kEntries], zero_next[kEntries], entry_k = s.slice * W::kStep + (t >> 1) * (uint32_t)W::kSpan;
-    auto fetch = [&]() {
-        if constexpr (W::kCodes) {
-#pragma unroll
-            for (uint32_t i = 0; i < kEntries; ++i) {  // (behind a row's end the last one again)
-                const uint32_t at = min((entry_k + 2u * i * (uint32_t)W::kSpan) >> m.shift, m.groups - 1u) * m.rows + entry_row;
-                scale_next[i] = m.scales[at];
-                zero_next[i] = m.zeros[at];
-            }
-            entry_k += s.slices * W::kStep;
-        }
-    };
-    if (s.busy) {
-#pragma unroll
-        for (uint32_t i = 0; i < kStages; ++i) issue(s.ring + i * kStageBytes);
-        fetch();
-    }
-    uint32_t column[kNB];  // this lane's, for the second operand; those behind the last are any of the others: nobody looks at their sums
-#pragma unroll
-    for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) column[nb] = c.base + min(nb * 8u + g, n - 1u) * c.pitch + t * 16u;
-    uint32_t step = s.slice, at = s.ring;
-    const uint32_t bits = W::kCodes ? in_register(Widen<T>::kBits) : 0u;
-    for (uint32_t first = 0; first < s.steps; first += c.steps) {
-        const uint32_t end = min(s.steps, first + c.steps);
-        if (!staged) {
-            if (first) __syncthreads();  // (nobody reads what was there any more)
-            stage(first, end - first);
-            __syncthreads();
-        }
-        for (; s.busy && step < end; step += s.slices) {
-            uint32_t entries[kEntries];  // a scale's bits in fp32, the zero in the lowest four (a scale has 11 digits at most)
-            if constexpr (W::kCodes) {
-#pragma unroll
-                for (uint32_t i = 0; i < kEntries; ++i) {
-                    const float v = m.bf16_scales ? __uint_as_float(scale_next[i] << 16) : __half2float(__ushort_as_half((unsigned short)scale_next[i]));
-                    entries[i] = (__float_as_uint(v) & ~15u) | (zero_next[i] & m.zero_mask) | m.zero_else;
-                }
-                fetch();
-            }
-            ptx::cp_async_wait_group<kStages - 1>();
-            __syncwarp();
-            const uint32_t x_at = (step - first) * (W::kUnits * 16u);
-#pragma unroll
-            for (uint32_t b = 0; b < W::kBlocks; ++b) {
-                constexpr uint32_t kRegs = W::kCodes ? W::kWords : 4u;
-                uint32_t w_lo[kRegs], w_hi[kRegs];
-                const uint32_t piece = W::kBlocks == 2 ? 4u * b + t : W::kBlocks == 4 ? 2u * b + (t >> 1) : b, rest = W::kBlocks == 2 ? 0u : W::kBlocks == 4 ? (t & 1u) * 8u : t * 4u;
-                const uint32_t from = at + g * kStepBytes + (piece ^ shared_swizzle(g)) * 16u + rest;
-                ld_shared<4 * kRegs>(from, w_lo);
-                ld_shared<4 * kRegs>(from + 8u * kStepBytes, w_hi);
-                if (b + 1 == W::kBlocks) {  // the stage is read: what comes kStages steps later may be copied there
-                    __syncwarp();
-                    issue(at);
-                    at = at + kStageBytes == s.ring + kStages * kStageBytes ? s.ring : at + kStageBytes;
-                }
-                if constexpr (!W::kCodes) {
-#pragma unroll
-                    for (int plane = 0; plane < kPlanes; ++plane)
-#pragma unroll
-                        for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
-                            const uint4 x = ptx::ld_shared_v4(column[nb] + x_at + b * 64u + plane * c.plane);
-                            fp4::mma_16x8x16<T>(sums[nb], w_lo[0], w_hi[0], w_lo[1], w_hi[1], x.x, x.y);
-                            fp4::mma_16x8x16<T>(sums[nb], w_lo[2], w_hi[2], w_lo[3], w_hi[3], x.z, x.w);
-                        }
-                } else {
-                    const uint32_t source = (lane & ~3u) | (b & 1u) << 1;
-                    const uint32_t e_lo = __shfl_sync(0xFFFFFFFFu, entries[b >> 1], source), e_hi = __shfl_sync(0xFFFFFFFFu, entries[b >> 1], source | 1u);
-                    const Widen<T> widen_lo(e_lo & 15u), widen_hi(e_hi & 15u);
-                    float part[kNB][4];
-#pragma unroll
-                    for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) part[nb][0] = part[nb][1] = part[nb][2] = part[nb][3] = 0.f;
-#pragma unroll
-                    for (uint32_t w = 0; w < W::kWords; ++w) {
-                        uint32_t a_lo[4], a_hi[4];
-                        widen_lo(w_lo[w], bits, a_lo);
-                        widen_hi(w_hi[w], bits, a_hi);
-#pragma unroll
-                        for (int plane = 0; plane < kPlanes; ++plane)
-#pragma unroll
-                            for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
-                                const uint4 x = ptx::ld_shared_v4(column[nb] + x_at + (b * W::kWords + w) * 64u + plane * c.plane);
-                                fp4::mma_16x8x16<T>(part[nb], a_lo[0], a_hi[0], a_lo[1], a_hi[1], x.x, x.y);
-                                fp4::mma_16x8x16<T>(part[nb], a_lo[2], a_hi[2], a_lo[3], a_hi[3], x.z, x.w);
-                            }
-                    }
-                    const float s_lo = __uint_as_float(e_lo & ~15u), s_hi = __uint_as_float(e_hi & ~15u);
-#pragma unroll
-                    for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
-                        float x0 = 1.f, x1 = 1.f;
-                        if constexpr (kScaled) {
-                            const uint32_t group = min((step * W::kStep + b * (uint32_t)W::kSpan) >> c.shift, c.groups - 1u), j = nb * 8u + t * 2u;
-                            x0 = __uint_as_float(ptx::ld_shared_u32(c.scales + (min(j, n - 1u) * c.groups + group) * 4u));
-                            x1 = __uint_as_float(ptx::ld_shared_u32(c.scales + (min(j + 1u, n - 1u) * c.groups + group) * 4u));
-                        }
-#pragma unroll
-                        for (uint32_t e = 0; e < 4; ++e) sums[nb][e] = fmaf(kScaled ? part[nb][e] * (e & 1u ? x1 : x0) : part[nb][e], e < 2 ? s_lo : s_hi, sums[nb][e]);
-                    }
-                }
-            }
-        }
-    }
-    __syncwarp();
-}
-
-// A warp's sums to its ring, [column][row], and one of a tile's from those of its slices, in order.
-template <int kNB>
-B200_DEVICE void leave_sums(float *ring, const float (&sums)[kNB][4]) {
-    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
-#pragma unroll
-    for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) ring[(nb * 8u + t * 2u + (e & 1u)) * kTileRows + (e >> 1) * 8u + g] = sums[nb][e];
-}
-B200_DEVICE float joined(const float *rings, uint32_t ring_floats, uint32_t first_warp, uint32_t slices, uint32_t column, uint32_t row) {
-    float v = 0.f;
-    for (uint32_t z = 0; z < slices; ++z) v += rings[(first_warp + z) * ring_floats + column * kTileRows + row];
-    return v;
-}
-
-// How a block goes through `tiles` of its own with up to `warps` warps: as many tiles at a time in every round, each cut along k as far as there are warps and steps.
+// How a block goes through `tiles` of its own with up to `warps` warps: as many tiles at a time in every round, each cut along k as far as there are warps and steps.  More
+// than one round means whole tiles.
 struct Split {
     uint32_t at_once, slices, rounds;
     __host__ __device__ Split(uint32_t tiles, uint32_t steps, uint32_t warps) {
@@ -310,6 +150,219 @@ struct Split {
         if (slices < 1) slices = 1;
     }
 };
+
+// The warp's number, by an operation whose result the compiler knows to be one for all lanes: what follows from it takes no lane's registers.
+B200_DEVICE uint32_t warp_index() { return __reduce_max_sync(0xFFFFFFFFu, threadIdx.x >> 5); }
+
+// What a warp does: tiles first, first + at_once ... below `end` (none, where it is beyond `at_once` or `end`), of each the steps slice, slice + slices ...
+struct Share {
+    uint32_t first, end;
+    uint32_t slice, slices, at_once, rounds;
+    uint32_t steps;   // of a whole row
+    uint32_t window;  // steps that the columns have room for
+    uint32_t ring;    // shared memory
+    B200_DEVICE Share(const Split &split, uint32_t begin, uint32_t end_, uint32_t warp, uint32_t steps_, uint32_t window_, uint32_t ring_)
+        : first(begin + warp / split.slices), end(end_), slice(warp % split.slices), slices(split.slices), at_once(split.at_once), rounds(split.rounds), steps(steps_), window(window_), ring(ring_) {
+        if (warp / split.slices >= split.at_once) first = end_;
+    }
+};
+
+// All threads of a block come here alike.  rows_of(tile, r) is row r (0 to 15) of a tile in the matrix, columns_of(tile) what it is multiplied with.  stage(first step, steps) brings columns to shared
+// memory, all of them before the first tile, or (window < steps) window by window in every round.  done(tile, sums) gets a tile's sums in one warp: rows g (e < 2) and g + 8,
+// columns 8 nb + 2 t + e % 2.
+template <class W, int kNB, int kPlanes, bool kScaled, int kStages, class RowsOf, class ColumnsOf, class Stage, class Done>
+B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, ColumnsOf &&columns_of, Stage &&stage, Done &&done) {
+    using T = typename W::T;
+    static_assert(kStages == 2 || kStages == 4, "a ring of one step or two");
+    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+    // Copies run kStages stages ahead: piece t of rows g and g + 8.
+    const uint32_t own = g * kHalfBytes + (t ^ shared_swizzle(g)) * 16u, last_copy = s.steps * kStepBytes;
+    uint32_t copy_tile = s.first, copied = 0;  // the next copy's tile, and bytes of a row up to it
+    const uint8_t *lo = nullptr, *hi = nullptr;
+    auto copy_from = [&]() {
+        copied = s.slice * kStepBytes + t * 16u;
+        lo = m.values + rows_of(copy_tile, g) * m.pitch + copied;
+        hi = m.values + rows_of(copy_tile, g + 8u) * m.pitch + copied;
+    };
+    auto issue = [&](uint32_t at, uint32_t half) {  // `half` of the next step
+        const uint32_t place = copied + half * kHalfBytes;
+        if constexpr (W::kCodes) {
+            const bool there = copy_tile < s.end && place < m.row_bytes;  // (codes behind a row's end meet zeros, whatever they are)
+            ptx::cp_async_16_if(there, at + own, lo + half * kHalfBytes);
+            ptx::cp_async_16_if(there, at + own + 8u * kHalfBytes, hi + half * kHalfBytes);
+        } else if (copy_tile < s.end) {  // zeros behind a row's end
+            const uint32_t left = place < m.row_bytes ? min(16u, m.row_bytes - place) : 0u, back = left ? half * kHalfBytes : 0u - copied;
+            ptx::cp_async_16(at + own, lo + (int32_t)back, left);
+            ptx::cp_async_16(at + own + 8u * kHalfBytes, hi + (int32_t)back, left);
+        }
+        if (half == 1u) {
+            const uint32_t ahead = s.slices * kStepBytes;
+            copied += ahead;
+            lo += ahead;
+            hi += ahead;
+            if (copied >= last_copy) {
+                copy_tile += s.at_once;
+                if (copy_tile < s.end) copy_from();
+                else copied = 0;
+            }
+        }
+        ptx::cp_async_commit();
+    };
+    // Scales and zeros come by ordinary loads a step ahead, each to one lane of the four that need it: of row g (even t) or g + 8, blocks t / 2 + 2 i.
+    constexpr uint32_t kEntries = W::kEntries;
+    uint32_t scale_next[kEntries], zero_next[kEntries], entry_tile = s.first, entry_row = 0, entry_k = 0;
+    const uint32_t entry_first = s.slice * W::kStep + (t >> 1) * (uint32_t)W::kSpan, entry_end = s.steps * W::kStep;
+    auto entries_from = [&]() {
+        entry_k = entry_first;
+        entry_row = (uint32_t)rows_of(entry_tile, g + (t & 1u) * 8u);
+    };
+    auto fetch = [&]() {
+        if constexpr (W::kCodes) {
+#pragma unroll
+            for (uint32_t i = 0; i < kEntries; ++i) {  // (behind a row's end the last one again)
+                const uint32_t at = min((entry_k + 2u * i * (uint32_t)W::kSpan) >> m.shift, m.groups - 1u) * m.rows + entry_row;
+                scale_next[i] = m.scales[at];
+                zero_next[i] = m.zeros[at];
+            }
+            entry_k += s.slices * W::kStep;
+            if (entry_k >= entry_end) {
+                entry_tile += s.at_once;
+                if (entry_tile < s.end) entries_from();
+            }
+        }
+    };
+    if (s.first < s.end) {
+        copy_from();
+#pragma unroll
+        for (uint32_t i = 0; i < kStages; ++i) issue(s.ring + i * kStageBytes, i % 2u);
+        if constexpr (W::kCodes) {
+            entries_from();
+            fetch();
+        }
+    }
+    const bool whole = s.window >= s.steps;
+    if (whole) {
+        stage(0u, s.steps);
+        __syncthreads();
+    }
+    const uint32_t bits = W::kCodes ? in_register(Widen<T>::kBits) : 0u;
+    uint32_t pair = s.ring, tile = s.first;  // a step's two stages
+    float sums[kNB][4];
+    for (uint32_t round = 0; round < s.rounds; ++round, tile += s.at_once) {
+        const bool busy = tile < s.end;
+        const Columns c = busy ? columns_of(tile) : Columns{};
+        uint32_t column[kNB];  // this lane's, for the second operand; those behind the last are any of the others: nobody looks at their sums
+#pragma unroll
+        for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
+            column[nb] = c.base + min(nb * 8u + g, c.n - 1u) * c.pitch + t * 16u;
+            sums[nb][0] = sums[nb][1] = sums[nb][2] = sums[nb][3] = 0.f;
+        }
+        uint32_t step = s.slice;
+        for (uint32_t first = 0; first < s.steps; first += s.window) {
+            const uint32_t end = min(s.steps, first + s.window);
+            if (!whole) {
+                __syncthreads();  // (nobody reads what was there any more)
+                stage(first, end - first);
+                __syncthreads();
+            }
+            for (; busy && step < end; step += s.slices) {
+                float scale[kEntries];
+                uint32_t minus[kEntries];
+                if constexpr (W::kCodes) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kEntries; ++i) {
+                        scale[i] = m.bf16_scales ? __uint_as_float(scale_next[i] << 16) : __half2float(__ushort_as_half((unsigned short)scale_next[i]));
+                        minus[i] = Widen<T>::minus((zero_next[i] & m.zero_mask) | m.zero_else);
+                    }
+                    fetch();
+                }
+                const uint32_t x_at = (step - first) * (W::kUnits * 16u);
+#pragma unroll
+                for (uint32_t b = 0; b < W::kBlocks; ++b) {
+                    constexpr uint32_t kRegs = W::kCodes ? W::kWords : 4u, kHalf = W::kBlocks / 2;  // blocks of a stage
+                    const uint32_t at = pair + b / kHalf * kStageBytes;
+                    if (b % kHalf == 0u) {
+                        ptx::cp_async_wait_group<kStages - 1>();
+                        if (kHalf > 1) __syncwarp();  // (else a lane reads what it copied itself)
+                    }
+                    uint32_t w_lo[kRegs], w_hi[kRegs];
+                    const uint32_t piece = kHalf == 1 ? t : kHalf == 2 ? 2u * (b % 2u) + (t >> 1) : b % 4u, rest = kHalf == 1 ? 0u : kHalf == 2 ? (t & 1u) * 8u : t * 4u;
+                    const uint32_t from = at + g * kHalfBytes + (piece ^ shared_swizzle(g)) * 16u + rest;
+                    ld_shared<4 * kRegs>(from, w_lo);
+                    ld_shared<4 * kRegs>(from + 8u * kHalfBytes, w_hi);
+                    if (b % kHalf == kHalf - 1u) {  // the stage is read: what comes kStages later may be copied there
+                        if (kHalf > 1) __syncwarp();
+                        issue(at, b / kHalf);
+                        if (kStages == 4 && b + 1 == W::kBlocks) pair = 2u * s.ring + 2u * kStageBytes - pair;  // (the other two)
+                    }
+                    if constexpr (!W::kCodes) {
+#pragma unroll
+                        for (int plane = 0; plane < kPlanes; ++plane)
+#pragma unroll
+                            for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
+                                const uint4 x = ptx::ld_shared_v4(column[nb] + x_at + b * 64u + plane * c.plane);
+                                fp4::mma_16x8x16<T>(sums[nb], w_lo[0], w_hi[0], w_lo[1], w_hi[1], x.x, x.y);
+                                fp4::mma_16x8x16<T>(sums[nb], w_lo[2], w_hi[2], w_lo[3], w_hi[3], x.z, x.w);
+                            }
+                    } else {
+                        const uint32_t source = (lane & ~3u) | (b & 1u) << 1;
+                        const float s_lo = __shfl_sync(0xFFFFFFFFu, scale[b >> 1], source), s_hi = __shfl_sync(0xFFFFFFFFu, scale[b >> 1], source | 1u);
+                        const Widen<T> widen_lo(__shfl_sync(0xFFFFFFFFu, minus[b >> 1], source)), widen_hi(__shfl_sync(0xFFFFFFFFu, minus[b >> 1], source | 1u));
+                        float part[kNB][4];
+#pragma unroll
+                        for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) part[nb][0] = part[nb][1] = part[nb][2] = part[nb][3] = 0.f;
+#pragma unroll
+                        for (uint32_t w = 0; w < W::kWords; ++w) {
+                            uint32_t a_lo[4], a_hi[4];
+                            widen_lo(w_lo[w], bits, a_lo);
+                            widen_hi(w_hi[w], bits, a_hi);
+#pragma unroll
+                            for (int plane = 0; plane < kPlanes; ++plane)
+#pragma unroll
+                                for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
+                                    const uint4 x = ptx::ld_shared_v4(column[nb] + x_at + (b * W::kWords + w) * 64u + plane * c.plane);
+                                    fp4::mma_16x8x16<T>(part[nb], a_lo[0], a_hi[0], a_lo[1], a_hi[1], x.x, x.y);
+                                    fp4::mma_16x8x16<T>(part[nb], a_lo[2], a_hi[2], a_lo[3], a_hi[3], x.z, x.w);
+                                }
+                        }
+#pragma unroll
+                        for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
+                            float x0 = 1.f, x1 = 1.f;
+                            if constexpr (kScaled) {
+                                const uint32_t group = min((step * W::kStep + b * (uint32_t)W::kSpan) >> c.shift, c.groups - 1u), j = nb * 8u + t * 2u;
+                                x0 = __uint_as_float(ptx::ld_shared_u32(c.scales + (min(j, c.n - 1u) * c.groups + group) * 4u));
+                                x1 = __uint_as_float(ptx::ld_shared_u32(c.scales + (min(j + 1u, c.n - 1u) * c.groups + group) * 4u));
+                            }
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e) sums[nb][e] = fmaf(kScaled ? part[nb][e] * (e & 1u ? x1 : x0) : part[nb][e], e < 2 ? s_lo : s_hi, sums[nb][e]);
+                        }
+                    }
+                }
+            }
+        }
+        if (s.slices == 1 && busy) done(tile, sums);
+    }
+    if (s.slices > 1) {  // (one round) the slices' sums meet in the first one's warp, in order
+        __syncwarp();
+        const bool busy = s.first < s.end;
+#pragma unroll
+        for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
+            if (busy && s.slice) ptx::st_shared_v4(s.ring + (nb * 32u + lane) * 16u, *reinterpret_cast<const uint4 *>(sums[nb]));
+        __syncthreads();
+        if (busy && s.slice == 0) {
+            for (uint32_t z = 1; z < s.slices; ++z)
+#pragma unroll
+                for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
+                    const uint4 v = ptx::ld_shared_v4(s.ring + z * (kStages * kStageBytes) + (nb * 32u + lane) * 16u);
+                    sums[nb][0] += __uint_as_float(v.x);
+                    sums[nb][1] += __uint_as_float(v.y);
+                    sums[nb][2] += __uint_as_float(v.z);
+                    sums[nb][3] += __uint_as_float(v.w);
+                }
+            done(s.first, sums);
+        }
+    }
+}
 
 // Sources of columns: eight values of k, from 8 u on, of column j as a unit.
 template <typename T>
@@ -336,16 +389,18 @@ struct Eights {  // e4m3, as fp16
     B200_DEVICE uint4 operator()(uint32_t j, uint32_t u) const {
         const uint8_t *p = x + (int64_t)j * across + (int64_t)u * 8;
         const uint32_t left = u * 8u < k ? k - u * 8u : 0u;
-        alignas(8) uint16_t v[4];
+        uint32_t v[2] = {0u, 0u};
         if (wide && left >= 8u) {
-            *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(p);
+            const uint2 both = *reinterpret_cast<const uint2 *>(p);
+            v[0] = both.x;
+            v[1] = both.y;
         } else {
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) v[e] = (uint16_t)((2 * e < left ? p[2 * e] : 0u) | (2 * e + 1 < left ? p[2 * e + 1] : 0u) << 8);
+            for (uint32_t e = 0; e < 8; ++e) v[e / 4] |= (e < left ? (uint32_t)p[e] : 0u) << e % 4 * 8;
         }
         uint32_t h[4];
 #pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h[e]) : "h"(v[e]));
+        for (uint32_t e = 0; e < 4; ++e) asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h[e]) : "h"((uint16_t)(v[e / 2] >> e % 2 * 16)));
         return make_uint4(h[0], h[1], h[2], h[3]);
     }
 };
@@ -353,12 +408,12 @@ struct Eights {  // e4m3, as fp16
 // `count` steps of n columns from step `first` on to shared memory, by all threads.  A warp takes 32 neighbouring units of a column, or, where neighbours lie across
 // the columns, up to 32 columns of a unit.
 template <class W, class Source>
-B200_DEVICE void stage_columns(const Source &from, const Columns &c, uint32_t first, uint32_t count, uint32_t n, bool across) {
+B200_DEVICE void stage_columns(const Source &from, uint32_t base, uint32_t pitch, uint32_t first, uint32_t count, uint32_t n, bool across) {
     const uint32_t units = count * W::kUnits, u0 = first * W::kUnits, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31u;
-    auto put = [&](uint32_t j, uint32_t u, uint4 v) { ptx::st_shared_v4(c.base + j * c.pitch + unit_place<W>(u) * 16u, unit_order<W>(v)); };
+    auto put = [&](uint32_t j, uint32_t u, uint4 v) { ptx::st_shared_v4(base + j * pitch + unit_place<W>(u), unit_order<W>(v)); };
     if (across) {
         for (uint32_t u = warp; u < units; u += warps)
-            if (lane < n) put(lane, u, from(lane, u0 + u));
+            for (uint32_t j = lane; j < n; j += 32u) put(j, u, from(j, u0 + u));
         return;
     }
     // pieces of 32 units, all columns of one after the other; four at a time

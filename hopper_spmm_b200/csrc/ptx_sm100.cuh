@@ -216,8 +216,9 @@ B200_DEVICE void st_shared_u16(uint32_t addr, uint16_t v) {
 B200_DEVICE void cp_async_16(uint32_t dst, const void *src, uint32_t src_bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
 }
-B200_DEVICE void cp_async_16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// The same, all 16 of them, where `on`.
+B200_DEVICE void cp_async_16_if(bool on, uint32_t dst, const void *src) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %2, 0;\n@q cp.async.cg.shared.global [%0], [%1], 16;\n}\n" ::"r"(dst), "l"(src), "r"((uint32_t)on) : "memory");
 }
 // Copies 4 bytes global -> shared (cached in L1: neighbouring words are fetched next).
 B200_DEVICE void cp_async_4(uint32_t dst, const void *src) {

@@ -1,4 +1,4 @@
-// The MMA of a warp on operands in registers: 16 rows x 8 columns x 16 values of k, sums in fp32.
+// The MMAs of a warp on operands in registers, sums in fp32.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -10,6 +10,7 @@
 namespace b200spmm {
 namespace fp4 {
 
+// 16 rows x 8 columns x 16 values of k in fp16 or bf16.
 template <typename T>
 B200_DEVICE void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
