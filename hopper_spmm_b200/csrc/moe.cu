@@ -29,7 +29,8 @@ constexpr uint32_t kLogitTokens = 4, kLogitThreads = 256;
 struct MoeParams {
     Matrix gate_up, down;
     uint32_t experts, hidden, inner, top, tokens, pairs;
-    uint32_t up_run, up_columns, down_run, down_columns;  // columns of a run, and that a block has room for, in either product
+    uint32_t run, up_columns, down_columns;  // columns of a run, and that a block has room for, in either product
+    uint4 *routing;  // as the first blocks found it
     bool renormalize;
     const void *x, *router;
     int64_t ldx, ld_router, ldy;
@@ -99,104 +100,125 @@ struct Routing {
     int32_t *ids;       // [pairs]
     uint16_t *pairs;    // [pairs] by expert, ascending
     uint16_t *starts;   // [experts + 1]: of an expert's pairs
+    uint16_t *ranks;    // [pairs] among its expert's
     uint32_t *runs;     // expert << 16 | first of its pairs
     uint32_t *n_runs;
 };
 // (an expert with n pairs has at most n runs)
-__host__ __device__ inline uint32_t routing_bytes(uint32_t pairs, uint32_t experts) { return (10u * pairs + 2u * experts + 2u + 16u + 15u + 127u) / 128u * 128u; }
+__host__ __device__ inline uint32_t routing_bytes(uint32_t pairs, uint32_t experts) { return (12u * pairs + 2u * experts + 2u + 16u + 127u) / 128u * 128u; }
 B200_DEVICE Routing routing_at(uint8_t *at, uint32_t pairs, uint32_t experts) {
     Routing r;
     r.n_runs = reinterpret_cast<uint32_t *>(at);
     r.ids = reinterpret_cast<int32_t *>(at + 16u);
     r.runs = reinterpret_cast<uint32_t *>(r.ids + pairs);
     r.pairs = reinterpret_cast<uint16_t *>(r.runs + pairs);
-    r.starts = r.pairs + pairs;
+    r.ranks = r.pairs + pairs;
+    r.starts = r.ranks + pairs;
     return r;
 }
 
-// One warp: the `top` largest logits of token t, in order; lane j's share of choice j.
-B200_DEVICE void choose(const MoeParams &p, uint32_t t, int32_t *ids, bool write) {
+B200_DEVICE double value_of(uint64_t key) { return __longlong_as_double((long long)(key >> 63 ? key ^ 1ull << 63 : ~key)); }
+
+// One warp: the `top` largest logits of token t, in order; lane j's share of choice j.  Up to 32 kKeys experts, whose keys a lane keeps (0: none, or taken).
+template <int kKeys>
+B200_DEVICE void choose_of(const MoeParams &p, uint32_t t, int32_t *ids, bool write) {
     const double *l = p.logits + (uint64_t)t * p.experts;
     const uint32_t lane = threadIdx.x & 31u;
-    uint64_t last = 0;
-    uint32_t last_at = 0, mine = 0;
+    uint64_t keys[kKeys], mine = 0, most = 0;
+    uint32_t mine_at = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < (uint32_t)kKeys; ++i) keys[i] = lane + 32u * i < p.experts ? key_of(l[lane + 32u * i]) : 0ull;
+    float sum = 0.f;
     for (uint32_t j = 0; j < p.top; ++j) {
         uint64_t best = 0;
-        uint32_t best_at = 0xFFFFFFFFu;
-        for (uint32_t e = lane; e < p.experts; e += 32u) {  // the first of the largest that come after the last choice
-            const uint64_t k = key_of(l[e]);
-            if ((j == 0 || k < last || (k == last && e > last_at)) && (best_at == 0xFFFFFFFFu || k > best)) {
-                best = k;
-                best_at = e;
+        uint32_t best_at = lane;
+#pragma unroll
+        for (uint32_t i = 0; i < (uint32_t)kKeys; ++i)
+            if (keys[i] > best) {
+                best = keys[i];
+                best_at = lane + 32u * i;
             }
+        const uint32_t high = __reduce_max_sync(0xFFFFFFFFu, (uint32_t)(best >> 32));
+        const uint32_t low = __reduce_max_sync(0xFFFFFFFFu, (uint32_t)(best >> 32) == high ? (uint32_t)best : 0u);
+        const uint64_t key = (uint64_t)high << 32 | low;
+        const uint32_t at = __reduce_min_sync(0xFFFFFFFFu, best == key ? best_at : 0xFFFFFFFFu);  // (of equal ones the first)
+        if (j == 0) {
+            most = key;
+            if (!p.renormalize)
+#pragma unroll
+                for (uint32_t i = 0; i < (uint32_t)kKeys; ++i)
+                    if (keys[i]) sum += expf((float)(value_of(keys[i]) - value_of(most)));
         }
-        const bool any = best_at != 0xFFFFFFFFu;
-        const uint32_t high = __reduce_max_sync(0xFFFFFFFFu, any ? (uint32_t)(best >> 32) : 0u);
-        const bool in = any && (uint32_t)(best >> 32) == high;
-        const uint32_t low = __reduce_max_sync(0xFFFFFFFFu, in ? (uint32_t)best : 0u);
-        last = (uint64_t)high << 32 | low;
-        last_at = __reduce_min_sync(0xFFFFFFFFu, in && (uint32_t)best == low ? best_at : 0xFFFFFFFFu);
-        if (lane == j) mine = last_at;
+#pragma unroll
+        for (uint32_t i = 0; i < (uint32_t)kKeys; ++i)
+            if (at == lane + 32u * i) keys[i] = 0;
+        if (lane == j) {
+            mine = key;
+            mine_at = at;
+        }
     }
-    const uint32_t first = __shfl_sync(0xFFFFFFFFu, mine, 0);
-    const double most = l[first];
     const bool chosen = lane < p.top;
-    const float e = chosen ? expf((float)(l[mine] - most)) : 0.f;
-    float sum = e;
-    if (!p.renormalize) {
-        sum = 0.f;
-        for (uint32_t i = lane; i < p.experts; i += 32u) sum += expf((float)(l[i] - most));
-    }
+    const float e = chosen ? expf((float)(value_of(mine) - value_of(most))) : 0.f;
+    if (p.renormalize) sum = e;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
     if (chosen) {
-        ids[t * p.top + lane] = (int32_t)mine;
+        ids[t * p.top + lane] = (int32_t)mine_at;
         if (write) {
-            p.ids[t * p.top + lane] = (int32_t)mine;
+            p.ids[t * p.top + lane] = (int32_t)mine_at;
             p.shares[t * p.top + lane] = e / sum;
         }
     }
 }
+B200_DEVICE void choose(const MoeParams &p, uint32_t t, int32_t *ids, bool write) {
+    if (p.experts <= 64u) choose_of<2>(p, t, ids, write);
+    else if (p.experts <= 256u) choose_of<8>(p, t, ids, write);
+    else choose_of<32>(p, t, ids, write);
+}
 
 // The runs, of up to `most` pairs, from the ids in shared memory, by all threads.
 B200_DEVICE void find_runs(const MoeParams &p, const Routing &r, uint32_t most) {
+    for (uint32_t e = threadIdx.x; e < p.experts; e += kThreads) r.starts[e] = 0;
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < p.experts; e += kThreads) {
-        uint32_t n = 0;
-        for (uint32_t i = 0; i < p.pairs; ++i) n += r.ids[i] == (int32_t)e ? 1u : 0u;
-        r.starts[e] = (uint16_t)n;
-    }
-    __syncthreads();
-    if (threadIdx.x < 32u) {  // the starts in place of the numbers, and the runs
+    if (threadIdx.x < 32u) {
+        const uint32_t lane = threadIdx.x;
+        // how many pairs of its expert come before each, 32 pairs at a time, and so how many each expert has
+        for (uint32_t i0 = 0; i0 < p.pairs; i0 += 32u) {
+            const int32_t id = i0 + lane < p.pairs ? r.ids[i0 + lane] : -1;
+            const uint32_t same = __match_any_sync(0xFFFFFFFFu, id), before = __popc(same & ((1u << lane) - 1u));
+            const uint32_t n = id >= 0 ? r.starts[id] : 0u;
+            __syncwarp();
+            if (id >= 0) {
+                r.ranks[i0 + lane] = (uint16_t)(n + before);
+                if (before == 0) r.starts[id] = (uint16_t)(n + __popc(same));
+            }
+            __syncwarp();
+        }
+        // the starts in place of the numbers, and the runs
         uint32_t pairs = 0, runs = 0;
         for (uint32_t e0 = 0; e0 < p.experts; e0 += 32u) {
-            const uint32_t e = e0 + threadIdx.x, n = e < p.experts ? r.starts[e] : 0u, m = (n + most - 1u) / most;
-            uint32_t n_to = n, m_to = m;  // up to this one
+            const uint32_t e = e0 + lane, n = e < p.experts ? r.starts[e] : 0u, m = (n + most - 1u) / most;
+            uint32_t both_to = n << 16 | m;  // up to this one (at most 8,192 of either)
 #pragma unroll
             for (uint32_t d = 1; d < 32u; d *= 2u) {
-                const uint32_t a = __shfl_up_sync(0xFFFFFFFFu, n_to, d), b = __shfl_up_sync(0xFFFFFFFFu, m_to, d);
-                if (threadIdx.x >= d) {
-                    n_to += a;
-                    m_to += b;
-                }
+                const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, both_to, d);
+                if (lane >= d) both_to += v;
             }
-            if (e < p.experts) r.starts[e] = (uint16_t)(pairs + n_to - n);
-            for (uint32_t i = 0; i < m; ++i) r.runs[runs + m_to - m + i] = e << 16 | (pairs + n_to - n + i * most);
-            pairs += __shfl_sync(0xFFFFFFFFu, n_to, 31);
-            runs += __shfl_sync(0xFFFFFFFFu, m_to, 31);
+            const uint32_t start = pairs + (both_to >> 16) - n, run = runs + (both_to & 0xFFFFu) - m;
+            if (e < p.experts) r.starts[e] = (uint16_t)start;
+            for (uint32_t i = 0; i < m; ++i) r.runs[run + i] = e << 16 | (start + i * most);
+            const uint32_t all = __shfl_sync(0xFFFFFFFFu, both_to, 31);
+            pairs += all >> 16;
+            runs += all & 0xFFFFu;
         }
-        if (threadIdx.x == 0) {
+        if (lane == 0) {
             r.starts[p.experts] = (uint16_t)pairs;
             *r.n_runs = runs;
         }
     }
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < p.experts; e += kThreads) {
-        uint32_t to = r.starts[e];
-        if (to == r.starts[e + 1u]) continue;
-        for (uint32_t i = 0; i < p.pairs; ++i)
-            if (r.ids[i] == (int32_t)e) r.pairs[to++] = (uint16_t)i;
-    }
+    for (uint32_t i = threadIdx.x; i < p.pairs; i += kThreads)
+        if (r.ids[i] >= 0) r.pairs[r.starts[r.ids[i]] + r.ranks[i]] = (uint16_t)i;
     __syncthreads();
 }
 B200_DEVICE uint32_t run_expert(const Routing &r, uint32_t run) { return r.runs[run] >> 16; }
@@ -283,7 +305,10 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const MoeParams p)
             if (write) p.ids[i] = id;
         }
     }
-    find_runs(p, r, p.up_run);
+    __syncthreads();
+    find_runs(p, r, p.run);
+    if (write)
+        for (uint32_t i = threadIdx.x; i < routing_bytes(p.pairs, p.experts) / 16u; i += kThreads) p.routing[i] = reinterpret_cast<const uint4 *>(smem + kWarps * kRingBytes<W>)[i];
     each_part(r, (p.inner + 7u) / 8u, p.up_columns, [&](uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n, uint32_t longest) {
         if (longest <= 8u) gate_up_part<W, 1>(p, r, smem, columns_at, begin, end, pair0, n);
         else gate_up_part<W, 2>(p, r, smem, columns_at, begin, end, pair0, n);
@@ -369,8 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const MoeParams p) {
     const Routing r = routing_at(smem + kWarps * kRingBytes<W>, p.pairs, p.experts);
     const uint32_t columns_at = kWarps * kRingBytes<W> + routing_bytes(p.pairs, p.experts);
     ptx::wait_for_grids_before();
-    for (uint32_t i = threadIdx.x; i < p.pairs; i += kThreads) r.ids[i] = p.ids[i];
-    find_runs(p, r, p.down_run);
+    for (uint32_t i = threadIdx.x; i < routing_bytes(p.pairs, p.experts) / 16u; i += kThreads) reinterpret_cast<uint4 *>(smem + kWarps * kRingBytes<W>)[i] = p.routing[i];
+    __syncthreads();
     each_part(r, (p.hidden + kTileRows - 1u) / kTileRows, p.down_columns, [&](uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n, uint32_t longest) {
         if (longest <= 8u) down_part<W, 1>(p, r, smem, columns_at, begin, end, pair0, n);
         else down_part<W, 2>(p, r, smem, columns_at, begin, end, pair0, n);
@@ -396,7 +421,7 @@ __global__ void __launch_bounds__(kSumThreads) sum_kernel(const MoeParams p) {
 
 // Where the parts of the workspace begin.
 struct Layout {
-    uint64_t logits, ids, shares, h, parts, bytes;
+    uint64_t logits, ids, shares, routing, h, parts, bytes;
     uint32_t h_ld;
 };
 Layout layout_of(const b200spmm_moe_t *m, uint64_t tokens) {
@@ -412,6 +437,7 @@ Layout layout_of(const b200spmm_moe_t *m, uint64_t tokens) {
     l.logits = take(tokens * m->experts * 8);
     l.ids = take(pairs * 4);
     l.shares = take(pairs * 4);
+    l.routing = take(routing_bytes((uint32_t)pairs, (uint32_t)m->experts));
     l.h = take(pairs * l.h_ld * 4);
     l.parts = take(pairs * m->hidden * 4);
     l.bytes = at;
@@ -449,55 +475,43 @@ Matrix plain_matrix(const void *values, int64_t ld, uint64_t cols) {
     return out;
 }
 
-// Columns that a block has room for, in `planes` parts, and of a run.
+// Columns that a block has room for, in `planes` parts.
 template <class W>
-bool room_for(const MoeParams &p, uint32_t k, uint32_t planes, uint32_t *columns, uint32_t *run) {
+uint32_t room_for(const MoeParams &p, uint32_t k, uint32_t planes) {
     const uint32_t taken = kWarps * kRingBytes<W> + routing_bytes(p.pairs, p.experts), steps = (k + W::kStep - 1) / W::kStep;
     const uint64_t each = (uint64_t)planes * ((uint64_t)steps * W::kUnits * 16u + 192u) + 4u;
-    *columns = (uint32_t)std::min<uint64_t>(p.pairs, (kMaxSmem - taken) / each);
-    *run = std::min(kRun, *columns);
-    return *columns > 0;
+    return (uint32_t)std::min<uint64_t>(p.pairs, (kMaxSmem - taken) / each);
 }
-template <class W>
-int launch_gate_up(MoeParams *p, uint32_t blocks, cudaStream_t stream) {
-    static std::atomic<uint64_t> allowed{0};
-    if (!room_for<W>(*p, p->hidden, 1, &p->up_columns, &p->up_run)) return B200SPMM_ERR_UNSUPPORTED;
-    B200_CUDA_TRY(allow_smem(gate_up_kernel<W>, allowed));
-    B200_CUDA_TRY(launch_after(gate_up_kernel<W>, dim3(blocks), kThreads, kMaxSmem, 1, stream, *p));
+template <class Up, class Down>
+int launch_products(MoeParams p, cudaStream_t stream) {
+    static std::atomic<uint64_t> up_allowed{0}, down_allowed{0};
+    p.up_columns = room_for<Up>(p, p.hidden, 1);
+    p.down_columns = room_for<Down>(p, p.inner, 2);
+    p.run = std::min({kRun, p.up_columns, p.down_columns});
+    if (p.run == 0) return B200SPMM_ERR_UNSUPPORTED;
+    // (there are as many runs as pairs, or fewer)
+    auto blocks = [&](uint32_t tiles) { return (uint32_t)std::min<uint64_t>(fp4::sm_count(), (uint64_t)p.pairs * tiles); };
+    B200_CUDA_TRY(allow_smem(gate_up_kernel<Up>, up_allowed));
+    B200_CUDA_TRY(allow_smem(down_kernel<Down>, down_allowed));
+    B200_CUDA_TRY(launch_after(gate_up_kernel<Up>, dim3(blocks((p.inner + 7) / 8)), kThreads, kMaxSmem, 1, stream, p));
+    B200_CUDA_TRY(launch_after(down_kernel<Down>, dim3(blocks((p.hidden + kTileRows - 1) / kTileRows)), kThreads, kMaxSmem, 1, stream, p));
+    B200_CUDA_TRY(launch_after(sum_kernel, dim3((p.hidden + kSumThreads - 1) / kSumThreads, p.tokens), kSumThreads, 0, 1, stream, p));
     return B200SPMM_OK;
 }
-template <class W>
-int launch_down(MoeParams *p, uint32_t blocks, cudaStream_t stream) {
-    static std::atomic<uint64_t> allowed{0};
-    if (!room_for<W>(*p, p->inner, 2, &p->down_columns, &p->down_run)) return B200SPMM_ERR_UNSUPPORTED;
-    B200_CUDA_TRY(allow_smem(down_kernel<W>, allowed));
-    B200_CUDA_TRY(launch_after(down_kernel<W>, dim3(blocks), kThreads, kMaxSmem, 1, stream, *p));
-    return B200SPMM_OK;
+template <class Up>
+int launch_down_for(const MoeParams &p, uint32_t span, cudaStream_t stream) {
+    using B = __nv_bfloat16;  // for its range: inner values are as large as they are, and codes are exact in either type
+    return span == 32 ? launch_products<Up, Weights<B, 32>>(p, stream) : span == 64 ? launch_products<Up, Weights<B, 64>>(p, stream) : launch_products<Up, Weights<B, 128>>(p, stream);
 }
 
 template <typename T>
-int launch_moe(const b200spmm_moe_t *m, MoeParams p, double *logits, cudaStream_t stream) {
+int launch_moe(const b200spmm_moe_t *m, const MoeParams &p, double *logits, cudaStream_t stream) {
     if (logits) {
         B200_CUDA_TRY(launch_after(logits_kernel<T>, dim3(p.experts, (p.tokens + kLogitTokens - 1) / kLogitTokens), kLogitThreads, 0, 1, stream, p, logits));
     }
-    const uint64_t most = p.pairs;  // runs that there may be
-    auto blocks = [&](uint32_t tiles) { return (uint32_t)std::min<uint64_t>(fp4::sm_count(), most * tiles); };
-    const uint32_t up = blocks((p.inner + 7) / 8), down = blocks((p.hidden + kTileRows - 1) / kTileRows);
-    int st;
-    if (m->gate_up) {
-        const uint32_t a = span_of(m->gate_up), b = span_of(m->down);
-        st = a == 32 ? launch_gate_up<Weights<T, 32>>(&p, up, stream) : a == 64 ? launch_gate_up<Weights<T, 64>>(&p, up, stream) : launch_gate_up<Weights<T, 128>>(&p, up, stream);
-        if (st != B200SPMM_OK) return st;
-        // bf16 for its range: inner values are as large as they are, and codes are exact in either type
-        using B = __nv_bfloat16;
-        st = b == 32 ? launch_down<Weights<B, 32>>(&p, down, stream) : b == 64 ? launch_down<Weights<B, 64>>(&p, down, stream) : launch_down<Weights<B, 128>>(&p, down, stream);
-    } else {
-        st = launch_gate_up<Weights<T, 0>>(&p, up, stream);
-        if (st == B200SPMM_OK) st = launch_down<Weights<T, 0>>(&p, down, stream);
-    }
-    if (st != B200SPMM_OK) return st;
-    B200_CUDA_TRY(launch_after(sum_kernel, dim3((p.hidden + kSumThreads - 1) / kSumThreads, p.tokens), kSumThreads, 0, 1, stream, p));
-    return B200SPMM_OK;
+    if (!m->gate_up) return launch_products<Weights<T, 0>, Weights<T, 0>>(p, stream);
+    const uint32_t a = span_of(m->gate_up), b = span_of(m->down);
+    return a == 32 ? launch_down_for<Weights<T, 32>>(p, b, stream) : a == 64 ? launch_down_for<Weights<T, 64>>(p, b, stream) : launch_down_for<Weights<T, 128>>(p, b, stream);
 }
 
 // ids null: they are found from the logits, and left, with the shares, at out_ids and out_shares where those are wanted.
@@ -530,6 +544,7 @@ int run_moe(const b200spmm_moe_t *m, const void *x, int64_t ldx, int64_t tokens,
     p.id_bytes = id_bytes;
     p.ids = out_ids ? out_ids : reinterpret_cast<int32_t *>(ws + l.ids);
     p.shares = shares ? const_cast<float *>(shares) : out_shares ? out_shares : reinterpret_cast<float *>(ws + l.shares);  // (given ones are only read)
+    p.routing = reinterpret_cast<uint4 *>(ws + l.routing);
     p.h = reinterpret_cast<float *>(ws + l.h);
     p.h_ld = l.h_ld;
     p.parts = reinterpret_cast<float *>(ws + l.parts);
