@@ -28,7 +28,7 @@ struct Int4Params {
 };
 
 template <int kNB>
-constexpr uint32_t kMaxWarps = kNB <= 1 ? 28 : kNB <= 2 ? 24 : 16;
+constexpr uint32_t kMaxWarps = kNB <= 1 ? 28 : kNB <= 2 ? 24 : kNB <= 3 ? 20 : 16;
 
 // A lane's sums to C.
 template <typename T, int kNB>
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps<kNB>, 1) int4_kernel(const Int4
     using W = Weights<T, kSpan>;
     extern __shared__ __align__(128) uint8_t smem[];
     const uint32_t base = ptx::smem_u32(smem), warp = warp_index(), g = (threadIdx.x & 31u) >> 2;
-    constexpr uint32_t ring_bytes = kRing * kStageBytes;
+    constexpr uint32_t ring_bytes = kRingOf<W, kNB, kRing>;
     const uint32_t j0 = blockIdx.y * (8u * kNB);
     Columns c;
     c.base = base + p.warps * ring_bytes;
@@ -95,7 +95,7 @@ int launch(Int4Params p, cudaStream_t stream) {
     const Split split((p.tiles + blocks - 1) / blocks, p.steps, kMaxWarps<kNB>);
     p.warps = split.at_once * split.slices;
     // the columns as a whole, or as much of them as there is room for
-    const uint64_t taken = (uint64_t)p.warps * kRing * kStageBytes + (kScaled ? (uint64_t)p.cols * p.x_groups * 4u : 0u);
+    const uint64_t taken = (uint64_t)p.warps * kRingOf<W, kNB, kRing> + (kScaled ? (uint64_t)p.cols * p.x_groups * 4u : 0u);
     p.window = steps_that_fit<W>(p.steps, p.cols, 1, taken);
     if (kRing == 4 && p.window < p.steps) return launch<T, kSpan, kNB, kScaled, 2>(p, stream);  // (half the ring, more room)
     if (p.window == 0) return B200SPMM_ERR_UNSUPPORTED;
@@ -108,9 +108,13 @@ int launch(Int4Params p, cudaStream_t stream) {
 
 template <typename T, int kSpan, bool kScaled>
 int launch_width(const Int4Params &p, cudaStream_t stream) {
-    if (p.n <= 8) return launch<T, kSpan, 1, kScaled, 4>(p, stream);
-    if (p.n <= 16) return launch<T, kSpan, 2, kScaled, 4>(p, stream);
-    return launch<T, kSpan, 4, kScaled, 4>(p, stream);
+    // as few reads of the matrix as go with 40 columns at once, and as many columns in each
+    const uint32_t passes = (p.n + 39) / 40, eights = ((p.n + passes - 1) / passes + 7) / 8;
+    if (eights <= 1) return launch<T, kSpan, 1, kScaled, 4>(p, stream);
+    if (eights == 2) return launch<T, kSpan, 2, kScaled, 4>(p, stream);
+    if (eights == 3) return launch<T, kSpan, 3, kScaled, 4>(p, stream);
+    if (eights == 4) return launch<T, kSpan, 4, kScaled, 4>(p, stream);
+    return launch<T, kSpan, 5, kScaled, 4>(p, stream);
 }
 template <typename T, bool kScaled>
 int launch_span(const Int4Params &p, uint32_t span, cudaStream_t stream) {

@@ -20,9 +20,9 @@ namespace {
 constexpr uint32_t kWarps = 24, kThreads = 32 * kWarps;
 constexpr uint32_t kRun = 16;  // columns that a tile meets at once, at most
 template <class W>
-constexpr int kRing = 4;  // stages of a warp
+constexpr int kRing = 2 * W::kPieces;  // stages of a warp: two steps
 template <class W>
-constexpr uint32_t kRingBytes = kRing<W> * kStageBytes;
+constexpr uint32_t kRingBytes = kRingOf<W, 2, kRing<W>>;
 constexpr uint32_t kMaxTokens = 256, kMaxExperts = 1024, kMaxTop = 32;
 constexpr uint32_t kLogitTokens = 4, kLogitThreads = 256;
 

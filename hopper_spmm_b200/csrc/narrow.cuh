@@ -1,7 +1,7 @@
 // A few columns times rows of a weight matrix that is read once: what a block of threads does.
 //
 // Bound: one read of the matrix.  Each warp copies its own rows to a ring of its own in shared memory (cp.async, 16 bytes a lane), so no warp waits for
-// another while k goes by, and a wait is one for the warp's own copies.  A warp has a tile of 16 rows at a time, or every `slices`-th step of 128 bytes of
+// another while k goes by, and a wait is one for the warp's own copies.  A warp has a tile of 16 rows at a time, or every `slices`-th step of
 // those rows; its copies run ahead into its next tile.  The columns lie in shared memory for all warps, as a whole where there is room, else piece by piece.  16 rows x 8
 // columns meet in mma.sync: at this width a product is a small part of the work, and for tcgen05 widened weights would have to go through shared or tensor memory.
 //
@@ -9,7 +9,6 @@
 // agree, so a lane takes neighbours of its rows: of 4-bit integers kSpan / 4 of every kSpan, the widest span that has one scale (and one of the columns'
 // scales), whose sum is multiplied by them in fp32; of 16-bit values 8 of every 32.  Columns are stored in units of 8 values of k, in the order in which lanes
 // t = 0..3 read them side by side, each unit as the pairs that a mask takes out of a word of eight codes: 0 4, 1 5, 2 6, 3 7.
-// A step's first and second 64 bytes of a row are copied and waited for by themselves, so that less of the ring is idle.
 //
 // What it spends its time on is instructions, not bytes: the same copies with nothing else take 19.7 us for 28672 x 8192 codes, 120 MB.
 #pragma once
@@ -23,7 +22,7 @@
 namespace b200spmm {
 namespace narrow {
 
-constexpr uint32_t kTileRows = 16, kStepBytes = 128, kHalfBytes = kStepBytes / 2, kStageBytes = kTileRows * kHalfBytes;  // (a stage is half a step)
+constexpr uint32_t kTileRows = 16, kStepBytes = 128;  // of a row, in a step
 constexpr uint32_t kMaxSmem = 227 * 1024;
 constexpr uint32_t kWholeGroup = 31;  // a shift that leaves one group, however long a row is
 
@@ -40,16 +39,20 @@ struct Matrix {
     bool bf16_scales;
 };
 
-// T: the type of the MMA's operands.  kSpan: columns of 4-bit integers that share their scales, 32, 64 or 128; 0: the weights are T themselves.
+// T: the type of the MMA's operands.  kSpan: columns of 4-bit integers that share their scales, 32, 64 or 128; 0: the weights are T themselves.  kPiece: bytes of a row in a
+// stage of the ring: 128 neighbouring bytes go to shared memory in one access where 64 and 64 take two; with 64 a lane of codes in spans of 128 reads what it copied itself and
+// the ring comes free sooner.  (Experts in 16 bits, one token 37.4 us with 64, 36.7 with 128; in 4 bits, 8 tokens 149 and 155.)
 template <typename T_, int kSpan_>
 struct Weights {
     using T = T_;
     static constexpr int kSpan = kSpan_;
     static constexpr bool kCodes = kSpan > 0;
+    static constexpr uint32_t kPiece = kCodes ? 64 : 128, kPieces = kStepBytes / kPiece, kStageBytes = kTileRows * kPiece;
     static constexpr uint32_t kStep = kCodes ? 2 * kStepBytes : kStepBytes / 2;  // values of k
     static constexpr uint32_t kUnits = kStep / 8;                                // of a column, in a step
     static constexpr uint32_t kBlocks = kCodes ? kStep / (kCodes ? kSpan : 1) : 2;  // of a step, with a scale each; halves
-    static constexpr uint32_t kWords = kCodes ? 8 / kBlocks : 1;                 // of a lane in a block: units of 8 values
+    static constexpr uint32_t kOfStage = kBlocks / kPieces;                      // blocks of a stage
+    static constexpr uint32_t kWords = kCodes ? kSpan / 32 : 1;                  // of a lane in a block: units of 8 values
     static constexpr uint32_t kEntries = kCodes ? kBlocks / 2 : 1;               // scales that a lane fetches for its warp
 };
 
@@ -73,7 +76,12 @@ B200_DEVICE uint4 unit_order(uint4 v) {
         return v;
 }
 
-B200_DEVICE uint32_t shared_swizzle(uint32_t row) { return (row & 2u) | (row >> 2 & 1u); }  // of a stage's four pieces of a row: no two lanes of a load meet in a bank
+// Where piece `p` of 16 bytes of row r lies in a stage: no two lanes of a load meet in a bank.
+template <class W>
+B200_DEVICE uint32_t stage_place(uint32_t r, uint32_t p) {
+    const uint32_t swap = W::kPiece == 128 ? (r & 1u) << 2 | (r & 2u) | (r >> 2 & 1u) : (r & 2u) | (r >> 2 & 1u);
+    return r * W::kPiece + (p ^ swap) * 16u;
+}
 
 // (w & mask) | bits in one instruction: with both as constants the compiler makes two of it (28672 x 8192 times one column: 38 us for 33).
 template <uint32_t kMask>
@@ -131,6 +139,13 @@ struct Columns {
     uint32_t scales, groups, shift;
 };
 
+// A unit of a lane's column, by lanes that have one; the others' registers hold what they held, and so do the sums of columns that nobody looks at.  (A load
+// takes four accesses with all lanes, one with those of a single column.  Registers that are written under a condition live on: the same few are used again.)
+B200_DEVICE void column_unit(bool has, uint32_t addr, uint4 &v) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %5, 0;\n@q ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n}\n"
+                 : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w) : "r"(addr), "r"((uint32_t)has) : "memory");
+}
+
 template <int kBytes>
 B200_DEVICE void ld_shared(uint32_t addr, uint32_t *v) {
     if constexpr (kBytes == 16) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
@@ -154,6 +169,10 @@ struct Split {
 // The warp's number, by an operation whose result the compiler knows to be one for all lanes: what follows from it takes no lane's registers.
 B200_DEVICE uint32_t warp_index() { return __reduce_max_sync(0xFFFFFFFFu, threadIdx.x >> 5); }
 
+// Bytes of a warp's ring, where its sums go in the end.
+template <class W, int kNB, int kStages>
+constexpr uint32_t kRingOf = kStages * W::kStageBytes > kNB * 512u ? kStages * W::kStageBytes : kNB * 512u;
+
 // What a warp does: tiles first, first + at_once ... below `end` (none, where it is beyond `at_once` or `end`), of each the steps slice, slice + slices ...
 struct Share {
     uint32_t first, end;
@@ -173,29 +192,43 @@ struct Share {
 template <class W, int kNB, int kPlanes, bool kScaled, int kStages, class RowsOf, class ColumnsOf, class Stage, class Done>
 B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, ColumnsOf &&columns_of, Stage &&stage, Done &&done) {
     using T = typename W::T;
-    static_assert(kStages == 2 || kStages == 4, "a ring of one step or two");
+    static_assert(kStages == W::kPieces || kStages == 2 * W::kPieces, "a ring of one step or two");
     const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
-    // Copies run kStages stages ahead: piece t of rows g and g + 8.
-    const uint32_t own = g * kHalfBytes + (t ^ shared_swizzle(g)) * 16u, last_copy = s.steps * kStepBytes;
-    uint32_t copy_tile = s.first, copied = 0;  // the next copy's tile, and bytes of a row up to it
+    // Copies run kStages stages ahead.  A lane copies 16 bytes of rows r, r + 8 and, with 128 bytes of a row, r + 4, r + 12.
+    constexpr uint32_t kLanes = W::kPiece / 16;  // of a row
+    const uint32_t copy_row = lane / kLanes, copy_piece = lane % kLanes, own = stage_place<W>(copy_row, copy_piece), last_copy = s.steps * kStepBytes;
+    uint32_t copy_tile = s.first, copied = 0, lo_4 = 0, hi_4 = 0;  // the next copy's tile, and bytes of a row up to it; from a row to the fourth after it
     const uint8_t *lo = nullptr, *hi = nullptr;
     auto copy_from = [&]() {
-        copied = s.slice * kStepBytes + t * 16u;
-        lo = m.values + rows_of(copy_tile, g) * m.pitch + copied;
-        hi = m.values + rows_of(copy_tile, g + 8u) * m.pitch + copied;
+        copied = s.slice * kStepBytes + copy_piece * 16u;
+        const uint64_t row_lo = rows_of(copy_tile, copy_row), row_hi = rows_of(copy_tile, copy_row + 8u);
+        lo = m.values + row_lo * m.pitch + copied;
+        hi = m.values + row_hi * m.pitch + copied;
+        if (W::kPiece == 128) {
+            lo_4 = (uint32_t)((rows_of(copy_tile, copy_row + 4u) - row_lo) * m.pitch);
+            hi_4 = (uint32_t)((rows_of(copy_tile, copy_row + 12u) - row_hi) * m.pitch);
+        }
     };
-    auto issue = [&](uint32_t at, uint32_t half) {  // `half` of the next step
-        const uint32_t place = copied + half * kHalfBytes;
+    auto issue = [&](uint32_t at, uint32_t piece) {  // of the next step
+        const uint32_t place = copied + piece * W::kPiece;
         if constexpr (W::kCodes) {
             const bool there = copy_tile < s.end && place < m.row_bytes;  // (codes behind a row's end meet zeros, whatever they are)
-            ptx::cp_async_16_if(there, at + own, lo + half * kHalfBytes);
-            ptx::cp_async_16_if(there, at + own + 8u * kHalfBytes, hi + half * kHalfBytes);
+            ptx::cp_async_16_if(there, at + own, lo + piece * W::kPiece);
+            ptx::cp_async_16_if(there, at + own + 8u * W::kPiece, hi + piece * W::kPiece);
+            if (W::kPiece == 128) {  // (the place of a row's piece is another four rows further on: their lowest bit of three)
+                ptx::cp_async_16_if(there, at + (own ^ 16u) + 4u * W::kPiece, lo + lo_4);
+                ptx::cp_async_16_if(there, at + (own ^ 16u) + 12u * W::kPiece, hi + hi_4);
+            }
         } else if (copy_tile < s.end) {  // zeros behind a row's end
-            const uint32_t left = place < m.row_bytes ? min(16u, m.row_bytes - place) : 0u, back = left ? half * kHalfBytes : 0u - copied;
+            const uint32_t left = place < m.row_bytes ? min(16u, m.row_bytes - place) : 0u, back = left ? piece * W::kPiece : 0u - copied;
             ptx::cp_async_16(at + own, lo + (int32_t)back, left);
-            ptx::cp_async_16(at + own + 8u * kHalfBytes, hi + (int32_t)back, left);
+            ptx::cp_async_16(at + own + 8u * W::kPiece, hi + (int32_t)back, left);
+            if (W::kPiece == 128) {
+                ptx::cp_async_16(at + (own ^ 16u) + 4u * W::kPiece, lo + lo_4 + (int32_t)back, left);
+                ptx::cp_async_16(at + (own ^ 16u) + 12u * W::kPiece, hi + hi_4 + (int32_t)back, left);
+            }
         }
-        if (half == 1u) {
+        if (piece + 1u == W::kPieces) {
             const uint32_t ahead = s.slices * kStepBytes;
             copied += ahead;
             lo += ahead;
@@ -234,7 +267,7 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, Col
     if (s.first < s.end) {
         copy_from();
 #pragma unroll
-        for (uint32_t i = 0; i < kStages; ++i) issue(s.ring + i * kStageBytes, i % 2u);
+        for (uint32_t i = 0; i < kStages; ++i) issue(s.ring + i * W::kStageBytes, i % W::kPieces);
         if constexpr (W::kCodes) {
             entries_from();
             fetch();
@@ -246,15 +279,18 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, Col
         __syncthreads();
     }
     const uint32_t bits = W::kCodes ? in_register(Widen<T>::kBits) : 0u;
-    uint32_t pair = s.ring, tile = s.first;  // a step's two stages
+    uint32_t here = s.ring, tile = s.first;  // a step's stages
+    uint4 xs[2] = {};
     float sums[kNB][4];
     for (uint32_t round = 0; round < s.rounds; ++round, tile += s.at_once) {
         const bool busy = tile < s.end;
         const Columns c = busy ? columns_of(tile) : Columns{};
-        uint32_t column[kNB];  // this lane's, for the second operand; those behind the last are any of the others: nobody looks at their sums
+        uint32_t column[kNB];  // this lane's, for the second operand, where it has one
+        bool has[kNB];
 #pragma unroll
         for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
-            column[nb] = c.base + min(nb * 8u + g, c.n - 1u) * c.pitch + t * 16u;
+            has[nb] = nb * 8u + g < c.n;
+            column[nb] = c.base + (nb * 8u + g) * c.pitch + t * 16u;
             sums[nb][0] = sums[nb][1] = sums[nb][2] = sums[nb][3] = 0.f;
         }
         uint32_t step = s.slice;
@@ -279,28 +315,30 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, Col
                 const uint32_t x_at = (step - first) * (W::kUnits * 16u);
 #pragma unroll
                 for (uint32_t b = 0; b < W::kBlocks; ++b) {
-                    constexpr uint32_t kRegs = W::kCodes ? W::kWords : 4u, kHalf = W::kBlocks / 2;  // blocks of a stage
-                    const uint32_t at = pair + b / kHalf * kStageBytes;
-                    if (b % kHalf == 0u) {
+                    constexpr uint32_t kRegs = W::kCodes ? W::kWords : 4u;
+                    const uint32_t at = here + b / W::kOfStage * W::kStageBytes, in = b % W::kOfStage;
+                    constexpr bool kOwn = W::kPiece == 64 && W::kOfStage == 1;  // a lane reads what it copied itself
+                    if (in == 0u) {
                         ptx::cp_async_wait_group<kStages - 1>();
-                        if (kHalf > 1) __syncwarp();  // (else a lane reads what it copied itself)
+                        if (!kOwn) __syncwarp();
                     }
                     uint32_t w_lo[kRegs], w_hi[kRegs];
-                    const uint32_t piece = kHalf == 1 ? t : kHalf == 2 ? 2u * (b % 2u) + (t >> 1) : b % 4u, rest = kHalf == 1 ? 0u : kHalf == 2 ? (t & 1u) * 8u : t * 4u;
-                    const uint32_t from = at + g * kHalfBytes + (piece ^ shared_swizzle(g)) * 16u + rest;
+                    const uint32_t piece = !W::kCodes || W::kSpan == 128 ? 4u * in + t : W::kSpan == 64 ? 2u * in + (t >> 1) : in;
+                    const uint32_t from = at + stage_place<W>(g, piece) + (!W::kCodes || W::kSpan == 128 ? 0u : W::kSpan == 64 ? (t & 1u) * 8u : t * 4u);
                     ld_shared<4 * kRegs>(from, w_lo);
-                    ld_shared<4 * kRegs>(from + 8u * kHalfBytes, w_hi);
-                    if (b % kHalf == kHalf - 1u) {  // the stage is read: what comes kStages later may be copied there
-                        if (kHalf > 1) __syncwarp();
-                        issue(at, b / kHalf);
-                        if (kStages == 4 && b + 1 == W::kBlocks) pair = 2u * s.ring + 2u * kStageBytes - pair;  // (the other two)
+                    ld_shared<4 * kRegs>(from + 8u * W::kPiece, w_hi);
+                    if (in + 1u == W::kOfStage) {  // the stage is read: what comes kStages later may be copied there
+                        if (!kOwn) __syncwarp();
+                        issue(at, b / W::kOfStage);
+                        if (kStages != W::kPieces && b + 1 == W::kBlocks) here = 2u * s.ring + W::kPieces * W::kStageBytes - here;  // (the other step's)
                     }
                     if constexpr (!W::kCodes) {
 #pragma unroll
                         for (int plane = 0; plane < kPlanes; ++plane)
 #pragma unroll
                             for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
-                                const uint4 x = ptx::ld_shared_v4(column[nb] + x_at + b * 64u + plane * c.plane);
+                                uint4 &x = xs[(b + nb + plane) % 2u];
+                                column_unit(has[nb], column[nb] + x_at + b * 64u + plane * c.plane, x);
                                 fp4::mma_16x8x16<T>(sums[nb], w_lo[0], w_hi[0], w_lo[1], w_hi[1], x.x, x.y);
                                 fp4::mma_16x8x16<T>(sums[nb], w_lo[2], w_hi[2], w_lo[3], w_hi[3], x.z, x.w);
                             }
@@ -320,7 +358,8 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, Col
                             for (int plane = 0; plane < kPlanes; ++plane)
 #pragma unroll
                                 for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
-                                    const uint4 x = ptx::ld_shared_v4(column[nb] + x_at + (b * W::kWords + w) * 64u + plane * c.plane);
+                                    uint4 &x = xs[(w + nb + plane) % 2u];
+                                    column_unit(has[nb], column[nb] + x_at + (b * W::kWords + w) * 64u + plane * c.plane, x);
                                     fp4::mma_16x8x16<T>(part[nb], a_lo[0], a_hi[0], a_lo[1], a_hi[1], x.x, x.y);
                                     fp4::mma_16x8x16<T>(part[nb], a_lo[2], a_hi[2], a_lo[3], a_hi[3], x.z, x.w);
                                 }
@@ -353,7 +392,7 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, Col
             for (uint32_t z = 1; z < s.slices; ++z)
 #pragma unroll
                 for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
-                    const uint4 v = ptx::ld_shared_v4(s.ring + z * (kStages * kStageBytes) + (nb * 32u + lane) * 16u);
+                    const uint4 v = ptx::ld_shared_v4(s.ring + z * kRingOf<W, kNB, kStages> + (nb * 32u + lane) * 16u);
                     sums[nb][0] += __uint_as_float(v.x);
                     sums[nb][1] += __uint_as_float(v.y);
                     sums[nb][2] += __uint_as_float(v.z);
@@ -416,12 +455,11 @@ B200_DEVICE void stage_columns(const Source &from, uint32_t base, uint32_t pitch
             for (uint32_t j = lane; j < n; j += 32u) put(j, u, from(j, u0 + u));
         return;
     }
-    // pieces of 32 units, all columns of one after the other; four at a time
+    // pieces of 32 units, all columns of one after the other, four at a time
     constexpr uint32_t kBatch = 4;
-    uint32_t j = 0, u = warp * 32u + lane;
-    while (true) {
-        uint4 v[kBatch];
-        uint32_t js[kBatch], us[kBatch];
+    uint32_t j = 0, u = warp * 32u + lane, js[kBatch], us[kBatch];
+    uint4 v[kBatch];
+    auto ask = [&]() {
 #pragma unroll
         for (uint32_t b = 0; b < kBatch; ++b) {
             while (u >= units && j < n) {
@@ -433,10 +471,14 @@ B200_DEVICE void stage_columns(const Source &from, uint32_t base, uint32_t pitch
             if (j < n) v[b] = from(j, u0 + u);
             u += warps * 32u;
         }
+    };
+    ask();
+    while (true) {
 #pragma unroll
         for (uint32_t b = 0; b < kBatch; ++b)
             if (js[b] < n) put(js[b], us[b], v[b]);
         if (js[kBatch - 1] >= n) return;
+        ask();
     }
 }
 
