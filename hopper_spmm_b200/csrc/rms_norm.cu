@@ -19,6 +19,7 @@ namespace {
 constexpr float kTop = 448.f;  // the largest number of e4m3
 constexpr uint32_t kPer = 8;   // values of a row that a thread has at a time, so that a warp has 256 neighbours
 constexpr uint32_t kSpan = 32 * kPer;
+constexpr uint32_t kTiny = 0x0D800000u;  // the bits of 2^-100
 
 struct NormParams {
     const void *x, *r, *w;
@@ -28,9 +29,13 @@ struct NormParams {
     uint64_t rows;
     uint32_t cols, groups;
     int w_type, out_type;
-    uint32_t group;  // columns that share a scale; 0: the row does
+    uint32_t group, group_shift;  // columns that share a scale, a power of two; 0: the row does
     float eps;
 };
+
+// What a kernel is made for: any weight and result, or a weight of X's type and e4m3 with a scale of the row, of groups, or a result of X's type.  (Asked while it runs, that
+// takes 26 branches for 8 values.)
+enum : int { kAny, kRow, kGroups, kSame };
 
 template <int kBytes> struct Access;
 template <> struct Access<1> { using Type = uint8_t; };
@@ -75,8 +80,9 @@ B200_DEVICE void times_weight_as(const void *w, uint32_t cols, uint32_t col, flo
 #pragma unroll
     for (uint32_t i = 0; i < kPer; ++i) v[i] *= raw[i / kE][i % kE];
 }
-template <int kE>
+template <typename X, int kE, int kKind>
 B200_DEVICE void times_weight(const NormParams &p, uint32_t col, float (&v)[kPer]) {
+    if constexpr (kKind != kAny) return times_weight_as<X, kE>(p.w, p.cols, col, v);
     if (!p.w) return;
     if (p.w_type == B200SPMM_T_F32) times_weight_as<float, kE>(p.w, p.cols, col, v);
     else if (p.w_type == B200SPMM_T_F16) times_weight_as<__half, kE>(p.w, p.cols, col, v);
@@ -112,7 +118,7 @@ B200_DEVICE uint32_t bits_of(float v) { return __float_as_uint(v) & 0x7FFFFFFFu;
 
 // R: the residual's type, void for none.  kV: times eight values of a row that a thread keeps; 0: none, the row is read again.  kE: neighbours that are read
 // and written at once, on whose size all rows start and end; lane l's are kE from kE l on in each 32 kE columns.
-template <typename X, typename R, int kV, int kE>
+template <typename X, typename R, int kV, int kE, int kKind>
 __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
     constexpr bool kKeep = kV > 0, kAdds = !std::is_void<R>::value;
     constexpr int kKept = kKeep ? kV : 1;
@@ -161,7 +167,7 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
         }
     };
     if constexpr (kKeep) load(first, h);
-    const bool eights = p.out_type == B200SPMM_T_E4M3, of_row = eights && p.group == 0;
+    const bool eights = kKind == kAny ? p.out_type == B200SPMM_T_E4M3 : kKind != kSame, of_row = kKind == kAny ? eights && p.group == 0 : kKind == kRow;
     auto sums = [&]() {
         Both b{0.f, 0u};
         each([&](uint32_t col, float (&v)[kPer]) {
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
                 float y[kPer];
 #pragma unroll
                 for (uint32_t e = 0; e < kPer; ++e) y[e] = v[e];
-                times_weight<kE>(p, col, y);
+                times_weight<X, kE, kKind>(p, col, y);
 #pragma unroll
                 for (uint32_t e = 0; e < kPer; ++e) b.top = max(b.top, bits_of(y[e]));
             }
@@ -211,18 +217,17 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
         }
     }
     // Values are quotients of h w and its largest: the norm cancels, and fewer roundings stand between a value and its type's border.
-    auto scale_of = [&](uint32_t top) {  // from the largest |h w|, as bits; NaN where its y is infinite or NaN
+    // A scale, and what brings |h w| to values; from the largest |h w|, as bits.  Below 2^-100 the latter is for |h w| times 2^100, and 0 where the values are to be zeros.
+    auto scales_of = [&](uint32_t top, float *scale, float *inverse) {
         const float y = __uint_as_float(top) * factor;
-        return y < __uint_as_float(kInfBits) ? y / kTop : __uint_as_float(0x7FFFFFFFu);
+        *scale = y < __uint_as_float(kInfBits) ? y * (1.f / kTop) : __uint_as_float(0x7FFFFFFFu);
+        *inverse = *scale > 0.f ? __frcp_rn(__uint_as_float(top) * (top < kTiny ? 0x1p100f : 1.f) * (1.f / kTop)) : 0.f;
     };
-    // 448 over the largest; 0 where the values are to be zeros.  Below 2^-100, where it would leave fp32's range, for values times 2^100.
-    auto is_tiny = [](uint32_t top) { return top < 0x0D800000u; };
-    auto inverse_of = [&](uint32_t top, float scale) { return scale > 0.f ? kTop / (__uint_as_float(top) * (is_tiny(top) ? 0x1p100f : 1.f)) : 0.f; };
     float inverse = 0.f;
     if (of_row) {
-        const float scale = scale_of(all.top);
+        float scale;
+        scales_of(all.top, &scale, &inverse);
         if (threadIdx.x == 0) p.scales[row] = scale;
-        inverse = inverse_of(all.top, scale);
     }
     const uint32_t lanes = min(32u, p.group / kE), together = max(1u, p.group / (32u * kE));  // of a group: lanes, and times 32 kE columns of a thread
     each([&](uint32_t col, float (&v)[kPer]) {
@@ -233,7 +238,7 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
                 keep_sum(col, whole[0]);
             }
         }
-        times_weight<kE>(p, col, v);
+        times_weight<X, kE, kKind>(p, col, v);
         uint32_t tops[kJ];
         float inverses[kJ];
         if (eights && !of_row) {
@@ -253,11 +258,13 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
             }
 #pragma unroll
             for (uint32_t j = 0; j < kJ; ++j) {
-                for (uint32_t d = lanes >> 1; d > 0; d >>= 1) tops[j] = max(tops[j], __shfl_xor_sync(0xFFFFFFFFu, tops[j], d));
+#pragma unroll
+                for (uint32_t d = 1; d < 32u; d *= 2u)
+                    if (d < lanes) tops[j] = max(tops[j], __shfl_xor_sync(0xFFFFFFFFu, tops[j], d));
                 const uint32_t at = col + j * 32u * kE;
-                const float scale = scale_of(tops[j]);
-                if (at < p.cols && at % p.group == 0) p.scales[row * p.groups + at / p.group] = scale;
-                inverses[j] = inverse_of(tops[j], scale);
+                float scale;
+                scales_of(tops[j], &scale, inverses + j);
+                if (at < p.cols && (at & (p.group - 1u)) == 0) p.scales[row * p.groups + (at >> p.group_shift)] = scale;
             }
         }
 #pragma unroll
@@ -266,15 +273,17 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
             const bool there = at < p.cols;
             if (eights) {
                 const uint32_t top = of_row ? all.top : tops[j];
-                const float up = is_tiny(top) ? 0x1p100f : 1.f, by = of_row ? inverse : inverses[j];
+                const float by = of_row ? inverse : inverses[j];
+                if (top < kTiny || by == 0.f)
+#pragma unroll
+                    for (uint32_t e = 0; e < (uint32_t)kE; ++e) v[j * kE + e] = by == 0.f ? 0.f : v[j * kE + e] * 0x1p100f;
                 Raw<uint8_t, kE> q;
 #pragma unroll
                 for (uint32_t e = 0; e < (uint32_t)kE; e += 2) {
                     uint16_t two;
-                    const float a = v[j * kE + e] * up * by, b = kE > 1 ? v[j * kE + (kE > 1 ? e + 1 : e)] * up * by : 0.f;
-                    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(by == 0.f ? 0.f : b), "f"(by == 0.f ? 0.f : a));
-                    reinterpret_cast<uint8_t *>(q.u)[e] = (uint8_t)two;
-                    if (kE > 1) reinterpret_cast<uint8_t *>(q.u)[e + 1] = (uint8_t)(two >> 8);
+                    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(kE > 1 ? v[j * kE + (kE > 1 ? e + 1 : e)] * by : 0.f), "f"(v[j * kE + e] * by));
+                    if constexpr (kE > 1) reinterpret_cast<uint16_t *>(q.u)[e / 2] = two;
+                    else reinterpret_cast<uint8_t *>(q.u)[0] = (uint8_t)two;
                 }
                 if (there) q.store(static_cast<uint8_t *>(p.out) + (int64_t)row * p.ldo + at);
             } else if (there) {
@@ -282,7 +291,8 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
 #pragma unroll
                 for (uint32_t e = 0; e < (uint32_t)kE; ++e) y[e] = v[j * kE + e] * factor;
                 const int64_t to = (int64_t)row * p.ldo + at;
-                if (p.out_type == B200SPMM_T_F32) store_as<float, kE>(p.out, to, y);
+                if constexpr (kKind != kAny) store_as<X, kE>(p.out, to, y);
+                else if (p.out_type == B200SPMM_T_F32) store_as<float, kE>(p.out, to, y);
                 else if (p.out_type == B200SPMM_T_F16) store_as<__half, kE>(p.out, to, y);
                 else store_as<__nv_bfloat16, kE>(p.out, to, y);
             }
@@ -297,41 +307,55 @@ bool goes_by(const b200spmm_rms_norm_t *a, uint32_t e) {
            fits(a->out, a->ldo, a->out_dtype) && fits(a->weight, e, a->w_dtype);
 }
 
-template <typename X, typename R, int kE>
-int launch(const NormParams &p, cudaStream_t stream) {
-    const uint32_t spans = (p.cols + kSpan - 1) / kSpan;
-    uint32_t warps = 1, rows_of_block = 4;
-    if (spans > 4) {  // else a warp a row.  Few rows: as many threads as there are values; many: four times eight of them a thread
-        rows_of_block = 1;
-        const uint32_t kept = p.rows <= 2ull * sm_count() ? 1 : 4;
-        warps = std::min(32u, (spans + kept - 1) / kept);
-    }
-    const uint32_t per = (spans + warps - 1) / warps;
-    const uint64_t blocks = (p.rows + rows_of_block - 1) / rows_of_block;
-    if (blocks > 0x7FFFFFFFull) return B200SPMM_ERR_UNSUPPORTED;
-    auto kernel = per <= 1 ? rms_norm_kernel<X, R, 1, kE> : per <= 4 ? rms_norm_kernel<X, R, 4, kE> : rms_norm_kernel<X, R, 0, kE>;
+template <typename X, typename R, int kV, int kE, int kKind>
+int launch_kernel(const NormParams &p, uint64_t blocks, dim3 threads, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(32 * warps, rows_of_block);
+    cfg.blockDim = threads;
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, NormParams(p)));
+    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, rms_norm_kernel<X, R, kV, kE, kKind>, NormParams(p)));
     return B200SPMM_OK;
 }
 
-template <typename X, int kE>
-int launch_for(const NormParams &p, int r_type, cudaStream_t stream) {
-    if (!p.r) return launch<X, void, kE>(p, stream);
-    if (r_type == B200SPMM_T_F32) return launch<X, float, kE>(p, stream);
-    return launch<X, X, kE>(p, stream);
+template <typename X, typename R>
+int launch(const NormParams &p, uint32_t e, int kind, cudaStream_t stream) {
+    const uint32_t spans = (p.cols + kSpan - 1) / kSpan;
+    uint32_t warps = 1, rows_of_block = 4;
+    const bool few = p.rows <= 2ull * sm_count();
+    if (spans > 4 || (few && spans > 1)) {  // else a warp a row.  Few rows: as many threads as there are values; many: four times eight of them a thread
+        rows_of_block = 1;
+        warps = std::min(32u, few ? spans : (spans + 3) / 4);
+    }
+    const uint32_t per = (spans + warps - 1) / warps;
+    const uint64_t blocks = (p.rows + rows_of_block - 1) / rows_of_block;
+    if (blocks > 0x7FFFFFFFull) return B200SPMM_ERR_UNSUPPORTED;
+    const dim3 threads(32 * warps, rows_of_block);
+    // kernels of their own for what many rows of ordinary sizes are; else one that asks while it runs
+    auto of = [&](auto v, auto n, auto k) { return launch_kernel<X, R, decltype(v)::value, decltype(n)::value, decltype(k)::value>(p, blocks, threads, stream); };
+    auto kinds = [&](auto n) {
+        using V = std::integral_constant<int, 4>;
+        if (kind == kRow) return of(V(), n, std::integral_constant<int, kRow>());
+        if (kind == kGroups) return of(V(), n, std::integral_constant<int, kGroups>());
+        return of(V(), n, std::integral_constant<int, kSame>());
+    };
+    auto any = [&](auto n) {
+        using A = std::integral_constant<int, kAny>;
+        return per <= 1 ? of(std::integral_constant<int, 1>(), n, A()) : per <= 4 ? of(std::integral_constant<int, 4>(), n, A()) : of(std::integral_constant<int, 0>(), n, A());
+    };
+    if (per > 1 && per <= 4 && kind != kAny && e > 1) return e == 8 ? kinds(std::integral_constant<int, 8>()) : kinds(std::integral_constant<int, 2>());
+    return e == 8 ? any(std::integral_constant<int, 8>()) : any(std::integral_constant<int, 1>());
 }
+
 template <typename X>
-int launch_for(const NormParams &p, int r_type, uint32_t e, cudaStream_t stream) {
-    return e == 8 ? launch_for<X, 8>(p, r_type, stream) : e == 2 ? launch_for<X, 2>(p, r_type, stream) : launch_for<X, 1>(p, r_type, stream);
+int launch_for(const NormParams &p, int r_type, uint32_t e, int kind, cudaStream_t stream) {
+    if (!p.r) return launch<X, void>(p, e, kind, stream);
+    if (r_type == B200SPMM_T_F32) return launch<X, float>(p, e, kind, stream);
+    return launch<X, X>(p, e, kind, stream);
 }
 
 }  // namespace
@@ -364,11 +388,14 @@ extern "C" int b200spmm_rms_norm(const b200spmm_rms_norm_t *a, void *stream) {
         p.w_type = a->w_dtype;
         p.out_type = a->out_dtype;
         p.group = (uint32_t)a->group;
+        p.group_shift = a->group == 128 ? 7 : a->group == 64 ? 6 : 5;
         p.eps = a->eps;
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
         const uint32_t e = goes_by(a, 8) ? 8 : goes_by(a, 2) ? 2 : 1;
-        if (a->x_dtype == B200SPMM_T_F32) return launch_for<float>(p, a->r_dtype, e, s);
-        if (a->x_dtype == B200SPMM_T_F16) return launch_for<__half>(p, a->r_dtype, e, s);
-        return launch_for<__nv_bfloat16>(p, a->r_dtype, e, s);
+        const bool same = a->weight && a->w_dtype == a->x_dtype && (e4m3 || a->out_dtype == a->x_dtype);
+        const int kind = !same ? kAny : !e4m3 ? kSame : a->group ? kGroups : kRow;
+        if (a->x_dtype == B200SPMM_T_F32) return launch_for<float>(p, a->r_dtype, e, kind, s);
+        if (a->x_dtype == B200SPMM_T_F16) return launch_for<__half>(p, a->r_dtype, e, kind, s);
+        return launch_for<__nv_bfloat16>(p, a->r_dtype, e, kind, s);
     });
 }
