@@ -254,13 +254,67 @@ struct Gathered {
     B200_DEVICE uint4 operator()(uint32_t j, uint32_t u) const { return x(pairs[j] / top, u); }
 };
 
+// Columns that become fp16 are scaled by a power of two that takes their largest number to [2^14, 2^15): what lies more than 2^31 below it loses digits.
+B200_DEVICE int power_of(uint32_t top) { return max(-126, min(126, 14 - ((int)(top >> 23) - 127))); }
+
+// The largest finite |.| of n columns, as fp32's bits, by all threads: top_of(j, u) is that of unit u of column j.  32 divides `units`.
+// (Calls of their own, as all that brings columns: inlined, they take registers from the loops that follow.)
+template <class TopOf>
+B200_DEVICE void find_tops(uint32_t *tops, uint32_t n, uint32_t units, TopOf top_of) {
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) tops[i] = 0u;
+    __syncthreads();
+    const uint32_t lane = threadIdx.x & 31u, pieces = units / 32u;
+    constexpr uint32_t kBatch = 4;
+    for (uint32_t q = threadIdx.x >> 5; q < n * pieces; q += kBatch * kWarps) {
+        uint32_t top[kBatch];
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; ++b) {
+            const uint32_t at = q + b * kWarps;
+            top[b] = at < n * pieces ? top_of(at / pieces, at % pieces * 32u + lane) : 0u;
+        }
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; ++b) {
+            const uint32_t at = q + b * kWarps, most = __reduce_max_sync(0xFFFFFFFFu, top[b]);
+            if (lane == 0 && at < n * pieces) atomicMax(tops + at / pieces, most);
+        }
+    }
+    __syncthreads();
+}
+
+// Tokens of pairs as columns of fp16, from bf16.
+struct Converted {
+    Gathered<__nv_bfloat16> from;
+    const uint32_t *tops;
+    B200_DEVICE uint32_t top_of(uint32_t j, uint32_t u) const {
+        const uint4 v = from(j, u);
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w, a = w << 16 & 0x7FFF0000u, b = w & 0x7FFF0000u;
+            top = max(top, max(a < fp4::kInfBits ? a : 0u, b < fp4::kInfBits ? b : 0u));
+        }
+        return top;
+    }
+    B200_DEVICE uint4 operator()(uint32_t j, uint32_t u) const {
+        const uint4 v = from(j, u);
+        const float by = fp4::exp2_int(power_of(tops[j]));
+        auto two = [&](uint32_t w) {
+            const __half2 h = __floats2half2_rn(__uint_as_float(w << 16) * by, __uint_as_float(w & 0xFFFF0000u) * by);
+            return *reinterpret_cast<const uint32_t *>(&h);
+        };
+        return make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
+    }
+};
+
 // ------------------------------------------------------------------ gate, up, SiLU
 
-template <class W, int kNB>
+// X: x's type.  Codes are widened to fp16 either way, which takes five operations a word of eight where bf16 takes seven: bf16 columns are brought to fp16.
+template <class W, typename X, int kNB>
 B200_DEVICE void gate_up_part(const MoeParams &p, const Routing &r, uint8_t *smem, uint32_t columns_at, uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n) {
-    using T = typename W::T;
+    constexpr bool kConvert = !std::is_same<typename W::T, X>::value;
     const uint32_t base = ptx::smem_u32(smem), warp = warp_index(), lane = threadIdx.x & 31u;
     const uint32_t steps = (p.hidden + W::kStep - 1) / W::kStep, of_run = (p.inner + 7u) / 8u, pitch = column_pitch<W>(steps);
+    uint32_t *tops = reinterpret_cast<uint32_t *>(smem + columns_at + p.up_columns * pitch);
     const Split split(end - begin, steps, kWarps);
     const Share s(split, begin, end, warp, steps, steps, base + warp * kRingBytes<W>);
     multiply<W, kNB, 1, false, kRing<W>>(
@@ -274,7 +328,14 @@ B200_DEVICE void gate_up_part(const MoeParams &p, const Routing &r, uint8_t *sme
             return Columns{base + columns_at + (run_start(r, run) - pair0) * pitch, pitch, 0, run_end(r, run) - run_start(r, run), 0, 0, 0};
         },
         [&](uint32_t first, uint32_t count) {
-            stage_columns<W>(Gathered<T>{Plain<T>{static_cast<const T *>(p.x), 1, p.ldx, p.x_wide, p.hidden}, r.pairs + pair0, p.top}, base + columns_at, pitch, first, count, n, false);
+            const Gathered<X> from{Plain<X>{static_cast<const X *>(p.x), 1, p.ldx, p.x_wide, p.hidden}, r.pairs + pair0, p.top};
+            if constexpr (kConvert) {
+                const Converted to{from, tops};
+                find_tops(tops, n, count * W::kUnits, [&](uint32_t j, uint32_t u) { return to.top_of(j, u); });
+                stage_columns<W>(to, base + columns_at, pitch, first, count, n, false);
+            } else {
+                stage_columns<W>(from, base + columns_at, pitch, first, count, n, false);
+            }
         },
         [&](uint32_t tile, const float(&sums)[kNB][4]) {
             const uint32_t run = tile / of_run, i = tile % of_run * 8u + (lane >> 2), start = run_start(r, run), of = run_end(r, run) - start;
@@ -283,12 +344,14 @@ B200_DEVICE void gate_up_part(const MoeParams &p, const Routing &r, uint8_t *sme
 #pragma unroll
                 for (uint32_t e = 0; e < 2; ++e) {
                     const uint32_t j = nb * 8u + (lane & 3u) * 2u + e;
-                    if (j < of && i < p.inner) p.h[(uint64_t)r.pairs[start + j] * p.h_ld + i] = sums[nb][e] / (1.f + expf(-sums[nb][e])) * sums[nb][e + 2];
+                    if (j >= of || i >= p.inner) continue;
+                    const float back = kConvert ? fp4::exp2_int(-power_of(tops[start + j - pair0])) : 1.f, gate = sums[nb][e] * back;
+                    p.h[(uint64_t)r.pairs[start + j] * p.h_ld + i] = gate / (1.f + expf(-gate)) * (sums[nb][e + 2] * back);
                 }
         });
 }
 
-template <class W>
+template <class W, typename X>
 __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const MoeParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
     const Routing r = routing_at(smem + kWarps * kRingBytes<W>, p.pairs, p.experts);
@@ -310,20 +373,17 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const MoeParams p)
     if (write)
         for (uint32_t i = threadIdx.x; i < routing_bytes(p.pairs, p.experts) / 16u; i += kThreads) p.routing[i] = reinterpret_cast<const uint4 *>(smem + kWarps * kRingBytes<W>)[i];
     each_part(r, (p.inner + 7u) / 8u, p.up_columns, [&](uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n, uint32_t longest) {
-        if (longest <= 8u) gate_up_part<W, 1>(p, r, smem, columns_at, begin, end, pair0, n);
-        else gate_up_part<W, 2>(p, r, smem, columns_at, begin, end, pair0, n);
+        if (longest <= 8u) gate_up_part<W, X, 1>(p, r, smem, columns_at, begin, end, pair0, n);
+        else gate_up_part<W, X, 2>(p, r, smem, columns_at, begin, end, pair0, n);
     });
 }
 
 // ------------------------------------------------------------------ down
 
-// Inner values as a sum of two 16-bit numbers, the second what the first leaves over: fp16 has 22 digits that way, bf16 16.  fp16 gets them scaled by a power of two that takes
-// the pair's largest to [2^14, 2^15).
+// Inner values as one 16-bit number or the sum of two, the second what the first leaves over: fp16 has 11 or 22 digits that way, bf16 16 with two.
 template <typename T>
-B200_DEVICE void split_unit(const float *from, uint32_t left, float by, uint4 *high, uint4 *low) {
-    alignas(16) float v[8];
-    reinterpret_cast<float4 *>(v)[0] = reinterpret_cast<const float4 *>(from)[0];
-    reinterpret_cast<float4 *>(v)[1] = reinterpret_cast<const float4 *>(from)[1];
+B200_DEVICE void split_unit(const float4 (&from)[2], uint32_t left, float by, uint4 *high, uint4 *low) {
+    const float v[8] = {from[0].x, from[0].y, from[0].z, from[0].w, from[1].x, from[1].y, from[1].z, from[1].w};
     alignas(16) T a[8], b[8];
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) {
@@ -336,46 +396,72 @@ B200_DEVICE void split_unit(const float *from, uint32_t left, float by, uint4 *h
     *low = *reinterpret_cast<const uint4 *>(b);
 }
 
-template <class W, int kNB>
-B200_DEVICE void down_part(const MoeParams &p, const Routing &r, uint8_t *smem, uint32_t columns_at, uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n) {
+// Inner values of n pairs as columns, by all threads.
+template <class W, int kPlanes>
+__device__ __noinline__ void stage_inner(const float *h, uint32_t h_ld, uint32_t inner, const uint16_t *pairs, uint32_t n, uint32_t base, uint32_t pitch, uint32_t plane, uint32_t *tops) {
     using T = typename W::T;
     constexpr bool kScale = std::is_same<T, __half>::value;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    // (a row of h has room for whole units; what lies behind its end does not count)
+    auto load = [&](uint32_t j, uint32_t u, float4(&v)[2]) {
+        const float4 *from = reinterpret_cast<const float4 *>(h + (uint64_t)pairs[j] * h_ld + u * 8u);
+        v[0] = v[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (u * 8u < inner) {
+            v[0] = from[0];
+            v[1] = from[1];
+        }
+    };
+    const uint32_t room = (inner + W::kStep - 1) / W::kStep * W::kUnits, units = (room + 31u) / 32u * 32u, pieces = units / 32u;
+    if constexpr (kScale)
+        find_tops(tops, n, units, [&](uint32_t j, uint32_t u) {
+            float4 v[2];
+            load(j, u, v);
+            const float w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+            uint32_t top = 0;
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                const uint32_t b = __float_as_uint(w[e]) & 0x7FFFFFFFu;
+                if (u * 8u + e < inner && b < fp4::kInfBits) top = max(top, b);
+            }
+            return top;
+        });
+    constexpr uint32_t kBatch = 3;
+    for (uint32_t q = warp; q < n * pieces; q += kBatch * kWarps) {
+        float4 v[kBatch][2];
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; ++b) {
+            const uint32_t at = q + b * kWarps;
+            if (at < n * pieces) load(at / pieces, at % pieces * 32u + lane, v[b]);
+        }
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; ++b) {
+            const uint32_t at = q + b * kWarps, j = at / pieces, u = at % pieces * 32u + lane;
+            if (at >= n * pieces || u >= room) continue;
+            uint4 high, low;
+            split_unit<T>(v[b], u * 8u < inner ? inner - u * 8u : 0u, kScale ? fp4::exp2_int(power_of(tops[j])) : 1.f, &high, &low);
+            const uint32_t to = base + j * pitch + unit_place<W>(u);
+            ptx::st_shared_v4(to, unit_order<W>(high));
+            if (kPlanes > 1) ptx::st_shared_v4(to + plane, unit_order<W>(low));
+        }
+    }
+}
+
+template <class W, int kPlanes, int kNB>
+B200_DEVICE void down_part(const MoeParams &p, const Routing &r, uint8_t *smem, uint32_t columns_at, uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n) {
+    constexpr bool kScale = std::is_same<typename W::T, __half>::value;
     const uint32_t base = ptx::smem_u32(smem), warp = warp_index(), lane = threadIdx.x & 31u;
     const uint32_t steps = (p.inner + W::kStep - 1) / W::kStep, of_run = (p.hidden + kTileRows - 1u) / kTileRows, pitch = column_pitch<W>(steps), plane = p.down_columns * pitch;
-    float *scales = reinterpret_cast<float *>(smem + columns_at + 2u * plane);  // of the columns
+    uint32_t *tops = reinterpret_cast<uint32_t *>(smem + columns_at + kPlanes * plane);
     const Split split(end - begin, steps, kWarps);
     const Share s(split, begin, end, warp, steps, steps, base + warp * kRingBytes<W>);
-    multiply<W, kNB, 2, false, kRing<W>>(
+    multiply<W, kNB, kPlanes, false, kRing<W>>(
         p.down, s,
         [&](uint32_t tile, uint32_t row) { return (uint64_t)run_expert(r, tile / of_run) * p.hidden + min(tile % of_run * kTileRows + row, p.hidden - 1u); },
         [&](uint32_t tile) {
             const uint32_t run = tile / of_run;
             return Columns{base + columns_at + (run_start(r, run) - pair0) * pitch, pitch, plane, run_end(r, run) - run_start(r, run), 0, 0, 0};
         },
-        [&](uint32_t, uint32_t count) {
-            const uint32_t units = count * W::kUnits;
-            for (uint32_t j = warp; j < n; j += kWarps) {
-                const float *h = p.h + (uint64_t)r.pairs[pair0 + j] * p.h_ld;
-                float by = 1.f;
-                if constexpr (kScale) {
-                    uint32_t top = 0;
-                    for (uint32_t i = lane; i < p.inner; i += 32u) {
-                        const uint32_t b = __float_as_uint(h[i]) & 0x7FFFFFFFu;
-                        if (b < fp4::kInfBits) top = max(top, b);
-                    }
-                    top = __reduce_max_sync(0xFFFFFFFFu, top);
-                    by = fp4::exp2_int(max(-126, min(126, 14 - ((int)(top >> 23) - 127))));
-                    if (lane == 0) scales[j] = by;
-                }
-                for (uint32_t u = lane; u < units; u += 32u) {
-                    uint4 high = make_uint4(0u, 0u, 0u, 0u), low = high;
-                    if (u * 8u < p.inner) split_unit<T>(h + u * 8u, p.inner - u * 8u, by, &high, &low);
-                    const uint32_t to = base + columns_at + j * pitch + unit_place<W>(u);
-                    ptx::st_shared_v4(to, unit_order<W>(high));
-                    ptx::st_shared_v4(to + plane, unit_order<W>(low));
-                }
-            }
-        },
+        [&](uint32_t, uint32_t) { stage_inner<W, kPlanes>(p.h, p.h_ld, p.inner, r.pairs + pair0, n, base + columns_at, pitch, plane, tops); },
         [&](uint32_t tile, const float(&sums)[kNB][4]) {
             const uint32_t run = tile / of_run, row = tile % of_run * kTileRows + (lane >> 2), start = run_start(r, run), of = run_end(r, run) - start;
 #pragma unroll
@@ -383,12 +469,13 @@ B200_DEVICE void down_part(const MoeParams &p, const Routing &r, uint8_t *smem, 
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e) {
                     const uint32_t j = nb * 8u + (lane & 3u) * 2u + (e & 1u), at = row + (e >> 1) * 8u;
-                    if (j < of && at < p.hidden) p.parts[(uint64_t)r.pairs[start + j] * p.hidden + at] = kScale ? sums[nb][e] / scales[start + j - pair0] : sums[nb][e];
+                    if (j < of && at < p.hidden)
+                        p.parts[(uint64_t)r.pairs[start + j] * p.hidden + at] = kScale ? sums[nb][e] * fp4::exp2_int(-power_of(tops[start + j - pair0])) : sums[nb][e];
                 }
         });
 }
 
-template <class W>
+template <class W, int kPlanes>
 __global__ void __launch_bounds__(kThreads, 1) down_kernel(const MoeParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
     const Routing r = routing_at(smem + kWarps * kRingBytes<W>, p.pairs, p.experts);
@@ -397,8 +484,8 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const MoeParams p) {
     for (uint32_t i = threadIdx.x; i < routing_bytes(p.pairs, p.experts) / 16u; i += kThreads) reinterpret_cast<uint4 *>(smem + kWarps * kRingBytes<W>)[i] = p.routing[i];
     __syncthreads();
     each_part(r, (p.hidden + kTileRows - 1u) / kTileRows, p.down_columns, [&](uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n, uint32_t longest) {
-        if (longest <= 8u) down_part<W, 1>(p, r, smem, columns_at, begin, end, pair0, n);
-        else down_part<W, 2>(p, r, smem, columns_at, begin, end, pair0, n);
+        if (longest <= 8u) down_part<W, kPlanes, 1>(p, r, smem, columns_at, begin, end, pair0, n);
+        else down_part<W, kPlanes, 2>(p, r, smem, columns_at, begin, end, pair0, n);
     });
 }
 
@@ -482,26 +569,29 @@ uint32_t room_for(const MoeParams &p, uint32_t k, uint32_t planes) {
     const uint64_t each = (uint64_t)planes * ((uint64_t)steps * W::kUnits * 16u + 192u) + 4u;
     return (uint32_t)std::min<uint64_t>(p.pairs, (kMaxSmem - taken) / each);
 }
-template <class Up, class Down>
+template <class Up, typename X, class Down, int kPlanes>
 int launch_products(MoeParams p, cudaStream_t stream) {
     static std::atomic<uint64_t> up_allowed{0}, down_allowed{0};
     p.up_columns = room_for<Up>(p, p.hidden, 1);
-    p.down_columns = room_for<Down>(p, p.inner, 2);
+    p.down_columns = room_for<Down>(p, p.inner, kPlanes);
     p.run = std::min({kRun, p.up_columns, p.down_columns});
     if (p.run == 0) return B200SPMM_ERR_UNSUPPORTED;
     // (there are as many runs as pairs, or fewer)
     auto blocks = [&](uint32_t tiles) { return (uint32_t)std::min<uint64_t>(fp4::sm_count(), (uint64_t)p.pairs * tiles); };
-    B200_CUDA_TRY(allow_smem(gate_up_kernel<Up>, up_allowed));
-    B200_CUDA_TRY(allow_smem(down_kernel<Down>, down_allowed));
-    B200_CUDA_TRY(launch_after(gate_up_kernel<Up>, dim3(blocks((p.inner + 7) / 8)), kThreads, kMaxSmem, 1, stream, p));
-    B200_CUDA_TRY(launch_after(down_kernel<Down>, dim3(blocks((p.hidden + kTileRows - 1) / kTileRows)), kThreads, kMaxSmem, 1, stream, p));
+    B200_CUDA_TRY(allow_smem(gate_up_kernel<Up, X>, up_allowed));
+    B200_CUDA_TRY(allow_smem(down_kernel<Down, kPlanes>, down_allowed));
+    B200_CUDA_TRY(launch_after(gate_up_kernel<Up, X>, dim3(blocks((p.inner + 7) / 8)), kThreads, kMaxSmem, 1, stream, p));
+    B200_CUDA_TRY(launch_after(down_kernel<Down, kPlanes>, dim3(blocks((p.hidden + kTileRows - 1) / kTileRows)), kThreads, kMaxSmem, 1, stream, p));
     B200_CUDA_TRY(launch_after(sum_kernel, dim3((p.hidden + kSumThreads - 1) / kSumThreads, p.tokens), kSumThreads, 0, 1, stream, p));
     return B200SPMM_OK;
 }
-template <class Up>
+// Inner values beside codes: 22 digits where y is fp16; 11 where it is bf16, with 8 of its own.
+template <int kUp, typename X>
 int launch_down_for(const MoeParams &p, uint32_t span, cudaStream_t stream) {
-    using B = __nv_bfloat16;  // for its range: inner values are as large as they are, and codes are exact in either type
-    return span == 32 ? launch_products<Up, Weights<B, 32>>(p, stream) : span == 64 ? launch_products<Up, Weights<B, 64>>(p, stream) : launch_products<Up, Weights<B, 128>>(p, stream);
+    using Up = Weights<__half, kUp>;
+    constexpr int kPlanes = std::is_same<X, __half>::value ? 2 : 1;
+    return span == 32 ? launch_products<Up, X, Weights<__half, 32>, kPlanes>(p, stream) : span == 64 ? launch_products<Up, X, Weights<__half, 64>, kPlanes>(p, stream)
+                                                                                                     : launch_products<Up, X, Weights<__half, 128>, kPlanes>(p, stream);
 }
 
 template <typename T>
@@ -509,9 +599,9 @@ int launch_moe(const b200spmm_moe_t *m, const MoeParams &p, double *logits, cuda
     if (logits) {
         B200_CUDA_TRY(launch_after(logits_kernel<T>, dim3(p.experts, (p.tokens + kLogitTokens - 1) / kLogitTokens), kLogitThreads, 0, 1, stream, p, logits));
     }
-    if (!m->gate_up) return launch_products<Weights<T, 0>, Weights<T, 0>>(p, stream);
+    if (!m->gate_up) return launch_products<Weights<T, 0>, T, Weights<T, 0>, 2>(p, stream);
     const uint32_t a = span_of(m->gate_up), b = span_of(m->down);
-    return a == 32 ? launch_down_for<Weights<T, 32>>(p, b, stream) : a == 64 ? launch_down_for<Weights<T, 64>>(p, b, stream) : launch_down_for<Weights<T, 128>>(p, b, stream);
+    return a == 32 ? launch_down_for<32, T>(p, b, stream) : a == 64 ? launch_down_for<64, T>(p, b, stream) : launch_down_for<128, T>(p, b, stream);
 }
 
 // ids null: they are found from the logits, and left, with the shares, at out_ids and out_shares where those are wanted.

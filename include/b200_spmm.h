@@ -628,7 +628,8 @@ int b200spmm_int4_product(const b200spmm_int4_t *a, const void *d_B, int64_t ldb
  *     their sum where `renormalize`;     y = sum over them of share x down_e (silu(gate_e x) * (up_e x))
  * x, y and the router have one type, fp16 or bf16.  Experts: experts x 2 inner rows of `hidden` columns (for each expert first the gate's rows, then up's) and experts x hidden rows
  * of `inner` columns, one after the other: in 4-bit integers (gate_up, down), or in x's type (gate_up_16, down_16, rows ld elements apart, a multiple of 8, 16-byte
- * aligned), the others null.  Logits are added up in 64 bits, the inner values kept in 32 and multiplied as a sum of two 16-bit numbers.
+ * aligned), the others null.  Logits are added up in 64 bits; the inner values are kept in 32 and multiplied as the sum of two 16-bit
+ * numbers, by codes and for bf16 as one of fp16 (11 digits), scaled by powers of two.
  * experts up to 1024, top_k up to 32.  A row of x with NaN gives NaN in its own row of y alone.
  */
 typedef struct {

@@ -49,7 +49,8 @@ class Case:
 
         A sum of K products takes K / 16 additions of the MMA (16-bit experts) or span / 16 of them and one rounding of fp32 for each span (codes), and up to 24 that join parts:
         `off` of the sum of magnitudes.  An inner value is off by what its gate (SiLU's slope is at most 1.1) and up are, and 2^-20 of itself for exp, the division and the product.
-        It is multiplied as two 16-bit numbers: 2^-16 is lost (bf16; fp16 2^-22, and 2^-38 of the pair's largest).  Their products take twice the additions."""
+        It is multiplied as two 16-bit numbers, of which 2^-16 is lost (bf16) or 2^-22 (fp16), or, by codes and for bf16, as one of fp16: 2^-11; fp16, scaled, loses
+        2^-38 of the pair's largest besides (half of its smallest step, 2^-25, of 2^14 or more; and so, 2^-39, do bf16 columns that are brought to fp16).  Two take twice the additions."""
         x, want, bound = x.double(), torch.zeros(x.shape, dtype=torch.float64, device="cuda"), torch.zeros(x.shape, dtype=torch.float64, device="cuda")
         span = 0 if self.group == 0 else min(128, self.group or 128)
 
@@ -58,7 +59,8 @@ class Case:
                 return planes * span / 16 * 2.0 ** -22 + (-(-k // span) + 24 + 2) * 2.0 ** -24
             return (planes * -(-k // 16) + 24) * 2.0 ** -22
 
-        lost = 2.0 ** -16 if span or self.dtype == BF16 else 2.0 ** -22
+        one = span and self.dtype == BF16
+        lost = 2.0 ** -11 if one else 2.0 ** -16 if self.dtype == BF16 else 2.0 ** -22
         for e in range(self.E):
             t, j = torch.where(ids == e)
             if len(t) == 0:
@@ -66,12 +68,15 @@ class Case:
             gate_up, down = self.expert(e)
             (g, u), (mg, mu) = (x[t] @ gate_up.t()).split(self.I, 1), (x[t].abs() @ gate_up.abs().t()).split(self.I, 1)
             dg, du = mg * off(self.H, 1), mu * off(self.H, 1)
+            if one:  # (of the weights' sum of magnitudes)
+                far = x[t].abs().amax(1, keepdim=True) * gate_up.abs().sum(1) * 2.0 ** -39
+                dg, du = dg + far[:, :self.I], du + far[:, self.I:]
             silu = g * torch.sigmoid(g)
             h = silu * u
             dh = 1.1 * dg * (u.abs() + du) + silu.abs() * du + h.abs() * 2.0 ** -20
             dh = dh + h.abs() * lost + h.abs().amax(1, keepdim=True) * 2.0 ** -38
             out, mag = h @ down.t(), h.abs() @ down.abs().t()
-            d = mag * off(self.I, 2) + dh @ down.abs().t()
+            d = mag * off(self.I, 1 if one else 2) + dh @ down.abs().t()
             s = shares[t, j].double()[:, None]
             want.index_add_(0, t, s * out)
             bound.index_add_(0, t, s.abs() * (d + out.abs() * (self.top + 1) * 2.0 ** -24))
