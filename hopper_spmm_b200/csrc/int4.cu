@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps<kNB>, 1) int4_kernel(const Int4
     const uint32_t base = ptx::smem_u32(smem), warp = warp_index(), g = (threadIdx.x & 31u) >> 2;
     constexpr uint32_t ring_bytes = kRingOf<W, kNB, kRing>;
     const uint32_t j0 = blockIdx.y * (8u * kNB);
-    Columns c;
+    Columns c{};
     c.base = base + p.warps * ring_bytes;
     c.pitch = column_pitch<W>(p.window);
     c.plane = 0;
@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps<kNB>, 1) int4_kernel(const Int4
         for (uint32_t i = threadIdx.x; i < c.n * p.x_groups; i += blockDim.x) to[i] = p.x_scales[(uint64_t)j0 * p.x_groups + i];
     }
     multiply<W, kNB, 1, kScaled, kRing>(
-        p.m, s, [&](uint32_t tile, uint32_t r) { return (uint64_t)min(tile * kTileRows + r, p.rows - 1u); }, [&](uint32_t) { return c; },
+        p.m, s, [](uint32_t tile) { return tile; }, [&](uint32_t tile, uint32_t r) { return (uint64_t)min(tile * kTileRows + r, p.rows - 1u); }, [&](uint32_t) { return c; },
         [&](uint32_t first, uint32_t count) {
             if constexpr (kScaled)
                 stage_columns<W>(Eights{static_cast<const uint8_t *>(p.x) + (int64_t)j0 * p.across, p.across, p.wide, p.k}, c.base, c.pitch, first, count, c.n, false);

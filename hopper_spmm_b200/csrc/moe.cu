@@ -17,7 +17,7 @@ namespace b200spmm {
 namespace narrow {
 namespace {
 
-constexpr uint32_t kWarps = 24, kThreads = 32 * kWarps;
+constexpr uint32_t kWarps = 20, kThreads = 32 * kWarps;
 constexpr uint32_t kRun = 16;  // columns that a tile meets at once, at most
 template <class W>
 constexpr int kRing = 2 * W::kPieces;  // stages of a warp: two steps
@@ -29,6 +29,7 @@ constexpr uint32_t kLogitTokens = 4, kLogitThreads = 256;
 struct MoeParams {
     Matrix gate_up, down;
     uint32_t experts, hidden, inner, top, tokens, pairs;
+    bool all_tokens;  // are columns of the first product, in all blocks
     uint32_t run, up_columns, down_columns;  // columns of a run, and that a block has room for, in either product
     uint4 *routing;  // as the first blocks found it
     bool renormalize;
@@ -170,8 +171,49 @@ B200_DEVICE void choose_of(const MoeParams &p, uint32_t t, int32_t *ids, bool wr
         }
     }
 }
-B200_DEVICE void choose(const MoeParams &p, uint32_t t, int32_t *ids, bool write) {
-    if (p.experts <= 64u) choose_of<2>(p, t, ids, write);
+// The same for up to 128 experts, from how many keys are before each: all compared with all, without a round that waits for the last.  `keys`: shared memory of the warp.
+template <int kKeys>
+B200_DEVICE void choose_by_rank(const MoeParams &p, uint32_t t, int32_t *ids, bool write, uint64_t *keys) {
+    const double *l = p.logits + (uint64_t)t * p.experts;
+    const uint32_t lane = threadIdx.x & 31u;
+    uint64_t mine[kKeys], most = 0;
+    uint32_t rank[kKeys] = {};
+#pragma unroll
+    for (uint32_t i = 0; i < (uint32_t)kKeys; ++i) {
+        mine[i] = lane + 32u * i < p.experts ? key_of(l[lane + 32u * i]) : 0ull;
+        if (lane + 32u * i < p.experts) keys[lane + 32u * i] = mine[i];
+    }
+    __syncwarp();
+#pragma unroll 4
+    for (uint32_t e = 0; e < p.experts; ++e) {
+        const uint64_t k = keys[e];
+        most = k > most ? k : most;
+#pragma unroll
+        for (uint32_t i = 0; i < (uint32_t)kKeys; ++i) rank[i] += k > mine[i] || (k == mine[i] && e < lane + 32u * i) ? 1u : 0u;
+    }
+    float part[kKeys], sum = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < (uint32_t)kKeys; ++i) {
+        const bool chosen = mine[i] && rank[i] < p.top;
+        part[i] = mine[i] && (chosen || !p.renormalize) ? expf((float)(value_of(mine[i]) - value_of(most))) : 0.f;
+        sum += part[i];
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+#pragma unroll
+    for (uint32_t i = 0; i < (uint32_t)kKeys; ++i) {
+        if (!mine[i] || rank[i] >= p.top) continue;
+        ids[t * p.top + rank[i]] = (int32_t)(lane + 32u * i);
+        if (write) {
+            p.ids[t * p.top + rank[i]] = (int32_t)(lane + 32u * i);
+            p.shares[t * p.top + rank[i]] = part[i] / sum;
+        }
+    }
+    __syncwarp();
+}
+B200_DEVICE void choose(const MoeParams &p, uint32_t t, int32_t *ids, bool write, uint64_t *keys) {
+    if (p.experts <= 64u) choose_by_rank<2>(p, t, ids, write, keys);
+    else if (p.experts <= 128u) choose_by_rank<4>(p, t, ids, write, keys);
     else if (p.experts <= 256u) choose_of<8>(p, t, ids, write);
     else choose_of<32>(p, t, ids, write);
 }
@@ -199,7 +241,7 @@ B200_DEVICE void find_runs(const MoeParams &p, const Routing &r, uint32_t most) 
         for (uint32_t e0 = 0; e0 < p.experts; e0 += 32u) {
             const uint32_t e = e0 + lane, n = e < p.experts ? r.starts[e] : 0u, m = (n + most - 1u) / most;
             uint32_t both_to = n << 16 | m;  // up to this one (at most 8,192 of either)
-#pragma unroll
+#pragma unroll 1
             for (uint32_t d = 1; d < 32u; d *= 2u) {
                 const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, both_to, d);
                 if (lane >= d) both_to += v;
@@ -245,6 +287,15 @@ B200_DEVICE void each_part(const Routing &r, uint32_t of_run, uint32_t room, Par
     }
 }
 
+// What a tile of a run is.
+struct Place {
+    uint32_t tile, expert, start, n;  // of the run; its expert and pairs
+};
+B200_DEVICE Place place_in(const Routing &r, uint32_t of_run, uint32_t tile) {
+    const uint32_t run = tile / of_run, start = run_start(r, run);
+    return {tile - run * of_run, run_expert(r, run), start, run_end(r, run) - start};
+}
+
 // Tokens of pairs as columns.
 template <typename T>
 struct Gathered {
@@ -281,9 +332,10 @@ B200_DEVICE void find_tops(uint32_t *tops, uint32_t n, uint32_t units, TopOf top
     __syncthreads();
 }
 
-// Tokens of pairs as columns of fp16, from bf16.
+// Columns of fp16 from those of bf16.
+template <class From>
 struct Converted {
-    Gathered<__nv_bfloat16> from;
+    From from;
     const uint32_t *tops;
     B200_DEVICE uint32_t top_of(uint32_t j, uint32_t u) const {
         const uint4 v = from(j, u);
@@ -319,36 +371,51 @@ B200_DEVICE void gate_up_part(const MoeParams &p, const Routing &r, uint8_t *sme
     const Share s(split, begin, end, warp, steps, steps, base + warp * kRingBytes<W>);
     multiply<W, kNB, 1, false, kRing<W>>(
         p.gate_up, s,
-        [&](uint32_t tile, uint32_t row) {
-            const uint32_t i = min(tile % of_run * 8u + row % 8u, p.inner - 1u);
-            return ((uint64_t)run_expert(r, tile / of_run) * 2u + row / 8u) * p.inner + i;
-        },
-        [&](uint32_t tile) {
-            const uint32_t run = tile / of_run;
-            return Columns{base + columns_at + (run_start(r, run) - pair0) * pitch, pitch, 0, run_end(r, run) - run_start(r, run), 0, 0, 0};
+        [&](uint32_t tile) { return place_in(r, of_run, tile); },
+        [&](const Place &at, uint32_t row) { return ((uint64_t)at.expert * 2u + row / 8u) * p.inner + min(at.tile * 8u + row % 8u, p.inner - 1u); },
+        [&](const Place &at) {
+            if (p.all_tokens) return Columns{base + columns_at, pitch, 0, at.n, 0, 0, 0, r.pairs + at.start, p.top};
+            return Columns{base + columns_at + (at.start - pair0) * pitch, pitch, 0, at.n, 0, 0, 0, nullptr, 1};
         },
         [&](uint32_t first, uint32_t count) {
+            if (p.all_tokens) return;
             const Gathered<X> from{Plain<X>{static_cast<const X *>(p.x), 1, p.ldx, p.x_wide, p.hidden}, r.pairs + pair0, p.top};
             if constexpr (kConvert) {
-                const Converted to{from, tops};
+                const Converted<Gathered<X>> to{from, tops};
                 find_tops(tops, n, count * W::kUnits, [&](uint32_t j, uint32_t u) { return to.top_of(j, u); });
                 stage_columns<W>(to, base + columns_at, pitch, first, count, n, false);
             } else {
                 stage_columns<W>(from, base + columns_at, pitch, first, count, n, false);
             }
         },
-        [&](uint32_t tile, const float(&sums)[kNB][4]) {
-            const uint32_t run = tile / of_run, i = tile % of_run * 8u + (lane >> 2), start = run_start(r, run), of = run_end(r, run) - start;
+        [&](const Place &at, const float(&sums)[kNB][4]) {
+            const uint32_t i = at.tile * 8u + (lane >> 2);
 #pragma unroll
             for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
 #pragma unroll
                 for (uint32_t e = 0; e < 2; ++e) {
                     const uint32_t j = nb * 8u + (lane & 3u) * 2u + e;
-                    if (j >= of || i >= p.inner) continue;
-                    const float back = kConvert ? fp4::exp2_int(-power_of(tops[start + j - pair0])) : 1.f, gate = sums[nb][e] * back;
-                    p.h[(uint64_t)r.pairs[start + j] * p.h_ld + i] = gate / (1.f + expf(-gate)) * (sums[nb][e + 2] * back);
+                    if (j >= at.n || i >= p.inner) continue;
+                    const uint32_t pair = r.pairs[at.start + j];
+                    const float back = kConvert ? fp4::exp2_int(-power_of(tops[p.all_tokens ? pair / p.top : at.start + j - pair0])) : 1.f, gate = sums[nb][e] * back;
+                    p.h[(uint64_t)pair * p.h_ld + i] = gate / (1.f + expf(-gate)) * (sums[nb][e + 2] * back);
                 }
         });
+}
+
+// All tokens as columns, where there is room for them: they need no routing.
+template <class W, typename X>
+B200_DEVICE void stage_tokens(const MoeParams &p, uint8_t *smem, uint32_t columns_at) {
+    const uint32_t steps = (p.hidden + W::kStep - 1) / W::kStep, pitch = column_pitch<W>(steps), at = ptx::smem_u32(smem) + columns_at;
+    uint32_t *tops = reinterpret_cast<uint32_t *>(smem + columns_at + p.up_columns * pitch);
+    const Plain<X> from{static_cast<const X *>(p.x), 1, p.ldx, p.x_wide, p.hidden};
+    if constexpr (!std::is_same<typename W::T, X>::value) {
+        const Converted<Plain<X>> to{from, tops};
+        find_tops(tops, p.tokens, steps * W::kUnits, [&](uint32_t j, uint32_t u) { return to.top_of(j, u); });
+        stage_columns<W>(to, at, pitch, 0, steps, p.tokens, false);
+    } else {
+        stage_columns<W>(from, at, pitch, 0, steps, p.tokens, false);
+    }
 }
 
 template <class W, typename X>
@@ -358,8 +425,10 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const MoeParams p)
     const uint32_t columns_at = kWarps * kRingBytes<W> + routing_bytes(p.pairs, p.experts);
     ptx::wait_for_grids_before();
     const bool write = blockIdx.x == 0;
+    if (p.all_tokens) stage_tokens<W, X>(p, smem, columns_at);
     if (p.logits) {
-        for (uint32_t t = threadIdx.x >> 5; t < p.tokens; t += kWarps) choose(p, t, r.ids, write);
+        for (uint32_t t = threadIdx.x >> 5; t < p.tokens; t += kWarps)
+            choose(p, t, r.ids, write, reinterpret_cast<uint64_t *>(smem + (threadIdx.x >> 5) * kRingBytes<W>));
     } else {
         for (uint32_t i = threadIdx.x; i < p.pairs; i += kThreads) {
             const int64_t e = p.id_bytes == 8 ? static_cast<const int64_t *>(p.ids_in)[i] : static_cast<const int32_t *>(p.ids_in)[i];
@@ -372,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const MoeParams p)
     find_runs(p, r, p.run);
     if (write)
         for (uint32_t i = threadIdx.x; i < routing_bytes(p.pairs, p.experts) / 16u; i += kThreads) p.routing[i] = reinterpret_cast<const uint4 *>(smem + kWarps * kRingBytes<W>)[i];
-    each_part(r, (p.inner + 7u) / 8u, p.up_columns, [&](uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n, uint32_t longest) {
+    each_part(r, (p.inner + 7u) / 8u, p.all_tokens ? p.pairs : p.up_columns, [&](uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n, uint32_t longest) {
         if (longest <= 8u) gate_up_part<W, X, 1>(p, r, smem, columns_at, begin, end, pair0, n);
         else gate_up_part<W, X, 2>(p, r, smem, columns_at, begin, end, pair0, n);
     });
@@ -456,21 +525,18 @@ B200_DEVICE void down_part(const MoeParams &p, const Routing &r, uint8_t *smem, 
     const Share s(split, begin, end, warp, steps, steps, base + warp * kRingBytes<W>);
     multiply<W, kNB, kPlanes, false, kRing<W>>(
         p.down, s,
-        [&](uint32_t tile, uint32_t row) { return (uint64_t)run_expert(r, tile / of_run) * p.hidden + min(tile % of_run * kTileRows + row, p.hidden - 1u); },
-        [&](uint32_t tile) {
-            const uint32_t run = tile / of_run;
-            return Columns{base + columns_at + (run_start(r, run) - pair0) * pitch, pitch, plane, run_end(r, run) - run_start(r, run), 0, 0, 0};
-        },
+        [&](uint32_t tile) { return place_in(r, of_run, tile); },
+        [&](const Place &at, uint32_t row) { return (uint64_t)at.expert * p.hidden + min(at.tile * kTileRows + row, p.hidden - 1u); },
+        [&](const Place &at) { return Columns{base + columns_at + (at.start - pair0) * pitch, pitch, plane, at.n, 0, 0, 0, nullptr, 1}; },
         [&](uint32_t, uint32_t) { stage_inner<W, kPlanes>(p.h, p.h_ld, p.inner, r.pairs + pair0, n, base + columns_at, pitch, plane, tops); },
-        [&](uint32_t tile, const float(&sums)[kNB][4]) {
-            const uint32_t run = tile / of_run, row = tile % of_run * kTileRows + (lane >> 2), start = run_start(r, run), of = run_end(r, run) - start;
+        [&](const Place &at, const float(&sums)[kNB][4]) {
 #pragma unroll
             for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e) {
-                    const uint32_t j = nb * 8u + (lane & 3u) * 2u + (e & 1u), at = row + (e >> 1) * 8u;
-                    if (j < of && at < p.hidden)
-                        p.parts[(uint64_t)r.pairs[start + j] * p.hidden + at] = kScale ? sums[nb][e] * fp4::exp2_int(-power_of(tops[start + j - pair0])) : sums[nb][e];
+                    const uint32_t j = nb * 8u + (lane & 3u) * 2u + (e & 1u), row = at.tile * kTileRows + (lane >> 2) + (e >> 1) * 8u;
+                    if (j < at.n && row < p.hidden)
+                        p.parts[(uint64_t)r.pairs[at.start + j] * p.hidden + row] = kScale ? sums[nb][e] * fp4::exp2_int(-power_of(tops[at.start + j - pair0])) : sums[nb][e];
                 }
         });
 }
@@ -567,13 +633,16 @@ template <class W>
 uint32_t room_for(const MoeParams &p, uint32_t k, uint32_t planes) {
     const uint32_t taken = kWarps * kRingBytes<W> + routing_bytes(p.pairs, p.experts), steps = (k + W::kStep - 1) / W::kStep;
     const uint64_t each = (uint64_t)planes * ((uint64_t)steps * W::kUnits * 16u + 192u) + 4u;
-    return (uint32_t)std::min<uint64_t>(p.pairs, (kMaxSmem - taken) / each);
+    return (uint32_t)std::min<uint64_t>(p.pairs, (kMaxSmem - taken) / each);  // (as many as there are pairs at most)
 }
 template <class Up, typename X, class Down, int kPlanes>
 int launch_products(MoeParams p, cudaStream_t stream) {
     static std::atomic<uint64_t> up_allowed{0}, down_allowed{0};
     p.up_columns = room_for<Up>(p, p.hidden, 1);
     p.down_columns = room_for<Down>(p, p.inner, kPlanes);
+    // Columns of all tokens are there before the routing is, those of a block's own pairs are fewer: one token 37.2 us with all and 38.4 with its own, 8 with 4-bit experts 149.4
+    // and 147.1.
+    p.all_tokens = p.tokens <= std::min(4u, p.up_columns);
     p.run = std::min({kRun, p.up_columns, p.down_columns});
     if (p.run == 0) return B200SPMM_ERR_UNSUPPORTED;
     // (there are as many runs as pairs, or fewer)

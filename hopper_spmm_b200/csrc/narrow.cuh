@@ -137,6 +137,9 @@ struct Widen<__nv_bfloat16> {
 struct Columns {
     uint32_t base, pitch, plane, n;
     uint32_t scales, groups, shift;
+    const uint16_t *order;  // column j of a tile is order[j] / each of those in shared memory; null: j
+    uint32_t each;
+    B200_DEVICE uint32_t address(uint32_t j) const { return base + (order ? order[j] / each : j) * pitch; }
 };
 
 // A unit of a lane's column, by lanes that have one; the others' registers hold what they held, and so do the sums of columns that nobody looks at.  (A load
@@ -186,11 +189,11 @@ struct Share {
     }
 };
 
-// All threads of a block come here alike.  rows_of(tile, r) is row r (0 to 15) of a tile in the matrix, columns_of(tile) what it is multiplied with.  stage(first step, steps) brings columns to shared
-// memory, all of them before the first tile, or (window < steps) window by window in every round.  done(tile, sums) gets a tile's sums in one warp: rows g (e < 2) and g + 8,
-// columns 8 nb + 2 t + e % 2.
-template <class W, int kNB, int kPlanes, bool kScaled, int kStages, class RowsOf, class ColumnsOf, class Stage, class Done>
-B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, ColumnsOf &&columns_of, Stage &&stage, Done &&done) {
+// All threads of a block come here alike.  place_of(tile) is what the others are told of a tile (a number's quotients, say, that they would all take); rows_of(place, r) row r
+// (0 to 15) of it in the matrix, columns_of(place) what it is multiplied with.  stage(first step, steps) brings columns to shared memory, all of them before the first tile, or
+// (window < steps) window by window in every round.  done(place, sums) gets a tile's sums in one warp: rows g (e < 2) and g + 8, columns 8 nb + 2 t + e % 2.
+template <class W, int kNB, int kPlanes, bool kScaled, int kStages, class PlaceOf, class RowsOf, class ColumnsOf, class Stage, class Done>
+B200_DEVICE void multiply(const Matrix &m, const Share &s, PlaceOf &&place_of, RowsOf &&rows_of, ColumnsOf &&columns_of, Stage &&stage, Done &&done) {
     using T = typename W::T;
     static_assert(kStages == W::kPieces || kStages == 2 * W::kPieces, "a ring of one step or two");
     const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
@@ -201,12 +204,13 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, Col
     const uint8_t *lo = nullptr, *hi = nullptr;
     auto copy_from = [&]() {
         copied = s.slice * kStepBytes + copy_piece * 16u;
-        const uint64_t row_lo = rows_of(copy_tile, copy_row), row_hi = rows_of(copy_tile, copy_row + 8u);
+        const auto place = place_of(copy_tile);
+        const uint64_t row_lo = rows_of(place, copy_row), row_hi = rows_of(place, copy_row + 8u);
         lo = m.values + row_lo * m.pitch + copied;
         hi = m.values + row_hi * m.pitch + copied;
         if (W::kPiece == 128) {
-            lo_4 = (uint32_t)((rows_of(copy_tile, copy_row + 4u) - row_lo) * m.pitch);
-            hi_4 = (uint32_t)((rows_of(copy_tile, copy_row + 12u) - row_hi) * m.pitch);
+            lo_4 = (uint32_t)((rows_of(place, copy_row + 4u) - row_lo) * m.pitch);
+            hi_4 = (uint32_t)((rows_of(place, copy_row + 12u) - row_hi) * m.pitch);
         }
     };
     auto issue = [&](uint32_t at, uint32_t piece) {  // of the next step
@@ -247,7 +251,7 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, Col
     const uint32_t entry_first = s.slice * W::kStep + (t >> 1) * (uint32_t)W::kSpan, entry_end = s.steps * W::kStep;
     auto entries_from = [&]() {
         entry_k = entry_first;
-        entry_row = (uint32_t)rows_of(entry_tile, g + (t & 1u) * 8u);
+        entry_row = (uint32_t)rows_of(place_of(entry_tile), g + (t & 1u) * 8u);
     };
     auto fetch = [&]() {
         if constexpr (W::kCodes) {
@@ -266,7 +270,7 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, Col
     };
     if (s.first < s.end) {
         copy_from();
-#pragma unroll
+#pragma unroll 1
         for (uint32_t i = 0; i < kStages; ++i) issue(s.ring + i * W::kStageBytes, i % W::kPieces);
         if constexpr (W::kCodes) {
             entries_from();
@@ -284,13 +288,13 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, Col
     float sums[kNB][4];
     for (uint32_t round = 0; round < s.rounds; ++round, tile += s.at_once) {
         const bool busy = tile < s.end;
-        const Columns c = busy ? columns_of(tile) : Columns{};
+        const Columns c = busy ? columns_of(place_of(tile)) : Columns{};
         uint32_t column[kNB];  // this lane's, for the second operand, where it has one
         bool has[kNB];
 #pragma unroll
         for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
             has[nb] = nb * 8u + g < c.n;
-            column[nb] = c.base + (nb * 8u + g) * c.pitch + t * 16u;
+            column[nb] = (has[nb] ? c.address(nb * 8u + g) : c.base) + t * 16u;
             sums[nb][0] = sums[nb][1] = sums[nb][2] = sums[nb][3] = 0.f;
         }
         uint32_t step = s.slice;
@@ -379,7 +383,7 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, Col
                 }
             }
         }
-        if (s.slices == 1 && busy) done(tile, sums);
+        if (s.slices == 1 && busy) done(place_of(tile), sums);
     }
     if (s.slices > 1) {  // (one round) the slices' sums meet in the first one's warp, in order
         __syncwarp();
@@ -398,7 +402,7 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, RowsOf &&rows_of, Col
                     sums[nb][2] += __uint_as_float(v.z);
                     sums[nb][3] += __uint_as_float(v.w);
                 }
-            done(s.first, sums);
+            done(place_of(s.first), sums);
         }
     }
 }
@@ -434,8 +438,11 @@ struct Eights {  // e4m3, as fp16
             v[0] = both.x;
             v[1] = both.y;
         } else {
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) v[e / 4] |= (e < left ? (uint32_t)p[e] : 0u) << e % 4 * 8;
+#pragma unroll 1
+            for (uint32_t e = 0; e < 8u; ++e) {
+                v[0] = v[0] >> 8 | v[1] << 24;
+                v[1] = v[1] >> 8 | (e < left ? (uint32_t)p[e] : 0u) << 24;
+            }
         }
         uint32_t h[4];
 #pragma unroll
