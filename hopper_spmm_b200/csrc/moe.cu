@@ -614,7 +614,7 @@ int check_moe(const b200spmm_moe_t *m) {
             if (codes[i]->rows != rows[i] || codes[i]->cols != cols[i] || codes[i]->device != m->device) return B200SPMM_ERR_INVALID_ARG;
         } else {
             if (ld[i] < (int64_t)cols[i]) return B200SPMM_ERR_INVALID_ARG;
-            if (ld[i] % 8 != 0 || !fp4::aligned(plain[i], 16)) return B200SPMM_ERR_UNSUPPORTED;
+            if (ld[i] % 8 != 0 || ld[i] > 1 << 28 || !fp4::aligned(plain[i], 16)) return B200SPMM_ERR_UNSUPPORTED;
         }
     }
     return B200SPMM_OK;
@@ -636,7 +636,7 @@ uint32_t room_for(const MoeParams &p, uint32_t k, uint32_t planes) {
     return (uint32_t)std::min<uint64_t>(p.pairs, (kMaxSmem - taken) / each);  // (as many as there are pairs at most)
 }
 template <class Up, typename X, class Down, int kPlanes>
-int launch_products(MoeParams p, cudaStream_t stream) {
+int launch_all(MoeParams p, double *logits, cudaStream_t stream) {
     static std::atomic<uint64_t> up_allowed{0}, down_allowed{0};
     p.up_columns = room_for<Up>(p, p.hidden, 1);
     p.down_columns = room_for<Down>(p, p.inner, kPlanes);
@@ -649,6 +649,7 @@ int launch_products(MoeParams p, cudaStream_t stream) {
     auto blocks = [&](uint32_t tiles) { return (uint32_t)std::min<uint64_t>(fp4::sm_count(), (uint64_t)p.pairs * tiles); };
     B200_CUDA_TRY(allow_smem(gate_up_kernel<Up, X>, up_allowed));
     B200_CUDA_TRY(allow_smem(down_kernel<Down, kPlanes>, down_allowed));
+    if (logits) B200_CUDA_TRY(launch_after(logits_kernel<X>, dim3(p.experts, (p.tokens + kLogitTokens - 1) / kLogitTokens), kLogitThreads, 0, 1, stream, p, logits));
     B200_CUDA_TRY(launch_after(gate_up_kernel<Up, X>, dim3(blocks((p.inner + 7) / 8)), kThreads, kMaxSmem, 1, stream, p));
     B200_CUDA_TRY(launch_after(down_kernel<Down, kPlanes>, dim3(blocks((p.hidden + kTileRows - 1) / kTileRows)), kThreads, kMaxSmem, 1, stream, p));
     B200_CUDA_TRY(launch_after(sum_kernel, dim3((p.hidden + kSumThreads - 1) / kSumThreads, p.tokens), kSumThreads, 0, 1, stream, p));
@@ -656,21 +657,19 @@ int launch_products(MoeParams p, cudaStream_t stream) {
 }
 // Inner values beside codes: 22 digits where y is fp16; 11 where it is bf16, with 8 of its own.
 template <int kUp, typename X>
-int launch_down_for(const MoeParams &p, uint32_t span, cudaStream_t stream) {
+int launch_codes(const MoeParams &p, uint32_t span, double *logits, cudaStream_t stream) {
     using Up = Weights<__half, kUp>;
     constexpr int kPlanes = std::is_same<X, __half>::value ? 2 : 1;
-    return span == 32 ? launch_products<Up, X, Weights<__half, 32>, kPlanes>(p, stream) : span == 64 ? launch_products<Up, X, Weights<__half, 64>, kPlanes>(p, stream)
-                                                                                                     : launch_products<Up, X, Weights<__half, 128>, kPlanes>(p, stream);
+    return span == 32   ? launch_all<Up, X, Weights<__half, 32>, kPlanes>(p, logits, stream)
+           : span == 64 ? launch_all<Up, X, Weights<__half, 64>, kPlanes>(p, logits, stream)
+                        : launch_all<Up, X, Weights<__half, 128>, kPlanes>(p, logits, stream);
 }
 
 template <typename T>
 int launch_moe(const b200spmm_moe_t *m, const MoeParams &p, double *logits, cudaStream_t stream) {
-    if (logits) {
-        B200_CUDA_TRY(launch_after(logits_kernel<T>, dim3(p.experts, (p.tokens + kLogitTokens - 1) / kLogitTokens), kLogitThreads, 0, 1, stream, p, logits));
-    }
-    if (!m->gate_up) return launch_products<Weights<T, 0>, T, Weights<T, 0>, 2>(p, stream);
+    if (!m->gate_up) return launch_all<Weights<T, 0>, T, Weights<T, 0>, 2>(p, logits, stream);
     const uint32_t a = span_of(m->gate_up), b = span_of(m->down);
-    return a == 32 ? launch_down_for<32, T>(p, b, stream) : a == 64 ? launch_down_for<64, T>(p, b, stream) : launch_down_for<128, T>(p, b, stream);
+    return a == 32 ? launch_codes<32, T>(p, b, logits, stream) : a == 64 ? launch_codes<64, T>(p, b, logits, stream) : launch_codes<128, T>(p, b, logits, stream);
 }
 
 // ids null: they are found from the logits, and left, with the shares, at out_ids and out_shares where those are wanted.

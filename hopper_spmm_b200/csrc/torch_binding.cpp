@@ -649,7 +649,7 @@ PyObject *moe_layer(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
             if (!w || !is_16(*w) || w->dim() != 3 || w->size(0) != E || w->size(1) != rows[i] || w->size(2) != cols[i])
                 return refuse("gate_up must be [experts, 2 inner, hidden] and down [experts, hidden, inner], float16 or bfloat16");
             const int64_t ld = w->stride(1);
-            if ((cols[i] > 1 && w->stride(2) != 1) || ld < cols[i] || ld % 8 != 0 || (E > 1 && w->stride(0) != rows[i] * ld) || reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 != 0)
+            if ((cols[i] > 1 && w->stride(2) != 1) || ld < cols[i] || ld % 8 != 0 || ld > 1 << 28 || (E > 1 && w->stride(0) != rows[i] * ld) || reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 != 0)
                 return refuse("rows of 16-bit experts must start on 16 bytes, a multiple of 8 elements apart, and experts follow one another: pad the last dimension");
             joins(*w, true);
             (i ? m.down_16 : m.gate_up_16) = w->data_ptr();

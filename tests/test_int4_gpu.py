@@ -90,6 +90,12 @@ def test_strides_offsets_and_results(rows, cols, n, dtype):
     assert (room == -7).all()
 
 
+def test_columns_that_come_piece_by_piece_in_every_round():
+    # more tiles than a block has warps, and columns that do not fit as a whole
+    m, x = ref.matrix(148 * 16 * 17 + 3, 4100, 64, 1), normal(33, 4100, 2, F16)
+    ref.check_product(m.linear(x).t(), ref.values_of(m), x.double().t(), 64)
+
+
 def test_infinities_and_nan():
     m = ref.matrix(200, 300, 64, 1, BF16)
     s = m.scales

@@ -101,7 +101,8 @@ class Case:
 
 
 # experts, hidden, inner, chosen, tokens
-SIZES = [(4, 64, 40, 2, 1), (8, 256, 128, 3, 5), (10, 1000, 333, 4, 17), (64, 512, 96, 8, 3), (5, 130, 1000, 5, 40), (3, 2049, 64, 1, 9), (1, 72, 8, 1, 2), (300, 96, 24, 2, 33), (16, 4100, 70, 2, 12), (4, 48, 2500, 4, 70)]
+SIZES = [(4, 64, 40, 2, 1), (8, 256, 128, 3, 5), (10, 1000, 333, 4, 17), (64, 512, 96, 8, 3), (5, 130, 1000, 5, 40), (3, 2049, 64, 1, 9), (1, 72, 8, 1, 2), (300, 96, 24, 2, 33), (16, 4100, 70, 2, 12), (4, 48, 2500, 4, 70), (100, 64, 16, 6, 4),
+         (300, 64, 16, 3, 2)]
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
@@ -334,3 +335,48 @@ def test_a_decoding_step(n, dtype):
         g.replay()
     torch.cuda.synchronize()
     assert torch.equal(z2, z) and torch.equal(k2, h2)
+
+
+def test_sizes_that_no_block_has_room_for():
+    def weights(*shape):
+        return torch.zeros(*shape, dtype=F16, device="cuda")
+    for hidden, inner in ((120_000, 8), (16, 60_000)):
+        layer = hs.MoeLayer(weights(2, hidden), weights(2, 2 * inner, hidden), weights(2, hidden, inner), top_k=1)
+        with pytest.raises(capi.SpmmError) as e:
+            layer.forward(weights(3, hidden))
+        assert e.value.status == capi.ERR_UNSUPPORTED
+    # the largest that is promised, with as many pairs as there may be
+    layer = hs.MoeLayer(None, weights(1024, 16, 24_000), weights(1024, 24_000, 8), top_k=32)
+    ids = torch.zeros(256, 32, dtype=torch.int32, device="cuda")
+    assert not layer.experts(weights(256, 24_000), ids, torch.ones(256, 32, device="cuda")).any()
+    layer = hs.MoeLayer(None, weights(2, 24_000, 16), weights(2, 16, 12_000), top_k=32)
+    assert not layer.experts(weights(256, 16), ids, torch.ones(256, 32, device="cuda")).any()
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch, hopper_spmm_b200 as hs
+E4M3 = torch.float8_e4m3fn
+g0 = torch.Generator(device="cuda").manual_seed(1)
+def rand(*s): return torch.randn(*s, generator=g0, device="cuda").half() * 0.1
+x, w = rand(5, 256), rand(256)
+W = hs.Int4Matrix(256, 256, 64, values=torch.randint(0, 256, (256, 128), device="cuda", dtype=torch.uint8), scales=rand(4, 256).abs())
+layer = hs.MoeLayer(rand(4, 256), rand(4, 128, 256), rand(4, 256, 64), top_k=2)
+def step():
+    a = hs.rms_norm(x, w, dtype=E4M3, group=64)
+    y = W.linear(a, dtype=torch.float16)
+    return y, layer.forward(hs.rms_norm(y, w))
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
