@@ -7,6 +7,10 @@
 // (narrow.cuh).  A tile of the first product is 8 rows of the gate and the same 8 of up: both values of an inner value lie in one lane.  The second product's results are
 // left for each pair; a last kernel adds them up in the order of the token's choices.
 // The routing is cheap and needed by every block: each finds the runs for itself, from the logits, before its first tile.
+//
+// One token, 8 of 64 experts of 2048 x 1024 in bf16, 101 MB: 37 us for 15.4 at a copy's rate.  The experts' bytes come at 6.5 to 7 TB/s; the rest is what stands before them: four
+// launches, logits 3 us, the choice and its runs 5, the first copies 2 to 4.  Much of that is waiting for instructions that are run once and that the weights have pushed out of L2.
+// 8 tokens through 64 experts of 4096 x 2048 in 4 bits, 554 MB: 147 us for 85; 32 through 128, 1.1 GB: 304 for 172: the instructions that a step of codes takes, as in int4.cu.
 #include <type_traits>
 
 #include "entry.hpp"

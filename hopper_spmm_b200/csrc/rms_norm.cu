@@ -6,6 +6,10 @@
 // that, while its sum of squares and, for a scale of the whole row, its max |h w| are reduced together: y is the product of h w with one positive number,
 // so the largest |y| is the largest |h w| times it, and one reduction serves both.  Scales of groups of 32, 64 and 128 come from 4, 8 or 16 neighbouring lanes.
 // Rows longer than a block's registers (32,768 columns) are read a second time.
+//
+// 8192 x 8192 bf16 with a bf16 residual, to e4m3 with scales of 128: 80 us, 5.9 TB/s, 90 % of a copy's rate (104 before kernels were made for the weight's and the
+// result's type, 170 before all loads of a row came before the first use of one).  5001 x 4090, whose rows start on 4 bytes, with an fp32 residual and scales of 32: 61 us, 3.8 TB/s, issue: two
+// values an access, and a scale's arithmetic for each two of a lane.  8 x 8192: 2.8 us, a launch and one reduction.
 #include <type_traits>
 
 #include "entry.hpp"

@@ -56,7 +56,7 @@ class Int4Matrix:
 
     def linear(self, X, out=None, dtype=None, stream=None):
         """Y = X Wᵀ, [n, rows], for a few tokens that lie row by row: X [n, cols] float16 or bfloat16, or an Fp8Matrix.  Y in ``dtype`` (float32; with
-        ``out``, its type); sums in fp32.  The matrix is read once for every 32 rows of X.  Asynchronous; there is no gradient: X may not require one
+        ``out``, its type); sums in fp32.  The matrix is read once for every 40 rows of X.  Asynchronous; there is no gradient: X may not require one
         while gradients are recorded."""
         return self._product(X, out, dtype, stream, True)
 

@@ -614,7 +614,7 @@ typedef struct {
 } b200spmm_int4_t;
 
 /*
- * C[a.rows, n] = A B with few columns: A is read once for every 32.  B [a.cols, n] in fp16 or bf16, ldb elements between rows, or between columns where transposed; or in
+ * C[a.rows, n] = A B with few columns: A is read once for every 40.  B [a.cols, n] in fp16 or bf16, ldb elements between rows, or between columns where transposed; or in
  * e4m3 (transposed only), column j being value x b_scales[j, k / b_group], b_scales [n, groups of a column] contiguous and b_group 0 (one scale for a column) or 32, 64
  * or 128: what b200spmm_rms_norm writes.  b_scales and b_group are for e4m3 alone.  Sums in fp32, a
  * scale multiplying the sum over its group (an infinite one gives infinities or NaN); C as that of b200spmm_fp4_dense_product.
