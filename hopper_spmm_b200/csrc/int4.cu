@@ -7,8 +7,8 @@
 //
 // 28672 x 8192 in groups of 128 with zeros, 123 MB, 18.8 us at a copy's rate: one fp16 column 29.6 us, 8 in e4m3 36.  Of the 29.6 multiplying takes 21 (5.5 TB/s: 320 instructions
 // for a step of 16 rows x 256 codes fill what issue slots there are), from 3.2 us on, when the columns are there; 1,792 tiles are 12 for 132 blocks and 13 for 16, which end 2 to 4 us
-// after the others.  8 columns of 8,192 take half of the shared memory and 3 us longer to come.  14331 x 4090 in groups of 64 times 33 columns: 49 us, five MMAs for
-// each operand and columns that start on 4 bytes (61 in two reads of the matrix).
+// after the others.  8 columns of 8,192 take half of the shared memory and 3 us longer to come.  14331 x 4090 in groups of 64 times 33 columns: 41 us, five MMAs for
+// each operand and columns that start on 4 bytes (49 where they came value by value, 61 in two reads of the matrix).
 #include "entry.hpp"
 #include "fp4_store.cuh"
 #include "launch.hpp"
@@ -25,7 +25,7 @@ struct Int4Params {
     uint32_t rows, k, n;
     const void *x;
     int64_t along, across;
-    bool wide;
+    bool wide, even;
     const float *x_scales;
     uint32_t x_groups, x_shift;
     Target c;
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps<kNB>, 1) int4_kernel(const Int4
             if constexpr (kScaled)
                 stage_columns<W>(Eights{static_cast<const uint8_t *>(p.x) + (int64_t)j0 * p.across, p.across, p.wide, p.k}, c.base, c.pitch, first, count, c.n, false);
             else
-                stage_columns<W>(Plain<T>{static_cast<const T *>(p.x) + (int64_t)j0 * p.across, p.along, p.across, p.wide, p.k}, c.base, c.pitch, first, count, c.n, p.along != 1);
+                stage_columns<W>(Plain<T>{static_cast<const T *>(p.x) + (int64_t)j0 * p.across, p.along, p.across, p.wide, p.even, p.k}, c.base, c.pitch, first, count, c.n, p.along != 1);
         },
         [&](uint32_t tile, const float(&sums)[kNB][4]) {
             const uint32_t row = tile * kTileRows + g;
@@ -168,6 +168,7 @@ extern "C" int b200spmm_int4_product(const b200spmm_int4_t *a, const void *d_B, 
         p.across = b_transposed ? ldb : 1;
         const uint32_t unit = eights ? 8 : 16;
         p.wide = p.along == 1 && aligned(d_B, unit) && (n == 1 || p.across * (eights ? 1 : 2) % unit == 0);
+        p.even = !eights && p.along == 1 && aligned(d_B, 4) && (n == 1 || p.across % 2 == 0);
         p.x_scales = d_b_scales;
         p.x_groups = b_group ? (p.k + b_group - 1) / b_group : 1;
         p.x_shift = narrow::shift_of(b_group);

@@ -59,8 +59,8 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const MoeParams p
     __shared__ double shared[kLogitThreads / 32][kLogitTokens];
     ptx::wait_for_grids_before();
     const uint32_t e = blockIdx.x, t0 = blockIdx.y * kLogitTokens, n = min(kLogitTokens, p.tokens - t0), lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const Plain<T> w{static_cast<const T *>(p.router) + (int64_t)e * p.ld_router, 1, 0, p.router_wide, p.hidden};
-    const Plain<T> x{static_cast<const T *>(p.x) + (int64_t)t0 * p.ldx, 1, p.ldx, p.x_wide, p.hidden};
+    const Plain<T> w{static_cast<const T *>(p.router) + (int64_t)e * p.ld_router, 1, 0, p.router_wide, false, p.hidden};
+    const Plain<T> x{static_cast<const T *>(p.x) + (int64_t)t0 * p.ldx, 1, p.ldx, p.x_wide, false, p.hidden};
     double sum[kLogitTokens] = {};
     for (uint32_t u = threadIdx.x; u * 8u < p.hidden; u += kLogitThreads) {
         const uint4 a = w(0, u);
@@ -383,7 +383,7 @@ B200_DEVICE void gate_up_part(const MoeParams &p, const Routing &r, uint8_t *sme
         },
         [&](uint32_t first, uint32_t count) {
             if (p.all_tokens) return;
-            const Gathered<X> from{Plain<X>{static_cast<const X *>(p.x), 1, p.ldx, p.x_wide, p.hidden}, r.pairs + pair0, p.top};
+            const Gathered<X> from{Plain<X>{static_cast<const X *>(p.x), 1, p.ldx, p.x_wide, false, p.hidden}, r.pairs + pair0, p.top};
             if constexpr (kConvert) {
                 const Converted<Gathered<X>> to{from, tops};
                 find_tops(tops, n, count * W::kUnits, [&](uint32_t j, uint32_t u) { return to.top_of(j, u); });
@@ -412,7 +412,7 @@ template <class W, typename X>
 B200_DEVICE void stage_tokens(const MoeParams &p, uint8_t *smem, uint32_t columns_at) {
     const uint32_t steps = (p.hidden + W::kStep - 1) / W::kStep, pitch = column_pitch<W>(steps), at = ptx::smem_u32(smem) + columns_at;
     uint32_t *tops = reinterpret_cast<uint32_t *>(smem + columns_at + p.up_columns * pitch);
-    const Plain<X> from{static_cast<const X *>(p.x), 1, p.ldx, p.x_wide, p.hidden};
+    const Plain<X> from{static_cast<const X *>(p.x), 1, p.ldx, p.x_wide, false, p.hidden};
     if constexpr (!std::is_same<typename W::T, X>::value) {
         const Converted<Plain<X>> to{from, tops};
         find_tops(tops, p.tokens, steps * W::kUnits, [&](uint32_t j, uint32_t u) { return to.top_of(j, u); });

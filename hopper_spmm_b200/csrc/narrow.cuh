@@ -413,11 +413,16 @@ struct Plain {  // 16-bit values `along` elements apart along k, `across` betwee
     const T *x;
     int64_t along, across;
     bool wide;  // neighbours along k, and every column starts on 16 bytes
+    bool even;  // ... on 4
     uint32_t k;
     B200_DEVICE uint4 operator()(uint32_t j, uint32_t u) const {
         const T *p = x + (int64_t)j * across + (int64_t)u * 8 * along;
         const uint32_t left = u * 8u < k ? k - u * 8u : 0u;
         if (wide && left >= 8u) return *reinterpret_cast<const uint4 *>(p);
+        if (even && left >= 8u) {
+            const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
+            return make_uint4(q[0], q[1], q[2], q[3]);
+        }
         alignas(16) T v[8];
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) v[e] = e < left ? p[(int64_t)e * along] : fp4::Elem<T>::from_float(0.f);
