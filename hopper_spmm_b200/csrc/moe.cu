@@ -110,7 +110,7 @@ struct Routing {
     uint32_t *n_runs;
 };
 // (an expert with n pairs has at most n runs)
-__host__ __device__ inline uint32_t routing_bytes(uint32_t pairs, uint32_t experts) { return (12u * pairs + 2u * experts + 2u + 16u + 127u) / 128u * 128u; }
+__host__ __device__ constexpr uint32_t routing_bytes(uint32_t pairs, uint32_t experts) { return (12u * pairs + 2u * experts + 2u + 16u + 127u) / 128u * 128u; }
 B200_DEVICE Routing routing_at(uint8_t *at, uint32_t pairs, uint32_t experts) {
     Routing r;
     r.n_runs = reinterpret_cast<uint32_t *>(at);
@@ -635,6 +635,7 @@ Matrix plain_matrix(const void *values, int64_t ld, uint64_t cols) {
 // Columns that a block has room for, in `planes` parts.
 template <class W>
 uint32_t room_for(const MoeParams &p, uint32_t k, uint32_t planes) {
+    static_assert(kWarps * kRingBytes<W> + routing_bytes(kMaxTokens * kMaxTop, kMaxExperts) < kMaxSmem, "the largest routing has room beside the rings");
     const uint32_t taken = kWarps * kRingBytes<W> + routing_bytes(p.pairs, p.experts), steps = (k + W::kStep - 1) / W::kStep;
     const uint64_t each = (uint64_t)planes * ((uint64_t)steps * W::kUnits * 16u + 192u) + 4u;
     return (uint32_t)std::min<uint64_t>(p.pairs, (kMaxSmem - taken) / each);  // (as many as there are pairs at most)

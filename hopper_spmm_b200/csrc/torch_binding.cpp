@@ -16,6 +16,9 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <memory>
+#include <vector>
+
 #include "../../include/b200_spmm.h"
 
 namespace {
@@ -503,9 +506,29 @@ PyObject *rms_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
-// A matrix of 4-bit integers: what the C ABI gets of it, behind a capsule.  The tensors stay alive beside it.
+// A tensor whose address a capsule keeps.  What it was stays alive with it, so that nothing else can come to lie there; a call refuses one that has become another since
+// (`t.data = ...`, a module's `.to()`, `resize_`), or that has come to want a gradient.
+struct Held {
+    at::Tensor now, was;
+    const void *at;
+    explicit Held(const at::Tensor &t) : now(t), was(t.detach()), at(t.data_ptr()) {}
+    bool same() const { return now.data_ptr() == at && now.scalar_type() == was.scalar_type() && now.sizes() == was.sizes() && now.strides() == was.strides(); }
+};
+const char *fault_of(const std::vector<Held> &held) {
+    for (const Held &h : held) {
+        if (!h.same()) return "a tensor that was kept has another storage, type or shape now: make the matrix or the layer anew";
+        if (wants_gradient(h.now)) return kNoGradient;
+    }
+    return nullptr;
+}
+
+// A matrix of 4-bit integers: what the C ABI gets of it, behind a capsule.
 constexpr const char *kInt4 = "b200spmm_int4_t";
-void free_int4(PyObject *capsule) { delete static_cast<b200spmm_int4_t *>(PyCapsule_GetPointer(capsule, kInt4)); }
+struct Int4 {
+    b200spmm_int4_t m{};
+    std::vector<Held> held;
+};
+void free_int4(PyObject *capsule) { delete static_cast<Int4 *>(PyCapsule_GetPointer(capsule, kInt4)); }
 
 // int4_matrix(values, scales, zeros or None, rows, cols, group) -> capsule
 PyObject *int4_matrix(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
@@ -531,7 +554,8 @@ PyObject *int4_matrix(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     if (wants_gradient(*s)) return refuse(kNoGradient);
     if (s->device() != v->device() || (z && z->device() != v->device())) return refuse("values, scales and zeros must be on one device");
     if (!v->is_cuda()) return refuse("values, scales and zeros must be on a CUDA device");
-    auto *m = new b200spmm_int4_t{};
+    auto made = std::make_unique<Int4>();
+    b200spmm_int4_t *m = &made->m;
     m->rows = (uint64_t)rows;
     m->cols = (uint64_t)cols;
     m->group = (int32_t)group;
@@ -540,8 +564,10 @@ PyObject *int4_matrix(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     m->values = v->data_ptr();
     m->scales = s->data_ptr();
     m->zeros = z ? static_cast<const uint8_t *>(z->data_ptr()) : nullptr;
-    PyObject *out = PyCapsule_New(m, kInt4, free_int4);
-    if (!out) delete m;
+    made->held = {Held(*v), Held(*s)};
+    if (z) made->held.emplace_back(*z);
+    PyObject *out = PyCapsule_New(made.get(), kInt4, free_int4);
+    if (out) made.release();
     return out;
     END_HANDLE_TH_ERRORS
 }
@@ -554,9 +580,11 @@ PyObject *int4_product(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
         PyErr_SetString(PyExc_TypeError, "int4_product takes 7 arguments");
         return nullptr;
     }
-    const auto *a = static_cast<const b200spmm_int4_t *>(PyCapsule_GetPointer(args[0], kInt4));
+    const auto *matrix = static_cast<const Int4 *>(PyCapsule_GetPointer(args[0], kInt4));
     const long group = PyLong_AsLong(args[3]), type = PyLong_AsLong(args[5]);
     if (PyErr_Occurred()) return nullptr;
+    const b200spmm_int4_t *a = &matrix->m;
+    if (const char *fault = fault_of(matrix->held)) return refuse(fault);
     const bool first = args[6] == Py_True, eights = args[2] != Py_None;
     const at::Tensor *B = cuda_tensor(args[1]), *s = eights ? cuda_tensor(args[2]) : nullptr;
     Dense b;
@@ -566,9 +594,11 @@ PyObject *int4_product(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
         return refuse(eights ? "the 8-bit matrix must have the matrix's columns, on its device, with unit stride along its rows"
                              : first ? "X must be a CUDA float16 or bfloat16 tensor of shape [n, cols] on the matrix's device with unit stride along rows or columns"
                                      : "B must be a CUDA float16 or bfloat16 tensor of shape [cols, n] on the matrix's device with unit stride along rows or columns");
-    if (eights && (!s || s->get_device() != a->device)) return refuse("the 8-bit matrix's scales must be on the matrix's device");
-    if (wants_gradient(*B)) return refuse(kNoGradient);
     const int64_t n = B->size(lies_first ? 0 : 1);
+    if (eights && (!s || s->get_device() != a->device || s->scalar_type() != at::kFloat || (group != 0 && group != 32 && group != 64 && group != 128) || s->dim() != 2 || s->size(0) != n ||
+                   s->size(1) != (group ? ((int64_t)a->cols + group - 1) / group : 1) || !s->is_contiguous()))
+        return refuse("the 8-bit matrix's scales must be contiguous float32, [n, groups of a row], on the matrix's device");
+    if (wants_gradient(*B) || (s && wants_gradient(*s))) return refuse(kNoGradient);
     if (eights && b.transposed) b = {b.ptr, (int64_t)a->cols, false};  // (one row)
     at::Tensor C;
     Dense c;
@@ -590,6 +620,7 @@ constexpr const char *kMoe = "b200spmm_moe_t";
 struct Moe {
     b200spmm_moe_t m{};
     b200spmm_int4_t gate_up{}, down{};
+    std::vector<Held> held;
 };
 void free_moe(PyObject *capsule) { delete static_cast<Moe *>(PyCapsule_GetPointer(capsule, kMoe)); }
 
@@ -606,7 +637,8 @@ PyObject *moe_layer(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     if (H < 1 || I < 1 || H > 0x1000000 || I > 0x1000000) return refuse("the hidden and inner sizes must lie between 1 and 2^24");
     if (top < 1 || top > 32) return refuse("top_k must lie between 1 and 32");
     if (args[0] != Py_None && top > E) return refuse("top_k must not be above the number of experts");
-    Moe made;
+    auto layer = std::make_unique<Moe>();
+    Moe &made = *layer;
     b200spmm_moe_t &m = made.m;
     m.experts = (uint64_t)E;
     m.hidden = (uint64_t)H;
@@ -623,6 +655,7 @@ PyObject *moe_layer(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
         if (typed) m.dtype = type;
         m.device = device;
         lost = lost || wants_gradient(t);
+        made.held.emplace_back(t);
     };
     auto is_16 = [](const at::Tensor &t) { return (t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16) && t.layout() == at::kStrided && !t.is_neg(); };
     if (args[0] != Py_None) {
@@ -636,8 +669,10 @@ PyObject *moe_layer(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     }
     if (PyCapsule_IsValid(args[1], kInt4) != PyCapsule_IsValid(args[2], kInt4)) return refuse("gate_up and down must both be Int4Matrix, or both 16-bit tensors");
     if (PyCapsule_IsValid(args[1], kInt4)) {
-        made.gate_up = *static_cast<const b200spmm_int4_t *>(PyCapsule_GetPointer(args[1], kInt4));
-        made.down = *static_cast<const b200spmm_int4_t *>(PyCapsule_GetPointer(args[2], kInt4));
+        const auto *up = static_cast<const Int4 *>(PyCapsule_GetPointer(args[1], kInt4)), *down = static_cast<const Int4 *>(PyCapsule_GetPointer(args[2], kInt4));
+        made.gate_up = up->m;
+        made.down = down->m;
+        for (const Int4 *codes : {up, down}) made.held.insert(made.held.end(), codes->held.begin(), codes->held.end());
         if (made.gate_up.rows != (uint64_t)(E * 2 * I) || made.gate_up.cols != (uint64_t)H || made.down.rows != (uint64_t)(E * H) || made.down.cols != (uint64_t)I)
             return refuse("gate_up must have experts x 2 inner rows of the hidden size, down experts x hidden rows of the inner size");
         one_device = one_device && made.gate_up.device == made.down.device && (m.device == -1 || m.device == made.gate_up.device);
@@ -659,7 +694,9 @@ PyObject *moe_layer(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     if (lost) return refuse(kNoGradient);
     if (!one_type) return refuse("the router and 16-bit experts must have one type");
     if (!cuda || !one_device) return refuse("all parts of the layer must be on one CUDA device");
-    PyObject *out = PyCapsule_New(new Moe(made), kMoe, free_moe);
+    if (const char *fault = fault_of(made.held)) return refuse(fault);
+    PyObject *out = PyCapsule_New(layer.get(), kMoe, free_moe);
+    if (out) layer.release();
     return out;
     END_HANDLE_TH_ERRORS
 }
@@ -673,6 +710,7 @@ PyObject *moe(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     }
     const auto *layer = static_cast<const Moe *>(PyCapsule_GetPointer(args[0], kMoe));
     if (!layer) return nullptr;
+    if (const char *fault = fault_of(layer->held)) return refuse(fault);
     b200spmm_moe_t m = layer->m;
     const at::Tensor *X = cuda_tensor(args[1]);
     Rows x, y;

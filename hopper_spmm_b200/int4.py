@@ -19,7 +19,7 @@ class Int4Matrix:
     """A rows x cols matrix of 4-bit integers.  ``group``: neighbours of a row that share a scale, a power of two from 32 on, or None for a whole row.
     ``values`` uint8 [rows, pitch]: two codes from 0 to 15 to a byte, the lower half first, pitch 16 bytes for every 32 columns begun.  ``scales``
     float16 or bfloat16 [groups of a row, rows].  ``zeros`` uint8 [groups of a row, rows], 0 to 15; None: 8 everywhere.  All contiguous, on one CUDA
-    device; they are kept, not copied."""
+    device; they are kept, not copied: their values may change, and a call refuses them once they have another storage, type or shape."""
 
     __slots__ = ("rows", "cols", "group", "_arrays", "_m")
 

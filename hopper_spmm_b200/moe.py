@@ -21,7 +21,8 @@ class MoeLayer:
     ``router`` [experts, hidden], float16 or bfloat16: shares are the softmax of x routerᵀ, of the largest (of equal ones the first), divided by their sum where
     ``renormalize``.  None: for ``experts`` alone, whose number is then given where the matrices are Int4Matrix.
     ``gate_up``: [experts, 2 inner, hidden], the gate's rows before up's, and ``down`` [experts, hidden, inner], of the router's type, rows starting on 16
-    bytes; or Int4Matrix of experts * 2 * inner rows and of experts * hidden rows.  All are kept, not copied."""
+    bytes; or Int4Matrix of experts * 2 * inner rows and of experts * hidden rows.  All are kept, not copied: their
+    values may change, and a call refuses them once they have another storage, type or shape."""
 
     __slots__ = ("top_k", "renormalize", "_parts", "_m")
 

@@ -194,6 +194,51 @@ def test_refusals_on_the_gpu():
         hs.Int4Matrix(40, 64, 32, values=v, scales=s.cpu(), zeros=z)
 
 
+def test_scales_that_are_not_the_values_are_refused():
+    m, X = ref.matrix(40, 64, 32, 1), hs.rms_norm(normal(8, 64, 1, F16), dtype=E4M3, group=32)
+    scales = X.scales
+    for bad in (scales[:, :1].contiguous(), scales[:7], scales.half(), scales.t().contiguous().t(), scales.cpu(), scales[0], None):
+        X.scales = bad
+        with pytest.raises(ValueError, match="scales|X must"):
+            m.linear(X)
+    X.scales, X.group = scales, None
+    with pytest.raises(ValueError, match="scales"):
+        m.linear(X)
+    X.group, X.scales = 32, scales.clone().requires_grad_()
+    with pytest.raises(ValueError, match="no backward"):
+        m.linear(X)
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_kept_tensors_that_have_become_others_are_refused(which):
+    kept = ref.arrays(40, 64, 32, 1)
+    m, x = hs.Int4Matrix(40, 64, 32, values=kept[0], scales=kept[1], zeros=kept[2]), normal(8, 64, 1, F16)
+    want, t = m.linear(x), kept[which]
+    old = t.data
+    for new in (old.clone(), old.float(), old.t(), old[:1], old.cpu()):
+        t.data = new
+        with pytest.raises(ValueError, match="anew"):
+            m.linear(x)
+    t.data = old
+    assert torch.equal(m.linear(x), want)
+    t.mul_(1)  # (its values may change: they are read by every call)
+    assert torch.equal(m.linear(x), want)
+    t.resize_(4000, 1000)
+    with pytest.raises(ValueError, match="anew"):
+        m.linear(x)
+
+
+def test_kept_scales_that_come_to_want_a_gradient_are_refused():
+    kept = ref.arrays(40, 64, 32, 1)
+    m, x = hs.Int4Matrix(40, 64, 32, values=kept[0], scales=kept[1], zeros=kept[2]), normal(8, 64, 1, F16)
+    want = m.linear(x)
+    kept[1].requires_grad_()
+    with pytest.raises(ValueError, match="no backward"):
+        m.linear(x)
+    with torch.no_grad():
+        assert torch.equal(m.linear(x), want)
+
+
 def test_the_same_call_gives_the_same_bits_on_every_stream_and_in_graphs():
     m, x = ref.matrix(4000, 2048, 64, 1), normal(9, 2048, 2, BF16)
     X = hs.rms_norm(x, dtype=E4M3, group=64)

@@ -259,6 +259,26 @@ def test_refusals_on_the_gpu():
 
 
 @pytest.mark.parametrize("group", [0, 64], ids=str)
+def test_kept_tensors_that_have_become_others_are_refused(group):
+    c = Case(6, 128, 64, 2, F16, group)
+    x = tokens_of(4, 128, 2, F16)
+    want = c.layer.forward(x)
+    for t in c.layer._tensors():
+        old = t.data
+        for new in (old.clone(), old.float(), old.cpu(), old[:, :1]):  # (the first row of one is all of it)
+            t.data = new
+            with pytest.raises(ValueError, match="anew"):
+                c.layer.forward(x)
+        t.data = old
+        assert torch.equal(c.layer.forward(x), want)
+    c.router.requires_grad_()
+    with pytest.raises(ValueError, match="no backward"):
+        c.layer.forward(x)
+    with torch.no_grad():
+        assert torch.equal(c.layer.forward(x), want)
+
+
+@pytest.mark.parametrize("group", [0, 64], ids=str)
 def test_the_same_bits_on_every_stream_and_in_graphs(group):
     c = Case(16, 512, 256, 3, BF16, group)
     x = tokens_of(9, 512, 2, BF16)
