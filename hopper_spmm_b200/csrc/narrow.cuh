@@ -41,7 +41,7 @@ struct Matrix {
 
 // T: the type of the MMA's operands.  kSpan: columns of 4-bit integers that share their scales, 32, 64 or 128; 0: the weights are T themselves.  kPiece: bytes of a row in a
 // stage of the ring: 128 neighbouring bytes go to shared memory in one access where 64 and 64 take two; with 64 a lane of codes in spans of 128 reads what it copied itself and
-// the ring comes free sooner.  (Experts in 16 bits, one token 37.4 us with 64, 36.7 with 128; in 4 bits, 8 tokens 149 and 155.)
+// waits for nobody before it does.  (Experts in 16 bits, one token 37.4 us with 64, 36.7 with 128; in 4 bits, 8 tokens 149 and 155.)
 template <typename T_, int kSpan_>
 struct Weights {
     using T = T_;
@@ -332,7 +332,7 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, PlaceOf &&place_of, R
                     ld_shared<4 * kRegs>(from, w_lo);
                     ld_shared<4 * kRegs>(from + 8u * W::kPiece, w_hi);
                     if (in + 1u == W::kOfStage) {  // the stage is read: what comes kStages later may be copied there
-                        if (!kOwn) __syncwarp();
+                        __syncwarp();  // (where a lane read what it copied itself too: nothing else orders its loads before the bytes of a copy that it asks for next)
                         issue(at, b / W::kOfStage);
                         if (kStages != W::kPieces && b + 1 == W::kBlocks) here = 2u * s.ring + W::kPieces * W::kStageBytes - here;  // (the other step's)
                     }
