@@ -7,7 +7,8 @@
 //
 // Lane 4 g + t of a warp holds rows g and g + 8 of the tile.  Which values of k an operand position of the MMA stands for is free as long as both operands
 // agree, so a lane takes neighbours of its rows: of 4-bit integers kSpan / 4 of every kSpan, the widest span that has one scale (and one of the columns'
-// scales), whose sum is multiplied by them in fp32; of 16-bit values 8 of every 32.  Columns are stored in units of 8 values of k, in the order in which lanes
+// scales), whose sum is multiplied by them in fp32; of 16-bit values 8 of every 32, and
+// the sum over a step's 64 goes to one in fp32: the MMA cuts off what it adds up, a row of 24,000 in one accumulator was 2e-4 off.  Columns are stored in units of 8 values of k, in the order in which lanes
 // t = 0..3 read them side by side, each unit as the pairs that a mask takes out of a word of eight codes: 0 4, 1 5, 2 6, 3 7.
 //
 // What it spends its time on is instructions, not bytes: the same copies with nothing else take 19.7 us for 28672 x 8192 codes, 120 MB.
@@ -317,6 +318,7 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, PlaceOf &&place_of, R
                     fetch();
                 }
                 const uint32_t x_at = (step - first) * (W::kUnits * 16u);
+                float part[kNB][4];  // of a block of codes, or of a step of 16-bit weights
 #pragma unroll
                 for (uint32_t b = 0; b < W::kBlocks; ++b) {
                     constexpr uint32_t kRegs = W::kCodes ? W::kWords : 4u;
@@ -336,6 +338,10 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, PlaceOf &&place_of, R
                         issue(at, b / W::kOfStage);
                         if (kStages != W::kPieces && b + 1 == W::kBlocks) here = 2u * s.ring + W::kPieces * W::kStageBytes - here;  // (the other step's)
                     }
+                    if (W::kCodes || b == 0) {
+#pragma unroll
+                        for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) part[nb][0] = part[nb][1] = part[nb][2] = part[nb][3] = 0.f;
+                    }
                     if constexpr (!W::kCodes) {
 #pragma unroll
                         for (int plane = 0; plane < kPlanes; ++plane)
@@ -343,16 +349,19 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, PlaceOf &&place_of, R
                             for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
                                 uint4 &x = xs[(b + nb + plane) % 2u];
                                 column_unit(has[nb], column[nb] + x_at + b * 64u + plane * c.plane, x);
-                                fp4::mma_16x8x16<T>(sums[nb], w_lo[0], w_hi[0], w_lo[1], w_hi[1], x.x, x.y);
-                                fp4::mma_16x8x16<T>(sums[nb], w_lo[2], w_hi[2], w_lo[3], w_hi[3], x.z, x.w);
+                                fp4::mma_16x8x16<T>(part[nb], w_lo[0], w_hi[0], w_lo[1], w_hi[1], x.x, x.y);
+                                fp4::mma_16x8x16<T>(part[nb], w_lo[2], w_hi[2], w_lo[3], w_hi[3], x.z, x.w);
                             }
+                        if (b + 1u == W::kBlocks) {  // (the MMA cuts off what it adds up: a row's sum is rounded here instead)
+#pragma unroll
+                            for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
+#pragma unroll
+                                for (uint32_t e = 0; e < 4; ++e) sums[nb][e] += part[nb][e];
+                        }
                     } else {
                         const uint32_t source = (lane & ~3u) | (b & 1u) << 1;
                         const float s_lo = __shfl_sync(0xFFFFFFFFu, scale[b >> 1], source), s_hi = __shfl_sync(0xFFFFFFFFu, scale[b >> 1], source | 1u);
                         const Widen<T> widen_lo(__shfl_sync(0xFFFFFFFFu, minus[b >> 1], source)), widen_hi(__shfl_sync(0xFFFFFFFFu, minus[b >> 1], source | 1u));
-                        float part[kNB][4];
-#pragma unroll
-                        for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) part[nb][0] = part[nb][1] = part[nb][2] = part[nb][3] = 0.f;
 #pragma unroll
                         for (uint32_t w = 0; w < W::kWords; ++w) {
                             uint32_t a_lo[4], a_hi[4];

@@ -400,3 +400,38 @@ print("captured")
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=240)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+# ---------------------------------------------------------------- long rows
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
+@pytest.mark.parametrize("which", ["gate_up", "down"])
+def test_sums_of_16_bit_experts_over_long_rows_are_as_exact_as_over_short_ones(which, dtype):
+    # Two experts that give the same number: one from thousands of products 1 - 2^-14 = (1 + 2^-7) (1 - 2^-7), one from two terms.  The sum of 64 of them is a multiple of 2^-8 below 64, all sums
+    # of those are multiples of 2^-9 below 2^15: exact in fp32.  But a sum of the MMA that runs on through the row meets each product's 2^-14 with 28 digits.  A gate of 32 or more is its own SiLU;
+    # inner values are the same for both, or exact in 8 digits: the difference is zero.
+    # Two pairs have room in a block, so there are 256 runs, and 12 tiles in each: most warps have whole rows.
+    hidden, inner = (24_000, 96) if which == "gate_up" else (192, 12_000)
+    near = 1 + 2.0 ** -7
+    gate_up, down = torch.zeros(2, 2 * inner, hidden, dtype=dtype, device="cuda"), torch.zeros(2, hidden, inner, dtype=dtype, device="cuda")
+    gate_up[:, :inner, 0] = 32
+    if which == "gate_up":
+        x = torch.full((256, hidden), near, dtype=dtype, device="cuda")
+        gate_up[0, inner] = 1 - 2.0 ** -7
+        gate_up[1, inner, 1], gate_up[1, inner, 2] = 23808, 4.5  # 24,000 (1 - 2^-7)
+        down[:, 0, 0] = 1
+    else:
+        x = torch.ones(256, hidden, dtype=dtype, device="cuda")
+        gate_up[:, inner:, 0] = near
+        down[0, 0] = 1 - 2.0 ** -7
+        down[1, 0, 1], down[1, 0, 2] = 11904, 2.25
+    layer = hs.MoeLayer(None, gate_up, down, top_k=2)
+    ids, shares = torch.arange(2, device="cuda", dtype=torch.int32).repeat(256, 1), torch.zeros(256, 2, device="cuda")
+    shares[:, 0] = 1 / 16
+    total = (1 - 2.0 ** -14) * (24_000 * 32 * near if which == "gate_up" else 12_000 * 32) / 16
+    for one in (shares, shares.roll(1, 1)):
+        y = layer.experts(x, ids, one)
+        # (h and its two parts are off by 2^-16 at most, where they do not cancel)
+        assert (y[:, 0].double() - total).abs().max() <= total * (EPS[dtype] + 2.0 ** -16) and not y[:, 1:].any()
+    shares[:, 1] = -1 / 16
+    assert not layer.experts(x, ids, shares).any()
