@@ -660,11 +660,11 @@ int launch_all(MoeParams p, double *logits, cudaStream_t stream) {
     B200_CUDA_TRY(launch_after(sum_kernel, dim3((p.hidden + kSumThreads - 1) / kSumThreads, p.tokens), kSumThreads, 0, 1, stream, p));
     return B200SPMM_OK;
 }
-// Inner values beside codes: 22 digits where y is fp16; 11 where it is bf16, with 8 of its own.
+// Inner values beside codes have 22 digits, for bf16 too: with 11 they are the largest error of a layer before its result is rounded.
 template <int kUp, typename X>
 int launch_codes(const MoeParams &p, uint32_t span, double *logits, cudaStream_t stream) {
     using Up = Weights<__half, kUp>;
-    constexpr int kPlanes = std::is_same<X, __half>::value ? 2 : 1;
+    constexpr int kPlanes = 2;
     return span == 32   ? launch_all<Up, X, Weights<__half, 32>, kPlanes>(p, logits, stream)
            : span == 64 ? launch_all<Up, X, Weights<__half, 64>, kPlanes>(p, logits, stream)
                         : launch_all<Up, X, Weights<__half, 128>, kPlanes>(p, logits, stream);

@@ -629,7 +629,7 @@ int b200spmm_int4_product(const b200spmm_int4_t *a, const void *d_B, int64_t ldb
  * x, y and the router have one type, fp16 or bf16.  Experts: experts x 2 inner rows of `hidden` columns (for each expert first the gate's rows, then up's) and experts x hidden rows
  * of `inner` columns, one after the other: in 4-bit integers (gate_up, down), or in x's type (gate_up_16, down_16, rows ld elements apart, a multiple of 8, 16-byte
  * aligned), the others null.  Logits are added up in 64 bits; the inner values are kept in 32 and multiplied as the sum of two 16-bit
- * numbers, by codes and for bf16 as one of fp16 (11 digits), scaled by powers of two.
+ * numbers: of x's type with 16-bit experts (22 digits in fp16, 16 in bf16), by codes of fp16, scaled by powers of two.
  * experts up to 1024, top_k up to 32; hidden and inner as far as a block's shared memory holds a column beside the routing (else B200SPMM_ERR_UNSUPPORTED):
  * 24,000 and 12,000 always, three times that with few tokens.  A row of x with NaN gives NaN in its own row of y alone.
  */

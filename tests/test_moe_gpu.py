@@ -435,3 +435,39 @@ def test_sums_of_16_bit_experts_over_long_rows_are_as_exact_as_over_short_ones(w
         assert (y[:, 0].double() - total).abs().max() <= total * (EPS[dtype] + 2.0 ** -16) and not y[:, 1:].any()
     shares[:, 1] = -1 / 16
     assert not layer.experts(x, ids, shares).any()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128], ids=str)
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
+def test_inner_values_beside_codes_have_22_digits(dtype, group):
+    # Two experts that differ in up's scales by a 128th, one taken from the other: what is left shows roundings of inner values that a layer's own result would hide.
+    H, I = 128, 24
+    c = Case(2, H, I, 2, dtype, group)
+    for m, rows in ((c.gate_up, 2 * I), (c.down, H)):
+        m.values[rows:] = m.values[:rows]
+        m.zeros[:, rows:] = m.zeros[:, :rows]
+        m.scales[:, rows:] = m.scales[:, :rows]
+    c.gate_up.scales[:, 3 * I:] *= 1 + 2.0 ** -7
+    x = rand(20, H, seed=2, dtype=dtype)
+    ids, shares = torch.arange(2, device="cuda").repeat(20, 1), torch.tensor([1.0, -1.0], device="cuda").repeat(20, 1)
+    y = c.layer.experts(x, ids, shares).double()
+    want = bound = 0
+    for e in range(2):
+        # as Case.check, with 2^-22 of an inner value and 2^-38 of a token's largest for its two parts; the gates are the same, and so is what they are off
+        gate_up, down = c.expert(e)
+        (g, u), (_, mu) = (x.double() @ gate_up.t()).split(I, 1), (x.double().abs() @ gate_up.abs().t()).split(I, 1)
+        off = group / 16 * 2.0 ** -22 + (-(-H // group) + 24 + 2) * 2.0 ** -24
+        silu = g * torch.sigmoid(g)
+        h = silu * u
+        dh = silu.abs() * (mu * off + x.double().abs().amax(1, keepdim=True) * gate_up.abs().sum(1)[I:] * 2.0 ** -39)
+        dh = dh + h.abs() * (2.0 ** -22 + 2.0 ** -23) + h.abs().amax(1, keepdim=True) * 2.0 ** -38
+        want = want + (1 - 2 * e) * (h @ down.t())
+        bound = bound + dh @ down.abs().t() + h.abs() @ down.abs().t() * (2 * group / 16 * 2.0 ** -22 + 27 * 2.0 ** -24)
+    gate_up, down = c.expert(0)
+    # (the gates' own error, and the exponential's, are those of the difference)
+    g, mg = x.double() @ gate_up[:I].t(), x.double().abs() @ gate_up[:I].abs().t()
+    du = (x.double() @ (gate_up[I:] - c.expert(1)[0][I:]).t()).abs()
+    bound = bound + (du * (1.1 * mg * 2.0 ** -18 + (g * torch.sigmoid(g)).abs() * 2.0 ** -20)) @ down.abs().t()
+    bound = bound + (want.abs() + bound) * EPS[dtype] + TINY[dtype]
+    worst = ((y - want).abs() / bound).max().item()
+    assert worst <= 1, f"{worst:.2f} times the bound"
