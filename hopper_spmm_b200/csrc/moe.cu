@@ -52,7 +52,8 @@ struct MoeParams {
     float *parts;          // [pairs][hidden]
 };
 
-// ------------------------------------------------------------------ logits, in 64 bits: products of 16-bit numbers are exact in fp32, eight of them are added there
+// ------------------------------------------------------------------ logits, in 64 bits: products of 16-bit numbers are exact there, and beyond fp32's range (in fp32, eight at a time, a small
+// term beside two large ones that cancel was lost, and the experts whose logits it told apart were exchanged; bf16's largest products were infinite)
 
 template <typename T>
 __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const MoeParams p, double *logits) {
@@ -71,10 +72,8 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const MoeParams p
 #pragma unroll
         for (uint32_t j = 0; j < kLogitTokens; ++j) {
             if (j >= n) break;
-            float s = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s = fmaf(fp4::Elem<T>::to_float(reinterpret_cast<const T *>(&a)[i]), fp4::Elem<T>::to_float(reinterpret_cast<const T *>(&b[j])[i]), s);
-            sum[j] += (double)s;
+            for (int i = 0; i < 8; ++i) sum[j] = fma((double)fp4::Elem<T>::to_float(reinterpret_cast<const T *>(&a)[i]), (double)fp4::Elem<T>::to_float(reinterpret_cast<const T *>(&b[j])[i]), sum[j]);
         }
     }
 #pragma unroll

@@ -471,3 +471,42 @@ def test_inner_values_beside_codes_have_22_digits(dtype, group):
     bound = bound + (want.abs() + bound) * EPS[dtype] + TINY[dtype]
     worst = ((y - want).abs() / bound).max().item()
     assert worst <= 1, f"{worst:.2f} times the bound"
+
+
+# ---------------------------------------------------------------- logits
+
+@pytest.mark.parametrize("tokens", [1, 3, 9])
+@pytest.mark.parametrize("experts", [40, 100, 200, 500])  # each way of choosing
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
+def test_experts_are_told_apart_by_small_terms_beside_large_ones_that_cancel(dtype, experts, tokens):
+    # Products of 2^14 and -2^14 in every eight of the row, and 2^-12 times whole numbers beside them: exact in 64 bits in any order, while in fp32 neighbours of 2^14 are 2^-10 apart.
+    H = 512
+    rank = torch.randperm(experts, generator=torch.Generator(device="cuda").manual_seed(experts), device="cuda")
+    router = torch.zeros(experts, H, dtype=dtype, device="cuda")
+    router[:, 0::8], router[:, 7::8] = 1, -1
+    router[:, 3] = (rank % 8).to(dtype) * 2.0 ** -6
+    router[:, 460] = (rank // 8).to(dtype) * 2.0 ** -3  # (up to 63)
+    x = torch.zeros(tokens, H, dtype=dtype, device="cuda")
+    x[:, 0::8] = x[:, 7::8] = 2.0 ** 14
+    x[:, 3] = x[:, 460] = 2.0 ** -6
+    layer = hs.MoeLayer(router, torch.zeros(experts, 16, H, dtype=dtype, device="cuda"), torch.zeros(experts, H, 8, dtype=dtype, device="cuda"), top_k=20)
+    _, ids, shares = layer.forward(x, return_routing=True)
+    logits = x.double() @ router.double().t()
+    want = rank.argsort(descending=True)[:20]
+    assert torch.equal(logits[0], rank.double() * 2.0 ** -12) and (ids == want).all()
+    want = torch.softmax(logits.gather(1, ids.long()), 1)
+    # each exponential is off by the 2 units of its last place that expf may be, the sum by 5 roundings, the quotient by one; the difference of two logits is exact in fp32
+    assert ((shares.double() / want - 1).abs() <= 2 * 2.0 ** -22 + 6 * 2.0 ** -24).all()
+
+
+def test_logits_beyond_the_range_of_32_bits():
+    # products of 2^140, which are no infinities in 64 bits, beside ones of 2^90, which there are within their 53 digits
+    router, x = torch.zeros(6, 64, dtype=BF16, device="cuda"), torch.zeros(2, 64, dtype=BF16, device="cuda")
+    router[:, 5] = router[:, 11] = 2.0 ** 70
+    router[:, 7] = torch.tensor([3, 1, 4, 1, 5, 9], device="cuda") * 2.0 ** 45
+    router[3, 11] = 2.0 ** 71
+    x[:, 5], x[:, 11], x[:, 7] = 2.0 ** 70, -2.0 ** 70, 2.0 ** 45
+    layer = hs.MoeLayer(router, torch.zeros(6, 16, 64, dtype=BF16, device="cuda"), torch.zeros(6, 64, 8, dtype=BF16, device="cuda"), top_k=6)
+    _, ids, shares = layer.forward(x, return_routing=True)
+    assert ids.tolist() == [[5, 4, 2, 0, 1, 3]] * 2  # (the last one's logit is -2^140)
+    assert shares.tolist() == [[1, 0, 0, 0, 0, 0]] * 2
