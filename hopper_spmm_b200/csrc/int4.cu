@@ -30,6 +30,7 @@ struct Int4Params {
     uint32_t x_groups, x_shift;
     Target c;
     uint32_t tiles, warps, steps, window, cols;  // of all blocks together; of a block; of a row; that the columns have room for; of a pass, at most
+    uint32_t scales;  // of a column, in a window
 };
 
 template <int kNB>
@@ -64,22 +65,23 @@ __global__ void __launch_bounds__(32 * kMaxWarps<kNB>, 1) int4_kernel(const Int4
     c.plane = 0;
     c.n = min(8u * kNB, p.n - j0);
     c.scales = c.base + p.cols * c.pitch;
-    c.groups = p.x_groups;
+    c.groups = p.scales;
     c.shift = p.x_shift;
     const uint32_t begin = (uint32_t)((uint64_t)p.tiles * blockIdx.x / gridDim.x), end = (uint32_t)((uint64_t)p.tiles * (blockIdx.x + 1u) / gridDim.x);
     const Split split(end - begin, p.steps, p.warps);
     const Share s(split, begin, end, warp, p.steps, p.window, base + warp * ring_bytes);
     ptx::wait_for_grids_before();
-    if constexpr (kScaled) {
-        float *to = reinterpret_cast<float *>(smem + (c.scales - base));
-        for (uint32_t i = threadIdx.x; i < c.n * p.x_groups; i += blockDim.x) to[i] = p.x_scales[(uint64_t)j0 * p.x_groups + i];
-    }
     multiply<W, kNB, 1, kScaled, kRing>(
         p.m, s, [](uint32_t tile) { return tile; }, [&](uint32_t tile, uint32_t r) { return (uint64_t)min(tile * kTileRows + r, p.rows - 1u); }, [&](uint32_t) { return c; },
         [&](uint32_t first, uint32_t count) {
-            if constexpr (kScaled)
+            if constexpr (kScaled) {
+                // a warp takes a column's; behind a row's end the last one again
+                float *to = reinterpret_cast<float *>(smem + (c.scales - base));
+                const uint32_t group = (uint32_t)((uint64_t)first * W::kStep >> p.x_shift);
+                for (uint32_t j = threadIdx.x >> 5; j < c.n; j += blockDim.x >> 5)
+                    for (uint32_t i = threadIdx.x & 31u; i < p.scales; i += 32u) to[j * p.scales + i] = p.x_scales[(uint64_t)(j0 + j) * p.x_groups + min(group + i, p.x_groups - 1u)];
                 stage_columns<W>(Eights{static_cast<const uint8_t *>(p.x) + (int64_t)j0 * p.across, p.across, p.wide, p.k}, c.base, c.pitch, first, count, c.n, false);
-            else
+            } else
                 stage_columns<W>(Plain<T>{static_cast<const T *>(p.x) + (int64_t)j0 * p.across, p.along, p.across, p.wide, p.even, p.k}, c.base, c.pitch, first, count, c.n, p.along != 1);
         },
         [&](uint32_t tile, const float(&sums)[kNB][4]) {
@@ -99,12 +101,14 @@ int launch(Int4Params p, cudaStream_t stream) {
     p.cols = std::min<uint32_t>(8 * kNB, p.n);
     const Split split((p.tiles + blocks - 1) / blocks, p.steps, kMaxWarps<kNB>);
     p.warps = split.at_once * split.slices;
-    // the columns as a whole, or as much of them as there is room for
-    const uint64_t taken = (uint64_t)p.warps * kRingOf<W, kNB, kRing> + (kScaled ? (uint64_t)p.cols * p.x_groups * 4u : 0u);
-    p.window = steps_that_fit<W>(p.steps, p.cols, 1, taken);
+    // the columns as a whole, or as much of them as there is room for, with their scales: one of a column, or of every group
+    const bool of_column = p.x_shift == kWholeGroup;
+    const uint32_t ring = p.warps * kRingOf<W, kNB, kRing>, of_step = kScaled && !of_column ? W::kStep >> p.x_shift : 0u;
+    p.window = steps_that_fit<W>(p.steps, p.cols, of_step * 4u, ring + (kScaled && of_column ? p.cols * 4u : 0u));
     if (kRing == 4 && p.window < p.steps) return launch<T, kSpan, kNB, kScaled, 2>(p, stream);  // (half the ring, more room)
     if (p.window == 0) return B200SPMM_ERR_UNSUPPORTED;
-    const uint32_t bytes = (uint32_t)taken + p.cols * column_pitch<W>(p.window);
+    p.scales = of_column ? 1u : of_step * p.window;
+    const uint32_t bytes = ring + p.cols * (column_pitch<W>(p.window) + (kScaled ? p.scales * 4u : 0u));
     static std::atomic<uint64_t> allowed{0};
     B200_CUDA_TRY(allow_smem(kernel, allowed));
     B200_CUDA_TRY(launch_after(kernel, dim3(blocks, passes), 32u * p.warps, bytes, 1, stream, p));

@@ -45,13 +45,14 @@ inline Matrix matrix_of(const b200spmm_int4_t *m) {
     return out;
 }
 
-// How many of `steps` of `cols` columns, in `planes` parts, there is room for beside `taken` bytes of a block's shared memory.
+// How many of `steps` of `cols` columns there is room for beside `taken` bytes of a block's shared memory; a column has `scales` bytes of them for each step.
 template <class W>
-uint32_t steps_that_fit(uint32_t steps, uint32_t cols, uint32_t planes, uint64_t taken) {
+uint32_t steps_that_fit(uint32_t steps, uint32_t cols, uint32_t scales, uint64_t taken) {
+    static_assert(W::kUnits * 16u % 128u == 0, "a column's steps are multiples of what it is rounded up to");
     if (taken >= kMaxSmem) return 0;
-    const uint64_t pitch = (kMaxSmem - taken) / (cols * planes);  // bytes that a column may take
-    if (pitch < column_pitch<W>(1)) return 0;
-    return (uint32_t)std::min<uint64_t>((pitch - 64) / 128 * 128 / (W::kUnits * 16u), steps);
+    const uint64_t room = (kMaxSmem - taken) / cols;  // bytes that a column may take
+    if (room < column_pitch<W>(0)) return 0;
+    return (uint32_t)std::min<uint64_t>((room - column_pitch<W>(0)) / (W::kUnits * 16u + scales), steps);
 }
 
 // Lets a kernel have so much shared memory, once for each device; `allowed` keeps which.

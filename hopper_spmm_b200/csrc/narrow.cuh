@@ -134,7 +134,8 @@ struct Widen<__nv_bfloat16> {
     }
 };
 
-// The columns of a tile in shared memory: column j at base + j * pitch (and `plane` further on its second part, where it is the sum of two), and their scales.
+// The columns of a tile in shared memory: column j at base + j * pitch (and `plane` further on its second part, where it is the sum of two), and their scales, `groups` of each: of the
+// steps that are there, which begin with a group.
 struct Columns {
     uint32_t base, pitch, plane, n;
     uint32_t scales, groups, shift;
@@ -381,7 +382,7 @@ B200_DEVICE void multiply(const Matrix &m, const Share &s, PlaceOf &&place_of, R
                         for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb) {
                             float x0 = 1.f, x1 = 1.f;
                             if constexpr (kScaled) {
-                                const uint32_t group = min((step * W::kStep + b * (uint32_t)W::kSpan) >> c.shift, c.groups - 1u), j = nb * 8u + t * 2u;
+                                const uint32_t group = ((step - first) * W::kStep + b * (uint32_t)W::kSpan) >> c.shift, j = nb * 8u + t * 2u;
                                 x0 = __uint_as_float(ptx::ld_shared_u32(c.scales + (min(j, c.n - 1u) * c.groups + group) * 4u));
                                 x1 = __uint_as_float(ptx::ld_shared_u32(c.scales + (min(j + 1u, c.n - 1u) * c.groups + group) * 4u));
                             }

@@ -277,3 +277,19 @@ def test_the_matrix_is_that_of_its_arrays():
     m.zeros.copy_(z)
     ref.check_product(m.linear(x).t(), ref.values_of(m), x.double().t(), 32)
     assert m.nbytes == v.numel() + 2 * s.numel() + z.numel() and m.device == v.device
+
+
+# columns whose scales as a whole leave no room for a step of them (a column of 53,248 with scales of 32 has 6.6 KB of them); more tiles than a block has warps, with columns and scales that
+# come piece by piece in every round
+@pytest.mark.parametrize("rows,cols,n,group,x_group", [(40, 53_248, 33, 64, 32), (50, 53_248, 40, 128, 32), (33, 53_250, 80, 32, 32), (40, 65_536, 24, 128, 32), (20, 200_001, 8, None, 32),
+                                                       (20, 131_072, 16, 64, 32), (40, 100_000, 40, 128, 64), (40, 100_100, 40, 128, None), (148 * 16 * 17 + 3, 4100, 33, 64, 32)])
+def test_long_columns_in_8_bits(rows, cols, n, group, x_group):
+    m = ref.matrix(rows, cols, group, rows + n)
+    X = hs.rms_norm(normal(n, cols, 3, BF16), dtype=E4M3, group=x_group)
+    x = X.values.double() * X.scales.double().repeat_interleave(x_group or cols, 1)[:, :cols]
+    y = m.linear(X)
+    ref.check_product(y.t(), ref.values_of(m), x.t(), span(m, x_group))
+    # one column at a time has all its scales beside it
+    for j in (0, n - 1):
+        one = hs.Fp8Matrix(X.values[j:j + 1], X.scales[j:j + 1], x_group)
+        ref.check_product(m.linear(one).t(), ref.values_of(m), x[j:j + 1].t(), span(m, x_group))
