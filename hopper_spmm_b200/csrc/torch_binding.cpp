@@ -10,6 +10,7 @@
 #define HAS_EMPTY_CUDA 1
 #endif
 #include <ATen/record_function.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAStream.h>
 #include <ATen/core/grad_mode.h>
@@ -372,9 +373,11 @@ PyObject *fp4_dense_product(PyObject *, PyObject *const *args, Py_ssize_t n_args
 
 // ---- around weights in few bits
 
-// Whether a gradient would be lost: the tensor wants one and gradients are recorded.
-bool wants_gradient(const at::Tensor &t) { return t.requires_grad() && at::GradMode::is_enabled(); }
-constexpr const char *kNoGradient = "there is no backward pass: call it under torch.no_grad(), or with tensors that require no gradient";
+// Whether a gradient would be lost: the tensor wants one and gradients are recorded, or it has a tangent and those are taken along.
+bool wants_gradient(const at::Tensor &t) {
+    return (t.requires_grad() && at::GradMode::is_enabled()) || (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode());
+}
+constexpr const char *kNoGradient = "there is no backward pass, nor a forward-mode one: call it under torch.no_grad(), or with tensors that require no gradient and have no tangent";
 
 // Rows of neighbours: the address and the distance of rows, in elements.
 struct Rows {

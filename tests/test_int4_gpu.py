@@ -293,3 +293,21 @@ def test_long_columns_in_8_bits(rows, cols, n, group, x_group):
     for j in (0, n - 1):
         one = hs.Fp8Matrix(X.values[j:j + 1], X.scales[j:j + 1], x_group)
         ref.check_product(m.linear(one).t(), ref.values_of(m), x[j:j + 1].t(), span(m, x_group))
+
+
+# ---------------------------------------------------------------- what autograd is told
+
+def test_tangents_are_refused():
+    from torch.autograd import forward_ad
+    m, x = ref.matrix(40, 64, 32, 1), normal(8, 64, 1, F16)
+    X = hs.rms_norm(x, dtype=E4M3, group=32)
+    v, s, z = ref.arrays(40, 64, 32, 1)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        of_dual = hs.Fp8Matrix(X.values, X.scales, 32)
+        of_dual.scales = dual(X.scales)
+        for call in (lambda: m.linear(dual(x)), lambda: m.matmul(dual(x.t())), lambda: m.linear(of_dual), lambda: m.linear(x, dual(torch.empty(8, 40, device="cuda"))),
+                     lambda: hs.Int4Matrix(40, 64, 32, values=v, scales=dual(s), zeros=z)):
+            with pytest.raises(ValueError, match="no backward"):
+                call()

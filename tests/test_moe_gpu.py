@@ -510,3 +510,22 @@ def test_logits_beyond_the_range_of_32_bits():
     _, ids, shares = layer.forward(x, return_routing=True)
     assert ids.tolist() == [[5, 4, 2, 0, 1, 3]] * 2  # (the last one's logit is -2^140)
     assert shares.tolist() == [[1, 0, 0, 0, 0, 0]] * 2
+
+
+# ---------------------------------------------------------------- what autograd is told
+
+@pytest.mark.parametrize("group", [0, 64], ids=str)
+def test_tangents_are_refused(group):
+    from torch.autograd import forward_ad
+    c = Case(6, 128, 64, 2, F16, group)
+    x, ids, shares = tokens_of(4, 128, 2, F16), torch.zeros(4, 2, dtype=torch.int32, device="cuda"), torch.ones(4, 2, device="cuda")
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: c.layer.forward(dual(x)), lambda: c.layer.experts(x, ids, dual(shares)), lambda: c.layer.forward(x, dual(x.clone())),
+                     lambda: hs.MoeLayer(dual(c.router), c.gate_up, c.down, top_k=2)):
+            with pytest.raises(ValueError, match="no backward"):
+                call()
+        if not group:
+            with pytest.raises(ValueError, match="no backward"):
+                hs.MoeLayer(c.router, c.gate_up, dual(c.down), top_k=2)

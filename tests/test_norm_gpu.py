@@ -253,3 +253,21 @@ def test_streams_and_graphs():
         for g, out in graphs:
             for a, b in zip(out, want):
                 assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- what autograd is told
+
+def test_tangents_are_refused():
+    from torch.autograd import forward_ad
+    x, w, r = normal(4, 64, 1), torch.ones(64, device="cuda"), normal(4, 64, 2)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: hs.rms_norm(dual(x), w), lambda: hs.rms_norm(x, dual(w)), lambda: hs.rms_norm(x, w, residual=dual(r)), lambda: hs.rms_norm(x, w, out=dual(x.clone())),
+                     lambda: hs.rms_norm(x, w, residual=r, sum_out=dual(r.clone()))):
+            with pytest.raises(ValueError, match="no backward"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="no backward"):  # (it takes tangents along)
+                call()
+        check_values(hs.rms_norm(forward_ad.unpack_dual(dual(x)).primal, w), reference(x, w, 1e-6))
+    check_values(hs.rms_norm(x, w), reference(x, w, 1e-6))
