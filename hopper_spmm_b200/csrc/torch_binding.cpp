@@ -285,9 +285,18 @@ at::Tensor product_workspace(const b200spmm_fp4_t &a, const Dense *b, int64_t n,
     return new_cuda({(int64_t)*bytes}, at::kByte, like);
 }
 
+// Autograd is told that a caller's tensor has other values now: what saved it for a backward pass must not use it any more.
+void written(const at::Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written(PyObject *arg) {
+    if (arg != Py_None) written(THPVariable_Unpack(arg));
+}
+
 PyObject *result_of(int st, PyObject *arg, at::Tensor &&C) {
     if (st != B200SPMM_OK) return PyLong_FromLong(st);
     if (arg != Py_None) {
+        written(C);
         Py_INCREF(arg);
         return arg;
     }
@@ -502,6 +511,8 @@ PyObject *rms_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
         st = b200spmm_rms_norm(&p, stream);
     }
     if (st != B200SPMM_OK) return three(PyLong_FromLong(st), again(Py_None), again(Py_None));
+    for (int i : {4, 5}) written(args[i]);
+    if (e4m3 && args[5] != Py_None) written(args[6]);
     PyObject *a = out.defined() ? THPVariable_Wrap(std::move(out)) : again(args[5]);
     PyObject *b = scales.defined() ? THPVariable_Wrap(std::move(scales)) : again(Py_None);
     PyObject *c = sum.defined() ? THPVariable_Wrap(std::move(sum)) : again(args[4]);
@@ -770,6 +781,7 @@ PyObject *moe(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
                    : b200spmm_moe(&m, x.ptr, x.ld, tokens, y.ptr, y.ld, i, s, ws, bytes, stream);
     }
     if (st != B200SPMM_OK) return three(PyLong_FromLong(st), again(Py_None), again(Py_None));
+    written(args[2]);
     PyObject *a = Y.defined() ? THPVariable_Wrap(std::move(Y)) : again(args[2]);
     PyObject *b = routing ? THPVariable_Wrap(std::move(new_ids)) : again(Py_None), *c = routing ? THPVariable_Wrap(std::move(new_shares)) : again(Py_None);
     return three(a, b, c);

@@ -311,3 +311,16 @@ def test_tangents_are_refused():
                      lambda: hs.Int4Matrix(40, 64, 32, values=v, scales=dual(s), zeros=z)):
             with pytest.raises(ValueError, match="no backward"):
                 call()
+
+
+def test_autograd_is_told_of_results_that_are_written_in_place():
+    m, x = ref.matrix(40, 64, 32, 1), normal(8, 64, 1, F16)
+    for call, shape in ((m.linear, (8, 40)), (lambda x, y: m.matmul(x.t(), y), (40, 8))):
+        y = torch.zeros(shape, device="cuda")
+        loss = (torch.ones(shape, device="cuda", requires_grad=True) * y).sum()
+        assert call(x, y) is y
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        before = x._version, y._version
+        call(x, y)
+        assert (x._version, y._version) == (before[0], before[1] + 1)

@@ -529,3 +529,18 @@ def test_tangents_are_refused(group):
         if not group:
             with pytest.raises(ValueError, match="no backward"):
                 hs.MoeLayer(c.router, c.gate_up, dual(c.down), top_k=2)
+
+
+def test_autograd_is_told_of_results_that_are_written_in_place():
+    c = Case(6, 128, 64, 2, F16)
+    x = tokens_of(4, 128, 2, F16)
+    _, ids, shares = c.layer.forward(x, return_routing=True)
+    for call in (c.layer.forward, lambda x, y: c.layer.experts(x, ids, shares, y)):
+        y = torch.zeros_like(x)
+        loss = (torch.ones_like(x, requires_grad=True) * y).sum()
+        assert call(x, y) is y
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        before = x._version, y._version, ids._version, shares._version
+        call(x, y)
+        assert (x._version, y._version, ids._version, shares._version) == (before[0], before[1] + 1, *before[2:])

@@ -271,3 +271,32 @@ def test_tangents_are_refused():
                 call()
         check_values(hs.rms_norm(forward_ad.unpack_dual(dual(x)).primal, w), reference(x, w, 1e-6))
     check_values(hs.rms_norm(x, w), reference(x, w, 1e-6))
+
+
+def saved_by(t):
+    """A loss whose backward pass needs t."""
+    return (torch.ones(t.shape, dtype=t.dtype, device=t.device, requires_grad=True) * t).sum()
+
+
+def test_autograd_is_told_of_results_that_are_written_in_place():
+    x, r, w = normal(4, 64, 1), normal(4, 64, 2), torch.ones(64, device="cuda")
+    losses = saved_by(x), saved_by(r)
+    hs.rms_norm(x, w, residual=r, sum_out=r, out=x)
+    for loss in losses:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    m = hs.rms_norm(x, w, dtype=E4M3, group=32)
+    before = m.values._version, m.scales._version, x._version
+    loss = saved_by(m.scales)
+    hs.rms_norm(x, w, out=m)
+    assert (m.values._version, m.scales._version, x._version) == (before[0] + 1, before[1] + 1, before[2])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    # what is only read is as it was
+    loss = saved_by(x)
+    hs.rms_norm(x, w, residual=r)
+    loss.backward()
+    with torch.inference_mode():
+        y = torch.empty_like(x)
+        check_values(hs.rms_norm(x, w, out=y), reference(x, w, 1e-6))
+    check_values(hs.rms_norm(x, w, out=y), reference(x, w, 1e-6))  # (its kind has no versions)
