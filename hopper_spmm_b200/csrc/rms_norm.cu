@@ -386,7 +386,11 @@ extern "C" int b200spmm_rms_norm(const b200spmm_rms_norm_t *a, void *stream) {
     if (a->weight && !aligned(a->weight, size_of(a->w_dtype))) return B200SPMM_ERR_INVALID_ARG;
     if (e4m3 && !empty && (!a->scales || !aligned(a->scales, 4))) return B200SPMM_ERR_INVALID_ARG;
     return on_device(a->device, [&]() -> int {
-        if (empty) return B200SPMM_OK;
+        if (empty) {
+            // (a row without columns has one scale all the same)
+            if (e4m3 && a->group == 0 && a->rows && a->scales) B200_CUDA_TRY(cudaMemsetAsync(a->scales, 0, a->rows * 4, static_cast<cudaStream_t>(stream)));
+            return B200SPMM_OK;
+        }
         NormParams p{a->x, a->residual, a->weight, a->sum, a->out, a->scales, a->ldx, a->ldr, a->lds, a->ldo, a->rows, (uint32_t)a->cols};
         p.groups = a->group ? ((uint32_t)a->cols + a->group - 1) / a->group : 1;
         p.w_type = a->w_dtype;

@@ -300,3 +300,11 @@ def test_autograd_is_told_of_results_that_are_written_in_place():
         y = torch.empty_like(x)
         check_values(hs.rms_norm(x, w, out=y), reference(x, w, 1e-6))
     check_values(hs.rms_norm(x, w, out=y), reference(x, w, 1e-6))  # (its kind has no versions)
+
+
+def test_rows_without_columns_have_scales_of_zero():
+    x = torch.empty(5, 0, dtype=F16, device="cuda")
+    m = hs.Fp8Matrix(x.to(E4M3), torch.full((5, 1), 7.0, device="cuda"))
+    hs.rms_norm(x, out=m)
+    assert not m.scales.any()
+    assert not hs.rms_norm(x, dtype=E4M3).scales.any()
