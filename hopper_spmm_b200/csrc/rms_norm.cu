@@ -7,7 +7,7 @@
 // so the largest |y| is the largest |h w| times it, and one reduction serves both.  Scales of groups of 32, 64 and 128 come from 4, 8 or 16 neighbouring lanes.
 // Rows longer than a block's registers (32,768 columns) are read a second time.
 //
-// 8192 x 8192 bf16 with a bf16 residual, to e4m3 with scales of 128: 80 us, 5.9 TB/s, 90 % of a copy's rate (104 before kernels were made for the weight's and the
+// 8192 x 8192 bf16 with a bf16 residual, to e4m3 with scales of 128: 81 us, 5.8 TB/s, 89 % of a copy's rate (104 before kernels were made for the weight's and the
 // result's type, 170 before all loads of a row came before the first use of one).  5001 x 4090, whose rows start on 4 bytes, with an fp32 residual and scales of 32: 61 us, 3.8 TB/s, issue: two
 // values an access, and a scale's arithmetic for each two of a lane.  8 x 8192: 2.8 us, a launch and one reduction.
 #include <type_traits>
@@ -118,6 +118,11 @@ B200_DEVICE Both reduce(Both b, bool whole_block, Both *shared) {
     return b;
 }
 
+// Two products in one instruction.
+B200_DEVICE void times_two(float &a, float &b, float by) {
+    asm("{\n.reg .b64 v, w;\nmov.b64 v, {%0, %1};\nmov.b64 w, {%2, %2};\nmul.rn.f32x2 v, v, w;\nmov.b64 {%0, %1}, v;\n}\n" : "+f"(a), "+f"(b) : "f"(by));
+}
+
 B200_DEVICE uint32_t bits_of(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // R: the residual's type, void for none.  kV: times eight values of a row that a thread keeps; 0: none, the row is read again.  kE: neighbours that are read
@@ -200,8 +205,8 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
     if constexpr (kKeep) each([&](uint32_t col, float (&v)[kPer]) { keep_sum(col, v); });
     Both all = sums();
     float factor = 1.f / sqrtf(all.sum / (float)p.cols + p.eps);
-    if (!(all.sum <= 1e37f) || all.sum < 1e-28f) {
-        // squares beyond fp32's range, or zeros: from values that are scaled so that the largest lies in [1, 2)
+    if (!(all.sum <= 1e37f) || all.sum < 1e-28f || (of_row && (all.top >= kInfBits || (all.top < kTiny && all.top != 0u)))) {
+        // squares beyond fp32's range, or h w where the norm would not be, or zeros: from values that are scaled so that the largest lies in [1, 2)
         Both most{0.f, 0u};
         each([&](uint32_t, float (&v)[kPer]) {
 #pragma unroll
@@ -233,6 +238,11 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
         scales_of(all.top, &scale, &inverse);
         if (threadIdx.x == 0) p.scales[row] = scale;
     }
+    // What h is multiplied by before w, which may lie as far from 1 as h: y / w, or, for scales of groups, the power of two next below the norm's reciprocal, which leaves the quotients as they are.
+    const uint32_t power = __float_as_uint(factor) & kInfBits;
+    const bool in_two = eights && !of_row && down == 1.f && power != 0u && power != kInfBits;
+    const float first_by = !eights ? factor : in_two ? __uint_as_float(power) : 1.f;
+    if (in_two) factor = __uint_as_float((__float_as_uint(factor) & ~kInfBits) | 0x3F800000u);
     const uint32_t lanes = min(32u, p.group / kE), together = max(1u, p.group / (32u * kE));  // of a group: lanes, and times 32 kE columns of a thread
     each([&](uint32_t col, float (&v)[kPer]) {
         if constexpr (!kKeep) {
@@ -242,6 +252,9 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
                 keep_sum(col, whole[0]);
             }
         }
+        if (kKind != kRow)
+#pragma unroll
+            for (uint32_t e = 0; e < kPer; e += 2) times_two(v[e], v[e + 1], first_by);
         times_weight<X, kE, kKind>(p, col, v);
         uint32_t tops[kJ];
         float inverses[kJ];
@@ -291,9 +304,7 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormParams p) {
                 }
                 if (there) q.store(static_cast<uint8_t *>(p.out) + (int64_t)row * p.ldo + at);
             } else if (there) {
-                float y[kE];
-#pragma unroll
-                for (uint32_t e = 0; e < (uint32_t)kE; ++e) y[e] = v[j * kE + e] * factor;
+                const float *y = v + j * kE;
                 const int64_t to = (int64_t)row * p.ldo + at;
                 if constexpr (kKind != kAny) store_as<X, kE>(p.out, to, y);
                 else if (p.out_type == B200SPMM_T_F32) store_as<float, kE>(p.out, to, y);

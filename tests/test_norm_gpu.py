@@ -308,3 +308,15 @@ def test_rows_without_columns_have_scales_of_zero():
     hs.rms_norm(x, out=m)
     assert not m.scales.any()
     assert not hs.rms_norm(x, dtype=E4M3).scales.any()
+
+
+@pytest.mark.parametrize("cols", [100, 5000, 5002, 40000])
+@pytest.mark.parametrize("spread,far", [(1e18, 1e25), (1e15, 1e35), (1e-13, 1e-30), (1e-12, 1e-28), (1e36, 1e36), (1e-30, 1e-25), (1e17, 1e-37), (1e-12, 1e36)])
+def test_weights_as_far_from_one_as_the_values(spread, far, cols):
+    # h w leaves fp32's range, y does not
+    x = normal(6, cols, 1).clamp(-4, 4) * spread
+    w = (normal(1, cols, 2)[0].clamp(-4, 4).abs() + 0.5) * far
+    want = reference(x, w, 0.0)
+    check_values(hs.rms_norm(x, w, 0.0), want)
+    for group in (None, 32, 64, 128):
+        check_eights(hs.rms_norm(x, w, 0.0, dtype=E4M3, group=group), want)
