@@ -27,6 +27,7 @@ template <class W>
 constexpr int kRing = 2 * W::kPieces;  // stages of a warp: two steps
 template <class W>
 constexpr uint32_t kRingBytes = kRingOf<W, 2, kRing<W>>;
+constexpr int kHalves = 2;  // numbers that an inner value is the sum of
 constexpr uint32_t kMaxTokens = 256, kMaxExperts = 1024, kMaxTop = 32;
 constexpr uint32_t kLogitTokens = 4, kLogitThreads = 256;
 
@@ -34,7 +35,7 @@ struct MoeParams {
     Matrix gate_up, down;
     uint32_t experts, hidden, inner, top, tokens, pairs;
     bool all_tokens;  // are columns of the first product, in all blocks
-    uint32_t run, up_columns, down_columns;  // columns of a run, and that a block has room for, in either product
+    uint32_t run, up_columns, down_columns;  // columns of a run, and that a block has room for as a whole, in either product
     uint4 *routing;  // as the first blocks found it
     bool renormalize;
     const void *x, *router;
@@ -272,14 +273,14 @@ B200_DEVICE uint32_t run_end(const Routing &r, uint32_t run) {  // (the last one
     return run + 1u < *r.n_runs ? run_start(r, run + 1u) : r.starts[run_expert(r, run) + 1u];
 }
 
-// A block's share of `of_run` tiles of every run, in parts whose columns have room: part(first, end, first run's pairs, how many, the longest run's).
+// A block's share of `of_run` tiles of every run, in parts whose columns have room, or of a single run: part(first, end, first run's pairs, how many, the longest run's).
 template <class Part>
 B200_DEVICE void each_part(const Routing &r, uint32_t of_run, uint32_t room, Part &&part) {
     const uint32_t all = *r.n_runs * of_run, end = (uint32_t)((uint64_t)all * (blockIdx.x + 1u) / gridDim.x);
     for (uint32_t at = (uint32_t)((uint64_t)all * blockIdx.x / gridDim.x); at < end;) {
         const uint32_t run0 = at / of_run, pair0 = run_start(r, run0);
         uint32_t run = run0, longest = 0;
-        while (run * of_run < end && run < *r.n_runs && run_end(r, run) - pair0 <= room) {
+        while (run * of_run < end && run < *r.n_runs && (run == run0 || run_end(r, run) - pair0 <= room)) {
             longest = max(longest, run_end(r, run) - run_start(r, run));
             ++run;
         }
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const MoeParams p)
 
 // ------------------------------------------------------------------ down
 
-// Inner values as one 16-bit number or the sum of two, the second what the first leaves over: fp16 has 11 or 22 digits that way, bf16 16 with two.
+// Inner values as the sum of two 16-bit numbers, the second what the first leaves over: fp16 has 22 digits that way, bf16 16.
 template <typename T>
 B200_DEVICE void split_unit(const float4 (&from)[2], uint32_t left, float by, uint4 *high, uint4 *low) {
     const float v[8] = {from[0].x, from[0].y, from[0].z, from[0].w, from[1].x, from[1].y, from[1].z, from[1].w};
@@ -468,9 +469,10 @@ B200_DEVICE void split_unit(const float4 (&from)[2], uint32_t left, float by, ui
     *low = *reinterpret_cast<const uint4 *>(b);
 }
 
-// Inner values of n pairs as columns, by all threads.
-template <class W, int kPlanes>
-__device__ __noinline__ void stage_inner(const float *h, uint32_t h_ld, uint32_t inner, const uint16_t *pairs, uint32_t n, uint32_t base, uint32_t pitch, uint32_t plane, uint32_t *tops) {
+// Inner values of n pairs as columns, by all threads; kPieces: `count` steps from step `first` on, and `anew` where their largest ones are not known yet, else all steps.
+template <class W, bool kPieces>
+__device__ __noinline__ void stage_inner(const float *h, uint32_t h_ld, uint32_t inner, const uint16_t *pairs, uint32_t n, uint32_t base, uint32_t pitch, uint32_t plane, uint32_t *tops,
+                                         uint32_t first, uint32_t count, bool anew) {
     using T = typename W::T;
     constexpr bool kScale = std::is_same<T, __half>::value;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -483,9 +485,9 @@ __device__ __noinline__ void stage_inner(const float *h, uint32_t h_ld, uint32_t
             v[1] = from[1];
         }
     };
-    const uint32_t room = (inner + W::kStep - 1) / W::kStep * W::kUnits, units = (room + 31u) / 32u * 32u, pieces = units / 32u;
-    if constexpr (kScale)
-        find_tops(tops, n, units, [&](uint32_t j, uint32_t u) {
+    const uint32_t u0 = kPieces ? first * W::kUnits : 0u, room = (kPieces ? count : (inner + W::kStep - 1) / W::kStep) * W::kUnits, pieces = (room + 31u) / 32u;
+    if (kScale && (!kPieces || anew))
+        find_tops(tops, n, (inner + 255u) / 256u * 32u, [&](uint32_t j, uint32_t u) {
             float4 v[2];
             load(j, u, v);
             const float w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
@@ -503,35 +505,42 @@ __device__ __noinline__ void stage_inner(const float *h, uint32_t h_ld, uint32_t
 #pragma unroll
         for (uint32_t b = 0; b < kBatch; ++b) {
             const uint32_t at = q + b * kWarps;
-            if (at < n * pieces) load(at / pieces, at % pieces * 32u + lane, v[b]);
+            if (at < n * pieces) load(at / pieces, u0 + at % pieces * 32u + lane, v[b]);
         }
 #pragma unroll
         for (uint32_t b = 0; b < kBatch; ++b) {
             const uint32_t at = q + b * kWarps, j = at / pieces, u = at % pieces * 32u + lane;
             if (at >= n * pieces || u >= room) continue;
             uint4 high, low;
-            split_unit<T>(v[b], u * 8u < inner ? inner - u * 8u : 0u, kScale ? fp4::exp2_int(power_of(tops[j])) : 1.f, &high, &low);
+            split_unit<T>(v[b], (u0 + u) * 8u < inner ? inner - (u0 + u) * 8u : 0u, kScale ? fp4::exp2_int(power_of(tops[j])) : 1.f, &high, &low);
             const uint32_t to = base + j * pitch + unit_place<W>(u);
             ptx::st_shared_v4(to, unit_order<W>(high));
-            if (kPlanes > 1) ptx::st_shared_v4(to + plane, unit_order<W>(low));
+            ptx::st_shared_v4(to + plane, unit_order<W>(low));
         }
     }
 }
 
-template <class W, int kPlanes, int kNB>
+// kPieces: a part may be one run whose columns have no room as a whole.
+template <class W, int kNB, bool kPieces>
 B200_DEVICE void down_part(const MoeParams &p, const Routing &r, uint8_t *smem, uint32_t columns_at, uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n) {
     constexpr bool kScale = std::is_same<typename W::T, __half>::value;
     const uint32_t base = ptx::smem_u32(smem), warp = warp_index(), lane = threadIdx.x & 31u;
-    const uint32_t steps = (p.inner + W::kStep - 1) / W::kStep, of_run = (p.hidden + kTileRows - 1u) / kTileRows, pitch = column_pitch<W>(steps), plane = p.down_columns * pitch;
-    uint32_t *tops = reinterpret_cast<uint32_t *>(smem + columns_at + kPlanes * plane);
+    const uint32_t steps = (p.inner + W::kStep - 1) / W::kStep, of_run = (p.hidden + kTileRows - 1u) / kTileRows;
+    const uint32_t window = !kPieces || n <= p.down_columns ? steps : (((kMaxSmem - columns_at) / n - 4u) / kHalves - column_pitch<W>(0)) / (W::kUnits * 16u);
+    const uint32_t pitch = column_pitch<W>(window), plane = (kPieces ? n : p.down_columns) * pitch;
+    bool anew = true;
+    uint32_t *tops = reinterpret_cast<uint32_t *>(smem + columns_at + kHalves * plane);
     const Split split(end - begin, steps, kWarps);
-    const Share s(split, begin, end, warp, steps, steps, base + warp * kRingBytes<W>);
-    multiply<W, kNB, kPlanes, false, kRing<W>>(
+    const Share s(split, begin, end, warp, steps, window, base + warp * kRingBytes<W>);
+    multiply<W, kNB, kHalves, false, kRing<W>>(
         p.down, s,
         [&](uint32_t tile) { return place_in(r, of_run, tile); },
         [&](const Place &at, uint32_t row) { return (uint64_t)at.expert * p.hidden + min(at.tile * kTileRows + row, p.hidden - 1u); },
         [&](const Place &at) { return Columns{base + columns_at + (at.start - pair0) * pitch, pitch, plane, at.n, 0, 0, 0, nullptr, 1}; },
-        [&](uint32_t, uint32_t) { stage_inner<W, kPlanes>(p.h, p.h_ld, p.inner, r.pairs + pair0, n, base + columns_at, pitch, plane, tops); },
+        [&](uint32_t first, uint32_t count) {
+            stage_inner<W, kPieces>(p.h, p.h_ld, p.inner, r.pairs + pair0, n, base + columns_at, pitch, plane, tops, first, count, anew);
+            if (kPieces) anew = false;
+        },
         [&](const Place &at, const float(&sums)[kNB][4]) {
 #pragma unroll
             for (uint32_t nb = 0; nb < (uint32_t)kNB; ++nb)
@@ -544,7 +553,7 @@ B200_DEVICE void down_part(const MoeParams &p, const Routing &r, uint8_t *smem, 
         });
 }
 
-template <class W, int kPlanes>
+template <class W, bool kPieces>
 __global__ void __launch_bounds__(kThreads, 1) down_kernel(const MoeParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
     const Routing r = routing_at(smem + kWarps * kRingBytes<W>, p.pairs, p.experts);
@@ -553,8 +562,8 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const MoeParams p) {
     for (uint32_t i = threadIdx.x; i < routing_bytes(p.pairs, p.experts) / 16u; i += kThreads) reinterpret_cast<uint4 *>(smem + kWarps * kRingBytes<W>)[i] = p.routing[i];
     __syncthreads();
     each_part(r, (p.hidden + kTileRows - 1u) / kTileRows, p.down_columns, [&](uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n, uint32_t longest) {
-        if (longest <= 8u) down_part<W, kPlanes, 1>(p, r, smem, columns_at, begin, end, pair0, n);
-        else down_part<W, kPlanes, 2>(p, r, smem, columns_at, begin, end, pair0, n);
+        if (longest <= 8u) down_part<W, 1, kPieces>(p, r, smem, columns_at, begin, end, pair0, n);
+        else down_part<W, 2, kPieces>(p, r, smem, columns_at, begin, end, pair0, n);
     });
 }
 
@@ -639,23 +648,28 @@ uint32_t room_for(const MoeParams &p, uint32_t k, uint32_t planes) {
     const uint64_t each = (uint64_t)planes * ((uint64_t)steps * W::kUnits * 16u + 192u) + 4u;
     return (uint32_t)std::min<uint64_t>(p.pairs, (kMaxSmem - taken) / each);  // (as many as there are pairs at most)
 }
-template <class Up, typename X, class Down, int kPlanes>
+template <class Up, typename X, class Down>
 int launch_all(MoeParams p, double *logits, cudaStream_t stream) {
-    static std::atomic<uint64_t> up_allowed{0}, down_allowed{0};
+    static std::atomic<uint64_t> up_allowed{0}, down_allowed[2] = {};
     p.up_columns = room_for<Up>(p, p.hidden, 1);
-    p.down_columns = room_for<Down>(p, p.inner, kPlanes);
+    p.down_columns = room_for<Down>(p, p.inner, kHalves);
     // Columns of all tokens are there before the routing is, those of a block's own pairs are fewer: one token 37.2 us with all and 38.4 with its own, 8 with 4-bit experts 149.4
     // and 147.1.
     p.all_tokens = p.tokens <= std::min(4u, p.up_columns);
-    p.run = std::min({kRun, p.up_columns, p.down_columns});
-    if (p.run == 0) return B200SPMM_ERR_UNSUPPORTED;
+    // Inner values of a run come in pieces where it has no room for them as a whole: 32 tokens, 2 of 8 experts of 4096 x 14336 each in codes for fp16 375 us, in bf16 522, where shorter
+    // runs that read an expert again and again take 720 and 1,795; with a kernel for both, 8 tokens through 64 experts of 4096 x 2048 take 168 us for 157.
+    // (As many of them as a column of either half has room for with codes, of both with 16-bit experts: beyond that, a call is refused.)
+    p.run = std::min(kRun, p.up_columns);
+    if (p.run == 0 || room_for<Down>(p, p.inner, Down::kCodes ? 1 : kHalves) == 0) return B200SPMM_ERR_UNSUPPORTED;
     // (there are as many runs as pairs, or fewer)
     auto blocks = [&](uint32_t tiles) { return (uint32_t)std::min<uint64_t>(fp4::sm_count(), (uint64_t)p.pairs * tiles); };
     B200_CUDA_TRY(allow_smem(gate_up_kernel<Up, X>, up_allowed));
-    B200_CUDA_TRY(allow_smem(down_kernel<Down, kPlanes>, down_allowed));
+    const bool pieces = p.run > p.down_columns;
+    const auto down = pieces ? down_kernel<Down, true> : down_kernel<Down, false>;
+    B200_CUDA_TRY(allow_smem(down, down_allowed[pieces]));
     if (logits) B200_CUDA_TRY(launch_after(logits_kernel<X>, dim3(p.experts, (p.tokens + kLogitTokens - 1) / kLogitTokens), kLogitThreads, 0, 1, stream, p, logits));
     B200_CUDA_TRY(launch_after(gate_up_kernel<Up, X>, dim3(blocks((p.inner + 7) / 8)), kThreads, kMaxSmem, 1, stream, p));
-    B200_CUDA_TRY(launch_after(down_kernel<Down, kPlanes>, dim3(blocks((p.hidden + kTileRows - 1) / kTileRows)), kThreads, kMaxSmem, 1, stream, p));
+    B200_CUDA_TRY(launch_after(down, dim3(blocks((p.hidden + kTileRows - 1) / kTileRows)), kThreads, kMaxSmem, 1, stream, p));
     B200_CUDA_TRY(launch_after(sum_kernel, dim3((p.hidden + kSumThreads - 1) / kSumThreads, p.tokens), kSumThreads, 0, 1, stream, p));
     return B200SPMM_OK;
 }
@@ -663,15 +677,14 @@ int launch_all(MoeParams p, double *logits, cudaStream_t stream) {
 template <int kUp, typename X>
 int launch_codes(const MoeParams &p, uint32_t span, double *logits, cudaStream_t stream) {
     using Up = Weights<__half, kUp>;
-    constexpr int kPlanes = 2;
-    return span == 32   ? launch_all<Up, X, Weights<__half, 32>, kPlanes>(p, logits, stream)
-           : span == 64 ? launch_all<Up, X, Weights<__half, 64>, kPlanes>(p, logits, stream)
-                        : launch_all<Up, X, Weights<__half, 128>, kPlanes>(p, logits, stream);
+    return span == 32   ? launch_all<Up, X, Weights<__half, 32>>(p, logits, stream)
+           : span == 64 ? launch_all<Up, X, Weights<__half, 64>>(p, logits, stream)
+                        : launch_all<Up, X, Weights<__half, 128>>(p, logits, stream);
 }
 
 template <typename T>
 int launch_moe(const b200spmm_moe_t *m, const MoeParams &p, double *logits, cudaStream_t stream) {
-    if (!m->gate_up) return launch_all<Weights<T, 0>, T, Weights<T, 0>, 2>(p, logits, stream);
+    if (!m->gate_up) return launch_all<Weights<T, 0>, T, Weights<T, 0>>(p, logits, stream);
     const uint32_t a = span_of(m->gate_up), b = span_of(m->down);
     return a == 32 ? launch_codes<32, T>(p, b, logits, stream) : a == 64 ? launch_codes<64, T>(p, b, logits, stream) : launch_codes<128, T>(p, b, logits, stream);
 }

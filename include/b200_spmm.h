@@ -631,7 +631,8 @@ int b200spmm_int4_product(const b200spmm_int4_t *a, const void *d_B, int64_t ldb
  * aligned), the others null.  Logits are added up in 64 bits; the inner values are kept in 32 and multiplied as the sum of two 16-bit
  * numbers: of x's type with 16-bit experts (22 digits in fp16, 16 in bf16), by codes of fp16, scaled by powers of two.
  * experts up to 1024, top_k up to 32; hidden and inner as far as a block's shared memory holds a column beside the routing (else B200SPMM_ERR_UNSUPPORTED):
- * 24,000 and 12,000 always, three times that with few tokens.  A row of x with NaN gives NaN in its own row of y alone.
+ * 24,000 and 12,000 (24,000 by codes) always, three times that with few tokens.  An expert is read once for up to 16 of its tokens; for as many as columns of x have room, where those are fewer:
+ * 8 at a hidden size of 8,192.  A row of x with NaN gives NaN in its own row of y alone.
  */
 typedef struct {
     uint64_t experts, hidden, inner;

@@ -544,3 +544,26 @@ def test_autograd_is_told_of_results_that_are_written_in_place():
         before = x._version, y._version, ids._version, shares._version
         call(x, y)
         assert (x._version, y._version, ids._version, shares._version) == (before[0], before[1] + 1, *before[2:])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
+@pytest.mark.parametrize("group", [32, 64, 128], ids=str)
+@pytest.mark.parametrize("n", [1, 5])
+def test_inner_values_beside_codes_that_no_block_has_room_for(n, group, dtype):
+    # a column's two halves are 290 KB
+    c = Case(3, 72, 72_000, 2, dtype, group, router=False)
+    x = tokens_of(n, 72, 9, dtype)
+    ids, shares = torch.tensor([[0, 2]] * n, device="cuda"), torch.tensor([[0.75, -0.5]] * n, device="cuda")
+    c.check(c.layer.experts(x, ids, shares), x, ids, shares)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
+@pytest.mark.parametrize("group", [0, 64], ids=str)
+@pytest.mark.parametrize("tokens", [1, 9, 14, 16, 17, 40])
+def test_inner_values_of_a_run_in_pieces(tokens, group, dtype):
+    # 16 columns of 6,000 have no room as a whole, 8 or 9 do; hidden sizes with one round of a block's tiles, and with several
+    for hidden in (200, 148 * 16 * 21 + 5):
+        c = Case(2, hidden, 6000, 1, dtype, group, router=False)
+        x = tokens_of(tokens, hidden, 9, dtype)
+        ids, shares = (torch.arange(tokens, device="cuda") % 10 == 9).long()[:, None], torch.rand(tokens, 1, device="cuda")
+        c.check(c.layer.experts(x, ids, shares), x, ids, shares)
