@@ -567,3 +567,91 @@ def test_inner_values_of_a_run_in_pieces(tokens, group, dtype):
         x = tokens_of(tokens, hidden, 9, dtype)
         ids, shares = (torch.arange(tokens, device="cuda") % 10 == 9).long()[:, None], torch.rand(tokens, 1, device="cuda")
         c.check(c.layer.experts(x, ids, shares), x, ids, shares)
+
+
+# ---------------------------------------------------------------- codes: columns and inner values as scaled fp16
+
+@pytest.mark.parametrize("group", [32, 64, 128, None], ids=str)
+@pytest.mark.parametrize("spread", [1e-18, 1e-15, 1e-8, 1e-5, 1e5, 1e12, 1e16])
+def test_tokens_far_from_one_beside_codes(spread, group):
+    c = Case(4, 200, 72, 2, BF16, group)
+    x = (tokens_of(9, 200, 2, F32) * spread).to(BF16)
+    ids, shares = torch.tensor([[0, 3]] * 9, device="cuda"), torch.full((9, 2), 0.5, device="cuda")
+    c.check(c.layer.experts(x, ids, shares), x, ids, shares)
+    # and beside others of another size
+    x[::2] /= spread
+    c.check(c.layer.experts(x, ids, shares), x, ids, shares)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
+@pytest.mark.parametrize("group", [32, 64, 128], ids=str)
+def test_inner_values_beyond_the_range_of_fp16_and_far_below_it_beside_codes(group, dtype):
+    for spread in (300.0, 2.0 ** -8):
+        c = Case(4, 128, 64, 2, dtype, group)
+        c.gate_up.scales.mul_(spread)
+        c.down.scales.mul_(1e-4 if spread > 1 else 1.0)
+        x = tokens_of(7, 128, 2, dtype)
+        ids, shares = torch.tensor([[0, 3]] * 7, device="cuda"), torch.full((7, 2), 0.5, device="cuda")
+        c.check(c.layer.experts(x, ids, shares), x, ids, shares)
+
+
+@pytest.mark.parametrize("tokens", [3, 9])  # (all as columns before the routing, or those of runs)
+def test_values_up_to_31_binades_below_a_token_s_largest_are_exact_beside_codes(tokens):
+    # a value of 2^30 that meets nothing but codes of zero takes no digit from the others
+    c = Case(3, 128, 40, 2, BF16, 64)
+    v, z = c.gate_up.values, c.gate_up.zeros
+    v[:, 5] = (v[:, 5] & 0xF0) | z[0]  # column 10
+    x = rand(tokens, 128, seed=2, dtype=BF16)
+    ids, shares = torch.tensor([[0, 2]] * tokens, device="cuda"), torch.full((tokens, 2), 0.5, device="cuda")
+    x[:, 10] = 0
+    x = torch.where(x.abs() < 2.0 ** -3, 0.25, x)
+    x[:, 10] = 0
+    want = c.layer.experts(x, ids, shares)
+    c.check(want, x, ids, shares)
+    x[:, 10] = 2.0 ** 28
+    # the sums are of the same numbers in the same order, but for a power of two
+    assert torch.equal(c.layer.experts(x, ids, shares), want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
+@pytest.mark.parametrize("group", [0, 32, 64, 128], ids=str)
+@pytest.mark.parametrize("tokens", [3, 9])
+def test_infinities_and_nan_in_a_token_are_its_own(tokens, group, dtype):
+    c = Case(5, 200, 72, 2, dtype, group)
+    x = tokens_of(tokens, 200, 2, dtype)
+    ids = torch.tensor([[0, 3]] * tokens, device="cuda")  # the same runs for all
+    shares = torch.full((tokens, 2), 0.5, device="cuda")
+    want = c.layer.experts(x, ids, shares)
+    x[0, 77], x[2, 199] = torch.nan, -torch.inf
+    y = c.layer.experts(x, ids, shares)
+    assert torch.isnan(y[0]).all() and not torch.isfinite(y[2]).any()
+    others = [i for i in range(tokens) if i not in (0, 2)]
+    assert torch.equal(y[others], want[others])
+    z = c.layer.forward(x)
+    assert torch.isnan(z[0]).all() and not torch.isfinite(z[2]).any() and torch.isfinite(z[others]).all()
+
+
+# ---------------------------------------------------------------- the largest sizes
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
+@pytest.mark.parametrize("group", [0, 32, 64, 128], ids=str)
+@pytest.mark.parametrize("size", [(4, 64, 12_000, 2, 20), (2, 24_000, 16, 2, 20), (3, 72, 36_000, 1, 5), (3, 72_000, 8, 1, 5), (8, 4096, 14_336, 2, 32)], ids=str)
+def test_few_columns_have_room_in_a_block(size, group, dtype):
+    experts, hidden, inner, top, n = size
+    c = Case(experts, hidden, inner, top, dtype, group, seed=sum(size))
+    x = tokens_of(n, hidden, 9, dtype)
+    y, ids, shares = c.layer.forward(x, return_routing=True)
+    c.check_routing(x, ids, shares)
+    c.check(y, x, ids, shares)
+    assert torch.equal(c.layer.experts(x, ids, shares), y)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS)
+@pytest.mark.parametrize("group", [0, 64], ids=str)
+@pytest.mark.parametrize("hidden,inner", [(24_000, 24), (40, 12_000)])
+def test_one_column_has_room_beside_the_largest_routing(hidden, inner, group, dtype):
+    c = Case(5, hidden, inner, 32, dtype, group, router=False)
+    x = tokens_of(256, hidden, 2, dtype)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    ids, shares = torch.randint(-1, 5, (256, 32), generator=g, device="cuda"), torch.rand(256, 32, generator=g, device="cuda") - 0.3
+    c.check(c.layer.experts(x, ids, shares), x, ids, shares)
