@@ -7,7 +7,7 @@
 //
 // 28672 x 8192 in groups of 128 with zeros, 123 MB, 18.8 us at a copy's rate: one fp16 column 29.6 us, 8 in e4m3 36.  Of the 29.6 multiplying takes 21 (5.5 TB/s: 320 instructions
 // for a step of 16 rows x 256 codes fill what issue slots there are), from 3.2 us on, when the columns are there; 1,792 tiles are 12 for 132 blocks and 13 for 16, which end 2 to 4 us
-// after the others.  8 columns of 8,192 take half of the shared memory and 3 us longer to come.  14331 x 4090 in groups of 64 times 33 columns: 41 us, five MMAs for
+// after the others.  (Times of a captured loop; a call from Python takes the host 5 us or more.)  One column in bf16 31.5, 8 in fp16 30.7 and in bf16 32.5.  8 columns of 8,192 take half of the shared memory and 3 us longer to come.  14331 x 4090 in groups of 64 times 33 columns: 41 us, five MMAs for
 // each operand and columns that start on 4 bytes (49 where they came value by value, 61 in two reads of the matrix).
 #include "entry.hpp"
 #include "fp4_store.cuh"

@@ -10,7 +10,8 @@
 //
 // One token, 8 of 64 experts of 2048 x 1024 in bf16, 101 MB: 37 us for 15.4 at a copy's rate.  The experts' bytes come at 6.5 to 7 TB/s; the rest is what stands before them: four
 // launches, logits 3 us, the choice and its runs 5, the first copies 2 to 4.  Much of that is waiting for instructions that are run once and that the weights have pushed out of L2.
-// 8 tokens through 64 experts of 4096 x 2048 in 4 bits, 554 MB: 147 us for 85; 32 through 128, 1.1 GB: 304 for 172: the instructions that a step of codes takes, as in int4.cu.
+// 8 tokens through 64 experts of 4096 x 2048 in 4 bits, 554 MB: 157 us for 85; 32 through 128, 1.1 GB: 305 for 172: the instructions that a step of codes takes, as in int4.cu, and
+// in the second product two numbers for each inner value (with one of 11 digits, 146 us for the 157).  Times of a captured loop; a call from Python takes the host 5 us or more.
 #include <type_traits>
 
 #include "entry.hpp"
@@ -21,6 +22,7 @@ namespace b200spmm {
 namespace narrow {
 namespace {
 
+// With 16, 20 and 24 warps: one token in bf16 36.9, 36.9 and 37.8 us, 16 of them 147, 144 and 148; 8 with experts in 4 bits 160, 157 and 161, 32 through 128 experts 297, 305 and 315.
 constexpr uint32_t kWarps = 20, kThreads = 32 * kWarps;
 constexpr uint32_t kRun = 16;  // columns that a tile meets at once, at most
 template <class W>
@@ -364,7 +366,7 @@ struct Converted {
 
 // ------------------------------------------------------------------ gate, up, SiLU
 
-// X: x's type.  Codes are widened to fp16 either way, which takes five operations a word of eight where bf16 takes seven: bf16 columns are brought to fp16.
+// X: x's type.  Codes are widened to fp16 either way, which takes nine operations a word of eight where bf16 takes eleven: bf16 columns are brought to fp16.
 template <class W, typename X, int kNB>
 B200_DEVICE void gate_up_part(const MoeParams &p, const Routing &r, uint8_t *smem, uint32_t columns_at, uint32_t begin, uint32_t end, uint32_t pair0, uint32_t n) {
     constexpr bool kConvert = !std::is_same<typename W::T, X>::value;
@@ -653,8 +655,8 @@ int launch_all(MoeParams p, double *logits, cudaStream_t stream) {
     static std::atomic<uint64_t> up_allowed{0}, down_allowed[2] = {};
     p.up_columns = room_for<Up>(p, p.hidden, 1);
     p.down_columns = room_for<Down>(p, p.inner, kHalves);
-    // Columns of all tokens are there before the routing is, those of a block's own pairs are fewer: one token 37.2 us with all and 38.4 with its own, 8 with 4-bit experts 149.4
-    // and 147.1.
+    // Columns of all tokens are there before the routing is, those of a block's own pairs are fewer.  With all and with its own: 1, 2, 4, 8 and 16 tokens in
+    // bf16 36.9 and 38.6 us, 55.1 and 56.8, 83.8 and 85.4, 108.7 and 109.9, 143.9 and 144.5; with experts in 4 bits 53.3 and 56.9, 81.2 and 83.9, 120.8 and 121.6, 159.8 and 157.5, 214.5 and 209.1.
     p.all_tokens = p.tokens <= std::min(4u, p.up_columns);
     // Inner values of a run come in pieces where it has no room for them as a whole: 32 tokens, 2 of 8 experts of 4096 x 14336 each in codes for fp16 375 us, in bf16 522, where shorter
     // runs that read an expert again and again take 720 and 1,795; with a kernel for both, 8 tokens through 64 experts of 4096 x 2048 take 168 us for 157.
@@ -691,7 +693,7 @@ int launch_moe(const b200spmm_moe_t *m, const MoeParams &p, double *logits, cuda
 
 // ids null: they are found from the logits, and left, with the shares, at out_ids and out_shares where those are wanted.
 int run_moe(const b200spmm_moe_t *m, const void *x, int64_t ldx, int64_t tokens, const void *ids, int id_bytes, const float *shares, void *y, int64_t ldy, int32_t *out_ids,
-            float *out_shares, void *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
+            float *out_shares, void *workspace, cudaStream_t stream) {
     const Layout l = layout_of(m, (uint64_t)tokens);
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     MoeParams p{};
@@ -765,7 +767,7 @@ int b200spmm_moe(const b200spmm_moe_t *m, const void *d_x, int64_t ldx, int64_t 
     if (!fp4::aligned(d_ids, 4) || !fp4::aligned(d_shares, 4)) return B200SPMM_ERR_INVALID_ARG;
     return fp4::on_device(m->device, [&]() -> int {
         if (tokens == 0) return B200SPMM_OK;
-        return narrow::run_moe(m, d_x, ldx, tokens, nullptr, 0, nullptr, d_y, ldy, d_ids, d_shares, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+        return narrow::run_moe(m, d_x, ldx, tokens, nullptr, 0, nullptr, d_y, ldy, d_ids, d_shares, workspace, static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -777,7 +779,7 @@ int b200spmm_moe_experts(const b200spmm_moe_t *m, const void *d_x, int64_t ldx, 
     if (tokens > 0 && (!d_ids || !d_shares || !fp4::aligned(d_ids, id_bytes) || !fp4::aligned(d_shares, 4))) return B200SPMM_ERR_INVALID_ARG;
     return fp4::on_device(m->device, [&]() -> int {
         if (tokens == 0) return B200SPMM_OK;
-        return narrow::run_moe(m, d_x, ldx, tokens, d_ids, id_bytes, d_shares, d_y, ldy, nullptr, nullptr, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+        return narrow::run_moe(m, d_x, ldx, tokens, d_ids, id_bytes, d_shares, d_y, ldy, nullptr, nullptr, workspace, static_cast<cudaStream_t>(stream));
     });
 }
 

@@ -98,7 +98,8 @@ B200_DEVICE uint32_t in_register(uint32_t constant) {
 }
 
 // Eight codes less their zero, exactly: pairs 0 4, 1 5, 2 6, 3 7.  A code under the exponent of 1024 (or, four bits up, of 64 times 16; bf16: of 128) is that number and the
-// code; what is added takes the number and the zero away.
+// code; what is added takes the number and the zero away.  (The way of Y. J. Kim et al., "Who Says Elephants Can't Run", arXiv:2211.10017, with the zero in what is added.)  Nine operations a word
+// of eight for fp16: four masks, a shift, four additions; eleven for bf16.
 template <typename T> struct Widen;
 template <>
 struct Widen<__half> {

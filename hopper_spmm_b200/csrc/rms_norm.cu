@@ -8,8 +8,9 @@
 // Rows longer than a block's registers (32,768 columns) are read a second time.
 //
 // 8192 x 8192 bf16 with a bf16 residual, to e4m3 with scales of 128: 81 us, 5.8 TB/s, 89 % of a copy's rate (104 before kernels were made for the weight's and the
-// result's type, 170 before all loads of a row came before the first use of one).  5001 x 4090, whose rows start on 4 bytes, with an fp32 residual and scales of 32: 61 us, 3.8 TB/s, issue: two
-// values an access, and a scale's arithmetic for each two of a lane.  8 x 8192: 2.8 us, a launch and one reduction.
+// result's type, 170 before all loads of a row came before the first use of one).  5001 x 4090, whose rows start on 4 bytes, with an fp32 residual and scales of 32: 60 us, 3.8 TB/s, issue: two
+// values an access, and a scale's arithmetic for each two of a lane.  8 x 8192: 3.0 us in a captured loop, a launch and one reduction (a call from
+// Python takes the host 5 us or more).
 #include <type_traits>
 
 #include "entry.hpp"

@@ -56,8 +56,8 @@ class Int4Matrix:
 
     def linear(self, X, out=None, dtype=None, stream=None):
         """Y = X Wᵀ, [n, rows], for a few tokens that lie row by row: X [n, cols] float16 or bfloat16, or an Fp8Matrix.  Y in ``dtype`` (float32; with
-        ``out``, its type); sums in fp32.  The matrix is read once for every 40 rows of X.  Asynchronous; there is no gradient: X may not require one
-        while gradients are recorded."""
+        ``out``, its type); sums in fp32.  The matrix is read once for every 40 rows of X, of which there may be 65,535.  Asynchronous; there is no gradient: X may
+        not require one while gradients are recorded, nor have a tangent."""
         return self._product(X, out, dtype, stream, True)
 
     def matmul(self, B, C_out=None, dtype=None, stream=None):

@@ -5,7 +5,8 @@
     y, ids, shares = layer.forward(x, return_routing=True)
     y = layer.experts(x, ids, shares)                          # with a routing of the caller's own
 
-Experts in 16 bits, or in 4 as ``Int4Matrix``: of all experts, one after the other.  Each chosen expert is read once for all of its tokens (once for every 16).
+Experts in 16 bits, or in 4 as ``Int4Matrix``: of all experts, one after the other.  Each chosen expert is read once for all of its tokens (once for every
+16, or for as many as there is room for in a block's shared memory where those are fewer: 8 at a hidden size of 8,192).
 The reference has no such operator.
 """
 from __future__ import annotations
@@ -61,7 +62,7 @@ class MoeLayer:
 
     def forward(self, X, out=None, return_routing: bool = False, stream=None):
         """The layer for X [tokens, hidden], up to 256 tokens, in its type; with ``return_routing`` also ids [tokens, top_k] int32 and shares float32.
-        Asynchronous.  There is no gradient: nothing may require one while gradients are recorded."""
+        Asynchronous.  There is no gradient: nothing may require one while gradients are recorded, nor have a tangent."""
         return self._run(X, out, bool(return_routing), None, None, stream)
 
     def experts(self, X, ids, shares, out=None, stream=None):

@@ -70,8 +70,8 @@ def rms_norm(X, weight=None, eps: float = 1e-6, residual=None, sum_out=None, dty
 
     ``dtype``: y's (X's; with ``out``, its type); float8_e4m3fn gives an Fp8Matrix, with a scale of each row or, with ``group``, of so many columns.
     ``weight``: [cols], any of the three types.  Returns y, or with a residual (y, h), h in the residual's type in a new tensor or in ``sum_out``,
-    which may be ``residual`` itself, or X.  ``out``: a tensor, or an Fp8Matrix, for y; a tensor may be X.  Inputs that require a gradient are
-    refused while gradients are recorded: there is none."""
+    which may be ``residual`` itself, or X.  ``out``: a tensor, or an Fp8Matrix, for y; a tensor may be X.  Inputs that require a gradient
+    while gradients are recorded, or have a tangent, are refused: there is none.  What is written in place is new to autograd."""
     if stream is not None:
         mine = (out.values, out.scales) if isinstance(out, Fp8Matrix) else (out,)
         with _on(stream, *(t for t in (X, weight, residual, sum_out, *mine) if t is not None)):

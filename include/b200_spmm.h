@@ -579,7 +579,7 @@ int b200spmm_fp4_status(int device, void *stream);
 /*
  * The residual's addition and the RMS norm, row by row (no counterpart in the reference, as for all below):
  *     h = x + r        sum = h rounded to r_dtype        y = h / sqrt(mean(h^2) + eps) * w
- * with h in fp32 and y rounded once, to out_dtype: fp32, fp16, bf16, or e4m3.  e4m3 has a scale max |y| / 448 for each row (group 0) or for every
+ * with h in fp32 (y is that of the unrounded sum) and y rounded once, to out_dtype: fp32, fp16, bf16, or e4m3.  e4m3 has a scale max |y| / 448 for each row (group 0) or for every
  * `group` (32, 64, 128) neighbours of a row begun, in scales [rows, groups of a row], contiguous: y is value x scale, values are rounded to the
  * nearest, at most 448; a group of zeros has the scale 0, one with an infinity or NaN the scale NaN and zeros as values.
  * Squares that leave fp32's range are summed up again from scaled values.
@@ -617,7 +617,7 @@ typedef struct {
  * C[a.rows, n] = A B with few columns: A is read once for every 40.  B [a.cols, n] in fp16 or bf16, ldb elements between rows, or between columns where transposed; or in
  * e4m3 (transposed only), column j being value x b_scales[j, k / b_group], b_scales [n, groups of a column] contiguous and b_group 0 (one scale for a column) or 32, 64
  * or 128: what b200spmm_rms_norm writes.  b_scales and b_group are for e4m3 alone.  Sums in fp32, a
- * scale multiplying the sum over its group (an infinite one gives infinities or NaN); C as that of b200spmm_fp4_dense_product.
+ * scale multiplying the sum over its group (an infinite one gives infinities or NaN); C as that of b200spmm_fp4_dense_product.  n up to 65,535 (else B200SPMM_ERR_UNSUPPORTED).
  */
 int b200spmm_int4_product(const b200spmm_int4_t *a, const void *d_B, int64_t ldb, int64_t n, int b_dtype, int b_transposed, const float *d_b_scales, int b_group,
                           void *d_C, int64_t ldc, int c_dtype, int c_transposed, void *stream);
@@ -629,7 +629,8 @@ int b200spmm_int4_product(const b200spmm_int4_t *a, const void *d_B, int64_t ldb
  * x, y and the router have one type, fp16 or bf16.  Experts: experts x 2 inner rows of `hidden` columns (for each expert first the gate's rows, then up's) and experts x hidden rows
  * of `inner` columns, one after the other: in 4-bit integers (gate_up, down), or in x's type (gate_up_16, down_16, rows ld elements apart, a multiple of 8, 16-byte
  * aligned), the others null.  Logits are added up in 64 bits; the inner values are kept in 32 and multiplied as the sum of two 16-bit
- * numbers: of x's type with 16-bit experts (22 digits in fp16, 16 in bf16), by codes of fp16, scaled by powers of two.
+ * numbers: of x's type with 16-bit experts (22 digits in fp16, 16 in bf16), by codes of fp16, scaled by powers of two.  So are
+ * bf16's x and codes: values more than 2^31 below their token's largest finite one lose digits.
  * experts up to 1024, top_k up to 32; hidden and inner as far as a block's shared memory holds a column beside the routing (else B200SPMM_ERR_UNSUPPORTED):
  * 24,000 and 12,000 (24,000 by codes) always, three times that with few tokens.  An expert is read once for up to 16 of its tokens; for as many as columns of x have room, where those are fewer:
  * 8 at a hidden size of 8,192.  A row of x with NaN gives NaN in its own row of y alone.
